@@ -499,6 +499,135 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
                            int capacity, int length, const int32_t *length_dev, uint16_t *out, uint16_t *sum_out,
                            uint16_t *norm_out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- serving over a paged key/value cache ----------------------------------
+ *
+ * A pool of `pages` pages of `page` positions (a power of two, 8..1024) is
+ * shared by up to LRMOE_PAGE_MAX_ROWS rows (sequences).  Pool state, all on
+ * the device and owned by the caller: table [rows][max_pages] int32 (a row's
+ * pages in order), held [rows] int32 (pages of each row), lengths [rows] int32
+ * (cached positions), free_pages [pages] int32 (a stack), state [4] int32 =
+ * (free pages, epoch, status bits, 0).  A slot is page * page_size + row in the
+ * page.  No reference counterpart: the reference serves one sequence on the
+ * Transformers cache. */
+#define LRMOE_PAGE_MAX_ROWS 4096
+#define LRMOE_PAGE_STATUS_TOKENS 1  /* a negative count, or more new positions than `tokens` */
+#define LRMOE_PAGE_STATUS_ROW 2     /* a row's length or pages past max_pages, or negative */
+#define LRMOE_PAGE_STATUS_POOL 4    /* not enough free pages (or a stack that does not fit `pages`) */
+#define LRMOE_PAGE_STATUS_STALE 8   /* a commit of a plan that another commit or release came after */
+
+/* The page plan of a step in which row r gets new_tokens[r] positions after
+ * its lengths[r]: starts [rows + 1] (row r's positions are starts[r] ..
+ * starts[r + 1] - 1 of the step), kv_lengths [rows] (cached positions with
+ * the new ones), held_out [rows] (pages then), positions [tokens] and slots
+ * [tokens] int64 of the step's positions (0 and -1 past the last), and the
+ * table entries of the fresh pages, which are taken from the top of the free
+ * stack, rows in order; info [4] int32 = (status bits, positions, fresh
+ * pages, the state's epoch).  Nothing else of the pool changes until the
+ * commit: a plan can be made again.  All or nothing: with any status bit set
+ * the step is empty (starts all 0, slots all -1, kv_lengths = lengths). */
+int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, const int32_t *new_tokens,
+                    const int32_t *lengths, const int32_t *held, const int32_t *free_pages, const int32_t *state,
+                    int32_t *table, int32_t *starts, int32_t *kv_lengths, int32_t *held_out, int32_t *positions,
+                    int64_t *slots, int32_t *info, void *stream);
+
+/* Takes a plan's outputs into the pool: held, the free count, and lengths =
+ * kv_lengths; with accepted [rows] given (drafts that stand, as
+ * lrmoe_verify_drafts writes them) a row with n > 0 new positions grows by
+ * min(accepted + 1, n) instead (its further pages stay held).  The epoch goes
+ * up by one.  A plan with a status bit, or one whose epoch is not the
+ * state's, changes nothing but state's status bits. */
+int lrmoe_page_commit(int rows, const int32_t *starts, const int32_t *kv_lengths, const int32_t *held_new,
+                      const int32_t *info, const int32_t *accepted, int32_t *lengths, int32_t *held, int32_t *state,
+                      void *stream);
+
+/* Returns the pages of the rows with mask[r] != 0 (uint8) to the free stack
+ * and empties those rows (length and held 0).  The epoch goes up by one. */
+int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t *mask, const int32_t *table,
+                       int32_t *lengths, int32_t *held, int32_t *free_pages, int32_t *state, void *stream);
+
+/* The append of a step's positions, the part of [HF] Qwen3_5MoeAttention.forward
+ * 683-701 between the projections and the attention: per token and head,
+ * x rsqrt(mean(x^2) + eps) (1 + w) when its norm weight is given, then the
+ * rotation of the first `rotary` elements (e < rotary / 2: x_e cos_e -
+ * x_{e + rotary/2} sin_e, and x_{e + rotary/2} cos + x_e sin), keys and values
+ * into their slots of the paged caches and queries (optional) into q_out.  In
+ * fp32 with one rounding at the end (the Transformers forward rounds to bf16
+ * after every step).  A token whose slot lies outside the pool is left out
+ * altogether; of tokens with the same slot, which one stays is not defined.
+ * Strides are in elements and multiples of 8; the last dimension is
+ * contiguous; pointers 16-byte aligned.  All 16-bit tensors are bf16, or fp16
+ * with fp16 != 0. */
+typedef struct lrmoe_paged_append_args {
+    int32_t tokens, heads, kv_heads, dim; /* dim 64, 128 or 256; heads 0: no queries */
+    int32_t rotary;                       /* 0, or a multiple of 16 up to dim */
+    int32_t pages, page, fp16;
+    const void *q, *k, *v;                /* [tokens][heads or kv_heads][dim] */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const void *q_norm, *k_norm;          /* [dim], each may be NULL */
+    float eps;
+    int32_t rope_fp32;                    /* cos and sin are fp32, else of the tensors' type */
+    const void *cos, *sin;                /* [rope_rows][rotary] */
+    const int32_t *positions;             /* [tokens] row of cos/sin (outside: NaN elements); NULL: row t */
+    int32_t rope_rows, pad;
+    const int64_t *slots;                 /* [tokens] */
+    void *q_out;                          /* [tokens][heads][dim], contiguous */
+    void *k_cache, *v_cache;
+    int64_t k_page_stride, k_cache_head_stride, k_row_stride, v_page_stride, v_cache_head_stride, v_row_stride;
+} lrmoe_paged_append_args;
+int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
+
+/* Attention of a step's positions over the paged cache, the causal attention
+ * of [HF] Qwen3_5MoeAttention.forward 703-718: token t of sequence s (tokens
+ * starts[s] .. starts[s + 1] - 1, n in all) sees cached positions 0 ..
+ * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
+ * when a gate is given; softmax and sums in fp32.  A row that sees nothing
+ * (kv_lengths[s] < n) is 0.  What a row does not see cannot change it,
+ * infinities and NaN included.  Tokens outside starts[0] .. starts[seqs] - 1
+ * are left as they were.  A table entry outside [0, pages) in use makes its
+ * sequence's rows NaN; kv_lengths beyond max_pages pages are cut there.
+ * max_new (at least every n) only chooses the kernel.  Strides as
+ * lrmoe_paged_append's (out and gate: multiples of 4); cache rows 16-byte
+ * aligned.  Workspace of lrmoe_paged_attention_workspace_bytes(args) bytes,
+ * 256-byte aligned, not cleared, used by one stream at a time. */
+typedef struct lrmoe_paged_attention_args {
+    int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */
+    int32_t pages, page, max_pages, fp16;
+    float scale;
+    int32_t pad;
+    const void *q, *gate;                 /* [tokens][heads][dim]; gate may be NULL */
+    int64_t q_token_stride, q_head_stride, gate_token_stride, gate_head_stride;
+    const void *k_cache, *v_cache;
+    int64_t k_page_stride, k_head_stride, k_row_stride, v_page_stride, v_head_stride, v_row_stride;
+    const int32_t *table, *starts, *kv_lengths; /* [seqs][max_pages], [seqs + 1], [seqs] */
+    void *out;                            /* [tokens][heads][dim] */
+    int64_t out_token_stride, out_head_stride;
+} lrmoe_paged_attention_args;
+size_t lrmoe_paged_attention_workspace_bytes(const lrmoe_paged_attention_args *args);
+int lrmoe_paged_attention(const lrmoe_paged_attention_args *args, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* Verification of drafted tokens against the target's probabilities (the
+ * reference accepts greedily: edge35b/dflash_probe.py:122-128 compares the
+ * drafter's tokens with the target's best).  Rows starts[b] .. starts[b + 1]
+ * - 1 of target [rows][vocab] (row stride target_stride elements) are block
+ * b's: the probabilities after each fed token.  tokens [rows] int64 are the
+ * fed tokens, so draft i of the block is the token at row i + 1 and is
+ * accepted while uniforms[row i] * q < p, p and q its probability in row i of
+ * target and draft (draft NULL: q = 1).  accepted[b] counts the drafts before
+ * the first that fails.  next[b] is then drawn from max(p - q, 0) at that row
+ * (draft NULL: p without the failed token; p where nothing is left), or from
+ * p at the last row when every draft stands: the first token whose running
+ * sum passes samples[b] times the total, in 64 bits; entries that are
+ * negative or not finite carry no mass, a row without any mass gives -1, and
+ * so does a block without rows (accepted 0).  uniforms [rows] and samples
+ * [blocks] fp32 in [0, 1).  type 0 fp32, 1 bf16, 2 fp16, of target and draft.
+ * Workspace of lrmoe_verify_workspace_bytes bytes, 16-byte aligned. */
+size_t lrmoe_verify_workspace_bytes(int blocks, int vocab);
+int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t *tokens, const void *target,
+                        int64_t target_stride, const void *draft, int64_t draft_stride, const int32_t *starts,
+                        const float *uniforms, const float *samples, int32_t *accepted, int64_t *next,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,7 +68,48 @@ _SIGNATURES = {
                               C.c_size_t, _P], _I),
     "lrmoe_attn_decode_step": ([_P, _I, _P, C.c_float, _P, _P, _P, _P, _P, _P, C.c_float, _P, _P, _P, _P, _I, _I,
                                 _P, _P, _P, _P, _P, C.c_size_t, _P], _I),
+    "lrmoe_page_plan": ([_I] * 5 + [_P] * 13, _I),
+    "lrmoe_page_commit": ([_I] + [_P] * 9, _I),
+    "lrmoe_page_release": ([_I] * 3 + [_P] * 7, _I),
+    "lrmoe_paged_append": ([_P, _P], _I),
+    "lrmoe_paged_attention_workspace_bytes": ([_P], C.c_size_t),
+    "lrmoe_paged_attention": ([_P, _P, C.c_size_t, _P], _I),
+    "lrmoe_verify_workspace_bytes": ([_I, _I], C.c_size_t),
+    "lrmoe_verify_drafts": ([_I] * 4 + [_P, _P, C.c_int64, _P, C.c_int64] + [_P] * 6 + [C.c_size_t, _P], _I),
 }
+
+
+def _fields(kinds: str):
+    """ctypes fields from "type: name name; ..." in the header's order."""
+    types = {"i": C.c_int32, "l": C.c_int64, "f": C.c_float, "p": C.c_void_p}
+    return [(name, types[part.split(":")[0].strip()]) for part in kinds.split(";") for name in part.split(":")[1].split()]
+
+
+class PagedAppendArgs(C.Structure):
+    """lrmoe_paged_append_args."""
+
+    _fields_ = _fields(
+        "i: tokens heads kv_heads dim rotary pages page fp16; p: q k v;"
+        "l: q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride;"
+        "p: q_norm k_norm; f: eps; i: rope_fp32; p: cos sin positions; i: rope_rows pad; p: slots q_out k_cache v_cache;"
+        "l: k_page_stride k_cache_head_stride k_row_stride v_page_stride v_cache_head_stride v_row_stride")
+
+
+class PagedAttentionArgs(C.Structure):
+    """lrmoe_paged_attention_args."""
+
+    _fields_ = _fields(
+        "i: seqs tokens max_new heads kv_heads dim pages page max_pages fp16; f: scale; i: pad; p: q gate;"
+        "l: q_token_stride q_head_stride gate_token_stride gate_head_stride; p: k_cache v_cache;"
+        "l: k_page_stride k_head_stride k_row_stride v_page_stride v_head_stride v_row_stride;"
+        "p: table starts kv_lengths out; l: out_token_stride out_head_stride")
+
+
+PAGE_MAX_ROWS = 4096     # rows (sequences) of a page pool
+PAGE_STATUS_TOKENS = 1   # a negative count, or more new positions than the plan has room for
+PAGE_STATUS_ROW = 2      # a row past its pages, or corrupt
+PAGE_STATUS_POOL = 4     # not enough free pages
+PAGE_STATUS_STALE = 8    # a plan committed after another commit or release
 
 STAGE_ROUTE = 1
 STAGE_GATE_UP = 2

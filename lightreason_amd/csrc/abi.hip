@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "lrmoe_internal.h"
+#include "paged.h"
 
 namespace {
 
@@ -675,6 +676,200 @@ int lrmoe_attn_decode_step(const uint16_t* residual, int tokens, const uint16_t*
     return attn_decode(residual, tokens, q_proj, k_proj, v_proj, o_proj, q_norm, k_norm, eps, cos, sin, k_cache,
                        v_cache, capacity, length_dev != nullptr ? 0 : length, length_dev, out,
                        lrmoe::AttnGlue{input_norm, input_eps, norm_out, sum_out}, workspace, workspace_bytes, stream);
+}
+
+// ---- paged cache --------------------------------------------------------------
+
+static bool bad_page(int page) { return page < 8 || page > 1024 || (page & (page - 1)) != 0; }
+static bool bad_pool(int rows, int pages, int max_pages) {
+    return rows < 0 || rows > LRMOE_PAGE_MAX_ROWS || pages < 1 || max_pages < 1;
+}
+static int shift_of(int page) { return __builtin_ctz(static_cast<unsigned>(page)); }
+
+int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, const int32_t* new_tokens,
+                    const int32_t* lengths, const int32_t* held, const int32_t* free_pages, const int32_t* state,
+                    int32_t* table, int32_t* starts, int32_t* kv_lengths, int32_t* held_out, int32_t* positions,
+                    int64_t* slots, int32_t* info, void* stream) {
+    if (bad_pool(rows, pages, max_pages) || bad_page(page) || tokens < 0 || tokens > (1 << 24) ||
+        static_cast<int64_t>(max_pages) * page > INT32_MAX)
+        return LRMOE_E_ARG;
+    if (rows == 0) return LRMOE_OK;
+    if (!new_tokens || !lengths || !held || !free_pages || !state || !table || !starts || !kv_lengths || !held_out ||
+        !info || (tokens > 0 && (!positions || !slots)))
+        return LRMOE_E_ARG;
+    if (int d = check_device()) return d;
+    lrmoe::PagePlanArgs a{rows, pages, shift_of(page), max_pages, tokens, new_tokens, lengths, held, free_pages, state,
+                          table, starts, kv_lengths, held_out, positions, info, slots};
+    return status_of(lrmoe::launch_page_plan(a, as_stream(stream)));
+}
+
+int lrmoe_page_commit(int rows, const int32_t* starts, const int32_t* kv_lengths, const int32_t* held_new,
+                      const int32_t* info, const int32_t* accepted, int32_t* lengths, int32_t* held, int32_t* state,
+                      void* stream) {
+    if (rows < 0 || rows > LRMOE_PAGE_MAX_ROWS) return LRMOE_E_ARG;
+    if (rows == 0) return LRMOE_OK;
+    if (!starts || !kv_lengths || !held_new || !info || !lengths || !held || !state) return LRMOE_E_ARG;
+    if (int d = check_device()) return d;
+    lrmoe::PageCommitArgs a{rows, starts, kv_lengths, held_new, info, accepted, lengths, held, state};
+    return status_of(lrmoe::launch_page_commit(a, as_stream(stream)));
+}
+
+int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t* mask, const int32_t* table,
+                       int32_t* lengths, int32_t* held, int32_t* free_pages, int32_t* state, void* stream) {
+    if (bad_pool(rows, pages, max_pages)) return LRMOE_E_ARG;
+    if (rows == 0) return LRMOE_OK;
+    if (!mask || !table || !lengths || !held || !free_pages || !state) return LRMOE_E_ARG;
+    if (int d = check_device()) return d;
+    lrmoe::PageReleaseArgs a{rows, pages, max_pages, mask, table, lengths, held, free_pages, state};
+    return status_of(lrmoe::launch_page_release(a, as_stream(stream)));
+}
+
+static bool bad_dim(int dim) { return dim != 64 && dim != 128 && dim != 256; }
+
+int lrmoe_paged_append(const lrmoe_paged_append_args* p, void* stream) {
+    if (!p) return LRMOE_E_ARG;
+    if (p->tokens < 0 || p->tokens > (1 << 24) || p->heads < 0 || p->heads > 1024 || p->kv_heads < 1 ||
+        p->kv_heads > 1024 || bad_dim(p->dim) || p->rotary < 0 || p->rotary > p->dim || p->rotary % 16 != 0 ||
+        p->pages < 1 || bad_page(p->page) || (p->rotary > 0 && p->rope_rows < 1))
+        return LRMOE_E_ARG;
+    if (p->tokens == 0) return LRMOE_OK;
+    if (!p->k || !p->v || !p->slots || !p->k_cache || !p->v_cache || (p->heads > 0 && (!p->q || !p->q_out)) ||
+        (p->rotary > 0 && (!p->cos || !p->sin)))
+        return LRMOE_E_ARG;
+    for (const void* x : {p->q, p->k, p->v, p->q_norm, p->k_norm, p->cos, p->sin, static_cast<const void*>(p->q_out),
+                          static_cast<const void*>(p->k_cache), static_cast<const void*>(p->v_cache)})
+        if (misaligned(x, 16)) return LRMOE_E_ARG;
+    for (int64_t x : {p->q_token_stride, p->q_head_stride, p->k_token_stride, p->k_head_stride, p->v_token_stride,
+                      p->v_head_stride, p->k_page_stride, p->k_cache_head_stride, p->k_row_stride, p->v_page_stride,
+                      p->v_cache_head_stride, p->v_row_stride})
+        if (x % 8 != 0) return LRMOE_E_ARG;
+    if (static_cast<int64_t>(p->tokens) * (p->heads + 2 * p->kv_heads) * (p->dim / 8) > (INT64_C(1) << 38))
+        return LRMOE_E_ARG;  // a grid of at most 2^30 workgroups
+    if (int d = check_device()) return d;
+    lrmoe::PagedAppendArgs a{};
+    a.tokens = p->tokens;
+    a.heads = p->heads;
+    a.kv_heads = p->kv_heads;
+    a.rotary = p->rotary;
+    a.pages = p->pages;
+    a.page_shift = shift_of(p->page);
+    a.rope_rows = p->rope_rows;
+    a.rope_fp32 = p->rope_fp32;
+    a.eps = p->eps;
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.k = static_cast<const uint16_t*>(p->k);
+    a.v = static_cast<const uint16_t*>(p->v);
+    a.q_norm = static_cast<const uint16_t*>(p->q_norm);
+    a.k_norm = static_cast<const uint16_t*>(p->k_norm);
+    a.q_token_stride = p->q_token_stride;
+    a.q_head_stride = p->q_head_stride;
+    a.k_token_stride = p->k_token_stride;
+    a.k_head_stride = p->k_head_stride;
+    a.v_token_stride = p->v_token_stride;
+    a.v_head_stride = p->v_head_stride;
+    a.q_out = static_cast<uint16_t*>(p->q_out);
+    a.k_cache = static_cast<uint16_t*>(p->k_cache);
+    a.v_cache = static_cast<uint16_t*>(p->v_cache);
+    a.k_page_stride = p->k_page_stride;
+    a.k_cache_head_stride = p->k_cache_head_stride;
+    a.k_row_stride = p->k_row_stride;
+    a.v_page_stride = p->v_page_stride;
+    a.v_cache_head_stride = p->v_cache_head_stride;
+    a.v_row_stride = p->v_row_stride;
+    a.cos = p->cos;
+    a.sin = p->sin;
+    a.positions = p->positions;
+    a.slots = p->slots;
+    return status_of(lrmoe::launch_paged_append(a, p->fp16 != 0, p->dim, as_stream(stream)));
+}
+
+static bool bad_attention(const lrmoe_paged_attention_args* p) {
+    return p->seqs < 0 || p->seqs > LRMOE_PAGE_MAX_ROWS || p->tokens < 0 || p->tokens > (1 << 20) || p->max_new < 0 ||
+           p->heads < 1 || p->heads > 1024 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || bad_dim(p->dim) ||
+           p->pages < 1 || bad_page(p->page) || p->max_pages < 1 ||
+           static_cast<int64_t>(p->max_pages) * p->page > INT32_MAX;
+}
+
+size_t lrmoe_paged_attention_workspace_bytes(const lrmoe_paged_attention_args* p) {
+    if (!p || bad_attention(p)) return 0;
+    return lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new);
+}
+
+int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+    if (!p || bad_attention(p)) return LRMOE_E_ARG;
+    if (p->tokens == 0 || p->seqs == 0) return LRMOE_OK;
+    if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->starts || !p->kv_lengths || !p->out)
+        return LRMOE_E_ARG;
+    if (misaligned(p->q, 16) || misaligned(p->k_cache, 16) || misaligned(p->v_cache, 16) || misaligned(p->out, 8) ||
+        misaligned(p->gate, 8) || misaligned(workspace, 256))
+        return LRMOE_E_ARG;
+    for (int64_t x : {p->q_token_stride, p->q_head_stride, p->k_page_stride, p->k_head_stride, p->k_row_stride,
+                      p->v_page_stride, p->v_head_stride, p->v_row_stride})
+        if (x % 8 != 0) return LRMOE_E_ARG;
+    if (p->out_token_stride % 4 != 0 || p->out_head_stride % 4 != 0 ||
+        (p->gate && (p->gate_token_stride % 4 != 0 || p->gate_head_stride % 4 != 0)))
+        return LRMOE_E_ARG;
+    const size_t need =
+        lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new);
+    if (need > 0 && !workspace) return LRMOE_E_ARG;
+    if (workspace_bytes < need) return LRMOE_E_WORKSPACE;
+    if (int d = check_device()) return d;
+    lrmoe::PagedAttnArgs a{};
+    a.seqs = p->seqs;
+    a.tokens = p->tokens;
+    a.heads = p->heads;
+    a.kv_heads = p->kv_heads;
+    a.group = p->heads / p->kv_heads;
+    a.pages = p->pages;
+    a.page_shift = shift_of(p->page);
+    a.max_pages = p->max_pages;
+    a.scale = p->scale * 1.4426950408889634f;
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.gate = static_cast<const uint16_t*>(p->gate);
+    a.k_cache = static_cast<const uint16_t*>(p->k_cache);
+    a.v_cache = static_cast<const uint16_t*>(p->v_cache);
+    a.q_token_stride = p->q_token_stride;
+    a.q_head_stride = p->q_head_stride;
+    a.gate_token_stride = p->gate_token_stride;
+    a.gate_head_stride = p->gate_head_stride;
+    a.k_page_stride = p->k_page_stride;
+    a.k_head_stride = p->k_head_stride;
+    a.k_row_stride = p->k_row_stride;
+    a.v_page_stride = p->v_page_stride;
+    a.v_head_stride = p->v_head_stride;
+    a.v_row_stride = p->v_row_stride;
+    a.table = p->table;
+    a.starts = p->starts;
+    a.kv_lengths = p->kv_lengths;
+    a.out = static_cast<uint16_t*>(p->out);
+    a.out_token_stride = p->out_token_stride;
+    a.out_head_stride = p->out_head_stride;
+    return status_of(
+        lrmoe::launch_paged_attention(a, p->fp16 != 0, p->dim, p->max_new, workspace, as_stream(stream)));
+}
+
+size_t lrmoe_verify_workspace_bytes(int blocks, int vocab) {
+    if (blocks < 1 || blocks > 65535 || vocab < 1) return 0;
+    return lrmoe::verify_workspace_bytes(blocks, vocab);
+}
+
+int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t* tokens, const void* target,
+                        int64_t target_stride, const void* draft, int64_t draft_stride, const int32_t* starts,
+                        const float* uniforms, const float* samples, int32_t* accepted, int64_t* next,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+    if (blocks < 0 || blocks > 65535 || rows < 0 || vocab < 1 || type < 0 || type > 2) return LRMOE_E_ARG;
+    if (blocks == 0) return LRMOE_OK;
+    if (!starts || !samples || !accepted || !next || !workspace ||
+        (rows > 0 && (!tokens || !target || !uniforms || target_stride < vocab || (draft && draft_stride < vocab))))
+        return LRMOE_E_ARG;
+    if (misaligned(workspace, 16) || misaligned(target, type == 0 ? 4 : 2) || misaligned(draft, type == 0 ? 4 : 2))
+        return LRMOE_E_ARG;
+    if (workspace_bytes < lrmoe::verify_workspace_bytes(blocks, vocab)) return LRMOE_E_WORKSPACE;
+    if (int d = check_device()) return d;
+    lrmoe::VerifyArgs a{blocks,  rows,     vocab,    tokens, target, draft, target_stride, draft_stride,
+                        starts,  uniforms, samples,  accepted, next, static_cast<double*>(workspace)};
+    return status_of(lrmoe::launch_verify_drafts(a, type, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from .moe import DECODE_MAX_TOKENS, HIDDEN, TOPK, Workspace, moe_chain
 
 
@@ -119,3 +120,80 @@ class VerifyGraphs:
     def status(self) -> int:
         """Status word of the last replay (reads the device)."""
         return self.workspace.status()
+
+
+# ---- which drafts stand ---------------------------------------------------------
+
+_PROBABILITIES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows_of(t: torch.Tensor, name: str, shape, dtype, device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on {device}")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} needs a contiguous last dimension")
+    if len(shape) == 2 and shape[0] > 1 and t.stride(0) < shape[1]:
+        raise ValueError(f"{name} needs rows that do not overlap")
+
+
+def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tensor, uniforms: torch.Tensor,
+                  samples: torch.Tensor, *, draft: torch.Tensor | None = None, accepted: torch.Tensor | None = None,
+                  next_tokens: torch.Tensor | None = None):
+    """Which drafted tokens of each verify block stand, and the token after
+    them (``lrmoe_verify_drafts``): the rejection rule under which the
+    outputs follow the target's distribution whatever the drafter proposes.
+
+    ``tokens`` [rows] int64 are the fed tokens of every block, the last
+    committed one first, then its drafts; ``starts`` [blocks + 1] int32 the
+    blocks' first rows (a ``paged.PagePlan``'s); ``target`` [rows, vocab] the
+    target's probabilities after each fed token, ``draft`` [rows, vocab] the
+    drafter's of the same positions (fp32, bf16 or fp16; None for a drafter
+    that proposes its best token).  Draft i stands while uniforms[row i] * q <
+    p.  The next token is drawn from max(p - q, 0) at the first draft that
+    fails (from p where nothing is left), or from p at the last row: the first
+    whose running sum in 64 bits passes ``samples[b]`` of the total.
+    ``uniforms`` [rows] and ``samples`` [blocks] are fp32 in [0, 1).
+
+    Returns (accepted [blocks] int32, next_tokens [blocks] int64); a block
+    without rows gives (0, -1), a row of probabilities without mass -1.  A
+    block of one row is plain sampling.  ``PageTable.commit(plan, accepted)``
+    takes the result into the page pool."""
+    if not isinstance(target, torch.Tensor) or target.dim() != 2 or target.dtype not in _PROBABILITIES:
+        raise ValueError("target must be fp32, bf16 or fp16 [rows, vocab]")
+    rows, vocab = target.shape
+    dev = target.device
+    if dev.type != "cuda":
+        raise ValueError(f"target must be on a GPU, got {dev}")
+    if vocab < 1:
+        raise ValueError("the vocabulary is empty")
+    _rows_of(target, "target", (rows, vocab), target.dtype, dev)
+    if draft is not None:
+        _rows_of(draft, "draft", (rows, vocab), target.dtype, dev)
+    if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError("starts must be int32 [blocks + 1]")
+    blocks = starts.shape[0] - 1
+    if blocks > 65535:
+        raise ValueError(f"at most 65535 blocks, got {blocks}")
+    _rows_of(starts, "starts", (blocks + 1,), torch.int32, dev)
+    _rows_of(tokens, "tokens", (rows,), torch.int64, dev)
+    _rows_of(uniforms, "uniforms", (rows,), torch.float32, dev)
+    _rows_of(samples, "samples", (blocks,), torch.float32, dev)
+    if accepted is None:
+        accepted = torch.empty(blocks, dtype=torch.int32, device=dev)
+    _rows_of(accepted, "accepted", (blocks,), torch.int32, dev)
+    if next_tokens is None:
+        next_tokens = torch.empty(blocks, dtype=torch.int64, device=dev)
+    _rows_of(next_tokens, "next_tokens", (blocks,), torch.int64, dev)
+    if blocks == 0:
+        return accepted, next_tokens
+    with torch.cuda.device(dev):
+        # From torch's allocator, which keeps it for this stream's next calls
+        # (and, under capture, in the graph's own memory).
+        scratch = torch.empty(int(_native.library().lrmoe_verify_workspace_bytes(blocks, vocab)), dtype=torch.uint8,
+                              device=dev)
+        _native.call("lrmoe_verify_drafts", blocks, rows, vocab, _PROBABILITIES[target.dtype], tokens.data_ptr(),
+                     target.data_ptr(), max(target.stride(0), vocab), None if draft is None else draft.data_ptr(),
+                     0 if draft is None else max(draft.stride(0), vocab), starts.data_ptr(), uniforms.data_ptr(),
+                     samples.data_ptr(), accepted.data_ptr(), next_tokens.data_ptr(), scratch.data_ptr(),
+                     scratch.numel(), torch.cuda.current_stream(dev).cuda_stream)
+    return accepted, next_tokens
