@@ -18,42 +18,21 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The sequence that holds token t of starts[0 .. seqs], or -1.
-__device__ __forceinline__ int sequence_of(const int32_t* starts, int seqs, int t) {
-    if (t < starts[0] || t >= starts[seqs]) return -1;
-    int lo = 0, hi = seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= t) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-// One wave per (token, head): a lane per position for the scores (64 at a
-// time), a lane per D / 64 elements for the values, softmax statistics and
-// accumulators in fp32.  Positions that the row does not see are never read.
+// One row (token t of sequence b, head h) by one wave, reading only the
+// positions that the row sees: a lane per position for the scores (64 at a
+// time), a lane per D / 64 elements for the values.  The path of rows whose
+// tile holds values that are not finite and that some of its rows do not see
+// (in a tile's matrix product their zero weights would not hide them).
 template <bool FP16, int D>
-__global__ __launch_bounds__(kThreads) void attend_row_kernel(PagedAttnArgs a) {
-    constexpr int WAVES = kThreads / kWave;
+__device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t seen, float* qs, float* ps,
+                           int64_t* vs) {
     constexpr int E = D / kWave;
-    __shared__ float qs[WAVES][D];
-    __shared__ float ps[WAVES][kWave];
-    __shared__ int64_t vs[WAVES][kWave];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * WAVES + wave;
-    if (item >= static_cast<int64_t>(a.tokens) * a.heads) return;
-    const int t = static_cast<int>(item / a.heads), h = static_cast<int>(item % a.heads);
-    const int b = sequence_of(a.starts, a.seqs, t);
-    if (b < 0) return;
-    const int n = a.starts[b + 1] - a.starts[b];
-    const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
-    const int64_t kv = min(static_cast<int64_t>(max(a.kv_lengths[b], 0)), capacity);
-    const int64_t seen = kv - n + (t - a.starts[b]) + 1;
+    const int lane = threadIdx.x % kWave;
     const uint16_t* q = a.q + t * a.q_token_stride + h * a.q_head_stride;
-    const int64_t kh = static_cast<int64_t>(h / a.group);
+    const int64_t kh = h / a.group;
     // LDS rows here belong to one wave, whose accesses stay in order; the
-    // barriers below only keep the compiler from moving them.
-    for (int e = lane; e < D; e += kWave) qs[wave][e] = elem16<FP16>(q[e]) * a.scale;
+    // fences below only keep the compiler from moving them.
+    for (int e = lane; e < D; e += kWave) qs[e] = elem16<FP16>(q[e]) * a.scale;
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.max_pages;
     float m = -__builtin_inff(), l = 0.0f, acc[E] = {};
     bool bad = false;
@@ -64,25 +43,22 @@ __global__ __launch_bounds__(kThreads) void attend_row_kernel(PagedAttnArgs a) {
         if (p < seen) {
             int64_t block = table[p >> a.page_shift];
             bad |= block < 0 || block >= a.pages;
-            block = min(max(block, static_cast<int64_t>(0)), static_cast<int64_t>(a.pages) - 1);
+            block = block < 0 || block >= a.pages ? 0 : block;
             const int64_t row = p & ((1 << a.page_shift) - 1);
             const uint16_t* k = a.k_cache + block * a.k_page_stride + kh * a.k_head_stride + row * a.k_row_stride;
-            vs[wave][lane] = block * a.v_page_stride + kh * a.v_head_stride + row * a.v_row_stride;
+            vs[lane] = block * a.v_page_stride + kh * a.v_head_stride + row * a.v_row_stride;
             s = 0.0f;
             for (int e = 0; e < D; e += 8) {
                 float x[8];
                 unpack16<FP16>(ldg16(k + e), x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s = __builtin_fmaf(x[j], qs[wave][e + j], s);
+                for (int j = 0; j < 8; ++j) s = __builtin_fmaf(x[j], qs[e + j], s);
             }
         }
         float top = s;
 #pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            const float o = __shfl_xor(top, off);
-            top = top != top ? top : (o > top || o != o ? o : top);  // a NaN score stays
-        }
-        const float mn = top > m || top != top ? top : m;
+        for (int off = 1; off < kWave; off *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, off));
+        const float mn = __builtin_fmaxf(m, top);
         const float shift = mn == -__builtin_inff() ? 0.0f : mn;
         const float w = p < seen ? __builtin_exp2f(s - shift) : 0.0f;
         const float fall = __builtin_exp2f(m - shift);
@@ -91,15 +67,15 @@ __global__ __launch_bounds__(kThreads) void attend_row_kernel(PagedAttnArgs a) {
         for (int off = 1; off < kWave; off *= 2) sum += __shfl_xor(sum, off);
         l = l * fall + sum;
         m = mn;
-        ps[wave][lane] = w;
+        ps[lane] = w;
         wave_lds_fence();
 #pragma unroll
         for (int i = 0; i < E; ++i) acc[i] *= fall;
         const int count = static_cast<int>(min(static_cast<int64_t>(kWave), seen - base));
         for (int j = 0; j < count; ++j) {
-            const uint16_t* v = a.v_cache + vs[wave][j] + lane * E;
+            const uint16_t* v = a.v_cache + vs[j] + lane * E;
 #pragma unroll
-            for (int i = 0; i < E; ++i) acc[i] = __builtin_fmaf(ps[wave][j], elem16<FP16>(v[i]), acc[i]);
+            for (int i = 0; i < E; ++i) acc[i] = __builtin_fmaf(ps[j], elem16<FP16>(v[i]), acc[i]);
         }
         wave_lds_fence();
     }
@@ -115,19 +91,740 @@ __global__ __launch_bounds__(kThreads) void attend_row_kernel(PagedAttnArgs a) {
     }
 }
 
+// ---- the step's schedule ----------------------------------------------------------
+//
+// A sequence's rows (token-major, then the heads of one key/value head's
+// group) are cut into tiles of BM rows; a tile's positions into splits, so
+// that a few long sequences fill the chip: with W steps of positions in all,
+// a split holds more than W / target steps, so that there are at most target
+// splits and one per tile, and fewer than 2 target of tiles that are split.  Every workgroup works this
+// out for itself from starts and kv_lengths (up to 16 sequences per thread):
+// nothing of it depends on the host, and no launch precedes the attention's.
+
+struct Sequence {
+    int first, n, kv;  // first token, new tokens, cached positions
+};
+__device__ __forceinline__ Sequence sequence_at(const PagedAttnArgs& a, int b) {
+    Sequence s;
+    s.first = min(max(a.starts[b], 0), a.tokens);
+    s.n = max(min(a.starts[b + 1], a.tokens) - s.first, 0);
+    const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
+    s.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lengths[b], 0)), capacity));
+    return s;
+}
+// Positions that token i of the sequence sees.
+__device__ __forceinline__ int seen_by(const Sequence& s, int i) { return max(s.kv - s.n + i + 1, 0); }
+
+struct Split {
+    int b, tile, split, splits;
+    int64_t slot;  // of the tile's first partial rows, before the head; -1 for a sequence in one piece
+    Sequence seq;
+};
+
+__device__ __forceinline__ int tiles_of(const Sequence& s, int group, int bm) {
+    return static_cast<int>((static_cast<int64_t>(s.n) * group + bm - 1) / bm);
+}
+__device__ __forceinline__ int steps_of(int positions, int step) { return max((positions + step - 1) / step, 1); }
+// Positions that the tile's last row sees.
+__device__ __forceinline__ int tile_end(const Sequence& s, int group, int bm, int tile) {
+    const int64_t rows = min(static_cast<int64_t>(tile + 1) * bm, static_cast<int64_t>(s.n) * group);
+    return seen_by(s, static_cast<int>((rows - 1) / group));
+}
+
+// Steps per split: the first count above W / target, not under `least`.
+template <int BM, int STEP>
+__device__ __forceinline__ int split_steps(const PagedAttnArgs& a, int target, int least, double* lds) {
+    const int per = (a.seqs + kThreads - 1) / kThreads;
+    double work = 0.0;   // (a product of counts that a bad `starts` could make pass 64 bits)
+    for (int i = 0; i < per; ++i) {
+        const int b = threadIdx.x * per + i;
+        if (b >= a.seqs) break;
+        const Sequence s = sequence_at(a, b);
+        if (s.n > 0) work += static_cast<double>(tiles_of(s, a.group, BM)) * steps_of(s.kv, STEP);
+    }
+#pragma unroll
+    for (int off = 1; off < kWave; off *= 2) work += __shfl_xor(work, off);
+    if (__lane_id() == 0) lds[threadIdx.x / kWave] = work;
+    __syncthreads();
+    work = (lds[0] + lds[1] + lds[2] + lds[3]) * a.kv_heads;
+    __syncthreads();
+    const double c = work / target;
+    return max(c < 1.0e9 ? static_cast<int>(c) + 1 : 1 << 30, least);
+}
+template <int BM, int STEP>
+__device__ __forceinline__ int splits_of(const PagedAttnArgs& a, const Sequence& s, int per_split) {
+    return (steps_of(s.kv, STEP) + per_split - 1) / per_split;
+}
+// A tile takes its sequence's split count, or fewer where causality leaves it
+// fewer steps.
+template <int STEP>
+__device__ __forceinline__ int tile_splits(int splits, int end, int per_split) {
+    return min(splits, (steps_of(end, STEP) + per_split - 1) / per_split);
+}
+
+// Where each sequence's splits (of all its tiles, per head) begin, and its
+// partial slots; then the sequence of split `item` (in LDS as *found), heavy
+// tiles first.  Returns false past the last split.
+struct ScheduleLds {
+    double sums[kThreads / kWave];
+    Split found;
+    int64_t scan[2][kThreads / kWave];
+};
+template <int BM, int STEP>
+__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, ScheduleLds* lds,
+                                           int* per_split) {
+    const int c = split_steps<BM, STEP>(a, target, least, lds->sums);
+    *per_split = c;
+    const int per = (a.seqs + kThreads - 1) / kThreads;
+    int64_t items = 0, slots = 0;
+    for (int i = 0; i < per; ++i) {
+        const int b = threadIdx.x * per + i;
+        if (b >= a.seqs) break;
+        const Sequence s = sequence_at(a, b);
+        if (s.n == 0) continue;
+        const int splits = splits_of<BM, STEP>(a, s, c);
+        const int64_t all = static_cast<int64_t>(tiles_of(s, a.group, BM)) * splits;
+        items += all;
+        slots += splits > 1 ? all : 0;
+    }
+    int64_t at = items, slot = slots;
+#pragma unroll
+    for (int off = 1; off < kWave; off *= 2) {
+        const int64_t up = __shfl_up(at, off), us = __shfl_up(slot, off);
+        if (static_cast<int>(__lane_id()) >= off) {
+            at += up;
+            slot += us;
+        }
+    }
+    const int wave = threadIdx.x / kWave;
+    if (__lane_id() == kWave - 1) {
+        lds->scan[0][wave] = at;
+        lds->scan[1][wave] = slot;
+    }
+    if (threadIdx.x == 0) lds->found.b = -1;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        at += lds->scan[0][w];
+        slot += lds->scan[1][w];
+    }
+    at -= items;
+    slot -= slots;
+    if (item >= at && item < at + items) {
+        for (int i = 0; i < per; ++i) {
+            const int b = threadIdx.x * per + i;
+            if (b >= a.seqs) break;
+            const Sequence s = sequence_at(a, b);
+            if (s.n == 0) continue;
+            const int splits = splits_of<BM, STEP>(a, s, c), tiles = tiles_of(s, a.group, BM);
+            const int64_t all = static_cast<int64_t>(tiles) * splits;
+            if (item < at + all) {
+                const int local = static_cast<int>(item - at);
+                lds->found.b = b;
+                lds->found.tile = tiles - 1 - local / splits;
+                lds->found.split = local % splits;
+                lds->found.splits = splits;
+                lds->found.slot = splits > 1 ? slot + static_cast<int64_t>(lds->found.tile) * splits : -1;
+                lds->found.seq = s;
+                break;
+            }
+            at += all;
+            slot += splits > 1 ? all : 0;
+        }
+    }
+    __syncthreads();
+    return lds->found.b >= 0;
+}
+
+// Four elements d .. d + 3 of a row's result: sums over l, times the gate,
+// rounded once.
+template <bool FP16>
+__device__ __forceinline__ void store_row4(const PagedAttnArgs& a, const Sequence& s, int kh, int64_t row, int d,
+                                           float4 v, float l) {
+    const int64_t i = row / a.group;
+    const int64_t t = s.first + i, h = static_cast<int64_t>(kh) * a.group + (row - i * a.group);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    if (a.gate != nullptr) {
+        const uint2 g = *reinterpret_cast<const uint2*>(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d);
+        x[0] *= sigmoid(elem16<FP16>(g.x & 0xffff));
+        x[1] *= sigmoid(elem16<FP16>(g.x >> 16));
+        x[2] *= sigmoid(elem16<FP16>(g.y & 0xffff));
+        x[3] *= sigmoid(elem16<FP16>(g.y >> 16));
+    }
+    *reinterpret_cast<uint2*>(a.out + t * a.out_token_stride + h * a.out_head_stride + d) =
+        make_uint2(pack16_2<FP16>(x[0], x[1]), pack16_2<FP16>(x[2], x[3]));
+}
+
+// ---- the tile kernel --------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+
+template <bool FP16>
+__device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    if constexpr (FP16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+// gfx9 s_waitcnt immediate with expcnt at its maximum.
+constexpr int wait_imm(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
+template <int VM, int LGKM>
+__device__ __forceinline__ void wait_counts() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_imm(VM, LGKM));
+    asm volatile("" ::: "memory");
+}
+
+// 16 bytes per lane from global memory straight into LDS (lane i's to lds_at +
+// 16 i, lds_at the same in every lane).  Written as assembly because the
+// compiler puts a wait for every outstanding one before each LDS read, which
+// would end the read-ahead; it has no register output, and the waits are the
+// kernel's own (wait_counts before the barrier that publishes a tile).
+__device__ __forceinline__ void load_lds16(uint32_t lds_at, const void* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds_at), "v"(offset), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void load_lds16(uint32_t lds_at, const void* address) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds_at), "v"(address)
+                 : "memory");
+}
+
+__device__ const uint4 kZeros = {0u, 0u, 0u, 0u};  // what rows past a tile's end read
+
+// The LDS byte address of a __shared__ array.
+__device__ __forceinline__ uint32_t lds_address(void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)p));
+}
+
+// Swizzles of a tile row's 16-byte chunks in LDS.  Keys: 16 consecutive rows
+// read at one chunk fall on 16 different chunk places of 256 bytes.  Values:
+// the transposing read takes 2 (per 16 lanes) or 4 (per 32) chunks of four
+// rows at a time; they fall on different places of 128 and of 256 bytes.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+    return D == 64 ? (((row & 2) << 1) ^ ((row & 1) << 1)) : (((row & 3) << 2) ^ (row & 2));
+}
+
+// Rows [row0, row0 + ROWS) of a tile that starts at position `base`, from
+// pages of one cache into LDS.
+struct PageWindow {
+    int entry;   // lane i: table entry of page first + i
+    int first;   // first page of the window
+};
+struct CacheView {
+    const uint16_t* data;  // at the key/value head
+    int64_t page_stride;
+    int64_t row_stride;
+};
+
+template <int D, int ROWS, bool VALUES>
+__device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win, int pos,
+                                           int end, uint32_t lds_at, bool& bad) {
+    constexpr int PER = 512 / D;    // rows per load of the wave
+    constexpr int CHUNKS = D / 8;
+    const int lane = threadIdx.x % kWave;
+    const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
+#pragma unroll
+    for (int i = 0; i < ROWS / PER; ++i) {
+        const int row = i * PER;      // of the ROWS; the tile's rows are a multiple of 16 before it
+        const int p = pos + row;
+        const uint32_t at = lds_at + row * 2 * D;
+        const int chunk = lchunk ^ (VALUES ? v_swizzle<D>(row + lrow) : k_swizzle<D>(row + lrow));
+        const int page = p < end ? (p >> a.page_shift) - win.first : 0;
+        int entry = __builtin_amdgcn_readlane(win.entry, page);
+        if (p < end && static_cast<uint32_t>(entry) >= static_cast<uint32_t>(a.pages)) bad = true;
+        entry = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages) ? entry : 0;
+        const uint16_t* base =
+            c.data + entry * c.page_stride + (p & ((1 << a.page_shift) - 1)) * c.row_stride;
+        const uint32_t offset = static_cast<uint32_t>(lrow) * static_cast<uint32_t>(2 * c.row_stride) + 16 * chunk;
+        if (p + PER <= end) {
+            load_lds16(at, base, offset);
+        } else {
+            const uint8_t* from = reinterpret_cast<const uint8_t*>(base) + offset;
+            load_lds16(at, p + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
+        }
+    }
+}
+
+// Highest value and sum over the two lanes (q, q + 32) that share a row.
+__device__ __forceinline__ float pair_max(float v) {
+    const int x = __float_as_int(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+
+struct Partials {
+    float* o;     // [slot][BM][D] sums of exp2(s - m) v
+    float* ml;    // [slot][BM][2] m, sum of exp2(s - m)
+    int* dirty;   // [splits]
+    int slots, splits;  // how many there is room for
+};
+
+constexpr float kLowest = -1.7e38f;  // the running maximum before any position
+constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
+
+template <bool FP16, int D, int RB, int WQ, int WK, int NB>
+__global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
+    static_assert(WQ * WK == kThreads / kWave, "four waves");
+    constexpr int KT = 32 * NB;           // positions of a tile
+    constexpr int STEP = KT * WK;         // positions per step of the workgroup
+    constexpr int BM = 32 * RB * WQ;
+    constexpr int TILE = KT * 2 * D;      // bytes of a tile of keys or values
+    constexpr int STAGES = WK == 1 ? 2 : 1;
+    constexpr int KS = D / 16, DB = D / 32;
+    constexpr int ROWS = WK == 1 ? KT / 4 : KT;   // rows that a wave stages
+    constexpr int LOADS = ROWS * D / 512;         // of a key or value tile, per wave
+    __shared__ __align__(1024) uint8_t lds[2 * STAGES * WK * TILE];
+    __shared__ ScheduleLds plan;
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int hi = lane >> 5, q = lane & 31;
+    const int item = blockIdx.x / a.kv_heads, kh = blockIdx.x % a.kv_heads;
+    int per_split;
+    if (!find_split<BM, STEP>(a, item, target, least, &plan, &per_split)) return;
+    const Split sp = plan.found;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(BM), static_cast<int64_t>(sp.seq.n) * a.group -
+                                                                        static_cast<int64_t>(sp.tile) * BM));
+    const int64_t row_at = static_cast<int64_t>(sp.tile) * BM;
+    const int end = tile_end(sp.seq, a.group, BM, sp.tile);
+    const int least_seen = seen_by(sp.seq, static_cast<int>(row_at / a.group));
+    const int splits = tile_splits<STEP>(sp.splits, end, per_split);
+    if (sp.split >= splits) return;
+    const int steps_all = steps_of(end, STEP), share = (steps_all + splits - 1) / splits;
+    const int k0 = sp.split * share * STEP;
+    const int k1 = min(end, k0 + share * STEP);
+    const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
+    const int wq = wave % WQ, wk = WK == 1 ? 0 : wave;
+
+    // The maximum is taken before the scaling, so a negative scale turns the
+    // queries' signs instead, and scale 0 is queries of 0 (a hidden score of
+    // -inf must not meet a factor of 0).
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
+    const float scale = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
+    // Queries: lane (q, hi) holds elements 16 ks + 8 hi .. + 7 of row q.
+    uint4 qf[RB][KS];
+    int seen[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int r = (wq * RB + rb) * 32 + q;
+        const int64_t row = row_at + (r < rows ? r : 0);
+        const int i = static_cast<int>(row / a.group);
+        seen[rb] = r < rows ? seen_by(sp.seq, i) : 0;
+        const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
+                              (static_cast<int64_t>(kh) * a.group + (row - static_cast<int64_t>(i) * a.group)) *
+                                  a.q_head_stride;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 v = ldg16(src + 16 * ks + 8 * hi);
+            v.x = (v.x ^ flip) & keep; v.y = (v.y ^ flip) & keep; v.z = (v.z ^ flip) & keep; v.w = (v.w ^ flip) & keep;
+            qf[rb][ks] = v;
+        }
+    }
+
+    const CacheView kc = {a.k_cache + kh * a.k_head_stride, a.k_page_stride, a.k_row_stride};
+    const CacheView vc = {a.v_cache + kh * a.v_head_stride, a.v_page_stride, a.v_row_stride};
+    const int32_t* table = a.table + static_cast<int64_t>(sp.b) * a.max_pages;
+    const int last_page = max(end - 1, 0) >> a.page_shift;
+    const int stage_row = WK == 1 ? wave * ROWS : 0;
+    const int mine = k0 + wk * KT + stage_row;   // first position that this wave stages in a step
+    bool bad = false, dirty = false;
+    auto window_at = [&](int p) {
+        PageWindow w;
+        w.first = p >> a.page_shift;
+        w.entry = table[min(w.first + lane, last_page)];
+        return w;
+    };
+    PageWindow win = window_at(min(mine, max(end - 1, 0)));
+    // Moves the window when the ROWS positions from p on are not within it.
+    auto slide = [&](int p) {
+        if (p < end && (min(p + ROWS, end) - 1) >> a.page_shift >= win.first + kWave) win = window_at(p);
+    };
+    const uint32_t lds0 = lds_address(lds);
+    auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage * TILE : wk * TILE); };
+    auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
+    auto stage_k = [&](int j) {
+        stage_rows<D, ROWS, false>(a, kc, win, mine + j * STEP, k1, k_at(j & 1) + stage_row * 2 * D, bad);
+    };
+    auto stage_v = [&](int j) {
+        stage_rows<D, ROWS, true>(a, vc, win, mine + j * STEP, k1, v_at(j & 1) + stage_row * 2 * D, bad);
+    };
+
+    f32x16 o[RB][DB] = {};
+    float m[RB], l[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        m[rb] = kLowest;
+        l[rb] = 0.0f;
+    }
+    const int v_row = 4 * hi + ((lane & 15) >> 2);
+    const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const int v_off = v_row * 2 * D + (lane & 1) * 8;
+
+    // Scores of the tile at position base, softmax, and the weights packed for
+    // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
+    // row and the weights are the second product's operand as they are: of a
+    // step of 16 positions lane (q, hi) holds 4 hi + {0..3, 8..11}.
+    auto scores = [&](uint32_t kt, int base, uint4 (&pw)[RB][2 * NB]) {
+        f32x16 s[RB][NB] = {};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const uint32_t row = kt + (32 * nb + q) * 2 * D;
+            const int sw = k_swizzle<D>(q);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(row + (((2 * ks + hi) ^ sw) << 4));
+                const uint4 kf = make_uint4(kv.x, kv.y, kv.z, kv.w);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) s[rb][nb] = mfma32<FP16>(kf, qf[rb][ks], s[rb][nb]);
+            }
+        }
+        if (base + KT > least_seen) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int p = base + 32 * nb + 8 * (i >> 2) + 4 * hi + (i & 3);
+                        s[rb][nb][i] = p < seen[rb] ? s[rb][nb][i] : -__builtin_inff();
+                    }
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float top = s[rb][0][0];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[rb][nb][i]);
+            top = pair_max(top) * scale;
+            if (__any(top > m[rb] + kSlack)) {
+                const float mn = __builtin_fmaxf(m[rb], top);
+                const float fall = __builtin_amdgcn_exp2f(m[rb] - mn);
+                m[rb] = mn;
+                l[rb] *= fall;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[rb][db][i] *= fall;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][nb][8 * k + j], scale, -m[rb]));
+                        sum += w[j];
+                    }
+                    pw[rb][2 * nb + k] = pack16<FP16>(w);
+                }
+            l[rb] += sum;
+        }
+    };
+    auto values = [&](uint32_t vt, const uint4 (&pw)[RB][2 * NB]) {
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const uint32_t at = vt + 16 * k * 2 * D + v_off + (((4 * db + v_chunk) ^ v_swizzle<D>(v_row)) << 4);
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at));
+                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 8 * 2 * D));
+                const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, up);
+                const uint4 vf = make_uint4(x.x, x.y, y.x, y.y);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) o[rb][db] = mfma32<FP16>(vf, pw[rb][k], o[rb][db]);
+            }
+    };
+    // A value that is not finite among the tile's: all exponent bits set.
+    auto look = [&](uint32_t vt) {
+        constexpr uint32_t E = FP16 ? 0x7c00u : 0x7f80u;
+        for (int i = lane; i < TILE / 16; i += kWave) {
+            const u32x4 v = *reinterpret_cast<lds_u32x4*>(vt + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                dirty |= (v[j] & E) == E || ((v[j] >> 16) & E) == E;
+        }
+    };
+
+    uint4 pw[RB][2 * NB];
+    if constexpr (WK == 1) {
+        if (steps > 0) {
+            stage_k(0);
+            stage_v(0);
+        }
+        for (int j = 0; j < steps; ++j) {
+            const int base = k0 + j * STEP;
+            wait_counts<0, 0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (j + 1 < steps) {
+                slide(mine + (j + 1) * STEP);
+                stage_k(j + 1);
+                stage_v(j + 1);
+            }
+            scores(k_at(j & 1), base, pw);
+            if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
+            values(v_at(j & 1), pw);
+        }
+    } else {
+        if (steps > 0) {
+            stage_k(0);
+            stage_v(0);
+        }
+        for (int j = 0; j < steps; ++j) {
+            const int base = k0 + j * STEP + wk * KT;
+            wait_counts<LOADS, 15>();
+            scores(k_at(0), base, pw);
+            wait_counts<63, 0>();
+            const bool more = j + 1 < steps;
+            if (more) {
+                slide(mine + (j + 1) * STEP);
+                stage_k(j + 1);
+                wait_counts<LOADS, 15>();
+            } else {
+                wait_counts<0, 15>();
+            }
+            if (end > least_seen && base + KT > least_seen) look(v_at(0));
+            values(v_at(0), pw);
+            wait_counts<63, 0>();
+            if (more) stage_v(j + 1);
+        }
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int x = __float_as_int(l[rb]);
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        l[rb] = __int_as_float(r[0]) + __int_as_float(r[1]);
+    }
+    const int flags = __syncthreads_or((bad ? 1 : 0) | (dirty ? 2 : 0));
+    // (__syncthreads_or gives 0 or 1: the two flags one after the other)
+    const bool any_bad = flags && __syncthreads_or(bad);
+    const bool any_dirty = flags && __syncthreads_or(dirty);
+    if (threadIdx.x == 0) part.dirty[blockIdx.x] = any_dirty && !any_bad;
+
+    if constexpr (WK > 1) {
+        // The waves' sums over their own positions, joined in LDS in the
+        // waves' order.
+        float* ml = reinterpret_cast<float*>(lds);           // [WK][32][2]
+        float* acc = ml + WK * 32 * 2;                       // [WK][rows of the tile][D + 4]
+        constexpr int PITCH = D + 4;
+        constexpr int ROOM = (2 * WK * TILE - WK * 32 * 8) / (4 * WK * PITCH);   // rows that fit at once
+        if (hi == 0) {
+            ml[(wk * 32 + q) * 2] = m[0];
+            ml[(wk * 32 + q) * 2 + 1] = l[0];
+        }
+        __syncthreads();
+        float top = kLowest;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = __builtin_fmaxf(top, ml[(w * 32 + q) * 2]);
+        const float fall = __builtin_amdgcn_exp2f(m[0] - top);
+        for (int r0 = 0; r0 < rows; r0 += ROOM) {
+            if (r0 > 0) __syncthreads();
+            if (q >= r0 && q < min(rows, r0 + ROOM)) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        float4 v = make_float4(o[0][db][4 * g] * fall, o[0][db][4 * g + 1] * fall,
+                                               o[0][db][4 * g + 2] * fall, o[0][db][4 * g + 3] * fall);
+                        *reinterpret_cast<float4*>(acc + (wk * ROOM + q - r0) * PITCH + 32 * db + 8 * g + 4 * hi) = v;
+                    }
+            }
+            __syncthreads();
+            const int count = min(rows - r0, ROOM);
+            for (int i = threadIdx.x; i < count * (D / 4); i += kThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROOM + r) * PITCH + d);
+                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                }
+                float rm = kLowest, rl = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) rm = __builtin_fmaxf(rm, ml[(w * 32 + r0 + r) * 2]);
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                    rl += ml[(w * 32 + r0 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r0 + r) * 2] - rm);
+                if (any_bad) rl = __builtin_nanf("");
+                if (splits > 1) {
+                    const int64_t at = ((sp.slot + sp.split) * a.kv_heads + kh) * BM + r0 + r;
+                    *reinterpret_cast<float4*>(part.o + at * D + d) = v;
+                    if (d == 0) *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(rm, rl);
+                } else {
+                    store_row4<FP16>(a, sp.seq, kh, row_at + r0 + r, d, v, rl);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int r = (wq * RB + rb) * 32 + q;
+            const float sum = any_bad ? __builtin_nanf("") : l[rb];
+            const int64_t at = ((sp.slot + sp.split) * a.kv_heads + kh) * BM + r;
+            if (splits > 1 && r < rows && hi == 0)
+                *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(m[rb], sum);
+            if (r < rows) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int d = 32 * db + 8 * g + 4 * hi;
+                        const float4 v = make_float4(o[rb][db][4 * g], o[rb][db][4 * g + 1], o[rb][db][4 * g + 2],
+                                                     o[rb][db][4 * g + 3]);
+                        if (splits > 1) *reinterpret_cast<float4*>(part.o + at * D + d) = v;
+                        else store_row4<FP16>(a, sp.seq, kh, row_at + r, d, v, sum);
+                    }
+            }
+        }
+    }
+}
+
+// Joins the splits of each tile, in their order, and recomputes the rows of
+// dirty tiles one by one.  A workgroup takes pieces of PIECE rows of tiles.
+template <bool FP16, int D, int BM, int STEP>
+__global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a, Partials part, int target, int least) {
+    constexpr int WAVES = kThreads / kWave;
+    constexpr int PIECE = BM / 8 < 8 ? 8 : BM / 8;
+    constexpr int PIECES = BM / PIECE;
+    __shared__ ScheduleLds plan;
+    __shared__ float qs[WAVES][D];
+    __shared__ float ps[WAVES][kWave];
+    __shared__ int64_t vs[WAVES][kWave];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int kh = blockIdx.x % a.kv_heads, piece = blockIdx.x / a.kv_heads % PIECES;
+    const int item = blockIdx.x / a.kv_heads / PIECES;
+    int per_split;
+    if (!find_split<BM, STEP>(a, item, target, least, &plan, &per_split)) return;
+    const Split sp = plan.found;
+    if (sp.split != 0) return;
+    const int end = tile_end(sp.seq, a.group, BM, sp.tile);
+    const int splits = tile_splits<STEP>(sp.splits, end, per_split);
+    bool dirty = false;
+    for (int s = 0; s < splits; ++s) {
+        const int at = (item + s) * a.kv_heads + kh;
+        if (at < part.splits) dirty |= part.dirty[at] != 0;
+    }
+    if (splits == 1 && !dirty) return;
+    const int64_t row_at = static_cast<int64_t>(sp.tile) * BM;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(BM), static_cast<int64_t>(sp.seq.n) * a.group - row_at));
+    for (int r = piece * PIECE + wave; r < min(rows, (piece + 1) * PIECE); r += WAVES) {
+        if (dirty) {
+            const int i = static_cast<int>((row_at + r) / a.group);
+            attend_row<FP16, D>(a, sp.b, sp.seq.first + i, kh * a.group + static_cast<int>((row_at + r) % a.group),
+                                seen_by(sp.seq, i), qs[wave], ps[wave], vs[wave]);
+            continue;
+        }
+        float m = kLowest;
+        const int64_t step = static_cast<int64_t>(a.kv_heads) * BM;
+        const int64_t at = (sp.slot * a.kv_heads + kh) * BM + r;
+        for (int s = 0; s < splits; ++s) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
+        float l = 0.0f;
+        constexpr int E = D / 4 < kWave ? D / 4 : kWave;   // lanes that hold elements, four each
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int s = 0; s < splits; ++s) {
+            const float2 x = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
+            const float w = __builtin_amdgcn_exp2f(x.x - m);
+            l += w * x.y;
+            if (lane < E) {
+                const float4 y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
+                v.x = __builtin_fmaf(w, y.x, v.x);
+                v.y = __builtin_fmaf(w, y.y, v.y);
+                v.z = __builtin_fmaf(w, y.z, v.z);
+                v.w = __builtin_fmaf(w, y.w, v.w);
+            }
+        }
+        if (lane < E) store_row4<FP16>(a, sp.seq, kh, row_at + r, 4 * lane, v, l);
+    }
+}
+
+constexpr int kTarget = 512;   // splits that fill the chip (two per CU)
+
+struct Shape {
+    int bm, step, least;
+};
+// The kernel of a step: one 32-row tile of four position groups where every
+// sequence's rows fit into it, else tiles of 128 rows.
+Shape shape_of(int group, int max_new) {
+    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 2};
+    return {128, 64, 16};
+}
+int64_t most_splits(int tokens, int seqs, int group, int kv_heads, int bm) {
+    const int64_t tiles = static_cast<int64_t>(tokens) * group / bm + (seqs < tokens ? seqs : tokens);
+    return kTarget + kv_heads * tiles;
+}
+
 }  // namespace
 
-size_t paged_attn_workspace_bytes(int, int, int, int, int, int) { return 0; }
+namespace {
+struct Layout {
+    Partials part;
+    size_t bytes;
+};
+Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
+    const Shape sh = shape_of(heads / kv_heads, max_new);
+    const int64_t splits = most_splits(tokens, seqs, heads / kv_heads, kv_heads, sh.bm);
+    const int64_t slots = 2 * kTarget;
+    uint8_t* p = static_cast<uint8_t*>(base);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t* r = p + at;
+        at += (bytes + 255) & ~static_cast<size_t>(255);
+        return r;
+    };
+    Layout l;
+    l.part.splits = static_cast<int>(splits);
+    l.part.slots = static_cast<int>(slots);
+    l.part.dirty = reinterpret_cast<int*>(take(splits * 4));
+    l.part.ml = reinterpret_cast<float*>(take(slots * sh.bm * 8));
+    l.part.o = reinterpret_cast<float*>(take(slots * sh.bm * static_cast<size_t>(dim) * 4));
+    l.bytes = at;
+    return l;
+}
 
-hipError_t launch_paged_attention(const PagedAttnArgs& a, bool fp16, int dim, int, void*, hipStream_t stream) {
-    const int64_t items = static_cast<int64_t>(a.tokens) * a.heads;
-    const dim3 grid(static_cast<unsigned>((items + 3) / 4));
-#define LR_ROW(F, N) hipLaunchKernelGGL((attend_row_kernel<F, N>), grid, dim3(kThreads), 0, stream, a)
-    if (dim == 64) { if (fp16) LR_ROW(true, 64); else LR_ROW(false, 64); }
-    else if (dim == 128) { if (fp16) LR_ROW(true, 128); else LR_ROW(false, 128); }
-    else { if (fp16) LR_ROW(true, 256); else LR_ROW(false, 256); }
-#undef LR_ROW
+template <bool FP16, int D>
+hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
+    const Shape sh = shape_of(a.group, max_new);
+    const unsigned grid = part.splits;
+#define LR_ATTEND(RB, WQ, WK, NB)                                                                                 \
+    do {                                                                                                          \
+        constexpr int BM = 32 * RB * WQ, STEP = 32 * NB * WK, PIECES = BM / (BM / 8 < 8 ? 8 : BM / 8);            \
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, RB, WQ, WK, NB>), dim3(grid), dim3(kThreads), 0, stream,  \
+                           a, part, kTarget, sh.least);                                                           \
+        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, BM, STEP>), dim3(grid * PIECES), dim3(kThreads), 0,      \
+                           stream, a, part, kTarget, sh.least);                                                   \
+    } while (0)
+    if (sh.bm == 32) LR_ATTEND(1, 1, 4, 1);
+    else LR_ATTEND(1, 4, 1, 2);
+#undef LR_ATTEND
     return hipGetLastError();
+}
+}  // namespace
+
+size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
+    return carve(nullptr, tokens, seqs, heads, kv_heads, dim, max_new).bytes;
+}
+
+hipError_t launch_paged_attention(const PagedAttnArgs& a, bool fp16, int dim, int max_new, void* workspace,
+                                  hipStream_t stream) {
+    const Partials part = carve(workspace, a.tokens, a.seqs, a.heads, a.kv_heads, dim, max_new).part;
+    if (dim == 64) return fp16 ? launch<true, 64>(a, max_new, part, stream) : launch<false, 64>(a, max_new, part, stream);
+    if (dim == 128)
+        return fp16 ? launch<true, 128>(a, max_new, part, stream) : launch<false, 128>(a, max_new, part, stream);
+    return fp16 ? launch<true, 256>(a, max_new, part, stream) : launch<false, 256>(a, max_new, part, stream);
 }
 
 }  // namespace lrmoe
