@@ -786,8 +786,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args* p, void* stream) {
 static bool bad_attention(const lrmoe_paged_attention_args* p) {
     return p->seqs < 0 || p->seqs > LRMOE_PAGE_MAX_ROWS || p->tokens < 0 || p->tokens > (1 << 20) || p->max_new < 0 ||
            p->heads < 1 || p->heads > 1024 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || bad_dim(p->dim) ||
-           p->pages < 1 || bad_page(p->page) || p->max_pages < 1 ||
-           static_cast<int64_t>(p->max_pages) * p->page > INT32_MAX;
+           static_cast<int64_t>(p->tokens) * p->heads > (1 << 28) || p->pages < 1 || bad_page(p->page) ||
+           p->max_pages < 1 || static_cast<int64_t>(p->max_pages) * p->page > INT32_MAX;
 }
 
 size_t lrmoe_paged_attention_workspace_bytes(const lrmoe_paged_attention_args* p) {

@@ -5,6 +5,12 @@
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
+#include <stdlib.h>
+static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+#define TARGET_FEW envi("TF", 512)
+#define LEAST_FEW envi("LF", 1)
+#define TARGET_TILE envi("TT", 512)
+#define LEAST_TILE envi("LT", 16)
 
 namespace lrmoe {
 namespace {
@@ -97,63 +103,31 @@ __device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t 
 // group) are cut into tiles of BM rows; a tile's positions into splits, so
 // that a few long sequences fill the chip: with W steps of positions in all,
 // a split holds more than W / target steps, so that there are at most target
-// splits and one per tile, and fewer than 2 target of tiles that are split.  Every workgroup works this
-// out for itself from starts and kv_lengths (up to 16 sequences per thread):
-// nothing of it depends on the host, and no launch precedes the attention's.
+// splits and one per tile, and fewer than 2 target of tiles that are split.
+// Every wave works this out for itself from starts and kv_lengths (a lane per
+// sequence, cross-lane sums, no LDS and no barrier): nothing of it depends on
+// the host, no launch precedes the attention's, and what it costs is the one
+// round trip for the two arrays.
 
 struct Sequence {
     int first, n, kv;  // first token, new tokens, cached positions
 };
-__device__ __forceinline__ Sequence sequence_at(const PagedAttnArgs& a, int b) {
-    Sequence s;
-    s.first = min(max(a.starts[b], 0), a.tokens);
-    s.n = max(min(a.starts[b + 1], a.tokens) - s.first, 0);
-    const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
-    s.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lengths[b], 0)), capacity));
-    return s;
-}
 // Positions that token i of the sequence sees.
 __device__ __forceinline__ int seen_by(const Sequence& s, int i) { return max(s.kv - s.n + i + 1, 0); }
 
 struct Split {
     int b, tile, split, splits;
-    int64_t slot;  // of the tile's first partial rows, before the head; -1 for a sequence in one piece
+    int slot;       // of the tile's first partial rows, before the head
+    int per_split;  // steps
     Sequence seq;
 };
 
-__device__ __forceinline__ int tiles_of(const Sequence& s, int group, int bm) {
-    return static_cast<int>((static_cast<int64_t>(s.n) * group + bm - 1) / bm);
-}
+__device__ __forceinline__ int tiles_of(int n, int group, int bm) { return (n * group + bm - 1) / bm; }
 __device__ __forceinline__ int steps_of(int positions, int step) { return max((positions + step - 1) / step, 1); }
 // Positions that the tile's last row sees.
 __device__ __forceinline__ int tile_end(const Sequence& s, int group, int bm, int tile) {
-    const int64_t rows = min(static_cast<int64_t>(tile + 1) * bm, static_cast<int64_t>(s.n) * group);
-    return seen_by(s, static_cast<int>((rows - 1) / group));
-}
-
-// Steps per split: the first count above W / target, not under `least`.
-template <int BM, int STEP>
-__device__ __forceinline__ int split_steps(const PagedAttnArgs& a, int target, int least, double* lds) {
-    const int per = (a.seqs + kThreads - 1) / kThreads;
-    double work = 0.0;   // (a product of counts that a bad `starts` could make pass 64 bits)
-    for (int i = 0; i < per; ++i) {
-        const int b = threadIdx.x * per + i;
-        if (b >= a.seqs) break;
-        const Sequence s = sequence_at(a, b);
-        if (s.n > 0) work += static_cast<double>(tiles_of(s, a.group, BM)) * steps_of(s.kv, STEP);
-    }
-#pragma unroll
-    for (int off = 1; off < kWave; off *= 2) work += __shfl_xor(work, off);
-    if (__lane_id() == 0) lds[threadIdx.x / kWave] = work;
-    __syncthreads();
-    work = (lds[0] + lds[1] + lds[2] + lds[3]) * a.kv_heads;
-    __syncthreads();
-    const double c = work / target;
-    return max(c < 1.0e9 ? static_cast<int>(c) + 1 : 1 << 30, least);
-}
-template <int BM, int STEP>
-__device__ __forceinline__ int splits_of(const PagedAttnArgs& a, const Sequence& s, int per_split) {
-    return (steps_of(s.kv, STEP) + per_split - 1) / per_split;
+    const int rows = min((tile + 1) * bm, s.n * group);
+    return seen_by(s, (rows - 1) / group);
 }
 // A tile takes its sequence's split count, or fewer where causality leaves it
 // fewer steps.
@@ -162,86 +136,97 @@ __device__ __forceinline__ int tile_splits(int splits, int end, int per_split) {
     return min(splits, (steps_of(end, STEP) + per_split - 1) / per_split);
 }
 
-// Where each sequence's splits (of all its tiles, per head) begin, and its
-// partial slots; then the sequence of split `item` (in LDS as *found), heavy
-// tiles first.  Returns false past the last split.
-struct ScheduleLds {
-    double sums[kThreads / kWave];
-    Split found;
-    int64_t scan[2][kThreads / kWave];
-};
+// Inclusive sum over the lanes (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// The sequence, tile and split of item `item` (wave-uniform), heavy tiles
+// first; false past the last one, and for starts that are not ascending
+// within [0, tokens] (such a step is empty).
 template <int BM, int STEP>
-__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, ScheduleLds* lds,
-                                           int* per_split) {
-    const int c = split_steps<BM, STEP>(a, target, least, lds->sums);
-    *per_split = c;
-    const int per = (a.seqs + kThreads - 1) / kThreads;
-    int64_t items = 0, slots = 0;
-    for (int i = 0; i < per; ++i) {
-        const int b = threadIdx.x * per + i;
-        if (b >= a.seqs) break;
-        const Sequence s = sequence_at(a, b);
-        if (s.n == 0) continue;
-        const int splits = splits_of<BM, STEP>(a, s, c);
-        const int64_t all = static_cast<int64_t>(tiles_of(s, a.group, BM)) * splits;
-        items += all;
-        slots += splits > 1 ? all : 0;
-    }
-    int64_t at = items, slot = slots;
+__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out) {
+    constexpr int HELD = 4;   // sequences per lane that stay in registers
+    const int lane = threadIdx.x % kWave;
+    const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
+    Sequence s[HELD];
+    bool bad = false;
+    auto load = [&](int base) {
 #pragma unroll
-    for (int off = 1; off < kWave; off *= 2) {
-        const int64_t up = __shfl_up(at, off), us = __shfl_up(slot, off);
-        if (static_cast<int>(__lane_id()) >= off) {
-            at += up;
-            slot += us;
+        for (int k = 0; k < HELD; ++k) {
+            const int b = base + k * kWave + lane;
+            const bool in = b < a.seqs;
+            const int first = a.starts[in ? b : 0], next = a.starts[in ? b + 1 : 0], kv = a.kv_lengths[in ? b : 0];
+            bad |= first < 0 || next < first || next > a.tokens;
+            s[k].first = first;
+            s[k].n = next - first;   // 0 past the last sequence
+            s[k].kv = static_cast<int>(min(static_cast<int64_t>(max(kv, 0)), capacity));
         }
+    };
+    float work = 0.0f;
+    for (int base = 0; base < a.seqs; base += HELD * kWave) {
+        load(base);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+            if (s[k].n > 0) work += static_cast<float>(tiles_of(s[k].n, a.group, BM)) * steps_of(s[k].kv, STEP);
     }
-    const int wave = threadIdx.x / kWave;
-    if (__lane_id() == kWave - 1) {
-        lds->scan[0][wave] = at;
-        lds->scan[1][wave] = slot;
-    }
-    if (threadIdx.x == 0) lds->found.b = -1;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-        at += lds->scan[0][w];
-        slot += lds->scan[1][w];
-    }
-    at -= items;
-    slot -= slots;
-    if (item >= at && item < at + items) {
-        for (int i = 0; i < per; ++i) {
-            const int b = threadIdx.x * per + i;
-            if (b >= a.seqs) break;
-            const Sequence s = sequence_at(a, b);
-            if (s.n == 0) continue;
-            const int splits = splits_of<BM, STEP>(a, s, c), tiles = tiles_of(s, a.group, BM);
-            const int64_t all = static_cast<int64_t>(tiles) * splits;
+    if (__any(bad)) return false;
+    work = wave_butterfly_sum(work) * a.kv_heads;
+    const float each = work / target;
+    const int c = __builtin_amdgcn_readfirstlane(max(each < 1.0e9f ? static_cast<int>(each) + 1 : 1 << 30, least));
+    int at = 0, slot = 0;
+    for (int base = 0; base < a.seqs; base += HELD * kWave) {
+        if (a.seqs > HELD * kWave) load(base);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            if (base + k * kWave >= a.seqs) break;
+            const int splits = (steps_of(s[k].kv, STEP) + c - 1) / c;
+            const int items = tiles_of(s[k].n, a.group, BM) * splits, slots = splits > 1 ? items : 0;
+            const int upto = wave_scan(items), upto_slots = wave_scan(slots);
+            const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item < at + all) {
-                const int local = static_cast<int>(item - at);
-                lds->found.b = b;
-                lds->found.tile = tiles - 1 - local / splits;
-                lds->found.split = local % splits;
-                lds->found.splits = splits;
-                lds->found.slot = splits > 1 ? slot + static_cast<int64_t>(lds->found.tile) * splits : -1;
-                lds->found.seq = s;
-                break;
+                const int who = __builtin_ctzll(__ballot(item < at + upto));
+                const int local = item - at - __builtin_amdgcn_readlane(upto - items, who);
+                out->b = base + k * kWave + who;
+                out->splits = __builtin_amdgcn_readlane(splits, who);
+                out->seq.first = __builtin_amdgcn_readlane(s[k].first, who);
+                out->seq.n = __builtin_amdgcn_readlane(s[k].n, who);
+                out->seq.kv = __builtin_amdgcn_readlane(s[k].kv, who);
+                const int up = local / out->splits;
+                out->tile = tiles_of(out->seq.n, a.group, BM) - 1 - up;
+                out->split = local - up * out->splits;
+                out->slot = slot + __builtin_amdgcn_readlane(upto_slots - slots, who) + out->tile * out->splits;
+                out->per_split = c;
+                return true;
             }
             at += all;
-            slot += splits > 1 ? all : 0;
+            slot += __builtin_amdgcn_readlane(upto_slots, 63);
         }
     }
-    __syncthreads();
-    return lds->found.b >= 0;
+    return false;
 }
+
+// What the attention launch leaves for the merge, one per workgroup.
+struct Piece {
+    int splits;   // of the tile, at its first split; 0 elsewhere and past the last
+    int dirty;    // values that some of the tile's rows must not see
+    int b, tile, slot;
+    Sequence seq;
+};
 
 // Four elements d .. d + 3 of a row's result: sums over l, times the gate,
 // rounded once.
 template <bool FP16>
-__device__ __forceinline__ void store_row4(const PagedAttnArgs& a, const Sequence& s, int kh, int64_t row, int d,
+__device__ __forceinline__ void store_row4(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
                                            float4 v, float l) {
-    const int64_t i = row / a.group;
-    const int64_t t = s.first + i, h = static_cast<int64_t>(kh) * a.group + (row - i * a.group);
+    const int i = row / a.group;
+    const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
     if (a.gate != nullptr) {
@@ -367,8 +352,8 @@ __device__ __forceinline__ float pair_max(float v) {
 struct Partials {
     float* o;     // [slot][BM][D] sums of exp2(s - m) v
     float* ml;    // [slot][BM][2] m, sum of exp2(s - m)
-    int* dirty;   // [splits]
-    int slots, splits;  // how many there is room for
+    Piece* pieces;  // [workgroups of the attention launch]
+    int workgroups;
 };
 
 constexpr float kLowest = -1.7e38f;  // the running maximum before any position
@@ -386,21 +371,21 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     constexpr int ROWS = WK == 1 ? KT / 4 : KT;   // rows that a wave stages
     constexpr int LOADS = ROWS * D / 512;         // of a key or value tile, per wave
     __shared__ __align__(1024) uint8_t lds[2 * STAGES * WK * TILE];
-    __shared__ ScheduleLds plan;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int hi = lane >> 5, q = lane & 31;
     const int item = blockIdx.x / a.kv_heads, kh = blockIdx.x % a.kv_heads;
-    int per_split;
-    if (!find_split<BM, STEP>(a, item, target, least, &plan, &per_split)) return;
-    const Split sp = plan.found;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(BM), static_cast<int64_t>(sp.seq.n) * a.group -
-                                                                        static_cast<int64_t>(sp.tile) * BM));
-    const int64_t row_at = static_cast<int64_t>(sp.tile) * BM;
-    const int end = tile_end(sp.seq, a.group, BM, sp.tile);
-    const int least_seen = seen_by(sp.seq, static_cast<int>(row_at / a.group));
-    const int splits = tile_splits<STEP>(sp.splits, end, per_split);
-    if (sp.split >= splits) return;
+    Split sp;
+    const bool live = find_split<BM, STEP>(a, item, target, least, &sp);
+    const int end = live ? tile_end(sp.seq, a.group, BM, sp.tile) : 0;
+    const int splits = live ? tile_splits<STEP>(sp.splits, end, sp.per_split) : 0;
+    if (!live || sp.split >= splits) {
+        if (threadIdx.x == 0) part.pieces[blockIdx.x].splits = 0;
+        return;
+    }
+    const int row_at = sp.tile * BM;
+    const int rows = min(BM, sp.seq.n * a.group - row_at);
+    const int least_seen = seen_by(sp.seq, row_at / a.group);
     const int steps_all = steps_of(end, STEP), share = (steps_all + splits - 1) / splits;
     const int k0 = sp.split * share * STEP;
     const int k1 = min(end, k0 + share * STEP);
@@ -418,12 +403,11 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int r = (wq * RB + rb) * 32 + q;
-        const int64_t row = row_at + (r < rows ? r : 0);
-        const int i = static_cast<int>(row / a.group);
+        const int row = row_at + (r < rows ? r : 0);
+        const int i = row / a.group;
         seen[rb] = r < rows ? seen_by(sp.seq, i) : 0;
         const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
-                              (static_cast<int64_t>(kh) * a.group + (row - static_cast<int64_t>(i) * a.group)) *
-                                  a.q_head_stride;
+                              (kh * a.group + row - i * a.group) * a.q_head_stride;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             uint4 v = ldg16(src + 16 * ks + 8 * hi);
@@ -613,7 +597,8 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     // (__syncthreads_or gives 0 or 1: the two flags one after the other)
     const bool any_bad = flags && __syncthreads_or(bad);
     const bool any_dirty = flags && __syncthreads_or(dirty);
-    if (threadIdx.x == 0) part.dirty[blockIdx.x] = any_dirty && !any_bad;
+    if (threadIdx.x == 0)
+        part.pieces[blockIdx.x] = {sp.split == 0 ? splits : 0, any_dirty && !any_bad, sp.b, sp.tile, sp.slot, sp.seq};
 
     if constexpr (WK > 1) {
         // The waves' sums over their own positions, joined in LDS in the
@@ -661,7 +646,7 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
                     rl += ml[(w * 32 + r0 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r0 + r) * 2] - rm);
                 if (any_bad) rl = __builtin_nanf("");
                 if (splits > 1) {
-                    const int64_t at = ((sp.slot + sp.split) * a.kv_heads + kh) * BM + r0 + r;
+                    const int64_t at = (static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh) * BM + r0 + r;
                     *reinterpret_cast<float4*>(part.o + at * D + d) = v;
                     if (d == 0) *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(rm, rl);
                 } else {
@@ -674,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
         for (int rb = 0; rb < RB; ++rb) {
             const int r = (wq * RB + rb) * 32 + q;
             const float sum = any_bad ? __builtin_nanf("") : l[rb];
-            const int64_t at = ((sp.slot + sp.split) * a.kv_heads + kh) * BM + r;
+            const int64_t at = (static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh) * BM + r;
             if (splits > 1 && r < rows && hi == 0)
                 *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(m[rb], sum);
             if (r < rows) {
@@ -693,91 +678,96 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     }
 }
 
-// Joins the splits of each tile, in their order, and recomputes the rows of
-// dirty tiles one by one.  A workgroup takes pieces of PIECE rows of tiles.
-template <bool FP16, int D, int BM, int STEP>
-__global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a, Partials part, int target, int least) {
+// Joins the splits of each tile, in their order (a row's splits over the four
+// waves, then the waves), and recomputes the rows of dirty tiles one by one.
+// Workgroup (piece, i) takes rows i, i + gridDim.y, ... of its piece's tile.
+template <bool FP16, int D, int BM>
+__global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a, Partials part) {
     constexpr int WAVES = kThreads / kWave;
-    constexpr int PIECE = BM / 8 < 8 ? 8 : BM / 8;
-    constexpr int PIECES = BM / PIECE;
-    __shared__ ScheduleLds plan;
+    constexpr int E = D / 4;   // lanes that hold elements, four each
     __shared__ float qs[WAVES][D];
     __shared__ float ps[WAVES][kWave];
     __shared__ int64_t vs[WAVES][kWave];
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int kh = blockIdx.x % a.kv_heads, piece = blockIdx.x / a.kv_heads % PIECES;
-    const int item = blockIdx.x / a.kv_heads / PIECES;
-    int per_split;
-    if (!find_split<BM, STEP>(a, item, target, least, &plan, &per_split)) return;
-    const Split sp = plan.found;
-    if (sp.split != 0) return;
-    const int end = tile_end(sp.seq, a.group, BM, sp.tile);
-    const int splits = tile_splits<STEP>(sp.splits, end, per_split);
-    bool dirty = false;
-    for (int s = 0; s < splits; ++s) {
-        const int at = (item + s) * a.kv_heads + kh;
-        if (at < part.splits) dirty |= part.dirty[at] != 0;
+    __shared__ float sums[WAVES];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const Piece pc = part.pieces[blockIdx.x];
+    if (pc.splits == 0) return;
+    int dirty = pc.dirty;
+    for (int s = lane; s < pc.splits; s += kWave) {
+        const int at = static_cast<int>(blockIdx.x) + s * a.kv_heads;
+        if (at < part.workgroups) dirty |= part.pieces[at].dirty;
     }
-    if (splits == 1 && !dirty) return;
-    const int64_t row_at = static_cast<int64_t>(sp.tile) * BM;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(BM), static_cast<int64_t>(sp.seq.n) * a.group - row_at));
-    for (int r = piece * PIECE + wave; r < min(rows, (piece + 1) * PIECE); r += WAVES) {
-        if (dirty) {
-            const int i = static_cast<int>((row_at + r) / a.group);
-            attend_row<FP16, D>(a, sp.b, sp.seq.first + i, kh * a.group + static_cast<int>((row_at + r) % a.group),
-                                seen_by(sp.seq, i), qs[wave], ps[wave], vs[wave]);
-            continue;
+    const bool any_dirty = __any(dirty);
+    if (pc.splits == 1 && !any_dirty) return;
+    const int kh = blockIdx.x % a.kv_heads, row_at = pc.tile * BM;
+    const int rows = min(BM, pc.seq.n * a.group - row_at);
+    if (any_dirty) {
+        for (int r = blockIdx.y * WAVES + wave; r < rows; r += gridDim.y * WAVES) {
+            const int i = (row_at + r) / a.group;
+            attend_row<FP16, D>(a, pc.b, pc.seq.first + i, kh * a.group + row_at + r - i * a.group,
+                                seen_by(pc.seq, i), qs[wave], ps[wave], vs[wave]);
         }
+        return;
+    }
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * BM;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const int64_t at = (static_cast<int64_t>(pc.slot) * a.kv_heads + kh) * BM + r;
         float m = kLowest;
-        const int64_t step = static_cast<int64_t>(a.kv_heads) * BM;
-        const int64_t at = (sp.slot * a.kv_heads + kh) * BM + r;
-        for (int s = 0; s < splits; ++s) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
+        for (int s = lane; s < pc.splits; s += kWave) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, off));
         float l = 0.0f;
-        constexpr int E = D / 4 < kWave ? D / 4 : kWave;   // lanes that hold elements, four each
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+        for (int s = wave; s < pc.splits; s += WAVES) {
             const float2 x = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (lane < E) y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
             const float w = __builtin_amdgcn_exp2f(x.x - m);
-            l += w * x.y;
-            if (lane < E) {
-                const float4 y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
-                v.x = __builtin_fmaf(w, y.x, v.x);
-                v.y = __builtin_fmaf(w, y.y, v.y);
-                v.z = __builtin_fmaf(w, y.z, v.z);
-                v.w = __builtin_fmaf(w, y.w, v.w);
-            }
+            l = __builtin_fmaf(w, x.y, l);
+            v.x = __builtin_fmaf(w, y.x, v.x);
+            v.y = __builtin_fmaf(w, y.y, v.y);
+            v.z = __builtin_fmaf(w, y.z, v.z);
+            v.w = __builtin_fmaf(w, y.w, v.w);
         }
-        if (lane < E) store_row4<FP16>(a, sp.seq, kh, row_at + r, 4 * lane, v, l);
+        if (lane < E) *reinterpret_cast<float4*>(&qs[wave][4 * lane]) = v;
+        if (lane == 0) sums[wave] = l;
+        __syncthreads();
+        if (wave == 0 && lane < E) {
+            l = 0.0f;
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float4 y = *reinterpret_cast<const float4*>(&qs[w][4 * lane]);
+                l += sums[w];
+                v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+            }
+            store_row4<FP16>(a, pc.seq, kh, row_at + r, 4 * lane, v, l);
+        }
+        __syncthreads();
     }
 }
 
-constexpr int kTarget = 512;   // splits that fill the chip (two per CU)
-
 struct Shape {
-    int bm, step, least;
+    int bm, target, least;
 };
 // The kernel of a step: one 32-row tile of four position groups where every
 // sequence's rows fit into it, else tiles of 128 rows.
 Shape shape_of(int group, int max_new) {
-    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 2};
-    return {128, 64, 16};
-}
-int64_t most_splits(int tokens, int seqs, int group, int kv_heads, int bm) {
-    const int64_t tiles = static_cast<int64_t>(tokens) * group / bm + (seqs < tokens ? seqs : tokens);
-    return kTarget + kv_heads * tiles;
+    if (static_cast<int64_t>(max_new) * group <= 32) return {32, TARGET_FEW, LEAST_FEW};
+    return {128, TARGET_TILE, LEAST_TILE};
 }
 
-}  // namespace
-
-namespace {
 struct Layout {
     Partials part;
     size_t bytes;
 };
 Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
-    const Shape sh = shape_of(heads / kv_heads, max_new);
-    const int64_t splits = most_splits(tokens, seqs, heads / kv_heads, kv_heads, sh.bm);
-    const int64_t slots = 2 * kTarget;
+    const int group = heads / kv_heads;
+    const Shape sh = shape_of(group, max_new);
+    const int64_t tiles = static_cast<int64_t>(tokens) * group / sh.bm + (seqs < tokens ? seqs : tokens);
+    const int64_t workgroups = (sh.target / kv_heads + 1 + tiles) * kv_heads;
+    const int64_t slots = 2 * sh.target + 16;   // (16: the work is summed in 24 bits)
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -786,9 +776,8 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
         return r;
     };
     Layout l;
-    l.part.splits = static_cast<int>(splits);
-    l.part.slots = static_cast<int>(slots);
-    l.part.dirty = reinterpret_cast<int*>(take(splits * 4));
+    l.part.workgroups = static_cast<int>(workgroups);
+    l.part.pieces = reinterpret_cast<Piece*>(take(workgroups * sizeof(Piece)));
     l.part.ml = reinterpret_cast<float*>(take(slots * sh.bm * 8));
     l.part.o = reinterpret_cast<float*>(take(slots * sh.bm * static_cast<size_t>(dim) * 4));
     l.bytes = at;
@@ -798,20 +787,22 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
 template <bool FP16, int D>
 hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
     const Shape sh = shape_of(a.group, max_new);
-    const unsigned grid = part.splits;
+    const unsigned grid = part.workgroups;
+    const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
+    const unsigned rows = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
 #define LR_ATTEND(RB, WQ, WK, NB)                                                                                 \
     do {                                                                                                          \
-        constexpr int BM = 32 * RB * WQ, STEP = 32 * NB * WK, PIECES = BM / (BM / 8 < 8 ? 8 : BM / 8);            \
         hipLaunchKernelGGL((attend_tile_kernel<FP16, D, RB, WQ, WK, NB>), dim3(grid), dim3(kThreads), 0, stream,  \
-                           a, part, kTarget, sh.least);                                                           \
-        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, BM, STEP>), dim3(grid * PIECES), dim3(kThreads), 0,      \
-                           stream, a, part, kTarget, sh.least);                                                   \
+                           a, part, sh.target, sh.least);                                                         \
+        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * RB * WQ>), dim3(grid, rows), dim3(kThreads), 0,     \
+                           stream, a, part);                                                                      \
     } while (0)
     if (sh.bm == 32) LR_ATTEND(1, 1, 4, 1);
     else LR_ATTEND(1, 4, 1, 2);
 #undef LR_ATTEND
     return hipGetLastError();
 }
+
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
