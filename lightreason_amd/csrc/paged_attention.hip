@@ -7,7 +7,10 @@
 #include "paged.h"
 #include <stdlib.h>
 static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#define TARGET_FEW envi("TF", 512)
+#ifndef AHEADN
+#define AHEADN 4
+#endif
+#define TARGET_FEW envi("TF", 1024)
 #define LEAST_FEW envi("LF", 1)
 #define TARGET_TILE envi("TT", 512)
 #define LEAST_TILE envi("LT", 16)
@@ -245,6 +248,7 @@ __device__ __forceinline__ void store_row4(const PagedAttnArgs& a, const Sequenc
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) const uint8_t lds_u8;
 typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 
 template <bool FP16>
@@ -313,33 +317,67 @@ struct CacheView {
     int64_t row_stride;
 };
 
+// ROWS rows from position `pos` on, `row0` rows into their tile, for the
+// positions before `end` (zeros past it).  A page holds at least 8 rows, so
+// one table entry serves UNIT rows.
 template <int D, int ROWS, bool VALUES>
 __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win, int pos,
-                                           int end, uint32_t lds_at, bool& bad) {
+                                           int end, int row0, uint32_t lds_at, bool& bad) {
+    constexpr int UNIT = 8;
     constexpr int PER = 512 / D;    // rows per load of the wave
     constexpr int CHUNKS = D / 8;
     const int lane = threadIdx.x % kWave;
     const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
+    const uint32_t pitch = static_cast<uint32_t>(2 * c.row_stride);   // bytes
+    const uint32_t lane_at = static_cast<uint32_t>(lrow) * pitch;
+    auto chunk = [&](int row) {
+        return 16 * (lchunk ^ (VALUES ? v_swizzle<D>(row0 + row + lrow) : k_swizzle<D>(row0 + row + lrow)));
+    };
+    auto page_of = [&](int p) {
+        int entry = __builtin_amdgcn_readlane(win.entry, (p >> a.page_shift) - win.first);
+        const bool in = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages);
+        bad |= !in;
+        entry = in ? entry : 0;
+        return reinterpret_cast<const uint8_t*>(c.data + entry * c.page_stride) +
+               static_cast<uint64_t>(p & ((1 << a.page_shift) - 1)) * pitch;
+    };
+    if (pos + ROWS <= end) {
 #pragma unroll
-    for (int i = 0; i < ROWS / PER; ++i) {
-        const int row = i * PER;      // of the ROWS; the tile's rows are a multiple of 16 before it
-        const int p = pos + row;
-        const uint32_t at = lds_at + row * 2 * D;
-        const int chunk = lchunk ^ (VALUES ? v_swizzle<D>(row + lrow) : k_swizzle<D>(row + lrow));
-        const int page = p < end ? (p >> a.page_shift) - win.first : 0;
-        int entry = __builtin_amdgcn_readlane(win.entry, page);
-        if (p < end && static_cast<uint32_t>(entry) >= static_cast<uint32_t>(a.pages)) bad = true;
-        entry = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages) ? entry : 0;
-        const uint16_t* base =
-            c.data + entry * c.page_stride + (p & ((1 << a.page_shift) - 1)) * c.row_stride;
-        const uint32_t offset = static_cast<uint32_t>(lrow) * static_cast<uint32_t>(2 * c.row_stride) + 16 * chunk;
-        if (p + PER <= end) {
-            load_lds16(at, base, offset);
-        } else {
-            const uint8_t* from = reinterpret_cast<const uint8_t*>(base) + offset;
-            load_lds16(at, p + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
+        for (int u = 0; u < ROWS; u += UNIT) {
+            const uint8_t* base = page_of(pos + u);
+#pragma unroll
+            for (int i = 0; i < UNIT; i += PER)
+                load_lds16(lds_at + (u + i) * 2 * D, base + i * static_cast<uint64_t>(pitch), chunk(u + i) + lane_at);
+        }
+    } else {
+#pragma unroll 1
+        for (int u = 0; u < ROWS; u += UNIT) {
+            const uint8_t* base = pos + u < end ? page_of(pos + u) : nullptr;
+#pragma unroll
+            for (int i = 0; i < UNIT; i += PER) {
+                const uint8_t* from = base + i * static_cast<uint64_t>(pitch) + lane_at + chunk(u + i);
+                load_lds16(lds_at + (u + i) * 2 * D,
+                           pos + u + i + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
+            }
         }
     }
+}
+
+// Orders the LDS reads of FRAGS operand fragments (READS instructions each)
+// and the products that take them: AHEAD fragments before the first product,
+// then one more after each fragment's USES products.  Left to itself the
+// compiler reads each fragment right before its product, to save registers,
+// and every product waits for LDS.
+template <int FRAGS, int READS, int USES>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int AHEAD = AHEADN, PRODUCT = 0x8, LDS_READ = 0x100;
+    __builtin_amdgcn_sched_group_barrier(LDS_READ, AHEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < FRAGS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(PRODUCT, USES, 0);
+        __builtin_amdgcn_sched_group_barrier(LDS_READ, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD * USES, 0);
 }
 
 // Highest value and sum over the two lanes (q, q + 32) that share a row.
@@ -360,7 +398,7 @@ constexpr float kLowest = -1.7e38f;  // the running maximum before any position
 constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
 
 template <bool FP16, int D, int RB, int WQ, int WK, int NB>
-__global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
+__global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
     static_assert(WQ * WK == kThreads / kWave, "four waves");
     constexpr int KT = 32 * NB;           // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
@@ -438,10 +476,10 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage * TILE : wk * TILE); };
     auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
     auto stage_k = [&](int j) {
-        stage_rows<D, ROWS, false>(a, kc, win, mine + j * STEP, k1, k_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, false>(a, kc, win, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
     };
     auto stage_v = [&](int j) {
-        stage_rows<D, ROWS, true>(a, vc, win, mine + j * STEP, k1, v_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, true>(a, vc, win, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
     };
 
     f32x16 o[RB][DB] = {};
@@ -454,6 +492,8 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     const int v_row = 4 * hi + ((lane & 15) >> 2);
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const int v_off = v_row * 2 * D + (lane & 1) * 8;
+    constexpr int KSPAN = D == 64 ? 8 : 16;   // chunks that a swizzle moves among
+    constexpr int VSPAN = D == 64 ? 8 : 16;
 
     // Scores of the tile at position base, softmax, and the weights packed for
     // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
@@ -462,18 +502,20 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
     auto scores = [&](uint32_t kt, int base, uint4 (&pw)[RB][2 * NB]) {
         f32x16 s[RB][NB] = {};
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const uint32_t row = kt + (32 * nb + q) * 2 * D;
-            const int sw = k_swizzle<D>(q);
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(row + (((2 * ks + hi) ^ sw) << 4));
+                // chunk (2 ks + hi) ^ swizzle: the swizzle's reach as a lane's
+                // address, the rest of ks and the tile's rows as offsets
+                lds_u8* at = reinterpret_cast<lds_u8*>(kt + q * 2 * D + (((2 * ks % KSPAN + hi) ^ k_swizzle<D>(q)) << 4));
+                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(at + 32 * nb * 2 * D + 2 * ks / KSPAN * KSPAN * 16);
                 const uint4 kf = make_uint4(kv.x, kv.y, kv.z, kv.w);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) s[rb][nb] = mfma32<FP16>(kf, qf[rb][ks], s[rb][nb]);
             }
-        }
+        read_ahead<NB * KS, 1, RB>();
         if (base + KT > least_seen) {
+            asm volatile("" ::: "memory");   // a branch: not selects in every step
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -523,14 +565,17 @@ __global__ __launch_bounds__(kThreads) void attend_tile_kernel(PagedAttnArgs a, 
         for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const uint32_t at = vt + 16 * k * 2 * D + v_off + (((4 * db + v_chunk) ^ v_swizzle<D>(v_row)) << 4);
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at));
-                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(at + 8 * 2 * D));
+                lds_u8* at = reinterpret_cast<lds_u8*>(
+                    vt + v_off + (((4 * db % VSPAN + v_chunk) ^ v_swizzle<D>(v_row)) << 4));
+                at += 16 * k * 2 * D + 4 * db / VSPAN * VSPAN * 16;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
                 const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, up);
                 const uint4 vf = make_uint4(x.x, x.y, y.x, y.y);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) o[rb][db] = mfma32<FP16>(vf, pw[rb][k], o[rb][db]);
             }
+        read_ahead<2 * NB * DB, 2, RB>();
     };
     // A value that is not finite among the tile's: all exponent bits set.
     auto look = [&](uint32_t vt) {
@@ -798,7 +843,7 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
                            stream, a, part);                                                                      \
     } while (0)
     if (sh.bm == 32) LR_ATTEND(1, 1, 4, 1);
-    else LR_ATTEND(1, 4, 1, 2);
+    else LR_ATTEND(1, 4, 1, (D == 256 ? 1 : 2));
 #undef LR_ATTEND
     return hipGetLastError();
 }
