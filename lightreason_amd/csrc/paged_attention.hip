@@ -7,6 +7,9 @@
 #include "paged.h"
 #include <stdlib.h>
 static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+#ifndef KSWZ
+#define KSWZ 7
+#endif
 #ifndef AHEADN
 #define AHEADN 4
 #endif
@@ -299,7 +302,7 @@ __device__ __forceinline__ uint32_t lds_address(void* p) {
 // the transposing read takes 2 (per 16 lanes) or 4 (per 32) chunks of four
 // rows at a time; they fall on different places of 128 and of 256 bytes.
 template <int D>
-__device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+__device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & (KSWZ); }
 template <int D>
 __device__ __forceinline__ int v_swizzle(int row) {
     return D == 64 ? (((row & 2) << 1) ^ ((row & 1) << 1)) : (((row & 3) << 2) ^ (row & 2));
@@ -326,7 +329,10 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
     constexpr int UNIT = 8;
     constexpr int PER = 512 / D;    // rows per load of the wave
     constexpr int CHUNKS = D / 8;
-    const int lane = threadIdx.x % kWave;
+    // The lane is made opaque so that no lane's offsets stay in registers
+    // across steps: each load works its own out with two instructions.
+    int lane = threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
     const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
     const uint32_t pitch = static_cast<uint32_t>(2 * c.row_stride);   // bytes
     const uint32_t lane_at = static_cast<uint32_t>(lrow) * pitch;
@@ -398,7 +404,7 @@ constexpr float kLowest = -1.7e38f;  // the running maximum before any position
 constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
 
 template <bool FP16, int D, int RB, int WQ, int WK, int NB>
-__global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
+__global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 : 2)) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
     static_assert(WQ * WK == kThreads / kWave, "four waves");
     constexpr int KT = 32 * NB;           // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(PagedAttnArgs 
     const int v_row = 4 * hi + ((lane & 15) >> 2);
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const int v_off = v_row * 2 * D + (lane & 1) * 8;
-    constexpr int KSPAN = D == 64 ? 8 : 16;   // chunks that a swizzle moves among
+    constexpr int KSPAN = D == 64 ? 8 : KSWZ + 1;   // chunks that a swizzle moves among
     constexpr int VSPAN = D == 64 ? 8 : 16;
 
     // Scores of the tile at position base, softmax, and the weights packed for
@@ -561,6 +567,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile_kernel(PagedAttnArgs 
         }
     };
     auto values = [&](uint32_t vt, const uint4 (&pw)[RB][2 * NB]) {
+        __builtin_amdgcn_sched_barrier(0);   // the order below is kept within its own region only
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
@@ -800,7 +807,8 @@ struct Shape {
 // sequence's rows fit into it, else tiles of 128 rows.
 Shape shape_of(int group, int max_new) {
     if (static_cast<int64_t>(max_new) * group <= 32) return {32, TARGET_FEW, LEAST_FEW};
-    return {128, TARGET_TILE, LEAST_TILE};
+    if (envi("BM", 128) == 128) return {128, TARGET_TILE, LEAST_TILE};
+    return {256, TARGET_TILE, LEAST_TILE};
 }
 
 struct Layout {
@@ -843,7 +851,8 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
                            stream, a, part);                                                                      \
     } while (0)
     if (sh.bm == 32) LR_ATTEND(1, 1, 4, 1);
-    else LR_ATTEND(1, 4, 1, (D == 256 ? 1 : 2));
+    else if (sh.bm == 128) LR_ATTEND(1, 4, 1, (D == 256 ? 1 : 2));
+    else LR_ATTEND(2, 4, 1, (D == 256 ? 1 : 2));
 #undef LR_ATTEND
     return hipGetLastError();
 }
