@@ -7,6 +7,10 @@
 #include "paged.h"
 #include <stdlib.h>
 static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+#ifndef NB8
+#define NB8 2
+#define SUB8 2
+#endif
 #ifndef KSWZ
 #define KSWZ 7
 #endif
@@ -326,7 +330,7 @@ struct CacheView {
 template <int D, int ROWS, bool VALUES>
 __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win, int pos,
                                            int end, int row0, uint32_t lds_at, bool& bad) {
-    constexpr int UNIT = 8;
+    constexpr int UNIT = ROWS < 8 ? ROWS : 8;
     constexpr int PER = 512 / D;    // rows per load of the wave
     constexpr int CHUNKS = D / 8;
     // The lane is made opaque so that no lane's offsets stay in registers
@@ -403,16 +407,20 @@ struct Partials {
 constexpr float kLowest = -1.7e38f;  // the running maximum before any position
 constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
 
-template <bool FP16, int D, int RB, int WQ, int WK, int NB>
-__global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 : 2)) void attend_tile_kernel(PagedAttnArgs a, Partials part, int target, int least) {
-    static_assert(WQ * WK == kThreads / kWave, "four waves");
-    constexpr int KT = 32 * NB;           // positions of a tile
+// WQ waves by 32 rows, or WK waves that share the rows and take positions of
+// their own; tiles of KT positions, worked through 32 NB at a time.
+template <bool FP16, int D, int WQ, int WK, int NB, int SUB>
+__global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
+    PagedAttnArgs a, Partials part, int target, int least) {
+    constexpr int RB = 1;
+    constexpr int THREADS = kWave * WQ * WK;
+    constexpr int KT = 32 * NB * SUB;     // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
     constexpr int BM = 32 * RB * WQ;
     constexpr int TILE = KT * 2 * D;      // bytes of a tile of keys or values
     constexpr int STAGES = WK == 1 ? 2 : 1;
     constexpr int KS = D / 16, DB = D / 32;
-    constexpr int ROWS = WK == 1 ? KT / 4 : KT;   // rows that a wave stages
+    constexpr int ROWS = WK == 1 ? KT / WQ : KT;   // rows that a wave stages
     constexpr int LOADS = ROWS * D / 512;         // of a key or value tile, per wave
     __shared__ __align__(1024) uint8_t lds[2 * STAGES * WK * TILE];
     const int lane = threadIdx.x % kWave;
@@ -520,7 +528,7 @@ __global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 :
                 for (int rb = 0; rb < RB; ++rb) s[rb][nb] = mfma32<FP16>(kf, qf[rb][ks], s[rb][nb]);
             }
         read_ahead<NB * KS, 1, RB>();
-        if (base + KT > least_seen) {
+        if (base + 32 * NB > least_seen) {
             asm volatile("" ::: "memory");   // a branch: not selects in every step
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
@@ -587,7 +595,7 @@ __global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 :
     // A value that is not finite among the tile's: all exponent bits set.
     auto look = [&](uint32_t vt) {
         constexpr uint32_t E = FP16 ? 0x7c00u : 0x7f80u;
-        for (int i = lane; i < TILE / 16; i += kWave) {
+        for (int i = WK == 1 ? threadIdx.x : lane; i < TILE / 16; i += WK == 1 ? THREADS : kWave) {
             const u32x4 v = *reinterpret_cast<lds_u32x4*>(vt + 16 * i);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -611,9 +619,14 @@ __global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 :
                 stage_k(j + 1);
                 stage_v(j + 1);
             }
-            scores(k_at(j & 1), base, pw);
             if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
-            values(v_at(j & 1), pw);
+#pragma unroll 1
+            for (int u = 0; u < SUB; ++u) {
+                const int part_at = u * 32 * NB;
+                if (base + part_at >= k1) break;
+                scores(k_at(j & 1) + part_at * 2 * D, base + part_at, pw);
+                values(v_at(j & 1) + part_at * 2 * D, pw);
+            }
         }
     } else {
         if (steps > 0) {
@@ -682,7 +695,7 @@ __global__ __launch_bounds__(kThreads, (D * RB > 256 || WK > 1 && D == 256 ? 1 :
             }
             __syncthreads();
             const int count = min(rows - r0, ROOM);
-            for (int i = threadIdx.x; i < count * (D / 4); i += kThreads) {
+            for (int i = threadIdx.x; i < count * (D / 4); i += THREADS) {
                 const int r = i / (D / 4), d = i % (D / 4) * 4;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -843,16 +856,16 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
     const unsigned grid = part.workgroups;
     const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
     const unsigned rows = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
-#define LR_ATTEND(RB, WQ, WK, NB)                                                                                 \
+#define LR_ATTEND(WQ, WK, NB, SUB)                                                                                \
     do {                                                                                                          \
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, RB, WQ, WK, NB>), dim3(grid), dim3(kThreads), 0, stream,  \
-                           a, part, sh.target, sh.least);                                                         \
-        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * RB * WQ>), dim3(grid, rows), dim3(kThreads), 0,     \
-                           stream, a, part);                                                                      \
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB>), dim3(grid), dim3(kWave * WQ * WK), 0,  \
+                           stream, a, part, sh.target, sh.least);                                                 \
+        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ>), dim3(grid, rows), dim3(kThreads), 0, stream,  \
+                           a, part);                                                                              \
     } while (0)
-    if (sh.bm == 32) LR_ATTEND(1, 1, 4, 1);
-    else if (sh.bm == 128) LR_ATTEND(1, 4, 1, (D == 256 ? 1 : 2));
-    else LR_ATTEND(2, 4, 1, (D == 256 ? 1 : 2));
+    if (sh.bm == 32) LR_ATTEND(1, 4, 1, 1);
+    else if (sh.bm == 128) LR_ATTEND(4, 1, (D == 256 ? 1 : 2), 1);
+    else LR_ATTEND(8, 1, (D == 256 ? 1 : NB8), (D == 256 ? 2 : SUB8));
 #undef LR_ATTEND
     return hipGetLastError();
 }
