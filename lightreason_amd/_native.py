@@ -7,8 +7,12 @@ not gfx950 every entry point raises; there is no fallback.
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import nullcontext
 from functools import lru_cache
+from operator import attrgetter, methodcaller
 from pathlib import Path
+
+import torch
 
 LIBRARY = Path(__file__).resolve().parent / "liblrmoe.so"
 
@@ -180,3 +184,48 @@ def timing_collect(stage: int) -> tuple[float, int]:
     ms, n = C.c_double(0.0), C.c_int(0)
     call("lrmoe_timing_collect", int(stage), C.byref(ms), C.byref(n))
     return ms.value, n.value
+
+
+# ---- cheap calls ----------------------------------------------------------------
+
+_HERE = nullcontext()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream(device: torch.device) -> int:
+    """The hipStream_t of torch's current stream on `device`."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one (a launch goes to the
+    current device, whatever device its tensors are on)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_traits = attrgetter("dtype", "shape", "device")
+_stride = methodcaller("stride")
+
+
+def signature(tensors, *rest):
+    """What the checks of a call depend on: types, shapes, devices and strides
+    of its tensors (None for one that is left out) and its other arguments;
+    None where there is no such thing.  Addresses are not part of it: the
+    library checks their alignment in every call."""
+    try:
+        given = [t for t in tensors if t is not None]
+        key = (tuple(map(_traits, given)), tuple(map(_stride, given)), tuple([t is None for t in tensors]), rest)
+        hash(key)
+        return key
+    except (AttributeError, TypeError, RuntimeError):
+        return None
+
+
+def remember(forms: dict, key, form) -> None:
+    """Keep the checked form of a signature (a bounded number of them)."""
+    if key is not None:
+        if len(forms) >= 1024:
+            forms.clear()
+        forms[key] = form

@@ -37,8 +37,8 @@ HEAD_DIMS = (64, 128, 256)
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_stream = _native.current_stream
+_on = _native.on_device
 
 
 def _require(t: torch.Tensor, name: str, dtypes, shape, device=None, contiguous: bool = True) -> torch.Tensor:
@@ -65,7 +65,7 @@ def _strided(t: torch.Tensor, name: str, multiple: int) -> None:
                          f"and {2 * multiple}-byte alignment, got strides {tuple(t.stride())}")
 
 
-def _strides(t: torch.Tensor, multiple: int):
+def _strides(t: torch.Tensor):
     """Strides of all but the last dimension (of dimensions of one entry: 0)."""
     return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])]
 
@@ -148,7 +148,7 @@ class PageTable:
             out = self.new_plan(tokens)
         elif out.tokens != tokens or out.starts.shape[0] != self.rows + 1 or out.starts.device != self.device:
             raise ValueError(f"out must be a plan of this pool for {tokens} positions")
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             _native.call("lrmoe_page_plan", self.rows, self.pages, self.page, self.max_pages, tokens,
                          new_tokens.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(),
                          self.free_pages.data_ptr(), self.state.data_ptr(), self.table.data_ptr(),
@@ -166,7 +166,7 @@ class PageTable:
             _require(accepted, "accepted", (torch.int32,), (self.rows,), self.device)
         if plan.starts.shape[0] != self.rows + 1 or plan.starts.device != self.device:
             raise ValueError("the plan is not of this pool")
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             _native.call("lrmoe_page_commit", self.rows, plan.starts.data_ptr(), plan.kv_lengths.data_ptr(),
                          plan.held.data_ptr(), plan.info.data_ptr(), _ptr(accepted), self.lengths.data_ptr(),
                          self.held.data_ptr(), self.state.data_ptr(), _stream(self.device))
@@ -175,7 +175,7 @@ class PageTable:
         """Return the pages of the rows with mask[r] ([rows] bool or uint8 on
         the device) to the free stack and empty those rows."""
         _require(mask, "mask", (torch.bool, torch.uint8), (self.rows,), self.device)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             _native.call("lrmoe_page_release", self.rows, self.pages, self.max_pages, mask.data_ptr(),
                          self.table.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(),
                          self.free_pages.data_ptr(), self.state.data_ptr(), _stream(self.device))
@@ -249,6 +249,34 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     model's q and gate come interleaved from one projection).  A token whose
     slot lies outside the pool (-1: padding) is left out, its q_out row too;
     tokens must not share a slot."""
+    tensors = (k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out)
+    key = _native.signature(tensors, eps)
+    form = _APPENDS.get(key)
+    if form is None:
+        form = _check_append(*tensors, eps)
+        _native.remember(_APPENDS, key, form)
+    template, dev, q_shape = form
+    if q_shape is not None and q_out is None:
+        q_out = torch.empty(q_shape, dtype=q.dtype, device=dev)
+    if template is None:   # no tokens
+        return q_out
+    a = _native.PagedAppendArgs.from_buffer_copy(template)
+    a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.slots, a.positions = slots.data_ptr(), _ptr(positions)
+    a.q, a.q_out, a.q_norm, a.k_norm = _ptr(q), _ptr(q_out), _ptr(q_norm), _ptr(k_norm)
+    a.cos, a.sin = _ptr(cos), _ptr(sin)
+    with _on(dev):
+        _native.call("lrmoe_paged_append", C.addressof(a), _stream(dev))
+    return q_out
+
+
+_APPENDS: dict = {}   # arguments of a form (types, shapes, strides) that was checked, without the addresses
+
+
+def _check_append(k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out, eps):
+    """Checks the arguments of paged_append; returns the filled-in structure
+    but for the addresses (None without tokens), the device, and q_out's
+    shape."""
     N, K, D, dtype, dev = _dims(k, "k")
     _strided(k, "k", 8)
     if _heads(v, "v", N, D, dtype, dev) != K:
@@ -258,10 +286,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     heads = 0
     if q is not None:
         heads = _heads(q, "q", N, D, dtype, dev)
-        if q_out is None:
-            q_out = torch.empty((N, heads, D), dtype=dtype, device=dev)
-        _require(q_out, "q_out", (dtype,), (N, heads, D), dev)
-        _strided(q_out, "q_out", 8)
+        if q_out is not None:
+            _require(q_out, "q_out", (dtype,), (N, heads, D), dev)
+            _strided(q_out, "q_out", 8)
     elif q_out is not None or q_norm is not None:
         raise ValueError("q_out and q_norm come with q")
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
@@ -281,27 +308,23 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             _require(positions, "positions", (torch.int32,), (N,), dev)
         elif rows != N:
             raise ValueError(f"without positions cos must have one row per token ({N}), got {rows}")
-        if rows == 0:
+        if rows == 0 and N > 0:
             raise ValueError("cos has no rows")
     elif positions is not None:
         raise ValueError("positions come with cos and sin")
+    q_shape = (N, heads, D) if q is not None else None
     if N == 0:
-        return q_out
+        return None, dev, q_shape
     a = _native.PagedAppendArgs(tokens=N, heads=heads, kv_heads=K, dim=D, rotary=rotary, pages=pages, page=page,
-                                fp16=int(dtype == torch.float16), q=_ptr(q), k=k.data_ptr(), v=v.data_ptr(),
-                                q_norm=_ptr(q_norm), k_norm=_ptr(k_norm), eps=float(eps),
-                                rope_fp32=int(cos is not None and cos.dtype == torch.float32), cos=_ptr(cos),
-                                sin=_ptr(sin), positions=_ptr(positions), rope_rows=rows, slots=slots.data_ptr(),
-                                q_out=_ptr(q_out), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr())
+                                fp16=int(dtype == torch.float16), eps=float(eps),
+                                rope_fp32=int(cos is not None and cos.dtype == torch.float32), rope_rows=rows)
     if q is not None:
-        a.q_token_stride, a.q_head_stride = _strides(q, 8)
-    a.k_token_stride, a.k_head_stride = _strides(k, 8)
-    a.v_token_stride, a.v_head_stride = _strides(v, 8)
-    a.k_page_stride, a.k_cache_head_stride, a.k_row_stride = _strides(k_cache, 8)
-    a.v_page_stride, a.v_cache_head_stride, a.v_row_stride = _strides(v_cache, 8)
-    with torch.cuda.device(dev):
-        _native.call("lrmoe_paged_append", C.addressof(a), _stream(dev))
-    return q_out
+        a.q_token_stride, a.q_head_stride = _strides(q)
+    a.k_token_stride, a.k_head_stride = _strides(k)
+    a.v_token_stride, a.v_head_stride = _strides(v)
+    a.k_page_stride, a.k_cache_head_stride, a.k_row_stride = _strides(k_cache)
+    a.v_page_stride, a.v_cache_head_stride, a.v_row_stride = _strides(v_cache)
+    return a, dev, q_shape
 
 
 # ---- attention ------------------------------------------------------------------
@@ -309,12 +332,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 _WORKSPACES: dict = {}
 
 
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
+def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Scratch of the current stream, grown as calls need it.  A call under
     capture gets scratch of its own from its graph's memory, so that graphs
     replayed on different streams share none."""
-    if nbytes == 0:
-        return None
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device, _stream(device))
@@ -345,43 +366,68 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
     chooses the kernel: give it where the counts are known to be small."""
+    tensors = (q, k_cache, v_cache, table, starts, kv_lengths, gate, out)
+    key = _native.signature(tensors, max_new, scale)
+    form = _ATTENTIONS.get(key)
+    if form is None:
+        form = _check_attention(*tensors, max_new, scale)
+        _native.remember(_ATTENTIONS, key, form)
+    template, dev, nbytes = form
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if template is None:   # no tokens or no sequences
+        return out
+    a = _native.PagedAttentionArgs.from_buffer_copy(template)
+    a.q, a.k_cache, a.v_cache, a.gate = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(gate)
+    a.table, a.starts, a.kv_lengths = table.data_ptr(), starts.data_ptr(), kv_lengths.data_ptr()
+    a.out = out.data_ptr()
+    with _on(dev):
+        ws = _workspace(dev, nbytes)
+        _native.call("lrmoe_paged_attention", C.addressof(a), ws.data_ptr(), ws.numel(), _stream(dev))
+    return out
+
+
+_ATTENTIONS: dict = {}   # as _APPENDS
+
+
+def _check_attention(q, k_cache, v_cache, table, starts, kv_lengths, gate, out, max_new, scale):
+    """Checks the arguments of paged_attention; returns the filled-in
+    structure but for the addresses (None when there is nothing to do), the
+    device, and the bytes of workspace."""
     N, H, D, dtype, dev = _dims(q, "q")
     _strided(q, "q", 8)
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or k_cache.shape[1] < 1 or H % k_cache.shape[1]:
         raise ValueError(f"k_cache must be [pages, kv_heads, page, dim] with kv_heads a divisor of {H}")
     K = k_cache.shape[1]
     pages, page = _caches(k_cache, v_cache, K, D, dtype, dev)
-    if table.dim() != 2:
-        raise ValueError(f"table must be [seqs, max_pages], got {tuple(table.shape)}")
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError("table must be [seqs, max_pages]")
     S, width = table.shape
     _require(table, "table", (torch.int32,), (S, width), dev)
     _require(starts, "starts", (torch.int32,), (S + 1,), dev)
     _require(kv_lengths, "kv_lengths", (torch.int32,), (S,), dev)
-    if gate is not None and _heads(gate, "gate", N, D, dtype, dev, 4) != H:
-        raise ValueError(f"gate must have the {H} heads of q")
-    if out is None:
-        out = torch.empty((N, H, D), dtype=dtype, device=dev)
-    elif _heads(out, "out", N, D, dtype, dev, 4) != H:
-        raise ValueError(f"out must have the {H} heads of q")
+    for name, t in (("gate", gate), ("out", out)):
+        if t is not None and _heads(t, name, N, D, dtype, dev, 4) != H:
+            raise ValueError(f"{name} must have the {H} heads of q")
     max_new = N if max_new is None else _int(max_new, "max_new", 0, 2**31 - 1)
     if N == 0 or S == 0:
-        return out
+        return None, dev, 0
     a = _native.PagedAttentionArgs(seqs=S, tokens=N, max_new=min(max_new, N), heads=H, kv_heads=K, dim=D, pages=pages,
                                    page=page, max_pages=width, fp16=int(dtype == torch.float16),
-                                   scale=D ** -0.5 if scale is None else float(scale), q=q.data_ptr(),
-                                   gate=_ptr(gate), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
-                                   table=table.data_ptr(), starts=starts.data_ptr(), kv_lengths=kv_lengths.data_ptr(),
-                                   out=out.data_ptr())
-    a.q_token_stride, a.q_head_stride = _strides(q, 8)
+                                   scale=D ** -0.5 if scale is None else float(scale))
+    a.q_token_stride, a.q_head_stride = _strides(q)
     if gate is not None:
-        a.gate_token_stride, a.gate_head_stride = _strides(gate, 4)
-    a.k_page_stride, a.k_head_stride, a.k_row_stride = _strides(k_cache, 8)
-    a.v_page_stride, a.v_head_stride, a.v_row_stride = _strides(v_cache, 8)
-    a.out_token_stride, a.out_head_stride = _strides(out, 4)
-    with torch.cuda.device(dev):
-        ws = _workspace(dev, int(_native.library().lrmoe_paged_attention_workspace_bytes(C.addressof(a))))
-        _native.call("lrmoe_paged_attention", C.addressof(a), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev))
-    return out
+        a.gate_token_stride, a.gate_head_stride = _strides(gate)
+    a.k_page_stride, a.k_head_stride, a.k_row_stride = _strides(k_cache)
+    a.v_page_stride, a.v_head_stride, a.v_row_stride = _strides(v_cache)
+    if out is not None:
+        a.out_token_stride, a.out_head_stride = _strides(out)
+    else:
+        a.out_token_stride, a.out_head_stride = H * D, D
+    nbytes = int(_native.library().lrmoe_paged_attention_workspace_bytes(C.addressof(a)))
+    if nbytes == 0:
+        raise ValueError("paged_attention: sizes past what one call takes")
+    return a, dev, nbytes
 
 
 def paged_layer(attn, hidden: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,

@@ -158,6 +158,36 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
     without rows gives (0, -1), a row of probabilities without mass -1.  A
     block of one row is plain sampling.  ``PageTable.commit(plan, accepted)``
     takes the result into the page pool."""
+    tensors = (tokens, target, starts, uniforms, samples, draft, accepted, next_tokens)
+    key = _native.signature(tensors)
+    form = _VERIFIES.get(key)
+    if form is None:
+        form = _check_verify(*tensors)
+        _native.remember(_VERIFIES, key, form)
+    blocks, rows, vocab, kind, dev, nbytes, target_stride, draft_stride = form
+    if accepted is None:
+        accepted = torch.empty(blocks, dtype=torch.int32, device=dev)
+    if next_tokens is None:
+        next_tokens = torch.empty(blocks, dtype=torch.int64, device=dev)
+    if blocks == 0:
+        return accepted, next_tokens
+    with _native.on_device(dev):
+        # From torch's allocator, which keeps it for this stream's next calls
+        # (and, under capture, in the graph's own memory).
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _native.call("lrmoe_verify_drafts", blocks, rows, vocab, kind, tokens.data_ptr(), target.data_ptr(),
+                     target_stride, None if draft is None else draft.data_ptr(), draft_stride, starts.data_ptr(),
+                     uniforms.data_ptr(), samples.data_ptr(), accepted.data_ptr(), next_tokens.data_ptr(),
+                     scratch.data_ptr(), nbytes, _native.current_stream(dev))
+    return accepted, next_tokens
+
+
+_VERIFIES: dict = {}   # forms (types, shapes, strides) that were checked
+
+
+def _check_verify(tokens, target, starts, uniforms, samples, draft, accepted, next_tokens):
+    """Checks the arguments of verify_drafts; returns what the call derives
+    from them."""
     if not isinstance(target, torch.Tensor) or target.dim() != 2 or target.dtype not in _PROBABILITIES:
         raise ValueError("target must be fp32, bf16 or fp16 [rows, vocab]")
     rows, vocab = target.shape
@@ -174,26 +204,14 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
     blocks = starts.shape[0] - 1
     if blocks > 65535:
         raise ValueError(f"at most 65535 blocks, got {blocks}")
-    _rows_of(starts, "starts", (blocks + 1,), torch.int32, dev)
-    _rows_of(tokens, "tokens", (rows,), torch.int64, dev)
-    _rows_of(uniforms, "uniforms", (rows,), torch.float32, dev)
-    _rows_of(samples, "samples", (blocks,), torch.float32, dev)
-    if accepted is None:
-        accepted = torch.empty(blocks, dtype=torch.int32, device=dev)
-    _rows_of(accepted, "accepted", (blocks,), torch.int32, dev)
-    if next_tokens is None:
-        next_tokens = torch.empty(blocks, dtype=torch.int64, device=dev)
-    _rows_of(next_tokens, "next_tokens", (blocks,), torch.int64, dev)
-    if blocks == 0:
-        return accepted, next_tokens
-    with torch.cuda.device(dev):
-        # From torch's allocator, which keeps it for this stream's next calls
-        # (and, under capture, in the graph's own memory).
-        scratch = torch.empty(int(_native.library().lrmoe_verify_workspace_bytes(blocks, vocab)), dtype=torch.uint8,
-                              device=dev)
-        _native.call("lrmoe_verify_drafts", blocks, rows, vocab, _PROBABILITIES[target.dtype], tokens.data_ptr(),
-                     target.data_ptr(), max(target.stride(0), vocab), None if draft is None else draft.data_ptr(),
-                     0 if draft is None else max(draft.stride(0), vocab), starts.data_ptr(), uniforms.data_ptr(),
-                     samples.data_ptr(), accepted.data_ptr(), next_tokens.data_ptr(), scratch.data_ptr(),
-                     scratch.numel(), torch.cuda.current_stream(dev).cuda_stream)
-    return accepted, next_tokens
+    for name, t, shape, dtype in (("starts", starts, (blocks + 1,), torch.int32),
+                                  ("tokens", tokens, (rows,), torch.int64),
+                                  ("uniforms", uniforms, (rows,), torch.float32),
+                                  ("samples", samples, (blocks,), torch.float32)):
+        _rows_of(t, name, shape, dtype, dev)
+    for name, t, dtype in (("accepted", accepted, torch.int32), ("next_tokens", next_tokens, torch.int64)):
+        if t is not None:
+            _rows_of(t, name, (blocks,), dtype, dev)
+    nbytes = 0 if blocks == 0 else int(_native.library().lrmoe_verify_workspace_bytes(blocks, vocab))
+    return (blocks, rows, vocab, _PROBABILITIES[target.dtype], dev, nbytes, max(target.stride(0), vocab),
+            0 if draft is None else max(draft.stride(0), vocab))
