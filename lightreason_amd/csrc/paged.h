@@ -110,7 +110,7 @@ struct VerifyArgs {
     const float *uniforms, *samples;
     int32_t* accepted;
     int64_t* next;
-    double* sums;  // [seqs][chunks][2]
+    double* sums;  // scratch: a block's outcome, then the chunks' sums
 };
 hipError_t launch_verify_drafts(const VerifyArgs& a, int type, hipStream_t stream);
 size_t verify_workspace_bytes(int seqs, int vocab);
