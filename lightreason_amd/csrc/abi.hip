@@ -801,15 +801,16 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     if (p->tokens == 0 || p->seqs == 0) return LRMOE_OK;
     if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->starts || !p->kv_lengths || !p->out)
         return LRMOE_E_ARG;
-    if (misaligned(p->q, 16) || misaligned(p->k_cache, 16) || misaligned(p->v_cache, 16) || misaligned(p->out, 8) ||
-        misaligned(p->gate, 8) || misaligned(workspace, 256))
+    if (misaligned(p->q, 16) || misaligned(p->k_cache, 16) || misaligned(p->v_cache, 16) || misaligned(p->out, 16) ||
+        misaligned(p->gate, 16) || misaligned(workspace, 256))
         return LRMOE_E_ARG;
     for (int64_t x : {p->q_token_stride, p->q_head_stride, p->k_page_stride, p->k_head_stride, p->k_row_stride,
-                      p->v_page_stride, p->v_head_stride, p->v_row_stride})
+                      p->v_page_stride, p->v_head_stride, p->v_row_stride, p->out_token_stride, p->out_head_stride,
+                      p->gate ? p->gate_token_stride : 0, p->gate ? p->gate_head_stride : 0})
         if (x % 8 != 0) return LRMOE_E_ARG;
-    if (p->out_token_stride % 4 != 0 || p->out_head_stride % 4 != 0 ||
-        (p->gate && (p->gate_token_stride % 4 != 0 || p->gate_head_stride % 4 != 0)))
-        return LRMOE_E_ARG;
+    // A lane's offset within a page is formed in 32 bits.
+    for (int64_t x : {p->k_row_stride, p->v_row_stride})
+        if (x < 0 || x >= (1 << 27)) return LRMOE_E_ARG;
     const size_t need =
         lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new);
     if (need > 0 && !workspace) return LRMOE_E_ARG;

@@ -111,9 +111,11 @@ __device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t 
 //
 // A sequence's rows (token-major, then the heads of one key/value head's
 // group) are cut into tiles of BM rows; a tile's positions into splits, so
-// that a few long sequences fill the chip: with W steps of positions in all,
-// a split holds more than W / target steps, so that there are at most target
-// splits and one per tile, and fewer than 2 target of tiles that are split.
+// that a few long sequences fill the chip.  W is the sum over all tiles of
+// their steps (of a sequence's tiles the mean of the first's and the last's)
+// and one; a split holds more than W / target steps.  A sequence's tiles all
+// get its longest tile's split count, so there are at most 2 target splits
+// and one per tile, and fewer than 4 target slots for tiles that are split.
 // Every wave works this out for itself from starts and kv_lengths (a lane per
 // sequence, cross-lane sums, no LDS and no barrier): nothing of it depends on
 // the host, no launch precedes the attention's, and what it costs is the one
@@ -184,7 +186,11 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
         load(base);
 #pragma unroll
         for (int k = 0; k < HELD; ++k)
-            if (s[k].n > 0) work += static_cast<float>(tiles_of(s[k].n, a.group, BM)) * steps_of(s[k].kv, STEP);
+            if (s[k].n > 0) {
+                const int shortest = tile_end(s[k], a.group, BM, 0);
+                work += static_cast<float>(tiles_of(s[k].n, a.group, BM)) *
+                        (0.5f * (steps_of(s[k].kv, STEP) + steps_of(shortest, STEP)) + 1.0f);
+            }
     }
     if (__any(bad)) return false;
     work = wave_butterfly_sum(work) * a.kv_heads;
@@ -230,24 +236,24 @@ struct Piece {
     Sequence seq;
 };
 
-// Four elements d .. d + 3 of a row's result: sums over l, times the gate,
+// Eight elements d .. d + 7 of a row's result: sums over l, times the gate,
 // rounded once.
 template <bool FP16>
-__device__ __forceinline__ void store_row4(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
-                                           float4 v, float l) {
+__device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
+                                           const float* v, float l) {
     const int i = row / a.group;
     const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float x[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
     if (a.gate != nullptr) {
-        const uint2 g = *reinterpret_cast<const uint2*>(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d);
-        x[0] *= sigmoid(elem16<FP16>(g.x & 0xffff));
-        x[1] *= sigmoid(elem16<FP16>(g.x >> 16));
-        x[2] *= sigmoid(elem16<FP16>(g.y & 0xffff));
-        x[3] *= sigmoid(elem16<FP16>(g.y >> 16));
+        float g[8];
+        unpack16<FP16>(ldg16(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d), g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= sigmoid(g[k]);
     }
-    *reinterpret_cast<uint2*>(a.out + t * a.out_token_stride + h * a.out_head_stride + d) =
-        make_uint2(pack16_2<FP16>(x[0], x[1]), pack16_2<FP16>(x[2], x[3]));
+    *reinterpret_cast<uint4*>(a.out + t * a.out_token_stride + h * a.out_head_stride + d) = pack16<FP16>(x);
 }
 
 // ---- the tile kernel --------------------------------------------------------------
@@ -375,19 +381,19 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
 
 // Orders the LDS reads of FRAGS operand fragments (READS instructions each)
 // and the products that take them: AHEAD fragments before the first product,
-// then one more after each fragment's USES products.  Left to itself the
+// then one more after each product.  Left to itself the
 // compiler reads each fragment right before its product, to save registers,
 // and every product waits for LDS.
-template <int FRAGS, int READS, int USES>
+template <int FRAGS, int READS>
 __device__ __forceinline__ void read_ahead() {
     constexpr int AHEAD = AHEADN, PRODUCT = 0x8, LDS_READ = 0x100;
     __builtin_amdgcn_sched_group_barrier(LDS_READ, AHEAD * READS, 0);
 #pragma unroll
     for (int i = 0; i < FRAGS - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(PRODUCT, USES, 0);
+        __builtin_amdgcn_sched_group_barrier(PRODUCT, 1, 0);
         __builtin_amdgcn_sched_group_barrier(LDS_READ, READS, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD * USES, 0);
+    __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD, 0);
 }
 
 // Highest value and sum over the two lanes (q, q + 32) that share a row.
@@ -412,16 +418,18 @@ constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are
 template <bool FP16, int D, int WQ, int WK, int NB, int SUB>
 __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
     PagedAttnArgs a, Partials part, int target, int least) {
-    constexpr int RB = 1;
     constexpr int THREADS = kWave * WQ * WK;
-    constexpr int KT = 32 * NB * SUB;     // positions of a tile
+    constexpr int KB = 32 * NB;           // positions worked through at a time
+    constexpr int KT = KB * SUB;          // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
-    constexpr int BM = 32 * RB * WQ;
+    constexpr int BM = 32 * WQ;
     constexpr int TILE = KT * 2 * D;      // bytes of a tile of keys or values
     constexpr int STAGES = WK == 1 ? 2 : 1;
     constexpr int KS = D / 16, DB = D / 32;
     constexpr int ROWS = WK == 1 ? KT / WQ : KT;   // rows that a wave stages
-    constexpr int LOADS = ROWS * D / 512;         // of a key or value tile, per wave
+    constexpr int LOADS = ROWS * D / 512;          // of a key or value tile, per wave
+    constexpr int SPAN = D == 64 ? 8 : KSWZ + 1;   // chunks that the keys' swizzle moves among
+    constexpr int VSPAN = D == 64 ? 8 : 16;        // and the values'
     __shared__ __align__(1024) uint8_t lds[2 * STAGES * WK * TILE];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -442,7 +450,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int k0 = sp.split * share * STEP;
     const int k1 = min(end, k0 + share * STEP);
     const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
-    const int wq = wave % WQ, wk = WK == 1 ? 0 : wave;
+    const int wq = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
+    const int my_row = wq * 32 + q;
 
     // The maximum is taken before the scaling, so a negative scale turns the
     // queries' signs instead, and scale 0 is queries of 0 (a hidden score of
@@ -450,21 +459,19 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
     const float scale = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
     // Queries: lane (q, hi) holds elements 16 ks + 8 hi .. + 7 of row q.
-    uint4 qf[RB][KS];
-    int seen[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int r = (wq * RB + rb) * 32 + q;
-        const int row = row_at + (r < rows ? r : 0);
+    uint4 qf[KS];
+    int seen;
+    {
+        const int row = row_at + (my_row < rows ? my_row : 0);
         const int i = row / a.group;
-        seen[rb] = r < rows ? seen_by(sp.seq, i) : 0;
+        seen = my_row < rows ? seen_by(sp.seq, i) : 0;
         const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
                               (kh * a.group + row - i * a.group) * a.q_head_stride;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             uint4 v = ldg16(src + 16 * ks + 8 * hi);
             v.x = (v.x ^ flip) & keep; v.y = (v.y ^ flip) & keep; v.z = (v.z ^ flip) & keep; v.w = (v.w ^ flip) & keep;
-            qf[rb][ks] = v;
+            qf[ks] = v;
         }
     }
 
@@ -487,7 +494,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         if (p < end && (min(p + ROWS, end) - 1) >> a.page_shift >= win.first + kWave) win = window_at(p);
     };
     const uint32_t lds0 = lds_address(lds);
-    auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage * TILE : wk * TILE); };
+    auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * TILE; };
     auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
     auto stage_k = [&](int j) {
         stage_rows<D, ROWS, false>(a, kc, win, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
@@ -496,85 +503,71 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         stage_rows<D, ROWS, true>(a, vc, win, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
     };
 
-    f32x16 o[RB][DB] = {};
-    float m[RB], l[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        m[rb] = kLowest;
-        l[rb] = 0.0f;
-    }
+    f32x16 o[DB] = {};
+    float m = kLowest, l = 0.0f;
     const int v_row = 4 * hi + ((lane & 15) >> 2);
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const int v_off = v_row * 2 * D + (lane & 1) * 8;
-    constexpr int KSPAN = D == 64 ? 8 : KSWZ + 1;   // chunks that a swizzle moves among
-    constexpr int VSPAN = D == 64 ? 8 : 16;
 
-    // Scores of the tile at position base, softmax, and the weights packed for
+    // Scores of KB positions from base, softmax, and the weights packed for
     // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
     // row and the weights are the second product's operand as they are: of a
     // step of 16 positions lane (q, hi) holds 4 hi + {0..3, 8..11}.
-    auto scores = [&](uint32_t kt, int base, uint4 (&pw)[RB][2 * NB]) {
-        f32x16 s[RB][NB] = {};
+    auto scores = [&](uint32_t kt, int base, uint4 (&pw)[2 * NB]) {
+        f32x16 s[NB] = {};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 // chunk (2 ks + hi) ^ swizzle: the swizzle's reach as a lane's
                 // address, the rest of ks and the tile's rows as offsets
-                lds_u8* at = reinterpret_cast<lds_u8*>(kt + q * 2 * D + (((2 * ks % KSPAN + hi) ^ k_swizzle<D>(q)) << 4));
-                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(at + 32 * nb * 2 * D + 2 * ks / KSPAN * KSPAN * 16);
-                const uint4 kf = make_uint4(kv.x, kv.y, kv.z, kv.w);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) s[rb][nb] = mfma32<FP16>(kf, qf[rb][ks], s[rb][nb]);
+                lds_u8* at = reinterpret_cast<lds_u8*>(kt + q * 2 * D + (((2 * ks % SPAN + hi) ^ k_swizzle<D>(q)) << 4));
+                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(at + 32 * nb * 2 * D + 2 * ks / SPAN * SPAN * 16);
+                s[nb] = mfma32<FP16>(make_uint4(kv.x, kv.y, kv.z, kv.w), qf[ks], s[nb]);
             }
-        read_ahead<NB * KS, 1, RB>();
-        if (base + 32 * NB > least_seen) {
+        read_ahead<NB * KS, 1>();
+        if (base + KB > least_seen) {
             asm volatile("" ::: "memory");   // a branch: not selects in every step
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int p = base + 32 * nb + 8 * (i >> 2) + 4 * hi + (i & 3);
-                        s[rb][nb][i] = p < seen[rb] ? s[rb][nb][i] : -__builtin_inff();
-                    }
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float top = s[rb][0][0];
-#pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[rb][nb][i]);
-            top = pair_max(top) * scale;
-            if (__any(top > m[rb] + kSlack)) {
-                const float mn = __builtin_fmaxf(m[rb], top);
-                const float fall = __builtin_amdgcn_exp2f(m[rb] - mn);
-                m[rb] = mn;
-                l[rb] *= fall;
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[rb][db][i] *= fall;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][nb][8 * k + j], scale, -m[rb]));
-                        sum += w[j];
-                    }
-                    pw[rb][2 * nb + k] = pack16<FP16>(w);
+                for (int i = 0; i < 16; ++i) {
+                    const int p = base + 32 * nb + 8 * (i >> 2) + 4 * hi + (i & 3);
+                    s[nb][i] = p < seen ? s[nb][i] : -__builtin_inff();
                 }
-            l[rb] += sum;
         }
+        float top = s[0][0];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[nb][i]);
+        top = pair_max(top) * scale;
+        if (__any(top > m + kSlack)) {
+            const float mn = __builtin_fmaxf(m, top);
+            const float fall = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= fall;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= fall;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * k + j], scale, -m));
+                    sum += w[j];
+                }
+                pw[2 * nb + k] = pack16<FP16>(w);
+            }
+        l += sum;
     };
-    auto values = [&](uint32_t vt, const uint4 (&pw)[RB][2 * NB]) {
+    auto values = [&](uint32_t vt, const uint4 (&pw)[2 * NB]) {
         __builtin_amdgcn_sched_barrier(0);   // the order below is kept within its own region only
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k)
@@ -586,11 +579,9 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
                 const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
                 const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, up);
-                const uint4 vf = make_uint4(x.x, x.y, y.x, y.y);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) o[rb][db] = mfma32<FP16>(vf, pw[rb][k], o[rb][db]);
+                o[db] = mfma32<FP16>(make_uint4(x.x, x.y, y.x, y.y), pw[k], o[db]);
             }
-        read_ahead<2 * NB * DB, 2, RB>();
+        read_ahead<2 * NB * DB, 2>();
     };
     // A value that is not finite among the tile's: all exponent bits set.
     auto look = [&](uint32_t vt) {
@@ -598,17 +589,16 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         for (int i = WK == 1 ? threadIdx.x : lane; i < TILE / 16; i += WK == 1 ? THREADS : kWave) {
             const u32x4 v = *reinterpret_cast<lds_u32x4*>(vt + 16 * i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                dirty |= (v[j] & E) == E || ((v[j] >> 16) & E) == E;
+            for (int j = 0; j < 4; ++j) dirty |= (v[j] & E) == E || ((v[j] >> 16) & E) == E;
         }
     };
 
-    uint4 pw[RB][2 * NB];
+    uint4 pw[2 * NB];
+    if (steps > 0) {
+        stage_k(0);
+        stage_v(0);
+    }
     if constexpr (WK == 1) {
-        if (steps > 0) {
-            stage_k(0);
-            stage_v(0);
-        }
         for (int j = 0; j < steps; ++j) {
             const int base = k0 + j * STEP;
             wait_counts<0, 0>();
@@ -621,18 +611,15 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
             }
             if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
 #pragma unroll 1
-            for (int u = 0; u < SUB; ++u) {
-                const int part_at = u * 32 * NB;
-                if (base + part_at >= k1) break;
-                scores(k_at(j & 1) + part_at * 2 * D, base + part_at, pw);
-                values(v_at(j & 1) + part_at * 2 * D, pw);
+            for (int u = 0; u < KT && base + u < k1; u += KB) {
+                scores(k_at(j & 1) + u * 2 * D, base + u, pw);
+                values(v_at(j & 1) + u * 2 * D, pw);
             }
         }
     } else {
-        if (steps > 0) {
-            stage_k(0);
-            stage_v(0);
-        }
+        // A wave's tiles are its own: no barrier, and its next keys are on
+        // their way during its values' product, the next values during its
+        // keys'.
         for (int j = 0; j < steps; ++j) {
             const int base = k0 + j * STEP + wk * KT;
             wait_counts<LOADS, 15>();
@@ -652,18 +639,19 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
             if (more) stage_v(j + 1);
         }
     }
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int x = __float_as_int(l[rb]);
+    {
+        const int x = __float_as_int(l);
         const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        l[rb] = __int_as_float(r[0]) + __int_as_float(r[1]);
+        l = __int_as_float(r[0]) + __int_as_float(r[1]);
     }
-    const int flags = __syncthreads_or((bad ? 1 : 0) | (dirty ? 2 : 0));
-    // (__syncthreads_or gives 0 or 1: the two flags one after the other)
+    // (__syncthreads_or gives 0 or 1: the two flags one after the other.)
+    const bool flags = __syncthreads_or(bad || dirty);
     const bool any_bad = flags && __syncthreads_or(bad);
     const bool any_dirty = flags && __syncthreads_or(dirty);
     if (threadIdx.x == 0)
         part.pieces[blockIdx.x] = {sp.split == 0 ? splits : 0, any_dirty && !any_bad, sp.b, sp.tile, sp.slot, sp.seq};
+    const int64_t slot = static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh;
+    if (any_bad) l = __builtin_nanf("");
 
     if constexpr (WK > 1) {
         // The waves' sums over their own positions, joined in LDS in the
@@ -673,84 +661,103 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         constexpr int PITCH = D + 4;
         constexpr int ROOM = (2 * WK * TILE - WK * 32 * 8) / (4 * WK * PITCH);   // rows that fit at once
         if (hi == 0) {
-            ml[(wk * 32 + q) * 2] = m[0];
-            ml[(wk * 32 + q) * 2 + 1] = l[0];
+            ml[(wk * 32 + q) * 2] = m;
+            ml[(wk * 32 + q) * 2 + 1] = l;
         }
         __syncthreads();
         float top = kLowest;
 #pragma unroll
         for (int w = 0; w < WK; ++w) top = __builtin_fmaxf(top, ml[(w * 32 + q) * 2]);
-        const float fall = __builtin_amdgcn_exp2f(m[0] - top);
+        const float fall = __builtin_amdgcn_exp2f(m - top);
         for (int r0 = 0; r0 < rows; r0 += ROOM) {
             if (r0 > 0) __syncthreads();
             if (q >= r0 && q < min(rows, r0 + ROOM)) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        float4 v = make_float4(o[0][db][4 * g] * fall, o[0][db][4 * g + 1] * fall,
-                                               o[0][db][4 * g + 2] * fall, o[0][db][4 * g + 3] * fall);
-                        *reinterpret_cast<float4*>(acc + (wk * ROOM + q - r0) * PITCH + 32 * db + 8 * g + 4 * hi) = v;
-                    }
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4*>(acc + (wk * ROOM + q - r0) * PITCH + 32 * db + 8 * g + 4 * hi) =
+                            make_float4(o[db][4 * g] * fall, o[db][4 * g + 1] * fall, o[db][4 * g + 2] * fall,
+                                        o[db][4 * g + 3] * fall);
             }
             __syncthreads();
             const int count = min(rows - r0, ROOM);
-            for (int i = threadIdx.x; i < count * (D / 4); i += THREADS) {
-                const int r = i / (D / 4), d = i % (D / 4) * 4;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int i = threadIdx.x; i < count * (D / 8); i += THREADS) {
+                const int r = i / (D / 8), d = i % (D / 8) * 8;
+                float v[8] = {};
 #pragma unroll
-                for (int w = 0; w < WK; ++w) {
-                    const float4 x = *reinterpret_cast<const float4*>(acc + (w * ROOM + r) * PITCH + d);
-                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-                }
+                for (int w = 0; w < WK; ++w)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] += acc[(w * ROOM + r) * PITCH + d + k];
                 float rm = kLowest, rl = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WK; ++w) rm = __builtin_fmaxf(rm, ml[(w * 32 + r0 + r) * 2]);
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                     rl += ml[(w * 32 + r0 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r0 + r) * 2] - rm);
-                if (any_bad) rl = __builtin_nanf("");
                 if (splits > 1) {
-                    const int64_t at = (static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh) * BM + r0 + r;
-                    *reinterpret_cast<float4*>(part.o + at * D + d) = v;
+                    const int64_t at = slot * BM + r0 + r;
+                    *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(part.o + at * D + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
                     if (d == 0) *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(rm, rl);
                 } else {
-                    store_row4<FP16>(a, sp.seq, kh, row_at + r0 + r, d, v, rl);
+                    store_row8<FP16>(a, sp.seq, kh, row_at + r0 + r, d, v, rl);
                 }
             }
         }
+    } else if (splits > 1) {
+        // Partial rows as the lanes hold them: 1 KB per store.
+        float4* to = reinterpret_cast<float4*>(part.o + (slot * BM + wq * 32) * D) + lane;
+        if (hi == 0) *reinterpret_cast<float2*>(part.ml + 2 * (slot * BM + my_row)) = make_float2(m, l);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                to[(4 * db + g) * kWave] =
+                    make_float4(o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
     } else {
+        // Rows through LDS (the wave's own 32 rows, DBC blocks of 32 elements
+        // at a time), so that 8 elements of a row leave per lane.
+        constexpr int DBC = DB < 4 ? DB : 4;
+        constexpr int CHUNKS = 8 * DBC;   // of four floats, per row
+        static_assert(32 * 32 * DBC * 4 * WQ <= 2 * STAGES * WK * TILE, "the rows fit");
+        float4* mine_at = reinterpret_cast<float4*>(lds) + wave * 32 * CHUNKS;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const int r = (wq * RB + rb) * 32 + q;
-            const float sum = any_bad ? __builtin_nanf("") : l[rb];
-            const int64_t at = (static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh) * BM + r;
-            if (splits > 1 && r < rows && hi == 0)
-                *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(m[rb], sum);
-            if (r < rows) {
+        for (int d0 = 0; d0 < DB; d0 += DBC) {
+            wave_lds_fence();
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
+            for (int db = 0; db < DBC; ++db)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int d = 32 * db + 8 * g + 4 * hi;
-                        const float4 v = make_float4(o[rb][db][4 * g], o[rb][db][4 * g + 1], o[rb][db][4 * g + 2],
-                                                     o[rb][db][4 * g + 3]);
-                        if (splits > 1) *reinterpret_cast<float4*>(part.o + at * D + d) = v;
-                        else store_row4<FP16>(a, sp.seq, kh, row_at + r, d, v, sum);
-                    }
+                for (int g = 0; g < 4; ++g) {
+                    const int c = 8 * db + 2 * g + hi;
+                    mine_at[q * CHUNKS + (c ^ (q % CHUNKS))] =
+                        make_float4(o[d0 + db][4 * g] * inv, o[d0 + db][4 * g + 1] * inv, o[d0 + db][4 * g + 2] * inv,
+                                    o[d0 + db][4 * g + 3] * inv);
+                }
+            wave_lds_fence();
+#pragma unroll 1
+            for (int i = lane; i < 32 * CHUNKS / 2; i += kWave) {
+                const int r = i / (CHUNKS / 2), c = i % (CHUNKS / 2) * 2;
+                if (wq * 32 + r >= rows) continue;
+                const float4 x = mine_at[r * CHUNKS + (c ^ (r % CHUNKS))];
+                const float4 y = mine_at[r * CHUNKS + ((c + 1) ^ (r % CHUNKS))];
+                const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                store_row8<FP16>(a, sp.seq, kh, row_at + wq * 32 + r, 32 * d0 + 4 * c, v, 1.0f);
             }
         }
     }
 }
 
-// Joins the splits of each tile, in their order (a row's splits over the four
-// waves, then the waves), and recomputes the rows of dirty tiles one by one.
-// Workgroup (piece, i) takes rows i, i + gridDim.y, ... of its piece's tile.
-template <bool FP16, int D, int BM>
+// Joins the splits of each tile, in their order, and recomputes the rows of
+// dirty tiles one by one.  NATIVE: partial rows as the tile kernel's lanes
+// hold them, thread (wave, lane) takes that lane's elements of blocks
+// blockIdx.y, ... of 32; else row by row, a row's splits over the four waves,
+// then the waves, rows blockIdx.y, ....
+template <bool FP16, int D, int BM, bool NATIVE>
 __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a, Partials part) {
     constexpr int WAVES = kThreads / kWave;
-    constexpr int E = D / 4;   // lanes that hold elements, four each
-    __shared__ float qs[WAVES][D];
+    __shared__ __align__(16) float qs[WAVES][D];
     __shared__ float ps[WAVES][kWave];
     __shared__ int64_t vs[WAVES][kWave];
     __shared__ float sums[WAVES];
@@ -774,42 +781,87 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
         }
         return;
     }
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * BM;
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        const int64_t at = (static_cast<int64_t>(pc.slot) * a.kv_heads + kh) * BM + r;
-        float m = kLowest;
-        for (int s = lane; s < pc.splits; s += kWave) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
+    const int64_t slot = static_cast<int64_t>(pc.slot) * a.kv_heads + kh;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * BM;   // rows from one split to the next
+    if constexpr (NATIVE) {
+        constexpr int GROUPS = BM / 32, DB = D / 32;
+        for (int w = wave; w < GROUPS; w += WAVES) {
+            if (32 * w >= rows) break;
+            const int hi = lane >> 5, r = 32 * w + (lane & 31);
+            const float* ml = part.ml + 2 * (slot * BM + r);
+            float m = kLowest, l = 0.0f;
+            for (int s = 0; s < pc.splits; ++s) m = __builtin_fmaxf(m, ml[2 * s * step]);
+            for (int s = 0; s < pc.splits; ++s)
+                l = __builtin_fmaf(ml[2 * s * step + 1], __builtin_amdgcn_exp2f(ml[2 * s * step] - m), l);
+            for (int db = blockIdx.y; db < DB; db += gridDim.y) {
+                float4 v[4] = {};
+                const float4* from = reinterpret_cast<const float4*>(part.o + (slot * BM + 32 * w) * D) +
+                                     4 * db * kWave + lane;
+#pragma unroll 2
+                for (int s = 0; s < pc.splits; ++s) {
+                    const float x = __builtin_amdgcn_exp2f(ml[2 * s * step] - m);
 #pragma unroll
-        for (int off = 1; off < kWave; off *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, off));
-        float l = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int s = wave; s < pc.splits; s += WAVES) {
-            const float2 x = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (lane < E) y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
-            const float w = __builtin_amdgcn_exp2f(x.x - m);
-            l = __builtin_fmaf(w, x.y, l);
-            v.x = __builtin_fmaf(w, y.x, v.x);
-            v.y = __builtin_fmaf(w, y.y, v.y);
-            v.z = __builtin_fmaf(w, y.z, v.z);
-            v.w = __builtin_fmaf(w, y.w, v.w);
-        }
-        if (lane < E) *reinterpret_cast<float4*>(&qs[wave][4 * lane]) = v;
-        if (lane == 0) sums[wave] = l;
-        __syncthreads();
-        if (wave == 0 && lane < E) {
-            l = 0.0f;
-            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 y = from[s * step * (D / 4) + g * kWave];
+                        v[g].x = __builtin_fmaf(x, y.x, v[g].x);
+                        v[g].y = __builtin_fmaf(x, y.y, v[g].y);
+                        v[g].z = __builtin_fmaf(x, y.z, v[g].z);
+                        v[g].w = __builtin_fmaf(x, y.w, v[g].w);
+                    }
+                }
+                // Lane (q, hi) holds elements 8 g + 4 hi .. + 3: pairs of
+                // groups are exchanged so that each lane stores 8 in a row
+                // (hi = 0 groups 0 and 2, hi = 1 groups 1 and 3).
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float4 y = *reinterpret_cast<const float4*>(&qs[w][4 * lane]);
-                l += sums[w];
-                v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                for (int g = 0; g < 4; g += 2) {
+                    const float4 give = hi ? v[g] : v[g + 1], keep = hi ? v[g + 1] : v[g];
+                    const float4 got = make_float4(__shfl_xor(give.x, 32), __shfl_xor(give.y, 32),
+                                                   __shfl_xor(give.z, 32), __shfl_xor(give.w, 32));
+                    const float4 lo = hi ? got : keep, up = hi ? keep : got;
+                    const float x[8] = {lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
+                    if (r < rows) store_row8<FP16>(a, pc.seq, kh, row_at + r, 32 * db + 8 * (g + hi), x, l);
+                }
             }
-            store_row4<FP16>(a, pc.seq, kh, row_at + r, 4 * lane, v, l);
         }
-        __syncthreads();
+    } else {
+        constexpr int E = D / 8;   // lanes that store, eight elements each
+        constexpr int F = D / 4;   // lanes that sum, four each
+        for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+            const int64_t at = slot * BM + r;
+            float m = kLowest;
+            for (int s = lane; s < pc.splits; s += kWave) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
+#pragma unroll
+            for (int off = 1; off < kWave; off *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, off));
+            float l = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int s = wave; s < pc.splits; s += WAVES) {
+                const float2 x = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (lane < F) y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
+                const float w = __builtin_amdgcn_exp2f(x.x - m);
+                l = __builtin_fmaf(w, x.y, l);
+                v.x = __builtin_fmaf(w, y.x, v.x);
+                v.y = __builtin_fmaf(w, y.y, v.y);
+                v.z = __builtin_fmaf(w, y.z, v.z);
+                v.w = __builtin_fmaf(w, y.w, v.w);
+            }
+            if (lane < F) *reinterpret_cast<float4*>(&qs[wave][4 * lane]) = v;
+            if (lane == 0) sums[wave] = l;
+            __syncthreads();
+            if (wave == 0 && lane < E) {
+                l = 0.0f;
+                float x[8] = {};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    l += sums[w];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] += qs[w][8 * lane + k];
+                }
+                store_row8<FP16>(a, pc.seq, kh, row_at + r, 8 * lane, x, l);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -832,8 +884,8 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     const int group = heads / kv_heads;
     const Shape sh = shape_of(group, max_new);
     const int64_t tiles = static_cast<int64_t>(tokens) * group / sh.bm + (seqs < tokens ? seqs : tokens);
-    const int64_t workgroups = (sh.target / kv_heads + 1 + tiles) * kv_heads;
-    const int64_t slots = 2 * sh.target + 16;   // (16: the work is summed in 24 bits)
+    const int64_t workgroups = (2 * sh.target / kv_heads + 1 + tiles) * kv_heads;
+    const int64_t slots = 4 * sh.target + 16;   // (16: the work is summed in 24 bits)
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -855,13 +907,14 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
     const Shape sh = shape_of(a.group, max_new);
     const unsigned grid = part.workgroups;
     const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
-    const unsigned rows = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
+    // Merge workgroups per piece: a row each, or a block of 32 elements each.
+    const unsigned few = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
 #define LR_ATTEND(WQ, WK, NB, SUB)                                                                                \
     do {                                                                                                          \
         hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB>), dim3(grid), dim3(kWave * WQ * WK), 0,  \
                            stream, a, part, sh.target, sh.least);                                                 \
-        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ>), dim3(grid, rows), dim3(kThreads), 0, stream,  \
-                           a, part);                                                                              \
+        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ, WK == 1>),                                      \
+                           dim3(grid, WK == 1 ? D / 32 : few), dim3(kThreads), 0, stream, a, part);               \
     } while (0)
     if (sh.bm == 32) LR_ATTEND(1, 4, 1, 1);
     else if (sh.bm == 128) LR_ATTEND(4, 1, (D == 256 ? 1 : 2), 1);

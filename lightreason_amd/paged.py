@@ -212,11 +212,11 @@ def _caches(k_cache, v_cache, kv_heads, dim, dtype, dev):
     return pages, page
 
 
-def _heads(t, name, tokens, dim, dtype, dev, multiple=8):
+def _heads(t, name, tokens, dim, dtype, dev):
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, dim]")
     _require(t, name, (dtype,), (tokens, t.shape[1], dim), dev, contiguous=False)
-    _strided(t, name, multiple)
+    _strided(t, name, 8)
     return t.shape[1]
 
 
@@ -407,7 +407,7 @@ def _check_attention(q, k_cache, v_cache, table, starts, kv_lengths, gate, out, 
     _require(starts, "starts", (torch.int32,), (S + 1,), dev)
     _require(kv_lengths, "kv_lengths", (torch.int32,), (S,), dev)
     for name, t in (("gate", gate), ("out", out)):
-        if t is not None and _heads(t, name, N, D, dtype, dev, 4) != H:
+        if t is not None and _heads(t, name, N, D, dtype, dev) != H:
             raise ValueError(f"{name} must have the {H} heads of q")
     max_new = N if max_new is None else _int(max_new, "max_new", 0, 2**31 - 1)
     if N == 0 or S == 0:

@@ -129,9 +129,9 @@ def test_abi_attention_refuses_before_any_launch():
                dict(heads=0), dict(kv_heads=0), dict(heads=15), dict(heads=2048), dict(dim=96), dict(pages=0),
                dict(page=4), dict(page=48), dict(page=2048), dict(max_pages=0), dict(max_pages=1 << 28), dict(q=0),
                dict(k_cache=0), dict(v_cache=0), dict(table=0), dict(starts=0), dict(kv_lengths=0), dict(out=0),
-               dict(q=264), dict(k_cache=8), dict(v_cache=24), dict(out=4), dict(gate=4), dict(q_token_stride=4),
-               dict(k_row_stride=260), dict(v_page_stride=4), dict(out_token_stride=2),
-               dict(gate=256, gate_head_stride=3)):
+               dict(q=264), dict(k_cache=8), dict(v_cache=24), dict(out=8), dict(gate=8), dict(q_token_stride=4),
+               dict(k_row_stride=260), dict(v_page_stride=4), dict(out_token_stride=4),
+               dict(gate=256, gate_head_stride=4)):
         assert call(_attention_args(**kw)) == -1, kw
     assert call(_attention_args(), ws=8) == -1
     need = lib.lrmoe_paged_attention_workspace_bytes(C.addressof(_attention_args()))
