@@ -792,7 +792,8 @@ static bool bad_attention(const lrmoe_paged_attention_args* p) {
 
 size_t lrmoe_paged_attention_workspace_bytes(const lrmoe_paged_attention_args* p) {
     if (!p || bad_attention(p)) return 0;
-    return lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new);
+    return lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new,
+                                             static_cast<int64_t>(p->max_pages) * p->page);
 }
 
 int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, size_t workspace_bytes,
@@ -811,9 +812,8 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     // A lane's offset within a page is formed in 32 bits.
     for (int64_t x : {p->k_row_stride, p->v_row_stride})
         if (x < 0 || x >= (1 << 27)) return LRMOE_E_ARG;
-    const size_t need =
-        lrmoe::paged_attn_workspace_bytes(p->tokens, p->seqs, p->heads, p->kv_heads, p->dim, p->max_new);
-    if (need > 0 && !workspace) return LRMOE_E_ARG;
+    const size_t need = lrmoe_paged_attention_workspace_bytes(p);
+    if (!workspace) return LRMOE_E_ARG;
     if (workspace_bytes < need) return LRMOE_E_WORKSPACE;
     if (int d = check_device()) return d;
     lrmoe::PagedAttnArgs a{};

@@ -99,7 +99,8 @@ struct PagedAttnArgs {
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, bool fp16, int dim, int max_new, void* workspace,
                                   hipStream_t stream);
-size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new);
+size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new,
+                                  int64_t capacity);
 
 struct VerifyArgs {
     int seqs, rows, vocab;

@@ -7,10 +7,6 @@
 #include "paged.h"
 #include <stdlib.h>
 static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#ifndef NB8
-#define NB8 2
-#define SUB8 2
-#endif
 #ifndef KSWZ
 #define KSWZ 7
 #endif
@@ -19,7 +15,7 @@ static int envi(const char* n, int d) { const char* v = getenv(n); return v ? at
 #endif
 #define TARGET_FEW envi("TF", 1024)
 #define LEAST_FEW envi("LF", 1)
-#define TARGET_TILE envi("TT", 512)
+#define TARGET_TILE envi("TT", 400)
 #define LEAST_TILE envi("LT", 16)
 
 namespace lrmoe {
@@ -130,6 +126,7 @@ __device__ __forceinline__ int seen_by(const Sequence& s, int i) { return max(s.
 struct Split {
     int b, tile, split, splits;
     int slot;       // of the tile's first partial rows, before the head
+    int ordinal;    // of the tile among all tiles
     int per_split;  // steps
     Sequence seq;
 };
@@ -160,10 +157,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // The sequence, tile and split of item `item` (wave-uniform), heavy tiles
-// first; false past the last one, and for starts that are not ascending
-// within [0, tokens] (such a step is empty).
+// first, and how many tiles there are; false past the last item, and for
+// starts that are not ascending within [0, tokens] (such a step is empty).
 template <int BM, int STEP>
-__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out) {
+__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out, int* all_tiles) {
     constexpr int HELD = 4;   // sequences per lane that stay in registers
     const int lane = threadIdx.x % kWave;
     const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
@@ -182,29 +179,33 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
         }
     };
     float work = 0.0f;
+    int tiles = 0;
     for (int base = 0; base < a.seqs; base += HELD * kWave) {
         load(base);
 #pragma unroll
         for (int k = 0; k < HELD; ++k)
             if (s[k].n > 0) {
+                tiles += tiles_of(s[k].n, a.group, BM);
                 const int shortest = tile_end(s[k], a.group, BM, 0);
                 work += static_cast<float>(tiles_of(s[k].n, a.group, BM)) *
                         (0.5f * (steps_of(s[k].kv, STEP) + steps_of(shortest, STEP)) + 1.0f);
             }
     }
+    *all_tiles = 0;
     if (__any(bad)) return false;
+    *all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
     work = wave_butterfly_sum(work) * a.kv_heads;
     const float each = work / target;
     const int c = __builtin_amdgcn_readfirstlane(max(each < 1.0e9f ? static_cast<int>(each) + 1 : 1 << 30, least));
-    int at = 0, slot = 0;
+    int at = 0, slot = 0, ordinal = 0;
     for (int base = 0; base < a.seqs; base += HELD * kWave) {
         if (a.seqs > HELD * kWave) load(base);
 #pragma unroll
         for (int k = 0; k < HELD; ++k) {
             if (base + k * kWave >= a.seqs) break;
             const int splits = (steps_of(s[k].kv, STEP) + c - 1) / c;
-            const int items = tiles_of(s[k].n, a.group, BM) * splits, slots = splits > 1 ? items : 0;
-            const int upto = wave_scan(items), upto_slots = wave_scan(slots);
+            const int count = tiles_of(s[k].n, a.group, BM), items = count * splits, slots = splits > 1 ? items : 0;
+            const int upto = wave_scan(items), upto_slots = wave_scan(slots), upto_tiles = wave_scan(count);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item < at + all) {
                 const int who = __builtin_ctzll(__ballot(item < at + upto));
@@ -218,20 +219,22 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
                 out->tile = tiles_of(out->seq.n, a.group, BM) - 1 - up;
                 out->split = local - up * out->splits;
                 out->slot = slot + __builtin_amdgcn_readlane(upto_slots - slots, who) + out->tile * out->splits;
+                out->ordinal = ordinal + __builtin_amdgcn_readlane(upto_tiles - count, who) + out->tile;
                 out->per_split = c;
                 return true;
             }
             at += all;
             slot += __builtin_amdgcn_readlane(upto_slots, 63);
+            ordinal += __builtin_amdgcn_readlane(upto_tiles, 63);
         }
     }
     return false;
 }
 
-// What the attention launch leaves for the merge, one per workgroup.
+// What the attention launch leaves for the merge, one per tile and head.
 struct Piece {
-    int splits;   // of the tile, at its first split; 0 elsewhere and past the last
-    int dirty;    // values that some of the tile's rows must not see
+    int splits;   // 0 past the last tile
+    int item;     // workgroup of its first split (its further splits: every kv_heads-th from there)
     int b, tile, slot;
     Sequence seq;
 };
@@ -406,8 +409,9 @@ __device__ __forceinline__ float pair_max(float v) {
 struct Partials {
     float* o;     // [slot][BM][D] sums of exp2(s - m) v
     float* ml;    // [slot][BM][2] m, sum of exp2(s - m)
-    Piece* pieces;  // [workgroups of the attention launch]
-    int workgroups;
+    Piece* pieces;  // [tiles]
+    int* dirty;     // [workgroups of the attention launch]: values that some of the tile's rows must not see
+    int tiles, workgroups;
 };
 
 constexpr float kLowest = -1.7e38f;  // the running maximum before any position
@@ -436,13 +440,14 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int hi = lane >> 5, q = lane & 31;
     const int item = blockIdx.x / a.kv_heads, kh = blockIdx.x % a.kv_heads;
     Split sp;
-    const bool live = find_split<BM, STEP>(a, item, target, least, &sp);
-    const int end = live ? tile_end(sp.seq, a.group, BM, sp.tile) : 0;
-    const int splits = live ? tile_splits<STEP>(sp.splits, end, sp.per_split) : 0;
-    if (!live || sp.split >= splits) {
-        if (threadIdx.x == 0) part.pieces[blockIdx.x].splits = 0;
-        return;
-    }
+    int all_tiles;
+    const bool live = find_split<BM, STEP>(a, item, target, least, &sp, &all_tiles);
+    if (threadIdx.x == 0 && item >= all_tiles && static_cast<int>(blockIdx.x) < part.tiles)
+        part.pieces[blockIdx.x].splits = 0;
+    if (!live) return;
+    const int end = tile_end(sp.seq, a.group, BM, sp.tile);
+    const int splits = tile_splits<STEP>(sp.splits, end, sp.per_split);
+    if (sp.split >= splits) return;
     const int row_at = sp.tile * BM;
     const int rows = min(BM, sp.seq.n * a.group - row_at);
     const int least_seen = seen_by(sp.seq, row_at / a.group);
@@ -648,8 +653,12 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const bool flags = __syncthreads_or(bad || dirty);
     const bool any_bad = flags && __syncthreads_or(bad);
     const bool any_dirty = flags && __syncthreads_or(dirty);
-    if (threadIdx.x == 0)
-        part.pieces[blockIdx.x] = {sp.split == 0 ? splits : 0, any_dirty && !any_bad, sp.b, sp.tile, sp.slot, sp.seq};
+    if (threadIdx.x == 0) {
+        part.dirty[blockIdx.x] = any_dirty && !any_bad;
+        if (sp.split == 0)
+            part.pieces[sp.ordinal * a.kv_heads + kh] = {splits, static_cast<int>(blockIdx.x), sp.b, sp.tile, sp.slot,
+                                                         sp.seq};
+    }
     const int64_t slot = static_cast<int64_t>(sp.slot + sp.split) * a.kv_heads + kh;
     if (any_bad) l = __builtin_nanf("");
 
@@ -764,11 +773,8 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const Piece pc = part.pieces[blockIdx.x];
     if (pc.splits == 0) return;
-    int dirty = pc.dirty;
-    for (int s = lane; s < pc.splits; s += kWave) {
-        const int at = static_cast<int>(blockIdx.x) + s * a.kv_heads;
-        if (at < part.workgroups) dirty |= part.pieces[at].dirty;
-    }
+    int dirty = 0;
+    for (int s = lane; s < pc.splits; s += kWave) dirty |= part.dirty[pc.item + s * a.kv_heads];
     const bool any_dirty = __any(dirty);
     if (pc.splits == 1 && !any_dirty) return;
     const int kh = blockIdx.x % a.kv_heads, row_at = pc.tile * BM;
@@ -866,26 +872,30 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
 }
 
 struct Shape {
-    int bm, target, least;
+    int bm, step, target, least;
 };
 // The kernel of a step: one 32-row tile of four position groups where every
 // sequence's rows fit into it, else tiles of 128 rows.
-Shape shape_of(int group, int max_new) {
-    if (static_cast<int64_t>(max_new) * group <= 32) return {32, TARGET_FEW, LEAST_FEW};
-    if (envi("BM", 128) == 128) return {128, TARGET_TILE, LEAST_TILE};
-    return {256, TARGET_TILE, LEAST_TILE};
+Shape shape_of(int group, int max_new, int dim) {
+    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, TARGET_FEW, LEAST_FEW};
+    return {128, dim == 256 ? 32 : 64, TARGET_TILE, LEAST_TILE};
 }
 
 struct Layout {
     Partials part;
     size_t bytes;
 };
-Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
+Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim, int max_new, int64_t capacity) {
     const int group = heads / kv_heads;
-    const Shape sh = shape_of(group, max_new);
+    const Shape sh = shape_of(group, max_new, dim);
     const int64_t tiles = static_cast<int64_t>(tokens) * group / sh.bm + (seqs < tokens ? seqs : tokens);
-    const int64_t workgroups = (2 * sh.target / kv_heads + 1 + tiles) * kv_heads;
-    const int64_t slots = 4 * sh.target + 16;   // (16: the work is summed in 24 bits)
+    // A tile has at most one split per `least` steps of what a row can hold;
+    // tiles of one sequence, where it has several, count up to twice.
+    const int64_t most = (capacity / sh.step + sh.least) / sh.least;
+    const int64_t share = (sh.bm == 32 ? 1 : 2) * (sh.target / kv_heads + 1);   // splits beyond one per tile, per head
+    const int64_t per_head = tiles * most < share + tiles ? tiles * most : share + tiles;
+    const int64_t workgroups = per_head * kv_heads;
+    const int64_t slots = 2 * share * kv_heads + 16;   // (16: the work is summed in 24 bits)
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -895,7 +905,9 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     };
     Layout l;
     l.part.workgroups = static_cast<int>(workgroups);
-    l.part.pieces = reinterpret_cast<Piece*>(take(workgroups * sizeof(Piece)));
+    l.part.tiles = static_cast<int>(tiles * kv_heads);
+    l.part.pieces = reinterpret_cast<Piece*>(take(l.part.tiles * sizeof(Piece)));
+    l.part.dirty = reinterpret_cast<int*>(take(workgroups * 4));
     l.part.ml = reinterpret_cast<float*>(take(slots * sh.bm * 8));
     l.part.o = reinterpret_cast<float*>(take(slots * sh.bm * static_cast<size_t>(dim) * 4));
     l.bytes = at;
@@ -904,7 +916,7 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
 
 template <bool FP16, int D>
 hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
-    const Shape sh = shape_of(a.group, max_new);
+    const Shape sh = shape_of(a.group, max_new, D);
     const unsigned grid = part.workgroups;
     const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
     // Merge workgroups per piece: a row each, or a block of 32 elements each.
@@ -914,24 +926,25 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
         hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB>), dim3(grid), dim3(kWave * WQ * WK), 0,  \
                            stream, a, part, sh.target, sh.least);                                                 \
         hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ, WK == 1>),                                      \
-                           dim3(grid, WK == 1 ? D / 32 : few), dim3(kThreads), 0, stream, a, part);               \
+                           dim3(part.tiles, WK == 1 ? D / 32 : few), dim3(kThreads), 0, stream, a, part);               \
     } while (0)
     if (sh.bm == 32) LR_ATTEND(1, 4, 1, 1);
-    else if (sh.bm == 128) LR_ATTEND(4, 1, (D == 256 ? 1 : 2), 1);
-    else LR_ATTEND(8, 1, (D == 256 ? 1 : NB8), (D == 256 ? 2 : SUB8));
+    else LR_ATTEND(4, 1, (D == 256 ? 1 : 2), 1);
 #undef LR_ATTEND
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new) {
-    return carve(nullptr, tokens, seqs, heads, kv_heads, dim, max_new).bytes;
+size_t paged_attn_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int dim, int max_new,
+                                  int64_t capacity) {
+    return carve(nullptr, tokens, seqs, heads, kv_heads, dim, max_new, capacity).bytes;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, bool fp16, int dim, int max_new, void* workspace,
                                   hipStream_t stream) {
-    const Partials part = carve(workspace, a.tokens, a.seqs, a.heads, a.kv_heads, dim, max_new).part;
+    const Partials part = carve(workspace, a.tokens, a.seqs, a.heads, a.kv_heads, dim, max_new,
+                                static_cast<int64_t>(a.max_pages) << a.page_shift).part;
     if (dim == 64) return fp16 ? launch<true, 64>(a, max_new, part, stream) : launch<false, 64>(a, max_new, part, stream);
     if (dim == 128)
         return fp16 ? launch<true, 128>(a, max_new, part, stream) : launch<false, 128>(a, max_new, part, stream);
