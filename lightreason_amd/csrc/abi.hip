@@ -809,9 +809,9 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
                       p->v_page_stride, p->v_head_stride, p->v_row_stride, p->out_token_stride, p->out_head_stride,
                       p->gate ? p->gate_token_stride : 0, p->gate ? p->gate_head_stride : 0})
         if (x % 8 != 0) return LRMOE_E_ARG;
-    // A lane's offset within a page is formed in 32 bits.
+    // Offsets within a page are formed in 32 bits.
     for (int64_t x : {p->k_row_stride, p->v_row_stride})
-        if (x < 0 || x >= (1 << 27)) return LRMOE_E_ARG;
+        if (x < 0 || x >= (1 << 20)) return LRMOE_E_ARG;
     const size_t need = lrmoe_paged_attention_workspace_bytes(p);
     if (!workspace) return LRMOE_E_ARG;
     if (workspace_bytes < need) return LRMOE_E_WORKSPACE;

@@ -37,7 +37,11 @@ __device__ __forceinline__ void unpack16(uint4 w, float* x) {
 }
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack16_2(float lo, float hi) {
-    if constexpr (FP16) return f_to_f16(lo) | (f_to_f16(hi) << 16);
+    if constexpr (FP16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, f16x2));
+    }
     return pack_bf2(lo, hi);
 }
 template <bool FP16>

@@ -302,6 +302,26 @@ __device__ __forceinline__ void load_lds16(uint32_t lds_at, const void* address)
                  : "s"(lds_at), "v"(address)
                  : "memory");
 }
+// 1, 2 or 4 of them for rows that follow each other in memory as in LDS: an
+// instruction's offset moves both addresses.
+__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[1]) {
+    load_lds16(lds_at, base, o[0]);
+}
+__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[2]) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                 "global_load_lds_dwordx4 %2, %3 offset:1024"
+                 :
+                 : "s"(lds_at), "v"(o[0]), "v"(o[1]), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[4]) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                 "global_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+                 "global_load_lds_dwordx4 %4, %5 offset:3072"
+                 :
+                 : "s"(lds_at), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "s"(base)
+                 : "memory");
+}
 
 __device__ const uint4 kZeros = {0u, 0u, 0u, 0u};  // what rows past a tile's end read
 
@@ -333,51 +353,72 @@ struct CacheView {
     int64_t row_stride;
 };
 
-// ROWS rows from position `pos` on, `row0` rows into their tile, for the
-// positions before `end` (zeros past it).  A page holds at least 8 rows, so
-// one table entry serves UNIT rows.
+// What a lane adds to a staged row's address: its row and chunk within a load
+// of the wave, the chunk moved by the swizzle of the first load's rows.
+template <int D, bool VALUES>
+struct LaneAt {
+    uint32_t chunk;   // 16 (chunk ^ swizzle(row of the load))
+    uint32_t row;     // row times the pitch
+    __device__ __forceinline__ LaneAt(int lane, uint32_t pitch) {
+        constexpr int CHUNKS = D / 8;
+        const int r = lane / CHUNKS;
+        chunk = 16 * ((lane % CHUNKS) ^ (VALUES ? v_swizzle<D>(r) : k_swizzle<D>(r)));
+        row = r * pitch;
+    }
+};
+
+// ROWS rows from position `pos` on, `row0` rows (a multiple of 8) into their
+// tile, for the positions before `end` (zeros past it).  A page holds at
+// least 8 rows, so one table entry serves that many, or all ROWS.
 template <int D, int ROWS, bool VALUES>
-__device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win, int pos,
-                                           int end, int row0, uint32_t lds_at, bool& bad) {
-    constexpr int UNIT = ROWS < 8 ? ROWS : 8;
-    constexpr int PER = 512 / D;    // rows per load of the wave
-    constexpr int CHUNKS = D / 8;
-    // The lane is made opaque so that no lane's offsets stay in registers
-    // across steps: each load works its own out with two instructions.
-    int lane = threadIdx.x % kWave;
-    asm volatile("" : "+v"(lane));
-    const int lrow = lane / CHUNKS, lchunk = lane % CHUNKS;
+__device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win,
+                                           const LaneAt<D, VALUES>& lane_at, int pos, int end, int row0,
+                                           uint32_t lds_at, bool& bad) {
+    constexpr int UNIT = 8;
+    constexpr int PER = 512 / D;      // rows per load of the wave
+    constexpr int N = UNIT / PER;     // loads per unit
     const uint32_t pitch = static_cast<uint32_t>(2 * c.row_stride);   // bytes
-    const uint32_t lane_at = static_cast<uint32_t>(lrow) * pitch;
-    auto chunk = [&](int row) {
-        return 16 * (lchunk ^ (VALUES ? v_swizzle<D>(row0 + row + lrow) : k_swizzle<D>(row0 + row + lrow)));
-    };
+    // The swizzle of a load's rows: its own bits are apart from those of the
+    // rows within a load, so it is one more exclusive or.
+    auto swizzle = [&](int row) { return 16u * (VALUES ? v_swizzle<D>(row) : k_swizzle<D>(row)); };
     auto page_of = [&](int p) {
         int entry = __builtin_amdgcn_readlane(win.entry, (p >> a.page_shift) - win.first);
         const bool in = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages);
         bad |= !in;
         entry = in ? entry : 0;
         return reinterpret_cast<const uint8_t*>(c.data + entry * c.page_stride) +
-               static_cast<uint64_t>(p & ((1 << a.page_shift) - 1)) * pitch;
+               static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
+    };
+    auto unit = [&](int u, const uint8_t* base) {
+        uint32_t o[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = (lane_at.chunk ^ swizzle(row0 + u + i * PER)) + lane_at.row;
+        if (pitch == 2 * D) {
+            load_lds16_n(lds_at + u * 2 * D, base, o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) load_lds16(lds_at + (u + i * PER) * 2 * D, base + i * PER * pitch, o[i]);
+        }
     };
     if (pos + ROWS <= end) {
+        if (ROWS <= 1 << a.page_shift) {
+            const uint8_t* base = page_of(pos);
 #pragma unroll
-        for (int u = 0; u < ROWS; u += UNIT) {
-            const uint8_t* base = page_of(pos + u);
-#pragma unroll
-            for (int i = 0; i < UNIT; i += PER)
-                load_lds16(lds_at + (u + i) * 2 * D, base + i * static_cast<uint64_t>(pitch), chunk(u + i) + lane_at);
+            for (int u = 0; u < ROWS; u += UNIT) unit(u, base + u * pitch);
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < ROWS; u += UNIT) unit(u, page_of(pos + u));
         }
     } else {
+        int lane = threadIdx.x % kWave;
+        asm volatile("" : "+v"(lane));   // nothing of this path stays in registers through the others
+        const int lrow = lane / (D / 8);
 #pragma unroll 1
-        for (int u = 0; u < ROWS; u += UNIT) {
-            const uint8_t* base = pos + u < end ? page_of(pos + u) : nullptr;
-#pragma unroll
-            for (int i = 0; i < UNIT; i += PER) {
-                const uint8_t* from = base + i * static_cast<uint64_t>(pitch) + lane_at + chunk(u + i);
-                load_lds16(lds_at + (u + i) * 2 * D,
-                           pos + u + i + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
-            }
+        for (int r = 0; r < ROWS; r += PER) {
+            const uint8_t* base = pos + r < end ? page_of(pos + r) : nullptr;
+            const uint8_t* from = base + (lane_at.chunk ^ swizzle(row0 + r)) + lane_at.row;
+            load_lds16(lds_at + r * 2 * D,
+                       pos + r + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
         }
     }
 }
@@ -491,6 +532,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         PageWindow w;
         w.first = p >> a.page_shift;
         w.entry = table[min(w.first + lane, last_page)];
+        asm volatile("" : "+v"(w.entry));   // waited for here, not (with every staged row) where it is used
         return w;
     };
     PageWindow win = window_at(min(mine, max(end - 1, 0)));
@@ -501,11 +543,13 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const uint32_t lds0 = lds_address(lds);
     auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * TILE; };
     auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
+    const LaneAt<D, false> k_lane(lane, static_cast<uint32_t>(2 * kc.row_stride));
+    const LaneAt<D, true> v_lane(lane, static_cast<uint32_t>(2 * vc.row_stride));
     auto stage_k = [&](int j) {
-        stage_rows<D, ROWS, false>(a, kc, win, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, false>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
     };
     auto stage_v = [&](int j) {
-        stage_rows<D, ROWS, true>(a, vc, win, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, true>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
     };
 
     f32x16 o[DB] = {};
