@@ -348,9 +348,9 @@ struct PageWindow {
     int first;   // first page of the window
 };
 struct CacheView {
-    const uint16_t* data;  // at the key/value head
-    int64_t page_stride;
-    int64_t row_stride;
+    const uint8_t* data;  // at the key/value head
+    int64_t page;         // bytes from one page to the next
+    uint32_t pitch;       // bytes from one row to the next
 };
 
 // What a lane adds to a staged row's address: its row and chunk within a load
@@ -369,15 +369,16 @@ struct LaneAt {
 
 // ROWS rows from position `pos` on, `row0` rows (a multiple of 8) into their
 // tile, for the positions before `end` (zeros past it).  A page holds at
-// least 8 rows, so one table entry serves that many, or all ROWS.
-template <int D, int ROWS, bool VALUES>
+// least 8 rows, so one table entry serves that many, or all ROWS.  DENSE: the
+// rows of a page follow each other.
+template <int D, int ROWS, bool VALUES, bool DENSE>
 __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win,
                                            const LaneAt<D, VALUES>& lane_at, int pos, int end, int row0,
                                            uint32_t lds_at, bool& bad) {
     constexpr int UNIT = 8;
     constexpr int PER = 512 / D;      // rows per load of the wave
     constexpr int N = UNIT / PER;     // loads per unit
-    const uint32_t pitch = static_cast<uint32_t>(2 * c.row_stride);   // bytes
+    const uint32_t pitch = DENSE ? 2 * D : c.pitch;
     // The swizzle of a load's rows: its own bits are apart from those of the
     // rows within a load, so it is one more exclusive or.
     auto swizzle = [&](int row) { return 16u * (VALUES ? v_swizzle<D>(row) : k_swizzle<D>(row)); };
@@ -386,14 +387,13 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
         const bool in = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages);
         bad |= !in;
         entry = in ? entry : 0;
-        return reinterpret_cast<const uint8_t*>(c.data + entry * c.page_stride) +
-               static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
+        return c.data + entry * c.page + static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
     };
     auto unit = [&](int u, const uint8_t* base) {
         uint32_t o[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = (lane_at.chunk ^ swizzle(row0 + u + i * PER)) + lane_at.row;
-        if (pitch == 2 * D) {
+        if constexpr (DENSE) {
             load_lds16_n(lds_at + u * 2 * D, base, o);
         } else {
 #pragma unroll
@@ -460,7 +460,7 @@ constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are
 
 // WQ waves by 32 rows, or WK waves that share the rows and take positions of
 // their own; tiles of KT positions, worked through 32 NB at a time.
-template <bool FP16, int D, int WQ, int WK, int NB, int SUB>
+template <bool FP16, int D, int WQ, int WK, int NB, int SUB, bool DENSE>
 __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
     PagedAttnArgs a, Partials part, int target, int least) {
     constexpr int THREADS = kWave * WQ * WK;
@@ -521,8 +521,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         }
     }
 
-    const CacheView kc = {a.k_cache + kh * a.k_head_stride, a.k_page_stride, a.k_row_stride};
-    const CacheView vc = {a.v_cache + kh * a.v_head_stride, a.v_page_stride, a.v_row_stride};
+    const CacheView kc = {reinterpret_cast<const uint8_t*>(a.k_cache + kh * a.k_head_stride), 2 * a.k_page_stride,
+                          static_cast<uint32_t>(2 * a.k_row_stride)};
+    const CacheView vc = {reinterpret_cast<const uint8_t*>(a.v_cache + kh * a.v_head_stride), 2 * a.v_page_stride,
+                          static_cast<uint32_t>(2 * a.v_row_stride)};
     const int32_t* table = a.table + static_cast<int64_t>(sp.b) * a.max_pages;
     const int last_page = max(end - 1, 0) >> a.page_shift;
     const int stage_row = WK == 1 ? wave * ROWS : 0;
@@ -543,13 +545,13 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const uint32_t lds0 = lds_address(lds);
     auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * TILE; };
     auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
-    const LaneAt<D, false> k_lane(lane, static_cast<uint32_t>(2 * kc.row_stride));
-    const LaneAt<D, true> v_lane(lane, static_cast<uint32_t>(2 * vc.row_stride));
+    const LaneAt<D, false> k_lane(lane, DENSE ? 2 * D : kc.pitch);
+    const LaneAt<D, true> v_lane(lane, DENSE ? 2 * D : vc.pitch);
     auto stage_k = [&](int j) {
-        stage_rows<D, ROWS, false>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, false, DENSE>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
     };
     auto stage_v = [&](int j) {
-        stage_rows<D, ROWS, true>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, true, DENSE>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
     };
 
     f32x16 o[DB] = {};
@@ -963,12 +965,17 @@ hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hip
     const Shape sh = shape_of(a.group, max_new, D);
     const unsigned grid = part.workgroups;
     const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
+    const bool dense = a.k_row_stride == D && a.v_row_stride == D;
     // Merge workgroups per piece: a row each, or a block of 32 elements each.
     const unsigned few = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
 #define LR_ATTEND(WQ, WK, NB, SUB)                                                                                \
     do {                                                                                                          \
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB>), dim3(grid), dim3(kWave * WQ * WK), 0,  \
-                           stream, a, part, sh.target, sh.least);                                                 \
+        if (dense)                                                                                                \
+            hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB, true>), dim3(grid),                  \
+                               dim3(kWave * WQ * WK), 0, stream, a, part, sh.target, sh.least);                   \
+        else                                                                                                      \
+            hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB, false>), dim3(grid),                 \
+                               dim3(kWave * WQ * WK), 0, stream, a, part, sh.target, sh.least);                   \
         hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ, WK == 1>),                                      \
                            dim3(part.tiles, WK == 1 ? D / 32 : few), dim3(kThreads), 0, stream, a, part);               \
     } while (0)
