@@ -498,6 +498,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
     const int wq = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
     const int my_row = wq * 32 + q;
+    const bool works = wq * 32 < rows;   // a wave without rows only stages
 
     // The maximum is taken before the scaling, so a negative scale turns the
     // queries' signs instead, and scale 0 is queries of 0 (a hidden score of
@@ -662,7 +663,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
             }
             if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
 #pragma unroll 1
-            for (int u = 0; u < KT && base + u < k1; u += KB) {
+            for (int u = 0; works && u < KT && base + u < k1; u += KB) {
                 scores(k_at(j & 1) + u * 2 * D, base + u, pw);
                 values(v_at(j & 1) + u * 2 * D, pw);
             }
@@ -760,6 +761,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 }
             }
         }
+    } else if (!works) {
     } else if (splits > 1) {
         // Partial rows as the lanes hold them: 1 KB per store.
         float4* to = reinterpret_cast<float4*>(part.o + (slot * BM + wq * 32) * D) + lane;
@@ -815,7 +817,6 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
     __shared__ __align__(16) float qs[WAVES][D];
     __shared__ float ps[WAVES][kWave];
     __shared__ int64_t vs[WAVES][kWave];
-    __shared__ float sums[WAVES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const Piece pc = part.pieces[blockIdx.x];
     if (pc.splits == 0) return;
@@ -841,24 +842,45 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
             if (32 * w >= rows) break;
             const int hi = lane >> 5, r = 32 * w + (lane & 31);
             const float* ml = part.ml + 2 * (slot * BM + r);
-            float m = kLowest, l = 0.0f;
-            for (int s = 0; s < pc.splits; ++s) m = __builtin_fmaxf(m, ml[2 * s * step]);
-            for (int s = 0; s < pc.splits; ++s)
-                l = __builtin_fmaf(ml[2 * s * step + 1], __builtin_amdgcn_exp2f(ml[2 * s * step] - m), l);
             for (int db = blockIdx.y; db < DB; db += gridDim.y) {
                 float4 v[4] = {};
+                float m = kLowest, l = 0.0f;
                 const float4* from = reinterpret_cast<const float4*>(part.o + (slot * BM + 32 * w) * D) +
                                      4 * db * kWave + lane;
-#pragma unroll 2
-                for (int s = 0; s < pc.splits; ++s) {
-                    const float x = __builtin_amdgcn_exp2f(ml[2 * s * step] - m);
+                // Four splits at a time, all requested before the first is used.
+                for (int s0 = 0; s0 < pc.splits; s0 += 4) {
+                    float2 x[4];
+                    float4 y[4][4] = {};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        x[k] = make_float2(kLowest, 0.0f);
+                        if (s0 + k < pc.splits) {
+                            x[k] = *reinterpret_cast<const float2*>(ml + 2 * (s0 + k) * step);
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) y[k][g] = from[(s0 + k) * step * (D / 4) + g * kWave];
+                        }
+                    }
+                    float top = m;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top = __builtin_fmaxf(top, x[k].x);
+                    const float fall = __builtin_amdgcn_exp2f(m - top);
+                    l *= fall;
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const float4 y = from[s * step * (D / 4) + g * kWave];
-                        v[g].x = __builtin_fmaf(x, y.x, v[g].x);
-                        v[g].y = __builtin_fmaf(x, y.y, v[g].y);
-                        v[g].z = __builtin_fmaf(x, y.z, v[g].z);
-                        v[g].w = __builtin_fmaf(x, y.w, v[g].w);
+                        v[g].x *= fall; v[g].y *= fall; v[g].z *= fall; v[g].w *= fall;
+                    }
+                    m = top;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float f = __builtin_amdgcn_exp2f(x[k].x - m);
+                        l = __builtin_fmaf(f, x[k].y, l);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            v[g].x = __builtin_fmaf(f, y[k][g].x, v[g].x);
+                            v[g].y = __builtin_fmaf(f, y[k][g].y, v[g].y);
+                            v[g].z = __builtin_fmaf(f, y[k][g].z, v[g].z);
+                            v[g].w = __builtin_fmaf(f, y[k][g].w, v[g].w);
+                        }
                     }
                 }
                 // Lane (q, hi) holds elements 8 g + 4 hi .. + 3: pairs of
@@ -878,37 +900,58 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
     } else {
         constexpr int E = D / 8;   // lanes that store, eight elements each
         constexpr int F = D / 4;   // lanes that sum, four each
+        __shared__ float2 sums[WAVES];
         for (int r = blockIdx.y; r < rows; r += gridDim.y) {
             const int64_t at = slot * BM + r;
-            float m = kLowest;
-            for (int s = lane; s < pc.splits; s += kWave) m = __builtin_fmaxf(m, part.ml[2 * (at + s * step)]);
-#pragma unroll
-            for (int off = 1; off < kWave; off *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, off));
-            float l = 0.0f;
+            float m = kLowest, l = 0.0f;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (int s = wave; s < pc.splits; s += WAVES) {
-                const float2 x = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (lane < F) y = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
-                const float w = __builtin_amdgcn_exp2f(x.x - m);
-                l = __builtin_fmaf(w, x.y, l);
-                v.x = __builtin_fmaf(w, y.x, v.x);
-                v.y = __builtin_fmaf(w, y.y, v.y);
-                v.z = __builtin_fmaf(w, y.z, v.z);
-                v.w = __builtin_fmaf(w, y.w, v.w);
+            // Four splits of the wave at a time, their sums and rows all
+            // requested before the first is used.
+            for (int s0 = wave; s0 < pc.splits; s0 += 4 * WAVES) {
+                float2 x[4];
+                float4 y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int s = s0 + k * WAVES;
+                    x[k] = make_float2(kLowest, 0.0f);
+                    y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (s < pc.splits) {
+                        x[k] = *reinterpret_cast<const float2*>(part.ml + 2 * (at + s * step));
+                        if (lane < F) y[k] = *reinterpret_cast<const float4*>(part.o + (at + s * step) * D + 4 * lane);
+                    }
+                }
+                float top = m;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top = __builtin_fmaxf(top, x[k].x);
+                const float fall = __builtin_amdgcn_exp2f(m - top);
+                l *= fall;
+                v.x *= fall; v.y *= fall; v.z *= fall; v.w *= fall;
+                m = top;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float w = __builtin_amdgcn_exp2f(x[k].x - m);
+                    l = __builtin_fmaf(w, x[k].y, l);
+                    v.x = __builtin_fmaf(w, y[k].x, v.x);
+                    v.y = __builtin_fmaf(w, y[k].y, v.y);
+                    v.z = __builtin_fmaf(w, y[k].z, v.z);
+                    v.w = __builtin_fmaf(w, y[k].w, v.w);
+                }
             }
             if (lane < F) *reinterpret_cast<float4*>(&qs[wave][4 * lane]) = v;
-            if (lane == 0) sums[wave] = l;
+            if (lane == 0) sums[wave] = make_float2(m, l);
             __syncthreads();
             if (wave == 0 && lane < E) {
+                float top = kLowest;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, sums[w].x);
                 l = 0.0f;
                 float x[8] = {};
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
-                    l += sums[w];
+                    const float f = __builtin_amdgcn_exp2f(sums[w].x - top);
+                    l = __builtin_fmaf(f, sums[w].y, l);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] += qs[w][8 * lane + k];
+                    for (int k = 0; k < 8; ++k) x[k] = __builtin_fmaf(f, qs[w][8 * lane + k], x[k]);
                 }
                 store_row8<FP16>(a, pc.seq, kh, row_at + r, 8 * lane, x, l);
             }
