@@ -586,7 +586,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * are left as they were.  A table entry outside [0, pages) in use makes its
  * sequence's rows NaN; kv_lengths beyond max_pages pages are cut there.
  * max_new (at least every n) only chooses the kernel.  Strides as
- * lrmoe_paged_append's.  Workspace of lrmoe_paged_attention_workspace_bytes(args) bytes,
+ * lrmoe_paged_append's; row strides below 2^20, pages spread over at most
+ * 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args) bytes,
  * 256-byte aligned, not cleared, used by one stream at a time. */
 typedef struct lrmoe_paged_attention_args {
     int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */

@@ -812,6 +812,9 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     // Offsets within a page are formed in 32 bits.
     for (int64_t x : {p->k_row_stride, p->v_row_stride})
         if (x < 0 || x >= (1 << 20)) return LRMOE_E_ARG;
+    // And a page's place in 32 bits of 16 bytes.
+    for (int64_t x : {p->k_page_stride, p->v_page_stride})
+        if (x < 0 || x / 8 > (INT64_C(1) << 32) / p->pages) return LRMOE_E_ARG;
     const size_t need = lrmoe_paged_attention_workspace_bytes(p);
     if (!workspace) return LRMOE_E_ARG;
     if (workspace_bytes < need) return LRMOE_E_WORKSPACE;

@@ -16,7 +16,7 @@ static int envi(const char* n, int d) { const char* v = getenv(n); return v ? at
 #define TARGET_FEW envi("TF", 1024)
 #define LEAST_FEW envi("LF", 1)
 #define TARGET_TILE envi("TT", 400)
-#define LEAST_TILE envi("LT", 16)
+#define LEAST_TILE envi("LT", 8)
 
 namespace lrmoe {
 namespace {
@@ -341,15 +341,14 @@ __device__ __forceinline__ int v_swizzle(int row) {
     return D == 64 ? (((row & 2) << 1) ^ ((row & 1) << 1)) : (((row & 3) << 2) ^ (row & 2));
 }
 
-// Rows [row0, row0 + ROWS) of a tile that starts at position `base`, from
-// pages of one cache into LDS.
+// 64 pages of a sequence: where each one's rows are in the two caches, lane i
+// page first + i (in units of 16 bytes, so 32 bits reach 64 GiB).
 struct PageWindow {
-    int entry;   // lane i: table entry of page first + i
-    int first;   // first page of the window
+    uint32_t k, v;
+    int first;
 };
 struct CacheView {
     const uint8_t* data;  // at the key/value head
-    int64_t page;         // bytes from one page to the next
     uint32_t pitch;       // bytes from one row to the next
 };
 
@@ -374,7 +373,7 @@ struct LaneAt {
 template <int D, int ROWS, bool VALUES, bool DENSE>
 __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win,
                                            const LaneAt<D, VALUES>& lane_at, int pos, int end, int row0,
-                                           uint32_t lds_at, bool& bad) {
+                                           uint32_t lds_at) {
     constexpr int UNIT = 8;
     constexpr int PER = 512 / D;      // rows per load of the wave
     constexpr int N = UNIT / PER;     // loads per unit
@@ -383,11 +382,9 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
     // rows within a load, so it is one more exclusive or.
     auto swizzle = [&](int row) { return 16u * (VALUES ? v_swizzle<D>(row) : k_swizzle<D>(row)); };
     auto page_of = [&](int p) {
-        int entry = __builtin_amdgcn_readlane(win.entry, (p >> a.page_shift) - win.first);
-        const bool in = static_cast<uint32_t>(entry) < static_cast<uint32_t>(a.pages);
-        bad |= !in;
-        entry = in ? entry : 0;
-        return c.data + entry * c.page + static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
+        const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(
+            static_cast<int>(VALUES ? win.v : win.k), (p >> a.page_shift) - win.first));
+        return c.data + (static_cast<uint64_t>(at) << 4) + static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
     };
     auto unit = [&](int u, const uint8_t* base) {
         uint32_t o[N];
@@ -522,9 +519,9 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         }
     }
 
-    const CacheView kc = {reinterpret_cast<const uint8_t*>(a.k_cache + kh * a.k_head_stride), 2 * a.k_page_stride,
+    const CacheView kc = {reinterpret_cast<const uint8_t*>(a.k_cache + kh * a.k_head_stride),
                           static_cast<uint32_t>(2 * a.k_row_stride)};
-    const CacheView vc = {reinterpret_cast<const uint8_t*>(a.v_cache + kh * a.v_head_stride), 2 * a.v_page_stride,
+    const CacheView vc = {reinterpret_cast<const uint8_t*>(a.v_cache + kh * a.v_head_stride),
                           static_cast<uint32_t>(2 * a.v_row_stride)};
     const int32_t* table = a.table + static_cast<int64_t>(sp.b) * a.max_pages;
     const int last_page = max(end - 1, 0) >> a.page_shift;
@@ -534,8 +531,13 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     auto window_at = [&](int p) {
         PageWindow w;
         w.first = p >> a.page_shift;
-        w.entry = table[min(w.first + lane, last_page)];
-        asm volatile("" : "+v"(w.entry));   // waited for here, not (with every staged row) where it is used
+        uint32_t entry = static_cast<uint32_t>(table[min(w.first + lane, last_page)]);
+        bad |= end > 0 && entry >= static_cast<uint32_t>(a.pages);   // (of pages that the tile's rows see)
+        entry = entry < static_cast<uint32_t>(a.pages) ? entry : 0;
+        w.k = entry * static_cast<uint32_t>(a.k_page_stride >> 3);
+        w.v = entry * static_cast<uint32_t>(a.v_page_stride >> 3);
+        // waited for here, not (with every staged row) where it is used
+        asm volatile("" : "+v"(w.k), "+v"(w.v));
         return w;
     };
     PageWindow win = window_at(min(mine, max(end - 1, 0)));
@@ -549,10 +551,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const LaneAt<D, false> k_lane(lane, DENSE ? 2 * D : kc.pitch);
     const LaneAt<D, true> v_lane(lane, DENSE ? 2 * D : vc.pitch);
     auto stage_k = [&](int j) {
-        stage_rows<D, ROWS, false, DENSE>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, false, DENSE>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D);
     };
     auto stage_v = [&](int j) {
-        stage_rows<D, ROWS, true, DENSE>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D, bad);
+        stage_rows<D, ROWS, true, DENSE>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D);
     };
 
     f32x16 o[DB] = {};
