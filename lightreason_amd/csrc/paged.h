@@ -55,6 +55,17 @@ __device__ __forceinline__ float elem16(uint16_t bits) {
     return bf2f(bits);
 }
 
+// Inclusive sum over the lanes (DPP row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 struct PagePlanArgs {
     int rows, pages, page_shift, max_pages, tokens;
     const int32_t *new_tokens, *lengths, *held, *free_pages, *state;

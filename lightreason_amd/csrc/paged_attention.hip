@@ -145,17 +145,6 @@ __device__ __forceinline__ int tile_splits(int splits, int end, int per_split) {
     return min(splits, (steps_of(end, STEP) + per_split - 1) / per_split);
 }
 
-// Inclusive sum over the lanes (DPP row shifts, then row broadcasts).
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
 // The sequence, tile and split of item `item` (wave-uniform), heavy tiles
 // first, and how many tiles there are; false past the last item, and for
 // starts that are not ascending within [0, tokens] (such a step is empty).
