@@ -7,9 +7,6 @@
 #include "paged.h"
 #include <stdlib.h>
 static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#ifndef KSWZ
-#define KSWZ 7
-#endif
 #ifndef AHEADN
 #define AHEADN 4
 #endif
@@ -291,25 +288,27 @@ __device__ __forceinline__ void load_lds16(uint32_t lds_at, const void* address)
                  : "s"(lds_at), "v"(address)
                  : "memory");
 }
-// 1, 2 or 4 of them for rows that follow each other in memory as in LDS: an
-// instruction's offset moves both addresses.
-__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[1]) {
-    load_lds16(lds_at, base, o[0]);
-}
-__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[2]) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                 "global_load_lds_dwordx4 %2, %3 offset:1024"
-                 :
-                 : "s"(lds_at), "v"(o[0]), "v"(o[1]), "s"(base)
-                 : "memory");
-}
-__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, const uint32_t (&o)[4]) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
-                 "global_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-                 "global_load_lds_dwordx4 %4, %5 offset:3072"
-                 :
-                 : "s"(lds_at), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "s"(base)
-                 : "memory");
+// N of them for rows that follow each other in memory: an instruction's offset
+// moves both addresses by 1024, the rest of the step in LDS goes through m0.
+template <int N, int PAD>
+__device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, uint32_t offset) {
+    static_assert(N == 1 || N == 2 || N == 4, "rows of a unit");
+    if constexpr (N == 1)
+        load_lds16(lds_at, base, offset);
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                     :
+                     : "s"(lds_at), "v"(offset), "s"(base), "n"(PAD)
+                     : "memory", "scc");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:2048\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
+                     :
+                     : "s"(lds_at), "v"(offset), "s"(base), "n"(PAD)
+                     : "memory", "scc");
 }
 
 __device__ const uint4 kZeros = {0u, 0u, 0u, 0u};  // what rows past a tile's end read
@@ -319,16 +318,27 @@ __device__ __forceinline__ uint32_t lds_address(void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)p));
 }
 
-// Swizzles of a tile row's 16-byte chunks in LDS.  Keys: 16 consecutive rows
-// read at one chunk fall on 16 different chunk places of 256 bytes.  Values:
-// the transposing read takes 2 (per 16 lanes) or 4 (per 32) chunks of four
-// rows at a time; they fall on different places of 128 and of 256 bytes.
-template <int D>
-__device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & (KSWZ); }
-template <int D>
-__device__ __forceinline__ int v_swizzle(int row) {
-    return D == 64 ? (((row & 2) << 1) ^ ((row & 1) << 1)) : (((row & 3) << 2) ^ (row & 2));
-}
+// Where a tile's rows are in LDS.  A load of the wave writes 1024 bytes in
+// lane order, PER rows; the loads are PAD bytes apart, and a row's 16-byte
+// chunks are moved by an exclusive or that depends on the row's place in its
+// load only, so a lane's source offset is the same for every load.  Keys: the
+// 16 rows that a read of 64 lanes takes per cycle at one chunk fall on 16
+// different chunk places of 256 bytes; values: so do 4 chunks of 4 rows, which
+// the transposing read takes.  Few bits are moved, so that the products' reads
+// differ by constant offsets: one address for all keys at width 256 (two
+// below), two for all values (four at width 128).
+template <int D, bool VALUES>
+struct Place {
+    static constexpr int PER = 512 / D;   // rows per load
+    static constexpr int PAD = VALUES ? (D == 256 ? 64 : 0) : (D == 256 ? 32 : 64);
+    static constexpr int LOAD = 1024 + PAD;
+    static constexpr int MOVED = VALUES ? (D == 256 ? 8 : D == 128 ? 12 : 4) : (D == 256 ? 1 : 3);   // chunk bits
+    __device__ static __forceinline__ int swizzle(int row) {   // row within its load
+        if constexpr (VALUES) return D == 256 ? 8 * row : D == 128 ? 4 * row : 4 * ((row >> 1) & 1);
+        return D == 64 ? (row >> 1) & 3 : row;
+    }
+    static constexpr int bytes(int rows) { return rows / PER * LOAD; }
+};
 
 // 64 pages of a sequence: where each one's rows are in the two caches, lane i
 // page first + i (in units of 16 bytes, so 32 bits reach 64 GiB).
@@ -341,49 +351,34 @@ struct CacheView {
     uint32_t pitch;       // bytes from one row to the next
 };
 
-// What a lane adds to a staged row's address: its row and chunk within a load
-// of the wave, the chunk moved by the swizzle of the first load's rows.
+// What a lane adds to a load's address: its row and its chunk.
 template <int D, bool VALUES>
-struct LaneAt {
-    uint32_t chunk;   // 16 (chunk ^ swizzle(row of the load))
-    uint32_t row;     // row times the pitch
-    __device__ __forceinline__ LaneAt(int lane, uint32_t pitch) {
-        constexpr int CHUNKS = D / 8;
-        const int r = lane / CHUNKS;
-        chunk = 16 * ((lane % CHUNKS) ^ (VALUES ? v_swizzle<D>(r) : k_swizzle<D>(r)));
-        row = r * pitch;
-    }
-};
+__device__ __forceinline__ uint32_t lane_offset(int lane, uint32_t pitch) {
+    constexpr int CHUNKS = D / 8;
+    const int r = lane / CHUNKS;
+    return 16 * ((lane % CHUNKS) ^ Place<D, VALUES>::swizzle(r)) + r * pitch;
+}
 
-// ROWS rows from position `pos` on, `row0` rows (a multiple of 8) into their
-// tile, for the positions before `end` (zeros past it).  A page holds at
-// least 8 rows, so one table entry serves that many, or all ROWS.  DENSE: the
-// rows of a page follow each other.
+// ROWS rows from position `pos` on to `lds_at`, for the positions before `end`
+// (zeros past it).  A page holds at least 8 rows, so one table entry serves
+// that many, or all ROWS.  DENSE: the rows of a page follow each other.
 template <int D, int ROWS, bool VALUES, bool DENSE>
 __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheView& c, const PageWindow& win,
-                                           const LaneAt<D, VALUES>& lane_at, int pos, int end, int row0,
-                                           uint32_t lds_at) {
-    constexpr int UNIT = 8;
-    constexpr int PER = 512 / D;      // rows per load of the wave
-    constexpr int N = UNIT / PER;     // loads per unit
-    const uint32_t pitch = DENSE ? 2 * D : c.pitch;
-    // The swizzle of a load's rows: its own bits are apart from those of the
-    // rows within a load, so it is one more exclusive or.
-    auto swizzle = [&](int row) { return 16u * (VALUES ? v_swizzle<D>(row) : k_swizzle<D>(row)); };
+                                           uint32_t offset, int pos, int end, uint32_t lds_at) {
+    typedef Place<D, VALUES> P;
+    constexpr int UNIT = 8, N = UNIT / P::PER;
+    const uint32_t pitch = DENSE ? 2 * D : c.pitch;   // bytes
     auto page_of = [&](int p) {
         const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(
             static_cast<int>(VALUES ? win.v : win.k), (p >> a.page_shift) - win.first));
         return c.data + (static_cast<uint64_t>(at) << 4) + static_cast<uint32_t>(p & ((1 << a.page_shift) - 1)) * pitch;
     };
     auto unit = [&](int u, const uint8_t* base) {
-        uint32_t o[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = (lane_at.chunk ^ swizzle(row0 + u + i * PER)) + lane_at.row;
         if constexpr (DENSE) {
-            load_lds16_n(lds_at + u * 2 * D, base, o);
+            load_lds16_n<N, P::PAD>(lds_at + P::bytes(u), base, offset);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) load_lds16(lds_at + (u + i * PER) * 2 * D, base + i * PER * pitch, o[i]);
+            for (int i = 0; i < N; ++i) load_lds16(lds_at + P::bytes(u) + i * P::LOAD, base + i * P::PER * pitch, offset);
         }
     };
     if (pos + ROWS <= end) {
@@ -400,11 +395,10 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
         asm volatile("" : "+v"(lane));   // nothing of this path stays in registers through the others
         const int lrow = lane / (D / 8);
 #pragma unroll 1
-        for (int r = 0; r < ROWS; r += PER) {
+        for (int r = 0; r < ROWS; r += P::PER) {
             const uint8_t* base = pos + r < end ? page_of(pos + r) : nullptr;
-            const uint8_t* from = base + (lane_at.chunk ^ swizzle(row0 + r)) + lane_at.row;
-            load_lds16(lds_at + r * 2 * D,
-                       pos + r + lrow < end ? static_cast<const void*>(from) : static_cast<const void*>(&kZeros));
+            load_lds16(lds_at + P::bytes(r), pos + r + lrow < end ? static_cast<const void*>(base + offset)
+                                                                  : static_cast<const void*>(&kZeros));
         }
     }
 }
@@ -454,14 +448,15 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     constexpr int KT = KB * SUB;          // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
     constexpr int BM = 32 * WQ;
-    constexpr int TILE = KT * 2 * D;      // bytes of a tile of keys or values
+    typedef Place<D, false> KP;
+    typedef Place<D, true> VP;
+    constexpr int KTILE = KP::bytes(KT), VTILE = VP::bytes(KT);   // bytes of a tile of keys, of values
     constexpr int STAGES = WK == 1 ? 2 : 1;
     constexpr int KS = D / 16, DB = D / 32;
     constexpr int ROWS = WK == 1 ? KT / WQ : KT;   // rows that a wave stages
     constexpr int LOADS = ROWS * D / 512;          // of a key or value tile, per wave
-    constexpr int SPAN = D == 64 ? 8 : KSWZ + 1;   // chunks that the keys' swizzle moves among
-    constexpr int VSPAN = D == 64 ? 8 : 16;        // and the values'
-    __shared__ __align__(1024) uint8_t lds[2 * STAGES * WK * TILE];
+    constexpr int LDS = STAGES * WK * (KTILE + VTILE);
+    __shared__ __align__(1024) uint8_t lds[LDS];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int hi = lane >> 5, q = lane & 31;
@@ -535,22 +530,29 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         if (p < end && (min(p + ROWS, end) - 1) >> a.page_shift >= win.first + kWave) win = window_at(p);
     };
     const uint32_t lds0 = lds_address(lds);
-    auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * TILE; };
-    auto v_at = [&](int stage) { return lds0 + (STAGES * WK + (WK == 1 ? stage : wk)) * TILE; };
-    const LaneAt<D, false> k_lane(lane, DENSE ? 2 * D : kc.pitch);
-    const LaneAt<D, true> v_lane(lane, DENSE ? 2 * D : vc.pitch);
+    auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * KTILE; };
+    auto v_at = [&](int stage) { return lds0 + STAGES * WK * KTILE + (WK == 1 ? stage : wk) * VTILE; };
+    const uint32_t k_offset = lane_offset<D, false>(lane, DENSE ? 2 * D : kc.pitch);
+    const uint32_t v_offset = lane_offset<D, true>(lane, DENSE ? 2 * D : vc.pitch);
     auto stage_k = [&](int j) {
-        stage_rows<D, ROWS, false, DENSE>(a, kc, win, k_lane, mine + j * STEP, k1, stage_row, k_at(j & 1) + stage_row * 2 * D);
+        stage_rows<D, ROWS, false, DENSE>(a, kc, win, k_offset, mine + j * STEP, k1,
+                                          k_at(j & 1) + KP::bytes(stage_row));
     };
     auto stage_v = [&](int j) {
-        stage_rows<D, ROWS, true, DENSE>(a, vc, win, v_lane, mine + j * STEP, k1, stage_row, v_at(j & 1) + stage_row * 2 * D);
+        stage_rows<D, ROWS, true, DENSE>(a, vc, win, v_offset, mine + j * STEP, k1,
+                                         v_at(j & 1) + VP::bytes(stage_row));
     };
 
     f32x16 o[DB] = {};
     float m = kLowest, l = 0.0f;
+    // A lane's places in the products' reads: keys row q (chunk 2 ks + hi),
+    // values row 4 hi + i / 4 of 8 and chunk 4 db + 2 (lane / 16 % 2) + i % 4 / 2
+    // for lane i of 16, 8 bytes each.
     const int v_row = 4 * hi + ((lane & 15) >> 2);
-    const int v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const int v_off = v_row * 2 * D + (lane & 1) * 8;
+    const int k_off = q / KP::PER * KP::LOAD + q % KP::PER * 2 * D, k_move = KP::swizzle(q % KP::PER);
+    const int v_off = v_row / VP::PER * VP::LOAD + v_row % VP::PER * 2 * D +
+                      16 * (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    const int v_move = VP::swizzle(v_row % VP::PER);
 
     // Scores of KB positions from base, softmax, and the weights packed for
     // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
@@ -562,10 +564,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                // chunk (2 ks + hi) ^ swizzle: the swizzle's reach as a lane's
-                // address, the rest of ks and the tile's rows as offsets
-                lds_u8* at = reinterpret_cast<lds_u8*>(kt + q * 2 * D + (((2 * ks % SPAN + hi) ^ k_swizzle<D>(q)) << 4));
-                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(at + 32 * nb * 2 * D + 2 * ks / SPAN * SPAN * 16);
+                lds_u8* at = reinterpret_cast<lds_u8*>(kt + k_off + ((((2 * ks & KP::MOVED) + hi) ^ k_move) << 4));
+                const u32x4 kv = *reinterpret_cast<lds_u32x4*>(at + nb * KP::bytes(32) + ((2 * ks & ~KP::MOVED) << 4));
                 s[nb] = mfma32<FP16>(make_uint4(kv.x, kv.y, kv.z, kv.w), qf[ks], s[nb]);
             }
         read_ahead<NB * KS, 1>();
@@ -616,11 +616,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                lds_u8* at = reinterpret_cast<lds_u8*>(
-                    vt + v_off + (((4 * db % VSPAN + v_chunk) ^ v_swizzle<D>(v_row)) << 4));
-                at += 16 * k * 2 * D + 4 * db / VSPAN * VSPAN * 16;
+                lds_u8* at = reinterpret_cast<lds_u8*>(vt + v_off + (((4 * db & VP::MOVED) ^ v_move) << 4));
+                at += k * VP::bytes(16) + ((4 * db & ~VP::MOVED) << 4);
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 2 * D));
+                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + VP::bytes(8)));
                 const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, up);
                 o[db] = mfma32<FP16>(make_uint4(x.x, x.y, y.x, y.y), pw[k], o[db]);
             }
@@ -629,8 +628,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     // A value that is not finite among the tile's: all exponent bits set.
     auto look = [&](uint32_t vt) {
         constexpr uint32_t E = FP16 ? 0x7c00u : 0x7f80u;
-        for (int i = WK == 1 ? threadIdx.x : lane; i < TILE / 16; i += WK == 1 ? THREADS : kWave) {
-            const u32x4 v = *reinterpret_cast<lds_u32x4*>(vt + 16 * i);
+        for (int i = WK == 1 ? threadIdx.x : lane; i < KT * D / 8; i += WK == 1 ? THREADS : kWave) {
+            const u32x4 v = *reinterpret_cast<lds_u32x4*>(vt + i / kWave * VP::LOAD + i % kWave * 16);
 #pragma unroll
             for (int j = 0; j < 4; ++j) dirty |= (v[j] & E) == E || ((v[j] >> 16) & E) == E;
         }
@@ -655,8 +654,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
             if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
 #pragma unroll 1
             for (int u = 0; works && u < KT && base + u < k1; u += KB) {
-                scores(k_at(j & 1) + u * 2 * D, base + u, pw);
-                values(v_at(j & 1) + u * 2 * D, pw);
+                scores(k_at(j & 1) + KP::bytes(u), base + u, pw);
+                values(v_at(j & 1) + VP::bytes(u), pw);
             }
         }
     } else {
@@ -706,7 +705,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         float* ml = reinterpret_cast<float*>(lds);           // [WK][32][2]
         float* acc = ml + WK * 32 * 2;                       // [WK][rows of the tile][D + 4]
         constexpr int PITCH = D + 4;
-        constexpr int ROOM = (2 * WK * TILE - WK * 32 * 8) / (4 * WK * PITCH);   // rows that fit at once
+        constexpr int ROOM = (LDS - WK * 32 * 8) / (4 * WK * PITCH);   // rows that fit at once
         if (hi == 0) {
             ml[(wk * 32 + q) * 2] = m;
             ml[(wk * 32 + q) * 2 + 1] = l;
@@ -768,7 +767,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         // at a time), so that 8 elements of a row leave per lane.
         constexpr int DBC = DB < 4 ? DB : 4;
         constexpr int CHUNKS = 8 * DBC;   // of four floats, per row
-        static_assert(32 * 32 * DBC * 4 * WQ <= 2 * STAGES * WK * TILE, "the rows fit");
+        static_assert(32 * 32 * DBC * 4 * WQ <= LDS, "the rows fit");
         float4* mine_at = reinterpret_cast<float4*>(lds) + wave * 32 * CHUNKS;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
