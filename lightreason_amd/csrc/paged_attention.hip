@@ -181,6 +181,21 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
     if (__any(bad)) return false;
     *all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
     work = wave_butterfly_sum(work) * a.kv_heads;
+    // Up to 64 sequences of many tiles are taken longest first, so that none of
+    // the long ones starts last (nine prompts of 1-900 tokens over up to 5000
+    // cached: S1 us against S0 in their own order).
+    int who_is = lane;   // the sequence of this lane's s[0]
+    if (BM > 32 && a.seqs > 1 && a.seqs <= kWave) {
+        int rank = 0;
+        for (int j = 0; j < a.seqs; ++j) {
+            const int other = __builtin_amdgcn_readlane(s[0].kv, j);
+            rank += other > s[0].kv || (other == s[0].kv && j < lane);
+        }
+        if (lane >= a.seqs) rank = lane;
+        auto to_rank = [&](int v) { return __builtin_amdgcn_ds_permute(rank << 2, v); };
+        s[0] = {to_rank(s[0].first), to_rank(s[0].n), to_rank(s[0].kv)};
+        who_is = to_rank(lane);
+    }
     const float each = work / target;
     const int c = __builtin_amdgcn_readfirstlane(max(each < 1.0e9f ? static_cast<int>(each) + 1 : 1 << 30, least));
     int at = 0, slot = 0, ordinal = 0;
@@ -196,7 +211,7 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
             if (item < at + all) {
                 const int who = __builtin_ctzll(__ballot(item < at + upto));
                 const int local = item - at - __builtin_amdgcn_readlane(upto - items, who);
-                out->b = base + k * kWave + who;
+                out->b = base + k * kWave + (k == 0 ? __builtin_amdgcn_readlane(who_is, who) : who);
                 out->splits = __builtin_amdgcn_readlane(splits, who);
                 out->seq.first = __builtin_amdgcn_readlane(s[k].first, who);
                 out->seq.n = __builtin_amdgcn_readlane(s[k].n, who);
