@@ -501,23 +501,6 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     // -inf must not meet a factor of 0).
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
     const float scale = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale);
-    // Queries: lane (q, hi) holds elements 16 ks + 8 hi .. + 7 of row q.
-    uint4 qf[KS];
-    int seen;
-    {
-        const int row = row_at + (my_row < rows ? my_row : 0);
-        const int i = row / a.group;
-        seen = my_row < rows ? seen_by(sp.seq, i) : 0;
-        const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
-                              (kh * a.group + row - i * a.group) * a.q_head_stride;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            uint4 v = ldg16(src + 16 * ks + 8 * hi);
-            v.x = (v.x ^ flip) & keep; v.y = (v.y ^ flip) & keep; v.z = (v.z ^ flip) & keep; v.w = (v.w ^ flip) & keep;
-            qf[ks] = v;
-        }
-    }
-
     const CacheView kc = {reinterpret_cast<const uint8_t*>(a.k_cache + kh * a.k_head_stride),
                           static_cast<uint32_t>(2 * a.k_row_stride)};
     const CacheView vc = {reinterpret_cast<const uint8_t*>(a.v_cache + kh * a.v_head_stride),
@@ -527,10 +510,12 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int stage_row = WK == 1 ? wave * ROWS : 0;
     const int mine = k0 + wk * KT + stage_row;   // first position that this wave stages in a step
     bool bad = false, dirty = false;
-    auto window_at = [&](int p) {
+    auto request_window = [&](int p) {
+        return static_cast<uint32_t>(table[min((p >> a.page_shift) + lane, last_page)]);
+    };
+    auto window_of = [&](int p, uint32_t entry) {
         PageWindow w;
         w.first = p >> a.page_shift;
-        uint32_t entry = static_cast<uint32_t>(table[min(w.first + lane, last_page)]);
         bad |= end > 0 && entry >= static_cast<uint32_t>(a.pages);   // (of pages that the tile's rows see)
         entry = entry < static_cast<uint32_t>(a.pages) ? entry : 0;
         w.k = entry * static_cast<uint32_t>(a.k_page_stride >> 3);
@@ -539,10 +524,12 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         asm volatile("" : "+v"(w.k), "+v"(w.v));
         return w;
     };
-    PageWindow win = window_at(min(mine, max(end - 1, 0)));
+    const int window_from = min(mine, max(end - 1, 0));
+    PageWindow win = window_of(window_from, request_window(window_from));
     // Moves the window when the ROWS positions from p on are not within it.
     auto slide = [&](int p) {
-        if (p < end && (min(p + ROWS, end) - 1) >> a.page_shift >= win.first + kWave) win = window_at(p);
+        if (p < end && (min(p + ROWS, end) - 1) >> a.page_shift >= win.first + kWave)
+            win = window_of(p, request_window(p));
     };
     const uint32_t lds0 = lds_address(lds);
     auto k_at = [&](int stage) { return lds0 + (WK == 1 ? stage : wk) * KTILE; };
@@ -568,6 +555,33 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int v_off = v_row / VP::PER * VP::LOAD + v_row % VP::PER * 2 * D +
                       16 * (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
     const int v_move = VP::swizzle(v_row % VP::PER);
+
+    if (steps > 0) stage_k(0);
+    // Queries: lane (q, hi) holds elements 16 ks + 8 hi .. + 7 of row q.
+    uint4 qf[KS];
+    int seen;
+    {
+        const int row = row_at + (my_row < rows ? my_row : 0);
+        const int i = row / a.group;
+        seen = my_row < rows ? seen_by(sp.seq, i) : 0;
+        const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
+                              (kh * a.group + row - i * a.group) * a.q_head_stride;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = ldg16(src + 16 * ks + 8 * hi);
+    }
+    if (a.scale <= 0.0f) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            qf[ks] = make_uint4((qf[ks].x ^ flip) & keep, (qf[ks].y ^ flip) & keep, (qf[ks].z ^ flip) & keep,
+                                (qf[ks].w ^ flip) & keep);
+    }
+    // The queries are waited for here, with the first keys and in front of the
+    // first values: the compiler, which does not count the staged rows, would
+    // wait for every outstanding load at their first use inside the loop.
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+        asm volatile("" : "+v"(qf[ks].x), "+v"(qf[ks].y), "+v"(qf[ks].z), "+v"(qf[ks].w));
+    if (steps > 0) stage_v(0);
 
     // Scores of KB positions from base, softmax, and the weights packed for
     // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
@@ -651,10 +665,6 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     };
 
     uint4 pw[2 * NB];
-    if (steps > 0) {
-        stage_k(0);
-        stage_v(0);
-    }
     if constexpr (WK == 1) {
         for (int j = 0; j < steps; ++j) {
             const int base = k0 + j * STEP;
