@@ -86,7 +86,8 @@ _SIGNATURES = {
 def _fields(kinds: str):
     """ctypes fields from "type: name name; ..." in the header's order."""
     types = {"i": C.c_int32, "l": C.c_int64, "f": C.c_float, "p": C.c_void_p}
-    return [(name, types[part.split(":")[0].strip()]) for part in kinds.split(";") for name in part.split(":")[1].split()]
+    groups = [part.split(":") for part in kinds.split(";")]
+    return [(name, types[kind.strip()]) for kind, names in groups for name in names.split()]
 
 
 class PagedAppendArgs(C.Structure):
@@ -95,7 +96,8 @@ class PagedAppendArgs(C.Structure):
     _fields_ = _fields(
         "i: tokens heads kv_heads dim rotary pages page fp16; p: q k v;"
         "l: q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride;"
-        "p: q_norm k_norm; f: eps; i: rope_fp32; p: cos sin positions; i: rope_rows pad; p: slots q_out k_cache v_cache;"
+        "p: q_norm k_norm; f: eps; i: rope_fp32; p: cos sin positions; i: rope_rows pad;"
+        "p: slots q_out k_cache v_cache;"
         "l: k_page_stride k_cache_head_stride k_row_stride v_page_stride v_cache_head_stride v_row_stride")
 
 

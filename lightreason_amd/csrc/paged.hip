@@ -360,12 +360,10 @@ static void append_rows(const PagedAppendArgs& a, hipStream_t stream) {
     // 12.3 against 13.1), else one, where latency counts (1024 tokens 7.8 us
     // against 8.2 with four, 8 tokens 3.4 against 5.7).
     const int64_t pieces = (rows + 3) / 4;
-    if (a.tokens * pieces >= per * 768)
-        hipLaunchKernelGGL((paged_append_kernel<FP16, D, 4>), dim3(static_cast<unsigned>((a.tokens * pieces + per - 1) / per)),
-                           dim3(kThreads), 0, stream, a);
-    else
-        hipLaunchKernelGGL((paged_append_kernel<FP16, D, 1>), dim3(static_cast<unsigned>((a.tokens * rows + per - 1) / per)),
-                           dim3(kThreads), 0, stream, a);
+    const bool four = a.tokens * pieces >= per * 768;
+    const dim3 grid(static_cast<unsigned>((a.tokens * (four ? pieces : rows) + per - 1) / per));
+    if (four) hipLaunchKernelGGL((paged_append_kernel<FP16, D, 4>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((paged_append_kernel<FP16, D, 1>), grid, dim3(kThreads), 0, stream, a);
 }
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, bool fp16, int dim, hipStream_t stream) {

@@ -2,18 +2,37 @@
 // sequence b (n_b new positions, kv_b cached ones with them) sees positions
 // 0 .. kv_b - n_b + t: out = sum_p softmax(q . k_p scale)_p v_p, times
 // sigmoid(gate) when a gate is given.
+//
+// The rows that share keys and values (a sequence's new tokens, times the
+// query heads of one key/value head) form tiles of 32 or 128; a workgroup
+// takes a tile over a range of positions, in one pass: a block of scores
+// S^T = K Q^T, a running maximum m per row (sums are rescaled only when it
+// grew by more than 2^8: what is summed is relative to m, whatever m is, so
+// the result does not depend on it), weights exp2(s - m) rounded to the
+// tensors' type, and their product with the values into fp32 sums.  Both
+// products are 32x32x16 matrix instructions.  In the transposed form a lane
+// holds scores of one row only, so maxima and sums stay in the lane (and its
+// partner 32 lanes on), and the weights are the second product's operand as
+// they are, once the values are read in the matching order: the transposing
+// LDS read gives each lane four positions of one element.
+//
+// Keys and values go from the pages into LDS without passing registers, two
+// tiles ahead of their use, and are read from there by all four waves.  Width
+// 256 needs 192 registers per lane for queries and sums alone; what is left of
+// the 256 that two waves per SIMD may have goes to fragments read ahead
+// (read_ahead), which is why the LDS places (Place) are chosen for few
+// addresses.
+//
+// What bounds it (16 query over 2 key/value heads of 256, pages of 64): 4096
+// new positions over 28003 cached take 1.71 ms, 1.18 PFLOP/s; the matrix units
+// are busy in 67 % of the cycles and the card's power limit holds the clock at
+// 1.4-1.6 GHz then, LDS reads have no bank conflicts.  One decode position for
+// each of 64 sequences of 200-16000 takes 203 us, 5.4 TB/s of keys and values,
+// the rate of a large copy.  One sequence of 1000 takes 14.6 us, a chain of
+// reads (lengths, table, rows, partial rows) in two launches.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
-#include <stdlib.h>
-static int envi(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#ifndef AHEADN
-#define AHEADN 4
-#endif
-#define TARGET_FEW envi("TF", 1024)
-#define LEAST_FEW envi("LF", 1)
-#define TARGET_TILE envi("TT", 400)
-#define LEAST_TILE envi("LT", 8)
 
 namespace lrmoe {
 namespace {
@@ -146,7 +165,8 @@ __device__ __forceinline__ int tile_splits(int splits, int end, int per_split) {
 // first, and how many tiles there are; false past the last item, and for
 // starts that are not ascending within [0, tokens] (such a step is empty).
 template <int BM, int STEP>
-__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out, int* all_tiles) {
+__device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out,
+                                           int* all_tiles) {
     constexpr int HELD = 4;   // sequences per lane that stay in registers
     const int lane = threadIdx.x % kWave;
     const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
@@ -183,7 +203,7 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
     work = wave_butterfly_sum(work) * a.kv_heads;
     // Up to 64 sequences of many tiles are taken longest first, so that none of
     // the long ones starts last (nine prompts of 1-900 tokens over up to 5000
-    // cached: S1 us against S0 in their own order).
+    // cached: 290 us against 306 in their own order).
     int who_is = lane;   // the sequence of this lane's s[0]
     if (BM > 32 && a.seqs > 1 && a.seqs <= kWave) {
         int rank = 0;
@@ -420,12 +440,13 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
 
 // Orders the LDS reads of FRAGS operand fragments (READS instructions each)
 // and the products that take them: AHEAD fragments before the first product,
-// then one more after each product.  Left to itself the
-// compiler reads each fragment right before its product, to save registers,
-// and every product waits for LDS.
+// then one more after each.  Left to itself the compiler reads each fragment
+// right before its product, to save registers, and every product waits for
+// LDS (4096 positions over 28003 cached at width 256: 2.63 ms; 1.90 with four
+// ahead in both products; five or more cost spills or gain nothing).
 template <int FRAGS, int READS>
 __device__ __forceinline__ void read_ahead() {
-    constexpr int AHEAD = AHEADN, PRODUCT = 0x8, LDS_READ = 0x100;
+    constexpr int AHEAD = 4, PRODUCT = 0x8, LDS_READ = 0x100;
     __builtin_amdgcn_sched_group_barrier(LDS_READ, AHEAD * READS, 0);
 #pragma unroll
     for (int i = 0; i < FRAGS - AHEAD; ++i) {
@@ -435,7 +456,7 @@ __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD, 0);
 }
 
-// Highest value and sum over the two lanes (q, q + 32) that share a row.
+// Highest value over the two lanes (q, q + 32) that share a row.
 __device__ __forceinline__ float pair_max(float v) {
     const int x = __float_as_int(v);
     const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
@@ -443,24 +464,26 @@ __device__ __forceinline__ float pair_max(float v) {
 }
 
 struct Partials {
-    float* o;     // [slot][BM][D] sums of exp2(s - m) v
-    float* ml;    // [slot][BM][2] m, sum of exp2(s - m)
+    float* o;       // [slot][BM][D] sums of exp2(s - m) v
+    float* ml;      // [slot][BM][2] m, sum of exp2(s - m)
     Piece* pieces;  // [tiles]
-    int* dirty;     // [workgroups of the attention launch]: values that some of the tile's rows must not see
+    int* dirty;     // [workgroups of the attention launch]: the split holds values that some of its rows must not see
     int tiles, workgroups;
 };
 
 constexpr float kLowest = -1.7e38f;  // the running maximum before any position
 constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
 
-// WQ waves by 32 rows, or WK waves that share the rows and take positions of
-// their own; tiles of KT positions, worked through 32 NB at a time.
-template <bool FP16, int D, int WQ, int WK, int NB, int SUB, bool DENSE>
+// WQ waves of 32 rows each over the same tiles of 32 NB positions, which they
+// load together, two in flight (eight waves on one tile instead of two
+// workgroups of four per CU took 2.03 ms where these took 1.82: their barriers
+// keep them in step), or WK waves that share 32 rows and take tiles of their
+// own.
+template <bool FP16, int D, int WQ, int WK, int NB, bool DENSE>
 __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
     PagedAttnArgs a, Partials part, int target, int least) {
     constexpr int THREADS = kWave * WQ * WK;
-    constexpr int KB = 32 * NB;           // positions worked through at a time
-    constexpr int KT = KB * SUB;          // positions of a tile
+    constexpr int KT = 32 * NB;           // positions of a tile
     constexpr int STEP = KT * WK;         // positions per step of the workgroup
     constexpr int BM = 32 * WQ;
     typedef Place<D, false> KP;
@@ -583,10 +606,12 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         asm volatile("" : "+v"(qf[ks].x), "+v"(qf[ks].y), "+v"(qf[ks].z), "+v"(qf[ks].w));
     if (steps > 0) stage_v(0);
 
-    // Scores of KB positions from base, softmax, and the weights packed for
-    // the second product.  S^T = K Q^T, so a lane holds 16 NB positions of its
-    // row and the weights are the second product's operand as they are: of a
-    // step of 16 positions lane (q, hi) holds 4 hi + {0..3, 8..11}.
+    // Scores of the tile's KT positions from base, softmax, and the weights
+    // packed for the second product.  S^T = K Q^T, so a lane holds 16 NB
+    // positions of its row and the weights are the second product's operand as
+    // they are: of a step of 16 positions lane (q, hi) holds 4 hi + {0..3,
+    // 8..11}.  The weights are rounded to the tensors' type (a product of two
+    // 16-bit operands); their sum is not.
     auto scores = [&](uint32_t kt, int base, uint4 (&pw)[2 * NB]) {
         f32x16 s[NB] = {};
 #pragma unroll
@@ -598,7 +623,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 s[nb] = mfma32<FP16>(make_uint4(kv.x, kv.y, kv.z, kv.w), qf[ks], s[nb]);
             }
         read_ahead<NB * KS, 1>();
-        if (base + KB > least_seen) {
+        if (base + KT > least_seen) {
             asm volatile("" ::: "memory");   // a branch: not selects in every step
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -677,10 +702,9 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 stage_v(j + 1);
             }
             if (end > least_seen && base + KT > least_seen) look(v_at(j & 1));
-#pragma unroll 1
-            for (int u = 0; works && u < KT && base + u < k1; u += KB) {
-                scores(k_at(j & 1) + KP::bytes(u), base + u, pw);
-                values(v_at(j & 1) + VP::bytes(u), pw);
+            if (works) {
+                scores(k_at(j & 1), base, pw);
+                values(v_at(j & 1), pw);
             }
         }
     } else {
@@ -978,11 +1002,18 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
 struct Shape {
     int bm, step, target, least;
 };
-// The kernel of a step: one 32-row tile of four position groups where every
-// sequence's rows fit into it, else tiles of 128 rows.
+// The kernel of a step.  Where every sequence's rows fit into 32: one tile of
+// them, four waves on positions of their own, many splits (64 sequences of
+// 200-16000 positions: 204 us with a target of 1024, 227 with 512, 252 with
+// 2048; a split may be one step, so that a single sequence spreads).  Else
+// tiles of 128 rows, two workgroups per CU: a target of 400 lets the splits,
+// whose counts are rounded up, still fit the 512 places in one go (2048
+// positions from an empty cache: 87 us, 101 with 256, 114 with 512), and
+// splits of at least 8 steps, whose partial rows cost about as much (16
+// verify blocks: 35.6 us, 39.4 with 16).
 Shape shape_of(int group, int max_new, int dim) {
-    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, TARGET_FEW, LEAST_FEW};
-    return {128, dim == 256 ? 32 : 64, TARGET_TILE, LEAST_TILE};
+    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 1024, 1};
+    return {128, dim == 256 ? 32 : 64, 400, 8};
 }
 
 struct Layout {
@@ -994,12 +1025,13 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     const Shape sh = shape_of(group, max_new, dim);
     const int64_t tiles = static_cast<int64_t>(tokens) * group / sh.bm + (seqs < tokens ? seqs : tokens);
     // A tile has at most one split per `least` steps of what a row can hold;
-    // tiles of one sequence, where it has several, count up to twice.
+    // the tiles of a sequence of several count up to twice.
     const int64_t most = (capacity / sh.step + sh.least) / sh.least;
     const int64_t share = (sh.bm == 32 ? 1 : 2) * (sh.target / kv_heads + 1);   // splits beyond one per tile, per head
     const int64_t per_head = tiles * most < share + tiles ? tiles * most : share + tiles;
     const int64_t workgroups = per_head * kv_heads;
-    const int64_t slots = 2 * share * kv_heads + 16;   // (16: the work is summed in 24 bits)
+    const int64_t splits = 2 * share * kv_heads + 16;   // (16: the work is summed in 24 bits)
+    const int64_t slots = splits < workgroups ? splits : workgroups;
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1018,28 +1050,27 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     return l;
 }
 
+template <bool FP16, int D, int WQ, int WK, int NB>
+void launch_shape(const PagedAttnArgs& a, const Shape& sh, const Partials& part, int max_new, hipStream_t stream) {
+    const dim3 grid(part.workgroups), block(kWave * WQ * WK);
+    if (a.k_row_stride == D && a.v_row_stride == D)
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, true>), grid, block, 0, stream, a, part, sh.target,
+                           sh.least);
+    else
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, false>), grid, block, 0, stream, a, part,
+                           sh.target, sh.least);
+    // Merge workgroups per tile: a row each, or a block of 32 elements each.
+    const int64_t rows = static_cast<int64_t>(max_new) * a.group;
+    const unsigned each = WK == 1 ? D / 32 : static_cast<unsigned>(rows < 1 ? 1 : rows < 16 ? rows : 16);
+    hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ, WK == 1>), dim3(part.tiles, each), dim3(kThreads), 0,
+                       stream, a, part);
+}
+
 template <bool FP16, int D>
 hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
     const Shape sh = shape_of(a.group, max_new, D);
-    const unsigned grid = part.workgroups;
-    const int64_t most = static_cast<int64_t>(max_new) * a.group;   // rows of a tile
-    const bool dense = a.k_row_stride == D && a.v_row_stride == D;
-    // Merge workgroups per piece: a row each, or a block of 32 elements each.
-    const unsigned few = static_cast<unsigned>(most < 1 ? 1 : most < 16 ? most : 16);
-#define LR_ATTEND(WQ, WK, NB, SUB)                                                                                \
-    do {                                                                                                          \
-        if (dense)                                                                                                \
-            hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB, true>), dim3(grid),                  \
-                               dim3(kWave * WQ * WK), 0, stream, a, part, sh.target, sh.least);                   \
-        else                                                                                                      \
-            hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, SUB, false>), dim3(grid),                 \
-                               dim3(kWave * WQ * WK), 0, stream, a, part, sh.target, sh.least);                   \
-        hipLaunchKernelGGL((attend_merge_kernel<FP16, D, 32 * WQ, WK == 1>),                                      \
-                           dim3(part.tiles, WK == 1 ? D / 32 : few), dim3(kThreads), 0, stream, a, part);               \
-    } while (0)
-    if (sh.bm == 32) LR_ATTEND(1, 4, 1, 1);
-    else LR_ATTEND(4, 1, (D == 256 ? 1 : 2), 1);
-#undef LR_ATTEND
+    if (sh.bm == 32) launch_shape<FP16, D, 1, 4, 1>(a, sh, part, max_new, stream);
+    else launch_shape<FP16, D, 4, 1, (D == 256 ? 1 : 2)>(a, sh, part, max_new, stream);
     return hipGetLastError();
 }
 

@@ -126,7 +126,7 @@ class PageTable:
         """Key and value caches [layers, pages, kv_heads, page, head_dim] for
         this pool (uninitialised)."""
         shape = (layers, self.pages, kv_heads, self.page, head_dim)
-        return (torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device))
+        return tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
 
     def new_plan(self, tokens: int) -> PagePlan:
         """Empty outputs of a plan of up to ``tokens`` positions."""

@@ -535,8 +535,8 @@ def test_verified_tokens_follow_the_target(device):
     p = torch.tensor([0.4, 0.3, 0.15, 0.1, 0.05], device=device)
     q = torch.tensor([0.1, 0.2, 0.3, 0.2, 0.2], device=device)
     tokens = torch.multinomial(q, 2 * B, replacement=True, generator=g)
-    accepted, token = verify_drafts(tokens, p.expand(2 * B, 5).contiguous(), _ints(list(range(0, 2 * B + 1, 2)), device),
-                                    torch.rand(2 * B, generator=g, device=device),
+    accepted, token = verify_drafts(tokens, p.expand(2 * B, 5).contiguous(),
+                                    _ints(list(range(0, 2 * B + 1, 2)), device), torch.rand(2 * B, generator=g, device=device),
                                     torch.rand(B, generator=g, device=device), draft=q.expand(2 * B, 5).contiguous())
     first = torch.where(accepted == 1, tokens[1::2], token)
     share = torch.bincount(first, minlength=5).double() / B
