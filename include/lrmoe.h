@@ -583,11 +583,14 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * when a gate is given; softmax and sums in fp32.  A row that sees nothing
  * (kv_lengths[s] < n) is 0.  What a row does not see cannot change it,
  * infinities and NaN included.  Tokens outside starts[0] .. starts[seqs] - 1
- * are left as they were.  A table entry outside [0, pages) in use makes its
- * sequence's rows NaN; kv_lengths beyond max_pages pages are cut there.
- * max_new (at least every n) only chooses the kernel.  Strides as
- * lrmoe_paged_append's; row strides below 2^20, pages spread over at most
- * 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args) bytes,
+ * are left as they were, and all are when starts are not ascending within
+ * [0, tokens].  A table entry outside [0, pages) in use makes its sequence's
+ * rows NaN (those of earlier positions may keep their values); kv_lengths
+ * beyond max_pages pages are cut there.  max_new only chooses the kernel: at
+ * least every n, else the call is slower.  out must not overlap q or gate.
+ * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
+ * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
+ * bytes (about 210 MB at most for width 256, far less for short steps),
  * 256-byte aligned, not cleared, used by one stream at a time. */
 typedef struct lrmoe_paged_attention_args {
     int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */

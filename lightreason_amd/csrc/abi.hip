@@ -802,6 +802,7 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     if (p->tokens == 0 || p->seqs == 0) return LRMOE_OK;
     if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->starts || !p->kv_lengths || !p->out)
         return LRMOE_E_ARG;
+    if (p->out == p->q || p->out == p->gate) return LRMOE_E_ARG;
     if (misaligned(p->q, 16) || misaligned(p->k_cache, 16) || misaligned(p->v_cache, 16) || misaligned(p->out, 16) ||
         misaligned(p->gate, 16) || misaligned(workspace, 256))
         return LRMOE_E_ARG;

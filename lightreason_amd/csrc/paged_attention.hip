@@ -124,10 +124,11 @@ __device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t 
 // A sequence's rows (token-major, then the heads of one key/value head's
 // group) are cut into tiles of BM rows; a tile's positions into splits, so
 // that a few long sequences fill the chip.  W is the sum over all tiles of
-// their steps (of a sequence's tiles the mean of the first's and the last's)
-// and one; a split holds more than W / target steps.  A sequence's tiles all
-// get its longest tile's split count, so there are at most 2 target splits
-// and one per tile, and fewer than 4 target slots for tiles that are split.
+// their steps and one; a split holds more than W / target steps.  A sequence's
+// tiles all get its longest tile's split count, so tiles of 32 rows, all
+// counted as long as that one, make at most target splits and one per tile,
+// and fewer than 2 target slots for those that are split; longer tiles,
+// counted as the mean of the sequence's first and last, up to twice as many.
 // Every wave works this out for itself from starts and kv_lengths (a lane per
 // sequence, cross-lane sums, no LDS and no barrier): nothing of it depends on
 // the host, no launch precedes the attention's, and what it costs is the one
@@ -191,10 +192,10 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
 #pragma unroll
         for (int k = 0; k < HELD; ++k)
             if (s[k].n > 0) {
-                tiles += tiles_of(s[k].n, a.group, BM);
-                const int shortest = tile_end(s[k], a.group, BM, 0);
-                work += static_cast<float>(tiles_of(s[k].n, a.group, BM)) *
-                        (0.5f * (steps_of(s[k].kv, STEP) + steps_of(shortest, STEP)) + 1.0f);
+                const int count = tiles_of(s[k].n, a.group, BM), last = steps_of(s[k].kv, STEP);
+                const int first = BM > 32 ? steps_of(tile_end(s[k], a.group, BM, 0), STEP) : last;
+                tiles += count;
+                work += static_cast<float>(count) * (0.5f * (first + last) + 1.0f);
             }
     }
     *all_tiles = 0;
@@ -413,7 +414,8 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
             load_lds16_n<N, P::PAD>(lds_at + P::bytes(u), base, offset);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) load_lds16(lds_at + P::bytes(u) + i * P::LOAD, base + i * P::PER * pitch, offset);
+            for (int i = 0; i < N; ++i)
+                load_lds16(lds_at + P::bytes(u) + i * P::LOAD, base + i * P::PER * pitch, offset);
         }
     };
     if (pos + ROWS <= end) {

@@ -361,8 +361,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Softmax and sums are in fp32; the probabilities are rounded to the
     tensors' type before they meet the values.  A row that sees nothing is 0;
     what a row does not see cannot change it, infinities and NaN included;
-    tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``.
-    A table entry in use outside the pool makes its sequence's rows NaN.
+    tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``,
+    and all do when ``starts`` are not ascending within [0, tokens].  A table
+    entry in use outside the pool makes its sequence's rows NaN (those of
+    earlier positions may keep their values).  ``out`` must not overlap ``q``
+    or ``gate``.
 
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
     chooses the kernel: give it where the counts are known to be small."""

@@ -415,6 +415,62 @@ def test_attention_offsets_past_32_bits(device):
     assert bool(((out.double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("layout", [(16, 2, 256), (12, 3, 128), (1, 1, 64)])
+def test_attention_strided_caches_and_output(device, layout):
+    # Keys and values side by side in one pool of pages, rows of all heads
+    # together; the output one half of a wider buffer.
+    heads, K, D = layout
+    c, table, starts, kvs = _case(device, *layout, 16, [(77, 1), (333, 50), (1000, 3)], BF, seed=13, gate=True)
+    pages, page = c["k_cache"].shape[0], 16
+    pool = torch.empty(pages, page, 2, K, D, dtype=BF, device=device)
+    pool[:, :, 0], pool[:, :, 1] = c["k_cache"].transpose(1, 2), c["v_cache"].transpose(1, 2)
+    want = _run_attention(c)
+    wide = torch.full((c["q"].shape[0], heads, 2 * D), 5.0, dtype=BF, device=device)
+    c["k_cache"], c["v_cache"] = pool[:, :, 0].transpose(1, 2), pool[:, :, 1].transpose(1, 2)
+    out = _run_attention(c, out=wide[:, :, D:])
+    assert torch.equal(out, want) and bool((wide[:, :, :D] == 5.0).all())
+
+
+def test_attention_with_a_bound_that_is_too_small(device):
+    c, table, starts, kvs = _case(device, 16, 2, 256, 16, [(900, 300), (700, 700), (4000, 2)], BF, seed=14, gate=True)
+    _check(c, table, starts, kvs, _run_attention(c, max_new=1))
+    _check(c, table, starts, kvs, _run_attention(c, max_new=0))
+
+
+def test_attention_starts_out_of_order_are_an_empty_step(device):
+    c, *_ = _case(device, 8, 2, 64, 8, [(20, 2), (24, 3)], BF, seed=15)
+    out = torch.full(c["q"].shape, 3.0, dtype=BF, device=device)
+    for bad in ([0, 4, 2], [-1, 2, 5], [0, 2, 6]):
+        c["starts"] = _ints(bad, device)
+        assert bool((_run_attention(c, out=out) == 3.0).all())
+
+
+def test_calls_check_what_a_checked_form_cannot_tell(device):
+    from lightreason_amd.paged import paged_append, paged_attention
+
+    c, *_ = _case(device, 8, 2, 64, 8, [(20, 2), (24, 3)], BF, seed=16)
+    q = c["q"].contiguous()
+    args = (c["k_cache"], c["v_cache"], c["table"], c["starts"], c["kv_lengths"])
+    paged_attention(q, *args)
+    off = torch.empty(q.numel() + 4, dtype=BF, device=device)[4:].view(q.shape)   # the same form, 8 bytes off
+    with pytest.raises(ValueError):
+        paged_attention(off, *args)
+    with pytest.raises(ValueError):
+        paged_attention(q, *args, out=q)
+    k = torch.zeros(5, 2, 64, dtype=BF, device=device)
+    slots = torch.arange(5, device=device)
+    paged_append(k, k, *args[:2], slots)
+    with pytest.raises(ValueError):
+        paged_append(torch.empty(k.numel() + 4, dtype=BF, device=device)[4:].view(k.shape), k, *args[:2], slots)
+    with pytest.raises(ValueError):
+        paged_attention(q.cpu(), *args)
+    with pytest.raises(ValueError):
+        paged_attention(q, args[0], args[1][:, :, :4], *args[2:])
+    for kw in (dict(max_new=-1), dict(max_new=1.5), dict(gate=q[:, :4]), dict(out=q.half())):
+        with pytest.raises(ValueError):
+            paged_attention(q, *args, **kw)
+
+
 def test_attention_on_two_streams_at_once(device):
     cases = [_case(device, 16, 2, 256, 16, [(3000, 1)] * 8, BF, seed=s) for s in (1, 2)]
     want = [_run_attention(c[0], max_new=1) for c in cases]
@@ -535,9 +591,10 @@ def test_verified_tokens_follow_the_target(device):
     p = torch.tensor([0.4, 0.3, 0.15, 0.1, 0.05], device=device)
     q = torch.tensor([0.1, 0.2, 0.3, 0.2, 0.2], device=device)
     tokens = torch.multinomial(q, 2 * B, replacement=True, generator=g)
+    uniforms, samples = torch.rand(2 * B, generator=g, device=device), torch.rand(B, generator=g, device=device)
     accepted, token = verify_drafts(tokens, p.expand(2 * B, 5).contiguous(),
-                                    _ints(list(range(0, 2 * B + 1, 2)), device), torch.rand(2 * B, generator=g, device=device),
-                                    torch.rand(B, generator=g, device=device), draft=q.expand(2 * B, 5).contiguous())
+                                    _ints(list(range(0, 2 * B + 1, 2)), device), uniforms, samples,
+                                    draft=q.expand(2 * B, 5).contiguous())
     first = torch.where(accepted == 1, tokens[1::2], token)
     share = torch.bincount(first, minlength=5).double() / B
     # five standard deviations of a share of 40000 draws

@@ -113,7 +113,7 @@ def _attention_args(**kw):
     base = dict(seqs=1, tokens=1, max_new=1, heads=16, kv_heads=2, dim=256, pages=4, page=16, max_pages=4, scale=1.0,
                 q=256, q_token_stride=4096, q_head_stride=256, k_cache=256, v_cache=256, k_page_stride=8192,
                 k_head_stride=4096, k_row_stride=256, v_page_stride=8192, v_head_stride=4096, v_row_stride=256,
-                table=256, starts=256, kv_lengths=256, out=256, out_token_stride=4096, out_head_stride=256)
+                table=256, starts=256, kv_lengths=256, out=512, out_token_stride=4096, out_head_stride=256)
     base.update(kw)
     return _native.PagedAttentionArgs(**base)
 
@@ -131,7 +131,9 @@ def test_abi_attention_refuses_before_any_launch():
                dict(k_cache=0), dict(v_cache=0), dict(table=0), dict(starts=0), dict(kv_lengths=0), dict(out=0),
                dict(q=264), dict(k_cache=8), dict(v_cache=24), dict(out=8), dict(gate=8), dict(q_token_stride=4),
                dict(k_row_stride=260), dict(v_page_stride=4), dict(out_token_stride=4),
-               dict(gate=256, gate_head_stride=4)):
+               dict(gate=256, gate_head_stride=4), dict(out=256), dict(gate=512), dict(k_row_stride=1 << 20),
+               dict(v_row_stride=-8), dict(pages=1 << 30, k_page_stride=1 << 20), dict(v_page_stride=-8),
+               dict(tokens=1 << 19, heads=1024, kv_heads=1)):
         assert call(_attention_args(**kw)) == -1, kw
     assert call(_attention_args(), ws=8) == -1
     need = lib.lrmoe_paged_attention_workspace_bytes(C.addressof(_attention_args()))
