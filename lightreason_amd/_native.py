@@ -211,18 +211,19 @@ _traits = attrgetter("dtype", "shape", "device")
 _stride = methodcaller("stride")
 
 
-def signature(tensors, *rest):
-    """What the checks of a call depend on: types, shapes, devices and strides
-    of its tensors (None for one that is left out) and its other arguments;
-    None where there is no such thing.  Addresses are not part of it: the
-    library checks their alignment in every call."""
+def checked(forms: dict, tensors, *rest):
+    """(signature, form): what the checks of a call depend on -- types,
+    shapes, devices and strides of its tensors (None for one that is left
+    out) and its other arguments -- and the form kept for it, if any; (None,
+    None) where an argument is not what it should be.  Addresses are not part
+    of it: the library checks their alignment in every call."""
     try:
         given = [t for t in tensors if t is not None]
-        key = (tuple(map(_traits, given)), tuple(map(_stride, given)), tuple([t is None for t in tensors]), rest)
-        hash(key)
-        return key
+        missing = None if len(given) == len(tensors) else tuple([t is None for t in tensors])
+        key = (tuple(map(_traits, given)), tuple(map(_stride, given)), missing, rest)
+        return key, forms.get(key)
     except (AttributeError, TypeError, RuntimeError):
-        return None
+        return None, None
 
 
 def remember(forms: dict, key, form) -> None:
@@ -231,3 +232,19 @@ def remember(forms: dict, key, form) -> None:
         if len(forms) >= 1024:
             forms.clear()
         forms[key] = form
+
+
+_WORKSPACES: dict = {}
+
+
+def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch (not cleared) of torch's current stream on `device`, grown as
+    calls need it.  A call under capture gets scratch of its own from its
+    graph's memory, so that graphs replayed on different streams share none."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device, current_stream(device))
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _WORKSPACES[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws

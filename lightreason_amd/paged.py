@@ -250,8 +250,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     slot lies outside the pool (-1: padding) is left out, its q_out row too;
     tokens must not share a slot."""
     tensors = (k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out)
-    key = _native.signature(tensors, eps)
-    form = _APPENDS.get(key)
+    key, form = _native.checked(_APPENDS, tensors, eps)
     if form is None:
         form = _check_append(*tensors, eps)
         _native.remember(_APPENDS, key, form)
@@ -329,22 +328,6 @@ def _check_append(k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, po
 
 # ---- attention ------------------------------------------------------------------
 
-_WORKSPACES: dict = {}
-
-
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch of the current stream, grown as calls need it.  A call under
-    capture gets scratch of its own from its graph's memory, so that graphs
-    replayed on different streams share none."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device, _stream(device))
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _WORKSPACES[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws
-
-
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
                     starts: torch.Tensor, kv_lengths: torch.Tensor, *, max_new: int | None = None,
                     scale: float | None = None, gate: torch.Tensor | None = None,
@@ -370,8 +353,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
     chooses the kernel: give it where the counts are known to be small."""
     tensors = (q, k_cache, v_cache, table, starts, kv_lengths, gate, out)
-    key = _native.signature(tensors, max_new, scale)
-    form = _ATTENTIONS.get(key)
+    key, form = _native.checked(_ATTENTIONS, tensors, max_new, scale)
     if form is None:
         form = _check_attention(*tensors, max_new, scale)
         _native.remember(_ATTENTIONS, key, form)
@@ -385,7 +367,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a.table, a.starts, a.kv_lengths = table.data_ptr(), starts.data_ptr(), kv_lengths.data_ptr()
     a.out = out.data_ptr()
     with _on(dev):
-        ws = _workspace(dev, nbytes)
+        ws = _native.workspace(dev, nbytes)
         _native.call("lrmoe_paged_attention", C.addressof(a), ws.data_ptr(), ws.numel(), _stream(dev))
     return out
 

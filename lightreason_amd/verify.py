@@ -159,8 +159,7 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
     block of one row is plain sampling.  ``PageTable.commit(plan, accepted)``
     takes the result into the page pool."""
     tensors = (tokens, target, starts, uniforms, samples, draft, accepted, next_tokens)
-    key = _native.signature(tensors)
-    form = _VERIFIES.get(key)
+    key, form = _native.checked(_VERIFIES, tensors)
     if form is None:
         form = _check_verify(*tensors)
         _native.remember(_VERIFIES, key, form)
@@ -172,13 +171,11 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
     if blocks == 0:
         return accepted, next_tokens
     with _native.on_device(dev):
-        # From torch's allocator, which keeps it for this stream's next calls
-        # (and, under capture, in the graph's own memory).
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        scratch = _native.workspace(dev, nbytes)
         _native.call("lrmoe_verify_drafts", blocks, rows, vocab, kind, tokens.data_ptr(), target.data_ptr(),
                      target_stride, None if draft is None else draft.data_ptr(), draft_stride, starts.data_ptr(),
                      uniforms.data_ptr(), samples.data_ptr(), accepted.data_ptr(), next_tokens.data_ptr(),
-                     scratch.data_ptr(), nbytes, _native.current_stream(dev))
+                     scratch.data_ptr(), scratch.numel(), _native.current_stream(dev))
     return accepted, next_tokens
 
 
