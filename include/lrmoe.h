@@ -581,8 +581,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * starts[s] .. starts[s + 1] - 1, n in all) sees cached positions 0 ..
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
  * when a gate is given; softmax and sums in fp32.  A row that sees nothing
- * (kv_lengths[s] < n) is 0.  What a row does not see cannot change it,
- * infinities and NaN included.  Tokens outside starts[0] .. starts[seqs] - 1
+ * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
+ * row does not see cannot change it, infinities and NaN included.  Tokens outside starts[0] .. starts[seqs] - 1
  * are left as they were, and all are when starts are not ascending within
  * [0, tokens].  A table entry outside [0, pages) in use makes its sequence's
  * rows NaN (those of earlier positions may keep their values); kv_lengths

@@ -112,7 +112,7 @@ __device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t 
     const uint16_t* gate = a.gate + t * a.gate_token_stride + h * a.gate_head_stride + lane * E;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        float o = l == 0.0f ? 0.0f : acc[i] / l;
+        float o = seen > 0 ? acc[i] / l : 0.0f;
         if (nan) o = __builtin_nanf("");
         if (a.gate != nullptr) o *= sigmoid(elem16<FP16>(gate[i]));
         out[i] = static_cast<uint16_t>(FP16 ? f_to_f16(o) : f2bf(o));
@@ -261,14 +261,15 @@ struct Piece {
     Sequence seq;
 };
 
-// Eight elements d .. d + 7 of a row's result: sums over l, times the gate,
-// rounded once.
+// Eight elements d .. d + 7 of a row's result: sums over l (0 for a row that
+// sees nothing; where every score that it sees is -inf, l is 0 and the result
+// NaN, as the softmax is), times the gate, rounded once.
 template <bool FP16>
 __device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
                                            const float* v, float l) {
     const int i = row / a.group;
     const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = seen_by(s, i) > 0 ? 1.0f / l : 0.0f;
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
@@ -333,15 +334,15 @@ __device__ __forceinline__ void load_lds16_n(uint32_t lds_at, const void* base, 
         load_lds16(lds_at, base, offset);
     else if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400"
                      :
                      : "s"(lds_at), "v"(offset), "s"(base), "n"(PAD)
                      : "memory", "scc");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
-                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:2048\n\t"
-                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x800\n\t"
+                     "s_add_u32 m0, m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:0xc00"
                      :
                      : "s"(lds_at), "v"(offset), "s"(base), "n"(PAD)
                      : "memory", "scc");
@@ -458,6 +459,12 @@ __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD, 0);
 }
 
+// A product that no later operation is fused with.
+__device__ __forceinline__ float opaque(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Highest value over the two lanes (q, q + 32) that share a row.
 __device__ __forceinline__ float pair_max(float v) {
     const int x = __float_as_int(v);
@@ -473,8 +480,13 @@ struct Partials {
     int tiles, workgroups;
 };
 
-constexpr float kLowest = -1.7e38f;  // the running maximum before any position
-constexpr float kSlack = 8.0f;       // a maximum may lag by 2^8 before sums are rescaled
+constexpr float kLowest = -3.40282347e38f;  // the running maximum before any position: no finite score is below
+constexpr float kSlack = 8.0f;              // a maximum may lag by 2^8 before sums are rescaled
+// From this maximum on, a score's product with the scale is rounded before the
+// maximum is taken off it: the exact product (one fused operation, below)
+// differs from the maximum, which is a rounded one, by up to 2^-24 of it, and
+// weights of 2^that would leave fp16's range.
+constexpr float kRounded = 4194304.0f;
 
 // WQ waves of 32 rows each over the same tiles of 32 NB positions, which they
 // load together, two in flight (eight waves on one tile instead of two
@@ -651,6 +663,18 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[db][i] *= fall;
         }
+        float factor = scale, off = m;
+        if (__any(__builtin_fabsf(m) > kRounded && m != kLowest)) {
+            factor = 1.0f;
+            off = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float product = s[nb][i] * scale;
+                    s[nb][i] = opaque(product) - m;
+                }
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -659,7 +683,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 float w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * k + j], scale, -m));
+                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * k + j], factor, -off));
                     sum += w[j];
                 }
                 pw[2 * nb + k] = pack16<FP16>(w);
@@ -820,7 +844,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         constexpr int CHUNKS = 8 * DBC;   // of four floats, per row
         static_assert(32 * 32 * DBC * 4 * WQ <= LDS, "the rows fit");
         float4* mine_at = reinterpret_cast<float4*>(lds) + wave * 32 * CHUNKS;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = seen > 0 ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int d0 = 0; d0 < DB; d0 += DBC) {
             wave_lds_fence();

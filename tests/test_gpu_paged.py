@@ -437,6 +437,63 @@ def test_attention_with_a_bound_that_is_too_small(device):
     _check(c, table, starts, kvs, _run_attention(c, max_new=0))
 
 
+def _one_element(c, q0, keys):
+    """Queries of q0 in element 0 and 0 elsewhere; keys[p] in element 0 of
+    every position p of sequence 0."""
+    c["q"].zero_()
+    c["q"][..., 0] = q0
+    page = c["k_cache"].shape[2]
+    for p, x in enumerate(keys):
+        c["k_cache"][int(c["table"][0, p // page]), :, p % page, 0] = x
+
+
+@pytest.mark.parametrize("layout", [(16, 2, 256), (6, 2, 128), (8, 2, 64)])
+@pytest.mark.parametrize("dtype,q0,k0,scale", [(BF, 2.0 ** 64, -(2.0 ** 63), 1.0), (BF, 2.0 ** 20, 1.5 * 2.0 ** 20, 0.3),
+                                               (HF, 60000.0, 60000.0, 0.7), (HF, -60000.0, 60000.0, 0.7)])
+@pytest.mark.parametrize("kv,n", [(300, 1), (300, 200)])
+def test_attention_scores_at_the_ends_of_the_range(device, layout, dtype, q0, k0, scale, kv, n):
+    # Every third position has the row's highest score, the others one that is
+    # lower by far more than a softmax tells apart: their weights are exactly
+    # 1 and 0 and the result is a mean of values.  Error: fp32 sums of kv
+    # terms, a division (kv + 2 roundings of 2^-24 at most), one rounding.
+    c, table, starts, kvs = _case(device, *layout, 16, [(kv, n)], dtype, seed=20)
+    lower = k0 * (0.5 if q0 * k0 > 0 else 1.5)
+    _one_element(c, q0, [k0 if p % 3 == 1 else lower for p in range(kv)])
+    got = _run_attention(c, max_new=n, scale=scale)
+    v = ref.gathered(c["v_cache"], table[0][:-(-kv // 16)], kv)
+    used = (torch.arange(kv, device=device) % 3 == 1).double()
+    sums, sizes = (v * used[:, None]).cumsum(1), (v.abs() * used[:, None]).cumsum(1)
+    at = kv - n + torch.arange(n, device=device)
+    count = used.cumsum(0)[at][:, None, None]
+    group = layout[0] // layout[1]
+
+    def rows(x):
+        return x[:, at].transpose(0, 1).repeat_interleave(group, dim=1) / count
+    want, size = rows(sums), rows(sizes)
+    bound = want.abs() * ref.half_step(dtype) + size * (kv + 2) * 2.0 ** -24 * 1.01 + torch.finfo(dtype).tiny
+    live = count[:, 0, 0] > 0
+    assert bool(((got.double() - want).abs() <= bound)[live].all())
+
+
+@pytest.mark.parametrize("layout", [(16, 2, 256), (8, 2, 64)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_rows_whose_scores_are_all_minus_infinity_are_nan(device, layout, dtype):
+    # As the softmax of such a row is; a row that sees one finite score ignores them.
+    for kv, n in ((40, 40), (9, 1), (40, 1), (300, 300)):
+        c, table, starts, kvs = _case(device, *layout, 16, [(kv, n), (0, 2)], dtype, seed=21)
+        c["q"][..., 0] = 1.0
+        page = 16
+        for p in range(min(kv, 10)):
+            c["k_cache"][table[0][p // page], :, p % page, 0] = -math.inf
+        got = _run_attention(c, max_new=n)
+        lost = max(0, min(n, 10 - (kv - n)))   # rows that see such positions only
+        assert bool(torch.isnan(got[:lost]).all()) and bool((got[n:] == 0).all())
+        want, spread, score = ref.attention(c["q"], c["k_cache"], c["v_cache"], table, starts, kvs, layout[2] ** -0.5)
+        top = float(c["v_cache"][torch.isfinite(c["v_cache"])].abs().max())
+        bound = ref.attention_bound(want, spread, score, dtype, layout[2], kv, top)
+        assert bool(((got.double() - want).abs() <= bound)[lost:n].all())
+
+
 def test_attention_starts_out_of_order_are_an_empty_step(device):
     c, *_ = _case(device, 8, 2, 64, 8, [(20, 2), (24, 3)], BF, seed=15)
     out = torch.full(c["q"].shape, 3.0, dtype=BF, device=device)
