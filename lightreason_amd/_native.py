@@ -7,6 +7,7 @@ not gfx950 every entry point raises; there is no fallback.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from contextlib import nullcontext
 from functools import lru_cache
 from operator import attrgetter, methodcaller
@@ -234,17 +235,23 @@ def remember(forms: dict, key, form) -> None:
         forms[key] = form
 
 
-_WORKSPACES: dict = {}
+_WORKSPACES = threading.local()
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch (not cleared) of torch's current stream on `device`, grown as
-    calls need it.  A call under capture gets scratch of its own from its
-    graph's memory, so that graphs replayed on different streams share none."""
+    """Scratch (not cleared) of this thread on torch's current stream of
+    `device`, grown as calls need it: two threads' calls on one stream may
+    come with their launches mixed, so they share none.  A call under capture
+    gets scratch of its own from its graph's memory, so that graphs replayed
+    on different streams share none."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    try:
+        held = _WORKSPACES.held
+    except AttributeError:
+        held = _WORKSPACES.held = {}
     key = (device, current_stream(device))
-    ws = _WORKSPACES.get(key)
+    ws = held.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _WORKSPACES[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = held[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return ws

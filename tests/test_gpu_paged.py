@@ -528,6 +528,34 @@ def test_calls_check_what_a_checked_form_cannot_tell(device):
             paged_attention(q, *args, **kw)
 
 
+def test_threads_share_no_scratch(device):
+    # Two threads' calls on one stream may have their launches mixed.
+    import threading
+
+    from lightreason_amd import _native
+
+    mine, seen = _native.workspace(device, 1000), []
+    other = threading.Thread(target=lambda: seen.append(_native.workspace(device, 1000)))
+    other.start()
+    other.join()
+    assert _native.workspace(device, 1000).data_ptr() == mine.data_ptr() != seen[0].data_ptr()
+
+    cases = [_case(device, 16, 2, 256, 16, [(2000, 1)] * 4, BF, seed=s)[0] for s in (1, 2)]
+    want = [_run_attention(c, max_new=1) for c in cases]
+    got = [[], []]
+
+    def work(i):
+        for _ in range(20):
+            got[i].append(_run_attention(cases[i], max_new=1))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert [len(g) for g in got] == [20, 20]
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
 def test_attention_on_two_streams_at_once(device):
     cases = [_case(device, 16, 2, 256, 16, [(3000, 1)] * 8, BF, seed=s) for s in (1, 2)]
     want = [_run_attention(c[0], max_new=1) for c in cases]
