@@ -250,6 +250,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     slot lies outside the pool (-1: padding) is left out, its q_out row too;
     tokens must not share a slot."""
     tensors = (k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out)
+    eps = float(eps)   # a number, whatever held it: forms are kept by value
     key, form = _native.checked(_APPENDS, tensors, eps)
     if form is None:
         form = _check_append(*tensors, eps)
@@ -315,7 +316,7 @@ def _check_append(k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, po
     if N == 0:
         return None, dev, q_shape
     a = _native.PagedAppendArgs(tokens=N, heads=heads, kv_heads=K, dim=D, rotary=rotary, pages=pages, page=page,
-                                fp16=int(dtype == torch.float16), eps=float(eps),
+                                fp16=int(dtype == torch.float16), eps=eps,
                                 rope_fp32=int(cos is not None and cos.dtype == torch.float32), rope_rows=rows)
     if q is not None:
         a.q_token_stride, a.q_head_stride = _strides(q)
@@ -353,6 +354,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
     chooses the kernel: give it where the counts are known to be small."""
     tensors = (q, k_cache, v_cache, table, starts, kv_lengths, gate, out)
+    if scale is not None:
+        scale = float(scale)
     key, form = _native.checked(_ATTENTIONS, tensors, max_new, scale)
     if form is None:
         form = _check_attention(*tensors, max_new, scale)
@@ -399,7 +402,7 @@ def _check_attention(q, k_cache, v_cache, table, starts, kv_lengths, gate, out, 
         return None, dev, 0
     a = _native.PagedAttentionArgs(seqs=S, tokens=N, max_new=min(max_new, N), heads=H, kv_heads=K, dim=D, pages=pages,
                                    page=page, max_pages=width, fp16=int(dtype == torch.float16),
-                                   scale=D ** -0.5 if scale is None else float(scale))
+                                   scale=D ** -0.5 if scale is None else scale)
     a.q_token_stride, a.q_head_stride = _strides(q)
     if gate is not None:
         a.gate_token_stride, a.gate_head_stride = _strides(gate)

@@ -528,6 +528,22 @@ def test_calls_check_what_a_checked_form_cannot_tell(device):
             paged_attention(q, *args, **kw)
 
 
+def test_numbers_held_in_tensors_count_by_value(device):
+    from lightreason_amd.paged import paged_append
+
+    c, *rest = _case(device, 8, 2, 64, 8, [(20, 2), (24, 3)], BF, seed=17)
+    scale = torch.tensor(0.25)
+    for x in (0.25, 0.5):
+        scale.fill_(x)
+        _check(c, *rest, _run_attention(c, scale=scale), scale=x)
+    k, slots, eps = torch.ones(5, 2, 64, dtype=BF, device=device), torch.arange(5, device=device), torch.tensor(0.0)
+    norm = torch.zeros(64, dtype=BF, device=device)
+    for x, want in ((0.0, 1.0), (3.0, 0.5)):
+        eps.fill_(x)
+        paged_append(k, k, c["k_cache"], c["v_cache"], slots, k_norm=norm, eps=eps)
+        assert bool((c["k_cache"][0, :, :5] == want).all())
+
+
 def test_threads_share_no_scratch(device):
     # Two threads' calls on one stream may have their launches mixed.
     import threading
