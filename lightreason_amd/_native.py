@@ -113,6 +113,7 @@ class PagedAttentionArgs(C.Structure):
 
 
 PAGE_MAX_ROWS = 4096     # rows (sequences) of a page pool
+PAGE_MAX_POSITIONS = 1 << 30  # max_pages * page at most
 PAGE_STATUS_TOKENS = 1   # a negative count, or more new positions than the plan has room for
 PAGE_STATUS_ROW = 2      # a row past its pages, or corrupt
 PAGE_STATUS_POOL = 4     # not enough free pages

@@ -684,6 +684,10 @@ static bool bad_page(int page) { return page < 8 || page > 1024 || (page & (page
 static bool bad_pool(int rows, int pages, int max_pages) {
     return rows < 0 || rows > LRMOE_PAGE_MAX_ROWS || pages < 1 || max_pages < 1;
 }
+// (A row's positions, and a tile past them, stay within 31 bits.)
+static bool bad_capacity(int max_pages, int page) {
+    return static_cast<int64_t>(max_pages) * page > LRMOE_PAGE_MAX_POSITIONS;
+}
 static int shift_of(int page) { return __builtin_ctz(static_cast<unsigned>(page)); }
 
 int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, const int32_t* new_tokens,
@@ -691,7 +695,7 @@ int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, co
                     int32_t* table, int32_t* starts, int32_t* kv_lengths, int32_t* held_out, int32_t* positions,
                     int64_t* slots, int32_t* info, void* stream) {
     if (bad_pool(rows, pages, max_pages) || bad_page(page) || tokens < 0 || tokens > (1 << 24) ||
-        static_cast<int64_t>(max_pages) * page > INT32_MAX)
+        bad_capacity(max_pages, page))
         return LRMOE_E_ARG;
     if (rows == 0) return LRMOE_OK;
     if (!new_tokens || !lengths || !held || !free_pages || !state || !table || !starts || !kv_lengths || !held_out ||
@@ -787,7 +791,7 @@ static bool bad_attention(const lrmoe_paged_attention_args* p) {
     return p->seqs < 0 || p->seqs > LRMOE_PAGE_MAX_ROWS || p->tokens < 0 || p->tokens > (1 << 20) || p->max_new < 0 ||
            p->heads < 1 || p->heads > 1024 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || bad_dim(p->dim) ||
            static_cast<int64_t>(p->tokens) * p->heads > (1 << 28) || p->pages < 1 || bad_page(p->page) ||
-           p->max_pages < 1 || static_cast<int64_t>(p->max_pages) * p->page > INT32_MAX;
+           p->max_pages < 1 || bad_capacity(p->max_pages, p->page);
 }
 
 size_t lrmoe_paged_attention_workspace_bytes(const lrmoe_paged_attention_args* p) {

@@ -99,9 +99,10 @@ class PagePlan:
 
 class PageTable:
     """``pages`` pages of ``page`` positions shared by ``rows`` sequences of at
-    most ``max_pages`` pages each.  ``table`` [rows, max_pages], ``held`` and
-    ``lengths`` [rows], ``free_pages`` [pages] and ``state`` [4] (free pages,
-    epoch, status bits, 0) are int32 device tensors.
+    most ``max_pages`` pages each (no more than 2^30 positions).  ``table``
+    [rows, max_pages], ``held`` and ``lengths`` [rows], ``free_pages`` [pages]
+    and ``state`` [4] (free pages, epoch, status bits, 0) are int32 device
+    tensors.
 
     A step is ``plan`` -> its kernels -> ``commit``.  A plan changes nothing
     that counts until it is committed, so it may be made again; a plan made
@@ -113,7 +114,8 @@ class PageTable:
         self.page = _int(page, "page", 8, 1024)
         if page & (page - 1):
             raise ValueError(f"page must be a power of two, got {page}")
-        self.max_pages = _int(pages if max_pages is None else max_pages, "max_pages", 1, (2**31 - 1) // page)
+        self.max_pages = _int(pages if max_pages is None else max_pages, "max_pages", 1,
+                              _native.PAGE_MAX_POSITIONS // page)
         i32 = dict(dtype=torch.int32, device=device)
         self.table = torch.full((rows, self.max_pages), -1, **i32)
         self.held = torch.zeros(rows, **i32)

@@ -415,6 +415,18 @@ def test_attention_offsets_past_32_bits(device):
     assert bool(((out.double() - want).abs() <= bound).all())
 
 
+def test_attention_over_as_many_positions_as_a_row_can_hold(device):
+    # 2^30 positions, all in two pages: the attention over those 2048.  The
+    # longest chain of fp32 sums is a wave's share of a split, 2^18 at most.
+    c, table, starts, _ = _case(device, 2, 1, 64, 1024, [(2048, 2)], BF, seed=22)
+    c["table"] = c["table"][:, :2].repeat(1, 1 << 19).contiguous()
+    c["kv_lengths"] = _ints([1 << 30], device)
+    got = _run_attention(c, max_new=2)
+    want, spread, score = ref.attention(c["q"], c["k_cache"], c["v_cache"], table, starts, [2048], 64 ** -0.5)
+    bound = ref.attention_bound(want, spread, score, BF, 64, 1 << 18, 0.0)
+    assert bool(((got.double() - want).abs() <= bound)[1:].all())
+
+
 @pytest.mark.parametrize("layout", [(16, 2, 256), (12, 3, 128), (1, 1, 64)])
 def test_attention_strided_caches_and_output(device, layout):
     # Keys and values side by side in one pool of pages, rows of all heads

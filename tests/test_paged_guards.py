@@ -35,7 +35,8 @@ def test_structures_match_the_header():
 
 def test_page_table_refuses_bad_sizes():
     for kw in (dict(rows=0), dict(rows=4097), dict(pages=0), dict(page=4), dict(page=24), dict(page=2048),
-               dict(max_pages=0), dict(rows=2.0), dict(pages=True), dict(page=1024, max_pages=1 << 22)):
+               dict(max_pages=0), dict(rows=2.0), dict(pages=True), dict(page=1024, max_pages=1 << 22),
+               dict(page=1024, max_pages=(1 << 20) + 1)):
         args = dict(rows=2, pages=10, page=16, max_pages=None, device="cpu")
         args.update(kw)
         with pytest.raises(ValueError):
@@ -127,7 +128,8 @@ def test_abi_attention_refuses_before_any_launch():
     assert lib.lrmoe_paged_attention(None, 256, big, None) == -1
     for kw in (dict(seqs=-1), dict(seqs=4097), dict(tokens=-1), dict(tokens=(1 << 20) + 1), dict(max_new=-1),
                dict(heads=0), dict(kv_heads=0), dict(heads=15), dict(heads=2048), dict(dim=96), dict(pages=0),
-               dict(page=4), dict(page=48), dict(page=2048), dict(max_pages=0), dict(max_pages=1 << 28), dict(q=0),
+               dict(page=4), dict(page=48), dict(page=2048), dict(max_pages=0), dict(max_pages=1 << 28), dict(max_pages=(1 << 26) + 1),
+               dict(q=0),
                dict(k_cache=0), dict(v_cache=0), dict(table=0), dict(starts=0), dict(kv_lengths=0), dict(out=0),
                dict(q=264), dict(k_cache=8), dict(v_cache=24), dict(out=8), dict(gate=8), dict(q_token_stride=4),
                dict(k_row_stride=260), dict(v_page_stride=4), dict(out_token_stride=4),
