@@ -124,11 +124,11 @@ __device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t 
 // A sequence's rows (token-major, then the heads of one key/value head's
 // group) are cut into tiles of BM rows; a tile's positions into splits, so
 // that a few long sequences fill the chip.  W is the sum over all tiles of
-// their steps and one; a split holds more than W / target steps.  A sequence's
-// tiles all get its longest tile's split count, so tiles of 32 rows, all
-// counted as long as that one, make at most target splits and one per tile,
-// and fewer than 2 target slots for those that are split; longer tiles,
-// counted as the mean of the sequence's first and last, up to twice as many.
+// their steps and one; c steps, more than W / target, are the most of a split.
+// Tiles of 32 rows are all counted as long as their sequence's last, so they
+// make at most target splits and one per tile, and fewer than 2 target slots
+// for those that are split; longer tiles, counted as the mean of the
+// sequence's first and last, up to twice as many.
 // Every wave works this out for itself from starts and kv_lengths (a lane per
 // sequence, cross-lane sums, no LDS and no barrier): nothing of it depends on
 // the host, no launch precedes the attention's, and what it costs is the one
@@ -144,7 +144,6 @@ struct Split {
     int b, tile, split, splits;
     int slot;       // of the tile's first partial rows, before the head
     int ordinal;    // of the tile among all tiles
-    int per_split;  // steps
     Sequence seq;
 };
 
@@ -155,11 +154,12 @@ __device__ __forceinline__ int tile_end(const Sequence& s, int group, int bm, in
     const int rows = min((tile + 1) * bm, s.n * group);
     return seen_by(s, (rows - 1) / group);
 }
-// A tile takes its sequence's split count, or fewer where causality leaves it
-// fewer steps.
-template <int STEP>
-__device__ __forceinline__ int tile_splits(int splits, int end, int per_split) {
-    return min(splits, (steps_of(end, STEP) + per_split - 1) / per_split);
+// Tiles (of the sequence's `count`) of at most `splits` splits of c steps: the
+// first ones, which see least.
+template <int BM, int STEP>
+__device__ __forceinline__ int tiles_upto(const Sequence& s, int group, int count, int splits, int c) {
+    const int64_t tokens = static_cast<int64_t>(splits) * c * STEP - s.kv + s.n;   // that see no more than that
+    return tokens >= s.n ? count : tokens <= 0 ? 0 : static_cast<int>(tokens) * group / BM;
 }
 
 // The sequence, tile and split of item `item` (wave-uniform), heavy tiles
@@ -225,24 +225,42 @@ __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int
 #pragma unroll
         for (int k = 0; k < HELD; ++k) {
             if (base + k * kWave >= a.seqs) break;
+            // A tile of t splits stands in t - 1 of the sums over all splits
+            // but the first of the tiles that have more.
             const int splits = (steps_of(s[k].kv, STEP) + c - 1) / c;
-            const int count = tiles_of(s[k].n, a.group, BM), items = count * splits, slots = splits > 1 ? items : 0;
+            const int count = tiles_of(s[k].n, a.group, BM);
+            int items = count * splits, slots = splits > 1 ? items : 0;
+            if (count > 1 && splits > 1) {
+                for (int t = (steps_of(tile_end(s[k], a.group, BM, 0), STEP) + c - 1) / c; t < splits; ++t) {
+                    const int fewer = tiles_upto<BM, STEP>(s[k], a.group, count, t, c);
+                    items -= fewer;
+                    slots -= t == 1 ? 2 * fewer : fewer;
+                }
+            }
             const int upto = wave_scan(items), upto_slots = wave_scan(slots), upto_tiles = wave_scan(count);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             if (item < at + all) {
                 const int who = __builtin_ctzll(__ballot(item < at + upto));
-                const int local = item - at - __builtin_amdgcn_readlane(upto - items, who);
+                int local = item - at - __builtin_amdgcn_readlane(upto - items, who);
                 out->b = base + k * kWave + (k == 0 ? __builtin_amdgcn_readlane(who_is, who) : who);
-                out->splits = __builtin_amdgcn_readlane(splits, who);
+                out->slot = slot + __builtin_amdgcn_readlane(upto_slots - slots, who) + local;
                 out->seq.first = __builtin_amdgcn_readlane(s[k].first, who);
                 out->seq.n = __builtin_amdgcn_readlane(s[k].n, who);
                 out->seq.kv = __builtin_amdgcn_readlane(s[k].kv, who);
-                const int up = local / out->splits;
-                out->tile = tiles_of(out->seq.n, a.group, BM) - 1 - up;
-                out->split = local - up * out->splits;
-                out->slot = slot + __builtin_amdgcn_readlane(upto_slots - slots, who) + out->tile * out->splits;
+                // Tiles of most splits first, each one's splits together.
+                int t = __builtin_amdgcn_readlane(splits, who), upto_t = tiles_of(out->seq.n, a.group, BM);
+                for (;; --t) {
+                    const int upto_less = t > 1 ? tiles_upto<BM, STEP>(out->seq, a.group, upto_t, t - 1, c) : 0;
+                    if (local < (upto_t - upto_less) * t) break;
+                    local -= (upto_t - upto_less) * t;
+                    upto_t = upto_less;
+                }
+                const int up = local / t;
+                out->splits = t;
+                out->tile = upto_t - 1 - up;
+                out->split = local - up * t;
+                out->slot -= out->split;
                 out->ordinal = ordinal + __builtin_amdgcn_readlane(upto_tiles - count, who) + out->tile;
-                out->per_split = c;
                 return true;
             }
             at += all;
@@ -261,25 +279,41 @@ struct Piece {
     Sequence seq;
 };
 
-// Eight elements d .. d + 7 of a row's result: sums over l (0 for a row that
-// sees nothing; where every score that it sees is -inf, l is 0 and the result
-// NaN, as the softmax is), times the gate, rounded once.
-template <bool FP16>
-__device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
-                                           const float* v, float l) {
+// Eight gates d .. d + 7 of a row.
+__device__ __forceinline__ uint4 gate_of(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d) {
     const int i = row / a.group;
     const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
-    const float inv = seen_by(s, i) > 0 ? 1.0f / l : 0.0f;
+    return ldg16(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d);
+}
+// Eight elements d .. d + 7 of a row's result: x times the gate (when there
+// is one), rounded once.
+template <bool FP16>
+__device__ __forceinline__ void store_gated8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
+                                             const float* v, uint4 gate) {
+    const int i = row / a.group;
+    const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
     float x[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
+    for (int k = 0; k < 8; ++k) x[k] = v[k];
     if (a.gate != nullptr) {
         float g[8];
-        unpack16<FP16>(ldg16(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d), g);
+        unpack16<FP16>(gate, g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] *= sigmoid(g[k]);
     }
     *reinterpret_cast<uint4*>(a.out + t * a.out_token_stride + h * a.out_head_stride + d) = pack16<FP16>(x);
+}
+// The same of sums over l (0 for a row that sees nothing; where every score
+// that it sees is -inf, l is 0 and the result NaN, as the softmax is).
+template <bool FP16>
+__device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
+                                           const float* v, float l) {
+    const float inv = seen_by(s, row / a.group) > 0 ? 1.0f / l : 0.0f;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
+    store_gated8<FP16>(a, s, kh, row, d, x,
+                       a.gate == nullptr ? make_uint4(0u, 0u, 0u, 0u) : gate_of(a, s, kh, row, d));
 }
 
 // ---- the tile kernel --------------------------------------------------------------
@@ -520,8 +554,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         part.pieces[blockIdx.x].splits = 0;
     if (!live) return;
     const int end = tile_end(sp.seq, a.group, BM, sp.tile);
-    const int splits = tile_splits<STEP>(sp.splits, end, sp.per_split);
-    if (sp.split >= splits) return;
+    const int splits = sp.splits;
     const int row_at = sp.tile * BM;
     const int rows = min(BM, sp.seq.n * a.group - row_at);
     const int least_seen = seen_by(sp.seq, row_at / a.group);
@@ -845,27 +878,39 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         static_assert(32 * 32 * DBC * 4 * WQ <= LDS, "the rows fit");
         float4* mine_at = reinterpret_cast<float4*>(lds) + wave * 32 * CHUNKS;
         const float inv = seen > 0 ? 1.0f / l : 0.0f;
+        constexpr int PER = kWave / (CHUNKS / 2), ROUNDS = 32 / PER;   // rows at a time
+        const int c = lane % (CHUNKS / 2) * 2;
+        auto row_of = [&](int i) { return wq * 32 + i * PER + lane / (CHUNKS / 2); };
+        // The gates of all rows are requested before the first is used.
+        uint4 gates[DB / DBC][ROUNDS];
+        if (a.gate != nullptr) {
 #pragma unroll
-        for (int d0 = 0; d0 < DB; d0 += DBC) {
+            for (int i = 0; i < ROUNDS; ++i)
+#pragma unroll
+                for (int k = 0; k < DB / DBC; ++k)
+                    gates[k][i] = gate_of(a, sp.seq, kh, row_at + min(row_of(i), rows - 1), 32 * DBC * k + 4 * c);
+        }
+#pragma unroll
+        for (int k = 0; k < DB / DBC; ++k) {
             wave_lds_fence();
 #pragma unroll
             for (int db = 0; db < DBC; ++db)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int c = 8 * db + 2 * g + hi;
-                    mine_at[q * CHUNKS + (c ^ (q % CHUNKS))] =
-                        make_float4(o[d0 + db][4 * g] * inv, o[d0 + db][4 * g + 1] * inv, o[d0 + db][4 * g + 2] * inv,
-                                    o[d0 + db][4 * g + 3] * inv);
+                    const int at = 8 * db + 2 * g + hi;
+                    const f32x16& x = o[DBC * k + db];
+                    mine_at[q * CHUNKS + (at ^ (q % CHUNKS))] =
+                        make_float4(x[4 * g] * inv, x[4 * g + 1] * inv, x[4 * g + 2] * inv, x[4 * g + 3] * inv);
                 }
             wave_lds_fence();
-#pragma unroll 1
-            for (int i = lane; i < 32 * CHUNKS / 2; i += kWave) {
-                const int r = i / (CHUNKS / 2), c = i % (CHUNKS / 2) * 2;
-                if (wq * 32 + r >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < ROUNDS; ++i) {
+                const int r = row_of(i) - wq * 32;
                 const float4 x = mine_at[r * CHUNKS + (c ^ (r % CHUNKS))];
                 const float4 y = mine_at[r * CHUNKS + ((c + 1) ^ (r % CHUNKS))];
                 const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                store_row8<FP16>(a, sp.seq, kh, row_at + wq * 32 + r, 32 * d0 + 4 * c, v, 1.0f);
+                if (row_of(i) < rows)
+                    store_gated8<FP16>(a, sp.seq, kh, row_at + row_of(i), 32 * DBC * k + 4 * c, v, gates[k][i]);
             }
         }
     }
