@@ -830,6 +830,7 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     a.heads = p->heads;
     a.kv_heads = p->kv_heads;
     a.group = p->heads / p->kv_heads;
+    a.group_inverse = ((1 << 21) + a.group - 1) / a.group;
     a.pages = p->pages;
     a.page_shift = shift_of(p->page);
     a.max_pages = p->max_pages;

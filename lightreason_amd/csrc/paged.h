@@ -104,6 +104,7 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, bool fp16, int dim, hip
 
 struct PagedAttnArgs {
     int seqs, tokens, heads, kv_heads, group, pages, page_shift, max_pages;
+    int group_inverse;  // ceil(2^21 / group)
     float scale;  // of the scores, times log2(e): the softmax runs on powers of two
     const uint16_t *q, *gate, *k_cache, *v_cache;
     int64_t q_token_stride, q_head_stride, gate_token_stride, gate_head_stride;

@@ -39,7 +39,13 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __builtin_exp2f(-1.4426950408889634f * x)); }
+// By the exponential and reciprocal instructions, an ulp each (2^-23 of a
+// result that is rounded to 16 bits): the exact division and exponential take
+// some 40 instructions, which for the gates of 2048 positions of 16 heads of
+// 256 were more than the merge's memory time.
+__device__ __forceinline__ float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
 
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -52,7 +58,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 // tile holds values that are not finite and that some of its rows do not see
 // (in a tile's matrix product their zero weights would not hide them).
 template <bool FP16, int D>
-__device__ void attend_row(const PagedAttnArgs& a, int b, int t, int h, int64_t seen, float* qs, float* ps,
+__device__ void attend_row(const PagedAttnArgs& a, int b, int64_t t, int64_t h, int64_t seen, float* qs, float* ps,
                            int64_t* vs) {
     constexpr int E = D / kWave;
     const int lane = threadIdx.x % kWave;
@@ -279,19 +285,37 @@ struct Piece {
     Sequence seq;
 };
 
+// The rows of a tile: row r is that of token i and head j of the key/value
+// head's group, i and j the quotient and rest of first + r by the group.  That
+// is less than 1024 + 128, so its product with ceil(2^21 / group) holds the
+// quotient above bit 21: a division by a variable takes some 30 instructions.
+struct TileRows {
+    int token, head;   // of the step: those of i = 0 and j = 0
+    int first, seen;   // positions that token i = 0 sees (negative ones: none)
+};
+struct RowAt {
+    int64_t token, head;
+    int seen;
+};
+__device__ __forceinline__ TileRows rows_of(const PagedAttnArgs& a, const Sequence& s, int kh, int row_at) {
+    const int i = row_at / a.group;
+    return {s.first + i, kh * a.group, row_at - i * a.group, s.kv - s.n + i + 1};
+}
+__device__ __forceinline__ RowAt row_at_of(const PagedAttnArgs& a, const TileRows& t, int r) {
+    const uint32_t x = static_cast<uint32_t>(t.first + r);
+    const int i = static_cast<int>(__umul24(x, static_cast<uint32_t>(a.group_inverse)) >> 21);
+    return {t.token + i, t.head + static_cast<int>(x) - i * a.group, max(t.seen + i, 0)};
+}
+
 // Eight gates d .. d + 7 of a row.
-__device__ __forceinline__ uint4 gate_of(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d) {
-    const int i = row / a.group;
-    const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
-    return ldg16(a.gate + t * a.gate_token_stride + h * a.gate_head_stride + d);
+__device__ __forceinline__ uint4 gate_of(const PagedAttnArgs& a, const RowAt& r, int d) {
+    return ldg16(a.gate + r.token * a.gate_token_stride + r.head * a.gate_head_stride + d);
 }
 // Eight elements d .. d + 7 of a row's result: x times the gate (when there
 // is one), rounded once.
 template <bool FP16>
-__device__ __forceinline__ void store_gated8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
-                                             const float* v, uint4 gate) {
-    const int i = row / a.group;
-    const int64_t t = s.first + i, h = kh * a.group + row - i * a.group;
+__device__ __forceinline__ void store_gated8(const PagedAttnArgs& a, const RowAt& r, int d, const float* v,
+                                             uint4 gate) {
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = v[k];
@@ -301,19 +325,19 @@ __device__ __forceinline__ void store_gated8(const PagedAttnArgs& a, const Seque
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] *= sigmoid(g[k]);
     }
-    *reinterpret_cast<uint4*>(a.out + t * a.out_token_stride + h * a.out_head_stride + d) = pack16<FP16>(x);
+    *reinterpret_cast<uint4*>(a.out + r.token * a.out_token_stride + r.head * a.out_head_stride + d) =
+        pack16<FP16>(x);
 }
 // The same of sums over l (0 for a row that sees nothing; where every score
 // that it sees is -inf, l is 0 and the result NaN, as the softmax is).
 template <bool FP16>
-__device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const Sequence& s, int kh, int row, int d,
-                                           const float* v, float l) {
-    const float inv = seen_by(s, row / a.group) > 0 ? 1.0f / l : 0.0f;
+__device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const RowAt& r, int d, const float* v, float l) {
+    const uint4 gate = a.gate == nullptr ? make_uint4(0u, 0u, 0u, 0u) : gate_of(a, r, d);
+    const float inv = r.seen > 0 ? __builtin_amdgcn_rcpf(l) : 0.0f;
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
-    store_gated8<FP16>(a, s, kh, row, d, x,
-                       a.gate == nullptr ? make_uint4(0u, 0u, 0u, 0u) : gate_of(a, s, kh, row, d));
+    store_gated8<FP16>(a, r, d, x, gate);
 }
 
 // ---- the tile kernel --------------------------------------------------------------
@@ -557,7 +581,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int splits = sp.splits;
     const int row_at = sp.tile * BM;
     const int rows = min(BM, sp.seq.n * a.group - row_at);
-    const int least_seen = seen_by(sp.seq, row_at / a.group);
+    const TileRows places = rows_of(a, sp.seq, kh, row_at);
+    const int least_seen = max(places.seen, 0);
     const int steps_all = steps_of(end, STEP), share = (steps_all + splits - 1) / splits;
     const int k0 = sp.split * share * STEP;
     const int k1 = min(end, k0 + share * STEP);
@@ -631,11 +656,9 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     uint4 qf[KS];
     int seen;
     {
-        const int row = row_at + (my_row < rows ? my_row : 0);
-        const int i = row / a.group;
-        seen = my_row < rows ? seen_by(sp.seq, i) : 0;
-        const uint16_t* src = a.q + (sp.seq.first + i) * a.q_token_stride +
-                              (kh * a.group + row - i * a.group) * a.q_head_stride;
+        const RowAt r = row_at_of(a, places, my_row < rows ? my_row : 0);
+        seen = my_row < rows ? r.seen : 0;
+        const uint16_t* src = a.q + r.token * a.q_token_stride + r.head * a.q_head_stride;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[ks] = ldg16(src + 16 * ks + 8 * hi);
     }
@@ -855,7 +878,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                     *reinterpret_cast<float4*>(part.o + at * D + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
                     if (d == 0) *reinterpret_cast<float2*>(part.ml + 2 * at) = make_float2(rm, rl);
                 } else {
-                    store_row8<FP16>(a, sp.seq, kh, row_at + r0 + r, d, v, rl);
+                    store_row8<FP16>(a, row_at_of(a, places, r0 + r), d, v, rl);
                 }
             }
         }
@@ -877,18 +900,23 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         constexpr int CHUNKS = 8 * DBC;   // of four floats, per row
         static_assert(32 * 32 * DBC * 4 * WQ <= LDS, "the rows fit");
         float4* mine_at = reinterpret_cast<float4*>(lds) + wave * 32 * CHUNKS;
-        const float inv = seen > 0 ? 1.0f / l : 0.0f;
+        const float inv = seen > 0 ? __builtin_amdgcn_rcpf(l) : 0.0f;
         constexpr int PER = kWave / (CHUNKS / 2), ROUNDS = 32 / PER;   // rows at a time
         const int c = lane % (CHUNKS / 2) * 2;
         auto row_of = [&](int i) { return wq * 32 + i * PER + lane / (CHUNKS / 2); };
-        // The gates of all rows are requested before the first is used.
-        uint4 gates[DB / DBC][ROUNDS];
+        // All gates are requested in front of the first store: a load behind
+        // stores is waited for only when those have reached memory.  The loop
+        // below takes two rounds per pass and moves the rest of them down;
+        // unrolled it would take longer to fetch than to run.
+        constexpr int GATES = DB / DBC * ROUNDS;
+        uint4 gates[GATES] = {};
         if (a.gate != nullptr) {
 #pragma unroll
-            for (int i = 0; i < ROUNDS; ++i)
+            for (int i = 0; i < ROUNDS; ++i) {
+                const RowAt r = row_at_of(a, places, min(row_of(i), rows - 1));
 #pragma unroll
-                for (int k = 0; k < DB / DBC; ++k)
-                    gates[k][i] = gate_of(a, sp.seq, kh, row_at + min(row_of(i), rows - 1), 32 * DBC * k + 4 * c);
+                for (int k = 0; k < DB / DBC; ++k) gates[k * ROUNDS + i] = gate_of(a, r, 32 * DBC * k + 4 * c);
+            }
         }
 #pragma unroll
         for (int k = 0; k < DB / DBC; ++k) {
@@ -903,14 +931,19 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                         make_float4(x[4 * g] * inv, x[4 * g + 1] * inv, x[4 * g + 2] * inv, x[4 * g + 3] * inv);
                 }
             wave_lds_fence();
+#pragma unroll 1
+            for (int i = 0; i < ROUNDS; i += 2) {
 #pragma unroll
-            for (int i = 0; i < ROUNDS; ++i) {
-                const int r = row_of(i) - wq * 32;
-                const float4 x = mine_at[r * CHUNKS + (c ^ (r % CHUNKS))];
-                const float4 y = mine_at[r * CHUNKS + ((c + 1) ^ (r % CHUNKS))];
-                const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                if (row_of(i) < rows)
-                    store_gated8<FP16>(a, sp.seq, kh, row_at + row_of(i), 32 * DBC * k + 4 * c, v, gates[k][i]);
+                for (int j = 0; j < 2; ++j) {
+                    const int r = (i + j) * PER + lane / (CHUNKS / 2);
+                    const float4 x = mine_at[r * CHUNKS + (c ^ (r % CHUNKS))];
+                    const float4 y = mine_at[r * CHUNKS + ((c + 1) ^ (r % CHUNKS))];
+                    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    if (wq * 32 + r < rows)
+                        store_gated8<FP16>(a, row_at_of(a, places, wq * 32 + r), 32 * DBC * k + 4 * c, v, gates[j]);
+                }
+#pragma unroll
+                for (int j = 2; j < GATES; ++j) gates[j - 2] = gates[j];
             }
         }
     }
@@ -936,11 +969,11 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
     if (pc.splits == 1 && !any_dirty) return;
     const int kh = blockIdx.x % a.kv_heads, row_at = pc.tile * BM;
     const int rows = min(BM, pc.seq.n * a.group - row_at);
+    const TileRows places = rows_of(a, pc.seq, kh, row_at);
     if (any_dirty) {
         for (int r = blockIdx.y * WAVES + wave; r < rows; r += gridDim.y * WAVES) {
-            const int i = (row_at + r) / a.group;
-            attend_row<FP16, D>(a, pc.b, pc.seq.first + i, kh * a.group + row_at + r - i * a.group,
-                                seen_by(pc.seq, i), qs[wave], ps[wave], vs[wave]);
+            const RowAt at = row_at_of(a, places, r);
+            attend_row<FP16, D>(a, pc.b, at.token, at.head, at.seen, qs[wave], ps[wave], vs[wave]);
         }
         return;
     }
@@ -1003,7 +1036,7 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
                                                    __shfl_xor(give.z, 32), __shfl_xor(give.w, 32));
                     const float4 lo = hi ? got : keep, up = hi ? keep : got;
                     const float x[8] = {lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
-                    if (r < rows) store_row8<FP16>(a, pc.seq, kh, row_at + r, 32 * db + 8 * (g + hi), x, l);
+                    if (r < rows) store_row8<FP16>(a, row_at_of(a, places, r), 32 * db + 8 * (g + hi), x, l);
                 }
             }
         }
@@ -1063,7 +1096,7 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = __builtin_fmaf(f, qs[w][8 * lane + k], x[k]);
                 }
-                store_row8<FP16>(a, pc.seq, kh, row_at + r, 8 * lane, x, l);
+                store_row8<FP16>(a, row_at_of(a, places, r), 8 * lane, x, l);
             }
             __syncthreads();
         }
@@ -1077,14 +1110,15 @@ struct Shape {
 // them, four waves on positions of their own, many splits (64 sequences of
 // 200-16000 positions: 204 us with a target of 1024, 227 with 512, 252 with
 // 2048; a split may be one step, so that a single sequence spreads).  Else
-// tiles of 128 rows, two workgroups per CU: a target of 400 lets the splits,
-// whose counts are rounded up, still fit the 512 places in one go (2048
-// positions from an empty cache: 87 us, 101 with 256, 114 with 512), and
-// splits of at least 8 steps, whose partial rows cost about as much (16
-// verify blocks: 35.6 us, 39.4 with 16).
+// tiles of 128 rows, two workgroups per CU: a target of 256, which with a part
+// of a split per tile stays within the 512 places (16 verify blocks of 16:
+// 34.3 us, 35.0 with 320, 36.5 with 400, 37.0 with 192; 2048 positions from an
+// empty cache: 73.5, 73.4, 72.4, 78; 128, where the latter has no splits:
+// 45.7 and 88), and splits of at least 8 steps, whose partial rows cost about
+// as much (16 verify blocks: 35.6 us, 39.4 with 16).
 Shape shape_of(int group, int max_new, int dim) {
     if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 1024, 1};
-    return {128, dim == 256 ? 32 : 64, 400, 8};
+    return {128, dim == 256 ? 32 : 64, 256, 8};
 }
 
 struct Layout {
