@@ -432,6 +432,10 @@ def paged_layer(attn, hidden: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor
     from .attention import HEAD_DIM, HEADS, HIDDEN, KV_HEADS
 
     N = plan.tokens
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dim() != 4 or t.shape[0] != pages.pages or t.shape[2] != pages.page:
+            raise ValueError(f"{name} must be [{pages.pages}, {KV_HEADS}, {pages.page}, {HEAD_DIM}] as the pool's, got "
+                             f"{tuple(t.shape)}")
     _require(hidden, "hidden", (torch.bfloat16,), (N, HIDDEN), attn.device)
     q_gate = torch.nn.functional.linear(hidden, attn.q_proj).view(N, HEADS, 2 * HEAD_DIM)
     k = torch.nn.functional.linear(hidden, attn.k_proj).view(N, KV_HEADS, HEAD_DIM)

@@ -330,6 +330,14 @@ def test_attention_long(device, seqs, layout):
     _check(c, *rest, _run_attention(c, max_new=max(n for _, n in seqs)))
 
 
+@pytest.mark.parametrize("seqs,layout,dtype", [([(2500, 2500), (1, 1), (700, 690)], (16, 2, 256), BF),
+                                               ([(1900, 1900)], (7, 1, 128), HF), ([(5, 5), (4100, 1500)], (96, 2, 64), BF)])
+def test_attention_prompts_of_many_split_counts(device, seqs, layout, dtype):
+    # Tiles of one sequence with one split and with several.
+    c, *rest = _case(device, *layout, 32, seqs, dtype, seed=23, gate=True, pad=1)
+    _check(c, *rest, _run_attention(c, max_new=max(n for _, n in seqs)))
+
+
 def test_attention_many_rows(device):
     rng = random.Random(5)
     seqs = [(rng.randint(1, 60), 1) if rng.random() < 0.8 else (rng.randint(0, 9), 0) for _ in range(1500)]

@@ -97,6 +97,17 @@ def test_strides_are_checked():
     paged._strided(torch.zeros(1, 3, 65, dtype=BF)[:, :1, :64], "x", 8)
 
 
+def test_layer_refuses_caches_of_another_pool():
+    pt = paged.PageTable(2, 4, 16, device="cpu")
+    plan, hidden = pt.new_plan(3), torch.zeros(3, 2048, dtype=BF)
+    for pages, page in ((5, 16), (4, 32)):
+        other = _cache(pages=pages, page=page, dim=256)
+        with pytest.raises(ValueError, match="pool"):
+            paged.paged_layer(None, hidden, None, None, other, _cache(dim=256), pt, plan)
+        with pytest.raises(ValueError, match="pool"):
+            paged.paged_layer(None, hidden, None, None, _cache(dim=256), other, pt, plan)
+
+
 def test_verify_refuses():
     tokens = torch.zeros(4, dtype=torch.int64)
     p = torch.zeros(4, 10)
