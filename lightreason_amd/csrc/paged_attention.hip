@@ -31,7 +31,7 @@
 // (keys, softmax, values) is longer than two waves per SIMD cover and the
 // partial rows' 33 MB leave at the end, 13 of their merge.  One decode
 // position for each of 64 sequences of 200-16000 takes 203 us, 5.4 TB/s of
-// keys and values, the rate of a large copy.  One sequence of 1000 takes 14.5
+// keys and values, the rate of a large copy.  One sequence of 1000 takes 13.9
 // us, a chain of reads (lengths, table, rows, partial rows) in two launches.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
@@ -174,10 +174,10 @@ __device__ __forceinline__ int tiles_upto(const Sequence& s, int group, int coun
 // The sequence, tile and split of item `item` (wave-uniform), heavy tiles
 // first, and how many tiles there are; false past the last item, and for
 // starts that are not ascending within [0, tokens] (such a step is empty).
-template <int BM, int STEP>
+// HELD: sequences per lane that stay in registers.
+template <int BM, int STEP, int HELD>
 __device__ __forceinline__ bool find_split(const PagedAttnArgs& a, int item, int target, int least, Split* out,
                                            int* all_tiles) {
-    constexpr int HELD = 4;   // sequences per lane that stay in registers
     const int lane = threadIdx.x % kWave;
     const int64_t capacity = static_cast<int64_t>(a.max_pages) << a.page_shift;
     Sequence s[HELD];
@@ -576,7 +576,11 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     const int item = blockIdx.x / a.kv_heads, kh = blockIdx.x % a.kv_heads;
     Split sp;
     int all_tiles;
-    const bool live = find_split<BM, STEP>(a, item, target, least, &sp, &all_tiles);
+    // (A path of its own for up to 64 sequences where latency counts: one
+    // sequence of 1000 positions 14.3 -> 13.9 us; in the kernel of longer tiles
+    // it gained nothing.)
+    const bool live = WK > 1 && a.seqs <= kWave ? find_split<BM, STEP, 1>(a, item, target, least, &sp, &all_tiles)
+                                                : find_split<BM, STEP, 4>(a, item, target, least, &sp, &all_tiles);
     if (threadIdx.x == 0 && item >= all_tiles && static_cast<int>(blockIdx.x) < part.tiles)
         part.pieces[blockIdx.x].splits = 0;
     if (!live) return;
