@@ -591,7 +591,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * least every n, else the call is slower.  out must not overlap q or gate.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
  * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
- * bytes (about 210 MB at most for width 256, far less for short steps),
+ * bytes (at most 160 MB for width 256 and 16 key/value heads, 40 MB and less
+ * for a decode step of a few heads),
  * 256-byte aligned, not cleared, used by one stream at a time. */
 typedef struct lrmoe_paged_attention_args {
     int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */
