@@ -583,17 +583,17 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
  * when a gate is given; softmax and sums in fp32.  A row that sees nothing
  * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
- * row does not see cannot change it, infinities and NaN included.  Tokens outside starts[0] .. starts[seqs] - 1
- * are left as they were, and all are when starts are not ascending within
- * [0, tokens].  A table entry outside [0, pages) in use makes its sequence's
+ * row does not see cannot change it, infinities and NaN included.  Tokens
+ * outside starts[0] .. starts[seqs] - 1 are left as they were, and all are
+ * when starts are not ascending within [0, tokens].  A table entry outside [0, pages) in use makes its sequence's
  * rows NaN (those of earlier positions may keep their values); kv_lengths
  * beyond max_pages pages are cut there.  max_new only chooses the kernel: at
  * least every n, else the call is slower.  out must not overlap q or gate.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
  * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
  * bytes (at most 160 MB for width 256 and 16 key/value heads, 40 MB and less
- * for a decode step of a few heads),
- * 256-byte aligned, not cleared, used by one stream at a time. */
+ * for a decode step of a few heads), 256-byte aligned, not cleared, used by
+ * one stream at a time. */
 typedef struct lrmoe_paged_attention_args {
     int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */
     int32_t pages, page, max_pages, fp16;
