@@ -585,10 +585,11 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
  * row does not see cannot change it, infinities and NaN included.  Tokens
  * outside starts[0] .. starts[seqs] - 1 are left as they were, and all are
- * when starts are not ascending within [0, tokens].  A table entry outside [0, pages) in use makes its sequence's
- * rows NaN (those of earlier positions may keep their values); kv_lengths
- * beyond max_pages pages are cut there.  max_new only chooses the kernel: at
- * least every n, else the call is slower.  out must not overlap q or gate.
+ * when starts are not ascending within [0, tokens].  A table entry outside
+ * [0, pages) in use makes its sequence's rows NaN (those of earlier positions
+ * may keep their values); kv_lengths beyond max_pages pages are cut there.
+ * max_new only chooses the kernel: at least every n, else the call is slower.
+ * out must not overlap q or gate.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
  * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
  * bytes (at most 160 MB for width 256 and 16 key/value heads, 40 MB and less
