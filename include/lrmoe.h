@@ -506,7 +506,7 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
  * the device and owned by the caller: table [rows][max_pages] int32 (a row's
  * pages in order), held [rows] int32 (pages of each row), lengths [rows] int32
  * (cached positions), free_pages [pages] int32 (a stack), state [4] int32 =
- * (free pages, epoch, status bits, 0).  A slot is page * page_size + row in the
+ * (free pages, epoch, status bits, plans made in this epoch).  A slot is page * page_size + row in the
  * page.  No reference counterpart: the reference serves one sequence on the
  * Transformers cache. */
 #define LRMOE_PAGE_MAX_ROWS 4096
@@ -514,7 +514,7 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
 #define LRMOE_PAGE_STATUS_TOKENS 1  /* a negative count, or more new positions than `tokens` */
 #define LRMOE_PAGE_STATUS_ROW 2     /* a row's length or pages past max_pages, or negative */
 #define LRMOE_PAGE_STATUS_POOL 4    /* not enough free pages (or a stack that does not fit `pages`) */
-#define LRMOE_PAGE_STATUS_STALE 8   /* a commit of a plan that another commit or release came after */
+#define LRMOE_PAGE_STATUS_STALE 8   /* a commit of a plan that another plan, commit or release came after */
 
 /* The page plan of a step in which row r gets new_tokens[r] positions after
  * its lengths[r]: starts [rows + 1] (row r's positions are starts[r] ..
@@ -523,11 +523,15 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
  * [tokens] int64 of the step's positions (0 and -1 past the last), and the
  * table entries of the fresh pages, which are taken from the top of the free
  * stack, rows in order; info [4] int32 = (status bits, positions, fresh
- * pages, the state's epoch).  Nothing else of the pool changes until the
- * commit: a plan can be made again.  All or nothing: with any status bit set
- * the step is empty (starts all 0, slots all -1, kv_lengths = lengths). */
+ * pages, the plan's number).  Of the rest of the pool only state[3], from
+ * which the number comes, changes until the commit: a plan can be made again.
+ * Each one writes the same table entries, so the last one made is the one that
+ * counts: kernels of an earlier plan's step run before the next plan is made,
+ * and its commit is refused.  All or nothing: with any status bit set the step
+ * is empty (starts all 0, slots all -1, kv_lengths = lengths), the table is
+ * untouched and the plan before it still counts. */
 int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, const int32_t *new_tokens,
-                    const int32_t *lengths, const int32_t *held, const int32_t *free_pages, const int32_t *state,
+                    const int32_t *lengths, const int32_t *held, const int32_t *free_pages, int32_t *state,
                     int32_t *table, int32_t *starts, int32_t *kv_lengths, int32_t *held_out, int32_t *positions,
                     int64_t *slots, int32_t *info, void *stream);
 
@@ -535,8 +539,10 @@ int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, co
  * kv_lengths; with accepted [rows] given (drafts that stand, as
  * lrmoe_verify_drafts writes them) a row with n > 0 new positions grows by
  * min(accepted + 1, n) instead (its further pages stay held).  The epoch goes
- * up by one.  A plan with a status bit, or one whose epoch is not the
- * state's, changes nothing but state's status bits. */
+ * up by one.  A plan with a status bit, or one that is not the last made since
+ * the pool changed (outputs that no plan was made into among them), changes
+ * nothing but state's status bits.  Outputs of another pool's plan are not
+ * told apart: the caller keeps them with their pool. */
 int lrmoe_page_commit(int rows, const int32_t *starts, const int32_t *kv_lengths, const int32_t *held_new,
                       const int32_t *info, const int32_t *accepted, int32_t *lengths, int32_t *held, int32_t *state,
                       void *stream);

@@ -117,7 +117,7 @@ PAGE_MAX_POSITIONS = 1 << 30  # max_pages * page at most
 PAGE_STATUS_TOKENS = 1   # a negative count, or more new positions than the plan has room for
 PAGE_STATUS_ROW = 2      # a row past its pages, or corrupt
 PAGE_STATUS_POOL = 4     # not enough free pages
-PAGE_STATUS_STALE = 8    # a plan committed after another commit or release
+PAGE_STATUS_STALE = 8    # a plan committed after another plan, commit or release
 
 STAGE_ROUTE = 1
 STAGE_GATE_UP = 2

@@ -691,7 +691,7 @@ static bool bad_capacity(int max_pages, int page) {
 static int shift_of(int page) { return __builtin_ctz(static_cast<unsigned>(page)); }
 
 int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, const int32_t* new_tokens,
-                    const int32_t* lengths, const int32_t* held, const int32_t* free_pages, const int32_t* state,
+                    const int32_t* lengths, const int32_t* held, const int32_t* free_pages, int32_t* state,
                     int32_t* table, int32_t* starts, int32_t* kv_lengths, int32_t* held_out, int32_t* positions,
                     int64_t* slots, int32_t* info, void* stream) {
     if (bad_pool(rows, pages, max_pages) || bad_page(page) || tokens < 0 || tokens > (1 << 24) ||

@@ -68,8 +68,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 struct PagePlanArgs {
     int rows, pages, page_shift, max_pages, tokens;
-    const int32_t *new_tokens, *lengths, *held, *free_pages, *state;
-    int32_t *table, *starts, *kv_lengths, *held_out, *positions, *info;
+    const int32_t *new_tokens, *lengths, *held, *free_pages;
+    int32_t *state, *table, *starts, *kv_lengths, *held_out, *positions, *info;
     int64_t* slots;
 };
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t stream);

@@ -7,9 +7,10 @@
 // rows of up to 65 new positions).  Every workgroup scans
 // the per-row counts itself (4096 rows are 16 per thread) instead of handing
 // the scan on through memory, so one launch does the whole plan and no
-// workgroup waits for another.  The plan changes nothing of the pool: it
-// writes its own outputs and table entries past the rows' held pages, which
-// nobody reads before the commit.
+// workgroup waits for another.  The plan changes nothing that rows hold: it
+// writes its own outputs, its number, and table entries past the rows' held
+// pages.  Those are read by the step's attention and kept by its commit, so
+// only the plan that wrote them last can be committed.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
@@ -66,6 +67,14 @@ __device__ __forceinline__ int last_at_most(const int* from, int n, int x) {
     return lo;
 }
 
+// The number of the made-th plan (from 1 on) between two changes of the pool.
+// Two of them are equal only where the epochs' difference times the counts' is
+// about 2^31 or more (the factor is 2^32 over the golden ratio, whose multiples
+// keep apart).
+__device__ __forceinline__ int plan_number(int epoch, int made) {
+    return static_cast<int>(static_cast<uint32_t>(epoch) * 0x9e3779b1u + static_cast<uint32_t>(made));
+}
+
 __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
     __shared__ int starts[kPageMaxRows + 1];
     __shared__ int before[kPageMaxRows];
@@ -79,6 +88,8 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
     const int64_t row_limit = static_cast<int64_t>(a.max_pages) << a.page_shift;
     if (tid == 0) status = 0;
     const int count = a.state[0], epoch = a.state[1];
+    // (state[3] is the first workgroup's alone: it changes the word below.)
+    const int made = blockIdx.x == 0 && tid == 0 ? a.state[3] : 0;
     struct Row {
         int n, len, held;
     };
@@ -143,7 +154,10 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
             a.info[0] = refuse;
             a.info[1] = live;
             a.info[2] = taken;
-            a.info[3] = epoch;
+            // A refused plan writes no table entries and replaces no other.
+            const int number = static_cast<int>(static_cast<uint32_t>(made) + (ok ? 1u : 0u));
+            a.info[3] = plan_number(epoch, number);
+            if (ok) a.state[3] = number;
         }
     }
     __syncthreads();
@@ -169,8 +183,10 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
 }
 
 __global__ __launch_bounds__(kThreads) void page_commit_kernel(PageCommitArgs a) {
-    const int refuse = a.info[0] | (a.info[3] != a.state[1] ? kPageStatusStale : 0);
-    const int count = a.state[0], epoch = a.state[1], status = a.state[2];
+    const int count = a.state[0], epoch = a.state[1], status = a.state[2], made = a.state[3];
+    int refuse = a.info[0];
+    // Not the last plan made, or none at all since the pool changed.
+    if (a.info[3] != plan_number(epoch, made) || (refuse == 0 && made == 0)) refuse |= kPageStatusStale;
     __syncthreads();  // every thread has read the state that thread 0 changes
     if (refuse == 0) {
         for (int r = threadIdx.x; r < a.rows; r += kThreads) {
@@ -187,6 +203,7 @@ __global__ __launch_bounds__(kThreads) void page_commit_kernel(PageCommitArgs a)
         if (refuse == 0) {
             a.state[0] = count - a.info[2];
             a.state[1] = epoch + 1;
+            a.state[3] = 0;
         }
         a.state[2] = status | refuse;
     }
@@ -226,6 +243,7 @@ __global__ __launch_bounds__(kThreads) void page_release_kernel(PageReleaseArgs 
         if (ok) {
             a.state[0] = count + total;
             a.state[1] += 1;
+            a.state[3] = 0;
         } else {
             a.state[2] |= kPageStatusPool;
         }

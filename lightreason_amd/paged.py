@@ -27,7 +27,7 @@ is no CPU path: the calls raise when liblrmoe.so is missing.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -94,19 +94,22 @@ class PagePlan:
     held: torch.Tensor          # [rows] int32: pages then
     positions: torch.Tensor     # [tokens] int32
     slots: torch.Tensor         # [tokens] int64: page * page_size + offset
-    info: torch.Tensor          # [4] int32: status bits, positions, fresh pages, epoch
+    info: torch.Tensor          # [4] int32: status bits, positions, fresh pages, number
+    pool: "PageTable | None" = field(default=None, repr=False, compare=False)
 
 
 class PageTable:
     """``pages`` pages of ``page`` positions shared by ``rows`` sequences of at
     most ``max_pages`` pages each (no more than 2^30 positions).  ``table``
     [rows, max_pages], ``held`` and ``lengths`` [rows], ``free_pages`` [pages]
-    and ``state`` [4] (free pages, epoch, status bits, 0) are int32 device
-    tensors.
+    and ``state`` [4] (free pages, epoch, status bits, plans made in this
+    epoch) are int32 device tensors.
 
     A step is ``plan`` -> its kernels -> ``commit``.  A plan changes nothing
-    that counts until it is committed, so it may be made again; a plan made
-    before another commit or release is refused (status)."""
+    that rows hold until it is committed, so it may be made again, but every
+    plan writes its fresh pages into ``table``: the last one made is the one
+    whose kernels and commit may follow.  An earlier one, and one from before
+    another commit or release, is refused at its commit (status)."""
 
     def __init__(self, rows: int, pages: int, page: int, *, max_pages: int | None = None, device="cuda"):
         self.rows = _int(rows, "rows", 1, _native.PAGE_MAX_ROWS)
@@ -136,7 +139,7 @@ class PageTable:
         i32 = dict(dtype=torch.int32, device=self.device)
         return PagePlan(tokens, torch.zeros(self.rows + 1, **i32), torch.zeros(self.rows, **i32),
                         torch.zeros(self.rows, **i32), torch.zeros(tokens, **i32),
-                        torch.full((tokens,), -1, dtype=torch.int64, device=self.device), torch.zeros(4, **i32))
+                        torch.full((tokens,), -1, dtype=torch.int64, device=self.device), torch.zeros(4, **i32), self)
 
     def plan(self, new_tokens: torch.Tensor, tokens: int, *, out: PagePlan | None = None) -> PagePlan:
         """The plan of a step in which row r gets ``new_tokens[r]`` positions
@@ -145,11 +148,13 @@ class PageTable:
         from the top of the free stack, rows in order.  A step that does not
         fit is refused as a whole: its ``info[0]`` holds the status bits, its
         starts are all 0, and nothing it feeds writes anything."""
+        if out is not None and (out.pool not in (None, self) or out.tokens != tokens
+                                or out.starts.shape[0] != self.rows + 1 or out.starts.device != self.device):
+            raise ValueError(f"out must be a plan of this pool for {tokens} positions")
         _require(new_tokens, "new_tokens", (torch.int32,), (self.rows,), self.device)
         if out is None:
             out = self.new_plan(tokens)
-        elif out.tokens != tokens or out.starts.shape[0] != self.rows + 1 or out.starts.device != self.device:
-            raise ValueError(f"out must be a plan of this pool for {tokens} positions")
+        out.pool = self
         with _on(self.device):
             _native.call("lrmoe_page_plan", self.rows, self.pages, self.page, self.max_pages, tokens,
                          new_tokens.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(),
@@ -166,7 +171,7 @@ class PageTable:
         next step).  A refused or stale plan changes only the status."""
         if accepted is not None:
             _require(accepted, "accepted", (torch.int32,), (self.rows,), self.device)
-        if plan.starts.shape[0] != self.rows + 1 or plan.starts.device != self.device:
+        if plan.pool is not self:
             raise ValueError("the plan is not of this pool")
         with _on(self.device):
             _native.call("lrmoe_page_commit", self.rows, plan.starts.data_ptr(), plan.kv_lengths.data_ptr(),
@@ -192,7 +197,8 @@ class PageTable:
         texts = [text for bit, text in ((_native.PAGE_STATUS_TOKENS, "more new positions than the step has room for"),
                                         (_native.PAGE_STATUS_ROW, "a row longer than its pages, or a bad length"),
                                         (_native.PAGE_STATUS_POOL, "the pool is out of pages"),
-                                        (_native.PAGE_STATUS_STALE, "a plan older than the pool was committed"))
+                                        (_native.PAGE_STATUS_STALE, "a plan older than the pool, or than another plan, "
+                                                                    "was committed"))
                  if bits & bit]
         if texts:
             raise RuntimeError(f"{what}: " + "; ".join(texts))
@@ -432,6 +438,8 @@ def paged_layer(attn, hidden: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor
     from .attention import HEAD_DIM, HEADS, HIDDEN, KV_HEADS
 
     N = plan.tokens
+    if plan.pool is not pages:
+        raise ValueError("the plan is not of this pool")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if t.dim() != 4 or t.shape[0] != pages.pages or t.shape[2] != pages.page:
             raise ValueError(f"{name} must be [{pages.pages}, {KV_HEADS}, {pages.page}, {HEAD_DIM}] as the pool's, got "
