@@ -512,7 +512,7 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
 #define LRMOE_PAGE_MAX_ROWS 4096
 #define LRMOE_PAGE_MAX_POSITIONS (1 << 30) /* most of max_pages * page: positions that a row can hold */
 #define LRMOE_PAGE_STATUS_TOKENS 1  /* a negative count, or more new positions than `tokens` */
-#define LRMOE_PAGE_STATUS_ROW 2     /* a row's length or pages past max_pages, or negative */
+#define LRMOE_PAGE_STATUS_ROW 2     /* a row's length past its held pages, either past max_pages, or negative */
 #define LRMOE_PAGE_STATUS_POOL 4    /* not enough free pages (or a stack that does not fit `pages`) */
 #define LRMOE_PAGE_STATUS_STALE 8   /* a commit of a plan that another plan, commit or release came after */
 

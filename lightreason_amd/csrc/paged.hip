@@ -118,7 +118,8 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
     float size = 0.0f;
     each([&](int, const Row& x) {
         if (x.n < 0) bad |= kPageStatusTokens;
-        if (x.len < 0 || x.held < 0 || x.held > a.max_pages || static_cast<int64_t>(x.len) + x.n > row_limit)
+        if (x.len < 0 || x.held < 0 || x.held > a.max_pages || static_cast<int64_t>(x.len) + x.n > row_limit ||
+            x.len > static_cast<int64_t>(x.held) << a.page_shift)
             bad |= kPageStatusRow;
         tokens += x.n;
         fresh += max(need_of(x) - x.held, 0);
@@ -128,7 +129,8 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(PagePlanArgs a) {
     if (bad) atomicOr(&status, bad);
     __syncthreads();
     int refuse = status;
-    // (fresh pages are fewer than the new positions where nothing else is wrong)
+    // (a row's fresh pages are no more than its new positions where nothing
+    // else is wrong: its length lies within the pages that it holds)
     if (pre.huge || pre.total_a > a.tokens) refuse |= kPageStatusTokens;
     if ((refuse == 0 && pre.total_b > count) || count > a.pages) refuse |= kPageStatusPool;
     const bool ok = refuse == 0;

@@ -1,5 +1,5 @@
 """The page pool under calls that its documentation allows: plans that replace
-each other, and plans of other pools."""
+each other, plans of other pools, and rows whose lengths do not fit their pages."""
 
 from __future__ import annotations
 
@@ -101,3 +101,25 @@ def test_captured_plans_number_themselves(device):
         lengths = [a + b for a, b in zip(lengths, step)]
         assert pt.lengths.tolist() == lengths and pt.state[2].item() == 8 and _whole(pt)
         pt.state[2] = 0
+
+
+def test_rows_longer_than_their_pages_are_refused(device):
+    from lightreason_amd.paged import PageTable
+
+    pt = PageTable(3, 30, 16, device=device)
+    pt.commit(pt.plan(_ints([40, 16, 0], device), 56))
+    for lengths, ok in (([48, 16, 0], True), ([49, 16, 0], False), ([40, 17, 0], False), ([40, 16, 1], False)):
+        pt.lengths.copy_(_ints(lengths, device))
+        plan = pt.plan(_ints([0, 0, 1], device), 4)
+        assert plan.info.tolist()[:3] == ([0, 1, 1] if ok else [2, 0, 0])
+
+
+def test_long_rows_without_pages_do_not_wrap_the_count(device):
+    # 16 rows of 2^30 positions on pages of 8: their missing pages, 2^31, pass 31 bits.
+    from lightreason_amd.paged import PageTable
+
+    pt = PageTable(17, 30, 8, max_pages=4, device=device)
+    pt.max_pages = 1 << 27   # what the rows may hold; nothing is read past the pages that a row has
+    pt.lengths[:16] = 1 << 30
+    plan = pt.plan(_ints([0] * 16 + [1], device), 4)
+    assert plan.info.tolist()[:3] == [2, 0, 0] and set(plan.slots.tolist()) == {-1}
