@@ -547,6 +547,17 @@ int lrmoe_page_commit(int rows, const int32_t *starts, const int32_t *kv_lengths
                       const int32_t *info, const int32_t *accepted, int32_t *lengths, int32_t *held, int32_t *state,
                       void *stream);
 
+/* The commit of a step that also holds prompts: block_starts [rows + 1] are the
+ * starts that lrmoe_verify_drafts took, of blocks whose rows are the last
+ * positions of each row that have probabilities: all of a verify block's, the
+ * last one of a prompt's, none of a chunk's whose prompt goes on.  Only a
+ * block's rows after its first are drafts, so a row with n > 0 new positions
+ * grows by n less the drafts that fell, n - max(block, 1) + accepted + 1 kept
+ * within 1 .. n.  With block_starts = starts it is lrmoe_page_commit. */
+int lrmoe_page_commit_drafts(int rows, const int32_t *starts, const int32_t *kv_lengths, const int32_t *held_new,
+                             const int32_t *info, const int32_t *accepted, const int32_t *block_starts,
+                             int32_t *lengths, int32_t *held, int32_t *state, void *stream);
+
 /* Returns the pages of the rows with mask[r] != 0 (uint8) to the free stack
  * and empties those rows (length and held 0).  The epoch goes up by one. */
 int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t *mask, const int32_t *table,

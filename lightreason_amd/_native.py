@@ -75,6 +75,7 @@ _SIGNATURES = {
                                 _P, _P, _P, _P, _P, C.c_size_t, _P], _I),
     "lrmoe_page_plan": ([_I] * 5 + [_P] * 13, _I),
     "lrmoe_page_commit": ([_I] + [_P] * 9, _I),
+    "lrmoe_page_commit_drafts": ([_I] + [_P] * 10, _I),
     "lrmoe_page_release": ([_I] * 3 + [_P] * 7, _I),
     "lrmoe_paged_append": ([_P, _P], _I),
     "lrmoe_paged_attention_workspace_bytes": ([_P], C.c_size_t),

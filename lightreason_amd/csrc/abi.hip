@@ -707,15 +707,28 @@ int lrmoe_page_plan(int rows, int pages, int page, int max_pages, int tokens, co
     return status_of(lrmoe::launch_page_plan(a, as_stream(stream)));
 }
 
-int lrmoe_page_commit(int rows, const int32_t* starts, const int32_t* kv_lengths, const int32_t* held_new,
-                      const int32_t* info, const int32_t* accepted, int32_t* lengths, int32_t* held, int32_t* state,
-                      void* stream) {
+static int page_commit(int rows, const int32_t* starts, const int32_t* kv_lengths, const int32_t* held_new,
+                       const int32_t* info, const int32_t* accepted, const int32_t* block_starts, int32_t* lengths,
+                       int32_t* held, int32_t* state, void* stream) {
     if (rows < 0 || rows > LRMOE_PAGE_MAX_ROWS) return LRMOE_E_ARG;
     if (rows == 0) return LRMOE_OK;
     if (!starts || !kv_lengths || !held_new || !info || !lengths || !held || !state) return LRMOE_E_ARG;
     if (int d = check_device()) return d;
-    lrmoe::PageCommitArgs a{rows, starts, kv_lengths, held_new, info, accepted, lengths, held, state};
+    lrmoe::PageCommitArgs a{rows, starts, kv_lengths, held_new, info, accepted, block_starts, lengths, held, state};
     return status_of(lrmoe::launch_page_commit(a, as_stream(stream)));
+}
+
+int lrmoe_page_commit(int rows, const int32_t* starts, const int32_t* kv_lengths, const int32_t* held_new,
+                      const int32_t* info, const int32_t* accepted, int32_t* lengths, int32_t* held, int32_t* state,
+                      void* stream) {
+    return page_commit(rows, starts, kv_lengths, held_new, info, accepted, nullptr, lengths, held, state, stream);
+}
+
+int lrmoe_page_commit_drafts(int rows, const int32_t* starts, const int32_t* kv_lengths, const int32_t* held_new,
+                             const int32_t* info, const int32_t* accepted, const int32_t* block_starts,
+                             int32_t* lengths, int32_t* held, int32_t* state, void* stream) {
+    if (rows > 0 && (!accepted || !block_starts)) return LRMOE_E_ARG;
+    return page_commit(rows, starts, kv_lengths, held_new, info, accepted, block_starts, lengths, held, state, stream);
 }
 
 int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t* mask, const int32_t* table,

@@ -76,7 +76,7 @@ hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t stream);
 
 struct PageCommitArgs {
     int rows;
-    const int32_t *starts, *kv_lengths, *held_new, *info, *accepted;
+    const int32_t *starts, *kv_lengths, *held_new, *info, *accepted, *block_starts;
     int32_t *lengths, *held, *state;
 };
 hipError_t launch_page_commit(const PageCommitArgs& a, hipStream_t stream);

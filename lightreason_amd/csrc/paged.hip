@@ -196,7 +196,13 @@ __global__ __launch_bounds__(kThreads) void page_commit_kernel(PageCommitArgs a)
             if (a.accepted == nullptr) {
                 a.lengths[r] = a.kv_lengths[r];
             } else if (n > 0) {
-                a.lengths[r] += min(max(a.accepted[r], 0) + 1, n);
+                // The first row of a verified block is no draft, and positions
+                // of the step that the block has no row for are none either.
+                const int64_t block = a.block_starts == nullptr
+                                          ? n
+                                          : static_cast<int64_t>(a.block_starts[r + 1]) - a.block_starts[r];
+                const int64_t grown = n - max(block, INT64_C(1)) + max(a.accepted[r], 0) + 1;
+                a.lengths[r] += static_cast<int>(min(max(grown, INT64_C(1)), static_cast<int64_t>(n)));
             }
             a.held[r] = a.held_new[r];
         }

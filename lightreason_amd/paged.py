@@ -163,20 +163,34 @@ class PageTable:
                          out.positions.data_ptr(), out.slots.data_ptr(), out.info.data_ptr(), _stream(self.device))
         return out
 
-    def commit(self, plan: PagePlan, accepted: torch.Tensor | None = None) -> None:
+    def commit(self, plan: PagePlan, accepted: torch.Tensor | None = None, *,
+               starts: torch.Tensor | None = None) -> None:
         """Take a plan into the pool: lengths = plan.kv_lengths, or, with
         ``accepted`` ([rows] int32, from ``verify.verify_drafts``), lengths
         grown by accepted + 1 per row that took part (the last committed token
         and the drafts that stand; the rest of the block is overwritten by the
-        next step).  A refused or stale plan changes only the status."""
+        next step).  A refused or stale plan changes only the status.
+
+        A step that holds prompts too is verified over blocks of its own,
+        ``starts`` [rows + 1] int32 (those that ``verify_drafts`` took): every
+        position of a verify block, the last one of a prompt, none of a chunk
+        whose prompt goes on.  Give them here as well: only the drafts of a
+        block, its rows after the first, can fall; every other position
+        stays."""
         if accepted is not None:
             _require(accepted, "accepted", (torch.int32,), (self.rows,), self.device)
         if plan.pool is not self:
             raise ValueError("the plan is not of this pool")
+        name, blocks = "lrmoe_page_commit", ()
+        if starts is not None:
+            if accepted is None:
+                raise ValueError("starts come with accepted")
+            _require(starts, "starts", (torch.int32,), (self.rows + 1,), self.device)
+            name, blocks = "lrmoe_page_commit_drafts", (starts.data_ptr(),)
         with _on(self.device):
-            _native.call("lrmoe_page_commit", self.rows, plan.starts.data_ptr(), plan.kv_lengths.data_ptr(),
-                         plan.held.data_ptr(), plan.info.data_ptr(), _ptr(accepted), self.lengths.data_ptr(),
-                         self.held.data_ptr(), self.state.data_ptr(), _stream(self.device))
+            _native.call(name, self.rows, plan.starts.data_ptr(), plan.kv_lengths.data_ptr(), plan.held.data_ptr(),
+                         plan.info.data_ptr(), _ptr(accepted), *blocks, self.lengths.data_ptr(), self.held.data_ptr(),
+                         self.state.data_ptr(), _stream(self.device))
 
     def release(self, mask: torch.Tensor) -> None:
         """Return the pages of the rows with mask[r] ([rows] bool or uint8 on

@@ -145,7 +145,7 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
 
     ``tokens`` [rows] int64 are the fed tokens of every block, the last
     committed one first, then its drafts; ``starts`` [blocks + 1] int32 the
-    blocks' first rows (a ``paged.PagePlan``'s); ``target`` [rows, vocab] the
+    blocks' first rows (a ``paged.PagePlan``'s, or a caller's own); ``target`` [rows, vocab] the
     target's probabilities after each fed token, ``draft`` [rows, vocab] the
     drafter's of the same positions (fp32, bf16 or fp16; None for a drafter
     that proposes its best token).  Draft i stands while uniforms[row i] * q <
@@ -157,7 +157,11 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, starts: torch.Tens
     Returns (accepted [blocks] int32, next_tokens [blocks] int64); a block
     without rows gives (0, -1), a row of probabilities without mass -1.  A
     block of one row is plain sampling.  ``PageTable.commit(plan, accepted)``
-    takes the result into the page pool."""
+    takes the result into the page pool where a step's positions are all of
+    decode rows and verify blocks.  Every row of a block after its first counts
+    as a draft, so a prompt is a block of its last position alone (a chunk
+    whose prompt goes on: of none), and the step is committed with
+    ``commit(plan, accepted, starts=starts)``."""
     tensors = (tokens, target, starts, uniforms, samples, draft, accepted, next_tokens)
     key, form = _native.checked(_VERIFIES, tensors)
     if form is None:

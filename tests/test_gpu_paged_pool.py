@@ -1,10 +1,13 @@
 """The page pool under calls that its documentation allows: plans that replace
-each other, plans of other pools, and rows whose lengths do not fit their pages."""
+each other, plans of other pools, rows whose lengths do not fit their pages, and
+commits of steps that mix prompts with verify blocks."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+
+import paged_ref as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +126,58 @@ def test_long_rows_without_pages_do_not_wrap_the_count(device):
     pt.lengths[:16] = 1 << 30
     plan = pt.plan(_ints([0] * 16 + [1], device), 4)
     assert plan.info.tolist()[:3] == [2, 0, 0] and set(plan.slots.tolist()) == {-1}
+
+
+def test_accepted_counts_of_any_size(device):
+    from lightreason_amd.paged import PageTable
+
+    pt = PageTable(4, 10, 16, device=device)
+    plan = pt.plan(_ints([5, 7, 0, 3], device), 15)
+    pt.commit(plan, _ints([2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 1, -2 ** 31], device))
+    assert pt.lengths.tolist() == [5, 7, 0, 1]
+
+
+def test_a_step_of_prompts_and_verify_blocks(device):
+    """Prompts, a chunk of a prompt that goes on, verify blocks, a decode
+    position and rows that rest: probabilities only where something is drawn."""
+    from lightreason_amd.paged import PageTable
+    from lightreason_amd.verify import verify_drafts
+
+    g = torch.Generator(device=device).manual_seed(1)
+    pt = PageTable(7, 100, 16, device=device)
+    pt.commit(pt.plan(_ints([0, 10, 30, 16, 50, 0, 5], device), 111))
+    #        prompt, chunk, verify, verify, decode, rests, prompt of one
+    new = [40, 25, 5, 4, 1, 0, 1]
+    drawn = [1, 0, 5, 4, 1, 0, 1]   # rows of probabilities
+    plan = pt.plan(_ints(new, device), 80)
+    starts = [0]
+    for n in drawn:
+        starts.append(starts[-1] + n)
+    N, vocab = starts[-1], 300
+    target = torch.softmax(torch.empty(N, vocab, device=device).normal_(0, 2, generator=g), 1)
+    draft = target.clone()   # drafts stand ...
+    tokens = torch.multinomial(draft, 1, generator=g)[:, 0]
+    tokens[1:] = tokens[:-1].clone()
+    target[starts[2] + 2, tokens[starts[2] + 3]] = 0.0   # ... but for the third of the first block
+    uniforms, samples = torch.rand(N, generator=g, device=device), torch.rand(7, generator=g, device=device)
+    blocks = _ints(starts, device)
+    accepted, token = verify_drafts(tokens, target, blocks, uniforms, samples, draft=draft)
+    want = ref.verify(tokens, target, starts, uniforms.tolist(), samples.tolist(), draft)
+    assert accepted.tolist() == want[0] == [0, 0, 2, 3, 0, 0, 0] and token.tolist() == want[1]
+    pt.commit(plan, accepted, starts=blocks)
+    pt.check()
+    assert pt.lengths.tolist() == [40, 35, 33, 20, 51, 0, 6] and _whole(pt)
+    # blocks that are the step's own: as without starts
+    plan = pt.plan(_ints([3, 0, 2, 1, 1, 4, 1], device), 12)
+    accepted = _ints([1, 0, 1, 0, 0, 0, 0], device)
+    pt.commit(plan, accepted, starts=plan.starts)
+    assert pt.lengths.tolist() == [42, 35, 35, 21, 52, 1, 7]
+    # starts that fit no step: growth stays within 1 .. n
+    plan = pt.plan(_ints([3, 2, 1, 0, 0, 0, 0], device), 6)
+    pt.commit(plan, _ints([0, 9, -5, 0, 0, 0, 0], device), starts=_ints([0, 100, 50, 2 ** 31 - 1, -9, 0, 0, 0], device))
+    assert pt.lengths.tolist() == [43, 37, 36, 21, 52, 1, 7]
+    for bad in (blocks[:-1], blocks.long(), blocks.cpu()):
+        with pytest.raises(ValueError):
+            pt.commit(plan, accepted, starts=bad)
+    with pytest.raises(ValueError, match="accepted"):
+        pt.commit(plan, starts=blocks)

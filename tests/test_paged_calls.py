@@ -18,3 +18,17 @@ def test_plans_belong_to_their_pool():
     cache = torch.zeros(10, 2, 16, 256, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="pool"):
         paged.paged_layer(None, torch.zeros(4, 2048, dtype=torch.bfloat16), None, None, cache, cache, a, plan)
+
+
+def test_commit_of_blocks_refuses_before_any_launch():
+    from lightreason_amd import _native
+
+    lib, p = _native.library(), 256
+    assert lib.lrmoe_page_commit_drafts(-1, *([p] * 9), None) == -1
+    assert lib.lrmoe_page_commit_drafts(4097, *([p] * 9), None) == -1
+    for i in range(9):
+        assert lib.lrmoe_page_commit_drafts(1, *([p] * i + [None] + [p] * (8 - i)), None) == -1
+    assert lib.lrmoe_page_commit_drafts(0, *([None] * 9), None) == 0
+    pt = paged.PageTable(2, 10, 16, device="cpu")
+    with pytest.raises(ValueError, match="accepted"):
+        pt.commit(pt.new_plan(4), starts=torch.zeros(3, dtype=torch.int32))
