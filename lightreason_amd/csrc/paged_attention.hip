@@ -716,7 +716,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[nb][i]);
         top = pair_max(top) * scale;
-        if (__any(top > m + kSlack)) {
+        if (__any(top - m > kSlack)) {   // (the difference: a sum with m may be rounded up to top)
             const float mn = __builtin_fmaxf(m, top);
             const float fall = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
