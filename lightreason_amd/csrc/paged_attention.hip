@@ -6,10 +6,11 @@
 // The rows that share keys and values (a sequence's new tokens, times the
 // query heads of one key/value head) form tiles of 32 or 128; a workgroup
 // takes a tile over a range of positions, in one pass: a block of scores
-// S^T = K Q^T, a running maximum m per row (sums are rescaled only when it
-// grew by more than 2^8: what is summed is relative to m, whatever m is, so
-// the result does not depend on it), weights exp2(s - m) rounded to the
-// tensors' type, and their product with the values into fp32 sums.  Both
+// S^T = K Q^T, a running maximum per row and a point m at or (fp16) 2^7 below
+// it (moved, and the sums rescaled, only when the maximum grew by more than
+// 2^8: what is summed is relative to m, whatever m is, so the result does not
+// depend on it), weights exp2(s - m) rounded to the tensors' type, and their
+// product with the values into fp32 sums.  Both
 // products are 32x32x16 matrix instructions.  In the transposed form a lane
 // holds scores of one row only, so maxima and sums stay in the lane (and its
 // partner 32 lanes on), and the weights are the second product's operand as
@@ -543,6 +544,13 @@ struct Partials {
 
 constexpr float kLowest = -3.40282347e38f;  // the running maximum before any position: no finite score is below
 constexpr float kSlack = 8.0f;              // a maximum may lag by 2^8 before sums are rescaled
+// What is summed is relative to a point this far below the maximum (and above
+// it by no more than the slack later on).  fp16 weights then are 2^7 to 2^15 at
+// the top of its range, and keep all bits from 2^-21 of the highest down to
+// where they have none, 2^-32; at 2^0 to 2^8 those were 2^-14 and 2^-25, which
+// long rows of small weights add up to.  bf16 has the range of fp32.
+template <bool FP16>
+constexpr float kBelow = FP16 ? 7.0f : 0.0f;
 // From this maximum on, a score's product with the scale is rounded before the
 // maximum is taken off it: the exact product (one fused operation, below)
 // differs from the maximum, which is a rounded one, by up to 2^-24 of it, and
@@ -716,8 +724,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[nb][i]);
         top = pair_max(top) * scale;
-        if (__any(top - m > kSlack)) {   // (the difference: a sum with m may be rounded up to top)
-            const float mn = __builtin_fmaxf(m, top);
+        // (m is kBelow below the maximum of its time; the difference, as a sum
+        // with m may be rounded up to top)
+        if (__any(top - m > kSlack + kBelow<FP16>)) {
+            const float mn = __builtin_fmaxf(m, top - kBelow<FP16>);
             const float fall = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= fall;

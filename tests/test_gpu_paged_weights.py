@@ -30,3 +30,28 @@ def test_attention_weights_where_fp32_is_coarse(device, layout, kv, n):
     c["v_cache"].masked_fill_(torch.isfinite(c["v_cache"]), 1.0)
     got = _run_attention(c, max_new=n, scale=0.0433)
     assert bool(((got.double() - 1.0).abs() <= 2 * ref.half_step(HF) + kv * 2.0 ** -23).all())
+
+
+# ---- attention: many small weights ------------------------------------------------
+
+@pytest.mark.parametrize("layout,kv,n", [((2, 1, 64), 60001, 1), ((16, 2, 256), 30001, 2), ((8, 1, 128), 30001, 40),
+                                         ((16, 2, 256), 9001, 700)])
+def test_attention_fp16_small_weights_count(device, layout, kv, n):
+    # Every 32nd position has value 0 and the highest score, all others are 18
+    # below it: weights of 2^-26 of its, 31 for each, are the whole result.
+    # Relative to a point 2^7 or more below the highest, fp16 weights keep
+    # steps of 2^-24: half of one for each weight is 2^-32 of the highest, for
+    # 32 positions to each highest, with values of 30000; then the roundings
+    # of attention_bound for the result, the weights' sizes and the scores.
+    c, table, starts, kvs = _case(device, *layout, 64, [(kv, n)], HF, seed=27)
+    _one_element(c, 1.0, [18.0 if p % 32 == 0 else 0.0 for p in range(kv)])
+    c["v_cache"].masked_fill_(torch.isfinite(c["v_cache"]), 30000.0)
+    for p in range(0, kv, 32):
+        c["v_cache"][table[0][p // 64], :, p % 64] = 0.0
+    got = _run_attention(c, max_new=n, scale=1.0)
+    want, spread, score = ref.attention(c["q"], c["k_cache"], c["v_cache"], table, starts, kvs, 1.0)
+    h, D = ref.half_step(HF), layout[2]
+    soft = 2 * (D + 4) * 2.0 ** -24 * score + 2 * kv * 2.0 ** -24 + 2.0 ** -20
+    bound = h * want.abs() * (1 + 2.0 ** -6) + (h + soft) * spread + 32 * 2.0 ** -32 * 30000.0 + 2.0 ** -25
+    assert float(want.min()) > 0.01   # what was lost when they vanished
+    assert bool(((got.double() - want).abs() <= bound).all())
