@@ -600,7 +600,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
  * when a gate is given; softmax and sums in fp32.  A row that sees nothing
  * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
- * row does not see cannot change it, infinities and NaN included.  Tokens
+ * row does not see cannot change it (infinities and NaN no more than its last
+ * bits: rows next to some that see such values are summed in another order).  Tokens
  * outside starts[0] .. starts[seqs] - 1 are left as they were, and all are
  * when starts are not ascending within [0, tokens].  A table entry outside
  * [0, pages) in use makes its sequence's rows NaN (those of earlier positions

@@ -726,8 +726,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         top = pair_max(top) * scale;
         // (m is kBelow below the maximum of its time; the difference, as a sum
         // with m may be rounded up to top)
-        if (__any(top - m > kSlack + kBelow<FP16>)) {
-            const float mn = __builtin_fmaxf(m, top - kBelow<FP16>);
+        const bool grew = top - m > kSlack + kBelow<FP16>;
+        if (__any(grew)) {
+            // A row's own step: other rows may see what it does not.
+            const float mn = grew ? __builtin_fmaxf(m, top - kBelow<FP16>) : m;
             const float fall = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= fall;
@@ -737,15 +739,16 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 for (int i = 0; i < 16; ++i) o[db][i] *= fall;
         }
         float factor = scale, off = m;
-        if (__any(__builtin_fabsf(m) > kRounded && m != kLowest)) {
-            factor = 1.0f;
-            off = 0.0f;
+        const bool coarse = __builtin_fabsf(m) > kRounded && m != kLowest;
+        if (__any(coarse)) {
+            factor = coarse ? 1.0f : scale;
+            off = coarse ? 0.0f : m;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float product = s[nb][i] * scale;
-                    s[nb][i] = opaque(product) - m;
+                    s[nb][i] = coarse ? opaque(product) - m : s[nb][i];
                 }
         }
         float sum = 0.0f;

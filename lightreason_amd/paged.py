@@ -366,7 +366,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Softmax and sums are in fp32; the probabilities are rounded to the
     tensors' type before they meet the values.  A row that sees nothing is 0;
-    what a row does not see cannot change it, infinities and NaN included;
+    what a row does not see cannot change it (infinities and NaN no more than
+    its last bits: rows next to some that see such values are summed in
+    another order);
     tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``,
     and all do when ``starts`` are not ascending within [0, tokens].  A table
     entry in use outside the pool makes its sequence's rows NaN (those of
