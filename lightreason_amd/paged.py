@@ -21,7 +21,8 @@ has no counterpart.
 
 Nothing reads a device value on the host: every call can be captured into a
 HIP graph whose replays follow the counts and lengths on the device.  There
-is no CPU path: the calls raise when liblrmoe.so is missing.
+is no CPU path: the calls raise when liblrmoe.so is missing.  They serve only:
+no gradient is recorded, whatever their inputs require.
 """
 
 from __future__ import annotations
@@ -442,6 +443,7 @@ def _check_attention(q, k_cache, v_cache, table, starts, kv_lengths, gate, out, 
     return a, dev, nbytes
 
 
+@torch.no_grad()
 def paged_layer(attn, hidden: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
                 v_cache: torch.Tensor, pages: PageTable, plan: PagePlan, *, max_new: int | None = None) -> torch.Tensor:
     """One full-attention layer of the 35B model for a step: ``attn`` (an
