@@ -217,13 +217,14 @@ _stride = methodcaller("stride")
 def checked(forms: dict, tensors, *rest):
     """(signature, form): what the checks of a call depend on -- types,
     shapes, devices and strides of its tensors (None for one that is left
-    out) and its other arguments -- and the form kept for it, if any; (None,
-    None) where an argument is not what it should be.  Addresses are not part
-    of it: the library checks their alignment in every call."""
+    out), its other arguments and their types (1, 1.0 and True compare equal)
+    -- and the form kept for it, if any; (None, None) where an argument is not
+    what it should be.  Addresses are not part of it: the library checks their
+    alignment in every call."""
     try:
         given = [t for t in tensors if t is not None]
         missing = None if len(given) == len(tensors) else tuple([t is None for t in tensors])
-        key = (tuple(map(_traits, given)), tuple(map(_stride, given)), missing, rest)
+        key = (tuple(map(_traits, given)), tuple(map(_stride, given)), missing, rest, tuple(map(type, rest)))
         return key, forms.get(key)
     except (AttributeError, TypeError, RuntimeError):
         return None, None

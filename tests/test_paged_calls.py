@@ -32,3 +32,16 @@ def test_commit_of_blocks_refuses_before_any_launch():
     pt = paged.PageTable(2, 10, 16, device="cpu")
     with pytest.raises(ValueError, match="accepted"):
         pt.commit(pt.new_plan(4), starts=torch.zeros(3, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("first,others", [(1, (1.0, True)), (0, (False, 0.0)), (2.0, (2,)), (None, (0, False))])
+def test_checked_forms_tell_types_apart(first, others):
+    from lightreason_amd import _native
+
+    forms, t = {}, torch.zeros(2, 3)
+    key, form = _native.checked(forms, (t, None), first)
+    assert form is None
+    _native.remember(forms, key, "checked")
+    assert _native.checked(forms, (t, None), first)[1] == "checked"
+    for other in others:
+        assert _native.checked(forms, (t, None), other)[1] is None
