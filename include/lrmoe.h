@@ -573,7 +573,9 @@ int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t *mask, 
  * after every step).  A token whose slot lies outside the pool is left out
  * altogether; of tokens with the same slot, which one stays is not defined.
  * Strides are in elements and multiples of 8; the last dimension is
- * contiguous; pointers 16-byte aligned.  All 16-bit tensors are bf16, or fp16
+ * contiguous; pointers 16-byte aligned.  q_out may be q itself (the same
+ * strides); else it overlaps none of q, k and v (refused), and what a call
+ * writes overlaps nothing else that it reads or writes.  All 16-bit tensors are bf16, or fp16
  * with fp16 != 0. */
 typedef struct lrmoe_paged_append_args {
     int32_t tokens, heads, kv_heads, dim; /* dim 64, 128 or 256; heads 0: no queries */
@@ -607,7 +609,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * [0, pages) in use makes its sequence's rows NaN (those of earlier positions
  * may keep their values); kv_lengths beyond max_pages pages are cut there.
  * max_new only chooses the kernel: at least every n, else the call is slower.
- * out must not overlap q or gate.
+ * out must overlap neither q nor gate nor itself (refused; rows of one buffer
+ * may lie between each other), nor anything else that the call reads.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
  * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
  * bytes (at most 160 MB for width 256 and 16 key/value heads, 40 MB and less

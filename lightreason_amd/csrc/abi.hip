@@ -2,6 +2,7 @@
 // Host-side argument checks happen here; nothing is launched when they fail.
 #include <string.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "lrmoe_internal.h"
@@ -743,6 +744,64 @@ int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t* mask, 
 
 static bool bad_dim(int dim) { return dim != 64 && dim != 128 && dim != 256; }
 
+// Rows of `dim` 16-bit elements at token and head strides (in elements).
+struct HeadRows {
+    const void* base;
+    int64_t token, head;
+    int heads;
+};
+// Whether a row of one tensor and a row of another share an element; with
+// `same` whether two different rows of one tensor do.  Tensors apart in memory,
+// nearly all, are told by their ends.  Interleaved ones (rows of one buffer)
+// are gone through head by head: the tokens' distance that brings two rows
+// closest is a quotient where the token strides are equal; where they are not,
+// every token is tried, and more than 2^20 of those count as overlapping.
+static bool share_elements(const HeadRows& a, const HeadRows& b, int64_t tokens, int64_t dim, bool same = false) {
+    auto first = [&](const HeadRows& r) {
+        return static_cast<int64_t>(reinterpret_cast<uintptr_t>(r.base) / 2) +
+               std::min(INT64_C(0), (tokens - 1) * r.token) + std::min(INT64_C(0), (r.heads - 1) * r.head);
+    };
+    auto end = [&](const HeadRows& r) {
+        return static_cast<int64_t>(reinterpret_cast<uintptr_t>(r.base) / 2) +
+               std::max(INT64_C(0), (tokens - 1) * r.token) + std::max(INT64_C(0), (r.heads - 1) * r.head) + dim;
+    };
+    if (a.heads < 1 || b.heads < 1 || tokens < 1 || end(a) <= first(b) || end(b) <= first(a)) return false;
+    const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.base) / 2) -
+                          static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.base) / 2);
+    // Whether c + k stride lies within (-dim, dim) for some k of from .. to.
+    auto meets = [&](int64_t c, int64_t stride, int64_t from, int64_t to) {
+        if (stride == 0) return c > -dim && c < dim;
+        const int64_t near = -c / stride;
+        for (int64_t k = near - 1; k <= near + 1; ++k) {
+            const int64_t at = c + std::clamp(k, from, to) * stride;
+            if (at > -dim && at < dim) return true;
+        }
+        return false;
+    };
+    if (a.token != b.token && static_cast<int64_t>(a.heads) * b.heads * tokens > (1 << 20)) return true;
+    for (int i = 0; i < a.heads; ++i)
+        for (int j = same ? i : 0; j < b.heads; ++j) {
+            const int64_t c = apart + j * b.head - i * a.head;
+            if (a.token != b.token) {
+                for (int64_t t = 0; t < tokens; ++t)
+                    if (meets(c - t * a.token, b.token, 0, tokens - 1)) return true;
+            } else if (same && i == j) {
+                if (tokens > 1 && a.token > -dim && a.token < dim) return true;
+            } else if (meets(c, a.token, 1 - tokens, tokens - 1)) {
+                return true;
+            }
+        }
+    return false;
+}
+// Whether a tensor's rows follow each other without overlap, in either order of
+// its two strides (what nearly all tensors are).
+static bool nested_rows(const HeadRows& r, int64_t tokens, int64_t dim) {
+    if (tokens <= 1) return r.heads <= 1 || r.head >= dim;
+    if (r.heads <= 1) return r.token >= dim;
+    return (r.head >= dim && r.token >= (r.heads - 1) * r.head + dim) ||
+           (r.token >= dim && r.head >= (tokens - 1) * r.token + dim);
+}
+
 int lrmoe_paged_append(const lrmoe_paged_append_args* p, void* stream) {
     if (!p) return LRMOE_E_ARG;
     if (p->tokens < 0 || p->tokens > (1 << 24) || p->heads < 0 || p->heads > 1024 || p->kv_heads < 1 ||
@@ -760,6 +819,16 @@ int lrmoe_paged_append(const lrmoe_paged_append_args* p, void* stream) {
                       p->v_head_stride, p->k_page_stride, p->k_cache_head_stride, p->k_row_stride, p->v_page_stride,
                       p->v_cache_head_stride, p->v_row_stride})
         if (x % 8 != 0) return LRMOE_E_ARG;
+    // Queries may be normed and rotated in place, row for row.
+    const HeadRows q{p->q, p->q_token_stride, p->q_head_stride, p->heads};
+    const HeadRows q_out{p->q_out, static_cast<int64_t>(p->heads) * p->dim, p->dim, p->heads};
+    const bool in_place = q.base == q_out.base && (p->tokens == 1 || q.token == q_out.token) &&
+                          (p->heads <= 1 || q.head == q_out.head);
+    if (p->heads > 0 &&
+        ((!in_place && share_elements(q_out, q, p->tokens, p->dim)) ||
+         share_elements(q_out, {p->k, p->k_token_stride, p->k_head_stride, p->kv_heads}, p->tokens, p->dim) ||
+         share_elements(q_out, {p->v, p->v_token_stride, p->v_head_stride, p->kv_heads}, p->tokens, p->dim)))
+        return LRMOE_E_ARG;
     if (static_cast<int64_t>(p->tokens) * (p->heads + 2 * p->kv_heads) * (p->dim / 8) > (INT64_C(1) << 38))
         return LRMOE_E_ARG;  // a grid of at most 2^30 workgroups
     if (int d = check_device()) return d;
@@ -819,7 +888,6 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     if (p->tokens == 0 || p->seqs == 0) return LRMOE_OK;
     if (!p->q || !p->k_cache || !p->v_cache || !p->table || !p->starts || !p->kv_lengths || !p->out)
         return LRMOE_E_ARG;
-    if (p->out == p->q || p->out == p->gate) return LRMOE_E_ARG;
     if (misaligned(p->q, 16) || misaligned(p->k_cache, 16) || misaligned(p->v_cache, 16) || misaligned(p->out, 16) ||
         misaligned(p->gate, 16) || misaligned(workspace, 256))
         return LRMOE_E_ARG;
@@ -836,6 +904,12 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args* p, void* workspace, 
     const size_t need = lrmoe_paged_attention_workspace_bytes(p);
     if (!workspace) return LRMOE_E_ARG;
     if (workspace_bytes < need) return LRMOE_E_WORKSPACE;
+    const HeadRows out{p->out, p->out_token_stride, p->out_head_stride, p->heads};
+    if (share_elements(out, {p->q, p->q_token_stride, p->q_head_stride, p->heads}, p->tokens, p->dim) ||
+        (p->gate &&
+         share_elements(out, {p->gate, p->gate_token_stride, p->gate_head_stride, p->heads}, p->tokens, p->dim)) ||
+        (!nested_rows(out, p->tokens, p->dim) && share_elements(out, out, p->tokens, p->dim, true)))
+        return LRMOE_E_ARG;
     if (int d = check_device()) return d;
     lrmoe::PagedAttnArgs a{};
     a.seqs = p->seqs;

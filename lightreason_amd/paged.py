@@ -271,7 +271,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     caches may be strided views with a contiguous last dimension (the 35B
     model's q and gate come interleaved from one projection).  A token whose
     slot lies outside the pool (-1: padding) is left out, its q_out row too;
-    tokens must not share a slot."""
+    tokens must not share a slot.  ``q_out`` may be a contiguous ``q`` itself;
+    else it shares no element with ``q``, ``k`` or ``v`` (refused), nor the
+    caches with each other or an input."""
     tensors = (k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out)
     eps = float(eps)   # a number, whatever held it: forms are kept by value
     key, form = _native.checked(_APPENDS, tensors, eps)
@@ -373,8 +375,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``,
     and all do when ``starts`` are not ascending within [0, tokens].  A table
     entry in use outside the pool makes its sequence's rows NaN (those of
-    earlier positions may keep their values).  ``out`` must not overlap ``q``
-    or ``gate``.
+    earlier positions may keep their values).  ``out`` may share a buffer with
+    ``q`` and ``gate`` but no element with them or between its own rows
+    (refused), nor with anything else that is read.
 
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
     chooses the kernel: give it where the counts are known to be small."""

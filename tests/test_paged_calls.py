@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -45,3 +47,64 @@ def test_checked_forms_tell_types_apart(first, others):
     assert _native.checked(forms, (t, None), first)[1] == "checked"
     for other in others:
         assert _native.checked(forms, (t, None), other)[1] is None
+
+
+def _rows(base, shape, strides, dim):
+    return {base + t * strides[0] + h * strides[1] + d
+            for t in range(shape[0]) for h in range(shape[1]) for d in range(dim)}
+
+
+@pytest.mark.parametrize("which", ["q", "gate", "out"])
+def test_overlapping_outputs_of_the_attention_are_refused(which):
+    """Layouts in which out shares elements with q, with gate or with itself,
+    told by sets of addresses, are refused before any launch (addresses in
+    elements of 2 bytes; the calls that would pass are made on the GPU)."""
+    import random
+
+    from lightreason_amd import _native
+
+    lib, rng, D, refused = _native.library(), random.Random(which), 64, 0
+    for _ in range(400):
+        N, H = rng.choice([1, 2, 5]), rng.choice([1, 2, 4])
+        base = 1 << 20
+        out_at = base + 8 * rng.randint(-60, 60)
+
+        def strides():
+            pitch = rng.choice([D, D + 8, 2 * D, 0])
+            return rng.choice([(H * pitch, pitch), (H * pitch + 2 * D, pitch), (pitch, N * pitch), (2 * D, 4 * D)])
+        s, o = strides(), strides()
+        out = _rows(out_at, (N, H), o, D)
+        if which == "out":
+            shared = len(out) < N * H * D
+            other = dict(q=256, q_token_stride=H * D, q_head_stride=D)
+        else:
+            shared = bool(out & _rows(base, (N, H), s, D))
+            other = {which: 2 * base, f"{which}_token_stride": s[0], f"{which}_head_stride": s[1]}
+            if which == "gate":
+                other.update(q=256, q_token_stride=H * D, q_head_stride=D)
+        if not shared:
+            continue
+        refused += 1
+        a = _native.PagedAttentionArgs(
+            seqs=1, tokens=N, max_new=1, heads=H, kv_heads=1, dim=D, pages=4, page=16, max_pages=4, scale=1.0,
+            k_cache=256, v_cache=256, k_page_stride=1024, k_head_stride=1024, k_row_stride=64, v_page_stride=1024,
+            v_head_stride=1024, v_row_stride=64, table=256, starts=256, kv_lengths=256, out=2 * out_at,
+            out_token_stride=o[0], out_head_stride=o[1], **other)
+        assert lib.lrmoe_paged_attention(C.addressof(a), 256, 1 << 40, None) == -1, (N, H, s, o, out_at - base)
+    assert refused > 50
+
+
+def test_queries_written_over_other_inputs_are_refused():
+    from lightreason_amd import _native
+
+    lib, D, N, H = _native.library(), 64, 3, 2
+    far = {"q": 1 << 20, "k": 1 << 21, "v": 1 << 22, "q_out": 1 << 23}
+    for kw in (dict(q_out=far["q"] + 2 * 64), dict(q_out=far["q"] - 2 * 64), dict(q_out=far["k"] + 2 * 64),
+               dict(q_out=far["v"]), dict(q_out=far["q"], q_token_stride=256), dict(q_out=far["q"], q_head_stride=0)):
+        args = dict(tokens=N, heads=H, kv_heads=1, dim=D, pages=4, page=16, q_token_stride=H * D, q_head_stride=D,
+                    k_token_stride=D, k_head_stride=D, v_token_stride=D, v_head_stride=D, eps=1e-6, slots=256,
+                    k_cache=256, v_cache=512, k_page_stride=1024, k_cache_head_stride=1024, k_row_stride=64,
+                    v_page_stride=1024, v_cache_head_stride=1024, v_row_stride=64, **far)
+        args.update(kw)
+        a = _native.PagedAppendArgs(**args)
+        assert lib.lrmoe_paged_append(C.addressof(a), None) == -1, kw
