@@ -644,10 +644,11 @@ int lrmoe_paged_attention(const lrmoe_paged_attention_args *args, void *workspac
  * the first that fails.  next[b] is then drawn from max(p - q, 0) at that row
  * (draft NULL: p without the failed token; p where nothing is left), or from
  * p at the last row when every draft stands: the first token whose running
- * sum passes samples[b] times the total, in 64 bits; entries that are
- * negative or not finite carry no mass, a row without any mass gives -1, and
- * so does a block without rows (accepted 0).  uniforms [rows] and samples
- * [blocks] fp32 in [0, 1).  type 0 fp32, 1 bf16, 2 fp16, of target and draft.
+ * sum passes samples[b] times the total, in 64 bits; a token carries no mass
+ * where p, or p - q where that is drawn from, is not positive or not finite; a
+ * row without any mass gives -1, and so does a block without rows (accepted
+ * 0).  uniforms [rows] and samples [blocks] fp32 in [0, 1).  type 0 fp32, 1
+ * bf16, 2 fp16, of target and draft.
  * Workspace of lrmoe_verify_workspace_bytes bytes, 16-byte aligned. */
 size_t lrmoe_verify_workspace_bytes(int blocks, int vocab);
 int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t *tokens, const void *target,

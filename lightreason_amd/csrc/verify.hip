@@ -122,7 +122,8 @@ __device__ __forceinline__ Row row_of(const VerifyArgs& a, int first, int n, int
     return r;
 }
 __device__ __forceinline__ double rest_of(const Row& r, int64_t v, float p, float q) {
-    if (r.both) return mass_of(static_cast<double>(p) - static_cast<double>(q));
+    // (A token that the target gives no mass has none left, whatever q is.)
+    if (r.both) return p > 0.0f ? mass_of(static_cast<double>(p) - static_cast<double>(q)) : 0.0;
     return v == r.dropped ? 0.0 : mass_of(p);
 }
 
