@@ -575,8 +575,9 @@ int lrmoe_page_release(int rows, int pages, int max_pages, const uint8_t *mask, 
  * Strides are in elements and multiples of 8; the last dimension is
  * contiguous; pointers 16-byte aligned.  q_out may be q itself (the same
  * strides); else it overlaps none of q, k and v (refused), and what a call
- * writes overlaps nothing else that it reads or writes.  All 16-bit tensors are bf16, or fp16
- * with fp16 != 0. */
+ * writes overlaps nothing else that it reads or writes.  At most 2^24 tokens,
+ * and fewer than 2^32 threads, dim / 8 for every four head rows.  All 16-bit
+ * tensors are bf16, or fp16 with fp16 != 0. */
 typedef struct lrmoe_paged_append_args {
     int32_t tokens, heads, kv_heads, dim; /* dim 64, 128 or 256; heads 0: no queries */
     int32_t rotary;                       /* 0, or a multiple of 16 up to dim */

@@ -829,8 +829,10 @@ int lrmoe_paged_append(const lrmoe_paged_append_args* p, void* stream) {
          share_elements(q_out, {p->k, p->k_token_stride, p->k_head_stride, p->kv_heads}, p->tokens, p->dim) ||
          share_elements(q_out, {p->v, p->v_token_stride, p->v_head_stride, p->kv_heads}, p->tokens, p->dim)))
         return LRMOE_E_ARG;
-    if (static_cast<int64_t>(p->tokens) * (p->heads + 2 * p->kv_heads) * (p->dim / 8) > (INT64_C(1) << 38))
-        return LRMOE_E_ARG;  // a grid of at most 2^30 workgroups
+    // A launch holds fewer than 2^32 threads: dim / 8 for every four head rows.
+    if (static_cast<int64_t>(p->tokens) * ((p->heads + 2 * p->kv_heads + 3) / 4) * (p->dim / 8) >
+        (INT64_C(1) << 32) - 256)
+        return LRMOE_E_ARG;
     if (int d = check_device()) return d;
     lrmoe::PagedAppendArgs a{};
     a.tokens = p->tokens;

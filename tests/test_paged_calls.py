@@ -108,3 +108,15 @@ def test_queries_written_over_other_inputs_are_refused():
         args.update(kw)
         a = _native.PagedAppendArgs(**args)
         assert lib.lrmoe_paged_append(C.addressof(a), None) == -1, kw
+
+
+def test_appends_of_more_threads_than_a_launch_holds_are_refused():
+    from lightreason_amd import _native
+
+    lib = _native.library()
+    for tokens, kv_heads, dim in ((1 << 24, 1024, 256), (1 << 24, 16, 256), (1 << 20, 256, 256), (1 << 24, 64, 64)):
+        a = _native.PagedAppendArgs(
+            tokens=tokens, heads=0, kv_heads=kv_heads, dim=dim, pages=4, page=16, k=256, v=256, slots=256, k_cache=256,
+            v_cache=512, k_page_stride=1 << 20, k_cache_head_stride=1 << 14, k_row_stride=dim, v_page_stride=1 << 20,
+            v_cache_head_stride=1 << 14, v_row_stride=dim)
+        assert lib.lrmoe_paged_append(C.addressof(a), None) == -1, (tokens, kv_heads, dim)
