@@ -601,7 +601,9 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * of [HF] Qwen3_5MoeAttention.forward 703-718: token t of sequence s (tokens
  * starts[s] .. starts[s + 1] - 1, n in all) sees cached positions 0 ..
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
- * when a gate is given; softmax and sums in fp32.  A row that sees nothing
+ * when a gate is given; softmax and sums in fp32, the weights of the product
+ * with v rounded to the tensors' type, or to two numbers of it where max_new *
+ * heads / kv_heads is at most 128.  A row that sees nothing
  * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
  * row does not see cannot change it (infinities and NaN no more than its last
  * bits: rows next to some that see such values are summed in another order).  Tokens
@@ -609,7 +611,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * when starts are not ascending within [0, tokens].  A table entry outside
  * [0, pages) in use makes its sequence's rows NaN (those of earlier positions
  * may keep their values); kv_lengths beyond max_pages pages are cut there.
- * max_new only chooses the kernel: at least every n, else the call is slower.
+ * max_new only chooses the kernel, and with it that rounding: at least every
+ * n, else the call is slower.
  * out must overlap neither q nor gate nor itself (refused; rows of one buffer
  * may lie between each other), nor anything else that the call reads.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over

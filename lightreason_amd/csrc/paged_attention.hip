@@ -9,8 +9,8 @@
 // S^T = K Q^T, a running maximum per row and a point m at or (fp16) 2^7 below
 // it (moved, and the sums rescaled, only when the maximum grew by more than
 // 2^8: what is summed is relative to m, whatever m is, so the result does not
-// depend on it), weights exp2(s - m) rounded to the tensors' type, and their
-// product with the values into fp32 sums.  Both
+// depend on it), weights exp2(s - m) as one or two numbers of the tensors' type
+// (shape_of), and their product with the values into fp32 sums.  Both
 // products are 32x32x16 matrix instructions.  In the transposed form a lane
 // holds scores of one row only, so maxima and sums stay in the lane (and its
 // partner 32 lanes on), and the weights are the second product's operand as
@@ -509,16 +509,16 @@ __device__ __forceinline__ void stage_rows(const PagedAttnArgs& a, const CacheVi
 // right before its product, to save registers, and every product waits for
 // LDS (4096 positions over 28003 cached at width 256: 2.63 ms; 1.90 with four
 // ahead in both products; five or more cost spills or gain nothing).
-template <int FRAGS, int READS>
+template <int FRAGS, int READS, int PRODUCTS = 1>
 __device__ __forceinline__ void read_ahead() {
     constexpr int AHEAD = 4, PRODUCT = 0x8, LDS_READ = 0x100;
     __builtin_amdgcn_sched_group_barrier(LDS_READ, AHEAD * READS, 0);
 #pragma unroll
     for (int i = 0; i < FRAGS - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(PRODUCT, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(PRODUCT, PRODUCTS, 0);
         __builtin_amdgcn_sched_group_barrier(LDS_READ, READS, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(PRODUCT, AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(PRODUCT, PRODUCTS * AHEAD, 0);
 }
 
 // A product that no later operation is fused with.
@@ -561,8 +561,8 @@ constexpr float kRounded = 4194304.0f;
 // load together, two in flight (eight waves on one tile instead of two
 // workgroups of four per CU took 2.03 ms where these took 1.82: their barriers
 // keep them in step), or WK waves that share 32 rows and take tiles of their
-// own.
-template <bool FP16, int D, int WQ, int WK, int NB, bool DENSE>
+// own.  PARTS: 16-bit numbers that make up a weight in the second product.
+template <bool FP16, int D, int WQ, int WK, int NB, int PARTS, bool DENSE>
 __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
     PagedAttnArgs a, Partials part, int target, int least) {
     constexpr int THREADS = kWave * WQ * WK;
@@ -695,9 +695,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     // packed for the second product.  S^T = K Q^T, so a lane holds 16 NB
     // positions of its row and the weights are the second product's operand as
     // they are: of a step of 16 positions lane (q, hi) holds 4 hi + {0..3,
-    // 8..11}.  The weights are rounded to the tensors' type (a product of two
-    // 16-bit operands); their sum is not.
-    auto scores = [&](uint32_t kt, int base, uint4 (&pw)[2 * NB]) {
+    // 8..11}.  The product takes 16-bit operands, so the weights are rounded to
+    // the tensors' type, or split into two numbers of it, the second what the
+    // first leaves (16 bits and more of each weight); their sum is not rounded.
+    auto scores = [&](uint32_t kt, int base, uint4 (&pw)[2 * NB * PARTS]) {
         f32x16 s[NB] = {};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -762,11 +763,19 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                     w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * k + j], factor, -off));
                     sum += w[j];
                 }
-                pw[2 * nb + k] = pack16<FP16>(w);
+                const uint4 high = pack16<FP16>(w);
+                pw[(2 * nb + k) * PARTS] = high;
+                if constexpr (PARTS > 1) {
+                    float x[8];
+                    unpack16<FP16>(high, x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = w[j] - x[j];
+                    pw[(2 * nb + k) * PARTS + 1] = pack16<FP16>(x);
+                }
             }
         l += sum;
     };
-    auto values = [&](uint32_t vt, const uint4 (&pw)[2 * NB]) {
+    auto values = [&](uint32_t vt, const uint4 (&pw)[2 * NB * PARTS]) {
         __builtin_amdgcn_sched_barrier(0);   // the order below is kept within its own region only
 #pragma unroll
         for (int k = 0; k < 2 * NB; ++k)
@@ -777,9 +786,11 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
                 const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + VP::bytes(8)));
                 const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, up);
-                o[db] = mfma32<FP16>(make_uint4(x.x, x.y, y.x, y.y), pw[k], o[db]);
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+                    o[db] = mfma32<FP16>(make_uint4(x.x, x.y, y.x, y.y), pw[k * PARTS + part], o[db]);
             }
-        read_ahead<2 * NB * DB, 2>();
+        read_ahead<2 * NB * DB, 2, PARTS>();
     };
     // A value that is not finite among the tile's: all exponent bits set.
     auto look = [&](uint32_t vt) {
@@ -791,7 +802,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
         }
     };
 
-    uint4 pw[2 * NB];
+    uint4 pw[2 * NB * PARTS];
     if constexpr (WK == 1) {
         for (int j = 0; j < steps; ++j) {
             const int base = k0 + j * STEP;
@@ -1125,6 +1136,7 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
 
 struct Shape {
     int bm, step, target, least;
+    int parts;   // of a weight
 };
 // The kernel of a step.  Where every sequence's rows fit into 32: one tile of
 // them, four waves on positions of their own, many splits (64 sequences of
@@ -1137,9 +1149,18 @@ struct Shape {
 // the latter has no splits: 45.7 and 88), and splits of at least 8 steps,
 // whose partial rows cost about as much (the verify blocks: 35.6 us, 39.4 with
 // 16).
+// Weights are in two parts where every sequence's rows fit into one tile: each
+// key and value then meets at most 128 rows, HBM sets the pace and the further
+// products are nearly free (one sequence of 1000 positions 13.5 -> 13.7 us, 64
+// of 200-16000 202.2 -> 202.8, the verify blocks 37.7 -> 39.1), for results as
+// far from 64 bits as their own rounding is (1.7e-3 in bf16; 2.1e-3 to 2.3e-3
+// with one part).  Longer steps are bound by the products and keep to one, the
+// rounding of the Transformers forward (two: 2048 positions 68 -> 91 us, 4096
+// over 28003 1.66 -> 2.38 ms).
 Shape shape_of(int group, int max_new, int dim) {
-    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 1024, 1};
-    return {128, dim == 256 ? 32 : 64, 256, 8};
+    const int64_t rows = static_cast<int64_t>(max_new) * group;
+    if (rows <= 32) return {32, 128, 1024, 1, 2};
+    return {128, dim == 256 ? 32 : 64, 256, 8, rows <= 128 ? 2 : 1};
 }
 
 struct Layout {
@@ -1176,14 +1197,14 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     return l;
 }
 
-template <bool FP16, int D, int WQ, int WK, int NB>
+template <bool FP16, int D, int WQ, int WK, int NB, int PARTS>
 void launch_shape(const PagedAttnArgs& a, const Shape& sh, const Partials& part, int max_new, hipStream_t stream) {
     const dim3 grid(part.workgroups), block(kWave * WQ * WK);
     if (a.k_row_stride == D && a.v_row_stride == D)
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, true>), grid, block, 0, stream, a, part, sh.target,
-                           sh.least);
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, PARTS, true>), grid, block, 0, stream, a, part,
+                           sh.target, sh.least);
     else
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, false>), grid, block, 0, stream, a, part,
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, PARTS, false>), grid, block, 0, stream, a, part,
                            sh.target, sh.least);
     // Merge workgroups per tile: a row each, or a block of 32 elements each.
     const int64_t rows = static_cast<int64_t>(max_new) * a.group;
@@ -1195,8 +1216,10 @@ void launch_shape(const PagedAttnArgs& a, const Shape& sh, const Partials& part,
 template <bool FP16, int D>
 hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
     const Shape sh = shape_of(a.group, max_new, D);
-    if (sh.bm == 32) launch_shape<FP16, D, 1, 4, 1>(a, sh, part, max_new, stream);
-    else launch_shape<FP16, D, 4, 1, (D == 256 ? 1 : 2)>(a, sh, part, max_new, stream);
+    constexpr int NB = D == 256 ? 1 : 2;
+    if (sh.bm == 32) launch_shape<FP16, D, 1, 4, 1, 2>(a, sh, part, max_new, stream);
+    else if (sh.parts == 2) launch_shape<FP16, D, 4, 1, NB, 2>(a, sh, part, max_new, stream);
+    else launch_shape<FP16, D, 4, 1, NB, 1>(a, sh, part, max_new, stream);
     return hipGetLastError();
 }
 

@@ -367,8 +367,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     kv_heads); ``scale`` defaults to dim ** -0.5.  With ``gate`` [tokens,
     heads, dim] the result is multiplied by sigmoid(gate).
 
-    Softmax and sums are in fp32; the probabilities are rounded to the
-    tensors' type before they meet the values.  A row that sees nothing is 0;
+    Softmax and sums are in fp32.  Where ``max_new * heads // kv_heads`` is at
+    most 128 (decode and verify steps) the weights meet the values as two
+    numbers of the tensors' type, so the result is as good as its own rounding;
+    in longer steps they are rounded to the tensors' type, as in the
+    Transformers forward.  A row that sees nothing is 0;
     what a row does not see cannot change it (infinities and NaN no more than
     its last bits: rows next to some that see such values are summed in
     another order);
@@ -380,7 +383,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (refused), nor with anything else that is read.
 
     ``max_new`` -- at least every sequence's n, default ``tokens`` -- only
-    chooses the kernel: give it where the counts are known to be small."""
+    chooses the kernel (and the weights' rounding): give it where the counts
+    are known to be small."""
     tensors = (q, k_cache, v_cache, table, starts, kv_lengths, gate, out)
     if scale is not None:
         scale = float(scale)
