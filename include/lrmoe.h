@@ -616,10 +616,14 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * out must overlap neither q nor gate nor itself (refused; rows of one buffer
  * may lie between each other), nor anything else that the call reads.
  * Strides as lrmoe_paged_append's; row strides below 2^20, pages spread over
- * at most 64 GiB.  Workspace of lrmoe_paged_attention_workspace_bytes(args)
- * bytes (at most 160 MB for width 256 and 16 key/value heads, 40 MB and less
- * for a decode step of a few heads), 256-byte aligned, not cleared, used by
- * one stream at a time. */
+ * at most 64 GiB; at most 2^20 tokens and tokens * heads of 2^28.
+ * Workspace of lrmoe_paged_attention_workspace_bytes(args) bytes, 256-byte
+ * aligned, not cleared, used by one stream at a time.  With group = heads /
+ * kv_heads and tiles of R rows, R 32 where max_new * group <= 32 and else 128,
+ * it is no more than S R (4 dim + 8) + 36 T + 16384 bytes: S = 2 (1024 +
+ * kv_heads) + 16 or, for R 128, 4 (256 + kv_heads) + 16 partial tiles, and T =
+ * kv_heads (tokens group / R + min(seqs, tokens)) tiles (2 heads of width 256:
+ * 68 MB and 138 MB beside the tiles; less where rows hold few positions). */
 typedef struct lrmoe_paged_attention_args {
     int32_t seqs, tokens, max_new, heads, kv_heads, dim; /* dim 64, 128 or 256; heads a multiple of kv_heads */
     int32_t pages, page, max_pages, fp16;

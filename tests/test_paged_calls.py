@@ -120,3 +120,30 @@ def test_appends_of_more_threads_than_a_launch_holds_are_refused():
             v_cache=512, k_page_stride=1 << 20, k_cache_head_stride=1 << 14, k_row_stride=dim, v_page_stride=1 << 20,
             v_cache_head_stride=1 << 14, v_row_stride=dim)
         assert lib.lrmoe_paged_append(C.addressof(a), None) == -1, (tokens, kv_heads, dim)
+
+
+def test_workspaces_stay_within_the_bound_of_the_header():
+    import random
+
+    from lightreason_amd import _native
+
+    lib, rng, closest = _native.library(), random.Random(5), 0.0
+    for _ in range(3000):
+        kv_heads, group = rng.choice([1, 2, 4, 8, 16, 64, 1024]), rng.choice([1, 2, 3, 8, 16, 64])
+        dim = rng.choice([64, 128, 256])
+        heads = kv_heads * group
+        if heads > 1024:
+            continue
+        tokens = min(int(2 ** rng.uniform(0, 20)), (1 << 28) // heads)
+        seqs, max_new = int(2 ** rng.uniform(0, 12)), rng.choice([1, 2, 4, 9, 40, tokens])
+        page = 1 << rng.randint(3, 10)
+        a = _native.PagedAttentionArgs(seqs=seqs, tokens=tokens, max_new=max_new, heads=heads, kv_heads=kv_heads,
+                                       dim=dim, pages=1, page=page, max_pages=int(2 ** rng.uniform(0, 30)) // page or 1)
+        got = lib.lrmoe_paged_attention_workspace_bytes(C.addressof(a))
+        rows = 32 if max_new * group <= 32 else 128
+        partial = 2 * (1024 + kv_heads) + 16 if rows == 32 else 4 * (256 + kv_heads) + 16
+        tiles = kv_heads * (tokens * group // rows + min(seqs, tokens))
+        bound = partial * rows * (4 * dim + 8) + 36 * tiles + 16384
+        assert 0 < got <= bound, (heads, kv_heads, dim, tokens, seqs, max_new, page)
+        closest = max(closest, got / bound)
+    assert closest > 0.95
