@@ -10,7 +10,7 @@
 // it (moved, and the sums rescaled, only when the maximum grew by more than
 // 2^8: what is summed is relative to m, whatever m is, so the result does not
 // depend on it), weights exp2(s - m) as one or two numbers of the tensors' type
-// (shape_of), and their product with the values into fp32 sums.  Both
+// (PARTS), and their product with the values into fp32 sums.  Both
 // products are 32x32x16 matrix instructions.  In the transposed form a lane
 // holds scores of one row only, so maxima and sums stay in the lane (and its
 // partner 32 lanes on), and the weights are the second product's operand as
@@ -561,8 +561,8 @@ constexpr float kRounded = 4194304.0f;
 // load together, two in flight (eight waves on one tile instead of two
 // workgroups of four per CU took 2.03 ms where these took 1.82: their barriers
 // keep them in step), or WK waves that share 32 rows and take tiles of their
-// own.  PARTS: 16-bit numbers that make up a weight in the second product.
-template <bool FP16, int D, int WQ, int WK, int NB, int PARTS, bool DENSE>
+// own.
+template <bool FP16, int D, int WQ, int WK, int NB, bool DENSE>
 __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void attend_tile_kernel(
     PagedAttnArgs a, Partials part, int target, int least) {
     constexpr int THREADS = kWave * WQ * WK;
@@ -574,6 +574,16 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     constexpr int KTILE = KP::bytes(KT), VTILE = VP::bytes(KT);   // bytes of a tile of keys, of values
     constexpr int STAGES = WK == 1 ? 2 : 1;
     constexpr int KS = D / 16, DB = D / 32;
+    // 16-bit numbers that make up a weight in the second product.  Two where few
+    // rows share keys and values: HBM sets the pace, the further products are
+    // nearly free (one sequence of 1000 positions 13.5 -> 13.65 us, 64 of
+    // 200-16000 202.0 -> 202.5) and the result is as far from 64 bits as its own
+    // rounding is (bf16: 1.7e-3; 2.1e-3 to 2.3e-3 with one).  Tiles of 128 rows
+    // are bound by the products or by the chain of a step, and round a weight
+    // once, as the Transformers forward does (two: 16 verify blocks 37.5 -> 38.9
+    // us, 33.8 -> 38.7 with their keys cached; 2048 positions 68 -> 91 us; 4096
+    // over 28003 1.66 -> 2.38 ms).
+    constexpr int PARTS = WK == 1 ? 1 : 2;
     constexpr int ROWS = WK == 1 ? KT / WQ : KT;   // rows that a wave stages
     constexpr int LOADS = ROWS * D / 512;          // of a key or value tile, per wave
     constexpr int LDS = STAGES * WK * (KTILE + VTILE);
@@ -1136,7 +1146,6 @@ __global__ __launch_bounds__(kThreads) void attend_merge_kernel(PagedAttnArgs a,
 
 struct Shape {
     int bm, step, target, least;
-    int parts;   // of a weight
 };
 // The kernel of a step.  Where every sequence's rows fit into 32: one tile of
 // them, four waves on positions of their own, many splits (64 sequences of
@@ -1149,18 +1158,9 @@ struct Shape {
 // the latter has no splits: 45.7 and 88), and splits of at least 8 steps,
 // whose partial rows cost about as much (the verify blocks: 35.6 us, 39.4 with
 // 16).
-// Weights are in two parts where every sequence's rows fit into one tile: each
-// key and value then meets at most 128 rows, HBM sets the pace and the further
-// products are nearly free (one sequence of 1000 positions 13.5 -> 13.7 us, 64
-// of 200-16000 202.2 -> 202.8, the verify blocks 37.7 -> 39.1), for results as
-// far from 64 bits as their own rounding is (1.7e-3 in bf16; 2.1e-3 to 2.3e-3
-// with one part).  Longer steps are bound by the products and keep to one, the
-// rounding of the Transformers forward (two: 2048 positions 68 -> 91 us, 4096
-// over 28003 1.66 -> 2.38 ms).
 Shape shape_of(int group, int max_new, int dim) {
-    const int64_t rows = static_cast<int64_t>(max_new) * group;
-    if (rows <= 32) return {32, 128, 1024, 1, 2};
-    return {128, dim == 256 ? 32 : 64, 256, 8, rows <= 128 ? 2 : 1};
+    if (static_cast<int64_t>(max_new) * group <= 32) return {32, 128, 1024, 1};
+    return {128, dim == 256 ? 32 : 64, 256, 8};
 }
 
 struct Layout {
@@ -1197,14 +1197,14 @@ Layout carve(void* base, int tokens, int seqs, int heads, int kv_heads, int dim,
     return l;
 }
 
-template <bool FP16, int D, int WQ, int WK, int NB, int PARTS>
+template <bool FP16, int D, int WQ, int WK, int NB>
 void launch_shape(const PagedAttnArgs& a, const Shape& sh, const Partials& part, int max_new, hipStream_t stream) {
     const dim3 grid(part.workgroups), block(kWave * WQ * WK);
     if (a.k_row_stride == D && a.v_row_stride == D)
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, PARTS, true>), grid, block, 0, stream, a, part,
-                           sh.target, sh.least);
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, true>), grid, block, 0, stream, a, part, sh.target,
+                           sh.least);
     else
-        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, PARTS, false>), grid, block, 0, stream, a, part,
+        hipLaunchKernelGGL((attend_tile_kernel<FP16, D, WQ, WK, NB, false>), grid, block, 0, stream, a, part,
                            sh.target, sh.least);
     // Merge workgroups per tile: a row each, or a block of 32 elements each.
     const int64_t rows = static_cast<int64_t>(max_new) * a.group;
@@ -1216,10 +1216,8 @@ void launch_shape(const PagedAttnArgs& a, const Shape& sh, const Partials& part,
 template <bool FP16, int D>
 hipError_t launch(const PagedAttnArgs& a, int max_new, const Partials& part, hipStream_t stream) {
     const Shape sh = shape_of(a.group, max_new, D);
-    constexpr int NB = D == 256 ? 1 : 2;
-    if (sh.bm == 32) launch_shape<FP16, D, 1, 4, 1, 2>(a, sh, part, max_new, stream);
-    else if (sh.parts == 2) launch_shape<FP16, D, 4, 1, NB, 2>(a, sh, part, max_new, stream);
-    else launch_shape<FP16, D, 4, 1, NB, 1>(a, sh, part, max_new, stream);
+    if (sh.bm == 32) launch_shape<FP16, D, 1, 4, 1>(a, sh, part, max_new, stream);
+    else launch_shape<FP16, D, 4, 1, (D == 256 ? 1 : 2)>(a, sh, part, max_new, stream);
     return hipGetLastError();
 }
 

@@ -368,7 +368,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     heads, dim] the result is multiplied by sigmoid(gate).
 
     Softmax and sums are in fp32.  Where ``max_new * heads // kv_heads`` is at
-    most 128 (decode and verify steps) the weights meet the values as two
+    most 32 (decode and short verify steps) the weights meet the values as two
     numbers of the tensors' type, so the result is as good as its own rounding;
     in longer steps they are rounded to the tensors' type, as in the
     Transformers forward.  A row that sees nothing is 0;

@@ -62,9 +62,9 @@ def test_attention_fp16_small_weights_count(device, layout, kv, n):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("layout,seqs", [
     ((16, 2, 256), [(1, 1), (2, 1), (33, 1), (200, 1), (777, 1), (3000, 1)]),
-    ((16, 2, 256), [(2, 2), (5, 5), (100, 4), (129, 9), (1000, 16), (64, 3)]),
-    ((32, 8, 128), [(40, 32), (700, 30), (1500, 1)]), ((6, 2, 128), [(3, 3), (900, 10)]),
-    ((8, 8, 64), [(128, 128), (600, 77)]), ((8, 1, 64), [(90, 4), (5000, 1)])])
+    ((16, 2, 256), [(2, 2), (5, 3), (100, 4), (129, 4), (1000, 4), (64, 3)]),
+    ((32, 8, 128), [(40, 8), (700, 7), (1500, 1)]), ((6, 2, 128), [(3, 3), (900, 10)]),
+    ((8, 8, 64), [(32, 32), (600, 27)]), ((8, 1, 64), [(90, 4), (5000, 1)])])
 def test_attention_of_few_rows_is_as_good_as_its_rounding(device, layout, seqs, dtype):
     # A weight is the sum of two 16-bit numbers, the second within half a step
     # of what the first leaves: h^2 of the weight (fp16: 2^-32 of the highest,
@@ -72,7 +72,7 @@ def test_attention_of_few_rows_is_as_good_as_its_rounding(device, layout, seqs, 
     # the result's own rounding, scores, exponentials and sums in fp32.
     c, table, starts, kvs = _case(device, *layout, 16, seqs, dtype, seed=51, gate=True)
     rows = max(n for _, n in seqs)
-    assert rows * (layout[0] // layout[1]) <= 128
+    assert rows * (layout[0] // layout[1]) <= 32
     got = _run_attention(c, max_new=rows)
     D, h = layout[2], ref.half_step(dtype)
     want, spread, score = ref.attention(c["q"], c["k_cache"], c["v_cache"], table, starts, kvs, D ** -0.5, c["gate"])
