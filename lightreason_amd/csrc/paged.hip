@@ -3,7 +3,7 @@
 // rotated keys and values into their slots.
 //
 // The plan is integer work on a few kilobytes: what bounds it is latency (one
-// launch, two dependent round trips to memory: 4.7 us for 4 rows, 6.3 for 1000
+// launch, two dependent round trips to memory: 4-5 us for 4 rows, 6.4 for 1000
 // rows of up to 65 new positions).  Every workgroup scans
 // the per-row counts itself (4096 rows are 16 per thread) instead of handing
 // the scan on through memory, so one launch does the whole plan and no
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void page_release_kernel(PageReleaseArgs 
 // the rotation of the first `rotary` elements (element e of the first half
 // with e + rotary / 2) in fp32, one rounding to the tensor's type at the end.
 // A pass over the data: each row is read once and written once.  What bounds
-// it is HBM bandwidth (8192 tokens of 20 rows of 256: 30.5 us, 4.7 TB/s read
+// it is HBM bandwidth (6827 tokens of 20 rows of 256: 30.4 us, 4.7 TB/s read
 // and written; a device copy reaches 5.2), and in short steps the chain of
 // reads token -> slot and position -> cos and sin (8 tokens: 4.2 us); the rows
 // of a group share that chain, and are all requested before the first is used.
@@ -384,9 +384,9 @@ template <bool FP16, int D>
 static void append_rows(const PagedAppendArgs& a, hipStream_t stream) {
     const int64_t rows = a.heads + 2 * a.kv_heads, per = kThreads / (D / 8);   // groups of a workgroup
     // Four rows per group where that still makes three workgroups per CU (20
-    // rows of 256: 8192 tokens 33.3 us against 38.6 with one row, 2048 tokens
-    // 12.3 against 13.1), else one, where latency counts (1024 tokens 7.8 us
-    // against 8.2 with four, 8 tokens 3.4 against 5.7).
+    // rows of 256: 8192 tokens 32.7 us against 38 with one row, 2048 tokens 12.1
+    // against 13.0), else one, where latency counts (1024 tokens 7.9 us against
+    // 8.4 with four, 8 tokens 3.4 against 5.7).
     const int64_t pieces = (rows + 3) / 4;
     const bool four = a.tokens * pieces >= per * 768;
     const dim3 grid(static_cast<unsigned>((a.tokens * (four ? pieces : rows) + per - 1) / per));

@@ -17,10 +17,13 @@
 // they are, once the values are read in the matching order: the transposing
 // LDS read gives each lane four positions of one element.
 //
-// Keys and values go from the pages into LDS without passing registers, two
-// tiles ahead of their use, and are read from there by all four waves.  Width
-// 256 needs 192 registers per lane for queries and sums alone; what is left of
-// the 256 that two waves per SIMD may have goes to fragments read ahead
+// Keys and values go from the pages into LDS without passing registers.  In
+// tiles of 128 rows all four waves read what they load together, one tile of
+// positions ahead of its use in the other of two buffers; in tiles of 32 a wave
+// has one buffer of keys and one of values, each filled again once it is read,
+// the keys during the product with the values and those during the next keys'.
+// Width 256 needs 192 registers per lane for queries and sums alone; what is
+// left of the 256 that two waves per SIMD may have goes to fragments read ahead
 // (read_ahead), which is why the LDS places (Place) are chosen for few
 // addresses.
 //
@@ -28,12 +31,13 @@
 // new positions over 28003 cached take 1.66 ms, 1.21 PFLOP/s; the matrix units
 // are busy in 67 % of the cycles and the card's power limit holds the clock at
 // 1.4-1.6 GHz then, LDS reads have no bank conflicts.  2048 positions from an
-// empty cache take 73 us, 0.47 PFLOP/s: 59 of attention, where a step's chain
-// (keys, softmax, values) is longer than two waves per SIMD cover and the
-// partial rows' 33 MB leave at the end, 13 of their merge.  One decode
-// position for each of 64 sequences of 200-16000 takes 203 us, 5.4 TB/s of
-// keys and values, the rate of a large copy.  One sequence of 1000 takes 13.9
-// us, a chain of reads (lengths, table, rows, partial rows) in two launches.
+// empty cache take 74 us, 0.46 PFLOP/s: 60 of attention, whose 376 workgroups
+// of 1-34 steps load the CUs unevenly (by the schedule the fullest holds two of
+// 62 steps together, the mean is 32.5, a step of two workgroups takes 1.75 us),
+// 13 of the merge of 33 MB of partial rows.  One decode position for each of 64
+// sequences of 200-16000 takes 203 us, 5.4 TB/s of keys and values, the rate of
+// a large copy.  One sequence of 1000 takes 14.2 us, a chain of reads (lengths,
+// table, rows, partial rows) in two launches.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
@@ -337,7 +341,7 @@ __device__ __forceinline__ void store_gated8(const PagedAttnArgs& a, const RowAt
 template <bool FP16>
 __device__ __forceinline__ void store_row8(const PagedAttnArgs& a, const RowAt& r, int d, const float* v, float l) {
     const uint4 gate = a.gate == nullptr ? make_uint4(0u, 0u, 0u, 0u) : gate_of(a, r, d);
-    const float inv = r.seen > 0 ? __builtin_amdgcn_rcpf(l) : 0.0f;
+    const float inv = r.seen > 0 ? __builtin_amdgcn_rcpf(l) : 0.0f;   // (an ulp, as in sigmoid)
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = v[k] * inv;
@@ -558,7 +562,7 @@ constexpr float kBelow = FP16 ? 7.0f : 0.0f;
 constexpr float kRounded = 4194304.0f;
 
 // WQ waves of 32 rows each over the same tiles of 32 NB positions, which they
-// load together, two in flight (eight waves on one tile instead of two
+// load together, the next one in flight (eight waves on one tile instead of two
 // workgroups of four per CU took 2.03 ms where these took 1.82: their barriers
 // keep them in step), or WK waves that share 32 rows and take tiles of their
 // own.
