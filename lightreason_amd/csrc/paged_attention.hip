@@ -36,7 +36,7 @@
 // 62 steps together, the mean is 32.5, a step of two workgroups takes 1.75 us),
 // 13 of the merge of 33 MB of partial rows.  One decode position for each of 64
 // sequences of 200-16000 takes 203 us, 5.4 TB/s of keys and values, the rate of
-// a large copy.  One sequence of 1000 takes 14.2 us, a chain of reads (lengths,
+// a large copy.  One sequence of 1000 takes 14.3 us, a chain of reads (lengths,
 // table, rows, partial rows) in two launches.
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
@@ -64,7 +64,8 @@ __device__ __forceinline__ void wave_lds_fence() {
 // positions that the row sees: a lane per position for the scores (64 at a
 // time), a lane per D / 64 elements for the values.  The path of rows whose
 // tile holds values that are not finite and that some of its rows do not see
-// (in a tile's matrix product their zero weights would not hide them).
+// (in a tile's matrix product their zero weights would not hide them), and of
+// sums over weights in two parts that are not finite.
 template <bool FP16, int D>
 __device__ void attend_row(const PagedAttnArgs& a, int b, int64_t t, int64_t h, int64_t seen, float* qs, float* ps,
                            int64_t* vs) {
@@ -542,7 +543,7 @@ struct Partials {
     float* o;       // [slot][BM][D] sums of exp2(s - m) v
     float* ml;      // [slot][BM][2] m, sum of exp2(s - m)
     Piece* pieces;  // [tiles]
-    int* dirty;     // [workgroups of the attention launch]: the split holds values that some of its rows must not see
+    int* dirty;     // [workgroups of the attention launch]: the split's rows are to be recomputed one by one
     int tiles, workgroups;
 };
 
@@ -580,8 +581,8 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     constexpr int KS = D / 16, DB = D / 32;
     // 16-bit numbers that make up a weight in the second product.  Two where few
     // rows share keys and values: HBM sets the pace, the further products are
-    // nearly free (one sequence of 1000 positions 13.5 -> 13.65 us, 64 of
-    // 200-16000 202.0 -> 202.5) and the result is as far from 64 bits as its own
+    // nearly free (one sequence of 1000 positions 13.5 -> 13.75 us, 64 of
+    // 200-16000 201.8 -> 202.4) and the result is as far from 64 bits as its own
     // rounding is (bf16: 1.7e-3; 2.1e-3 to 2.3e-3 with one).  Tiles of 128 rows
     // are bound by the products or by the chain of a step, and round a weight
     // once, as the Transformers forward does (two: 16 verify blocks 37.5 -> 38.9
@@ -891,6 +892,10 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
         for (int w = 0; w < WK; ++w) top = __builtin_fmaxf(top, ml[(w * 32 + q) * 2]);
         const float fall = __builtin_amdgcn_exp2f(m - top);
+        // Sums that are not finite though the weights' is: the second part of a
+        // weight may turn an infinite value's product with the first into NaN,
+        // so the merge launch recomputes these rows too.
+        bool lost = false;
         for (int r0 = 0; r0 < rows; r0 += ROOM) {
             if (r0 > 0) __syncthreads();
             if (q >= r0 && q < min(rows, r0 + ROOM)) {
@@ -917,6 +922,9 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                     rl += ml[(w * 32 + r0 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r0 + r) * 2] - rm);
+                const bool weighs = __builtin_fabsf(rl) < __builtin_inff();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) lost |= weighs && !(__builtin_fabsf(v[k]) < __builtin_inff());
                 if (splits > 1) {
                     const int64_t at = slot * BM + r0 + r;
                     *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -927,6 +935,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 }
             }
         }
+        if (lost && !any_bad) part.dirty[blockIdx.x] = 1;   // (thread 0's store came before the barriers above)
     } else if (!works) {
     } else if (splits > 1) {
         // Partial rows as the lanes hold them: 1 KB per store.

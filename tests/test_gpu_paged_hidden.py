@@ -58,3 +58,24 @@ def test_attention_rows_that_see_a_value_that_is_not_finite(device, bad, layout)
         assert bool(((out.double() - want).abs() <= bound)[ok].all())
         if where == "v":
             c["v_cache"][page, :, 150 % 16, 5] = 1.0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("layout,seqs", [((16, 2, 256), [(230, 1), (64, 1), (5000, 2)]), ((8, 2, 64), [(90, 4), (3, 3)]),
+                                         ((32, 8, 128), [(700, 1), (300, 8)]), ((16, 2, 256), [(230, 20), (700, 1)])])
+def test_attention_infinite_values_that_a_row_sees(device, dtype, layout, seqs):
+    # A visible infinite value times a weight is infinite, as in the formula.
+    c, table, starts, kvs = _case(device, *layout, 16, seqs, dtype, seed=29, gate=True)
+    for s, (kv, n) in enumerate(seqs):
+        for p in {0, (kv - n) // 2, kv - n}:
+            row = c["v_cache"][table[s][p // 16], :, p % 16]
+            row[:, 5], row[:, 9], row[:, 11] = math.inf, -math.inf, math.nan
+    out = _run_attention(c, max_new=max(n for _, n in seqs))
+    want, spread, score = ref.attention(c["q"], c["k_cache"], c["v_cache"], table, starts, kvs, layout[2] ** -0.5,
+                                        c["gate"])
+    top = float(c["v_cache"][torch.isfinite(c["v_cache"])].abs().max())
+    bound = ref.attention_bound(want, spread, score, dtype, layout[2], max(kvs), top)
+    ok = torch.isfinite(want)
+    assert bool((~ok).any()) and torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out.double()[torch.isinf(want)], want[torch.isinf(want)])
+    assert bool(((out.double() - want).abs() <= bound)[ok].all())
