@@ -270,8 +270,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     row ``positions[t]``, or row t), all in fp32 and rounded once.  Inputs and
     caches may be strided views with a contiguous last dimension (the 35B
     model's q and gate come interleaved from one projection).  A token whose
-    slot lies outside the pool (-1: padding) is left out, its q_out row too;
-    tokens must not share a slot.  ``q_out`` may be a contiguous ``q`` itself;
+    slot lies outside the pool (-1: padding) is left out, its q_out row too
+    (whatever memory held where q_out is not given); tokens must not share a
+    slot.  ``q_out`` may be a contiguous ``q`` itself;
     else it shares no element with ``q``, ``k`` or ``v`` (refused), nor the
     caches with each other or an input."""
     tensors = (k, v, k_cache, v_cache, slots, q, q_norm, k_norm, cos, sin, positions, q_out)
@@ -375,8 +376,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     what a row does not see cannot change it (infinities and NaN no more than
     its last bits: rows next to some that see such values are summed in
     another order);
-    tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``,
-    and all do when ``starts`` are not ascending within [0, tokens].  A table
+    tokens outside starts[0] .. starts[seqs] - 1 stay as they were in ``out``
+    (whatever memory held where it is not given), and all do when ``starts`` are not ascending within [0, tokens].  A table
     entry in use outside the pool makes its sequence's rows NaN (those of
     earlier positions may keep their values).  ``out`` may share a buffer with
     ``q`` and ``gate`` but no element with them or between its own rows
