@@ -506,9 +506,9 @@ int lrmoe_attn_decode_step(const uint16_t *residual, int tokens, const uint16_t 
  * the device and owned by the caller: table [rows][max_pages] int32 (a row's
  * pages in order), held [rows] int32 (pages of each row), lengths [rows] int32
  * (cached positions), free_pages [pages] int32 (a stack), state [4] int32 =
- * (free pages, epoch, status bits, plans made in this epoch).  A slot is page * page_size + row in the
- * page.  No reference counterpart: the reference serves one sequence on the
- * Transformers cache. */
+ * (free pages, epoch, status bits, plans made in this epoch).  A slot is page *
+ * page_size + row in the page.  No reference counterpart: the reference serves
+ * one sequence on the Transformers cache. */
 #define LRMOE_PAGE_MAX_ROWS 4096
 #define LRMOE_PAGE_MAX_POSITIONS (1 << 30) /* most of max_pages * page: positions that a row can hold */
 #define LRMOE_PAGE_STATUS_TOKENS 1  /* a negative count, or more new positions than `tokens` */
@@ -603,11 +603,11 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
  * when a gate is given; softmax and sums in fp32, the weights of the product
  * with v rounded to the tensors' type, or to two numbers of it where max_new *
- * heads / kv_heads is at most 32.  A row that sees nothing
- * (kv_lengths[s] < n) is 0, one that sees only scores of -inf is NaN.  What a
- * row does not see cannot change it (infinities and NaN no more than its last
- * bits: rows next to some that see such values are summed in another order).  Tokens
- * outside starts[0] .. starts[seqs] - 1 are left as they were, and all are
+ * heads / kv_heads is at most 32.  A row that sees nothing (kv_lengths[s] < n)
+ * is 0, one that sees only scores of -inf is NaN.  What a row does not see
+ * cannot change it (infinities and NaN no more than its last bits: rows next to
+ * some that see such values are summed in another order).  Tokens outside
+ * starts[0] .. starts[seqs] - 1 are left as they were, and all are
  * when starts are not ascending within [0, tokens].  A table entry outside
  * [0, pages) in use makes its sequence's rows NaN (those of earlier positions
  * may keep their values); kv_lengths beyond max_pages pages are cut there.

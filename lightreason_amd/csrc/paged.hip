@@ -4,13 +4,17 @@
 //
 // The plan is integer work on a few kilobytes: what bounds it is latency (one
 // launch, two dependent round trips to memory: 4-5 us for 4 rows, 6.4 for 1000
-// rows of up to 65 new positions).  Every workgroup scans
-// the per-row counts itself (4096 rows are 16 per thread) instead of handing
-// the scan on through memory, so one launch does the whole plan and no
-// workgroup waits for another.  The plan changes nothing that rows hold: it
-// writes its own outputs, its number, and table entries past the rows' held
-// pages.  Those are read by the step's attention and kept by its commit, so
-// only the plan that wrote them last can be committed.
+// rows of up to 65 new positions).  Every workgroup scans the per-row counts
+// itself (4096 rows are 16 per thread) instead of handing the scan on through
+// memory, so one launch does the whole plan and no workgroup waits for another.
+// The plan changes nothing that rows hold: it writes its own outputs, its
+// number, and table entries past the rows' held pages.  Those are read by the
+// step's attention and kept by its commit, so only the plan that wrote them
+// last can be committed.
+//
+// Commit and release run in one workgroup: a plan with its commit takes 4.4 us
+// for 4 rows, 8 for 1000 and 29 for 4096; a release 2.4 us for 268 pages, 11
+// for 4288, 218 for 67,000 (a page per thread at a time; rows end seldom).
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
