@@ -602,8 +602,8 @@ int lrmoe_paged_append(const lrmoe_paged_append_args *args, void *stream);
  * starts[s] .. starts[s + 1] - 1, n in all) sees cached positions 0 ..
  * kv_lengths[s] - n + t; out = softmax(scale q . k) v, times sigmoid(gate)
  * when a gate is given; softmax and sums in fp32, the weights of the product
- * with v rounded to the tensors' type, or to two numbers of it where max_new *
- * heads / kv_heads is at most 32.  A row that sees nothing (kv_lengths[s] < n)
+ * with v rounded to the tensors' type, or (bf16) split into two numbers of it
+ * where max_new * heads / kv_heads is at most 32.  A row that sees nothing (kv_lengths[s] < n)
  * is 0, one that sees only scores of -inf is NaN.  What a row does not see
  * cannot change it (infinities and NaN no more than its last bits: rows next to
  * some that see such values are summed in another order).  Tokens outside

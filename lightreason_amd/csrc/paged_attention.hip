@@ -64,8 +64,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 // positions that the row sees: a lane per position for the scores (64 at a
 // time), a lane per D / 64 elements for the values.  The path of rows whose
 // tile holds values that are not finite and that some of its rows do not see
-// (in a tile's matrix product their zero weights would not hide them), and of
-// sums over weights in two parts that are not finite.
+// (in a tile's matrix product their zero weights would not hide them).
 template <bool FP16, int D>
 __device__ void attend_row(const PagedAttnArgs& a, int b, int64_t t, int64_t h, int64_t seen, float* qs, float* ps,
                            int64_t* vs) {
@@ -543,7 +542,7 @@ struct Partials {
     float* o;       // [slot][BM][D] sums of exp2(s - m) v
     float* ml;      // [slot][BM][2] m, sum of exp2(s - m)
     Piece* pieces;  // [tiles]
-    int* dirty;     // [workgroups of the attention launch]: the split's rows are to be recomputed one by one
+    int* dirty;     // [workgroups of the attention launch]: the split holds values that some of its rows must not see
     int tiles, workgroups;
 };
 
@@ -579,16 +578,17 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     constexpr int KTILE = KP::bytes(KT), VTILE = VP::bytes(KT);   // bytes of a tile of keys, of values
     constexpr int STAGES = WK == 1 ? 2 : 1;
     constexpr int KS = D / 16, DB = D / 32;
-    // 16-bit numbers that make up a weight in the second product.  Two where few
-    // rows share keys and values: HBM sets the pace, the further products are
-    // nearly free (one sequence of 1000 positions 13.5 -> 13.75 us, 64 of
-    // 200-16000 201.8 -> 202.4) and the result is as far from 64 bits as its own
-    // rounding is (bf16: 1.7e-3; 2.1e-3 to 2.3e-3 with one).  Tiles of 128 rows
-    // are bound by the products or by the chain of a step, and round a weight
-    // once, as the Transformers forward does (two: 16 verify blocks 37.5 -> 38.9
-    // us, 33.8 -> 38.7 with their keys cached; 2048 positions 68 -> 91 us; 4096
-    // over 28003 1.66 -> 2.38 ms).
-    constexpr int PARTS = WK == 1 ? 1 : 2;
+    // 16-bit numbers that make up a weight in the second product.  Two for bf16
+    // where few rows share keys and values: HBM sets the pace, the further
+    // products are nearly free (one sequence of 1000 positions 13.5 -> 13.7 us,
+    // 64 of 200-16000 201.8 -> 202.4) and the result is as far from 64 bits as
+    // its own rounding is (1.7e-3; 2.1e-3 to 2.3e-3 with one).  fp16 keeps three
+    // more bits in one (2.9e-4 against 2.1e-4).  Tiles of 128 rows are bound by
+    // the products or by the chain of a step, and round a weight once, as the
+    // Transformers forward does (two: 16 verify blocks 37.5 -> 38.9 us, 33.8 ->
+    // 38.7 with their keys cached; 2048 positions 68 -> 91 us; 4096 over 28003
+    // 1.66 -> 2.38 ms).
+    constexpr int PARTS = WK > 1 && !FP16 ? 2 : 1;
     constexpr int ROWS = WK == 1 ? KT / WQ : KT;   // rows that a wave stages
     constexpr int LOADS = ROWS * D / 512;          // of a key or value tile, per wave
     constexpr int LDS = STAGES * WK * (KTILE + VTILE);
@@ -712,7 +712,7 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
     // they are: of a step of 16 positions lane (q, hi) holds 4 hi + {0..3,
     // 8..11}.  The product takes 16-bit operands, so the weights are rounded to
     // the tensors' type, or split into two numbers of it, the second what the
-    // first leaves (16 bits and more of each weight); their sum is not rounded.
+    // first leaves (15 bits and more of each weight); their sum is not rounded.
     auto scores = [&](uint32_t kt, int base, uint4 (&pw)[2 * NB * PARTS]) {
         f32x16 s[NB] = {};
 #pragma unroll
@@ -778,14 +778,24 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                     w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][8 * k + j], factor, -off));
                     sum += w[j];
                 }
-                const uint4 high = pack16<FP16>(w);
-                pw[(2 * nb + k) * PARTS] = high;
-                if constexpr (PARTS > 1) {
-                    float x[8];
-                    unpack16<FP16>(high, x);
+                if constexpr (PARTS == 1) {
+                    pw[2 * nb + k] = pack16<FP16>(w);
+                } else {
+                    // The upper half of the weight's bits, and what that leaves,
+                    // kept above 0 with the weight: an infinite value's two
+                    // products then have one sign, and a weight of 0 has none.
+                    uint32_t high[4];
+                    float rest[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = w[j] - x[j];
-                    pw[(2 * nb + k) * PARTS + 1] = pack16<FP16>(x);
+                    for (int j = 0; j < 8; ++j)
+                        rest[j] = __builtin_amdgcn_fmed3f(
+                            w[j] - __uint_as_float(__float_as_uint(w[j]) & 0xffff0000u), 1.17549435e-38f, w[j]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        high[j] = __builtin_amdgcn_perm(__float_as_uint(w[2 * j + 1]), __float_as_uint(w[2 * j]),
+                                                        0x07060302u);
+                    pw[4 * nb + 2 * k] = make_uint4(high[0], high[1], high[2], high[3]);
+                    pw[4 * nb + 2 * k + 1] = pack16<false>(rest);
                 }
             }
         l += sum;
@@ -892,10 +902,6 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
         for (int w = 0; w < WK; ++w) top = __builtin_fmaxf(top, ml[(w * 32 + q) * 2]);
         const float fall = __builtin_amdgcn_exp2f(m - top);
-        // Sums that are not finite though the weights' is: the second part of a
-        // weight may turn an infinite value's product with the first into NaN,
-        // so the merge launch recomputes these rows too.
-        bool lost = false;
         for (int r0 = 0; r0 < rows; r0 += ROOM) {
             if (r0 > 0) __syncthreads();
             if (q >= r0 && q < min(rows, r0 + ROOM)) {
@@ -922,9 +928,6 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                     rl += ml[(w * 32 + r0 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r0 + r) * 2] - rm);
-                const bool weighs = __builtin_fabsf(rl) < __builtin_inff();
-#pragma unroll
-                for (int k = 0; k < 8; ++k) lost |= weighs && !(__builtin_fabsf(v[k]) < __builtin_inff());
                 if (splits > 1) {
                     const int64_t at = slot * BM + r0 + r;
                     *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -935,7 +938,6 @@ __global__ __launch_bounds__(kWave * WQ * WK, (WK > 1 && D == 256) ? 1 : 2) void
                 }
             }
         }
-        if (lost && !any_bad) part.dirty[blockIdx.x] = 1;   // (thread 0's store came before the barriers above)
     } else if (!works) {
     } else if (splits > 1) {
         // Partial rows as the lanes hold them: 1 KB per store.

@@ -368,11 +368,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     kv_heads); ``scale`` defaults to dim ** -0.5.  With ``gate`` [tokens,
     heads, dim] the result is multiplied by sigmoid(gate).
 
-    Softmax and sums are in fp32.  Where ``max_new * heads // kv_heads`` is at
-    most 32 (decode and short verify steps) the weights meet the values as two
-    numbers of the tensors' type, so the result is as good as its own rounding;
-    in longer steps they are rounded to the tensors' type, as in the
-    Transformers forward.  A row that sees nothing is 0;
+    Softmax and sums are in fp32.  The weights are rounded to the tensors' type
+    before they meet the values, as in the Transformers forward; bf16 ones meet
+    them as two bf16 numbers where ``max_new * heads // kv_heads`` is at most 32
+    (decode and short verify steps), so that the result is as good as its own
+    rounding.  A row that sees nothing is 0;
     what a row does not see cannot change it (infinities and NaN no more than
     its last bits: rows next to some that see such values are summed in
     another order);
