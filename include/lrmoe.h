@@ -664,6 +664,97 @@ int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t
                         const float *uniforms, const float *samples, int32_t *accepted, int64_t *next,
                         void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- the recurrent layers over packed sequences ----------------------------- */
+
+/* The gated delta rule over packed sequences, the recurrence of
+ * edge35b/delta_decode.py:11-36 (_delta) in fp32: for sequence s (tokens
+ * starts[s] .. starts[s + 1] - 1) and value head h, with the state S [dim]
+ * [value_dim] of its slot,
+ *     S *= exp(g);  u = beta (v - S^T k);  S += k u^T;  out = scale S^T q,
+ * q and k of key head h / (heads / key_heads), divided by sqrt(sum x^2 + 1e-6)
+ * with normalize.  Nothing is rounded but out.  initial [pool][heads][dim]
+ * [value_dim] fp32 is read at slot slots[s] (NULL: s), or is zero where it
+ * is NULL or fresh[s] != 0; final, of the same shape, is written at into[s]
+ * (NULL: s).  initial may be final, and a sequence's slots the same; no two
+ * sequences write one slot, and none writes a slot that another reads.  A
+ * sequence without tokens passes its state on.  One whose slot lies outside the
+ * pool is left out, its rows too; one whose starts are not in order within
+ * [0, tokens] counts as empty.  Rows outside starts[0] .. starts[seqs] - 1 stay
+ * as they were, or are set to 0 with clear.  What is not finite reaches later
+ * tokens of its sequence only.  max_new only chooses the kernel: at least every
+ * sequence's count where they are short.  Strides in elements, those of q, k, v
+ * and out multiples of 8 (4 for out) with the last dimension contiguous; q, k,
+ * v 16-byte and out 8-byte aligned; out shares no element with q, k and v
+ * (refused) or anything else that is read.  dim 64 or 128, value_dim a multiple
+ * of 32 up to 256, at most 2^20 tokens, 65536 sequences and tokens * heads of
+ * 2^26.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes, 256-byte
+ * aligned, not cleared, used by one stream at a time. */
+typedef struct lrmoe_delta_scan_args {
+    int32_t seqs, tokens, max_new, heads, key_heads, dim, value_dim, fp16;
+    int32_t normalize, beta_fp32, clear, pool;
+    float scale;
+    int32_t pad;
+    const void *q, *k, *v;                /* [tokens][key_heads][dim] twice, [tokens][heads][value_dim] */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const void *g, *beta;                 /* [tokens][heads]: log decay fp32; fp32 or of the tensors' type */
+    int64_t g_token_stride, beta_token_stride;
+    const int32_t *starts, *slots, *into; /* [seqs + 1], [seqs], [seqs] */
+    const void *fresh;                    /* [seqs] uint8, may be NULL */
+    const void *initial;
+    void *final, *out;                    /* out [tokens][heads][value_dim] */
+    int64_t out_token_stride, out_head_stride;
+} lrmoe_delta_scan_args;
+size_t lrmoe_delta_scan_workspace_bytes(const lrmoe_delta_scan_args *args);
+int lrmoe_delta_scan(const lrmoe_delta_scan_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- beam search -------------------------------------------------------------
+ *
+ * No reference counterpart (the reference decodes greedily). */
+
+/* The best continuations of `groups` groups of `beams` beams: row g beams + w of
+ * logits [groups * beams][vocab] (row stride `stride` elements; type 0 fp32, 1
+ * bf16, 2 fp16) holds beam w's next-token logits x, scores its score s; its
+ * continuation by token t has s + x_t - log sum exp x.  Logits that are not
+ * finite take no part; neither does a beam whose score is not finite; a beam
+ * with finished (uint8, may be NULL) != 0 has one continuation, itself, with
+ * token -1 and its score.  Of a group's continuations the `beams` best are kept
+ * (ties: lowest beam, then lowest token).  A beam's best one that is kept takes
+ * the beam's own row, the others in order of their scores the rows left over,
+ * lowest first, so that rows whose parent is another are those that died: their
+ * states and pages may be overwritten by the parents' (lrmoe_fork_rows,
+ * lrmoe_page_fork).  Rows without a continuation have token -1, their own row
+ * as parent and score -inf.  Sums are joined and scores compared in 64 bits.
+ * scores_out may be scores; beams 1..32, groups * beams at most 65535.
+ * Workspace of lrmoe_beam_workspace_bytes bytes, 16-byte aligned. */
+#define LRMOE_BEAM_MAX 32
+size_t lrmoe_beam_workspace_bytes(int groups, int beams, int vocab);
+int lrmoe_beam_select(int groups, int beams, int vocab, int type, const void *logits, int64_t stride,
+                      const float *scores, const uint8_t *finished, int64_t *tokens, int32_t *parents,
+                      float *scores_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Row r of every tensor becomes a copy of row parents[r].  A row that is its own
+ * parent stays; so does one whose parent lies outside [0, rows) or is not its
+ * own parent (nothing that is read is written).  tensors (on the host, as its
+ * numbers) holds a base address, the rows' stride and the bytes of a row, three
+ * int64 per tensor; at most LRMOE_FORK_TENSORS of them. */
+#define LRMOE_FORK_TENSORS 64
+int lrmoe_fork_rows(int rows, const int32_t *parents, int tensors, const int64_t *table, void *stream);
+
+/* Row r of a page pool takes over the cached positions of row parents[r] where
+ * that is another row (one that is its own parent): its length becomes the
+ * parent's, it gets the fresh pages that needs (from the top of the free stack,
+ * rows in order) and, in every cache, its pages the parent's contents; pages it
+ * holds beyond those stay held.  The epoch goes up by one.  All or nothing: with
+ * a parent outside [0, rows), one that is not its own, bad lengths or too few
+ * free pages only state's status bits change.  caches (on the host) holds for
+ * each of up to LRMOE_FORK_CACHES caches of 16-byte aligned rows: base address,
+ * layers, heads, bytes of a row, then the strides of a layer, a page, a head and
+ * a row in bytes, eight int64 each.  scratch holds rows + 1 int32. */
+#define LRMOE_FORK_CACHES 32
+int lrmoe_page_fork(int rows, int pages, int page, int max_pages, const int32_t *parents, int32_t *table,
+                    int32_t *lengths, int32_t *held, const int32_t *free_pages, int32_t *state, int caches,
+                    const int64_t *cache_table, int32_t *scratch, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,12 @@ _SIGNATURES = {
     "lrmoe_paged_append": ([_P, _P], _I),
     "lrmoe_paged_attention_workspace_bytes": ([_P], C.c_size_t),
     "lrmoe_paged_attention": ([_P, _P, C.c_size_t, _P], _I),
+    "lrmoe_page_fork": ([_I] * 4 + [_P] * 6 + [_I] + [_P] * 3, _I),
+    "lrmoe_delta_scan_workspace_bytes": ([_P], C.c_size_t),
+    "lrmoe_delta_scan": ([_P, _P, C.c_size_t, _P], _I),
+    "lrmoe_beam_workspace_bytes": ([_I] * 3, C.c_size_t),
+    "lrmoe_beam_select": ([_I] * 4 + [_P, C.c_int64] + [_P] * 6 + [C.c_size_t, _P], _I),
+    "lrmoe_fork_rows": ([_I, _P, _I, _P, _P], _I),
     "lrmoe_verify_workspace_bytes": ([_I, _I], C.c_size_t),
     "lrmoe_verify_drafts": ([_I] * 4 + [_P, _P, C.c_int64, _P, C.c_int64] + [_P] * 6 + [C.c_size_t, _P], _I),
 }
@@ -113,6 +119,19 @@ class PagedAttentionArgs(C.Structure):
         "p: table starts kv_lengths out; l: out_token_stride out_head_stride")
 
 
+class DeltaScanArgs(C.Structure):
+    """lrmoe_delta_scan_args."""
+
+    _fields_ = _fields(
+        "i: seqs tokens max_new heads key_heads dim value_dim fp16 normalize beta_fp32 clear pool; f: scale; i: pad;"
+        "p: q k v; l: q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride;"
+        "p: g beta; l: g_token_stride beta_token_stride; p: starts slots into fresh initial final out;"
+        "l: out_token_stride out_head_stride")
+
+
+BEAM_MAX = 32            # beams of a group
+FORK_TENSORS = 64        # tensors of one lrmoe_fork_rows call
+FORK_CACHES = 32         # caches of one lrmoe_page_fork call
 PAGE_MAX_ROWS = 4096     # rows (sequences) of a page pool
 PAGE_MAX_POSITIONS = 1 << 30  # max_pages * page at most
 PAGE_STATUS_TOKENS = 1   # a negative count, or more new positions than the plan has room for

@@ -6,7 +6,9 @@
 #include <mutex>
 
 #include "lrmoe_internal.h"
+#include "beam.h"
 #include "paged.h"
+#include "scan.h"
 
 namespace {
 
@@ -982,6 +984,194 @@ int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t
     lrmoe::VerifyArgs a{blocks,  rows,     vocab,    tokens, target, draft, target_stride, draft_stride,
                         starts,  uniforms, samples,  accepted, next, static_cast<double*>(workspace)};
     return status_of(lrmoe::launch_verify_drafts(a, type, as_stream(stream)));
+}
+
+// ---- recurrent layers over packed sequences -------------------------------------
+
+static bool bad_scan(const lrmoe_delta_scan_args* p) {
+    return p->seqs < 0 || p->seqs > 65536 || p->tokens < 0 || p->tokens > (1 << 20) || p->max_new < 0 || p->heads < 1 ||
+           p->heads > 1024 || p->key_heads < 1 || p->heads % p->key_heads != 0 || (p->dim != 64 && p->dim != 128) ||
+           p->value_dim < 32 || p->value_dim > 256 || p->value_dim % 32 != 0 || p->pool < 0 ||
+           static_cast<int64_t>(p->tokens) * p->heads > (1 << 26);
+}
+
+static lrmoe::ScanArgs scan_args(const lrmoe_delta_scan_args* p) {
+    lrmoe::ScanArgs a{};
+    a.seqs = p->seqs;
+    a.tokens = p->tokens;
+    a.heads = p->heads;
+    a.key_heads = p->key_heads;
+    a.group = p->heads / p->key_heads;
+    a.dim = p->dim;
+    a.value_dim = p->value_dim;
+    a.pool = p->pool;
+    a.normalize = p->normalize;
+    a.beta_fp32 = p->beta_fp32;
+    a.clear = p->clear;
+    a.scale = p->scale;
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.k = static_cast<const uint16_t*>(p->k);
+    a.v = static_cast<const uint16_t*>(p->v);
+    a.q_token = p->q_token_stride;
+    a.q_head = p->q_head_stride;
+    a.k_token = p->k_token_stride;
+    a.k_head = p->k_head_stride;
+    a.v_token = p->v_token_stride;
+    a.v_head = p->v_head_stride;
+    a.g = static_cast<const float*>(p->g);
+    a.beta = p->beta;
+    a.g_token = p->g_token_stride;
+    a.beta_token = p->beta_token_stride;
+    a.starts = p->starts;
+    a.from = p->slots;
+    a.into = p->into;
+    a.fresh = static_cast<const uint8_t*>(p->fresh);
+    a.initial = static_cast<const float*>(p->initial);
+    a.final = static_cast<float*>(p->final);
+    a.out = static_cast<uint16_t*>(p->out);
+    a.out_token = p->out_token_stride;
+    a.out_head = p->out_head_stride;
+    return a;
+}
+
+size_t lrmoe_delta_scan_workspace_bytes(const lrmoe_delta_scan_args* p) {
+    if (!p || bad_scan(p)) return 0;
+    return lrmoe::delta_scan_workspace_bytes(scan_args(p), p->fp16 != 0, p->max_new);
+}
+
+// What forward and gradient ask of a call's inputs.
+static bool bad_scan_inputs(const lrmoe_delta_scan_args* p) {
+    if (p->tokens > 0 && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return true;
+    if (!p->starts || misaligned(p->q, 16) || misaligned(p->k, 16) || misaligned(p->v, 16) || misaligned(p->g, 4) ||
+        misaligned(p->beta, p->beta_fp32 ? 4 : 2) || misaligned(p->starts, 4) || misaligned(p->slots, 4) ||
+        misaligned(p->into, 4) || misaligned(p->initial, 16))
+        return true;
+    for (int64_t x : {p->q_token_stride, p->q_head_stride, p->k_token_stride, p->k_head_stride, p->v_token_stride,
+                      p->v_head_stride})
+        if (x % 8 != 0) return true;
+    // Rows are addressed within 2^31 bytes of a chunk's first.
+    for (int64_t x : {p->q_token_stride, p->k_token_stride, p->v_token_stride})
+        if (x < 0 || x >= (1 << 23)) return true;
+    return false;
+}
+
+int lrmoe_delta_scan(const lrmoe_delta_scan_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!p || bad_scan(p)) return LRMOE_E_ARG;
+    if (p->seqs == 0) return LRMOE_OK;
+    if (bad_scan_inputs(p) || !p->final || (p->tokens > 0 && !p->out) || misaligned(p->final, 16) ||
+        misaligned(p->out, 8) || p->out_token_stride % 4 != 0 || p->out_head_stride % 4 != 0 || misaligned(workspace, 256))
+        return LRMOE_E_ARG;
+    const size_t need = lrmoe_delta_scan_workspace_bytes(p);
+    if (need > 0 && !workspace) return LRMOE_E_ARG;
+    if (workspace_bytes < need) return LRMOE_E_WORKSPACE;
+    if (p->tokens > 0) {
+        const int64_t wide = std::max(p->dim, p->value_dim);
+        const HeadRows out{p->out, p->out_token_stride, p->out_head_stride, p->heads};
+        auto meets = [&](const void* base, int64_t token, int64_t head, int heads, int64_t dim) {
+            // (Rows of two widths: as pieces of 32 elements, which both are made of.)
+            if (dim == p->value_dim) return share_elements(out, {base, token, head, heads}, p->tokens, dim);
+            for (int64_t i = 0; i < wide; i += 32)
+                for (int64_t j = 0; j < wide; j += 32)
+                    if (i < p->value_dim && j < dim &&
+                        share_elements({static_cast<const uint16_t*>(p->out) + i, out.token, out.head, out.heads},
+                                       {static_cast<const uint16_t*>(base) + j, token, head, heads}, p->tokens, 32))
+                        return true;
+            return false;
+        };
+        if (meets(p->q, p->q_token_stride, p->q_head_stride, p->key_heads, p->dim) ||
+            meets(p->k, p->k_token_stride, p->k_head_stride, p->key_heads, p->dim) ||
+            meets(p->v, p->v_token_stride, p->v_head_stride, p->heads, p->value_dim) ||
+            (!nested_rows(out, p->tokens, p->value_dim) && share_elements(out, out, p->tokens, p->value_dim, true)))
+            return LRMOE_E_ARG;
+    }
+    if (int d = check_device()) return d;
+    return status_of(lrmoe::launch_delta_scan(scan_args(p), p->fp16 != 0, p->max_new, workspace, as_stream(stream)));
+}
+
+// ---- beam search ------------------------------------------------------------------
+
+static bool bad_beams(int groups, int beams, int vocab) {
+    return groups < 0 || beams < 1 || beams > LRMOE_BEAM_MAX || static_cast<int64_t>(groups) * beams > 65535 ||
+           vocab < 1 || vocab > (1 << 30);
+}
+
+size_t lrmoe_beam_workspace_bytes(int groups, int beams, int vocab) {
+    if (bad_beams(groups, beams, vocab)) return 0;
+    return lrmoe::beam_workspace_bytes(groups, beams, vocab);
+}
+
+int lrmoe_beam_select(int groups, int beams, int vocab, int type, const void* logits, int64_t stride,
+                      const float* scores, const uint8_t* finished, int64_t* tokens, int32_t* parents,
+                      float* scores_out, void* workspace, size_t workspace_bytes, void* stream) {
+    if (bad_beams(groups, beams, vocab) || type < 0 || type > 2) return LRMOE_E_ARG;
+    if (groups == 0) return LRMOE_OK;
+    if (!logits || stride < vocab || !scores || !tokens || !parents || !scores_out || !workspace ||
+        misaligned(logits, type == 0 ? 4 : 2) || misaligned(workspace, 16))
+        return LRMOE_E_ARG;
+    if (workspace_bytes < lrmoe::beam_workspace_bytes(groups, beams, vocab)) return LRMOE_E_WORKSPACE;
+    if (int d = check_device()) return d;
+    lrmoe::BeamArgs a{groups, beams, vocab, logits, stride, scores, finished, tokens, parents, scores_out, nullptr,
+                      nullptr};
+    return status_of(lrmoe::launch_beam_select(a, type, workspace, as_stream(stream)));
+}
+
+int lrmoe_fork_rows(int rows, const int32_t* parents, int tensors, const int64_t* table, void* stream) {
+    if (rows < 0 || rows > (1 << 24) || tensors < 0 || tensors > LRMOE_FORK_TENSORS) return LRMOE_E_ARG;
+    if (rows == 0 || tensors == 0) return LRMOE_OK;
+    if (!parents || !table) return LRMOE_E_ARG;
+    lrmoe::ForkRowsArgs a{};
+    a.rows = rows;
+    a.tensors = tensors;
+    a.parents = parents;
+    for (int i = 0; i < tensors; ++i) {
+        const int64_t base = table[3 * i], stride = table[3 * i + 1], bytes = table[3 * i + 2];
+        // Rows lie behind one another, and their pieces can be counted.
+        if ((base == 0 && bytes > 0) || bytes < 0 || bytes > (INT64_C(1) << 40) || (rows > 1 && stride < bytes)) return LRMOE_E_ARG;
+        a.t[i] = {reinterpret_cast<uint8_t*>(base), stride, bytes, 0, 0};
+    }
+    int64_t pieces = 0;
+    for (int i = 0; i < tensors; ++i) pieces += ((a.t[i].bytes + 32767) / 32768) * rows;
+    if (pieces > 0x7fffffff) return LRMOE_E_ARG;
+    if (int d = check_device()) return d;
+    return status_of(lrmoe::launch_fork_rows(a, as_stream(stream)));
+}
+
+int lrmoe_page_fork(int rows, int pages, int page, int max_pages, const int32_t* parents, int32_t* table,
+                    int32_t* lengths, int32_t* held, const int32_t* free_pages, int32_t* state, int caches,
+                    const int64_t* cache_table, int32_t* scratch, void* stream) {
+    if (bad_pool(rows, pages, max_pages) || bad_page(page) || bad_capacity(max_pages, page) || caches < 0 ||
+        caches > LRMOE_FORK_CACHES)
+        return LRMOE_E_ARG;
+    if (rows == 0) return LRMOE_OK;
+    if (!parents || !table || !lengths || !held || !free_pages || !state || !scratch || (caches > 0 && !cache_table))
+        return LRMOE_E_ARG;
+    lrmoe::PageForkArgs a{};
+    a.rows = rows;
+    a.pages = pages;
+    a.page_shift = shift_of(page);
+    a.max_pages = max_pages;
+    a.parents = parents;
+    a.table = table;
+    a.lengths = lengths;
+    a.held = held;
+    a.free_pages = free_pages;
+    a.state = state;
+    a.before = scratch;
+    int64_t pieces = 0;
+    for (int i = 0; i < caches; ++i) {
+        const int64_t* c = cache_table + 8 * i;
+        if (c[0] == 0 || c[1] < 1 || c[1] > (1 << 20) || c[2] < 1 || c[2] > (1 << 20) || c[3] < 16 || c[3] > (1 << 20))
+            return LRMOE_E_ARG;
+        for (int j : {0, 3, 4, 5, 6, 7})
+            if (c[j] % 16 != 0 || c[j] < 0) return LRMOE_E_ARG;
+        a.cache[i] = {reinterpret_cast<uint8_t*>(c[0]), c[4], c[5], c[6], c[7], static_cast<int>(c[1]),
+                      static_cast<int>(c[2]), static_cast<int>(c[3]), 0};
+        pieces += c[1] * c[2];
+    }
+    if (pieces > (1 << 24)) return LRMOE_E_ARG;
+    a.pieces = static_cast<int>(pieces);
+    if (int d = check_device()) return d;
+    return status_of(lrmoe::launch_page_fork(a, as_stream(stream)));
 }
 
 }  // extern "C"

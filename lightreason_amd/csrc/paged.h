@@ -89,6 +89,21 @@ struct PageReleaseArgs {
 };
 hipError_t launch_page_release(const PageReleaseArgs& a, hipStream_t stream);
 
+struct ForkCache {
+    uint8_t* base;
+    int64_t layer_stride, page_stride, head_stride, row_stride;   // in bytes
+    int layers, heads, row_bytes, pad;
+};
+struct PageForkArgs {
+    int rows, pages, page_shift, max_pages, pieces;   // pieces: layers times heads of all caches
+    const int32_t* parents;
+    int32_t *table, *lengths, *held;
+    const int32_t* free_pages;
+    int32_t *state, *before;
+    ForkCache cache[LRMOE_FORK_CACHES];
+};
+hipError_t launch_page_fork(const PageForkArgs& a, hipStream_t stream);
+
 struct PagedAppendArgs {
     int tokens, heads, kv_heads, rotary, pages, page_shift, rope_rows, rope_fp32;
     float eps;

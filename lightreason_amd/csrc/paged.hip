@@ -262,6 +262,111 @@ __global__ __launch_bounds__(kThreads) void page_release_kernel(PageReleaseArgs 
     }
 }
 
+// ---- rows that take over their parents' positions -----------------------------
+
+// One workgroup: a row r whose parent p is another row, one that keeps its own,
+// gets p's length and as many pages as that needs (fresh ones as a plan takes
+// them, rows in order).  before[r] is the first of r's pages among all that are
+// to be copied, before[rows] their count (0 where the fork is refused).
+__global__ __launch_bounds__(kThreads) void page_fork_kernel(PageForkArgs a) {
+    __shared__ PrefixLds prefix;
+    __shared__ int status;
+    const int tid = threadIdx.x;
+    const int per = (a.rows + kThreads - 1) / kThreads;
+    const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+    const int page = 1 << a.page_shift;
+    const int count = a.state[0], epoch = a.state[1], earlier = a.state[2];
+    if (tid == 0) status = 0;
+    // (pages, fresh pages) of a row, -1 pages for one that is wrong
+    auto look = [&](int r, int& length, int& fresh) {
+        const int p = a.parents[r];
+        fresh = length = 0;
+        if (p == r) return 0;
+        if (p < 0 || p >= a.rows || a.parents[p] != p) return -1;
+        length = a.lengths[p];
+        const int held = a.held[r], parent_held = a.held[p];
+        if (held < 0 || held > a.max_pages || parent_held < 0 || parent_held > a.max_pages || length < 0 ||
+            length > static_cast<int64_t>(parent_held) << a.page_shift)
+            return -1;
+        const int need = static_cast<int>((static_cast<int64_t>(length) + page - 1) >> a.page_shift);
+        fresh = max(need - held, 0);
+        return need;
+    };
+    int bad = 0, pages = 0, fresh = 0;
+    float size = 0.0f;
+    for (int r = r0; r < r1; ++r) {
+        int length, more;
+        const int need = look(r, length, more);
+        bad |= need < 0;
+        pages += max(need, 0);
+        fresh += more;
+        size += static_cast<float>(max(need, 0));
+    }
+    const Prefix pre = block_prefix(pages, fresh, size, &prefix);
+    if (bad) atomicOr(&status, kPageStatusRow);
+    __syncthreads();
+    int refuse = status;
+    if (pre.huge) refuse |= kPageStatusRow;
+    if ((refuse == 0 && pre.total_b > count) || count > a.pages) refuse |= kPageStatusPool;
+    const bool ok = refuse == 0;
+    int at = pre.a, taken = pre.b;
+    for (int r = r0; r < r1; ++r) {
+        int length, more;
+        const int need = max(look(r, length, more), 0);
+        a.before[r] = ok ? at : 0;
+        if (!ok || a.parents[r] == r) continue;
+        const int held = a.held[r];
+        for (int j = 0; j < more; ++j)
+            a.table[static_cast<int64_t>(r) * a.max_pages + held + j] = a.free_pages[count - 1 - (taken + j)];
+        at += need;
+        taken += more;
+        // (No row reads these of another: parents keep theirs.)
+        a.held[r] = max(held, need);
+        a.lengths[r] = length;
+    }
+    if (tid == 0) {
+        a.before[a.rows] = ok ? pre.total_a : 0;
+        if (ok) {
+            a.state[0] = count - pre.total_b;
+            a.state[1] = epoch + 1;
+            a.state[3] = 0;
+        }
+        a.state[2] = earlier | refuse;
+    }
+}
+
+// The pages' contents, a page of one head of one layer per workgroup at a
+// time.  Pages that are read belong to rows that keep theirs, so none is
+// written.  Bound by HBM.
+__global__ __launch_bounds__(kThreads) void page_fork_copy(PageForkArgs a) {
+    const int total = a.before[a.rows];
+    const int64_t work = static_cast<int64_t>(total) * a.pieces;
+    for (int64_t i = blockIdx.x; i < work; i += gridDim.x) {
+        const int unit = static_cast<int>(i / a.pieces);
+        int piece = static_cast<int>(i - static_cast<int64_t>(unit) * a.pieces), c = 0;
+        while (piece >= a.cache[c].layers * a.cache[c].heads) {
+            piece -= a.cache[c].layers * a.cache[c].heads;
+            ++c;
+        }
+        const ForkCache& cache = a.cache[c];
+        // (Rows without pages to copy share their place with the next: the last
+        // of those is meant.)
+        const int r = last_at_most(a.before, a.rows, unit), j = unit - a.before[r], p = a.parents[r];
+        const int to = a.table[static_cast<int64_t>(r) * a.max_pages + j];
+        const int from = a.table[static_cast<int64_t>(p) * a.max_pages + j];
+        if (to < 0 || to >= a.pages || from < 0 || from >= a.pages) continue;
+        const int rows = min(a.lengths[r] - (j << a.page_shift), 1 << a.page_shift);
+        uint8_t* base = cache.base + piece / cache.heads * cache.layer_stride + piece % cache.heads * cache.head_stride;
+        uint8_t* d = base + to * cache.page_stride;
+        const uint8_t* s = base + from * cache.page_stride;
+        const int lanes = cache.row_bytes / 16;
+        for (int x = threadIdx.x; x < rows * lanes; x += kThreads) {
+            const int64_t at = x / lanes * cache.row_stride + x % lanes * 16;
+            *reinterpret_cast<u32x4*>(d + at) = *reinterpret_cast<const u32x4*>(s + at);
+        }
+    }
+}
+
 // ---- append ------------------------------------------------------------------
 
 // A group of D / 8 lanes takes ROWS head rows (query, key or value) of one
@@ -376,6 +481,12 @@ hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t stream) {
 
 hipError_t launch_page_commit(const PageCommitArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL(page_commit_kernel, dim3(1), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_page_fork(const PageForkArgs& a, hipStream_t stream) {
+    page_fork_kernel<<<1, kThreads, 0, stream>>>(a);
+    if (a.pieces > 0) page_fork_copy<<<2048, kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 

@@ -202,6 +202,52 @@ class PageTable:
                          self.table.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(),
                          self.free_pages.data_ptr(), self.state.data_ptr(), _stream(self.device))
 
+    def fork(self, parents: torch.Tensor, *caches: torch.Tensor) -> None:
+        """Rows take over their parents' cached positions: row r with
+        ``parents[r]`` ([rows] int32 on the device, as ``beam.beam_select``
+        gives them, flattened) other than r gets that row's length, the fresh
+        pages it needs and, in each of ``caches`` ([layers, pages, kv_heads,
+        page, dim] or one layer [pages, kv_heads, page, dim]; all of the pool's
+        key and value caches), copies of its pages.  A parent must be its own
+        parent.  A fork that does not fit, or whose parents are not so, changes
+        nothing but the status (``check``).  Plans made before are refused at
+        their commit."""
+        key, form = _native.checked(_FORKS, (parents, *caches), self.rows, self.pages, self.page, self.device)
+        if form is None:
+            form = self._check_fork(parents, caches)
+            _native.remember(_FORKS, key, form)
+        table = (C.c_int64 * (8 * len(caches) + 1))()
+        for i, (cache, layout) in enumerate(zip(caches, form)):
+            table[8 * i] = cache.data_ptr()
+            table[8 * i + 1:8 * i + 8] = layout
+        with _on(self.device):
+            scratch = _native.workspace(self.device, 4 * (self.rows + 1))
+            _native.call("lrmoe_page_fork", self.rows, self.pages, self.page, self.max_pages, parents.data_ptr(),
+                         self.table.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(),
+                         self.free_pages.data_ptr(), self.state.data_ptr(), len(caches), C.addressof(table),
+                         scratch.data_ptr(), _stream(self.device))
+
+    def _check_fork(self, parents, caches):
+        _require(parents, "parents", (torch.int32,), (self.rows,), self.device)
+        if len(caches) > _native.FORK_CACHES:
+            raise ValueError(f"at most {_native.FORK_CACHES} caches, got {len(caches)}")
+        form = []
+        for i, t in enumerate(caches):
+            if not isinstance(t, torch.Tensor) or t.dim() not in (4, 5) or t.device != self.device:
+                raise ValueError(f"cache {i} must be [pages, kv_heads, page, dim] or one of those per layer on "
+                                 f"{self.device}")
+            c = t if t.dim() == 5 else t[None]
+            layers, pages, heads, page, dim = c.shape
+            if (pages, page) != (self.pages, self.page) or min(layers, heads, dim) < 1:
+                raise ValueError(f"cache {i} must have {self.pages} pages of {self.page} positions, got {tuple(t.shape)}")
+            size = t.element_size()
+            strides = [size * x for x in _strides(c)]
+            if (dim > 1 and c.stride(4) != 1) or dim * size % 16 or any(x % 16 or x < 0 for x in strides):
+                raise ValueError(f"cache {i} needs a contiguous last dimension and rows and strides of multiples of 16 "
+                                 "bytes")
+            form.append((layers, heads, dim * size, *strides))
+        return form
+
     def status(self) -> int:
         """Status bits of the commits and releases so far (reads the device)."""
         return int(self.state[2].item())
@@ -217,6 +263,9 @@ class PageTable:
                  if bits & bit]
         if texts:
             raise RuntimeError(f"{what}: " + "; ".join(texts))
+
+
+_FORKS: dict = {}   # forms of fork's arguments (types, shapes, strides) that were checked
 
 
 # ---- append ---------------------------------------------------------------------

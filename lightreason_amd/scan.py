@@ -1,0 +1,236 @@
+"""The gated delta rule of the 35B model's linear-attention layers over packed
+sequences: prompts, training, and the steps of a server.
+
+* ``delta_scan(query, key, value, g, beta, starts)`` -- whole sequences, from a
+  first state or from zero, to outputs and last states
+  (``lrmoe_delta_scan``).
+* ``delta_step(..., states, slots=, into=)`` -- a step of prompts, decode
+  positions and verify blocks over a pool of states in HBM, as
+  ``paged.paged_attention`` serves the full-attention layers of the same step
+  (its ``starts`` are a ``paged.PagePlan``'s).
+
+``delta.delta_rule`` and ``delta.DeltaMixer`` serve one sequence of 1..16 tokens
+with the rounding points of the Transformers forward (edge35b/
+delta_decode.py:38-55); here a call holds any number of tokens of any number of
+sequences, key heads are shared by value heads, and the recurrence runs in fp32
+with one rounding, of the outputs.
+
+Nothing reads a device value on the host: every call can be captured into a HIP
+graph.  There is no CPU path: the calls raise when liblrmoe.so is missing.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native
+from .paged import _TYPES, _int, _on, _ptr, _require, _stream, _strided, _strides
+
+HEAD_DIMS = (64, 128)
+
+
+def _rows(t, name, tokens, dtype, dev):
+    """A [tokens, heads, width] tensor whose rows the kernels can read."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, width]")
+    _require(t, name, (dtype,), (tokens, *t.shape[1:]), dev, contiguous=False)
+    _strided(t, name, 8)
+
+
+def _per_head(t, name, dtypes, shape, dev):
+    _require(t, name, dtypes, shape, dev, contiguous=False)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} needs a contiguous last dimension")
+
+
+def _check(query, key, value, g, beta, starts, normalize, scale):
+    """Checks what every call has; returns the argument structure with sizes
+    and strides, and the device."""
+    if not isinstance(query, torch.Tensor) or query.dim() != 3:
+        raise ValueError("query must be [tokens, key_heads, dim]")
+    N, K, D = query.shape
+    dtype, dev = query.dtype, query.device
+    if dtype not in _TYPES:
+        raise ValueError(f"query must be bfloat16 or float16, got {dtype}")
+    if D not in HEAD_DIMS:
+        raise ValueError(f"query must have a head width of 64 or 128, got {D}")
+    if dev.type != "cuda":
+        raise ValueError(f"query must be on a GPU, got {dev}")
+    if K < 1:
+        raise ValueError("query has no heads")
+    _strided(query, "query", 8)
+    _rows(key, "key", N, dtype, dev)
+    if tuple(key.shape) != (N, K, D):
+        raise ValueError(f"key must have shape {(N, K, D)}, got {tuple(key.shape)}")
+    _rows(value, "value", N, dtype, dev)
+    H, E = value.shape[1:]
+    if H < 1 or H % K:
+        raise ValueError(f"value must have a multiple of the {K} key heads, got {H}")
+    if E % 32 or not 32 <= E <= 256:
+        raise ValueError(f"value must have a head width that is a multiple of 32 up to 256, got {E}")
+    _per_head(g, "g", (torch.float32,), (N, H), dev)
+    _per_head(beta, "beta", (torch.float32, dtype), (N, H), dev)
+    if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError("starts must be int32 [seqs + 1]")
+    S = starts.shape[0] - 1
+    _require(starts, "starts", (torch.int32,), (S + 1,), dev)
+    if S > 65536 or N > 1 << 20 or N * H > 1 << 26 or H > 1024:
+        raise ValueError(f"at most 65536 sequences, 2^20 tokens, 1024 heads and tokens * heads of 2^26, got {S}, {N}, "
+                         f"{H} and {N * H}")
+    a = _native.DeltaScanArgs(seqs=S, tokens=N, max_new=N, heads=H, key_heads=K, dim=D, value_dim=E,
+                              fp16=int(dtype == torch.float16), normalize=int(bool(normalize)),
+                              beta_fp32=int(beta.dtype == torch.float32), scale=D ** -0.5 if scale is None else scale)
+    a.q_token_stride, a.q_head_stride = _strides(query)
+    a.k_token_stride, a.k_head_stride = _strides(key)
+    a.v_token_stride, a.v_head_stride = _strides(value)
+    (a.g_token_stride,), (a.beta_token_stride,) = _strides(g), _strides(beta)
+    if N == 0:   # (any strides)
+        for name in ("q", "k", "v"):
+            setattr(a, f"{name}_token_stride", 0)
+            setattr(a, f"{name}_head_stride", 0)
+    return a, dev
+
+
+def _addresses(a, query, key, value, g, beta, starts):
+    if a.tokens:
+        a.q, a.k, a.v, a.g, a.beta = (t.data_ptr() for t in (query, key, value, g, beta))
+    a.starts = starts.data_ptr()
+
+
+def _launch(a, dev):
+    with _on(dev):
+        nbytes = int(_native.library().lrmoe_delta_scan_workspace_bytes(C.addressof(a)))
+        ws = _native.workspace(dev, nbytes)
+        _native.call("lrmoe_delta_scan", C.addressof(a), ws.data_ptr(), ws.numel(), _stream(dev))
+
+
+# ---- whole sequences ------------------------------------------------------------
+
+def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+               starts: torch.Tensor, *, initial: torch.Tensor | None = None, normalize: bool = False,
+               scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gated delta rule over packed sequences: query, key [tokens,
+    key_heads, dim] and value [tokens, heads, value_dim] (bf16 or fp16; dim 64
+    or 128, value_dim a multiple of 32 up to 256; value head h reads key head
+    h // (heads // key_heads)), g [tokens, heads] fp32 (log decay), beta
+    [tokens, heads] (fp32 or the tensors' type), ``starts`` [seqs + 1] int32 on
+    the device: sequence s is tokens starts[s] .. starts[s + 1] - 1, its first
+    state ``initial[s]`` ([seqs, heads, dim, value_dim] fp32; None: zero).  Per
+    token, all in fp32:
+
+        S = exp(g) S;  u = beta (v - S^T k);  S = S + k u^T;  out = scale S^T q
+
+    ``normalize`` divides q and k by sqrt(sum x^2 + 1e-6) first; ``scale``
+    defaults to dim ** -0.5.  Returns (out [tokens, heads, value_dim], the last
+    states [seqs, heads, dim, value_dim] fp32).  A sequence without tokens
+    passes its state on; rows of no sequence are 0; starts that are not in
+    order within [0, tokens] make a sequence empty.  What is not finite reaches
+    only later tokens of its sequence.  Tensors may be strided views with a
+    contiguous last dimension and strides that are multiples of 8."""
+    if scale is not None:
+        scale = float(scale)
+    tensors = (query, key, value, g, beta, starts, initial)
+    key_, form = _native.checked(_SCANS, tensors, normalize, scale)
+    if form is None:
+        a, dev = _check(query, key, value, g, beta, starts, normalize, scale)
+        shape = (a.seqs, a.heads, a.dim, a.value_dim)
+        if initial is not None:
+            _require(initial, "initial", (torch.float32,), shape, dev)
+        a.pool, a.clear = a.seqs, 1
+        a.out_token_stride, a.out_head_stride = a.heads * a.value_dim, a.value_dim
+        form = a, dev, shape
+        _native.remember(_SCANS, key_, form)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("delta_scan records no gradient")
+    return _scan(form, tensors)
+
+
+_SCANS: dict = {}   # arguments of a form (types, shapes, strides) that was checked, without the addresses
+
+
+def _scan(form, tensors):
+    template, dev, shape = form
+    query, key, value, g, beta, starts, initial = tensors
+    a = _native.DeltaScanArgs.from_buffer_copy(template)
+    out = torch.empty(value.shape, dtype=value.dtype, device=dev)
+    if a.seqs == 0:
+        return out.zero_(), torch.empty(shape, dtype=torch.float32, device=dev)
+    final = torch.empty(shape, dtype=torch.float32, device=dev)
+    _addresses(a, query, key, value, g, beta, starts)
+    a.initial, a.final, a.out = _ptr(initial), final.data_ptr(), out.data_ptr()
+    _launch(a, dev)
+    return out, final
+
+
+# ---- steps over a pool of states ------------------------------------------------
+
+@torch.no_grad()
+def delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+               starts: torch.Tensor, states: torch.Tensor, *, slots: torch.Tensor | None = None,
+               into: torch.Tensor | None = None, fresh: torch.Tensor | None = None, normalize: bool = False,
+               scale: float | None = None, max_new: int | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``delta_scan`` for a serving step over a pool ``states`` [pool, heads,
+    dim, value_dim] fp32: sequence s goes on from the state in slot
+    ``slots[s]`` ([seqs] int32; default s), or from zero where ``fresh[s]``
+    ([seqs] bool or uint8), and leaves its state in slot ``into[s]`` (default:
+    where it was read; another one keeps the old state, for a verify block of
+    which only some drafts may stand).  Returns ``out`` [tokens, heads,
+    value_dim].
+
+    A sequence whose slot lies outside the pool (-1: a row that rests) is left
+    out; rows of no sequence and of those stay as they were in ``out`` (whatever
+    memory held where it is not given).  No two sequences of a call write one
+    slot, and none writes a slot that another reads.  ``max_new`` -- at least
+    every sequence's count of tokens, default ``tokens`` -- only chooses the
+    kernel: give it where the counts are known to be small.  ``out`` shares no
+    element with query, key and value (refused).  No gradient is recorded."""
+    if scale is not None:
+        scale = float(scale)
+    tensors = (query, key, value, g, beta, starts, states, slots, into, fresh, out)
+    key_, form = _native.checked(_STEPS, tensors, normalize, scale, max_new)
+    if form is None:
+        form = _check_step(*tensors, normalize, scale, max_new)
+        _native.remember(_STEPS, key_, form)
+    template, dev = form
+    if out is None:
+        out = torch.empty(value.shape, dtype=value.dtype, device=dev)
+    if template.seqs == 0:
+        return out
+    a = _native.DeltaScanArgs.from_buffer_copy(template)
+    _addresses(a, query, key, value, g, beta, starts)
+    a.initial = a.final = states.data_ptr()
+    a.slots, a.into, a.fresh = _ptr(slots), _ptr(slots if into is None else into), _ptr(fresh)
+    if a.tokens:
+        a.out = out.data_ptr()
+    _launch(a, dev)
+    return out
+
+
+_STEPS: dict = {}   # as _SCANS
+
+
+def _check_step(query, key, value, g, beta, starts, states, slots, into, fresh, out, normalize, scale, max_new):
+    a, dev = _check(query, key, value, g, beta, starts, normalize, scale)
+    if not isinstance(states, torch.Tensor) or states.dim() != 4 or states.shape[0] < 1:
+        raise ValueError("states must be [pool, heads, dim, value_dim]")
+    _require(states, "states", (torch.float32,), (states.shape[0], a.heads, a.dim, a.value_dim), dev)
+    a.pool = states.shape[0]
+    if slots is None and a.pool < a.seqs:
+        raise ValueError(f"states must have a slot for each of the {a.seqs} sequences, or give slots")
+    for name, t in (("slots", slots), ("into", into)):
+        if t is not None:
+            _require(t, name, (torch.int32,), (a.seqs,), dev)
+    if fresh is not None:
+        _require(fresh, "fresh", (torch.bool, torch.uint8), (a.seqs,), dev)
+    if max_new is not None:
+        a.max_new = min(_int(max_new, "max_new", 0, 2**31 - 1), a.tokens)
+    if out is not None:
+        _require(out, "out", (value.dtype,), tuple(value.shape), dev, contiguous=False)
+        _strided(out, "out", 8)
+        a.out_token_stride, a.out_head_stride = _strides(out)
+    else:
+        a.out_token_stride, a.out_head_stride = a.heads * a.value_dim, a.value_dim
+    return a, dev

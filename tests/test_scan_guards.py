@@ -1,0 +1,133 @@
+"""Refusals of the scan's, beam search's and forks' calls on the host (no GPU)."""
+
+from __future__ import annotations
+
+import ctypes as C
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+from lightreason_amd import _native, beam, paged, scan
+
+BF = torch.bfloat16
+
+
+def test_structures_match_the_header():
+    text = (Path(__file__).resolve().parents[1] / "include" / "lrmoe.h").read_text()
+    for name, struct in (("lrmoe_delta_scan_args", _native.DeltaScanArgs),):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        fields = []
+        for line in body.split(";"):
+            words = re.findall(r"\w+", line)
+            fields += [w for w in words if w not in ("const", "void", "int32_t", "int64_t", "float")]
+        assert fields == [f for f, _ in struct._fields_]
+        assert C.sizeof(struct) == sum(C.sizeof(t) for _, t in struct._fields_)
+    for name, value in (("LRMOE_BEAM_MAX", _native.BEAM_MAX), ("LRMOE_FORK_TENSORS", _native.FORK_TENSORS),
+                        ("LRMOE_FORK_CACHES", _native.FORK_CACHES)):
+        assert int(re.search(r"#define %s (\d+)" % name, text).group(1)) == value
+
+
+def _scan_args(N=4, K=2, H=4, D=64, E=64, dtype=BF):
+    return dict(query=torch.zeros(N, K, D, dtype=dtype), key=torch.zeros(N, K, D, dtype=dtype),
+                value=torch.zeros(N, H, E, dtype=dtype), g=torch.zeros(N, H), beta=torch.zeros(N, H, dtype=dtype),
+                starts=torch.tensor([0, N], dtype=torch.int32))
+
+
+def test_scan_refuses_host_tensors_and_shapes():
+    for call in (scan.delta_scan, lambda **x: scan.delta_step(**x, states=torch.zeros(1, 4, 64, 64))):
+        with pytest.raises(ValueError, match="GPU"):
+            call(**_scan_args())
+        with pytest.raises(ValueError, match="bfloat16"):
+            call(**_scan_args(dtype=torch.float32))
+        with pytest.raises(ValueError, match="width"):
+            call(**_scan_args(D=96))
+        with pytest.raises(ValueError, match="key_heads"):
+            call(**{**_scan_args(), "query": torch.zeros(4, 64, dtype=BF)})
+        with pytest.raises(ValueError):
+            call(**{**_scan_args(), "query": [1]})
+
+
+def test_c_entry_points_refuse_misuse():
+    lib = _native.library()
+    good = dict(seqs=1, tokens=4, max_new=4, heads=4, key_heads=2, dim=64, value_dim=64, pool=1, scale=1.0,
+                q=256, k=256, v=1 << 20, g=256, beta=256, starts=256, initial=256, final=256, out=1 << 24,
+                q_token_stride=128, q_head_stride=64, k_token_stride=128, k_head_stride=64, v_token_stride=256,
+                v_head_stride=64, g_token_stride=4, beta_token_stride=4, out_token_stride=256, out_head_stride=64)
+    ws = C.c_void_p(256)
+
+    def call(nbytes=1 << 40, workspace=ws, **kw):
+        a = _native.DeltaScanArgs(**{**good, **kw})
+        return lib.lrmoe_delta_scan(C.addressof(a), workspace, nbytes, None)
+    for kw in (dict(seqs=-1), dict(seqs=65537), dict(tokens=-1), dict(tokens=(1 << 20) + 1), dict(heads=0),
+               dict(heads=3), dict(heads=1026), dict(key_heads=0), dict(dim=96), dict(dim=256), dict(value_dim=16),
+               dict(value_dim=288), dict(value_dim=72), dict(pool=-1), dict(max_new=-1), dict(q=None), dict(k=None),
+               dict(v=None), dict(g=None), dict(beta=None), dict(starts=None), dict(final=None), dict(out=None),
+               dict(q=264), dict(out=(1 << 24) + 4), dict(q_token_stride=129), dict(v_head_stride=4),
+               dict(k_token_stride=-8), dict(v_token_stride=1 << 23), dict(out_token_stride=2), dict(g=258),
+               dict(beta=257), dict(final=264), dict(workspace=None), dict(workspace=C.c_void_p(128)),
+               dict(tokens=1 << 20, heads=128, key_heads=1)):
+        assert call(**kw) == _native.LRMOE_E_ARG, kw
+    assert call(nbytes=0) == _native.LRMOE_E_WORKSPACE
+    assert call(seqs=0) == 0
+    assert lib.lrmoe_delta_scan(None, ws, 1 << 40, None) == _native.LRMOE_E_ARG
+    # out over what is read, and over itself
+    assert call(out=1 << 20) == _native.LRMOE_E_ARG
+    assert call(out=256 + 64) == _native.LRMOE_E_ARG
+    assert call(out_head_stride=32) == _native.LRMOE_E_ARG
+    assert call(q=1 << 26, k=1 << 27, out=(1 << 26) + 8, value_dim=128, v_token_stride=512, v_head_stride=128,
+                out_token_stride=512, out_head_stride=128) == _native.LRMOE_E_ARG
+
+    p = C.c_void_p(256)
+    assert lib.lrmoe_beam_workspace_bytes(1, 33, 10) == 0 and lib.lrmoe_beam_workspace_bytes(1, 4, 10) > 0
+    for args in ((1, 0, 10, 0), (1, 33, 10, 0), (-1, 4, 10, 0), (20000, 4, 10, 0), (1, 4, 0, 0), (1, 4, 10, 3)):
+        assert lib.lrmoe_beam_select(*args, p, 10, p, None, p, p, p, p, 1 << 30, None) == _native.LRMOE_E_ARG, args
+    assert lib.lrmoe_beam_select(1, 4, 10, 0, p, 9, p, None, p, p, p, p, 1 << 30, None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_beam_select(1, 4, 10, 0, None, 10, p, None, p, p, p, p, 1 << 30, None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_beam_select(1, 4, 10, 0, p, 10, p, None, p, p, p, p, 8, None) == _native.LRMOE_E_WORKSPACE
+    assert lib.lrmoe_beam_select(0, 4, 10, 0, None, 10, None, None, None, None, None, None, 0, None) == 0
+
+    table = (C.c_int64 * 3)(256, 64, 64)
+    assert lib.lrmoe_fork_rows(-1, p, 1, table, None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(4, None, 1, table, None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(4, p, 65, table, None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(4, p, 1, (C.c_int64 * 3)(256, 63, 64), None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(4, p, 1, (C.c_int64 * 3)(0, 64, 64), None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(1 << 20, p, 1, (C.c_int64 * 3)(256, 1 << 30, 1 << 30), None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(0, None, 1, table, None) == 0
+
+    row = (256, 2, 2, 128, 1 << 20, 1 << 12, 1 << 11, 128)
+    fork = lambda n=4, page=16, caches=1, row=row: lib.lrmoe_page_fork(n, 8, page, 4, p, p, p, p, p, p, caches,
+                                                                      (C.c_int64 * 8)(*row), p, None)
+    for kw in (dict(n=-1), dict(n=4097), dict(page=24), dict(caches=33), dict(caches=-1), dict(row=(0,) + row[1:]),
+               dict(row=(256, 0) + row[2:]), dict(row=(256, 2, 2, 8) + row[4:]), dict(row=row[:7] + (120,)),
+               dict(row=row[:4] + (-16,) + row[5:])):
+        assert fork(**kw) == _native.LRMOE_E_ARG, kw
+    assert fork(n=0) == 0
+
+
+def test_beam_refuses_host_tensors_and_shapes():
+    logits, scores = torch.zeros(8, 100), torch.zeros(2, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        beam.beam_select(logits, scores)
+    for l, s in ((logits[:7], scores), (logits.double(), scores), (logits, scores.double()), (logits[0], scores),
+                 (logits, scores[0]), (torch.zeros(66, 10), torch.zeros(2, 33)), (torch.zeros(8, 0), scores),
+                 (torch.zeros(65536, 1), torch.zeros(65536, 1)), ([1], scores), (logits, None)):
+        with pytest.raises(ValueError):
+            beam.beam_select(l, s)
+    with pytest.raises(ValueError):
+        beam.fork_rows(torch.zeros(3, dtype=torch.int64), [])
+    with pytest.raises(ValueError, match="GPU"):
+        beam.fork_rows(torch.zeros(3, dtype=torch.int32), [])
+    with pytest.raises(ValueError):
+        beam.fork_rows([0], [])
+
+
+def test_page_fork_refuses_host_tensors_and_shapes():
+    pool = paged.PageTable(2, 10, 16, device="cpu")
+    with pytest.raises(ValueError):
+        pool.fork(torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="GPU|cpu"):
+        pool.fork(torch.zeros(2, dtype=torch.int32))
