@@ -27,6 +27,68 @@ struct ScanArgs {
 hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int max_new, void* workspace, hipStream_t stream);
 size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new);
 
+// The chunked form (scan_chunk.hip).
+size_t scan_chunk_bytes(const ScanArgs& a, bool fp16);
+hipError_t launch_scan_chunks(const ScanArgs& a, bool fp16, void* workspace, const uint32_t** flags,
+                              hipStream_t stream);
+
+// ---- chunks ------------------------------------------------------------------
+//
+// Sequences are cut into chunks of 64 tokens.  Sequence s has the chunk slots
+// from starts[s] / 64 + s on (rounded down): ceil(n / 64) of them never reach
+// the next sequence's, whatever the counts, and tokens / 64 + seqs hold all, so
+// that slots need no scan over the sequences.
+constexpr int kChunk = 64;
+
+__device__ __forceinline__ int scan_first_chunk(const int32_t* starts, int s) { return (starts[s] >> 6) + s; }
+
+// Fragments of 16 bytes per lane, as the matrix instructions' A operands.  The
+// tokens of a chunk, where they are summed over, come in this order: step ks
+// (of 32), lane group g (of 16 lanes), element j: token 32 ks + 4 g + j for
+// j < 4, 32 ks + 16 + 4 g + j - 4 from there on: what a lane of the waves 2 ks
+// and 2 ks + 1 holds of a product's rows.  Of a lower triangular 64 x 64 matrix
+// the blocks (ks, row tile w) with 2 ks <= w are kept, of an upper one those
+// with 2 ks + 1 >= w: six each.
+constexpr int kBlocks = 6;
+constexpr int kFragBytes = 1024;
+__host__ __device__ __forceinline__ constexpr int lower_block(int ks, int w) { return ks == 0 ? w : 2 + w; }
+__host__ __device__ __forceinline__ constexpr int upper_block(int ks, int w) { return ks == 1 ? w : 4 + w; }
+
+// What the first launch leaves the second, per chunk slot and value head (or
+// key head), in this order in the workspace.
+struct ScanChunks {
+    int slots, parts;      // parts: bf16 numbers that a q or k is (1, or 2 for fp16)
+    uint8_t *t, *p;        // [slots][heads]: 3 and 2 parts of 6 blocks
+    float* vec;            // [slots][heads][256]: factors of K S, of Q S and of K^T U per token, then the chunk's decay
+    uint8_t *kt, *qt;      // [slots][key_heads][dim / 16][2][parts]: K^T, and for the gradient Q^T
+    uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of fp16 inputs as bf16 parts
+    uint32_t* flags;       // [seqs][heads][value_dim / 32]
+};
+
+// An fp32 number as three bf16 ones, each the upper half of the bits that are
+// left: their sum is the number (24 bits), of two the first 16 bits.
+struct Split2 {
+    uint32_t part[3];   // bf16 pairs
+};
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+template <int PARTS>
+__device__ __forceinline__ Split2 split2(float lo, float hi) {
+    Split2 s;
+    s.part[0] = high_halves(lo, hi);
+    if constexpr (PARTS > 1) {
+        lo -= high_part(lo), hi -= high_part(hi);
+        s.part[1] = high_halves(lo, hi);
+    }
+    if constexpr (PARTS > 2) {
+        lo -= high_part(lo), hi -= high_part(hi);
+        s.part[2] = high_halves(lo, hi);
+    }
+    return s;
+}
+
 // Tokens of a sequence: [a, b), empty where starts do not lie in order within
 // [0, tokens].
 struct ScanSeq {

@@ -37,20 +37,24 @@ __device__ __forceinline__ void recur_load(const ScanArgs& a, RecurToken<D, FP16
                          : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[t * a.beta_token + h]);
 }
 
+//
+// With flags given only the blocks of columns that they mark are computed: those
+// in which the chunked form met a number that is not finite.
 template <int D, bool FP16>
-__global__ __launch_bounds__(256) void scan_recur(ScanArgs a) {
+__global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* flags) {
     constexpr int ROWS = D / 8;
     const int lane = threadIdx.x % kWave;
     const int blocks = a.value_dim / 32;
     const int64_t wave = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kWave;
     if (wave >= static_cast<int64_t>(a.seqs) * a.heads * blocks) return;
+    if (flags != nullptr && flags[wave] == 0) return;
     const int cb = static_cast<int>(wave % blocks);
     const int h = static_cast<int>(wave / blocks % a.heads), s = static_cast<int>(wave / blocks / a.heads);
     const int kh = h / a.group;
     const int rows0 = ROWS * (lane / 8), col = 32 * cb + 4 * (lane % 8);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
     // Rows of no sequence.
-    if (a.clear && (s == 0 || s == a.seqs - 1)) {
+    if (a.clear && flags == nullptr && (s == 0 || s == a.seqs - 1)) {
         const int64_t row0 = h * a.out_head + col;
         const int head = min(max(a.starts[0], 0), a.tokens), tail = min(max(a.starts[a.seqs], 0), a.tokens);
         if (s == 0)
@@ -136,13 +140,24 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a) {
 
 }  // namespace
 
-size_t delta_scan_workspace_bytes(const ScanArgs&, bool, int) { return 256; }
+// Single tokens and short blocks go token by token: the state is read and
+// written once, whatever the form.
+static bool token_by_token(const ScanArgs&, int max_new) { return max_new <= 16; }
 
-hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int, void*, hipStream_t stream) {
+size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
+    return token_by_token(a, max_new) ? 256 : scan_chunk_bytes(a, fp16);
+}
+
+hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int max_new, void* workspace, hipStream_t stream) {
+    const uint32_t* flags = nullptr;
+    if (!token_by_token(a, max_new)) {
+        const hipError_t err = launch_scan_chunks(a, fp16, workspace, &flags, stream);
+        if (err != hipSuccess) return err;
+    }
     const int64_t waves = static_cast<int64_t>(a.seqs) * a.heads * (a.value_dim / 32);
     const int per = waves < 2048 ? 1 : 4;
     const dim3 grid(static_cast<uint32_t>((waves + per - 1) / per)), block(per * kWave);
-    auto run = [&](auto kernel) { kernel<<<grid, block, 0, stream>>>(a); };
+    auto run = [&](auto kernel) { kernel<<<grid, block, 0, stream>>>(a, flags); };
     if (a.dim == 64) {
         if (fp16) run(scan_recur<64, true>); else run(scan_recur<64, false>);
     } else {
