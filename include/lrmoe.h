@@ -703,9 +703,33 @@ typedef struct lrmoe_delta_scan_args {
     const void *initial;
     void *final, *out;                    /* out [tokens][heads][value_dim] */
     int64_t out_token_stride, out_head_stride;
+    void *tape;                           /* NULL, or what the gradient reads */
 } lrmoe_delta_scan_args;
 size_t lrmoe_delta_scan_workspace_bytes(const lrmoe_delta_scan_args *args);
 int lrmoe_delta_scan(const lrmoe_delta_scan_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The gradient of lrmoe_delta_scan: args as in the forward call, which was given
+ * a tape of lrmoe_delta_scan_tape_bytes(args) bytes (256-byte aligned; the
+ * states before every 64 tokens and the rows u, in two 16-bit parts each) and
+ * whose slots and pool are the sequences themselves (slots, into and fresh NULL,
+ * pool = seqs); initial, final and out are not read.  From the gradients of out
+ * and (d_final, may be NULL) of final it writes those of q, k, v, g, beta and
+ * (d_initial, may be NULL) initial: contiguous, of the inputs' shapes and types,
+ * summed over the value heads that share a key head; rows of no sequence are 0.
+ * No atomics: the same bits every time.  A gradient of a sequence with values
+ * that are not finite is not defined.  d_out 16-byte aligned with strides of
+ * multiples of 8; workspace as the forward's, of
+ * lrmoe_delta_scan_grad_workspace_bytes(args) bytes. */
+typedef struct lrmoe_delta_grad_args {
+    const void *d_out;                    /* [tokens][heads][value_dim] */
+    int64_t d_out_token_stride, d_out_head_stride;
+    const void *d_final, *tape;
+    void *dq, *dk, *dv, *dg, *dbeta, *d_initial;
+} lrmoe_delta_grad_args;
+size_t lrmoe_delta_scan_tape_bytes(const lrmoe_delta_scan_args *args);
+size_t lrmoe_delta_scan_grad_workspace_bytes(const lrmoe_delta_scan_args *args);
+int lrmoe_delta_scan_grad(const lrmoe_delta_scan_args *args, const lrmoe_delta_grad_args *grad, void *workspace,
+                          size_t workspace_bytes, void *stream);
 
 /* ---- beam search -------------------------------------------------------------
  *

@@ -83,6 +83,9 @@ _SIGNATURES = {
     "lrmoe_page_fork": ([_I] * 4 + [_P] * 6 + [_I] + [_P] * 3, _I),
     "lrmoe_delta_scan_workspace_bytes": ([_P], C.c_size_t),
     "lrmoe_delta_scan": ([_P, _P, C.c_size_t, _P], _I),
+    "lrmoe_delta_scan_tape_bytes": ([_P], C.c_size_t),
+    "lrmoe_delta_scan_grad_workspace_bytes": ([_P], C.c_size_t),
+    "lrmoe_delta_scan_grad": ([_P, _P, _P, C.c_size_t, _P], _I),
     "lrmoe_beam_workspace_bytes": ([_I] * 3, C.c_size_t),
     "lrmoe_beam_select": ([_I] * 4 + [_P, C.c_int64] + [_P] * 6 + [C.c_size_t, _P], _I),
     "lrmoe_fork_rows": ([_I, _P, _I, _P, _P], _I),
@@ -126,7 +129,13 @@ class DeltaScanArgs(C.Structure):
         "i: seqs tokens max_new heads key_heads dim value_dim fp16 normalize beta_fp32 clear pool; f: scale; i: pad;"
         "p: q k v; l: q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride;"
         "p: g beta; l: g_token_stride beta_token_stride; p: starts slots into fresh initial final out;"
-        "l: out_token_stride out_head_stride")
+        "l: out_token_stride out_head_stride; p: tape")
+
+
+class DeltaGradArgs(C.Structure):
+    """lrmoe_delta_grad_args."""
+
+    _fields_ = _fields("p: d_out; l: d_out_token_stride d_out_head_stride; p: d_final tape dq dk dv dg dbeta d_initial")
 
 
 BEAM_MAX = 32            # beams of a group

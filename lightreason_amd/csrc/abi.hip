@@ -1031,6 +1031,7 @@ static lrmoe::ScanArgs scan_args(const lrmoe_delta_scan_args* p) {
     a.out = static_cast<uint16_t*>(p->out);
     a.out_token = p->out_token_stride;
     a.out_head = p->out_head_stride;
+    a.tape = static_cast<uint8_t*>(p->tape);
     return a;
 }
 
@@ -1059,7 +1060,8 @@ int lrmoe_delta_scan(const lrmoe_delta_scan_args* p, void* workspace, size_t wor
     if (!p || bad_scan(p)) return LRMOE_E_ARG;
     if (p->seqs == 0) return LRMOE_OK;
     if (bad_scan_inputs(p) || !p->final || (p->tokens > 0 && !p->out) || misaligned(p->final, 16) ||
-        misaligned(p->out, 8) || p->out_token_stride % 4 != 0 || p->out_head_stride % 4 != 0 || misaligned(workspace, 256))
+        misaligned(p->out, 8) || p->out_token_stride % 4 != 0 || p->out_head_stride % 4 != 0 ||
+        misaligned(workspace, 256) || misaligned(p->tape, 256))
         return LRMOE_E_ARG;
     const size_t need = lrmoe_delta_scan_workspace_bytes(p);
     if (need > 0 && !workspace) return LRMOE_E_ARG;
@@ -1086,6 +1088,46 @@ int lrmoe_delta_scan(const lrmoe_delta_scan_args* p, void* workspace, size_t wor
     }
     if (int d = check_device()) return d;
     return status_of(lrmoe::launch_delta_scan(scan_args(p), p->fp16 != 0, p->max_new, workspace, as_stream(stream)));
+}
+
+size_t lrmoe_delta_scan_tape_bytes(const lrmoe_delta_scan_args* p) {
+    if (!p || bad_scan(p)) return 0;
+    return lrmoe::delta_scan_tape_bytes(scan_args(p));
+}
+
+size_t lrmoe_delta_scan_grad_workspace_bytes(const lrmoe_delta_scan_args* p) {
+    if (!p || bad_scan(p)) return 0;
+    return lrmoe::delta_scan_grad_workspace_bytes(scan_args(p), p->fp16 != 0);
+}
+
+int lrmoe_delta_scan_grad(const lrmoe_delta_scan_args* p, const lrmoe_delta_grad_args* d, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    if (!p || !d || bad_scan(p) || p->slots || p->into || p->fresh || p->pool != p->seqs) return LRMOE_E_ARG;
+    if (p->seqs == 0) return LRMOE_OK;
+    if (bad_scan_inputs(p) || !d->tape || misaligned(d->tape, 256) || misaligned(workspace, 256) ||
+        (p->tokens > 0 && (!d->d_out || !d->dq || !d->dk || !d->dv || !d->dg || !d->dbeta)))
+        return LRMOE_E_ARG;
+    for (const void* x : {d->d_out, d->d_final, static_cast<const void*>(d->dq), static_cast<const void*>(d->dk),
+                          static_cast<const void*>(d->dv), static_cast<const void*>(d->dg),
+                          static_cast<const void*>(d->dbeta), static_cast<const void*>(d->d_initial)})
+        if (misaligned(x, 16)) return LRMOE_E_ARG;
+    if (d->d_out_token_stride % 8 != 0 || d->d_out_head_stride % 8 != 0) return LRMOE_E_ARG;
+    if (!workspace) return LRMOE_E_ARG;
+    if (workspace_bytes < lrmoe_delta_scan_grad_workspace_bytes(p)) return LRMOE_E_WORKSPACE;
+    if (int e = check_device()) return e;
+    lrmoe::ScanGradArgs g{};
+    g.d_out = static_cast<const uint16_t*>(d->d_out);
+    g.d_out_token = d->d_out_token_stride;
+    g.d_out_head = d->d_out_head_stride;
+    g.d_final = static_cast<const float*>(d->d_final);
+    g.tape = static_cast<const uint8_t*>(d->tape);
+    g.dq = static_cast<uint16_t*>(d->dq);
+    g.dk = static_cast<uint16_t*>(d->dk);
+    g.dv = static_cast<uint16_t*>(d->dv);
+    g.dg = static_cast<float*>(d->dg);
+    g.dbeta = d->dbeta;
+    g.d_initial = static_cast<float*>(d->d_initial);
+    return status_of(lrmoe::launch_delta_scan_grad(scan_args(p), g, p->fp16 != 0, workspace, as_stream(stream)));
 }
 
 // ---- beam search ------------------------------------------------------------------

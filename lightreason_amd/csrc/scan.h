@@ -23,9 +23,25 @@ struct ScanArgs {
     float* final;
     uint16_t* out;
     int64_t out_token, out_head;
+    uint8_t* tape;   // what the gradient needs: the chunks' first states and u, or NULL
+};
+struct ScanGradArgs {
+    const uint16_t* d_out;
+    int64_t d_out_token, d_out_head;
+    const float* d_final;
+    const uint8_t* tape;
+    uint16_t *dq, *dk, *dv;
+    float* dg;
+    void* dbeta;
+    float* d_initial;
 };
 hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int max_new, void* workspace, hipStream_t stream);
 size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new);
+
+size_t delta_scan_tape_bytes(const ScanArgs& a);
+size_t delta_scan_grad_workspace_bytes(const ScanArgs& a, bool fp16);
+hipError_t launch_delta_scan_grad(const ScanArgs& a, const ScanGradArgs& d, bool fp16, void* workspace,
+                                  hipStream_t stream);
 
 // The chunked form (scan_chunk.hip).
 size_t scan_chunk_bytes(const ScanArgs& a, bool fp16);
@@ -63,7 +79,24 @@ struct ScanChunks {
     uint8_t *kt, *qt;      // [slots][key_heads][dim / 16][2][parts]: K^T, and for the gradient Q^T
     uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of fp16 inputs as bf16 parts
     uint32_t* flags;       // [seqs][heads][value_dim / 32]
+    // For the gradient: t and p hold the transposed matrices, 3 parts each, and
+    double* sums;          // [slots][heads][64]: running sums of g
+    float* norms;          // [slots][key_heads][128]: factors of k and of q
+    uint16_t *ds, *dr;     // [slots][heads][2][dim][value_dim], [slots][heads][2][64][value_dim]
 };
+
+// A beta of 0 is taken as 2^-40: u = beta w then still tells w, which beta's
+// gradient is made of; no output changes by more than 2^-40 of its terms.
+__device__ __forceinline__ float scan_beta(float b) {
+    return __builtin_fabsf(b) < 0x1p-40f ? __builtin_copysignf(0x1p-40f, b) : b;
+}
+
+__host__ __device__ __forceinline__ int scan_slots(int tokens, int seqs) { return tokens / kChunk + seqs; }
+// The tape: states in two bf16 parts [slots][heads][2][dim][value_dim], then u
+// [slots][heads][2][64][value_dim].
+__host__ __device__ __forceinline__ int64_t tape_states(int64_t slots, int heads, int dim, int value_dim) {
+    return slots * heads * 2 * dim * value_dim;
+}
 
 // An fp32 number as three bf16 ones, each the upper half of the bits that are
 // left: their sum is the number (24 bits), of two the first 16 bits.

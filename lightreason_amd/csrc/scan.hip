@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* fl
 }  // namespace
 
 // Single tokens and short blocks go token by token: the state is read and
-// written once, whatever the form.
-static bool token_by_token(const ScanArgs&, int max_new) { return max_new <= 16; }
+// written once, whatever the form.  (The tape is the chunked form's.)
+static bool token_by_token(const ScanArgs& a, int max_new) { return max_new <= 16 && a.tape == nullptr; }
 
 size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
     return token_by_token(a, max_new) ? 256 : scan_chunk_bytes(a, fp16);

@@ -119,7 +119,7 @@ __device__ __forceinline__ void store_parts(uint8_t* to, const float (&x)[8]) {
             make_uint4(s[0].part[p], s[1].part[p], s[2].part[p], s[3].part[p]);
 }
 
-template <int D, bool FP16>
+template <int D, bool FP16, bool GRAD>
 __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChunks w) {
     constexpr int RAW = D + 8;   // 16-bit elements of a row in LDS
     constexpr int PARTS = FP16 ? 2 : 1;
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
             q2 = n % 4 == i ? qq[i] : q2;
         }
         lds.rk[16 * wave + n] = a.normalize ? 1.0f / __builtin_sqrtf(k2 + 1e-6f) : 1.0f;
-        lds.rq[16 * wave + n] = a.scale * (a.normalize ? 1.0f / __builtin_sqrtf(q2 + 1e-6f) : 1.0f);
+        lds.rq[16 * wave + n] = a.normalize ? 1.0f / __builtin_sqrtf(q2 + 1e-6f) : 1.0f;
     }
     // Fragments of K^T: row m of tile t is element 32 (t / 2) + 8 (m / 4) + 4 (t
     // % 2) + m % 4, so that a lane's rows of two tiles are eight in a row.
@@ -185,6 +185,16 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
         for (int j = 0; j < 8; ++j)
             x[j] = elem16<FP16>(raw_k[(32 * ks + 16 * (j / 4) + 4 * g + j % 4) * RAW + d]);
         store_parts<PARTS>(w.kt + ((by_key * (D / 16 * 2) + f) * PARTS) * kFragBytes + lane * 16, x);
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = elem16<FP16>(raw_q[(32 * ks + 16 * (j / 4) + 4 * g + j % 4) * RAW + d]);
+            store_parts<PARTS>(w.qt + ((by_key * (D / 16 * 2) + f) * PARTS) * kFragBytes + lane * 16, x);
+        }
+    }
+    if constexpr (GRAD) {
+        __syncthreads();   // (the norms)
+        if (tid < 2 * kChunk) w.norms[by_key * 2 * kChunk + tid] = tid < kChunk ? lds.rk[tid] : lds.rq[tid - kChunk];
     }
     if constexpr (FP16) {
         for (int ks = 0; ks < D / 32; ++ks) {
@@ -192,8 +202,10 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
             const int64_t at = (((by_key * 4 + wave) * (D / 32) + ks) * PARTS) * kFragBytes + lane * 16;
             unpack16<FP16>(*reinterpret_cast<const uint4*>(raw_k + (16 * wave + n) * RAW + 32 * ks + 8 * g), x);
             store_parts<PARTS>(w.kf + at, x);
-            unpack16<FP16>(*reinterpret_cast<const uint4*>(raw_q + (16 * wave + n) * RAW + 32 * ks + 8 * g), x);
-            store_parts<PARTS>(w.qf + at, x);
+            if constexpr (!GRAD) {
+                unpack16<FP16>(*reinterpret_cast<const uint4*>(raw_q + (16 * wave + n) * RAW + 32 * ks + 8 * g), x);
+                store_parts<PARTS>(w.qf + at, x);
+            }
         }
     }
     for (int hv = 0; hv < a.group; ++hv) {
@@ -210,12 +222,13 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
             }
             const double sum = wave_scan_f64(gl);
             lds.sum[lane] = sum;
-            lds.beta[lane] = b;
+            lds.beta[lane] = lane < count ? scan_beta(b) : 0.0f;
+            if constexpr (GRAD) w.sums[by_head * kChunk + lane] = sum;
             const double last = __shfl(sum, kWave - 1);
             const float decay = expf(static_cast<float>(sum)), rest = expf(static_cast<float>(last - sum));
             float* vec = w.vec + by_head * 256;
             vec[lane] = decay * lds.rk[lane];
-            vec[64 + lane] = decay * lds.rq[lane];
+            vec[64 + lane] = decay * lds.rq[lane] * a.scale;
             vec[128 + lane] = rest * lds.rk[lane];
             if (lane == kWave - 1) vec[192] = decay;
         }
@@ -229,12 +242,30 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
                 const int i = 16 * wave + 4 * g + r;
                 const float fade = expf(static_cast<float>(lds.sum[i] - lds.sum[j])) * lds.rk[j];
                 lds.a[i * kPitch + j] = j < i ? fade * lds.rk[i] * lds.beta[j] * kk[t][r] : 0.0f;
-                lds.b[i * kPitch + j] = j <= i ? fade * lds.rq[i] * qk[t][r] : 0.0f;
+                lds.b[i * kPitch + j] = j <= i ? fade * lds.rq[i] * a.scale * qk[t][r] : 0.0f;
             }
         }
         __syncthreads();
         invert(lds, wave, lane);
         const int row = 16 * wave + n;
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (2 * ks + 1 < wave) continue;
+                float x[8], y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = 32 * ks + 16 * (j / 4) + 4 * g + j % 4;
+                    const bool in = 2 * ks + j / 4 >= wave;
+                    x[j] = in ? lds.beta[i] * lds.t[i * kPitch + row] : 0.0f;
+                    y[j] = in ? lds.b[i * kPitch + row] : 0.0f;
+                }
+                const int64_t block = by_head * kBlocks + upper_block(ks, wave);
+                store_parts<3>(w.t + block * 3 * kFragBytes + lane * 16, x);
+                store_parts<3>(w.p + block * 3 * kFragBytes + lane * 16, y);
+            }
+            continue;
+        }
         const float b = lds.beta[row];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -280,6 +311,21 @@ __device__ __forceinline__ void put_parts(uint4 (&to)[PARTS][KS][NC][kWave], int
         reinterpret_cast<uint2*>(&to[p][ks][c][lane])[half] = make_uint2(lo.part[p], hi.part[p]);
 }
 
+// Four rows of a lane's columns, from row `row` on, as two bf16 parts of a
+// [rows][value_dim] matrix, `apart` elements from part to part.
+template <int NC>
+__device__ __forceinline__ void put_rows(uint16_t* to, int64_t apart, int value_dim, int row, int col,
+                                         const f32x4 (&x)[NC]) {
+    static_assert(NC == 2, "pairs of columns");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const Split2 s = split2<2>(x[0][i], x[1][i]);
+        uint16_t* p = to + static_cast<int64_t>(row + i) * value_dim + col;
+        *reinterpret_cast<uint32_t*>(p) = s.part[0];
+        *reinterpret_cast<uint32_t*>(p + apart) = s.part[1];
+    }
+}
+
 template <int D, int NC, bool FP16>
 struct ScanLoads {
     static constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64;
@@ -303,7 +349,7 @@ __device__ __forceinline__ float col_value(const uint32_t (&v)[NC / 2 + NC % 2],
     return elem16<FP16>(static_cast<uint16_t>(c % 2 ? v[c / 2] >> 16 : v[c / 2]));
 }
 
-template <int D, int NC, bool FP16>
+template <int D, int NC, bool FP16, bool TAPE>
 __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32;
     __shared__ ScanLds<D, NC> lds;
@@ -350,6 +396,8 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                                                static_cast<int64_t>(row_of(x, i)) * a.value_dim + col + c];
     const int chunks = (seq.n + kChunk - 1) / kChunk;
     const int64_t slot0 = scan_first_chunk(a.starts, s);
+    uint16_t* tape_s = reinterpret_cast<uint16_t*>(a.tape);
+    uint16_t* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
     ScanLoads<D, NC, FP16> x;
     auto load_rows = [&](int ch) {
         if constexpr (FP16) {
@@ -420,6 +468,12 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 put_parts<3>(lds.s, (wave * TPW + i) / 2, (wave * TPW + i) % 2, c, lane, S[i][c]);
+        const int64_t taped = (slot0 + ch) * a.heads + h;
+        if constexpr (TAPE) {
+#pragma unroll
+            for (int i = 0; i < TPW; ++i)
+                put_rows<NC>(tape_s + taped * 2 * size, size, a.value_dim, row_of(i, 0), col, S[i]);
+        }
         __syncthreads();
         f32x4 ks[NC], qs[NC];
 #pragma unroll
@@ -469,6 +523,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
             put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * x.fu);
         }
+        if constexpr (TAPE)
+            put_rows<NC>(tape_u + taped * 2 * kChunk * a.value_dim, kChunk * a.value_dim, a.value_dim, 16 * wave + 4 * g,
+                         col, u);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
@@ -533,9 +590,545 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                         static_cast<int64_t>(row_of(x1, i)) * a.value_dim + col + c] = S[x1][c][i];
 }
 
-ScanChunks layout(const ScanArgs& a, bool fp16, uint8_t* base, size_t* bytes) {
+// ---- the gradient: chunk after chunk, backwards -----------------------------------
+
+// With dS the gradient of the state after a chunk and do that of its outputs,
+//     X_j = sum_i P_ij do_i + e^(G_63 - G_j) dS^T k_j,     dR = (beta (I + L beta)^-1)^T X = dv,
+//     dS <- e^(G_63) dS + sum_i scale e^(G_i) q_i do_i^T - sum_i e^(G_i) k_i dR_i^T:
+// the forward launch with the matrices transposed, for the same columns.
+template <int D, int NC, int PARTS>
+struct ScanGradLds {
+    uint4 s[3][D / 32][NC][kWave];
+    uint4 o[PARTS][2][NC][kWave];   // do
+    uint4 x[3][2][NC][kWave];
+    uint4 oq[3][2][NC][kWave];      // do times the factors of q
+    uint4 rk[3][2][NC][kWave];      // - dR times the factors of k
+};
+
+template <int D, bool FP16>
+__global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
+    constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32, NC = 2;
+    __shared__ ScanGradLds<D, NC, PARTS> lds;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int blocks = a.value_dim / (16 * NC), per = (gridDim.x + 7) / 8;
+    const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
+    if (item >= a.seqs * a.heads * blocks) return;
+    const int cb = item % blocks, h = item / blocks % a.heads, s = item / blocks / a.heads, kh = h / a.group;
+    const int col = 16 * NC * cb + NC * n;
+    const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
+    if (s == 0 || s == a.seqs - 1) {
+        // Rows of no sequence have no gradient.
+        const int head = min(max(a.starts[0], 0), a.tokens), tail = min(max(a.starts[a.seqs], 0), a.tokens);
+        auto clear = [&](int from, int to) {
+            const int rows = to - from;
+            for (int i = tid; i < rows * 32; i += kThreads)
+                d.dv[(static_cast<int64_t>(from + i / 32) * a.heads + h) * a.value_dim + 32 * cb + i % 32] = 0;
+            if (cb != 0) return;
+            for (int i = tid; i < rows; i += kThreads) {
+                const int64_t at = static_cast<int64_t>(from + i) * a.heads + h;
+                d.dg[at] = 0.0f;
+                if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = 0.0f;
+                else static_cast<uint16_t*>(d.dbeta)[at] = 0;
+            }
+            if (h % a.group != 0) return;
+            for (int i = tid; i < rows * D; i += kThreads) {
+                const int64_t at = (static_cast<int64_t>(from + i / D) * a.key_heads + kh) * D + i % D;
+                d.dq[at] = 0;
+                d.dk[at] = 0;
+            }
+        };
+        if (s == 0) clear(0, head);
+        if (s == a.seqs - 1) clear(tail, a.tokens);
+    }
+    const int64_t size = static_cast<int64_t>(D) * a.value_dim;
+    f32x4 S[TPW][NC];
+    auto row_of = [&](int x, int i) {
+        const int t = wave * TPW + x;
+        return 32 * (t / 2) + 8 * g + 4 * (t % 2) + i;
+    };
+    auto state_at = [&](int x, int i) {
+        return (static_cast<int64_t>(s) * a.heads + h) * size + static_cast<int64_t>(row_of(x, i)) * a.value_dim + col;
+    };
+#pragma unroll
+    for (int x = 0; x < TPW; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) S[x][c][i] = d.d_final != nullptr ? d.d_final[state_at(x, i) + c] : 0.0f;
+    const int chunks = (seq.n + kChunk - 1) / kChunk;
+    const int64_t slot0 = scan_first_chunk(a.starts, s);
+    uint4 k[KS][PARTS], tt[2][3], pt[2][3], kt[TPW][2][PARTS], qt[TPW][2][PARTS];
+    uint32_t o[4][1];
+    f32x4 fk, fq, fu;
+    float decay = 0.0f;
+    const int r0 = 16 * wave + 4 * g;
+    auto load_k = [&](int ch) {
+        if constexpr (FP16) {
+            const int64_t at = (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes + lane * 16;
+#pragma unroll
+            for (int i = 0; i < KS * PARTS; ++i) k[i / PARTS][i % PARTS] = ldg16(w.kf + at + i * kFragBytes);
+        } else {
+            const int t = ch * kChunk + 16 * wave + n;
+            const bool in = t < seq.n;
+            const int64_t row = seq.a + (in ? t : 0);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                k[i][0] = make_uint4(0u, 0u, 0u, 0u);
+                if (in) k[i][0] = ldg16(a.k + row * a.k_token + kh * a.k_head + 32 * i + 8 * g);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = ch * kChunk + r0 + i;
+            o[i][0] = 0u;
+            if (t < seq.n)
+                load_cols<NC>(o[i], d.d_out + static_cast<int64_t>(seq.a + t) * d.d_out_token + h * d.d_out_head + col);
+        }
+        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
+        fk = *reinterpret_cast<const f32x4*>(vec + r0);
+        fq = *reinterpret_cast<const f32x4*>(vec + 64 + r0);
+        fu = *reinterpret_cast<const f32x4*>(vec + 128 + r0);
+        decay = vec[192];
+    };
+    auto load_matrices = [&](int ch) {
+        const int64_t at = ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes + lane * 16;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            if (wave < 2) {
+                tt[0][p] = ldg16(w.t + at + (upper_block(0, wave) * 3 + p) * kFragBytes);
+                pt[0][p] = ldg16(w.p + at + (upper_block(0, wave) * 3 + p) * kFragBytes);
+            }
+            tt[1][p] = ldg16(w.t + at + (upper_block(1, wave) * 3 + p) * kFragBytes);
+            pt[1][p] = ldg16(w.p + at + (upper_block(1, wave) * 3 + p) * kFragBytes);
+        }
+    };
+    auto load_transposed = [&](int ch) {
+        const int64_t by_key = (slot0 + ch) * a.key_heads + kh;
+#pragma unroll
+        for (int i = 0; i < TPW * 2 * PARTS; ++i) {
+            const int64_t at = ((by_key * (D / 16) + wave * TPW) * 2 * PARTS + i) * kFragBytes + lane * 16;
+            kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = ldg16(w.kt + at);
+            qt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = ldg16(w.qt + at);
+        }
+    };
+    if (chunks > 0) {
+        load_k(chunks - 1);
+        load_matrices(chunks - 1);
+        load_transposed(chunks - 1);
+    }
+    for (int ch = chunks - 1; ch >= 0; --ch) {
+        const int next = max(ch - 1, 0);
+        const int64_t by_head = (slot0 + ch) * a.heads + h;
+        f32x4 od[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) od[c][i] = col_value<NC, FP16>(o[i], c);
+            put_parts<PARTS>(lds.o, wave / 2, wave % 2, c, lane, od[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < TPW; ++i) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                put_parts<3>(lds.s, (wave * TPW + i) / 2, (wave * TPW + i) % 2, c, lane, S[i][c]);
+            put_rows<NC>(w.ds + by_head * 2 * size, size, a.value_dim, row_of(i, 0), col, S[i]);
+        }
+        __syncthreads();
+        f32x4 x[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            x[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    const uint4 b = lds.s[p][i][c][lane];
+#pragma unroll
+                    for (int r = 0; r < PARTS; ++r)
+                        if (r + p < 3) x[c] = mfma16x16x32(k[i][r], b, x[c]);
+                }
+            x[c] *= fu;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (2 * i + 1 < wave) continue;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint4 b = lds.o[p][i][c][lane];
+#pragma unroll
+                    for (int r = 0; r + p < 3; ++r) x[c] = mfma16x16x32(pt[i][r], b, x[c]);
+                }
+            }
+            put_parts<3>(lds.x, wave / 2, wave % 2, c, lane, x[c]);
+        }
+        const f32x4 factor_k = fk, factor_q = fq;
+        const float fade = decay;
+        load_k(next);
+        __syncthreads();
+        f32x4 dr[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            dr[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (2 * i + 1 < wave) continue;
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    const uint4 b = lds.x[p][i][c][lane];
+#pragma unroll
+                    for (int r = 0; r + p < 3; ++r) dr[c] = mfma16x16x32(tt[i][r], b, dr[c]);
+                }
+            }
+            put_parts<3>(lds.rk, wave / 2, wave % 2, c, lane, -(dr[c] * factor_k));
+            put_parts<3>(lds.oq, wave / 2, wave % 2, c, lane, od[c] * factor_q);
+        }
+        load_matrices(next);
+        put_rows<NC>(w.dr + by_head * 2 * kChunk * a.value_dim, kChunk * a.value_dim, a.value_dim, r0, col, dr);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = ch * kChunk + r0 + i;
+            if (t < seq.n)
+                *reinterpret_cast<uint32_t*>(d.dv + (static_cast<int64_t>(seq.a + t) * a.heads + h) * a.value_dim + col) =
+                    pack16_2<FP16>(dr[0][i], dr[1][i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPW; ++i)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                S[i][c] *= fade;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        const uint4 bq = lds.oq[p][j][c][lane], bk = lds.rk[p][j][c][lane];
+#pragma unroll
+                        for (int r = 0; r < PARTS; ++r)
+                            if (r + p < 3) {
+                                S[i][c] = mfma16x16x32(qt[i][j][r], bq, S[i][c]);
+                                S[i][c] = mfma16x16x32(kt[i][j][r], bk, S[i][c]);
+                            }
+                    }
+            }
+        load_transposed(next);
+    }
+    if (d.d_initial != nullptr) {
+#pragma unroll
+        for (int x = 0; x < TPW; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) d.d_initial[state_at(x, i) + c] = S[x][c][i];
+    }
+}
+
+// ---- the gradient: what does not hand on a state ------------------------------------
+
+// With S the state before a chunk, dS the gradient of that after it, and per
+// value head B1_ij = e^(G_i - G_j) do_i . u_j (j <= i), B2_ij = e^(G_i - G_j) dR_i . u_j
+// (j < i), for the normalized q and k:
+//     dq_i = scale (e^(G_i) S do_i + sum_j B1_ij k_j),
+//     dk_i = -(e^(G_i) S dR_i + sum_j B2_ij k_j) + e^(G_63 - G_i) dS u_i
+//            + sum_j (B1_ji scale q_j - B2_ji k_j),
+// the first bracket by k_i's own row, the rest by its column.  The running sum
+// G_i has the gradient q_i . dq_i + k_i . (dk_i by its row) - k_i . (dk_i by its
+// column), the last one <state after, dS> as well, and g_t the sum of those from
+// t on.  dbeta_i = w_i . du_i = u_i . dR_i / beta_i^2.
+//
+// A workgroup has a chunk and a key head and goes through its value heads; wave
+// w has the token rows of tile w, in the accumulators' layout with the columns
+// of the K^T fragments' rows.
+struct ScanInputsLds {
+    float b1[kChunk * kPitch], b2[kChunk * kPitch];   // then dq and dk, 16 bit
+    double sum[kChunk];
+    float rk[kChunk], rq[kChunk], row[kChunk], state[4];
+};
+
+__device__ __forceinline__ float sum_over_16(float v) {
+    v = v + __int_as_float(lane_xor<1>(__float_as_int(v)));
+    v = v + __int_as_float(lane_xor<2>(__float_as_int(v)));
+    v = butterfly_step4(v);
+    return butterfly_step8(v);
+}
+
+template <int D, bool FP16>
+__global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
+    constexpr int PARTS = FP16 ? 2 : 1, TILES = D / 16, RAW = D + 8;
+    __shared__ ScanInputsLds lds;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
+    const int s = find_sequence(a.starts, a.seqs, slot);
+    const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
+    const int first = (slot - scan_first_chunk(a.starts, s)) * kChunk;
+    if (first < 0 || first >= seq.n) return;
+    const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
+    const int64_t by_key = static_cast<int64_t>(slot) * a.key_heads + kh;
+    const int E = a.value_dim, r0 = 16 * wave + 4 * g;
+    if (tid < kChunk) {
+        lds.rk[tid] = w.norms[by_key * 2 * kChunk + tid];
+        lds.rq[tid] = w.norms[by_key * 2 * kChunk + kChunk + tid];
+    }
+    // Element of column n of tile t (as the fragments' rows), and the raw q and k there.
+    auto element = [&](int t) { return 32 * (t / 2) + 8 * (n / 4) + 4 * (t % 2) + n % 4; };
+    uint16_t q[TILES][4], k[TILES][4];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[t][i] = k[t][i] = 0;
+            if (r0 + i < count) {
+                q[t][i] = a.q[static_cast<int64_t>(t0 + r0 + i) * a.q_token + kh * a.q_head + element(t)];
+                k[t][i] = a.k[static_cast<int64_t>(t0 + r0 + i) * a.k_token + kh * a.k_head + element(t)];
+            }
+        }
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 dq[TILES], dk[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) dq[t] = dk[t] = zero;
+    const int64_t states = tape_states(w.slots, a.heads, D, E);
+    for (int hv = 0; hv < a.group; ++hv) {
+        const int h = kh * a.group + hv;
+        const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h, size = static_cast<int64_t>(D) * E;
+        const uint16_t* tape = reinterpret_cast<const uint16_t*>(d.tape);
+        const uint16_t* S = tape + by_head * 2 * size;
+        const uint16_t* U = tape + states + by_head * 2 * kChunk * E;
+        const uint16_t* dS = w.ds + by_head * 2 * size;
+        const uint16_t* dR = w.dr + by_head * 2 * kChunk * E;
+        if (tid < kChunk) lds.sum[tid] = w.sums[by_head * kChunk + tid];
+        f32x4 so[TILES], sr[TILES], su[TILES], ou[4], ru[4];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) so[t] = sr[t] = su[t] = zero;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) ou[t] = ru[t] = zero;
+        float both = 0.0f;   // <S, dS>, a quarter of the tiles per wave
+        for (int e = 8 * g; e < E; e += 32) {
+            const int row = 16 * wave + n;
+            uint4 o[PARTS], u[2], r[2];
+            {
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (row < count) x = ldg16(d.d_out + static_cast<int64_t>(t0 + row) * d.d_out_token + h * d.d_out_head + e);
+                if constexpr (FP16) {
+                    float f[8];
+                    unpack16<true>(x, f);
+                    Split2 p[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) o[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
+                } else {
+                    o[0] = x;
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                u[p] = ldg16(U + (p * kChunk + row) * E + e);
+                r[p] = ldg16(dR + (p * kChunk + row) * E + e);
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                uint4 bs[2], bd[2];
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    bs[p] = ldg16(S + p * size + static_cast<int64_t>(element(t)) * E + e);
+                    bd[p] = ldg16(dS + p * size + static_cast<int64_t>(element(t)) * E + e);
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int x = 0; x + p < 2; ++x) {
+                        if (x < PARTS) so[t] = mfma16x16x32(o[x], bs[p], so[t]);
+                        sr[t] = mfma16x16x32(r[x], bs[p], sr[t]);
+                        su[t] = mfma16x16x32(u[x], bd[p], su[t]);
+                    }
+                if (t % 4 == wave) {
+                    float x[8], x1[8], y[8], y1[8];
+                    unpack8(bs[0], x), unpack8(bs[1], x1), unpack8(bd[0], y), unpack8(bd[1], y1);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) both = __builtin_fmaf(x[j] + x1[j], y[j] + y1[j], both);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (t > wave) continue;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint4 b = ldg16(U + (p * kChunk + 16 * t + n) * E + e);
+#pragma unroll
+                    for (int x = 0; x + p < 2; ++x) {
+                        if (x < PARTS) ou[t] = mfma16x16x32(o[x], b, ou[t]);
+                        ru[t] = mfma16x16x32(r[x], b, ru[t]);
+                    }
+                }
+            }
+        }
+        both = wave_butterfly_sum(both);
+        if (lane == 0) lds.state[wave] = both;
+        __syncthreads();   // (sums, and the last head's matrices are done with)
+        const double last = lds.sum[kChunk - 1];
+        f32x4 decay, rest;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            decay[i] = expf(static_cast<float>(lds.sum[r0 + i]));
+            rest[i] = expf(static_cast<float>(last - lds.sum[r0 + i]));
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (t > wave) continue;
+            const int j = 16 * t + n;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = r0 + r;
+                const float fade = expf(static_cast<float>(lds.sum[i] - lds.sum[j]));
+                lds.b1[i * kPitch + j] = j <= i ? fade * ou[t][r] : 0.0f;
+                lds.b2[i * kPitch + j] = j < i ? fade * ru[t][r] : 0.0f;
+                if (i == j && i < count) {
+                    const int64_t at = static_cast<int64_t>(t0 + i) * a.heads + h, from = static_cast<int64_t>(t0 + i) * a.beta_token + h;
+                    const float b = scan_beta(a.beta_fp32 ? static_cast<const float*>(a.beta)[from]
+                                                          : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[from]));
+                    const float db = ru[t][r] / b / b;
+                    if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = db;
+                    else static_cast<uint16_t*>(d.dbeta)[at] = static_cast<uint16_t>(pack16_2<FP16>(db, 0.0f));
+                }
+            }
+        }
+        __syncthreads();
+        // The four products over tokens: rows of B1 and B2, then their columns.
+        f32x4 by_q[TILES], by_row[TILES], by_col[TILES];
+        f32x4 dot_state = zero;   // k_i . (dS u_i) e^(G_63 - G_i)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            by_q[t] = so[t] * decay;
+            by_row[t] = sr[t] * decay;
+            by_col[t] = su[t] * rest;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot_state[i] = __builtin_fmaf(elem16<FP16>(k[t][i]), by_col[t][i], dot_state[i]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            uint4 q_row[2], k_row[2], q_col[2], k_col[2];
+            const bool rows = 2 * ks <= wave, cols = 2 * ks + 1 >= wave;
+            {
+                float x[4][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int block = 2 * ks + j / 4, o = 16 * block + 4 * g + j % 4, own = 16 * wave + n;
+                    const bool low = block <= wave, high = block >= wave;
+                    const float rk = lds.rk[o], rq = lds.rq[o] * a.scale;
+                    x[0][j] = low ? lds.b1[own * kPitch + o] * rk : 0.0f;
+                    x[1][j] = low ? lds.b2[own * kPitch + o] * rk : 0.0f;
+                    x[2][j] = high ? lds.b1[o * kPitch + own] * rq : 0.0f;
+                    x[3][j] = high ? -lds.b2[o * kPitch + own] * rk : 0.0f;
+                }
+                auto parts = [&](uint4 (&to)[2], const float (&f)[8]) {
+                    Split2 p[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) to[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
+                };
+                parts(q_row, x[0]);
+                parts(k_row, x[1]);
+                parts(q_col, x[2]);
+                parts(k_col, x[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const int64_t at = ((by_key * TILES * 2 + t * 2 + ks) * PARTS + p) * kFragBytes + lane * 16;
+                    const uint4 bk = ldg16(w.kt + at), bq = ldg16(w.qt + at);
+#pragma unroll
+                    for (int x = 0; x + p < 2; ++x) {
+                        if (rows) {
+                            by_q[t] = mfma16x16x32(q_row[x], bk, by_q[t]);
+                            by_row[t] = mfma16x16x32(k_row[x], bk, by_row[t]);
+                        }
+                        if (cols) {
+                            by_col[t] = mfma16x16x32(q_col[x], bq, by_col[t]);
+                            by_col[t] = mfma16x16x32(k_col[x], bk, by_col[t]);
+                        }
+                    }
+                }
+        }
+        f32x4 dot_q = zero, dot_k = zero;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dot_q[i] = __builtin_fmaf(elem16<FP16>(q[t][i]), by_q[t][i], dot_q[i]);
+                dot_k[i] = __builtin_fmaf(elem16<FP16>(k[t][i]), -by_row[t][i] - by_col[t][i], dot_k[i]);
+            }
+            dq[t] += by_q[t];
+            dk[t] += by_col[t] - by_row[t];
+        }
+        float moved = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float rk = lds.rk[r0 + i];
+            const float sum = sum_over_16(dot_q[i] * lds.rq[r0 + i] * a.scale + dot_k[i] * rk);
+            moved += sum_over_16(dot_state[i] * rk);
+            if (n == 0) lds.row[r0 + i] = sum;
+        }
+        moved += __shfl_xor(moved, 16);
+        moved += __shfl_xor(moved, 32);
+        const float before = lds.state[0] + lds.state[1] + lds.state[2] + lds.state[3];
+        __syncthreads();
+        if (lane == 0) lds.state[wave] = moved;
+        __syncthreads();
+        if (wave == 0) {
+            // From t on: the whole less what lies before.
+            const float after = lds.state[0] + lds.state[1] + lds.state[2] + lds.state[3] +
+                                before * expf(static_cast<float>(last));
+            float x = lds.row[kChunk - 1 - lane];
+#pragma unroll
+            for (int off = 1; off < kWave; off <<= 1) {
+                const float other = __shfl_up(x, off);
+                if (lane >= off) x += other;
+            }
+            const int t = kChunk - 1 - lane;
+            if (t < count) d.dg[static_cast<int64_t>(t0 + t) * a.heads + h] = x + after;
+        }
+        __syncthreads();
+    }
+    // Through the norms, and out by rows.
+    uint16_t* out = reinterpret_cast<uint16_t*>(lds.b1);
+    for (int side = 0; side < 2; ++side) {
+        f32x4 factor, back = zero;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) factor[i] = side ? lds.rk[r0 + i] : lds.rq[r0 + i];
+        if (a.normalize) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float dot = 0.0f;
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+                    dot = __builtin_fmaf(elem16<FP16>(side ? k[t][i] : q[t][i]), side ? dk[t][i] : dq[t][i], dot);
+                back[i] = sum_over_16(dot) * factor[i] * factor[i];
+            }
+        }
+        const float by = side ? 1.0f : a.scale;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = elem16<FP16>(side ? k[t][i] : q[t][i]);
+                const float y = (side ? dk[t][i] : dq[t][i]) - x * back[i];
+                out[(r0 + i) * RAW + element(t)] = static_cast<uint16_t>(pack16_2<FP16>(y * factor[i] * by, 0.0f));
+            }
+        __syncthreads();
+        uint16_t* to = side ? d.dk : d.dq;
+        for (int i = tid; i < kChunk * D / 8; i += kThreads) {
+            const int r = i / (D / 8), e = i % (D / 8) * 8;
+            if (r < count)
+                *reinterpret_cast<uint4*>(to + (static_cast<int64_t>(t0 + r) * a.key_heads + kh) * D + e) =
+                    *reinterpret_cast<const uint4*>(out + r * RAW + e);
+        }
+        __syncthreads();
+    }
+}
+
+ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t* bytes) {
     ScanChunks w{};
-    w.slots = a.tokens / kChunk + a.seqs;
+    w.slots = scan_slots(a.tokens, a.seqs);
     w.parts = fp16 ? 2 : 1;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -544,44 +1137,88 @@ ScanChunks layout(const ScanArgs& a, bool fp16, uint8_t* base, size_t* bytes) {
         return base + here;
     };
     const size_t by_head = static_cast<size_t>(w.slots) * a.heads, by_key = static_cast<size_t>(w.slots) * a.key_heads;
+    const size_t transposed = by_key * (a.dim / 16) * 2 * w.parts * kFragBytes;
     w.t = take(by_head * kBlocks * 3 * kFragBytes);
-    w.p = take(by_head * kBlocks * 2 * kFragBytes);
+    w.p = take(by_head * kBlocks * (grad ? 3 : 2) * kFragBytes);
     w.vec = reinterpret_cast<float*>(take(by_head * 256 * sizeof(float)));
-    w.kt = take(by_key * (a.dim / 16) * 2 * w.parts * kFragBytes);
-    if (fp16) {
-        w.kf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
-        w.qf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
+    w.kt = take(transposed);
+    if (fp16) w.kf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
+    if (grad) {
+        const size_t columns = static_cast<size_t>(a.value_dim) * sizeof(uint16_t);
+        w.qt = take(transposed);
+        w.sums = reinterpret_cast<double*>(take(by_head * kChunk * sizeof(double)));
+        w.norms = reinterpret_cast<float*>(take(by_key * 2 * kChunk * sizeof(float)));
+        w.ds = reinterpret_cast<uint16_t*>(take(by_head * 2 * a.dim * columns));
+        w.dr = reinterpret_cast<uint16_t*>(take(by_head * 2 * kChunk * columns));
+    } else {
+        if (fp16) w.qf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
+        w.flags = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(a.seqs) * a.heads * (a.value_dim / 32) * 4));
     }
-    w.flags = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(a.seqs) * a.heads * (a.value_dim / 32) * 4));
     *bytes = at;
     return w;
 }
 
+// A launch holds fewer than 2^31 workgroups: slots * key_heads stay below
+// (2^14 + 2^16) 2^10.
 template <int D, bool FP16>
 void launch(const ScanArgs& a, const ScanChunks& w, hipStream_t stream) {
-    scan_prepare<D, FP16><<<static_cast<uint32_t>(w.slots) * a.key_heads, kThreads, 0, stream>>>(a, w);
+    scan_prepare<D, FP16, false><<<static_cast<uint32_t>(w.slots) * a.key_heads, kThreads, 0, stream>>>(a, w);
     const int items = a.seqs * a.heads * (a.value_dim / 32);
-    scan_chunks<D, 2, FP16><<<(items + 7) / 8 * 8, kThreads, 0, stream>>>(a, w);
+    const int grid = (items + 7) / 8 * 8;
+    if (a.tape != nullptr) scan_chunks<D, 2, FP16, true><<<grid, kThreads, 0, stream>>>(a, w);
+    else scan_chunks<D, 2, FP16, false><<<grid, kThreads, 0, stream>>>(a, w);
+}
+
+template <int D, bool FP16>
+void launch_grad(const ScanArgs& a, const ScanGradArgs& d, const ScanChunks& w, hipStream_t stream) {
+    const uint32_t chunks = static_cast<uint32_t>(w.slots) * a.key_heads;
+    scan_prepare<D, FP16, true><<<chunks, kThreads, 0, stream>>>(a, w);
+    const int items = a.seqs * a.heads * (a.value_dim / 32);
+    scan_chunks_grad<D, FP16><<<(items + 7) / 8 * 8, kThreads, 0, stream>>>(a, d, w);
+    scan_inputs_grad<D, FP16><<<chunks, kThreads, 0, stream>>>(a, d, w);
 }
 
 }  // namespace
 
 size_t scan_chunk_bytes(const ScanArgs& a, bool fp16) {
     size_t bytes = 0;
-    layout(a, fp16, nullptr, &bytes);
+    layout(a, fp16, false, nullptr, &bytes);
     return bytes;
 }
 
 hipError_t launch_scan_chunks(const ScanArgs& a, bool fp16, void* workspace, const uint32_t** flags,
                               hipStream_t stream) {
     size_t bytes = 0;
-    const ScanChunks w = layout(a, fp16, static_cast<uint8_t*>(workspace), &bytes);
+    const ScanChunks w = layout(a, fp16, false, static_cast<uint8_t*>(workspace), &bytes);
     if (a.dim == 64) {
         if (fp16) launch<64, true>(a, w, stream); else launch<64, false>(a, w, stream);
     } else {
         if (fp16) launch<128, true>(a, w, stream); else launch<128, false>(a, w, stream);
     }
     *flags = w.flags;
+    return hipGetLastError();
+}
+
+size_t delta_scan_tape_bytes(const ScanArgs& a) {
+    return static_cast<size_t>(scan_slots(a.tokens, a.seqs)) * a.heads * 2 * (a.dim + kChunk) * a.value_dim *
+           sizeof(uint16_t);
+}
+
+size_t delta_scan_grad_workspace_bytes(const ScanArgs& a, bool fp16) {
+    size_t bytes = 0;
+    layout(a, fp16, true, nullptr, &bytes);
+    return bytes;
+}
+
+hipError_t launch_delta_scan_grad(const ScanArgs& a, const ScanGradArgs& d, bool fp16, void* workspace,
+                                  hipStream_t stream) {
+    size_t bytes = 0;
+    const ScanChunks w = layout(a, fp16, true, static_cast<uint8_t*>(workspace), &bytes);
+    if (a.dim == 64) {
+        if (fp16) launch_grad<64, true>(a, d, w, stream); else launch_grad<64, false>(a, d, w, stream);
+    } else {
+        if (fp16) launch_grad<128, true>(a, d, w, stream); else launch_grad<128, false>(a, d, w, stream);
+    }
     return hipGetLastError();
 }
 

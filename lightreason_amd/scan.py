@@ -128,7 +128,13 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     passes its state on; rows of no sequence are 0; starts that are not in
     order within [0, tokens] make a sequence empty.  What is not finite reaches
     only later tokens of its sequence.  Tensors may be strided views with a
-    contiguous last dimension and strides that are multiples of 8."""
+    contiguous last dimension and strides that are multiples of 8.
+
+    Gradients flow to query, key, value, g, beta and initial, once (no second
+    derivatives); they take the same bits every time.  For them the call keeps
+    the states before every 64 tokens and u, 4 (dim + 64) value_dim / 64 bytes a
+    token and head.  The gradient of a sequence with values that are not finite
+    is not defined."""
     if scale is not None:
         scale = float(scale)
     tensors = (query, key, value, g, beta, starts, initial)
@@ -143,25 +149,72 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
         form = a, dev, shape
         _native.remember(_SCANS, key_, form)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError("delta_scan records no gradient")
-    return _scan(form, tensors)
+        return _DeltaScan.apply(form, *tensors)
+    return _scan(form, tensors)[:2]
 
 
 _SCANS: dict = {}   # arguments of a form (types, shapes, strides) that was checked, without the addresses
 
 
-def _scan(form, tensors):
+def _scan(form, tensors, taped=False):
+    """(out, final, tape): the tape only where it is asked for."""
     template, dev, shape = form
     query, key, value, g, beta, starts, initial = tensors
     a = _native.DeltaScanArgs.from_buffer_copy(template)
     out = torch.empty(value.shape, dtype=value.dtype, device=dev)
     if a.seqs == 0:
-        return out.zero_(), torch.empty(shape, dtype=torch.float32, device=dev)
+        return out.zero_(), torch.empty(shape, dtype=torch.float32, device=dev), None
     final = torch.empty(shape, dtype=torch.float32, device=dev)
     _addresses(a, query, key, value, g, beta, starts)
     a.initial, a.final, a.out = _ptr(initial), final.data_ptr(), out.data_ptr()
+    tape = None
+    if taped:
+        nbytes = int(_native.library().lrmoe_delta_scan_tape_bytes(C.addressof(a)))
+        tape = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a.tape = tape.data_ptr()
     _launch(a, dev)
-    return out, final
+    return out, final, tape
+
+
+class _DeltaScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, form, *tensors):
+        out, final, tape = _scan(form, tensors, taped=True)
+        ctx.form = form
+        ctx.first = tensors[6] is not None
+        ctx.save_for_backward(*tensors[:6], *(() if tape is None else (tape,)))
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_final):
+        template, dev, shape = ctx.form
+        query, key, value, g, beta, starts, *tape = ctx.saved_tensors
+        need = ctx.needs_input_grad   # (form, query, key, value, g, beta, starts, initial)
+        if not tape:   # no sequences
+            zeros = [torch.zeros_like(t) if n else None for t, n in zip((query, key, value, g, beta), need[1:6])]
+            first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
+            return None, *zeros, None, first
+        a = _native.DeltaScanArgs.from_buffer_copy(template)
+        _addresses(a, query, key, value, g, beta, starts)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value, g, beta)]
+        first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
+        d = _native.DeltaGradArgs(tape=tape[0].data_ptr(), d_initial=_ptr(first))
+        # Of a gradient that torch hands in, expanded or transposed, a plain copy is taken.
+        bad = d_out.stride(-1) != 1 or d_out.data_ptr() % 16 or any(x % 8 for x in d_out.stride()[:-1])
+        d_out = d_out.contiguous() if bad else d_out
+        d_final = d_final.contiguous()
+        d_final = d_final.clone() if d_final.data_ptr() % 16 else d_final
+        d.d_out_token_stride, d.d_out_head_stride = _strides(d_out)
+        d.d_final = d_final.data_ptr()
+        if a.tokens:
+            d.d_out, d.dq, d.dk, d.dv, d.dg, d.dbeta = (t.data_ptr() for t in (d_out, *grads))
+        with _on(dev):
+            nbytes = int(_native.library().lrmoe_delta_scan_grad_workspace_bytes(C.addressof(a)))
+            ws = _native.workspace(dev, nbytes)
+            _native.call("lrmoe_delta_scan_grad", C.addressof(a), C.addressof(d), ws.data_ptr(), ws.numel(),
+                         _stream(dev))
+        return None, *(t if n else None for t, n in zip(grads, need[1:6])), None, first
 
 
 # ---- steps over a pool of states ------------------------------------------------

@@ -16,7 +16,8 @@ BF = torch.bfloat16
 
 def test_structures_match_the_header():
     text = (Path(__file__).resolve().parents[1] / "include" / "lrmoe.h").read_text()
-    for name, struct in (("lrmoe_delta_scan_args", _native.DeltaScanArgs),):
+    for name, struct in (("lrmoe_delta_scan_args", _native.DeltaScanArgs),
+                         ("lrmoe_delta_grad_args", _native.DeltaGradArgs)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
         fields = []
@@ -79,6 +80,22 @@ def test_c_entry_points_refuse_misuse():
     assert call(out_head_stride=32) == _native.LRMOE_E_ARG
     assert call(q=1 << 26, k=1 << 27, out=(1 << 26) + 8, value_dim=128, v_token_stride=512, v_head_stride=128,
                 out_token_stride=512, out_head_stride=128) == _native.LRMOE_E_ARG
+
+    back = dict(d_out=256, tape=256, dq=256, dk=256, dv=256, dg=256, dbeta=256, d_out_token_stride=256,
+                d_out_head_stride=64)
+
+    def gradient(nbytes=1 << 40, workspace=ws, args=(), **kw):
+        a = _native.DeltaScanArgs(**{**good, **dict(args)})
+        d = _native.DeltaGradArgs(**{**back, **kw})
+        return lib.lrmoe_delta_scan_grad(C.addressof(a), C.addressof(d), workspace, nbytes, None)
+    for kw in (dict(d_out=None), dict(tape=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(dg=None),
+               dict(dbeta=None), dict(dq=264), dict(d_final=264), dict(d_initial=264), dict(tape=320),
+               dict(d_out_token_stride=4), dict(args=dict(slots=256)), dict(args=dict(into=256)),
+               dict(args=dict(fresh=256)), dict(args=dict(pool=2)), dict(args=dict(dim=32)), dict(args=dict(q=None)),
+               dict(workspace=None)):
+        assert gradient(**kw) == _native.LRMOE_E_ARG, kw
+    assert gradient(nbytes=0) == _native.LRMOE_E_WORKSPACE
+    assert gradient(args=dict(seqs=0, pool=0)) == 0
 
     p = C.c_void_p(256)
     assert lib.lrmoe_beam_workspace_bytes(1, 33, 10) == 0 and lib.lrmoe_beam_workspace_bytes(1, 4, 10) > 0
