@@ -47,11 +47,16 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* fl
     const int blocks = a.value_dim / 32;
     const int64_t wave = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kWave;
     if (wave >= static_cast<int64_t>(a.seqs) * a.heads * blocks) return;
-    if (flags != nullptr && flags[wave] == 0) return;
+    uint32_t marks[2] = {1u, 1u};   // of the wave's first and last 16 columns
+    if (flags != nullptr) {
+        marks[0] = flags[2 * wave], marks[1] = flags[2 * wave + 1];
+        if ((marks[0] | marks[1]) == 0) return;
+    }
     const int cb = static_cast<int>(wave % blocks);
     const int h = static_cast<int>(wave / blocks % a.heads), s = static_cast<int>(wave / blocks / a.heads);
     const int kh = h / a.group;
     const int rows0 = ROWS * (lane / 8), col = 32 * cb + 4 * (lane % 8);
+    const bool marked = marks[lane % 8 / 4] != 0;
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
     // Rows of no sequence.
     if (a.clear && flags == nullptr && (s == 0 || s == a.seqs - 1)) {
@@ -127,10 +132,11 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* fl
         for (int i = 0; i < ROWS; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) S[i][j] = __builtin_fmaf(k[i], u[j], decay * S[i][j]);
-        if (lane < 8)
+        if (lane < 8 && marked)
             *reinterpret_cast<uint2*>(a.out + t * a.out_token + h * a.out_head + col) =
                 make_uint2(pack16_2<FP16>(out[0], out[1]), pack16_2<FP16>(out[2], out[3]));
     }
+    if (!marked) return;
     float* p = a.final + (static_cast<int64_t>(into) * a.heads + h) * state_size +
                static_cast<int64_t>(rows0) * a.value_dim + col;
 #pragma unroll

@@ -47,6 +47,8 @@ __device__ __forceinline__ int find_sequence(const int32_t* starts, int seqs, in
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+__device__ __forceinline__ float power(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
+
 __device__ __forceinline__ double wave_scan_f64(double v) {
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
@@ -66,37 +68,53 @@ struct PrepareLds {
     float beta[kChunk], rk[kChunk], rq[kChunk];
 };
 
+// The value of lane L of a lane's row of 16.
+template <int L>
+__device__ __forceinline__ float row_lane(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + L, 0xf, 0xf, false));
+}
+// Subtracts row L's multiple from the rows below it.
+template <int L>
+__device__ __forceinline__ void eliminate(const float (&m)[16], float (&x)[4]) {
+    if constexpr (L < 15) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = __builtin_fmaf(-m[L], row_lane<L>(x[c]), x[c]);
+        eliminate<L + 1>(m, x);
+    }
+}
+
 // t = (I + a)^-1 for the strictly lower triangular a, by blocks of 16: those of
-// the diagonal by substitution, a lane per column; below, block column by block
-// column, T_ij = -T_ii sum_k A_ik T_kj with fp32 matrix instructions, a wave per
-// block column.
+// the diagonal by substitution, a wave per block, lane n of group g with row n
+// and columns 4 g .. + 3 (a row is handed to the others by a DPP broadcast);
+// below, block column by block column, T_ij = -T_ii sum_k A_ik T_kj with fp32
+// matrix instructions, a wave per block column.
 __device__ __forceinline__ void invert(PrepareLds& lds, int wave, int lane) {
     const int n = lane % 16, g = lane / 16;
-    float x[16];
+    {
+        float m[16], x[4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        float acc = r == n ? 1.0f : 0.0f;
-        const float* row = lds.a + (16 * wave + r) * kPitch + 16 * wave;
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(lds.a + (16 * wave + n) * kPitch + 16 * wave + 4 * i);
 #pragma unroll
-        for (int l = 0; l < r; ++l) acc = __builtin_fmaf(-row[l], x[l], acc);
-        x[r] = acc;
+            for (int j = 0; j < 4; ++j) m[4 * i + j] = v[j];
+            x[i] = n == 4 * g + i ? 1.0f : 0.0f;
+        }
+        eliminate<0>(m, x);
+        *reinterpret_cast<f32x4*>(lds.t + (16 * wave + n) * kPitch + 16 * wave + 4 * g) = (f32x4){x[0], x[1], x[2], x[3]};
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (r / 4 == g) lds.t[(16 * wave + r) * kPitch + 16 * wave + n] = x[r];
     __syncthreads();
     const int j = wave;
     for (int i = j + 1; i < 4; ++i) {
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = j; k < i; ++k) {
-            const float* row = lds.a + (16 * i + n) * kPitch + 16 * k + 4 * g;
+            const f32x4 row = *reinterpret_cast<const f32x4*>(lds.a + (16 * i + n) * kPitch + 16 * k + 4 * g);
             const float* col = lds.t + (16 * k + 4 * g) * kPitch + 16 * j + n;
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 acc = __builtin_amdgcn_mfma_f32_16x16x4f32(row[s], col[s * kPitch], acc, 0, 0, 0);
         }
         f32x4 out = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float* row = lds.t + (16 * i + n) * kPitch + 16 * i + 4 * g;
+        const f32x4 row = *reinterpret_cast<const f32x4*>(lds.t + (16 * i + n) * kPitch + 16 * i + 4 * g);
 #pragma unroll
         for (int s = 0; s < 4; ++s) out = __builtin_amdgcn_mfma_f32_16x16x4f32(row[s], acc[s], out, 0, 0, 0);
 #pragma unroll
@@ -124,7 +142,8 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
     constexpr int RAW = D + 8;   // 16-bit elements of a row in LDS
     constexpr int PARTS = FP16 ? 2 : 1;
     __shared__ PrepareLds lds;
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
     const int s = find_sequence(a.starts, a.seqs, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
@@ -220,16 +239,18 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
                 b = a.beta_fp32 ? static_cast<const float*>(a.beta)[t * a.beta_token + h]
                                 : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[t * a.beta_token + h]);
             }
-            const double sum = wave_scan_f64(gl);
+            // (In powers of two.)
+            const double sum = wave_scan_f64(gl * 1.4426950408889634);
             lds.sum[lane] = sum;
             lds.beta[lane] = lane < count ? scan_beta(b) : 0.0f;
             if constexpr (GRAD) w.sums[by_head * kChunk + lane] = sum;
             const double last = __shfl(sum, kWave - 1);
-            const float decay = expf(static_cast<float>(sum)), rest = expf(static_cast<float>(last - sum));
+            const float decay = power(sum), rest = power(last - sum);
             float* vec = w.vec + by_head * 256;
-            vec[lane] = decay * lds.rk[lane];
-            vec[64 + lane] = decay * lds.rq[lane] * a.scale;
-            vec[128 + lane] = rest * lds.rk[lane];
+            const bool in = lane < count;   // (rows past the sequence repeat its last one)
+            vec[lane] = in ? decay * lds.rk[lane] : 0.0f;
+            vec[64 + lane] = in ? decay * lds.rq[lane] * a.scale : 0.0f;
+            vec[128 + lane] = in ? rest * lds.rk[lane] : 0.0f;
             if (lane == kWave - 1) vec[192] = decay;
         }
         __syncthreads();
@@ -240,7 +261,7 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * wave + 4 * g + r;
-                const float fade = expf(static_cast<float>(lds.sum[i] - lds.sum[j])) * lds.rk[j];
+                const float fade = power(lds.sum[i] - lds.sum[j]) * lds.rk[j];
                 lds.a[i * kPitch + j] = j < i ? fade * lds.rk[i] * lds.beta[j] * kk[t][r] : 0.0f;
                 lds.b[i * kPitch + j] = j <= i ? fade * lds.rq[i] * a.scale * qk[t][r] : 0.0f;
             }
@@ -336,14 +357,11 @@ struct ScanLoads {
 };
 
 template <int NC>
-__device__ __forceinline__ void load_cols(uint32_t (&v)[NC / 2 + NC % 2], const uint16_t* p) {
-    if constexpr (NC == 1) v[0] = *p;
-    if constexpr (NC == 2) v[0] = *reinterpret_cast<const uint32_t*>(p);
-    if constexpr (NC == 4) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        v[0] = x.x, v[1] = x.y;
-    }
+__device__ __forceinline__ void load_cols(uint32_t (&v)[NC / 2 + NC % 2], const uint8_t* p, uint32_t at) {
+    if constexpr (NC == 1) v[0] = *reinterpret_cast<const uint16_t*>(p + at);
+    if constexpr (NC == 2) v[0] = *reinterpret_cast<const uint32_t*>(p + at);
 }
+__device__ __forceinline__ uint4 frag16(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint4*>(p + at); }
 template <int NC, bool FP16>
 __device__ __forceinline__ float col_value(const uint32_t (&v)[NC / 2 + NC % 2], int c) {
     return elem16<FP16>(static_cast<uint16_t>(c % 2 ? v[c / 2] >> 16 : v[c / 2]));
@@ -353,7 +371,8 @@ template <int D, int NC, bool FP16, bool TAPE>
 __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32;
     __shared__ ScanLds<D, NC> lds;
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     // Blocks of one head, and of one key head, on the same XCD.
     const int blocks = a.value_dim / (16 * NC), per = (gridDim.x + 7) / 8;
     const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
@@ -370,12 +389,12 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             for (int i = tid; i < (a.tokens - tail) * 16 * NC; i += kThreads)
                 row[(tail + i / (16 * NC)) * a.out_token + i % (16 * NC)] = 0;
     }
-    uint32_t* flag = w.flags + (static_cast<int64_t>(s) * a.heads + h) * (a.value_dim / 32) + 16 * NC * cb / 32;
+    uint32_t* flag = w.flags + (static_cast<int64_t>(s) * a.heads + h) * (a.value_dim / 16) + NC * cb;
     const int into = scan_slot(a.into, s, a.pool);
     const bool fresh = a.initial == nullptr || (a.fresh != nullptr && a.fresh[s] != 0);
     const int from = fresh ? 0 : scan_slot(a.from, s, a.pool);
     if (into < 0 || from < 0) {
-        if (tid == 0) *flag = 0;
+        if (tid < NC) flag[tid] = 0;
         return;
     }
     const int64_t size = static_cast<int64_t>(D) * a.value_dim;
@@ -399,66 +418,81 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
     uint16_t* tape_s = reinterpret_cast<uint16_t*>(a.tape);
     uint16_t* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
     ScanLoads<D, NC, FP16> x;
+    // Addresses are a scalar base per chunk and offsets of 32 bits; rows past the
+    // sequence repeat its last one (their factors are 0, and their u).
+    const int r0 = 16 * wave + 4 * g;
+    const uint32_t frag = lane * 16;
     auto load_rows = [&](int ch) {
         if constexpr (FP16) {
-            const int64_t at = (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes + lane * 16;
+            const int64_t at = (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes;
 #pragma unroll
             for (int i = 0; i < KS * PARTS; ++i) {
-                x.k[i / PARTS][i % PARTS] = ldg16(w.kf + at + i * kFragBytes);
-                x.q[i / PARTS][i % PARTS] = ldg16(w.qf + at + i * kFragBytes);
+                x.k[i / PARTS][i % PARTS] = frag16(w.kf + at + i * kFragBytes, frag);
+                x.q[i / PARTS][i % PARTS] = frag16(w.qf + at + i * kFragBytes, frag);
             }
         } else {
-            const int t = ch * kChunk + 16 * wave + n;
-            const bool in = t < seq.n;
-            const int64_t row = seq.a + (in ? t : 0);
+            const int64_t t = seq.a + ch * kChunk;
+            const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k + t * a.k_token + kh * a.k_head);
+            const uint8_t* q = reinterpret_cast<const uint8_t*>(a.q + t * a.q_token + kh * a.q_head);
+            const uint32_t row = min(16 * wave + n, seq.n - 1 - ch * kChunk);
+            const uint32_t k_at = row * (2 * static_cast<uint32_t>(a.k_token)) + 16 * g;
+            const uint32_t q_at = row * (2 * static_cast<uint32_t>(a.q_token)) + 16 * g;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                x.k[i][0] = x.q[i][0] = make_uint4(0u, 0u, 0u, 0u);
-                if (in) {
-                    x.k[i][0] = ldg16(a.k + row * a.k_token + kh * a.k_head + 32 * i + 8 * g);
-                    x.q[i][0] = ldg16(a.q + row * a.q_token + kh * a.q_head + 32 * i + 8 * g);
-                }
+                x.k[i][0] = frag16(k + 64 * i, k_at);
+                x.q[i][0] = frag16(q + 64 * i, q_at);
             }
+        }
+    };
+    auto load_values = [&](int ch) {
+        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
+        x.fk = *reinterpret_cast<const f32x4*>(vec + r0);
+        const uint8_t* v = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
+                                                            h * a.v_head + 16 * NC * cb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t row = min(r0 + i, seq.n - 1 - ch * kChunk);
+            load_cols<NC>(x.v[i], v, row * (2 * static_cast<uint32_t>(a.v_token)) + 2 * NC * n);
         }
     };
     auto load_t = [&](int ch) {
-        const int64_t at = (((slot0 + ch) * a.heads + h) * kBlocks) * 3 * kFragBytes + lane * 16;
+        const uint8_t* t = w.t + ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes;
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-            x.t[0][p] = ldg16(w.t + at + (lower_block(0, wave) * 3 + p) * kFragBytes);
-            if (wave >= 2) x.t[1][p] = ldg16(w.t + at + (lower_block(1, wave) * 3 + p) * kFragBytes);
+            x.t[0][p] = frag16(t + (lower_block(0, wave) * 3 + p) * kFragBytes, frag);
+            x.t[1][p] = frag16(t + (lower_block(1, max(wave, 2)) * 3 + p) * kFragBytes, frag);
         }
     };
-    auto load_rest = [&](int ch) {
-        const int64_t by_head = (slot0 + ch) * a.heads + h, by_key = (slot0 + ch) * a.key_heads + kh;
-        const int64_t at = by_head * kBlocks * 2 * kFragBytes + lane * 16;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            x.p[0][p] = ldg16(w.p + at + (lower_block(0, wave) * 2 + p) * kFragBytes);
-            if (wave >= 2) x.p[1][p] = ldg16(w.p + at + (lower_block(1, wave) * 2 + p) * kFragBytes);
-        }
-#pragma unroll
-        for (int i = 0; i < TPW * 2 * PARTS; ++i)
-            x.kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] =
-                ldg16(w.kt + ((by_key * (D / 16) + wave * TPW) * 2 * PARTS + i) * kFragBytes + lane * 16);
-        const float* vec = w.vec + by_head * 256;
-        const int r0 = 16 * wave + 4 * g;
-        x.fk = *reinterpret_cast<const f32x4*>(vec + r0);
+    auto load_factors = [&](int ch) {
+        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
         x.fq = *reinterpret_cast<const f32x4*>(vec + 64 + r0);
         x.fu = *reinterpret_cast<const f32x4*>(vec + 128 + r0);
         x.decay = vec[192];
+    };
+    auto load_rest = [&](int ch) {
+        const int64_t by_head = (slot0 + ch) * a.heads + h, by_key = (slot0 + ch) * a.key_heads + kh;
+        const uint8_t* at = w.p + by_head * kBlocks * 2 * kFragBytes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = ch * kChunk + r0 + i;
-#pragma unroll
-            for (int c = 0; c < NC / 2 + NC % 2; ++c) x.v[i][c] = 0u;
-            if (t < seq.n) load_cols<NC>(x.v[i], a.v + static_cast<int64_t>(seq.a + t) * a.v_token + h * a.v_head + col);
+        for (int p = 0; p < 2; ++p) {
+            x.p[0][p] = frag16(at + (lower_block(0, wave) * 2 + p) * kFragBytes, frag);
+            x.p[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * 2 + p) * kFragBytes, frag);
         }
+        const uint8_t* kt = w.kt + ((by_key * (D / 16) + wave * TPW) * 2 * PARTS) * kFragBytes;
+#pragma unroll
+        for (int i = 0; i < TPW * 2 * PARTS; ++i)
+            x.kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(kt + i * kFragBytes, frag);
     };
     if (chunks > 0) {
+        // (In the loop's order, so that its waits count the same loads.)
         load_rows(0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(0);
+        __builtin_amdgcn_sched_barrier(0);
         load_t(0);
+        load_factors(0);
+        __builtin_amdgcn_sched_barrier(0);
         load_rest(0);
+        __builtin_amdgcn_sched_barrier(0);
     }
     bool odd = false;   // a number that is not finite
     for (int ch = 0; ch < chunks; ++ch) {
@@ -491,7 +525,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                         if (r + p < 2) qs[c] = mfma16x16x32(x.q[i][r], b, qs[c]);
                     }
                 }
+        __builtin_amdgcn_sched_barrier(0);
         load_rows(next);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             f32x4 r;
@@ -499,6 +535,8 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             for (int i = 0; i < 4; ++i) r[i] = col_value<NC, FP16>(x.v[i], c) - x.fk[i] * ks[c][i];
             put_parts<3>(lds.r, wave / 2, wave % 2, c, lane, r);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(next);
         __syncthreads();
         f32x4 u[NC];
 #pragma unroll
@@ -515,7 +553,11 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
         load_t(next);
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 fq = x.fq;
+        const float decay = x.decay;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -523,6 +565,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
             put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * x.fu);
         }
+        load_factors(next);
         if constexpr (TAPE)
             put_rows<NC>(tape_u + taped * 2 * kChunk * a.value_dim, kChunk * a.value_dim, a.value_dim, 16 * wave + 4 * g,
                          col, u);
@@ -531,7 +574,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                S[i][c] *= x.decay;
+                S[i][c] *= decay;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -545,7 +588,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
         f32x4 o[NC];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            o[c] = qs[c] * x.fq;
+            o[c] = qs[c] * fq;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 if (2 * k > wave) continue;
@@ -557,6 +600,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_rest(next);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = ch * kChunk + 16 * wave + 4 * g + i;
@@ -564,22 +610,18 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             uint16_t* to = a.out + static_cast<int64_t>(seq.a + t) * a.out_token + h * a.out_head + col;
             if constexpr (NC == 1) {
                 *to = static_cast<uint16_t>(pack16_2<FP16>(o[0][i], 0.0f));
-            } else if constexpr (NC == 2) {
-                *reinterpret_cast<uint32_t*>(to) = pack16_2<FP16>(o[0][i], o[1][i]);
             } else {
-                *reinterpret_cast<uint2*>(to) =
-                    make_uint2(pack16_2<FP16>(o[0][i], o[1][i]), pack16_2<FP16>(o[NC - 2][i], o[NC - 1][i]));
+                *reinterpret_cast<uint32_t*>(to) = pack16_2<FP16>(o[0][i], o[1][i]);
             }
         }
-        load_rest(next);
     }
     // Where a value was not finite, a product's zero weights have let it through
     // to earlier tokens: the next launch goes through these columns again.
     if (__syncthreads_or(odd)) {
-        if (tid == 0) *flag = 1;
+        if (tid < NC) flag[tid] = 1;
         return;
     }
-    if (tid == 0) *flag = 0;
+    if (tid < NC) flag[tid] = 0;
 #pragma unroll
     for (int x1 = 0; x1 < TPW; ++x1)
 #pragma unroll
@@ -609,7 +651,8 @@ template <int D, bool FP16>
 __global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32, NC = 2;
     __shared__ ScanGradLds<D, NC, PARTS> lds;
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int blocks = a.value_dim / (16 * NC), per = (gridDim.x + 7) / 8;
     const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
     if (item >= a.seqs * a.heads * blocks) return;
@@ -682,7 +725,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, Scan
             const int t = ch * kChunk + r0 + i;
             o[i][0] = 0u;
             if (t < seq.n)
-                load_cols<NC>(o[i], d.d_out + static_cast<int64_t>(seq.a + t) * d.d_out_token + h * d.d_out_head + col);
+                load_cols<NC>(o[i], reinterpret_cast<const uint8_t*>(d.d_out + static_cast<int64_t>(seq.a + t) * d.d_out_token + h * d.d_out_head + col), 0);
         }
         const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
         fk = *reinterpret_cast<const f32x4*>(vec + r0);
@@ -854,7 +897,8 @@ template <int D, bool FP16>
 __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TILES = D / 16, RAW = D + 8;
     __shared__ ScanInputsLds lds;
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
     const int s = find_sequence(a.starts, a.seqs, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
@@ -967,8 +1011,8 @@ __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, Scan
         f32x4 decay, rest;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            decay[i] = expf(static_cast<float>(lds.sum[r0 + i]));
-            rest[i] = expf(static_cast<float>(last - lds.sum[r0 + i]));
+            decay[i] = power(lds.sum[r0 + i]);
+            rest[i] = power(last - lds.sum[r0 + i]);
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -977,7 +1021,7 @@ __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, Scan
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = r0 + r;
-                const float fade = expf(static_cast<float>(lds.sum[i] - lds.sum[j]));
+                const float fade = power(lds.sum[i] - lds.sum[j]);
                 lds.b1[i * kPitch + j] = j <= i ? fade * ou[t][r] : 0.0f;
                 lds.b2[i * kPitch + j] = j < i ? fade * ru[t][r] : 0.0f;
                 if (i == j && i < count) {
@@ -1077,7 +1121,7 @@ __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, Scan
         if (wave == 0) {
             // From t on: the whole less what lies before.
             const float after = lds.state[0] + lds.state[1] + lds.state[2] + lds.state[3] +
-                                before * expf(static_cast<float>(last));
+                                before * power(last);
             float x = lds.row[kChunk - 1 - lane];
 #pragma unroll
             for (int off = 1; off < kWave; off <<= 1) {
@@ -1152,7 +1196,7 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
         w.dr = reinterpret_cast<uint16_t*>(take(by_head * 2 * kChunk * columns));
     } else {
         if (fp16) w.qf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
-        w.flags = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(a.seqs) * a.heads * (a.value_dim / 32) * 4));
+        w.flags = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(a.seqs) * a.heads * (a.value_dim / 16) * 4));
     }
     *bytes = at;
     return w;
@@ -1166,6 +1210,7 @@ void launch(const ScanArgs& a, const ScanChunks& w, hipStream_t stream) {
     const int items = a.seqs * a.heads * (a.value_dim / 32);
     const int grid = (items + 7) / 8 * 8;
     if (a.tape != nullptr) scan_chunks<D, 2, FP16, true><<<grid, kThreads, 0, stream>>>(a, w);
+    else if (items <= 128) scan_chunks<D, 1, FP16, false><<<(2 * items + 7) / 8 * 8, kThreads, 0, stream>>>(a, w);
     else scan_chunks<D, 2, FP16, false><<<grid, kThreads, 0, stream>>>(a, w);
 }
 
