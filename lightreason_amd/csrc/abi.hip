@@ -1111,7 +1111,9 @@ int lrmoe_delta_scan_grad(const lrmoe_delta_scan_args* p, const lrmoe_delta_grad
                           static_cast<const void*>(d->dv), static_cast<const void*>(d->dg),
                           static_cast<const void*>(d->dbeta), static_cast<const void*>(d->d_initial)})
         if (misaligned(x, 16)) return LRMOE_E_ARG;
-    if (d->d_out_token_stride % 8 != 0 || d->d_out_head_stride % 8 != 0) return LRMOE_E_ARG;
+    if (d->d_out_token_stride % 8 != 0 || d->d_out_head_stride % 8 != 0 || d->d_out_token_stride < 0 ||
+        d->d_out_token_stride >= (1 << 23))
+        return LRMOE_E_ARG;
     if (!workspace) return LRMOE_E_ARG;
     if (workspace_bytes < lrmoe_delta_scan_grad_workspace_bytes(p)) return LRMOE_E_WORKSPACE;
     if (int e = check_device()) return e;

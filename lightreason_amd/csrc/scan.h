@@ -82,7 +82,7 @@ struct ScanChunks {
     // For the gradient: t and p hold the transposed matrices, 3 parts each, and
     double* sums;          // [slots][heads][64]: running sums of g
     float* norms;          // [slots][key_heads][128]: factors of k and of q
-    uint16_t *ds, *dr;     // [slots][heads][2][dim][value_dim], [slots][heads][2][64][value_dim]
+    float *ds, *dr;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
 };
 
 // A beta of 0 is taken as 2^-40: u = beta w then still tells w, which beta's
@@ -92,32 +92,25 @@ __device__ __forceinline__ float scan_beta(float b) {
 }
 
 __host__ __device__ __forceinline__ int scan_slots(int tokens, int seqs) { return tokens / kChunk + seqs; }
-// The tape: states in two bf16 parts [slots][heads][2][dim][value_dim], then u
-// [slots][heads][2][64][value_dim].
+// The tape, fp32: states [slots][heads][dim][value_dim], then u [slots][heads][64]
+// [value_dim].
 __host__ __device__ __forceinline__ int64_t tape_states(int64_t slots, int heads, int dim, int value_dim) {
-    return slots * heads * 2 * dim * value_dim;
+    return slots * heads * dim * value_dim;
 }
 
-// An fp32 number as three bf16 ones, each the upper half of the bits that are
-// left: their sum is the number (24 bits), of two the first 16 bits.
+// An fp32 number as the sum of bf16 ones, each the rest rounded to nearest: two
+// are within 2^-17 of it, three all of its 24 bits.
 struct Split2 {
-    uint32_t part[3];   // bf16 pairs
+    uint32_t part[3];   // pairs
 };
-__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
-    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 template <int PARTS>
 __device__ __forceinline__ Split2 split2(float lo, float hi) {
     Split2 s;
-    s.part[0] = high_halves(lo, hi);
-    if constexpr (PARTS > 1) {
-        lo -= high_part(lo), hi -= high_part(hi);
-        s.part[1] = high_halves(lo, hi);
-    }
-    if constexpr (PARTS > 2) {
-        lo -= high_part(lo), hi -= high_part(hi);
-        s.part[2] = high_halves(lo, hi);
+    s.part[0] = pack_bf2(lo, hi);
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) {
+        lo -= lo_bf(s.part[p - 1]), hi -= hi_bf(s.part[p - 1]);
+        s.part[p] = pack_bf2(lo, hi);
     }
     return s;
 }

@@ -47,6 +47,8 @@ __device__ __forceinline__ int find_sequence(const int32_t* starts, int seqs, in
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+__device__ __forceinline__ uint4 frag16(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint4*>(p + at); }
+
 __device__ __forceinline__ float power(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
 
 __device__ __forceinline__ double wave_scan_f64(double v) {
@@ -310,18 +312,7 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
 
 // ---- launch two: chunk after chunk -----------------------------------------------
 
-// A workgroup has 16 NC columns of a state; wave w its rows of the tiles w TPW
-// .. + TPW - 1, in the accumulators of the state's own update (column NC n + c
-// of the block in lane n of a group and tile c).  A step's products hand their
-// results on through LDS, as the B fragments of the next ones, which the lanes
-// write as they hold them.
-template <int D, int NC>
-struct ScanLds {
-    uint4 s[3][D / 32][NC][kWave];
-    uint4 r[3][2][NC][kWave];
-    uint4 u[2][2][NC][kWave];    // for the outputs
-    uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
-};
+constexpr int kChainThreads = 512;
 
 // Four values of a lane as half a B fragment (element 4 half on), in parts.
 template <int PARTS, int KS, int NC>
@@ -332,64 +323,81 @@ __device__ __forceinline__ void put_parts(uint4 (&to)[PARTS][KS][NC][kWave], int
         reinterpret_cast<uint2*>(&to[p][ks][c][lane])[half] = make_uint2(lo.part[p], hi.part[p]);
 }
 
-// Four rows of a lane's columns, from row `row` on, as two bf16 parts of a
-// [rows][value_dim] matrix, `apart` elements from part to part.
+// Four rows of a lane's NC columns of an fp32 matrix [rows][value_dim].
 template <int NC>
-__device__ __forceinline__ void put_rows(uint16_t* to, int64_t apart, int value_dim, int row, int col,
-                                         const f32x4 (&x)[NC]) {
-    static_assert(NC == 2, "pairs of columns");
+__device__ __forceinline__ void put_rows(float* to, int value_dim, const f32x4 (&x)[NC]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const Split2 s = split2<2>(x[0][i], x[1][i]);
-        uint16_t* p = to + static_cast<int64_t>(row + i) * value_dim + col;
-        *reinterpret_cast<uint32_t*>(p) = s.part[0];
-        *reinterpret_cast<uint32_t*>(p + apart) = s.part[1];
+        if constexpr (NC == 1) to[i * value_dim] = x[0][i];
+        else *reinterpret_cast<float2*>(to + i * value_dim) = make_float2(x[0][i], x[1][i]);
     }
 }
 
-template <int D, int NC, bool FP16>
-struct ScanLoads {
-    static constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64;
-    uint4 k[D / 32][PARTS], q[D / 32][PARTS], t[2][3], p[2][2], kt[TPW][2][PARTS];
-    uint32_t v[4][NC / 2 + NC % 2];
-    f32x4 fk, fq, fu;   // factors of the lane's four tokens
-    float decay;
+// The NC 16-bit values of a lane's columns, and one of them.
+template <int NC>
+__device__ __forceinline__ uint32_t load_cols(const uint8_t* p, uint32_t at) {
+    if constexpr (NC == 1) return *reinterpret_cast<const uint16_t*>(p + at);
+    return *reinterpret_cast<const uint32_t*>(p + at);
+}
+template <bool FP16>
+__device__ __forceinline__ float col_value(uint32_t v, int c) {
+    return elem16<FP16>(static_cast<uint16_t>(c ? v >> 16 : v));
+}
+template <int NC, bool FP16>
+__device__ __forceinline__ void store_cols(uint16_t* to, const f32x4 (&x)[NC], int i) {
+    if constexpr (NC == 1) *to = static_cast<uint16_t>(pack16_2<FP16>(x[0][i], 0.0f));
+    else *reinterpret_cast<uint32_t*>(to) = pack16_2<FP16>(x[0][i], x[1][i]);
+}
+
+// A workgroup's part of the work: a sequence, a value head and 16 NC columns.
+// Blocks of one head, and of one key head, are on the same XCD, whose cache
+// holds the fragments that they share.
+struct ScanItem {
+    int s, h, cb;
+    bool in;
+};
+__device__ __forceinline__ ScanItem scan_item(const ScanArgs& a, int columns) {
+    const int blocks = a.value_dim / columns, per = gridDim.x / 8;
+    const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
+    return {item / blocks / a.heads, item / blocks % a.heads, item % blocks, item < a.seqs * a.heads * blocks};
+}
+
+// Waves 0 to 3 have the state's rows of the tiles w TPW .. + TPW - 1, in the
+// accumulators of its own update (column NC n + c of the block in lane n of a
+// group and tile c), and the token rows of tile w on the way there; waves 4 to
+// 7 the outputs of those rows. The products hand their results on through LDS,
+// as the B fragments of the next ones, which the lanes write as they hold them.
+// A step is a chain of three products and hand-overs, and the instructions of
+// one wave on each SIMD; the outputs fill the gaps.
+template <int D, int NC>
+struct ScanLds {
+    uint4 s[3][D / 32][NC][kWave];
+    uint4 r[3][2][NC][kWave];
+    uint4 u[2][2][NC][kWave];    // for the outputs
+    uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
 };
 
-template <int NC>
-__device__ __forceinline__ void load_cols(uint32_t (&v)[NC / 2 + NC % 2], const uint8_t* p, uint32_t at) {
-    if constexpr (NC == 1) v[0] = *reinterpret_cast<const uint16_t*>(p + at);
-    if constexpr (NC == 2) v[0] = *reinterpret_cast<const uint32_t*>(p + at);
-}
-__device__ __forceinline__ uint4 frag16(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint4*>(p + at); }
-template <int NC, bool FP16>
-__device__ __forceinline__ float col_value(const uint32_t (&v)[NC / 2 + NC % 2], int c) {
-    return elem16<FP16>(static_cast<uint16_t>(c % 2 ? v[c / 2] >> 16 : v[c / 2]));
-}
-
 template <int D, int NC, bool FP16, bool TAPE>
-__global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunks w) {
+__global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32;
     __shared__ ScanLds<D, NC> lds;
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    // Blocks of one head, and of one key head, on the same XCD.
-    const int blocks = a.value_dim / (16 * NC), per = (gridDim.x + 7) / 8;
-    const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
-    if (item >= a.seqs * a.heads * blocks) return;
-    const int cb = item % blocks, h = item / blocks % a.heads, s = item / blocks / a.heads, kh = h / a.group;
-    const int col = 16 * NC * cb + NC * n;
+    const int role = __builtin_amdgcn_readfirstlane(tid / kWave), wave = role % 4;
+    const ScanItem item = scan_item(a, 16 * NC);
+    if (!item.in) return;
+    const int s = item.s, h = item.h, kh = h / a.group, col0 = 16 * NC * item.cb, col = col0 + NC * n;
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
     if (a.clear && (s == 0 || s == a.seqs - 1)) {
         const int head = min(max(a.starts[0], 0), a.tokens), tail = min(max(a.starts[a.seqs], 0), a.tokens);
-        uint16_t* row = a.out + h * a.out_head + 16 * NC * cb;
+        uint16_t* row = a.out + h * a.out_head + col0;
         if (s == 0)
-            for (int i = tid; i < head * 16 * NC; i += kThreads) row[i / (16 * NC) * a.out_token + i % (16 * NC)] = 0;
+            for (int i = tid; i < head * 16 * NC; i += kChainThreads)
+                row[i / (16 * NC) * a.out_token + i % (16 * NC)] = 0;
         if (s == a.seqs - 1)
-            for (int i = tid; i < (a.tokens - tail) * 16 * NC; i += kThreads)
+            for (int i = tid; i < (a.tokens - tail) * 16 * NC; i += kChainThreads)
                 row[(tail + i / (16 * NC)) * a.out_token + i % (16 * NC)] = 0;
     }
-    uint32_t* flag = w.flags + (static_cast<int64_t>(s) * a.heads + h) * (a.value_dim / 16) + NC * cb;
+    uint32_t* flag = w.flags + (static_cast<int64_t>(s) * a.heads + h) * (a.value_dim / 16) + NC * item.cb;
     const int into = scan_slot(a.into, s, a.pool);
     const bool fresh = a.initial == nullptr || (a.fresh != nullptr && a.fresh[s] != 0);
     const int from = fresh ? 0 : scan_slot(a.from, s, a.pool);
@@ -397,13 +405,103 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
         if (tid < NC) flag[tid] = 0;
         return;
     }
-    const int64_t size = static_cast<int64_t>(D) * a.value_dim;
-    f32x4 S[TPW][NC];
-    // Row i of the lane's of tile x.
-    auto row_of = [&](int x, int i) {
-        const int t = wave * TPW + x;
-        return 32 * (t / 2) + 8 * g + 4 * (t % 2) + i;
+    const int chunks = (seq.n + kChunk - 1) / kChunk;
+    const int64_t slot0 = scan_first_chunk(a.starts, s);
+    // Addresses are a scalar base per chunk and offsets of 32 bits; rows past the
+    // sequence repeat its last one (their factors are 0, and their u).
+    const int r0 = 16 * wave + 4 * g;
+    const uint32_t frag = lane * 16;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto load_rows = [&](uint4 (&to)[KS][PARTS], const uint16_t* rows, int64_t token, int64_t head, const uint8_t* frags,
+                         int ch) {
+        if constexpr (FP16) {
+            const uint8_t* at = frags + (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes;
+#pragma unroll
+            for (int i = 0; i < KS * PARTS; ++i) to[i / PARTS][i % PARTS] = frag16(at + i * kFragBytes, frag);
+        } else {
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(rows + (seq.a + ch * kChunk) * token + kh * head);
+            const uint32_t row = min(16 * wave + n, seq.n - 1 - ch * kChunk);
+            const uint32_t off = row * (2 * static_cast<uint32_t>(token)) + 16 * g;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) to[i][0] = frag16(at + 64 * i, off);
+        }
     };
+    auto load_blocks = [&](auto& to, const uint8_t* blocks, int ch) {
+        constexpr int P = sizeof(to) / sizeof(uint4) / 2;
+        const uint8_t* at = blocks + ((slot0 + ch) * a.heads + h) * kBlocks * P * kFragBytes;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            to[0][p] = frag16(at + (lower_block(0, wave) * P + p) * kFragBytes, frag);
+            to[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * P + p) * kFragBytes, frag);
+        }
+    };
+    auto factors = [&](int ch, int kind) {
+        return *reinterpret_cast<const f32x4*>(w.vec + ((slot0 + ch) * a.heads + h) * 256 + 64 * kind + r0);
+    };
+    if (role >= 4) {
+        uint4 q[KS][PARTS], p[2][2];
+        f32x4 fq;
+        if (chunks > 0) {
+            load_rows(q, a.q, a.q_token, a.q_head, w.qf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_blocks(p, w.p, 0);
+            fq = factors(0, 1);
+        }
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int next = min(ch + 1, chunks - 1);
+            __syncthreads();
+            f32x4 o[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] = zero;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const uint4 f = lds.s[b][i][c][lane];
+#pragma unroll
+                        for (int r = 0; r < PARTS && r + b < 2; ++r) o[c] = mfma16x16x32(q[i][r], f, o[c]);
+                    }
+            __builtin_amdgcn_sched_barrier(0);
+            load_rows(q, a.q, a.q_token, a.q_head, w.qf, next);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] *= fq;
+            __syncthreads();
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (2 * k > wave) continue;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const uint4 f = lds.u[b][k][c][lane];
+#pragma unroll
+                        for (int r = 0; r + b < 2; ++r) o[c] = mfma16x16x32(p[k][r], f, o[c]);
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_blocks(p, w.p, next);
+            fq = factors(next, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const int left = seq.n - ch * kChunk;
+            uint16_t* to = a.out + static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.out_token + h * a.out_head + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + i < left) store_cols<NC, FP16>(to + i * a.out_token, o, i);
+        }
+        __syncthreads_or(0);
+        return;
+    }
+    const int64_t size = static_cast<int64_t>(D) * a.value_dim;
+    // The first of the lane's four rows of tile x.
+    auto row_of = [&](int x) {
+        const int t = wave * TPW + x;
+        return 32 * (t / 2) + 8 * g + 4 * (t % 2);
+    };
+    f32x4 S[TPW][NC];
 #pragma unroll
     for (int x = 0; x < TPW; ++x)
 #pragma unroll
@@ -412,84 +510,38 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
             for (int c = 0; c < NC; ++c)
                 S[x][c][i] = fresh ? 0.0f
                                    : a.initial[(static_cast<int64_t>(from) * a.heads + h) * size +
-                                               static_cast<int64_t>(row_of(x, i)) * a.value_dim + col + c];
-    const int chunks = (seq.n + kChunk - 1) / kChunk;
-    const int64_t slot0 = scan_first_chunk(a.starts, s);
-    uint16_t* tape_s = reinterpret_cast<uint16_t*>(a.tape);
-    uint16_t* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
-    ScanLoads<D, NC, FP16> x;
-    // Addresses are a scalar base per chunk and offsets of 32 bits; rows past the
-    // sequence repeat its last one (their factors are 0, and their u).
-    const int r0 = 16 * wave + 4 * g;
-    const uint32_t frag = lane * 16;
-    auto load_rows = [&](int ch) {
-        if constexpr (FP16) {
-            const int64_t at = (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes;
-#pragma unroll
-            for (int i = 0; i < KS * PARTS; ++i) {
-                x.k[i / PARTS][i % PARTS] = frag16(w.kf + at + i * kFragBytes, frag);
-                x.q[i / PARTS][i % PARTS] = frag16(w.qf + at + i * kFragBytes, frag);
-            }
-        } else {
-            const int64_t t = seq.a + ch * kChunk;
-            const uint8_t* k = reinterpret_cast<const uint8_t*>(a.k + t * a.k_token + kh * a.k_head);
-            const uint8_t* q = reinterpret_cast<const uint8_t*>(a.q + t * a.q_token + kh * a.q_head);
-            const uint32_t row = min(16 * wave + n, seq.n - 1 - ch * kChunk);
-            const uint32_t k_at = row * (2 * static_cast<uint32_t>(a.k_token)) + 16 * g;
-            const uint32_t q_at = row * (2 * static_cast<uint32_t>(a.q_token)) + 16 * g;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                x.k[i][0] = frag16(k + 64 * i, k_at);
-                x.q[i][0] = frag16(q + 64 * i, q_at);
-            }
-        }
-    };
+                                               static_cast<int64_t>(row_of(x) + i) * a.value_dim + col + c];
+    float* tape_s = reinterpret_cast<float*>(a.tape);
+    float* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
+    uint4 k[KS][PARTS], t[2][3], kt[TPW][2][PARTS];
+    uint32_t v[4];
+    f32x4 fk, fu;
+    float decay = 0.0f;
     auto load_values = [&](int ch) {
-        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
-        x.fk = *reinterpret_cast<const f32x4*>(vec + r0);
-        const uint8_t* v = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
-                                                            h * a.v_head + 16 * NC * cb);
+        fk = factors(ch, 0);
+        const uint8_t* at = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
+                                                             h * a.v_head + col0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t row = min(r0 + i, seq.n - 1 - ch * kChunk);
-            load_cols<NC>(x.v[i], v, row * (2 * static_cast<uint32_t>(a.v_token)) + 2 * NC * n);
+            v[i] = load_cols<NC>(at, row * (2 * static_cast<uint32_t>(a.v_token)) + 2 * NC * n);
         }
-    };
-    auto load_t = [&](int ch) {
-        const uint8_t* t = w.t + ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            x.t[0][p] = frag16(t + (lower_block(0, wave) * 3 + p) * kFragBytes, frag);
-            x.t[1][p] = frag16(t + (lower_block(1, max(wave, 2)) * 3 + p) * kFragBytes, frag);
-        }
-    };
-    auto load_factors = [&](int ch) {
-        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
-        x.fq = *reinterpret_cast<const f32x4*>(vec + 64 + r0);
-        x.fu = *reinterpret_cast<const f32x4*>(vec + 128 + r0);
-        x.decay = vec[192];
     };
     auto load_rest = [&](int ch) {
-        const int64_t by_head = (slot0 + ch) * a.heads + h, by_key = (slot0 + ch) * a.key_heads + kh;
-        const uint8_t* at = w.p + by_head * kBlocks * 2 * kFragBytes;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            x.p[0][p] = frag16(at + (lower_block(0, wave) * 2 + p) * kFragBytes, frag);
-            x.p[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * 2 + p) * kFragBytes, frag);
-        }
-        const uint8_t* kt = w.kt + ((by_key * (D / 16) + wave * TPW) * 2 * PARTS) * kFragBytes;
+        fu = factors(ch, 2);
+        decay = w.vec[((slot0 + ch) * a.heads + h) * 256 + 192];
+        const uint8_t* at = w.kt + (((slot0 + ch) * a.key_heads + kh) * (D / 16) + wave * TPW) * 2 * PARTS * kFragBytes;
 #pragma unroll
         for (int i = 0; i < TPW * 2 * PARTS; ++i)
-            x.kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(kt + i * kFragBytes, frag);
+            kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
     };
     if (chunks > 0) {
         // (In the loop's order, so that its waits count the same loads.)
-        load_rows(0);
+        load_rows(k, a.k, a.k_token, a.k_head, w.kf, 0);
         __builtin_amdgcn_sched_barrier(0);
         load_values(0);
         __builtin_amdgcn_sched_barrier(0);
-        load_t(0);
-        load_factors(0);
+        load_blocks(t, w.t, 0);
         __builtin_amdgcn_sched_barrier(0);
         load_rest(0);
         __builtin_amdgcn_sched_barrier(0);
@@ -502,16 +554,10 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 put_parts<3>(lds.s, (wave * TPW + i) / 2, (wave * TPW + i) % 2, c, lane, S[i][c]);
-        const int64_t taped = (slot0 + ch) * a.heads + h;
-        if constexpr (TAPE) {
-#pragma unroll
-            for (int i = 0; i < TPW; ++i)
-                put_rows<NC>(tape_s + taped * 2 * size, size, a.value_dim, row_of(i, 0), col, S[i]);
-        }
         __syncthreads();
-        f32x4 ks[NC], qs[NC];
+        f32x4 r[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) ks[c] = qs[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NC; ++c) r[c] = zero;
 #pragma unroll
         for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -520,100 +566,73 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
                 for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.s[p][i][c][lane];
 #pragma unroll
-                    for (int r = 0; r < PARTS; ++r) {
-                        if (r + p < 3) ks[c] = mfma16x16x32(x.k[i][r], b, ks[c]);
-                        if (r + p < 2) qs[c] = mfma16x16x32(x.q[i][r], b, qs[c]);
-                    }
+                    for (int x = 0; x < PARTS && x + p < 3; ++x) r[c] = mfma16x16x32(k[i][x], b, r[c]);
                 }
         __builtin_amdgcn_sched_barrier(0);
-        load_rows(next);
+        load_rows(k, a.k, a.k_token, a.k_head, w.kf, next);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            f32x4 r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = col_value<NC, FP16>(x.v[i], c) - x.fk[i] * ks[c][i];
-            put_parts<3>(lds.r, wave / 2, wave % 2, c, lane, r);
+            for (int i = 0; i < 4; ++i) r[c][i] = col_value<FP16>(v[i], c) - fk[i] * r[c][i];
+            put_parts<3>(lds.r, wave / 2, wave % 2, c, lane, r[c]);
         }
         __builtin_amdgcn_sched_barrier(0);
         load_values(next);
+        if constexpr (TAPE) {
+            // (Behind the step's loads, whose waits would count the stores.)
+            float* to = tape_s + ((slot0 + ch) * a.heads + h) * size + col;
+#pragma unroll
+            for (int i = 0; i < TPW; ++i) put_rows<NC>(to + row_of(i) * a.value_dim, a.value_dim, S[i]);
+        }
         __syncthreads();
         f32x4 u[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            u[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NC; ++c) u[c] = zero;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (2 * k > wave) continue;
+        for (int i = 0; i < 2; ++i) {
+            if (2 * i > wave) continue;
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    const uint4 b = lds.r[p][k][c][lane];
+            for (int p = 0; p < 3; ++p)
 #pragma unroll
-                    for (int r = 0; r + p < 3; ++r) u[c] = mfma16x16x32(x.t[k][r], b, u[c]);
+                for (int c = 0; c < NC; ++c) {
+                    const uint4 b = lds.r[p][i][c][lane];
+#pragma unroll
+                    for (int x = 0; x + p < 3; ++x) u[c] = mfma16x16x32(t[i][x], b, u[c]);
                 }
-            }
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_t(next);
+        load_blocks(t, w.t, next);
         __builtin_amdgcn_sched_barrier(0);
-        const f32x4 fq = x.fq;
-        const float decay = x.decay;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+            put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
+            put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * fu);
 #pragma unroll
             for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[c][i]) & 0x7f800000u) == 0x7f800000u;
-            put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
-            put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * x.fu);
         }
-        load_factors(next);
         if constexpr (TAPE)
-            put_rows<NC>(tape_u + taped * 2 * kChunk * a.value_dim, kChunk * a.value_dim, a.value_dim, 16 * wave + 4 * g,
-                         col, u);
+            put_rows<NC>(tape_u + (((slot0 + ch) * a.heads + h) * kChunk + r0) * a.value_dim + col, a.value_dim, u);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                S[i][c] *= decay;
+            for (int c = 0; c < NC; ++c) S[i][c] *= decay;
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        const uint4 b = lds.uk[p][k][c][lane];
+            for (int p = 0; p < 3; ++p)
 #pragma unroll
-                        for (int r = 0; r < PARTS; ++r)
-                            if (r + p < 3) S[i][c] = mfma16x16x32(x.kt[i][k][r], b, S[i][c]);
-                    }
-            }
-        f32x4 o[NC];
+                for (int c = 0; c < NC; ++c) {
+                    const uint4 b = lds.uk[p][j][c][lane];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            o[c] = qs[c] * fq;
+                    for (int i = 0; i < TPW; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (2 * k > wave) continue;
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint4 b = lds.u[p][k][c][lane];
-#pragma unroll
-                    for (int r = 0; r + p < 2; ++r) o[c] = mfma16x16x32(x.p[k][r], b, o[c]);
+                        for (int x = 0; x < PARTS && x + p < 3; ++x) S[i][c] = mfma16x16x32(kt[i][j][x], b, S[i][c]);
                 }
-            }
-        }
         __builtin_amdgcn_sched_barrier(0);
         load_rest(next);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = ch * kChunk + 16 * wave + 4 * g + i;
-            if (t >= seq.n) continue;
-            uint16_t* to = a.out + static_cast<int64_t>(seq.a + t) * a.out_token + h * a.out_head + col;
-            if constexpr (NC == 1) {
-                *to = static_cast<uint16_t>(pack16_2<FP16>(o[0][i], 0.0f));
-            } else {
-                *reinterpret_cast<uint32_t*>(to) = pack16_2<FP16>(o[0][i], o[1][i]);
-            }
-        }
     }
     // Where a value was not finite, a product's zero weights have let it through
     // to earlier tokens: the next launch goes through these columns again.
@@ -623,13 +642,10 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
     }
     if (tid < NC) flag[tid] = 0;
 #pragma unroll
-    for (int x1 = 0; x1 < TPW; ++x1)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-                a.final[(static_cast<int64_t>(into) * a.heads + h) * size +
-                        static_cast<int64_t>(row_of(x1, i)) * a.value_dim + col + c] = S[x1][c][i];
+    for (int x = 0; x < TPW; ++x)
+        put_rows<NC>(a.final + (static_cast<int64_t>(into) * a.heads + h) * size +
+                         static_cast<int64_t>(row_of(x)) * a.value_dim + col,
+                     a.value_dim, S[x]);
 }
 
 // ---- the gradient: chunk after chunk, backwards -----------------------------------
@@ -637,44 +653,46 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks(ScanArgs a, ScanChunk
 // With dS the gradient of the state after a chunk and do that of its outputs,
 //     X_j = sum_i P_ij do_i + e^(G_63 - G_j) dS^T k_j,     dR = (beta (I + L beta)^-1)^T X = dv,
 //     dS <- e^(G_63) dS + sum_i scale e^(G_i) q_i do_i^T - sum_i e^(G_i) k_i dR_i^T:
-// the forward launch with the matrices transposed, for the same columns.
+// the forward launch with the matrices transposed, for the same columns. Waves 0
+// to 3 have the chain; waves 4 to 7 compute the two sums over do, which need no
+// dS, a chunk ahead.
 template <int D, int NC, int PARTS>
 struct ScanGradLds {
     uint4 s[3][D / 32][NC][kWave];
-    uint4 o[PARTS][2][NC][kWave];   // do
     uint4 x[3][2][NC][kWave];
-    uint4 oq[3][2][NC][kWave];      // do times the factors of q
-    uint4 rk[3][2][NC][kWave];      // - dR times the factors of k
+    uint4 rk[3][2][NC][kWave];           // - dR times the factors of k
+    uint4 o[PARTS][2][NC][kWave];        // do
+    uint4 oq[3][2][NC][kWave];           // do times the factors of q
+    f32x4 y[4][NC][kWave];               // sum P do, as the chain's accumulators
+    f32x4 z[2][D / 16][NC][kWave];       // sum q do, of two chunks
 };
 
 template <int D, bool FP16>
-__global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
+__global__ __launch_bounds__(kChainThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32, NC = 2;
     __shared__ ScanGradLds<D, NC, PARTS> lds;
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int blocks = a.value_dim / (16 * NC), per = (gridDim.x + 7) / 8;
-    const int item = blockIdx.x % 8 * per + blockIdx.x / 8;
-    if (item >= a.seqs * a.heads * blocks) return;
-    const int cb = item % blocks, h = item / blocks % a.heads, s = item / blocks / a.heads, kh = h / a.group;
-    const int col = 16 * NC * cb + NC * n;
+    const int role = __builtin_amdgcn_readfirstlane(tid / kWave), wave = role % 4;
+    const ScanItem item = scan_item(a, 16 * NC);
+    if (!item.in) return;
+    const int s = item.s, h = item.h, kh = h / a.group, col0 = 16 * NC * item.cb, col = col0 + NC * n;
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
     if (s == 0 || s == a.seqs - 1) {
         // Rows of no sequence have no gradient.
         const int head = min(max(a.starts[0], 0), a.tokens), tail = min(max(a.starts[a.seqs], 0), a.tokens);
         auto clear = [&](int from, int to) {
             const int rows = to - from;
-            for (int i = tid; i < rows * 32; i += kThreads)
-                d.dv[(static_cast<int64_t>(from + i / 32) * a.heads + h) * a.value_dim + 32 * cb + i % 32] = 0;
-            if (cb != 0) return;
-            for (int i = tid; i < rows; i += kThreads) {
+            for (int i = tid; i < rows * 32; i += kChainThreads)
+                d.dv[(static_cast<int64_t>(from + i / 32) * a.heads + h) * a.value_dim + col0 + i % 32] = 0;
+            if (item.cb != 0) return;
+            for (int i = tid; i < rows; i += kChainThreads) {
                 const int64_t at = static_cast<int64_t>(from + i) * a.heads + h;
                 d.dg[at] = 0.0f;
                 if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = 0.0f;
                 else static_cast<uint16_t*>(d.dbeta)[at] = 0;
             }
             if (h % a.group != 0) return;
-            for (int i = tid; i < rows * D; i += kThreads) {
+            for (int i = tid; i < rows * D; i += kChainThreads) {
                 const int64_t at = (static_cast<int64_t>(from + i / D) * a.key_heads + kh) * D + i % D;
                 d.dq[at] = 0;
                 d.dk[at] = 0;
@@ -683,184 +701,258 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, Scan
         if (s == 0) clear(0, head);
         if (s == a.seqs - 1) clear(tail, a.tokens);
     }
+    const int chunks = (seq.n + kChunk - 1) / kChunk;
+    const int64_t slot0 = scan_first_chunk(a.starts, s);
+    const int r0 = 16 * wave + 4 * g;
+    const uint32_t frag = lane * 16;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto load_blocks = [&](uint4 (&to)[2][3], const uint8_t* blocks, int ch) {
+        const uint8_t* at = blocks + ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            to[0][p] = frag16(at + (upper_block(0, min(wave, 1)) * 3 + p) * kFragBytes, frag);
+            to[1][p] = frag16(at + (upper_block(1, wave) * 3 + p) * kFragBytes, frag);
+        }
+    };
+    auto load_transposed = [&](uint4 (&to)[TPW][2][PARTS], const uint8_t* frags, int ch) {
+        const uint8_t* at = frags + (((slot0 + ch) * a.key_heads + kh) * (D / 16) + wave * TPW) * 2 * PARTS * kFragBytes;
+#pragma unroll
+        for (int i = 0; i < TPW * 2 * PARTS; ++i)
+            to[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
+    };
+    auto factors = [&](int ch, int kind) {
+        return *reinterpret_cast<const f32x4*>(w.vec + ((slot0 + ch) * a.heads + h) * 256 + 64 * kind + r0);
+    };
+    if (role >= 4) {
+        if (chunks == 0) return;
+        uint32_t o[4];
+        uint4 pt[2][3], qt[TPW][2][PARTS];
+        f32x4 fq;
+        auto load_out = [&](int ch) {
+            fq = factors(ch, 1);
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(
+                d.d_out + static_cast<int64_t>(seq.a + ch * kChunk) * d.d_out_token + h * d.d_out_head + col0);
+            const int left = seq.n - ch * kChunk;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t row = min(r0 + i, left - 1);
+                o[i] = load_cols<NC>(at, row * (2 * static_cast<uint32_t>(d.d_out_token)) + 2 * NC * n);
+            }
+        };
+        auto put_out = [&](int ch) {
+            const int left = seq.n - ch * kChunk;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                f32x4 x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = r0 + i < left ? col_value<FP16>(o[i], c) : 0.0f;
+                put_parts<PARTS>(lds.o, wave / 2, wave % 2, c, lane, x);
+                put_parts<3>(lds.oq, wave / 2, wave % 2, c, lane, x * fq);
+            }
+        };
+        f32x4 y[NC], z[TPW][NC];
+        auto products = [&] {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                y[c] = zero;
+#pragma unroll
+                for (int i = 0; i < TPW; ++i) z[i][c] = zero;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const uint4 b = lds.o[p][j][c][lane];
+                        if (2 * j + 1 < wave) continue;
+#pragma unroll
+                        for (int x = 0; x + p < 3; ++x) y[c] = mfma16x16x32(pt[j][x], b, y[c]);
+                    }
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        const uint4 b = lds.oq[p][j][c][lane];
+#pragma unroll
+                        for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                            for (int x = 0; x < PARTS && x + p < 3; ++x) z[i][c] = mfma16x16x32(qt[i][j][x], b, z[i][c]);
+                    }
+                }
+        };
+        auto hand_on = [&](int half) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                lds.y[wave][c][lane] = y[c];
+#pragma unroll
+                for (int i = 0; i < TPW; ++i) lds.z[half][wave * TPW + i][c][lane] = z[i][c];
+            }
+        };
+        load_out(chunks - 1);
+        load_blocks(pt, w.p, chunks - 1);
+        load_transposed(qt, w.qt, chunks - 1);
+        put_out(chunks - 1);
+        __syncthreads();
+        products();
+        hand_on((chunks - 1) % 2);
+        load_out(max(chunks - 2, 0));
+        __builtin_amdgcn_sched_barrier(0);
+        load_blocks(pt, w.p, max(chunks - 2, 0));
+        load_transposed(qt, w.qt, max(chunks - 2, 0));
+        __builtin_amdgcn_sched_barrier(0);
+        for (int ch = chunks - 1; ch >= 0; --ch) {
+            const int next = max(ch - 1, 0), after = max(ch - 2, 0);
+            __syncthreads();
+            put_out(next);
+            __builtin_amdgcn_sched_barrier(0);
+            load_out(after);
+            __syncthreads();
+            products();
+            __builtin_amdgcn_sched_barrier(0);
+            load_blocks(pt, w.p, after);
+            load_transposed(qt, w.qt, after);
+            __syncthreads();
+            hand_on((ch + 1) % 2);
+        }
+        return;
+    }
     const int64_t size = static_cast<int64_t>(D) * a.value_dim;
-    f32x4 S[TPW][NC];
-    auto row_of = [&](int x, int i) {
+    auto row_of = [&](int x) {
         const int t = wave * TPW + x;
-        return 32 * (t / 2) + 8 * g + 4 * (t % 2) + i;
+        return 32 * (t / 2) + 8 * g + 4 * (t % 2);
     };
-    auto state_at = [&](int x, int i) {
-        return (static_cast<int64_t>(s) * a.heads + h) * size + static_cast<int64_t>(row_of(x, i)) * a.value_dim + col;
+    auto state_at = [&](int x) {
+        return (static_cast<int64_t>(s) * a.heads + h) * size + static_cast<int64_t>(row_of(x)) * a.value_dim + col;
     };
+    f32x4 S[TPW][NC];
 #pragma unroll
     for (int x = 0; x < TPW; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) S[x][c][i] = d.d_final != nullptr ? d.d_final[state_at(x, i) + c] : 0.0f;
-    const int chunks = (seq.n + kChunk - 1) / kChunk;
-    const int64_t slot0 = scan_first_chunk(a.starts, s);
-    uint4 k[KS][PARTS], tt[2][3], pt[2][3], kt[TPW][2][PARTS], qt[TPW][2][PARTS];
-    uint32_t o[4][1];
-    f32x4 fk, fq, fu;
+            for (int c = 0; c < NC; ++c)
+                S[x][c][i] = d.d_final != nullptr ? d.d_final[state_at(x) + i * a.value_dim + c] : 0.0f;
+    uint4 k[KS][PARTS], tt[2][3], kt[TPW][2][PARTS];
+    f32x4 fk, fu;
     float decay = 0.0f;
-    const int r0 = 16 * wave + 4 * g;
     auto load_k = [&](int ch) {
+        fu = factors(ch, 2);
         if constexpr (FP16) {
-            const int64_t at = (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes + lane * 16;
+            const uint8_t* at = w.kf + (((slot0 + ch) * a.key_heads + kh) * 4 + wave) * KS * PARTS * kFragBytes;
 #pragma unroll
-            for (int i = 0; i < KS * PARTS; ++i) k[i / PARTS][i % PARTS] = ldg16(w.kf + at + i * kFragBytes);
+            for (int i = 0; i < KS * PARTS; ++i) k[i / PARTS][i % PARTS] = frag16(at + i * kFragBytes, frag);
         } else {
-            const int t = ch * kChunk + 16 * wave + n;
-            const bool in = t < seq.n;
-            const int64_t row = seq.a + (in ? t : 0);
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(a.k + (seq.a + ch * kChunk) * a.k_token + kh * a.k_head);
+            const uint32_t row = min(16 * wave + n, seq.n - 1 - ch * kChunk);
+            const uint32_t off = row * (2 * static_cast<uint32_t>(a.k_token)) + 16 * g;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                k[i][0] = make_uint4(0u, 0u, 0u, 0u);
-                if (in) k[i][0] = ldg16(a.k + row * a.k_token + kh * a.k_head + 32 * i + 8 * g);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = ch * kChunk + r0 + i;
-            o[i][0] = 0u;
-            if (t < seq.n)
-                load_cols<NC>(o[i], reinterpret_cast<const uint8_t*>(d.d_out + static_cast<int64_t>(seq.a + t) * d.d_out_token + h * d.d_out_head + col), 0);
-        }
-        const float* vec = w.vec + ((slot0 + ch) * a.heads + h) * 256;
-        fk = *reinterpret_cast<const f32x4*>(vec + r0);
-        fq = *reinterpret_cast<const f32x4*>(vec + 64 + r0);
-        fu = *reinterpret_cast<const f32x4*>(vec + 128 + r0);
-        decay = vec[192];
-    };
-    auto load_matrices = [&](int ch) {
-        const int64_t at = ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes + lane * 16;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            if (wave < 2) {
-                tt[0][p] = ldg16(w.t + at + (upper_block(0, wave) * 3 + p) * kFragBytes);
-                pt[0][p] = ldg16(w.p + at + (upper_block(0, wave) * 3 + p) * kFragBytes);
-            }
-            tt[1][p] = ldg16(w.t + at + (upper_block(1, wave) * 3 + p) * kFragBytes);
-            pt[1][p] = ldg16(w.p + at + (upper_block(1, wave) * 3 + p) * kFragBytes);
+            for (int i = 0; i < KS; ++i) k[i][0] = frag16(at + 64 * i, off);
         }
     };
-    auto load_transposed = [&](int ch) {
-        const int64_t by_key = (slot0 + ch) * a.key_heads + kh;
-#pragma unroll
-        for (int i = 0; i < TPW * 2 * PARTS; ++i) {
-            const int64_t at = ((by_key * (D / 16) + wave * TPW) * 2 * PARTS + i) * kFragBytes + lane * 16;
-            kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = ldg16(w.kt + at);
-            qt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = ldg16(w.qt + at);
-        }
+    auto load_t = [&](int ch) {
+        fk = factors(ch, 0);
+        load_blocks(tt, w.t, ch);
+    };
+    auto load_rest = [&](int ch) {
+        decay = w.vec[((slot0 + ch) * a.heads + h) * 256 + 192];
+        load_transposed(kt, w.kt, ch);
     };
     if (chunks > 0) {
         load_k(chunks - 1);
-        load_matrices(chunks - 1);
-        load_transposed(chunks - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(chunks - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rest(chunks - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
     }
     for (int ch = chunks - 1; ch >= 0; --ch) {
         const int next = max(ch - 1, 0);
         const int64_t by_head = (slot0 + ch) * a.heads + h;
-        f32x4 od[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) od[c][i] = col_value<NC, FP16>(o[i], c);
-            put_parts<PARTS>(lds.o, wave / 2, wave % 2, c, lane, od[c]);
-        }
-#pragma unroll
-        for (int i = 0; i < TPW; ++i) {
+        for (int i = 0; i < TPW; ++i)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 put_parts<3>(lds.s, (wave * TPW + i) / 2, (wave * TPW + i) % 2, c, lane, S[i][c]);
-            put_rows<NC>(w.ds + by_head * 2 * size, size, a.value_dim, row_of(i, 0), col, S[i]);
-        }
         __syncthreads();
         f32x4 x[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            x[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NC; ++c) x[c] = zero;
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.s[p][i][c][lane];
 #pragma unroll
-                    for (int r = 0; r < PARTS; ++r)
-                        if (r + p < 3) x[c] = mfma16x16x32(k[i][r], b, x[c]);
+                    for (int r = 0; r < PARTS && r + p < 3; ++r) x[c] = mfma16x16x32(k[i][r], b, x[c]);
                 }
-            x[c] *= fu;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (2 * i + 1 < wave) continue;
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    const uint4 b = lds.o[p][i][c][lane];
-#pragma unroll
-                    for (int r = 0; r + p < 3; ++r) x[c] = mfma16x16x32(pt[i][r], b, x[c]);
-                }
-            }
+        for (int c = 0; c < NC; ++c) {
+            x[c] = x[c] * fu + lds.y[wave][c][lane];
             put_parts<3>(lds.x, wave / 2, wave % 2, c, lane, x[c]);
         }
-        const f32x4 factor_k = fk, factor_q = fq;
-        const float fade = decay;
+        __builtin_amdgcn_sched_barrier(0);
         load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            float* to = w.ds + by_head * size + col;
+#pragma unroll
+            for (int i = 0; i < TPW; ++i) put_rows<NC>(to + row_of(i) * a.value_dim, a.value_dim, S[i]);
+        }
         __syncthreads();
         f32x4 dr[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            dr[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NC; ++c) dr[c] = zero;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (2 * i + 1 < wave) continue;
+        for (int i = 0; i < 2; ++i) {
+            if (2 * i + 1 < wave) continue;
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.x[p][i][c][lane];
 #pragma unroll
                     for (int r = 0; r + p < 3; ++r) dr[c] = mfma16x16x32(tt[i][r], b, dr[c]);
                 }
-            }
-            put_parts<3>(lds.rk, wave / 2, wave % 2, c, lane, -(dr[c] * factor_k));
-            put_parts<3>(lds.oq, wave / 2, wave % 2, c, lane, od[c] * factor_q);
         }
-        load_matrices(next);
-        put_rows<NC>(w.dr + by_head * 2 * kChunk * a.value_dim, kChunk * a.value_dim, a.value_dim, r0, col, dr);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = ch * kChunk + r0 + i;
-            if (t < seq.n)
-                *reinterpret_cast<uint32_t*>(d.dv + (static_cast<int64_t>(seq.a + t) * a.heads + h) * a.value_dim + col) =
-                    pack16_2<FP16>(dr[0][i], dr[1][i]);
+        for (int c = 0; c < NC; ++c) put_parts<3>(lds.rk, wave / 2, wave % 2, c, lane, -(dr[c] * fk));
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(next);
+        __builtin_amdgcn_sched_barrier(0);
+        put_rows<NC>(w.dr + (by_head * kChunk + r0) * a.value_dim + col, a.value_dim, dr);
+        {
+            const int left = seq.n - ch * kChunk;
+            uint16_t* to = d.dv + (static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.heads + h) * a.value_dim + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + i < left) store_cols<NC, FP16>(to + static_cast<int64_t>(i) * a.heads * a.value_dim, dr, i);
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                S[i][c] *= fade;
+            for (int c = 0; c < NC; ++c) S[i][c] = S[i][c] * decay + lds.z[ch % 2][wave * TPW + i][c][lane];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        const uint4 bq = lds.oq[p][j][c][lane], bk = lds.rk[p][j][c][lane];
+            for (int p = 0; p < 3; ++p)
 #pragma unroll
-                        for (int r = 0; r < PARTS; ++r)
-                            if (r + p < 3) {
-                                S[i][c] = mfma16x16x32(qt[i][j][r], bq, S[i][c]);
-                                S[i][c] = mfma16x16x32(kt[i][j][r], bk, S[i][c]);
-                            }
-                    }
-            }
-        load_transposed(next);
+                for (int c = 0; c < NC; ++c) {
+                    const uint4 b = lds.rk[p][j][c][lane];
+#pragma unroll
+                    for (int i = 0; i < TPW; ++i)
+#pragma unroll
+                        for (int r = 0; r < PARTS && r + p < 3; ++r) S[i][c] = mfma16x16x32(kt[i][j][r], b, S[i][c]);
+                }
+        __builtin_amdgcn_sched_barrier(0);
+        load_rest(next);
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (d.d_initial != nullptr) {
 #pragma unroll
-        for (int x = 0; x < TPW; ++x)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) d.d_initial[state_at(x, i) + c] = S[x][c][i];
+        for (int x = 0; x < TPW; ++x) put_rows<NC>(d.d_initial + state_at(x), a.value_dim, S[x]);
     }
 }
 
@@ -871,19 +963,36 @@ __global__ __launch_bounds__(kThreads, 2) void scan_chunks_grad(ScanArgs a, Scan
 // (j < i), for the normalized q and k:
 //     dq_i = scale (e^(G_i) S do_i + sum_j B1_ij k_j),
 //     dk_i = -(e^(G_i) S dR_i + sum_j B2_ij k_j) + e^(G_63 - G_i) dS u_i
-//            + sum_j (B1_ji scale q_j - B2_ji k_j),
-// the first bracket by k_i's own row, the rest by its column.  The running sum
-// G_i has the gradient q_i . dq_i + k_i . (dk_i by its row) - k_i . (dk_i by its
-// column), the last one <state after, dS> as well, and g_t the sum of those from
-// t on.  dbeta_i = w_i . du_i = u_i . dR_i / beta_i^2.
+//            + sum_j (B1_ji scale q_j - B2_ji k_j).
+// dbeta_i = w_i . du_i = u_i . dR_i / beta_i^2.  A decay g_t acts on what passes
+// from before t to t or later: its gradient is, with M_ij = scale B1_ij q_i . k_j
+// - B2_ij k_i . k_j,
+//     sum_(i >= t) e^(G_i) (scale q_i . S do_i - k_i . S dR_i) + sum_(j < t) e^(G_63 - G_j) k_j . dS u_j
+//     + e^(G_63) <S, dS> + sum_(i >= t > j) M_ij,
+// as a running sum of rows less columns, with the same numbers on both sides, so
+// that what lies within either side cancels to fp32's last bits.
 //
-// A workgroup has a chunk and a key head and goes through its value heads; wave
-// w has the token rows of tile w, in the accumulators' layout with the columns
-// of the K^T fragments' rows.
+// A workgroup has a chunk and a key head and goes through its value heads.  Its
+// eight waves have two row tiles (of 16 tokens) and a quarter of the columns of
+// dq and dk each. What is fp32 (S, dS, u, dR) is read once by the workgroup, 32
+// columns at a time, split into three bf16 numbers and shared through LDS: the
+// decays' gradient is fp32 and as exact as that. The second products, over
+// tokens, only reach dq and dk, which are rounded to 16 bits: two parts.
+constexpr int kGradThreads = 512;
+template <int D>
 struct ScanInputsLds {
-    float b1[kChunk * kPitch], b2[kChunk * kPitch];   // then dq and dk, 16 bit
+    union {
+        struct {
+            uint4 s[D / 16][3][kWave], ds[D / 16][3][kWave], u[4][3][kWave], r[4][3][kWave];
+        } stage;
+        struct {
+            float b1[kChunk * kPitch], b2[kChunk * kPitch];   // then dq and dk
+            uint4 frag[4][kBlocks][2][kWave];   // B1 and B2 by rows (lower blocks), by columns (upper ones)
+        } m;
+    };
     double sum[kChunk];
-    float rk[kChunk], rq[kChunk], row[kChunk], state[4];
+    float rk[kChunk], rq[kChunk], decay[kChunk], rest[kChunk];
+    float dot[4][kChunk], row[4][kChunk], col[4][kChunk], state[8], moved[8];
 };
 
 __device__ __forceinline__ float sum_over_16(float v) {
@@ -893,12 +1002,21 @@ __device__ __forceinline__ float sum_over_16(float v) {
     return butterfly_step8(v);
 }
 
+// Eight floats as a fragment of two parts.
+__device__ __forceinline__ void two_parts(uint4 (&to)[2], const float (&f)[8]) {
+    Split2 p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) to[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
+}
+
 template <int D, bool FP16>
-__global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
-    constexpr int PARTS = FP16 ? 2 : 1, TILES = D / 16, RAW = D + 8;
-    __shared__ ScanInputsLds lds;
+__global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
+    constexpr int PARTS = FP16 ? 2 : 1, TILES = D / 16, TPQ = D / 64, RAW = D + 8;
+    __shared__ ScanInputsLds<D> lds;
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), pair = wave % 2, quarter = wave / 2;
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
     const int s = find_sequence(a.starts, a.seqs, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
@@ -906,100 +1024,185 @@ __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, Scan
     if (first < 0 || first >= seq.n) return;
     const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
     const int64_t by_key = static_cast<int64_t>(slot) * a.key_heads + kh;
-    const int E = a.value_dim, r0 = 16 * wave + 4 * g;
+    const int E = a.value_dim;
     if (tid < kChunk) {
         lds.rk[tid] = w.norms[by_key * 2 * kChunk + tid];
         lds.rq[tid] = w.norms[by_key * 2 * kChunk + kChunk + tid];
     }
-    // Element of column n of tile t (as the fragments' rows), and the raw q and k there.
-    auto element = [&](int t) { return 32 * (t / 2) + 8 * (n / 4) + 4 * (t % 2) + n % 4; };
-    uint16_t q[TILES][4], k[TILES][4];
+    // Row i of the lane's of the wave's row tile x, and element of its column in
+    // the wave's column tile t.
+    auto row_of = [&](int x, int i) { return 32 * pair + 16 * x + 4 * g + i; };
+    auto element_of = [&](int tile) { return 32 * (tile / 2) + 8 * (n / 4) + 4 * (tile % 2) + n % 4; };
+    auto element = [&](int t) { return element_of(quarter * TPQ + t); };
+    uint32_t q[2][TPQ][2], k[2][TPQ][2];   // raw, rows in pairs
 #pragma unroll
-    for (int t = 0; t < TILES; ++t)
+    for (int t = 0; t < TPQ; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q[t][i] = k[t][i] = 0;
-            if (r0 + i < count) {
-                q[t][i] = a.q[static_cast<int64_t>(t0 + r0 + i) * a.q_token + kh * a.q_head + element(t)];
-                k[t][i] = a.k[static_cast<int64_t>(t0 + r0 + i) * a.k_token + kh * a.k_head + element(t)];
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                q[x][t][i] = k[x][t][i] = 0;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = row_of(x, 2 * i + j);
+                    if (row >= count) continue;
+                    const int64_t at = t0 + row;
+                    q[x][t][i] |= static_cast<uint32_t>(a.q[at * a.q_token + kh * a.q_head + element(t)]) << (16 * j);
+                    k[x][t][i] |= static_cast<uint32_t>(a.k[at * a.k_token + kh * a.k_head + element(t)]) << (16 * j);
+                }
             }
-        }
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    f32x4 dq[TILES], dk[TILES];
+    }
+    // q_i . k_j, or for the second two quarters k_i . k_j, of the tiles that the
+    // wave has of B1 or B2.
+    const int odd = quarter % 2;
+    f32x4 pairs[2][2];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) dq[t] = dk[t] = zero;
-    const int64_t states = tape_states(w.slots, a.heads, D, E);
+    for (int x = 0; x < 2; ++x) pairs[x][0] = pairs[x][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    {
+        const uint16_t* side = quarter < 2 ? a.q : a.k;
+        const int64_t token = quarter < 2 ? a.q_token : a.k_token, head = quarter < 2 ? a.q_head : a.k_head;
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+            const int e = 32 * ks + 8 * g;
+            uint4 of[2], with[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                // (Rows past the sequence repeat its last one: no gradient comes from them.)
+                of[x] = ldg16(side + (t0 + min(32 * pair + 16 * x + n, count - 1)) * token + kh * head + e);
+                with[x] = ldg16(a.k + (t0 + min(16 * (2 * x + odd) + n, count - 1)) * a.k_token + kh * a.k_head + e);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) pairs[x][c] = mfma_raw<FP16>(of[x], with[c], pairs[x][c]);
+        }
+    }
+    auto raw = [&](const uint32_t (&v)[2], int i) { return elem16<FP16>(static_cast<uint16_t>(v[i / 2] >> (16 * (i % 2)))); };
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 dq[2][TPQ], dk[2][TPQ];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int t = 0; t < TPQ; ++t) dq[x][t] = dk[x][t] = zero;
+    const int64_t size = static_cast<int64_t>(D) * E, states = tape_states(w.slots, a.heads, D, E);
+    const int rows = kChunk * E;
+    auto bytes = [](const void* p) { return static_cast<const uint8_t*>(p); };
     for (int hv = 0; hv < a.group; ++hv) {
         const int h = kh * a.group + hv;
-        const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h, size = static_cast<int64_t>(D) * E;
-        const uint16_t* tape = reinterpret_cast<const uint16_t*>(d.tape);
-        const uint16_t* S = tape + by_head * 2 * size;
-        const uint16_t* U = tape + states + by_head * 2 * kChunk * E;
-        const uint16_t* dS = w.ds + by_head * 2 * size;
-        const uint16_t* dR = w.dr + by_head * 2 * kChunk * E;
-        if (tid < kChunk) lds.sum[tid] = w.sums[by_head * kChunk + tid];
-        f32x4 so[TILES], sr[TILES], su[TILES], ou[4], ru[4];
+        const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h;
+        const float* tape = reinterpret_cast<const float*>(d.tape);
+        // The wave's share of a step's staging: a tile of S and dS, one of u or dR.
+        const bool has_tile = wave < TILES;
+        const uint32_t tile_at = 4 * (element_of(wave) * E + 8 * g), rows_at = 4 * ((16 * (wave % 4) + n) * E + 8 * g);
+        const uint8_t* at_s = bytes(tape + by_head * size);
+        const uint8_t* at_ds = bytes(w.ds + by_head * size);
+        const uint8_t* at_rows = bytes(wave < 4 ? tape + states + by_head * rows : w.dr + by_head * rows);
+        const uint16_t* out = d.d_out + static_cast<int64_t>(t0) * d.d_out_token + h * d.d_out_head;
+        if (tid < kChunk) {
+            const double sum = w.sums[by_head * kChunk + tid], last = w.sums[by_head * kChunk + kChunk - 1];
+            lds.sum[tid] = sum;
+            lds.decay[tid] = power(sum);
+            lds.rest[tid] = power(last - sum);
+        }
+        // S do, S dR and dS u of the wave's rows and columns; of do . u (the first
+        // two quarters) and dR . u the tiles of its rows and every other column.
+        f32x4 so[2][TPQ], sr[2][TPQ], su[2][TPQ], xu[2][2];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) so[t] = sr[t] = su[t] = zero;
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) ou[t] = ru[t] = zero;
-        float both = 0.0f;   // <S, dS>, a quarter of the tiles per wave
-        for (int e = 8 * g; e < E; e += 32) {
-            const int row = 16 * wave + n;
-            uint4 o[PARTS], u[2], r[2];
+            for (int t = 0; t < TPQ; ++t) so[x][t] = sr[x][t] = su[x][t] = zero;
+            xu[x][0] = xu[x][1] = zero;
+        }
+        float both = 0.0f;   // <S, dS>
+        uint4 raw_s[2], raw_ds[2], raw_rows[2], o[2][PARTS];
+        auto load = [&](int e0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (has_tile) {
+                    raw_s[i] = frag16(at_s + 4 * e0 + 16 * i, tile_at);
+                    raw_ds[i] = frag16(at_ds + 4 * e0 + 16 * i, tile_at);
+                }
+                raw_rows[i] = frag16(at_rows + 4 * e0 + 16 * i, rows_at);
+            }
+        };
+        auto floats = [](const uint4 (&v)[2], float (&f)[8]) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f[4 * i] = __uint_as_float(v[i].x), f[4 * i + 1] = __uint_as_float(v[i].y);
+                f[4 * i + 2] = __uint_as_float(v[i].z), f[4 * i + 3] = __uint_as_float(v[i].w);
+            }
+        };
+        auto stage = [&](uint4 (&to)[3][kWave], const float (&f)[8]) {
+            Split2 p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = split2<3>(f[2 * j], f[2 * j + 1]);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) to[j][lane] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
+        };
+        load(0);
+#pragma unroll 1
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            __syncthreads();   // (what was staged before is done with)
             {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (row < count) x = ldg16(d.d_out + static_cast<int64_t>(t0 + row) * d.d_out_token + h * d.d_out_head + e);
-                if constexpr (FP16) {
+                float f[8], f1[8];
+                if (has_tile) {
+                    floats(raw_s, f);
+                    floats(raw_ds, f1);
+                    stage(lds.stage.s[wave], f);
+                    stage(lds.stage.ds[wave], f1);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) both = __builtin_fmaf(f[j], f1[j], both);
+                }
+                floats(raw_rows, f);
+                if (wave < 4) stage(lds.stage.u[wave % 4], f);
+                else stage(lds.stage.r[wave % 4], f);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int row = 32 * pair + 16 * x + n;
+                const uint4 y = frag16(bytes(out), 2 * (min(row, count - 1) * static_cast<uint32_t>(d.d_out_token) + e0 + 8 * g));
+                o[x][0] = row < count ? y : make_uint4(0u, 0u, 0u, 0u);
+            }
+            load(e0 + 32 < E ? e0 + 32 : 0);
+            __syncthreads();
+            if constexpr (FP16) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
                     float f[8];
-                    unpack16<true>(x, f);
-                    Split2 p[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) o[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
-                } else {
-                    o[0] = x;
+                    unpack16<true>(o[x][0], f);
+                    two_parts(reinterpret_cast<uint4 (&)[2]>(o[x]), f);
                 }
             }
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                u[p] = ldg16(U + (p * kChunk + row) * E + e);
-                r[p] = ldg16(dR + (p * kChunk + row) * E + e);
-            }
+            for (int x = 0; x < 2; ++x) {
+                const int tile = 2 * pair + x;
+                uint4 u[3], r[3];
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                uint4 bs[2], bd[2];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    bs[p] = ldg16(S + p * size + static_cast<int64_t>(element(t)) * E + e);
-                    bd[p] = ldg16(dS + p * size + static_cast<int64_t>(element(t)) * E + e);
+                for (int p = 0; p < 3; ++p) {
+                    u[p] = lds.stage.u[tile][p][lane];
+                    r[p] = lds.stage.r[tile][p][lane];
                 }
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
+                for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                    for (int x = 0; x + p < 2; ++x) {
-                        if (x < PARTS) so[t] = mfma16x16x32(o[x], bs[p], so[t]);
-                        sr[t] = mfma16x16x32(r[x], bs[p], sr[t]);
-                        su[t] = mfma16x16x32(u[x], bd[p], su[t]);
+                    for (int t = 0; t < TPQ; ++t) {
+                        const uint4 bs = lds.stage.s[quarter * TPQ + t][p][lane], bd = lds.stage.ds[quarter * TPQ + t][p][lane];
+#pragma unroll
+                        for (int y = 0; y + p < 3; ++y) {
+                            if (y < PARTS) so[x][t] = mfma16x16x32(o[x][y], bs, so[x][t]);
+                            sr[x][t] = mfma16x16x32(r[y], bs, sr[x][t]);
+                            su[x][t] = mfma16x16x32(u[y], bd, su[x][t]);
+                        }
                     }
-                if (t % 4 == wave) {
-                    float x[8], x1[8], y[8], y1[8];
-                    unpack8(bs[0], x), unpack8(bs[1], x1), unpack8(bd[0], y), unpack8(bd[1], y1);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) both = __builtin_fmaf(x[j] + x1[j], y[j] + y1[j], both);
-                }
-            }
+                    for (int j = 0; j < 2; ++j) {
+                        if (2 * j + odd > tile) continue;
+                        const uint4 bu = lds.stage.u[2 * j + odd][p][lane];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t > wave) continue;
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint4 b = ldg16(U + (p * kChunk + 16 * t + n) * E + e);
-#pragma unroll
-                    for (int x = 0; x + p < 2; ++x) {
-                        if (x < PARTS) ou[t] = mfma16x16x32(o[x], b, ou[t]);
-                        ru[t] = mfma16x16x32(r[x], b, ru[t]);
+                        for (int y = 0; y + p < 3; ++y) {
+                            if (quarter >= 2) xu[x][j] = mfma16x16x32(r[y], bu, xu[x][j]);
+                            else if (y < PARTS) xu[x][j] = mfma16x16x32(o[x][y], bu, xu[x][j]);
+                        }
                     }
                 }
             }
@@ -1008,165 +1211,215 @@ __global__ __launch_bounds__(kThreads, 1) void scan_inputs_grad(ScanArgs a, Scan
         if (lane == 0) lds.state[wave] = both;
         __syncthreads();   // (sums, and the last head's matrices are done with)
         const double last = lds.sum[kChunk - 1];
-        f32x4 decay, rest;
+        float by_row[2][4], by_col[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            decay[i] = power(lds.sum[r0 + i]);
-            rest[i] = power(last - lds.sum[r0 + i]);
-        }
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t > wave) continue;
-            const int j = 16 * t + n;
+            for (int y = 0; y < 4; ++y) by_row[x][y] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = r0 + r;
-                const float fade = power(lds.sum[i] - lds.sum[j]);
-                lds.b1[i * kPitch + j] = j <= i ? fade * ou[t][r] : 0.0f;
-                lds.b2[i * kPitch + j] = j < i ? fade * ru[t][r] : 0.0f;
-                if (i == j && i < count) {
-                    const int64_t at = static_cast<int64_t>(t0 + i) * a.heads + h, from = static_cast<int64_t>(t0 + i) * a.beta_token + h;
-                    const float b = scan_beta(a.beta_fp32 ? static_cast<const float*>(a.beta)[from]
-                                                          : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[from]));
-                    const float db = ru[t][r] / b / b;
-                    if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = db;
-                    else static_cast<uint16_t*>(d.dbeta)[at] = static_cast<uint16_t>(pack16_2<FP16>(db, 0.0f));
-                }
-            }
-        }
-        __syncthreads();
-        // The four products over tokens: rows of B1 and B2, then their columns.
-        f32x4 by_q[TILES], by_row[TILES], by_col[TILES];
-        f32x4 dot_state = zero;   // k_i . (dS u_i) e^(G_63 - G_i)
+            for (int c = 0; c < 2; ++c) {
+                const int tile = 2 * c + odd;
+                if (tile > 2 * pair + x) continue;
+                const int j = 16 * tile + n;
+                const float factor = quarter < 2 ? lds.rk[j] * a.scale : -lds.rk[j];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            by_q[t] = so[t] * decay;
-            by_row[t] = sr[t] * decay;
-            by_col[t] = su[t] * rest;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dot_state[i] = __builtin_fmaf(elem16<FP16>(k[t][i]), by_col[t][i], dot_state[i]);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            uint4 q_row[2], k_row[2], q_col[2], k_col[2];
-            const bool rows = 2 * ks <= wave, cols = 2 * ks + 1 >= wave;
-            {
-                float x[4][8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int block = 2 * ks + j / 4, o = 16 * block + 4 * g + j % 4, own = 16 * wave + n;
-                    const bool low = block <= wave, high = block >= wave;
-                    const float rk = lds.rk[o], rq = lds.rq[o] * a.scale;
-                    x[0][j] = low ? lds.b1[own * kPitch + o] * rk : 0.0f;
-                    x[1][j] = low ? lds.b2[own * kPitch + o] * rk : 0.0f;
-                    x[2][j] = high ? lds.b1[o * kPitch + own] * rq : 0.0f;
-                    x[3][j] = high ? -lds.b2[o * kPitch + own] * rk : 0.0f;
-                }
-                auto parts = [&](uint4 (&to)[2], const float (&f)[8]) {
-                    Split2 p[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) to[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
-                };
-                parts(q_row, x[0]);
-                parts(k_row, x[1]);
-                parts(q_col, x[2]);
-                parts(k_col, x[3]);
-            }
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    const int64_t at = ((by_key * TILES * 2 + t * 2 + ks) * PARTS + p) * kFragBytes + lane * 16;
-                    const uint4 bk = ldg16(w.kt + at), bq = ldg16(w.qt + at);
-#pragma unroll
-                    for (int x = 0; x + p < 2; ++x) {
-                        if (rows) {
-                            by_q[t] = mfma16x16x32(q_row[x], bk, by_q[t]);
-                            by_row[t] = mfma16x16x32(k_row[x], bk, by_row[t]);
-                        }
-                        if (cols) {
-                            by_col[t] = mfma16x16x32(q_col[x], bq, by_col[t]);
-                            by_col[t] = mfma16x16x32(k_col[x], bk, by_col[t]);
-                        }
+                for (int y = 0; y < 4; ++y) {
+                    const int i = row_of(x, y);
+                    const float b = power(lds.sum[i] - lds.sum[j]) * xu[x][c][y];
+                    const float m = j < i ? b * pairs[x][c][y] * factor * (quarter < 2 ? lds.rq[i] : lds.rk[i]) : 0.0f;
+                    by_row[x][y] += m;
+                    by_col[c] += m;
+                    if (quarter < 2) {
+                        lds.m.b1[i * kPitch + j] = j <= i ? b : 0.0f;
+                        continue;
+                    }
+                    lds.m.b2[i * kPitch + j] = j < i ? b : 0.0f;
+                    if (i == j && i < count) {
+                        const int64_t at = static_cast<int64_t>(t0 + i) * a.heads + h;
+                        const int64_t from = static_cast<int64_t>(t0 + i) * a.beta_token + h;
+                        const float v = scan_beta(a.beta_fp32 ? static_cast<const float*>(a.beta)[from]
+                                                              : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[from]));
+                        const float db = xu[x][c][y] / v / v;
+                        if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = db;
+                        else static_cast<uint16_t*>(d.dbeta)[at] = static_cast<uint16_t>(pack16_2<FP16>(db, 0.0f));
                     }
                 }
-        }
-        f32x4 dot_q = zero, dot_k = zero;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dot_q[i] = __builtin_fmaf(elem16<FP16>(q[t][i]), by_q[t][i], dot_q[i]);
-                dot_k[i] = __builtin_fmaf(elem16<FP16>(k[t][i]), -by_row[t][i] - by_col[t][i], dot_k[i]);
             }
-            dq[t] += by_q[t];
-            dk[t] += by_col[t] - by_row[t];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float sum = sum_over_16(by_row[x][y]);
+                if (n == 0) lds.row[quarter][row_of(x, y)] = sum;
+            }
         }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float sum = butterfly_step32(butterfly_step16(by_col[c]));
+            if (g == 0) lds.col[2 * pair + quarter / 2][16 * (2 * c + odd) + n] = sum;
+        }
+        __syncthreads();
+        // The matrices as fragments: 24 of them, three per wave.
+#pragma unroll 1
+        for (int f = wave; f < 4 * kBlocks; f += kGradThreads / kWave) {
+            const int kind = f / kBlocks, block = f % kBlocks;
+            const bool by_rows = kind < 2;
+            const int ks = by_rows ? block >= 4 : block < 4;
+            const int tile = by_rows ? (ks ? block - 2 : block) : (ks ? block : block - 4);
+            const float* m = kind % 2 ? lds.m.b2 : lds.m.b1;
+            const int own = 16 * tile + n;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int of = 2 * ks + j / 4, o = 16 * of + 4 * g + j % 4;
+                const bool in = by_rows ? of <= tile : of >= tile;
+                const float v = in ? m[by_rows ? own * kPitch + o : o * kPitch + own] : 0.0f;
+                x[j] = v * (kind == 2 ? lds.rq[o] * a.scale : kind == 3 ? -lds.rk[o] : lds.rk[o]);
+            }
+            uint4 parts[2];
+            two_parts(parts, x);
+            lds.m.frag[kind][block][0][lane] = parts[0];
+            lds.m.frag[kind][block][1][lane] = parts[1];
+        }
+        // The states' parts of the decays' gradient, before the products over
+        // tokens join them.
         float moved = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float rk = lds.rk[r0 + i];
-            const float sum = sum_over_16(dot_q[i] * lds.rq[r0 + i] * a.scale + dot_k[i] * rk);
-            moved += sum_over_16(dot_state[i] * rk);
-            if (n == 0) lds.row[r0 + i] = sum;
-        }
-        moved += __shfl_xor(moved, 16);
-        moved += __shfl_xor(moved, 32);
-        const float before = lds.state[0] + lds.state[1] + lds.state[2] + lds.state[3];
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = row_of(x, i);
+                float of_q = 0.0f, of_k = 0.0f, of_u = 0.0f;
+#pragma unroll
+                for (int t = 0; t < TPQ; ++t) {
+                    so[x][t][i] *= lds.decay[row];
+                    sr[x][t][i] *= lds.decay[row];
+                    su[x][t][i] *= lds.rest[row];
+                    of_q = __builtin_fmaf(raw(q[x][t], i), so[x][t][i], of_q);
+                    of_k = __builtin_fmaf(raw(k[x][t], i), sr[x][t][i], of_k);
+                    of_u = __builtin_fmaf(raw(k[x][t], i), su[x][t][i], of_u);
+                }
+                of_u = sum_over_16(of_u * lds.rk[row]);
+                const float sum = sum_over_16(of_q * lds.rq[row] * a.scale - of_k * lds.rk[row]) - of_u;
+                if (n == 0) lds.dot[quarter][row] = sum;
+                moved += of_u;
+            }
+        moved = butterfly_step32(butterfly_step16(moved));
+        if (lane == 0) lds.moved[wave] = moved;
         __syncthreads();
-        if (lane == 0) lds.state[wave] = moved;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const int tile = 2 * pair + x;
+                uint4 kt[TPQ][PARTS], qt[TPQ][PARTS];
+#pragma unroll
+                for (int t = 0; t < TPQ; ++t)
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const int64_t at = (((by_key * TILES + quarter * TPQ + t) * 2 + ks) * PARTS + p) * kFragBytes;
+                        kt[t][p] = frag16(w.kt + at, lane * 16);
+                        qt[t][p] = frag16(w.qt + at, lane * 16);
+                    }
+#pragma unroll
+                for (int kind = 0; kind < 4; ++kind) {
+                    if (kind < 2 ? 2 * ks > tile : 2 * ks + 1 < tile) continue;
+                    const int block = kind < 2 ? lower_block(ks, tile) : upper_block(ks, tile);
+                    uint4 f[2];
+                    f[0] = lds.m.frag[kind][block][0][lane];
+                    f[1] = lds.m.frag[kind][block][1][lane];
+#pragma unroll
+                    for (int t = 0; t < TPQ; ++t)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                            for (int y = 0; y + p < 2; ++y) {
+                                if (kind == 0) so[x][t] = mfma16x16x32(f[y], kt[t][p], so[x][t]);
+                                if (kind == 1) sr[x][t] = mfma16x16x32(f[y], kt[t][p], sr[x][t]);
+                                if (kind == 2) su[x][t] = mfma16x16x32(f[y], qt[t][p], su[x][t]);
+                                if (kind == 3) su[x][t] = mfma16x16x32(f[y], kt[t][p], su[x][t]);
+                            }
+                }
+            }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int t = 0; t < TPQ; ++t) {
+                    dq[x][t][i] += so[x][t][i];
+                    dk[x][t][i] += su[x][t][i] - sr[x][t][i];
+                }
+            }
         __syncthreads();
         if (wave == 0) {
-            // From t on: the whole less what lies before.
-            const float after = lds.state[0] + lds.state[1] + lds.state[2] + lds.state[3] +
-                                before * power(last);
-            float x = lds.row[kChunk - 1 - lane];
+            // From t on: the sum over the rows from there, and the state's.
+            float after = 0.0f, before = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kGradThreads / kWave; ++i) {
+                after += lds.moved[i];
+                before += lds.state[i];
+            }
+            after = __builtin_fmaf(before, power(last), after);
+            const int t = kChunk - 1 - lane;
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x += lds.dot[i][t] + (lds.row[i][t] - lds.col[i][t]);
 #pragma unroll
             for (int off = 1; off < kWave; off <<= 1) {
                 const float other = __shfl_up(x, off);
                 if (lane >= off) x += other;
             }
-            const int t = kChunk - 1 - lane;
             if (t < count) d.dg[static_cast<int64_t>(t0 + t) * a.heads + h] = x + after;
         }
         __syncthreads();
     }
     // Through the norms, and out by rows.
-    uint16_t* out = reinterpret_cast<uint16_t*>(lds.b1);
-    for (int side = 0; side < 2; ++side) {
-        f32x4 factor, back = zero;
+    if (a.normalize) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) factor[i] = side ? lds.rk[r0 + i] : lds.rq[r0 + i];
-        if (a.normalize) {
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float dot = 0.0f;
+                float of_q = 0.0f, of_k = 0.0f;
 #pragma unroll
-                for (int t = 0; t < TILES; ++t)
-                    dot = __builtin_fmaf(elem16<FP16>(side ? k[t][i] : q[t][i]), side ? dk[t][i] : dq[t][i], dot);
-                back[i] = sum_over_16(dot) * factor[i] * factor[i];
+                for (int t = 0; t < TPQ; ++t) {
+                    of_q = __builtin_fmaf(raw(q[x][t], i), dq[x][t][i], of_q);
+                    of_k = __builtin_fmaf(raw(k[x][t], i), dk[x][t][i], of_k);
+                }
+                of_q = sum_over_16(of_q), of_k = sum_over_16(of_k);
+                if (n == 0) {
+                    lds.row[quarter][row_of(x, i)] = of_q;
+                    lds.col[quarter][row_of(x, i)] = of_k;
+                }
+            }
+    }
+    __syncthreads();
+    uint16_t* rows_q = reinterpret_cast<uint16_t*>(lds.m.b1);
+    uint16_t* rows_k = reinterpret_cast<uint16_t*>(lds.m.b2);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = row_of(x, i);
+            const float rq = lds.rq[row], rk = lds.rk[row];
+            float back_q = 0.0f, back_k = 0.0f;
+            if (a.normalize) {
+                back_q = rq * rq * ((lds.row[0][row] + lds.row[1][row]) + (lds.row[2][row] + lds.row[3][row]));
+                back_k = rk * rk * ((lds.col[0][row] + lds.col[1][row]) + (lds.col[2][row] + lds.col[3][row]));
+            }
+#pragma unroll
+            for (int t = 0; t < TPQ; ++t) {
+                const float y = (dq[x][t][i] - raw(q[x][t], i) * back_q) * rq * a.scale;
+                const float z = (dk[x][t][i] - raw(k[x][t], i) * back_k) * rk;
+                rows_q[row * RAW + element(t)] = static_cast<uint16_t>(pack16_2<FP16>(y, 0.0f));
+                rows_k[row * RAW + element(t)] = static_cast<uint16_t>(pack16_2<FP16>(z, 0.0f));
             }
         }
-        const float by = side ? 1.0f : a.scale;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = elem16<FP16>(side ? k[t][i] : q[t][i]);
-                const float y = (side ? dk[t][i] : dq[t][i]) - x * back[i];
-                out[(r0 + i) * RAW + element(t)] = static_cast<uint16_t>(pack16_2<FP16>(y * factor[i] * by, 0.0f));
-            }
-        __syncthreads();
-        uint16_t* to = side ? d.dk : d.dq;
-        for (int i = tid; i < kChunk * D / 8; i += kThreads) {
-            const int r = i / (D / 8), e = i % (D / 8) * 8;
-            if (r < count)
-                *reinterpret_cast<uint4*>(to + (static_cast<int64_t>(t0 + r) * a.key_heads + kh) * D + e) =
-                    *reinterpret_cast<const uint4*>(out + r * RAW + e);
-        }
-        __syncthreads();
+    __syncthreads();
+    for (int i = tid; i < kChunk * D / 8; i += kGradThreads) {
+        const int r = i / (D / 8), e = i % (D / 8) * 8;
+        if (r >= count) continue;
+        const int64_t to = (static_cast<int64_t>(t0 + r) * a.key_heads + kh) * D + e;
+        *reinterpret_cast<uint4*>(d.dq + to) = *reinterpret_cast<const uint4*>(rows_q + r * RAW + e);
+        *reinterpret_cast<uint4*>(d.dk + to) = *reinterpret_cast<const uint4*>(rows_k + r * RAW + e);
     }
 }
 
@@ -1188,12 +1441,12 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
     w.kt = take(transposed);
     if (fp16) w.kf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
     if (grad) {
-        const size_t columns = static_cast<size_t>(a.value_dim) * sizeof(uint16_t);
+        const size_t columns = static_cast<size_t>(a.value_dim) * sizeof(float);
         w.qt = take(transposed);
         w.sums = reinterpret_cast<double*>(take(by_head * kChunk * sizeof(double)));
         w.norms = reinterpret_cast<float*>(take(by_key * 2 * kChunk * sizeof(float)));
-        w.ds = reinterpret_cast<uint16_t*>(take(by_head * 2 * a.dim * columns));
-        w.dr = reinterpret_cast<uint16_t*>(take(by_head * 2 * kChunk * columns));
+        w.ds = reinterpret_cast<float*>(take(by_head * a.dim * columns));
+        w.dr = reinterpret_cast<float*>(take(by_head * kChunk * columns));
     } else {
         if (fp16) w.qf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
         w.flags = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(a.seqs) * a.heads * (a.value_dim / 16) * 4));
@@ -1209,9 +1462,9 @@ void launch(const ScanArgs& a, const ScanChunks& w, hipStream_t stream) {
     scan_prepare<D, FP16, false><<<static_cast<uint32_t>(w.slots) * a.key_heads, kThreads, 0, stream>>>(a, w);
     const int items = a.seqs * a.heads * (a.value_dim / 32);
     const int grid = (items + 7) / 8 * 8;
-    if (a.tape != nullptr) scan_chunks<D, 2, FP16, true><<<grid, kThreads, 0, stream>>>(a, w);
-    else if (items <= 128) scan_chunks<D, 1, FP16, false><<<(2 * items + 7) / 8 * 8, kThreads, 0, stream>>>(a, w);
-    else scan_chunks<D, 2, FP16, false><<<grid, kThreads, 0, stream>>>(a, w);
+    if (a.tape != nullptr) scan_chunks<D, 2, FP16, true><<<grid, kChainThreads, 0, stream>>>(a, w);
+    else if (items <= 128) scan_chunks<D, 1, FP16, false><<<(2 * items + 7) / 8 * 8, kChainThreads, 0, stream>>>(a, w);
+    else scan_chunks<D, 2, FP16, false><<<grid, kChainThreads, 0, stream>>>(a, w);
 }
 
 template <int D, bool FP16>
@@ -1219,8 +1472,8 @@ void launch_grad(const ScanArgs& a, const ScanGradArgs& d, const ScanChunks& w, 
     const uint32_t chunks = static_cast<uint32_t>(w.slots) * a.key_heads;
     scan_prepare<D, FP16, true><<<chunks, kThreads, 0, stream>>>(a, w);
     const int items = a.seqs * a.heads * (a.value_dim / 32);
-    scan_chunks_grad<D, FP16><<<(items + 7) / 8 * 8, kThreads, 0, stream>>>(a, d, w);
-    scan_inputs_grad<D, FP16><<<chunks, kThreads, 0, stream>>>(a, d, w);
+    scan_chunks_grad<D, FP16><<<(items + 7) / 8 * 8, kChainThreads, 0, stream>>>(a, d, w);
+    scan_inputs_grad<D, FP16><<<chunks, kGradThreads, 0, stream>>>(a, d, w);
 }
 
 }  // namespace
@@ -1245,8 +1498,7 @@ hipError_t launch_scan_chunks(const ScanArgs& a, bool fp16, void* workspace, con
 }
 
 size_t delta_scan_tape_bytes(const ScanArgs& a) {
-    return static_cast<size_t>(scan_slots(a.tokens, a.seqs)) * a.heads * 2 * (a.dim + kChunk) * a.value_dim *
-           sizeof(uint16_t);
+    return static_cast<size_t>(scan_slots(a.tokens, a.seqs)) * a.heads * (a.dim + kChunk) * a.value_dim * sizeof(float);
 }
 
 size_t delta_scan_grad_workspace_bytes(const ScanArgs& a, bool fp16) {

@@ -201,7 +201,7 @@ class _DeltaScan(torch.autograd.Function):
         first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
         d = _native.DeltaGradArgs(tape=tape[0].data_ptr(), d_initial=_ptr(first))
         # Of a gradient that torch hands in, expanded or transposed, a plain copy is taken.
-        bad = d_out.stride(-1) != 1 or d_out.data_ptr() % 16 or any(x % 8 for x in d_out.stride()[:-1])
+        bad = d_out.stride(-1) != 1 or d_out.data_ptr() % 16 or any(x % 8 or not 0 <= x < 1 << 23 for x in d_out.stride()[:-1])
         d_out = d_out.contiguous() if bad else d_out
         d_final = d_final.contiguous()
         d_final = d_final.clone() if d_final.data_ptr() % 16 else d_final
