@@ -47,6 +47,12 @@ __device__ __forceinline__ int find_sequence(const int32_t* starts, int seqs, in
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// A number of which the compiler knows nothing, least of all that it was there before.
+__device__ __forceinline__ int opaque(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ uint4 frag16(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint4*>(p + at); }
 
 __device__ __forceinline__ float power(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
@@ -990,8 +996,9 @@ struct ScanInputsLds {
             uint4 frag[4][kBlocks][2][kWave];   // B1 and B2 by rows (lower blocks), by columns (upper ones)
         } m;
     };
+    float qk[kChunk * kPitch], kk[kChunk * kPitch];   // raw
     double sum[kChunk];
-    float rk[kChunk], rq[kChunk], decay[kChunk], rest[kChunk];
+    float rk[kChunk], rq[kChunk], decay[kChunk], rest[kChunk], beta[kChunk], dbeta[kChunk];
     float dot[4][kChunk], row[4][kChunk], col[4][kChunk], state[8], moved[8];
 };
 
@@ -1015,7 +1022,8 @@ template <int D, bool FP16>
 __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TILES = D / 16, TPQ = D / 64, RAW = D + 8;
     __shared__ ScanInputsLds<D> lds;
-    const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
+    const int tid = threadIdx.x;
+    int lane = tid % kWave, n = lane % 16, g = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), pair = wave % 2, quarter = wave / 2;
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
     const int s = find_sequence(a.starts, a.seqs, slot);
@@ -1041,24 +1049,25 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                q[x][t][i] = k[x][t][i] = 0;
+                // (Rows past the sequence repeat its last one: what they meet is 0.)
+                uint32_t of_q[2], of_k[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int row = row_of(x, 2 * i + j);
-                    if (row >= count) continue;
-                    const int64_t at = t0 + row;
-                    q[x][t][i] |= static_cast<uint32_t>(a.q[at * a.q_token + kh * a.q_head + element(t)]) << (16 * j);
-                    k[x][t][i] |= static_cast<uint32_t>(a.k[at * a.k_token + kh * a.k_head + element(t)]) << (16 * j);
+                    const int64_t at = t0 + min(row_of(x, 2 * i + j), count - 1);
+                    of_q[j] = a.q[at * a.q_token + kh * a.q_head + element(t)];
+                    of_k[j] = a.k[at * a.k_token + kh * a.k_head + element(t)];
                 }
+                q[x][t][i] = of_q[0] | (of_q[1] << 16);
+                k[x][t][i] = of_k[0] | (of_k[1] << 16);
             }
     }
-    // q_i . k_j, or for the second two quarters k_i . k_j, of the tiles that the
-    // wave has of B1 or B2.
+    // q_i . k_j, or in the second two quarters k_i . k_j, of the wave's rows and
+    // every other column tile.
     const int odd = quarter % 2;
-    f32x4 pairs[2][2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) pairs[x][0] = pairs[x][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     {
+        f32x4 pairs[2][2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) pairs[x][0] = pairs[x][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         const uint16_t* side = quarter < 2 ? a.q : a.k;
         const int64_t token = quarter < 2 ? a.q_token : a.k_token, head = quarter < 2 ? a.q_head : a.k_head;
 #pragma unroll
@@ -1067,7 +1076,6 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
             uint4 of[2], with[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                // (Rows past the sequence repeat its last one: no gradient comes from them.)
                 of[x] = ldg16(side + (t0 + min(32 * pair + 16 * x + n, count - 1)) * token + kh * head + e);
                 with[x] = ldg16(a.k + (t0 + min(16 * (2 * x + odd) + n, count - 1)) * a.k_token + kh * a.k_head + e);
             }
@@ -1076,6 +1084,13 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
 #pragma unroll
                 for (int c = 0; c < 2; ++c) pairs[x][c] = mfma_raw<FP16>(of[x], with[c], pairs[x][c]);
         }
+        float* to = quarter < 2 ? lds.qk : lds.kk;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[row_of(x, i) * kPitch + 16 * (2 * c + odd) + n] = pairs[x][c][i];
     }
     auto raw = [&](const uint32_t (&v)[2], int i) { return elem16<FP16>(static_cast<uint16_t>(v[i / 2] >> (16 * (i % 2)))); };
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1088,6 +1103,10 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
     const int rows = kChunk * E;
     auto bytes = [](const void* p) { return static_cast<const uint8_t*>(p); };
     for (int hv = 0; hv < a.group; ++hv) {
+        // (Addresses are computed where they are used: kept over the loop they
+        // would take more registers than there are.)
+        lane = opaque(lane);
+        n = lane % 16, g = lane / 16;
         const int h = kh * a.group + hv;
         const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h;
         const float* tape = reinterpret_cast<const float*>(d.tape);
@@ -1098,12 +1117,6 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
         const uint8_t* at_ds = bytes(w.ds + by_head * size);
         const uint8_t* at_rows = bytes(wave < 4 ? tape + states + by_head * rows : w.dr + by_head * rows);
         const uint16_t* out = d.d_out + static_cast<int64_t>(t0) * d.d_out_token + h * d.d_out_head;
-        if (tid < kChunk) {
-            const double sum = w.sums[by_head * kChunk + tid], last = w.sums[by_head * kChunk + kChunk - 1];
-            lds.sum[tid] = sum;
-            lds.decay[tid] = power(sum);
-            lds.rest[tid] = power(last - sum);
-        }
         // S do, S dR and dS u of the wave's rows and columns; of do . u (the first
         // two quarters) and dR . u the tiles of its rows and every other column.
         f32x4 so[2][TPQ], sr[2][TPQ], su[2][TPQ], xu[2][2];
@@ -1140,6 +1153,17 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
             for (int j = 0; j < 3; ++j) to[j][lane] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
         };
         load(0);
+        __builtin_amdgcn_sched_barrier(0);
+        // (Used behind the loop: a row's running sum, the last one, raw beta.)
+        const double* sums = w.sums + by_head * kChunk;
+        const double sum = sums[lane], last = sums[kChunk - 1];
+        uint32_t raw_beta;
+        {
+            const int64_t at = static_cast<int64_t>(t0 + min(lane, count - 1)) * a.beta_token + h;
+            if (a.beta_fp32) raw_beta = static_cast<const uint32_t*>(a.beta)[at];
+            else raw_beta = static_cast<const uint16_t*>(a.beta)[at];
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
         for (int e0 = 0; e0 < E; e0 += 32) {
             __syncthreads();   // (what was staged before is done with)
@@ -1173,111 +1197,132 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
                     two_parts(reinterpret_cast<uint4 (&)[2]>(o[x]), f);
                 }
             }
+            uint4 u[2][3], r[2][3];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int tile = 2 * pair + x;
-                uint4 u[3], r[3];
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {
-                    u[p] = lds.stage.u[tile][p][lane];
-                    r[p] = lds.stage.r[tile][p][lane];
+                    u[x][p] = lds.stage.u[2 * pair + x][p][lane];
+                    r[x][p] = lds.stage.r[2 * pair + x][p][lane];
                 }
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                    for (int t = 0; t < TPQ; ++t) {
-                        const uint4 bs = lds.stage.s[quarter * TPQ + t][p][lane], bd = lds.stage.ds[quarter * TPQ + t][p][lane];
+                for (int t = 0; t < TPQ; ++t) {
+                    const uint4 bs = lds.stage.s[quarter * TPQ + t][p][lane], bd = lds.stage.ds[quarter * TPQ + t][p][lane];
 #pragma unroll
-                        for (int y = 0; y + p < 3; ++y) {
+                    for (int y = 0; y + p < 3; ++y)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
                             if (y < PARTS) so[x][t] = mfma16x16x32(o[x][y], bs, so[x][t]);
-                            sr[x][t] = mfma16x16x32(r[y], bs, sr[x][t]);
-                            su[x][t] = mfma16x16x32(u[y], bd, su[x][t]);
+                            sr[x][t] = mfma16x16x32(r[x][y], bs, sr[x][t]);
+                            su[x][t] = mfma16x16x32(u[x][y], bd, su[x][t]);
                         }
-                    }
+                }
+                // (Tiles above the diagonal are computed and not used.)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (2 * j + odd > tile) continue;
-                        const uint4 bu = lds.stage.u[2 * j + odd][p][lane];
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 bu = lds.stage.u[2 * j + odd][p][lane];
+                    if (quarter >= 2) {
 #pragma unroll
-                        for (int y = 0; y + p < 3; ++y) {
-                            if (quarter >= 2) xu[x][j] = mfma16x16x32(r[y], bu, xu[x][j]);
-                            else if (y < PARTS) xu[x][j] = mfma16x16x32(o[x][y], bu, xu[x][j]);
-                        }
+                        for (int y = 0; y + p < 3; ++y)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) xu[x][j] = mfma16x16x32(r[x][y], bu, xu[x][j]);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < PARTS && y + p < 3; ++y)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) xu[x][j] = mfma16x16x32(o[x][y], bu, xu[x][j]);
                     }
                 }
             }
         }
         both = wave_butterfly_sum(both);
         if (lane == 0) lds.state[wave] = both;
-        __syncthreads();   // (sums, and the last head's matrices are done with)
-        const double last = lds.sum[kChunk - 1];
-        float by_row[2][4], by_col[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y) by_row[x][y] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int tile = 2 * c + odd;
-                if (tile > 2 * pair + x) continue;
-                const int j = 16 * tile + n;
-                const float factor = quarter < 2 ? lds.rk[j] * a.scale : -lds.rk[j];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int i = row_of(x, y);
-                    const float b = power(lds.sum[i] - lds.sum[j]) * xu[x][c][y];
-                    const float m = j < i ? b * pairs[x][c][y] * factor * (quarter < 2 ? lds.rq[i] : lds.rk[i]) : 0.0f;
-                    by_row[x][y] += m;
-                    by_col[c] += m;
-                    if (quarter < 2) {
-                        lds.m.b1[i * kPitch + j] = j <= i ? b : 0.0f;
-                        continue;
-                    }
-                    lds.m.b2[i * kPitch + j] = j < i ? b : 0.0f;
-                    if (i == j && i < count) {
-                        const int64_t at = static_cast<int64_t>(t0 + i) * a.heads + h;
-                        const int64_t from = static_cast<int64_t>(t0 + i) * a.beta_token + h;
-                        const float v = scan_beta(a.beta_fp32 ? static_cast<const float*>(a.beta)[from]
-                                                              : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[from]));
-                        const float db = xu[x][c][y] / v / v;
-                        if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = db;
-                        else static_cast<uint16_t*>(d.dbeta)[at] = static_cast<uint16_t>(pack16_2<FP16>(db, 0.0f));
-                    }
-                }
-            }
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const float sum = sum_over_16(by_row[x][y]);
-                if (n == 0) lds.row[quarter][row_of(x, y)] = sum;
-            }
+        if (tid < kChunk) {
+            lds.sum[tid] = sum;
+            lds.decay[tid] = power(sum);
+            lds.rest[tid] = power(last - sum);
+            lds.beta[tid] = scan_beta(a.beta_fp32 ? __uint_as_float(raw_beta) : elem16<FP16>(static_cast<uint16_t>(raw_beta)));
         }
+        __syncthreads();   // (the staging is done with)
+        {
+            float* to = quarter < 2 ? lds.m.b1 : lds.m.b2;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const float sum = butterfly_step32(butterfly_step16(by_col[c]));
-            if (g == 0) lds.col[2 * pair + quarter / 2][16 * (2 * c + odd) + n] = sum;
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[row_of(x, i) * kPitch + 16 * (2 * c + odd) + n] = xu[x][c][i];
         }
         __syncthreads();
-        // The matrices as fragments: 24 of them, three per wave.
-#pragma unroll 1
-        for (int f = wave; f < 4 * kBlocks; f += kGradThreads / kWave) {
-            const int kind = f / kBlocks, block = f % kBlocks;
-            const bool by_rows = kind < 2;
-            const int ks = by_rows ? block >= 4 : block < 4;
-            const int tile = by_rows ? (ks ? block - 2 : block) : (ks ? block : block - 4);
-            const float* m = kind % 2 ? lds.m.b2 : lds.m.b1;
-            const int own = 16 * tile + n;
-            float x[8];
+        // Of the matrices a thread has row or column `own` and eight of the others,
+        // as a fragment has them: B1 and B2 with their decays and M's sum by rows,
+        const int tile = wave / 2, half = wave % 2, own = 16 * tile + n;
+        const float own_q = lds.rq[own] * a.scale, own_k = lds.rk[own];
+        if (2 * half <= tile) {
+            const double own_sum = lds.sum[own];
+            float by_row = 0.0f, x1[8], x2[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int of = 2 * ks + j / 4, o = 16 * of + 4 * g + j % 4;
-                const bool in = by_rows ? of <= tile : of >= tile;
-                const float v = in ? m[by_rows ? own * kPitch + o : o * kPitch + own] : 0.0f;
-                x[j] = v * (kind == 2 ? lds.rq[o] * a.scale : kind == 3 ? -lds.rk[o] : lds.rk[o]);
+                const int o = 32 * half + 16 * (j / 4) + 4 * g + j % 4, at = own * kPitch + o;
+                const float fade = power(own_sum - lds.sum[o]), rk = lds.rk[o], raw2 = lds.m.b2[at];
+                if (o == own) lds.dbeta[own] = raw2 / lds.beta[own] / lds.beta[own];
+                const float b1 = o <= own ? fade * lds.m.b1[at] : 0.0f, b2 = o < own ? fade * raw2 : 0.0f;
+                lds.m.b1[at] = b1;
+                lds.m.b2[at] = b2;
+                const float m = b1 * lds.qk[at] * (own_q * rk) - b2 * lds.kk[at] * (own_k * rk);
+                by_row += o < own ? m : 0.0f;
+                x1[j] = b1 * rk;
+                x2[j] = b2 * rk;
             }
+            by_row = butterfly_step32(butterfly_step16(by_row));
+            if (g == 0) lds.row[half][own] = by_row;
             uint4 parts[2];
-            two_parts(parts, x);
-            lds.m.frag[kind][block][0][lane] = parts[0];
-            lds.m.frag[kind][block][1][lane] = parts[1];
+            const int block = lower_block(half, tile);
+            two_parts(parts, x1);
+            lds.m.frag[0][block][0][lane] = parts[0];
+            lds.m.frag[0][block][1][lane] = parts[1];
+            two_parts(parts, x2);
+            lds.m.frag[1][block][0][lane] = parts[0];
+            lds.m.frag[1][block][1][lane] = parts[1];
+        } else if (g == 0) {
+            lds.row[half][own] = 0.0f;
+        }
+        __syncthreads();
+        // and by columns.
+        if (2 * half + 1 >= tile) {
+            float by_col = 0.0f, x1[8], x2[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int o = 32 * half + 16 * (j / 4) + 4 * g + j % 4, at = o * kPitch + own;
+                const bool in = o >= own;
+                const float rq = lds.rq[o] * a.scale, rk = lds.rk[o];
+                const float b1 = in ? lds.m.b1[at] : 0.0f, b2 = in ? lds.m.b2[at] : 0.0f;
+                const float m = b1 * lds.qk[at] * (rq * own_k) - b2 * lds.kk[at] * (rk * own_k);
+                by_col += o > own ? m : 0.0f;
+                x1[j] = b1 * rq;
+                x2[j] = -b2 * rk;
+            }
+            by_col = butterfly_step32(butterfly_step16(by_col));
+            if (g == 0) lds.col[half][own] = by_col;
+            uint4 parts[2];
+            const int block = upper_block(half, tile);
+            two_parts(parts, x1);
+            lds.m.frag[2][block][0][lane] = parts[0];
+            lds.m.frag[2][block][1][lane] = parts[1];
+            two_parts(parts, x2);
+            lds.m.frag[3][block][0][lane] = parts[0];
+            lds.m.frag[3][block][1][lane] = parts[1];
+        } else if (g == 0) {
+            lds.col[half][own] = 0.0f;
+        }
+        uint4 kt[TPQ][2][PARTS], qt[TPQ][2][PARTS];
+#pragma unroll
+        for (int i = 0; i < TPQ * 2 * PARTS; ++i) {
+            const int64_t at = ((by_key * TILES + quarter * TPQ) * 2 * PARTS + i) * kFragBytes;
+            kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(w.kt + at, lane * 16);
+            qt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(w.qt + at, lane * 16);
         }
         // The states' parts of the decays' gradient, before the products over
         // tokens join them.
@@ -1306,19 +1351,10 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
         if (lane == 0) lds.moved[wave] = moved;
         __syncthreads();
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
+            for (int x = 0; x < 2; ++x) {
                 const int tile = 2 * pair + x;
-                uint4 kt[TPQ][PARTS], qt[TPQ][PARTS];
-#pragma unroll
-                for (int t = 0; t < TPQ; ++t)
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const int64_t at = (((by_key * TILES + quarter * TPQ + t) * 2 + ks) * PARTS + p) * kFragBytes;
-                        kt[t][p] = frag16(w.kt + at, lane * 16);
-                        qt[t][p] = frag16(w.qt + at, lane * 16);
-                    }
 #pragma unroll
                 for (int kind = 0; kind < 4; ++kind) {
                     if (kind < 2 ? 2 * ks > tile : 2 * ks + 1 < tile) continue;
@@ -1332,10 +1368,10 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
                         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
                             for (int y = 0; y + p < 2; ++y) {
-                                if (kind == 0) so[x][t] = mfma16x16x32(f[y], kt[t][p], so[x][t]);
-                                if (kind == 1) sr[x][t] = mfma16x16x32(f[y], kt[t][p], sr[x][t]);
-                                if (kind == 2) su[x][t] = mfma16x16x32(f[y], qt[t][p], su[x][t]);
-                                if (kind == 3) su[x][t] = mfma16x16x32(f[y], kt[t][p], su[x][t]);
+                                if (kind == 0) so[x][t] = mfma16x16x32(f[y], kt[t][ks][p], so[x][t]);
+                                if (kind == 1) sr[x][t] = mfma16x16x32(f[y], kt[t][ks][p], sr[x][t]);
+                                if (kind == 2) su[x][t] = mfma16x16x32(f[y], qt[t][ks][p], su[x][t]);
+                                if (kind == 3) su[x][t] = mfma16x16x32(f[y], kt[t][ks][p], su[x][t]);
                             }
                 }
             }
@@ -1358,17 +1394,23 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
                 after += lds.moved[i];
                 before += lds.state[i];
             }
-            after = __builtin_fmaf(before, power(last), after);
+            after = __builtin_fmaf(before, lds.decay[kChunk - 1], after);
             const int t = kChunk - 1 - lane;
             float x = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x += lds.dot[i][t] + (lds.row[i][t] - lds.col[i][t]);
+            for (int i = 0; i < 4; ++i) x += lds.dot[i][t];
+            x += (lds.row[0][t] + lds.row[1][t]) - (lds.col[0][t] + lds.col[1][t]);
 #pragma unroll
             for (int off = 1; off < kWave; off <<= 1) {
                 const float other = __shfl_up(x, off);
                 if (lane >= off) x += other;
             }
-            if (t < count) d.dg[static_cast<int64_t>(t0 + t) * a.heads + h] = x + after;
+            if (t < count) {
+                const int64_t at = static_cast<int64_t>(t0 + t) * a.heads + h;
+                d.dg[at] = x + after;
+                if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = lds.dbeta[t];
+                else static_cast<uint16_t*>(d.dbeta)[at] = static_cast<uint16_t>(pack16_2<FP16>(lds.dbeta[t], 0.0f));
+            }
         }
         __syncthreads();
     }
