@@ -318,7 +318,8 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
 
 // ---- launch two: chunk after chunk -----------------------------------------------
 
-constexpr int kChainThreads = 512;
+constexpr int kChainThreads = 768;      // the chain, the outputs, the loads
+constexpr int kChainGradThreads = 512;
 
 // Four values of a lane as half a B fragment (element 4 half on), in parts.
 template <int PARTS, int KS, int NC>
@@ -371,22 +372,28 @@ __device__ __forceinline__ ScanItem scan_item(const ScanArgs& a, int columns) {
 // Waves 0 to 3 have the state's rows of the tiles w TPW .. + TPW - 1, in the
 // accumulators of its own update (column NC n + c of the block in lane n of a
 // group and tile c), and the token rows of tile w on the way there; waves 4 to
-// 7 the outputs of those rows. The products hand their results on through LDS,
-// as the B fragments of the next ones, which the lanes write as they hold them.
-// A step is a chain of three products and hand-overs, and the instructions of
-// one wave on each SIMD; the outputs fill the gaps.
-template <int D, int NC>
+// 7 the outputs of those rows; waves 8 to 11 read what the chain needs, a chunk
+// ahead. The products hand their results on through LDS, as the B fragments of
+// the next ones, which the lanes write as they hold them. A step is a chain of
+// three products and hand-overs, and the instructions of one wave on each SIMD;
+// the other waves' fill the gaps.
+template <int D, int NC, int PARTS>
 struct ScanLds {
     uint4 s[3][D / 32][NC][kWave];
     uint4 r[3][2][NC][kWave];
     uint4 u[2][2][NC][kWave];    // for the outputs
     uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
+    // What waves 4 to 7 have read for waves 0 to 3.
+    uint4 k[4][D / 32 * PARTS][kWave], t[4][6][kWave], kt[4][D / 64 * 2 * PARTS][kWave];
+    f32x4 vec[2][3][16];         // the factors, of two chunks
+    float decay[2];
+    uint32_t v[4][4][kWave];
 };
 
 template <int D, int NC, bool FP16, bool TAPE>
-__global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, ScanChunks w) {
+__global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32;
-    __shared__ ScanLds<D, NC> lds;
+    __shared__ ScanLds<D, NC, PARTS> lds;
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
     const int role = __builtin_amdgcn_readfirstlane(tid / kWave), wave = role % 4;
     const ScanItem item = scan_item(a, 16 * NC);
@@ -441,17 +448,88 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
             to[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * P + p) * kFragBytes, frag);
         }
     };
-    auto factors = [&](int ch, int kind) {
-        return *reinterpret_cast<const f32x4*>(w.vec + ((slot0 + ch) * a.heads + h) * 256 + 64 * kind + r0);
-    };
+    if (role >= 8) {
+        uint4 k[KS][PARTS], t[2][3], kt[TPW][2][PARTS];
+        uint32_t v[4];
+        f32x4 vec;
+        float decay;
+        auto load_kt = [&](int ch) {
+            const uint8_t* at = w.kt + (((slot0 + ch) * a.key_heads + kh) * (D / 16) + wave * TPW) * 2 * PARTS * kFragBytes;
+#pragma unroll
+            for (int i = 0; i < TPW * 2 * PARTS; ++i)
+                kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
+        };
+        auto load_values = [&](int ch) {
+            const float* from = w.vec + ((slot0 + ch) * a.heads + h) * 256;
+            vec = *reinterpret_cast<const f32x4*>(from + 64 * min(wave, 2) + 4 * n);
+            decay = from[192];
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
+                                                                 h * a.v_head + col0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t row = min(r0 + i, seq.n - 1 - ch * kChunk);
+                v[i] = load_cols<NC>(at, row * (2 * static_cast<uint32_t>(a.v_token)) + 2 * NC * n);
+            }
+        };
+        auto put_k = [&](int ch) {
+#pragma unroll
+            for (int i = 0; i < KS * PARTS; ++i) lds.k[wave][i][lane] = k[i / PARTS][i % PARTS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds.v[wave][i][lane] = v[i];
+            if (wave < 3 && g == 0) lds.vec[ch % 2][wave][n] = vec;
+            if (wave == 3) lds.decay[ch % 2] = decay;
+        };
+        auto put_t = [&] {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) lds.t[wave][i][lane] = t[i / 3][i % 3];
+        };
+        if (chunks > 0) {
+            load_rows(k, a.k, a.k_token, a.k_head, w.kf, 0);
+            load_values(0);
+            load_blocks(t, w.t, 0);
+            put_k(0);
+            put_t();
+            // (In the loop's order, so that its waits count the same loads.)
+            __builtin_amdgcn_sched_barrier(0);
+            load_kt(0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_rows(k, a.k, a.k_token, a.k_head, w.kf, min(1, chunks - 1));
+            load_values(min(1, chunks - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            load_blocks(t, w.t, min(1, chunks - 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int next = min(ch + 1, chunks - 1), after = min(ch + 2, chunks - 1);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TPW * 2 * PARTS; ++i) lds.kt[wave][i][lane] = kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS];
+            __builtin_amdgcn_sched_barrier(0);
+            load_kt(next);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            put_k(next);
+            __builtin_amdgcn_sched_barrier(0);
+            load_rows(k, a.k, a.k_token, a.k_head, w.kf, after);
+            load_values(after);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            put_t();
+            __builtin_amdgcn_sched_barrier(0);
+            load_blocks(t, w.t, after);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads_or(0);
+        return;
+    }
     if (role >= 4) {
+        __builtin_amdgcn_s_setprio(1);
         uint4 q[KS][PARTS], p[2][2];
-        f32x4 fq;
         if (chunks > 0) {
             load_rows(q, a.q, a.q_token, a.q_head, w.qf, 0);
             __builtin_amdgcn_sched_barrier(0);
             load_blocks(p, w.p, 0);
-            fq = factors(0, 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
         for (int ch = 0; ch < chunks; ++ch) {
             const int next = min(ch + 1, chunks - 1);
@@ -472,25 +550,27 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
             __builtin_amdgcn_sched_barrier(0);
             load_rows(q, a.q, a.q_token, a.q_head, w.qf, next);
             __builtin_amdgcn_sched_barrier(0);
+            {
+                const f32x4 fq = lds.vec[ch % 2][1][4 * wave + g];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) o[c] *= fq;
+                for (int c = 0; c < NC; ++c) o[c] *= fq;
+            }
             __syncthreads();
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (2 * k > wave) continue;
+            for (int j = 0; j < 2; ++j) {
+                if (2 * j > wave) continue;
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
-                        const uint4 f = lds.u[b][k][c][lane];
+                        const uint4 f = lds.u[b][j][c][lane];
 #pragma unroll
-                        for (int r = 0; r + b < 2; ++r) o[c] = mfma16x16x32(p[k][r], f, o[c]);
+                        for (int r = 0; r + b < 2; ++r) o[c] = mfma16x16x32(p[j][r], f, o[c]);
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
             load_blocks(p, w.p, next);
-            fq = factors(next, 1);
             __builtin_amdgcn_sched_barrier(0);
             const int left = seq.n - ch * kChunk;
             uint16_t* to = a.out + static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.out_token + h * a.out_head + col;
@@ -519,48 +599,18 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
                                                static_cast<int64_t>(row_of(x) + i) * a.value_dim + col + c];
     float* tape_s = reinterpret_cast<float*>(a.tape);
     float* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
-    uint4 k[KS][PARTS], t[2][3], kt[TPW][2][PARTS];
-    uint32_t v[4];
-    f32x4 fk, fu;
-    float decay = 0.0f;
-    auto load_values = [&](int ch) {
-        fk = factors(ch, 0);
-        const uint8_t* at = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
-                                                             h * a.v_head + col0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t row = min(r0 + i, seq.n - 1 - ch * kChunk);
-            v[i] = load_cols<NC>(at, row * (2 * static_cast<uint32_t>(a.v_token)) + 2 * NC * n);
-        }
-    };
-    auto load_rest = [&](int ch) {
-        fu = factors(ch, 2);
-        decay = w.vec[((slot0 + ch) * a.heads + h) * 256 + 192];
-        const uint8_t* at = w.kt + (((slot0 + ch) * a.key_heads + kh) * (D / 16) + wave * TPW) * 2 * PARTS * kFragBytes;
-#pragma unroll
-        for (int i = 0; i < TPW * 2 * PARTS; ++i)
-            kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
-    };
-    if (chunks > 0) {
-        // (In the loop's order, so that its waits count the same loads.)
-        load_rows(k, a.k, a.k_token, a.k_head, w.kf, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_values(0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_blocks(t, w.t, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_rest(0);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_s_setprio(2);
     bool odd = false;   // a number that is not finite
     for (int ch = 0; ch < chunks; ++ch) {
-        const int next = min(ch + 1, chunks - 1);
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 put_parts<3>(lds.s, (wave * TPW + i) / 2, (wave * TPW + i) % 2, c, lane, S[i][c]);
         __syncthreads();
+        uint4 k[KS * PARTS];
+#pragma unroll
+        for (int i = 0; i < KS * PARTS; ++i) k[i] = lds.k[wave][i][lane];
         f32x4 r[NC];
 #pragma unroll
         for (int c = 0; c < NC; ++c) r[c] = zero;
@@ -572,21 +622,20 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
                 for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.s[p][i][c][lane];
 #pragma unroll
-                    for (int x = 0; x < PARTS && x + p < 3; ++x) r[c] = mfma16x16x32(k[i][x], b, r[c]);
+                    for (int x = 0; x < PARTS && x + p < 3; ++x) r[c] = mfma16x16x32(k[i * PARTS + x], b, r[c]);
                 }
-        __builtin_amdgcn_sched_barrier(0);
-        load_rows(k, a.k, a.k_token, a.k_head, w.kf, next);
-        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 fk = lds.vec[ch % 2][0][4 * wave + g], fu = lds.vec[ch % 2][2][4 * wave + g];
+        const float decay = lds.decay[ch % 2];
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lds.v[wave][i][lane];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[c][i] = col_value<FP16>(v[i], c) - fk[i] * r[c][i];
             put_parts<3>(lds.r, wave / 2, wave % 2, c, lane, r[c]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        load_values(next);
         if constexpr (TAPE) {
-            // (Behind the step's loads, whose waits would count the stores.)
             float* to = tape_s + ((slot0 + ch) * a.heads + h) * size + col;
 #pragma unroll
             for (int i = 0; i < TPW; ++i) put_rows<NC>(to + row_of(i) * a.value_dim, a.value_dim, S[i]);
@@ -598,18 +647,18 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (2 * i > wave) continue;
+            uint4 t[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) t[p] = lds.t[wave][3 * i + p][lane];
 #pragma unroll
             for (int p = 0; p < 3; ++p)
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.r[p][i][c][lane];
 #pragma unroll
-                    for (int x = 0; x + p < 3; ++x) u[c] = mfma16x16x32(t[i][x], b, u[c]);
+                    for (int x = 0; x + p < 3; ++x) u[c] = mfma16x16x32(t[x], b, u[c]);
                 }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        load_blocks(t, w.t, next);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
@@ -620,6 +669,9 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
         if constexpr (TAPE)
             put_rows<NC>(tape_u + (((slot0 + ch) * a.heads + h) * kChunk + r0) * a.value_dim + col, a.value_dim, u);
         __syncthreads();
+        uint4 kt[TPW * 2 * PARTS];
+#pragma unroll
+        for (int i = 0; i < TPW * 2 * PARTS; ++i) kt[i] = lds.kt[wave][i][lane];
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
 #pragma unroll
@@ -634,11 +686,8 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks(ScanArgs a, Scan
 #pragma unroll
                     for (int i = 0; i < TPW; ++i)
 #pragma unroll
-                        for (int x = 0; x < PARTS && x + p < 3; ++x) S[i][c] = mfma16x16x32(kt[i][j][x], b, S[i][c]);
+                        for (int x = 0; x < PARTS && x + p < 3; ++x) S[i][c] = mfma16x16x32(kt[(2 * i + j) * PARTS + x], b, S[i][c]);
                 }
-        __builtin_amdgcn_sched_barrier(0);
-        load_rest(next);
-        __builtin_amdgcn_sched_barrier(0);
     }
     // Where a value was not finite, a product's zero weights have let it through
     // to earlier tokens: the next launch goes through these columns again.
@@ -674,7 +723,7 @@ struct ScanGradLds {
 };
 
 template <int D, bool FP16>
-__global__ __launch_bounds__(kChainThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
+__global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArgs a, ScanGradArgs d, ScanChunks w) {
     constexpr int PARTS = FP16 ? 2 : 1, TPW = D / 64, KS = D / 32, NC = 2;
     __shared__ ScanGradLds<D, NC, PARTS> lds;
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
@@ -688,17 +737,17 @@ __global__ __launch_bounds__(kChainThreads, 2) void scan_chunks_grad(ScanArgs a,
         const int head = min(max(a.starts[0], 0), a.tokens), tail = min(max(a.starts[a.seqs], 0), a.tokens);
         auto clear = [&](int from, int to) {
             const int rows = to - from;
-            for (int i = tid; i < rows * 32; i += kChainThreads)
+            for (int i = tid; i < rows * 32; i += kChainGradThreads)
                 d.dv[(static_cast<int64_t>(from + i / 32) * a.heads + h) * a.value_dim + col0 + i % 32] = 0;
             if (item.cb != 0) return;
-            for (int i = tid; i < rows; i += kChainThreads) {
+            for (int i = tid; i < rows; i += kChainGradThreads) {
                 const int64_t at = static_cast<int64_t>(from + i) * a.heads + h;
                 d.dg[at] = 0.0f;
                 if (a.beta_fp32) static_cast<float*>(d.dbeta)[at] = 0.0f;
                 else static_cast<uint16_t*>(d.dbeta)[at] = 0;
             }
             if (h % a.group != 0) return;
-            for (int i = tid; i < rows * D; i += kChainThreads) {
+            for (int i = tid; i < rows * D; i += kChainGradThreads) {
                 const int64_t at = (static_cast<int64_t>(from + i / D) * a.key_heads + kh) * D + i % D;
                 d.dq[at] = 0;
                 d.dk[at] = 0;
@@ -1514,7 +1563,7 @@ void launch_grad(const ScanArgs& a, const ScanGradArgs& d, const ScanChunks& w, 
     const uint32_t chunks = static_cast<uint32_t>(w.slots) * a.key_heads;
     scan_prepare<D, FP16, true><<<chunks, kThreads, 0, stream>>>(a, w);
     const int items = a.seqs * a.heads * (a.value_dim / 32);
-    scan_chunks_grad<D, FP16><<<(items + 7) / 8 * 8, kChainThreads, 0, stream>>>(a, d, w);
+    scan_chunks_grad<D, FP16><<<(items + 7) / 8 * 8, kChainGradThreads, 0, stream>>>(a, d, w);
     scan_inputs_grad<D, FP16><<<chunks, kGradThreads, 0, stream>>>(a, d, w);
 }
 
