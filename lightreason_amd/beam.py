@@ -115,19 +115,16 @@ def fork_rows(parents: torch.Tensor, tensors) -> None:
     if form is None:
         form = _check_rows(parents, tensors)
         _native.remember(_FORKS, key, form)
-    rows, dev, layout = form
+    rows, dev, parts = form
     if rows == 0:
         return
     with _native.on_device(dev):
         stream = _native.current_stream(dev)
-        for i in range(0, len(tensors), _native.FORK_TENSORS):
-            part = tensors[i:i + _native.FORK_TENSORS]
-            table = (C.c_int64 * (3 * len(part)))()
-            for j, t in enumerate(part):
-                table[3 * j] = t.data_ptr()
-                table[3 * j + 1], table[3 * j + 2] = layout[i + j]
-            if any(table[2::3]):
-                _native.call("lrmoe_fork_rows", rows, parents.data_ptr(), len(part), C.addressof(table), stream)
+        for i, table in parts:
+            n = len(table) // 3
+            table = (C.c_int64 * len(table)).from_buffer_copy(table)
+            table[::3] = [t.data_ptr() for t in tensors[i:i + n]]
+            _native.call("lrmoe_fork_rows", rows, parents.data_ptr(), n, C.addressof(table), stream)
 
 
 _FORKS: dict = {}   # as _SELECTS
@@ -152,4 +149,8 @@ def _check_rows(parents, tensors):
         if stride < nbytes:
             raise ValueError(f"tensor {i} has rows that overlap")
         layout.append((stride, nbytes))
-    return rows, dev, layout
+    parts = []   # of up to FORK_TENSORS tensors: the first, and the call's table but for the addresses
+    for i in range(0, len(tensors), _native.FORK_TENSORS):
+        part = layout[i:i + _native.FORK_TENSORS]
+        parts.append((i, (C.c_int64 * (3 * len(part)))(*[x for row in part for x in (0, *row)])))
+    return rows, dev, parts

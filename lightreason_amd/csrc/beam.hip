@@ -14,6 +14,7 @@ constexpr int kSlice = 2048;          // logits that a wave takes
 constexpr int kPer = kSlice / kWave;  // and a lane
 constexpr int kThreads = 256;
 constexpr int kJoinThreads = 512;
+constexpr int kKeep = 10;
 
 // A finite value and its token as one key: the larger value first, then the
 // lower token.  0 stands for no candidate.
@@ -34,6 +35,11 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     const uint32_t lo = wave_max_u32(static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
+// Orders a wave's LDS accesses (it runs in step).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 template <int TYPE>
@@ -47,6 +53,18 @@ __device__ __forceinline__ float load_logit(const void* row, int64_t i) {
 // score that is not finite).
 __device__ __forceinline__ bool beam_open(const BeamArgs& a, int row) {
     return finite_bits(a.scores[row]) && (a.finished == nullptr || a.finished[row] == 0);
+}
+
+// A list that a wave has gathered: at most kWave keys, of which it keeps the W
+// best, best first (lane r the r-th): a key's place is the number of larger ones.
+constexpr int kGather = kWave;
+__device__ __forceinline__ uint64_t gathered_best(const uint64_t* list, uint64_t* best, int n, int W, int lane) {
+    const uint64_t key = lane < n ? list[lane] : 0;
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += list[i] > key;
+    if (lane < n && place < W) best[place] = key;
+    wave_sync();
+    return lane < min(n, W) ? best[lane] : 0;
 }
 
 // The W best of a wave's keys, best first, as each lane's own calls to
@@ -64,11 +82,17 @@ __device__ __forceinline__ uint64_t wave_best(int W, int lane, Each&& each) {
     return mine;
 }
 
+// A wave takes 2048 logits of a row in registers: their maximum and sum of
+// exponentials, and the W best. Those are no smaller than the W-th largest of the
+// lanes' maxima, so that only what reaches it is gathered and ranked, W numbers
+// and a few more; where equal values make them more than a list holds, the
+// registers are gone through W times instead.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void beam_slices(BeamArgs a) {
-    const int lane = threadIdx.x % kWave;
+    __shared__ uint64_t lists[kThreads / kWave][kGather], bests[kThreads / kWave][kBeamMax];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int slices = (a.vocab + kSlice - 1) / kSlice;
-    const int slice = blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave;
+    const int slice = blockIdx.x * (kThreads / kWave) + wave;
     const int row = blockIdx.y;
     if (slice >= slices || !beam_open(a, row)) return;
     constexpr int SIZE = TYPE == 0 ? 4 : 2, VEC = 16 / SIZE;
@@ -76,42 +100,78 @@ __global__ __launch_bounds__(kThreads) void beam_slices(BeamArgs a) {
     const bool aligned = reinterpret_cast<uintptr_t>(base) % 16 == 0;
     const int first = slice * kSlice;
     float x[kPer];
+    if (aligned && first + kSlice <= a.vocab) {
+        uint4 raw[kPer / VEC];
 #pragma unroll
-    for (int i = 0; i < kPer / VEC; ++i) {
-        const int at = first + (i * kWave + lane) * VEC;
-        if (aligned && at + VEC <= a.vocab) {
-            const uint4 w = ldg16_nt(static_cast<const uint8_t*>(base) + static_cast<int64_t>(at) * SIZE);
+        for (int i = 0; i < kPer / VEC; ++i)
+            raw[i] = ldg16_nt(static_cast<const uint8_t*>(base) + static_cast<int64_t>(first + (i * kWave + lane) * VEC) * SIZE);
+#pragma unroll
+        for (int i = 0; i < kPer / VEC; ++i) {
             if constexpr (TYPE == 0) {
-                x[VEC * i] = __uint_as_float(w.x), x[VEC * i + 1] = __uint_as_float(w.y);
-                x[VEC * i + 2] = __uint_as_float(w.z), x[VEC * i + 3] = __uint_as_float(w.w);
+                x[VEC * i] = __uint_as_float(raw[i].x), x[VEC * i + 1] = __uint_as_float(raw[i].y);
+                x[VEC * i + 2] = __uint_as_float(raw[i].z), x[VEC * i + 3] = __uint_as_float(raw[i].w);
             } else {
-                unpack16<TYPE == 2>(w, x + VEC * i);
+                unpack16<TYPE == 2>(raw[i], x + VEC * i);
             }
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                x[VEC * i + j] = at + j < a.vocab ? load_logit<TYPE>(base, at + j) : -__builtin_inff();
+        for (int i = 0; i < kPer; ++i) {
+            const int at = first + (i / VEC * kWave + lane) * VEC + i % VEC;
+            x[i] = at < a.vocab ? load_logit<TYPE>(base, at) : -__builtin_inff();
         }
     }
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        x[i] = finite_bits(x[i]) ? x[i] : -__builtin_inff();
+        x[i] = finite_bits(x[i]) ? x[i] + 0.0f : -__builtin_inff();   // (-0 becomes +0)
         top = __builtin_fmaxf(top, x[i]);
     }
-    const uint64_t wave_top = wave_max_u64(finite_bits(top) ? beam_key(top, 0) : 0);
-    const float m = wave_top ? beam_value(wave_top) : 0.0f;
+    // The lanes' maxima, largest first, until W of them: the border.
+    uint32_t left = finite_bits(top) ? static_cast<uint32_t>(beam_key(top, 0) >> 32) : 0u;
+    uint32_t border = 0;
+    float m = 0.0f;
+    bool some = false;
+    for (int r = 0; r < a.beams; ++r) {
+        border = wave_max_u32(left);
+        if (r == 0) {
+            some = border != 0;
+            m = some ? beam_value(static_cast<uint64_t>(border) << 32) : 0.0f;
+        }
+        if (border == 0) break;
+        const uint64_t with = __ballot(left == border);
+        if (lane == __builtin_ctzll(with)) left = 0;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((x[i] - m) * 1.4426950408889634f);
     sum = wave_butterfly_sum(sum);
     const int64_t at = static_cast<int64_t>(row) * slices + slice;
-    if (lane == 0) a.sums[at] = make_float2(m, wave_top ? sum : 0.0f);
-    const uint64_t best = wave_best(a.beams, lane, [&](auto&& f) {
+    if (lane == 0) a.sums[at] = make_float2(m, some ? sum : 0.0f);
+    // (No border: fewer than W lanes have any.)
+    const float least = border ? beam_value(static_cast<uint64_t>(border) << 32) : -__builtin_inff();
+    int n = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (finite_bits(x[i])) f(beam_key(x[i], first + (i / VEC * kWave + lane) * VEC + i % VEC));
-    });
+    for (int i = 0; i < kPer; ++i) {
+        const bool in = x[i] >= least && finite_bits(x[i]);
+        const uint64_t with = __ballot(in);
+        if (with == 0) continue;
+        const int place = n + __popcll(with & ((UINT64_C(1) << lane) - 1));
+        if (in && place < kGather)
+            lists[wave][place] = beam_key(x[i], first + (i / VEC * kWave + lane) * VEC + i % VEC);
+        n += __popcll(with);
+    }
+    uint64_t best;
+    if (n <= kGather) {
+        wave_sync();
+        best = gathered_best(lists[wave], bests[wave], n, a.beams, lane);
+    } else {
+        best = wave_best(a.beams, lane, [&](auto&& f) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (finite_bits(x[i])) f(beam_key(x[i], first + (i / VEC * kWave + lane) * VEC + i % VEC));
+        });
+    }
     if (lane < a.beams)
         a.best[at * a.beams + lane] = make_uint2(static_cast<uint32_t>(best), static_cast<uint32_t>(best >> 32));
 }
@@ -138,19 +198,36 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(BeamArgs a) {
             continue;
         }
         const float2* sums = a.sums + static_cast<int64_t>(row) * slices;
+        const uint2* best = a.best + static_cast<int64_t>(row) * slices * W;
+        const int n = slices * W;
+        // Up to kKeep candidates a lane stay in registers.
+        uint64_t keys[kKeep];
+        const bool fits = n <= kKeep * kWave;
+        if (fits) {
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i) {
+                const int at = i * kWave + lane;
+                const uint2 x = best[min(at, n - 1)];
+                keys[i] = at < n ? (static_cast<uint64_t>(x.y) << 32) | x.x : 0;
+            }
+        }
         float m = -__builtin_inff();
         for (int i = lane; i < slices; i += kWave) m = sums[i].y > 0.0f ? __builtin_fmaxf(m, sums[i].x) : m;
         const uint64_t top = wave_max_u64(finite_bits(m) ? beam_key(m, 0) : 0);
         m = top ? beam_value(top) : 0.0f;
         double sum = 0.0;
         for (int i = lane; i < slices; i += kWave)
-            if (sums[i].y > 0.0f) sum += static_cast<double>(sums[i].y) * exp(static_cast<double>(sums[i].x) - m);
+            if (sums[i].y > 0.0f)
+                sum += static_cast<double>(sums[i].y) * __builtin_amdgcn_exp2f((sums[i].x - m) * 1.4426950408889634f);
 #pragma unroll
         for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off);
-        const uint2* best = a.best + static_cast<int64_t>(row) * slices * W;
         const uint64_t key = wave_best(W, lane, [&](auto&& f) {
-            for (int i = lane; i < slices * W; i += kWave)
-                f((static_cast<uint64_t>(best[i].y) << 32) | best[i].x);
+            if (fits) {
+#pragma unroll
+                for (int i = 0; i < kKeep; ++i) f(keys[i]);
+            } else {
+                for (int i = lane; i < n; i += kWave) f((static_cast<uint64_t>(best[i].y) << 32) | best[i].x);
+            }
         });
         if (lane < W) {
             score[w * W + lane] =
@@ -218,7 +295,15 @@ __device__ __forceinline__ void fork_copy(uint8_t* to, const uint8_t* from, int6
     T* d = reinterpret_cast<T*>(to);
     const T* s = reinterpret_cast<const T*>(from);
     const int n = static_cast<int>(bytes / sizeof(T));
-    for (int i = threadIdx.x; i < n; i += kThreads) d[i] = s[i];
+    int i = threadIdx.x;
+    for (; i + 3 * kThreads < n; i += 4 * kThreads) {
+        T v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = s[i + j * kThreads];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[i + j * kThreads] = v[j];
+    }
+    for (; i < n; i += kThreads) d[i] = s[i];
 }
 
 // A workgroup copies a piece of a row.  Rows that are read keep their places

@@ -95,14 +95,15 @@ struct ForkCache {
     int layers, heads, row_bytes, pad;
 };
 struct PageForkArgs {
-    int rows, pages, page_shift, max_pages, pieces;   // pieces: layers times heads of all caches
+    int rows, pages, page_shift, max_pages;
+    int pieces, share;   // layers times heads of all caches; those that a workgroup takes
     const int32_t* parents;
     int32_t *table, *lengths, *held;
     const int32_t* free_pages;
     int32_t *state, *before;
     ForkCache cache[LRMOE_FORK_CACHES];
 };
-hipError_t launch_page_fork(const PageForkArgs& a, hipStream_t stream);
+hipError_t launch_page_fork(PageForkArgs a, hipStream_t stream);
 
 struct PagedAppendArgs {
     int tokens, heads, kv_heads, rotary, pages, page_shift, rope_rows, rope_fp32;

@@ -15,6 +15,8 @@
 // Commit and release run in one workgroup: a plan with its commit takes 4.4 us
 // for 4 rows, 8 for 1000 and 29 for 4096; a release 2.4 us for 268 pages, 11
 // for 4288, 218 for 67,000 (a page per thread at a time; rows end seldom).
+#include <algorithm>
+
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
@@ -335,20 +337,17 @@ __global__ __launch_bounds__(kThreads) void page_fork_kernel(PageForkArgs a) {
     }
 }
 
-// The pages' contents, a page of one head of one layer per workgroup at a
-// time.  Pages that are read belong to rows that keep theirs, so none is
-// written.  Bound by HBM.
+// The pages' contents: a workgroup has a page and some of its pieces (a head of
+// a layer), at least kForkBytes in all, and a wave copies a piece at a time.
+// Pages that are read belong to rows that keep theirs, so none is written.
+// Bound by HBM.
+constexpr int kForkBytes = 65536;
 __global__ __launch_bounds__(kThreads) void page_fork_copy(PageForkArgs a) {
-    const int total = a.before[a.rows];
-    const int64_t work = static_cast<int64_t>(total) * a.pieces;
+    const int total = a.before[a.rows], lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int parts = (a.pieces + a.share - 1) / a.share;
+    const int64_t work = static_cast<int64_t>(total) * parts;
     for (int64_t i = blockIdx.x; i < work; i += gridDim.x) {
-        const int unit = static_cast<int>(i / a.pieces);
-        int piece = static_cast<int>(i - static_cast<int64_t>(unit) * a.pieces), c = 0;
-        while (piece >= a.cache[c].layers * a.cache[c].heads) {
-            piece -= a.cache[c].layers * a.cache[c].heads;
-            ++c;
-        }
-        const ForkCache& cache = a.cache[c];
+        const int unit = static_cast<int>(i / parts), first = static_cast<int>(i - static_cast<int64_t>(unit) * parts) * a.share;
         // (Rows without pages to copy share their place with the next: the last
         // of those is meant.)
         const int r = last_at_most(a.before, a.rows, unit), j = unit - a.before[r], p = a.parents[r];
@@ -356,13 +355,35 @@ __global__ __launch_bounds__(kThreads) void page_fork_copy(PageForkArgs a) {
         const int from = a.table[static_cast<int64_t>(p) * a.max_pages + j];
         if (to < 0 || to >= a.pages || from < 0 || from >= a.pages) continue;
         const int rows = min(a.lengths[r] - (j << a.page_shift), 1 << a.page_shift);
-        uint8_t* base = cache.base + piece / cache.heads * cache.layer_stride + piece % cache.heads * cache.head_stride;
-        uint8_t* d = base + to * cache.page_stride;
-        const uint8_t* s = base + from * cache.page_stride;
-        const int lanes = cache.row_bytes / 16;
-        for (int x = threadIdx.x; x < rows * lanes; x += kThreads) {
-            const int64_t at = x / lanes * cache.row_stride + x % lanes * 16;
-            *reinterpret_cast<u32x4*>(d + at) = *reinterpret_cast<const u32x4*>(s + at);
+        for (int k = first + wave; k < min(first + a.share, a.pieces); k += kThreads / kWave) {
+            int piece = k, c = 0;
+            while (piece >= a.cache[c].layers * a.cache[c].heads) {
+                piece -= a.cache[c].layers * a.cache[c].heads;
+                ++c;
+            }
+            const ForkCache& cache = a.cache[c];
+            uint8_t* base = cache.base + piece / cache.heads * cache.layer_stride + piece % cache.heads * cache.head_stride;
+            uint8_t* d = base + to * cache.page_stride;
+            const uint8_t* s = base + from * cache.page_stride;
+            const int lanes = cache.row_bytes / 16, n = rows * lanes;
+            if (cache.row_stride == cache.row_bytes) {
+                u32x4* dst = reinterpret_cast<u32x4*>(d);
+                const u32x4* src = reinterpret_cast<const u32x4*>(s);
+                int x = lane;
+                for (; x + 7 * kWave < n; x += 8 * kWave) {
+                    u32x4 v[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) v[y] = __builtin_nontemporal_load(src + x + y * kWave);
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) __builtin_nontemporal_store(v[y], dst + x + y * kWave);
+                }
+                for (; x < n; x += kWave) dst[x] = src[x];
+            } else {
+                for (int x = lane; x < n; x += kWave) {
+                    const int64_t at = x / lanes * cache.row_stride + x % lanes * 16;
+                    *reinterpret_cast<u32x4*>(d + at) = *reinterpret_cast<const u32x4*>(s + at);
+                }
+            }
         }
     }
 }
@@ -484,7 +505,12 @@ hipError_t launch_page_commit(const PageCommitArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-hipError_t launch_page_fork(const PageForkArgs& a, hipStream_t stream) {
+hipError_t launch_page_fork(PageForkArgs a, hipStream_t stream) {
+    int64_t bytes = 0;   // of a page in all caches
+    for (int c = 0; c < LRMOE_FORK_CACHES; ++c)
+        bytes += static_cast<int64_t>(a.cache[c].layers) * a.cache[c].heads * a.cache[c].row_bytes << a.page_shift;
+    const int64_t parts = std::max(bytes / kForkBytes, INT64_C(1));
+    a.share = static_cast<int>(std::max((a.pieces + parts - 1) / parts, INT64_C(1)));
     page_fork_kernel<<<1, kThreads, 0, stream>>>(a);
     if (a.pieces > 0) page_fork_copy<<<2048, kThreads, 0, stream>>>(a);
     return hipGetLastError();

@@ -99,9 +99,12 @@ def _addresses(a, query, key, value, g, beta, starts):
     a.starts = starts.data_ptr()
 
 
-def _launch(a, dev):
+def _scratch(a) -> int:
+    return int(_native.library().lrmoe_delta_scan_workspace_bytes(C.addressof(a)))
+
+
+def _launch(a, dev, nbytes):
     with _on(dev):
-        nbytes = int(_native.library().lrmoe_delta_scan_workspace_bytes(C.addressof(a)))
         ws = _native.workspace(dev, nbytes)
         _native.call("lrmoe_delta_scan", C.addressof(a), ws.data_ptr(), ws.numel(), _stream(dev))
 
@@ -172,7 +175,7 @@ def _scan(form, tensors, taped=False):
         nbytes = int(_native.library().lrmoe_delta_scan_tape_bytes(C.addressof(a)))
         tape = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         a.tape = tape.data_ptr()
-    _launch(a, dev)
+    _launch(a, dev, _scratch(a))
     return out, final, tape
 
 
@@ -247,7 +250,7 @@ def delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     if form is None:
         form = _check_step(*tensors, normalize, scale, max_new)
         _native.remember(_STEPS, key_, form)
-    template, dev = form
+    template, dev, nbytes = form
     if out is None:
         out = torch.empty(value.shape, dtype=value.dtype, device=dev)
     if template.seqs == 0:
@@ -258,7 +261,7 @@ def delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     a.slots, a.into, a.fresh = _ptr(slots), _ptr(slots if into is None else into), _ptr(fresh)
     if a.tokens:
         a.out = out.data_ptr()
-    _launch(a, dev)
+    _launch(a, dev, nbytes)
     return out
 
 
@@ -286,4 +289,4 @@ def _check_step(query, key, value, g, beta, starts, states, slots, into, fresh, 
         a.out_token_stride, a.out_head_stride = _strides(out)
     else:
         a.out_token_stride, a.out_head_stride = a.heads * a.value_dim, a.value_dim
-    return a, dev
+    return a, dev, _scratch(a)
