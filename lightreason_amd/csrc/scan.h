@@ -11,6 +11,7 @@ namespace lrmoe {
 struct ScanArgs {
     int seqs, tokens, heads, key_heads, group, dim, value_dim, pool;
     int normalize, beta_fp32, clear;
+    int token_wise;   // sequences of up to so many tokens go token by token
     float scale;
     const uint16_t *q, *k, *v;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;   // strides in elements
@@ -35,7 +36,7 @@ struct ScanGradArgs {
     void* dbeta;
     float* d_initial;
 };
-hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int max_new, void* workspace, hipStream_t stream);
+hipError_t launch_delta_scan(ScanArgs a, bool fp16, int max_new, void* workspace, hipStream_t stream);
 size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new);
 
 size_t delta_scan_tape_bytes(const ScanArgs& a);

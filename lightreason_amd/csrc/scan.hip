@@ -37,9 +37,9 @@ __device__ __forceinline__ void recur_load(const ScanArgs& a, RecurToken<D, FP16
                          : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[t * a.beta_token + h]);
 }
 
-//
-// With flags given only the blocks of columns that they mark are computed: those
-// in which the chunked form met a number that is not finite.
+// With flags given the chunked form has run: what is left are short sequences and
+// the blocks of columns that the flags mark, in which it met a number that is not
+// finite.
 template <int D, bool FP16>
 __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* flags) {
     constexpr int ROWS = D / 8;
@@ -47,17 +47,17 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* fl
     const int blocks = a.value_dim / 32;
     const int64_t wave = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / kWave;
     if (wave >= static_cast<int64_t>(a.seqs) * a.heads * blocks) return;
-    uint32_t marks[2] = {1u, 1u};   // of the wave's first and last 16 columns
-    if (flags != nullptr) {
-        marks[0] = flags[2 * wave], marks[1] = flags[2 * wave + 1];
-        if ((marks[0] | marks[1]) == 0) return;
-    }
     const int cb = static_cast<int>(wave % blocks);
     const int h = static_cast<int>(wave / blocks % a.heads), s = static_cast<int>(wave / blocks / a.heads);
     const int kh = h / a.group;
     const int rows0 = ROWS * (lane / 8), col = 32 * cb + 4 * (lane % 8);
-    const bool marked = marks[lane % 8 / 4] != 0;
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
+    bool marked = true;
+    if (flags != nullptr && seq.n > a.token_wise) {
+        const uint32_t first = flags[2 * wave], last = flags[2 * wave + 1];   // of 16 columns each
+        if ((first | last) == 0) return;
+        marked = (lane % 8 < 4 ? first : last) != 0;
+    }
     // Rows of no sequence.
     if (a.clear && flags == nullptr && (s == 0 || s == a.seqs - 1)) {
         const int64_t row0 = h * a.out_head + col;
@@ -146,17 +146,25 @@ __global__ __launch_bounds__(256) void scan_recur(ScanArgs a, const uint32_t* fl
 
 }  // namespace
 
-// Single tokens and short blocks go token by token: the state is read and
-// written once, whatever the form.  (The tape is the chunked form's.)
-static bool token_by_token(const ScanArgs& a, int max_new) { return max_new <= 16 && a.tape == nullptr; }
-
-size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
-    return token_by_token(a, max_new) ? 256 : scan_chunk_bytes(a, fp16);
+// Tokens up to which a sequence goes token by token: about what the chunked
+// form's launches and its chunk of 64 cost. Measured at 20 to 26 tokens where the
+// waves are few (1 sequence of 32 heads and 128 columns: 16 tokens 20 us against
+// 20, 32 tokens 37 against 23) and 35 to 55 where they fill the card (64 of
+// them: 32 tokens 226 against 324, 48 tokens 325 against 340). Sequences of one
+// call may go either way. (The tape is the chunked form's.)
+static int token_wise(const ScanArgs& a) {
+    if (a.tape != nullptr) return 0;
+    return static_cast<int64_t>(a.seqs) * a.heads * (a.value_dim / 32) <= 1024 ? 24 : 40;
 }
 
-hipError_t launch_delta_scan(const ScanArgs& a, bool fp16, int max_new, void* workspace, hipStream_t stream) {
+size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
+    return max_new <= token_wise(a) ? 256 : scan_chunk_bytes(a, fp16);
+}
+
+hipError_t launch_delta_scan(ScanArgs a, bool fp16, int max_new, void* workspace, hipStream_t stream) {
     const uint32_t* flags = nullptr;
-    if (!token_by_token(a, max_new)) {
+    a.token_wise = token_wise(a);
+    if (max_new > a.token_wise) {
         const hipError_t err = launch_scan_chunks(a, fp16, workspace, &flags, stream);
         if (err != hipSuccess) return err;
     }

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
     const int s = find_sequence(a.starts, a.seqs, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
     const int first = (slot - scan_first_chunk(a.starts, s)) * kChunk;
-    if (first < 0 || first >= seq.n) return;
+    if (first < 0 || first >= seq.n || seq.n <= a.token_wise) return;
     const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
     uint16_t* raw_k = reinterpret_cast<uint16_t*>(lds.a);
     uint16_t* raw_q = reinterpret_cast<uint16_t*>(lds.b);
@@ -438,6 +438,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             for (int i = tid; i < (a.tokens - tail) * 16 * NC; i += kChainThreads)
                 row[(tail + i / (16 * NC)) * a.out_token + i % (16 * NC)] = 0;
     }
+    if (seq.n <= a.token_wise) return;   // (the next launch's)
     uint32_t* flag = w.flags + (static_cast<int64_t>(s) * a.heads + h) * (a.value_dim / 16) + NC * item.cb;
     const int into = scan_slot(a.into, s, a.pool);
     const bool fresh = a.initial == nullptr || (a.fresh != nullptr && a.fresh[s] != 0);

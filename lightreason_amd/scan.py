@@ -8,6 +8,10 @@ sequences: prompts, training, and the steps of a server.
   positions and verify blocks over a pool of states in HBM, as
   ``paged.paged_attention`` serves the full-attention layers of the same step
   (its ``starts`` are a ``paged.PagePlan``'s).
+* ``fused_scan(model)`` -- a context manager under which every linear-attention
+  layer of a Transformers model runs its prompts and its training through
+  ``delta_scan``; inside ``delta.fused_delta`` the steps after a prompt are
+  native too.
 
 ``delta.delta_rule`` and ``delta.DeltaMixer`` serve one sequence of 1..16 tokens
 with the rounding points of the Transformers forward (edge35b/
@@ -22,6 +26,8 @@ graph.  There is no CPU path: the calls raise when liblrmoe.so is missing.
 from __future__ import annotations
 
 import ctypes as C
+import sys
+from contextlib import contextmanager
 
 import torch
 
@@ -290,3 +296,48 @@ def _check_step(query, key, value, g, beta, starts, states, slots, into, fresh, 
     else:
         a.out_token_stride, a.out_head_stride = a.heads * a.value_dim, a.value_dim
     return a, dev, _scratch(a)
+
+
+# ---- under a Transformers model -------------------------------------------------
+
+@contextmanager
+def fused_scan(model):
+    """Run the recurrence of every linear-attention layer's prompt and training
+    forward as one ``delta_scan`` call for the duration of the block, gradients
+    included: what the layers hand to ``torch_chunk_gated_delta_rule`` of their
+    Transformers module, any batch and any length.  (The function is the
+    module's, so other models of the class run through it meanwhile.)  Tensors
+    on the CPU or of another type than bf16 and fp16, and calls with
+    ``cu_seqlens``, run as before."""
+    name = "torch_chunk_gated_delta_rule"
+    def native(original):
+        def rule(query, key, value, g, beta, chunk_size=64, initial_state=None, output_final_state=False,
+                 use_qk_l2norm_in_kernel=False, **kwargs):
+            if query.device.type != "cuda" or query.dtype not in _TYPES or kwargs.get("cu_seqlens") is not None:
+                return original(query, key, value, g=g, beta=beta, chunk_size=chunk_size, initial_state=initial_state,
+                                output_final_state=output_final_state, use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel,
+                                **kwargs)
+            batch, tokens = query.shape[:2]
+            starts = torch.arange(batch + 1, dtype=torch.int32, device=query.device) * tokens
+            rows = [x.reshape(batch * tokens, *x.shape[2:]) for x in (query, key, value, g.float(), beta)]
+            first = None if initial_state is None else initial_state.float().contiguous()
+            out, final = delta_scan(*(x if x.stride(-1) == 1 else x.contiguous() for x in rows), starts, initial=first,
+                                    normalize=use_qk_l2norm_in_kernel)
+            return out.view(batch, tokens, *out.shape[1:]), final if output_final_state else None
+
+        rule.lrmoe_native = True
+        return rule
+
+    mixers = [getattr(layer, "linear_attn", None) for layer in model.model.layers]
+    modules = [sys.modules[m] for m in sorted({type(x).__module__ for x in mixers if x is not None})]
+    for module in modules:
+        if not hasattr(module, name):
+            raise ValueError(f"{module.__name__} has no {name}")
+    restore = [(module, getattr(module, name)) for module in modules]
+    try:
+        for module, original in restore:
+            setattr(module, name, native(original))
+        yield
+    finally:
+        for module, original in restore:
+            setattr(module, name, original)
