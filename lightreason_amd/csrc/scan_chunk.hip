@@ -55,6 +55,12 @@ __device__ __forceinline__ int opaque(int v) {
 
 __device__ __forceinline__ uint4 frag16(const uint8_t* p, uint32_t at) { return *reinterpret_cast<const uint4*>(p + at); }
 
+// Orders a wave's LDS accesses (it runs in step).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float power(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x)); }
 
 __device__ __forceinline__ double wave_scan_f64(double v) {
@@ -69,11 +75,10 @@ __device__ __forceinline__ double wave_scan_f64(double v) {
 // ---- launch one: what does not depend on the state ------------------------------
 
 struct PrepareLds {
-    float a[kChunk * kPitch];   // K rows, then I + L beta
-    float b[kChunk * kPitch];   // Q rows, then P
-    float t[kChunk * kPitch];   // the inverse
-    double sum[kChunk];
-    float beta[kChunk], rk[kChunk], rq[kChunk];
+    float a[kChunk * kPitch];   // K rows, then L beta, then P
+    float t[kChunk * kPitch];   // Q rows, then the inverse
+    double sum[4][kChunk];      // of four heads at a time
+    float beta[4][kChunk], rk[kChunk], rq[kChunk];
 };
 
 // The value of lane L of a lane's row of 16.
@@ -127,8 +132,7 @@ __device__ __forceinline__ void invert(PrepareLds& lds, int wave, int lane) {
         for (int s = 0; s < 4; ++s) out = __builtin_amdgcn_mfma_f32_16x16x4f32(row[s], acc[s], out, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds.t[(16 * i + 4 * g + r) * kPitch + 16 * j + n] = -out[r];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
     __syncthreads();
 }
@@ -146,7 +150,7 @@ __device__ __forceinline__ void store_parts(uint8_t* to, const float (&x)[8]) {
 }
 
 template <int D, bool FP16, bool GRAD>
-__global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChunks w) {
+__global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChunks w) {
     constexpr int RAW = D + 8;   // 16-bit elements of a row in LDS
     constexpr int PARTS = FP16 ? 2 : 1;
     __shared__ PrepareLds lds;
@@ -158,8 +162,19 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
     const int first = (slot - scan_first_chunk(a.starts, s)) * kChunk;
     if (first < 0 || first >= seq.n || seq.n <= a.token_wise) return;
     const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
+    // g and beta of the wave's head among four.
+    float raw_g;
+    uint32_t raw_beta;
+    auto load_gates = [&](int hv) {
+        const int h = kh * a.group + min(hv + wave, a.group - 1);
+        const int64_t t = t0 + min(lane, count - 1);
+        raw_g = a.g[t * a.g_token + h];
+        if (a.beta_fp32) raw_beta = static_cast<const uint32_t*>(a.beta)[t * a.beta_token + h];
+        else raw_beta = static_cast<const uint16_t*>(a.beta)[t * a.beta_token + h];
+    };
+    load_gates(0);
     uint16_t* raw_k = reinterpret_cast<uint16_t*>(lds.a);
-    uint16_t* raw_q = reinterpret_cast<uint16_t*>(lds.b);
+    uint16_t* raw_q = reinterpret_cast<uint16_t*>(lds.t);
     for (int i = tid; i < kChunk * D / 8; i += kThreads) {
         const int r = i / (D / 8), e = i % (D / 8) * 8;
         uint4 k = make_uint4(0u, 0u, 0u, 0u), q = k;
@@ -239,29 +254,30 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
         const int h = kh * a.group + hv;
         const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h;
         __syncthreads();   // (rows and the last head's matrices are done with)
-        if (wave == 0) {
-            float gl = 0.0f, b = 0.0f;
-            if (lane < count) {
-                const int64_t t = t0 + lane;
-                gl = scan_log(a.g[t * a.g_token + h]);
-                b = a.beta_fp32 ? static_cast<const float*>(a.beta)[t * a.beta_token + h]
-                                : elem16<FP16>(static_cast<const uint16_t*>(a.beta)[t * a.beta_token + h]);
-            }
-            // (In powers of two.)
-            const double sum = wave_scan_f64(gl * 1.4426950408889634);
-            lds.sum[lane] = sum;
-            lds.beta[lane] = lane < count ? scan_beta(b) : 0.0f;
-            if constexpr (GRAD) w.sums[by_head * kChunk + lane] = sum;
-            const double last = __shfl(sum, kWave - 1);
-            const float decay = power(sum), rest = power(last - sum);
-            float* vec = w.vec + by_head * 256;
+        if (hv % 4 == 0) {
+            // Running sums (in powers of two) and factors of the next four heads, a
+            // wave each.
+            const float beta = a.beta_fp32 ? __uint_as_float(raw_beta) : elem16<FP16>(static_cast<uint16_t>(raw_beta));
             const bool in = lane < count;   // (rows past the sequence repeat its last one)
-            vec[lane] = in ? decay * lds.rk[lane] : 0.0f;
-            vec[64 + lane] = in ? decay * lds.rq[lane] * a.scale : 0.0f;
-            vec[128 + lane] = in ? rest * lds.rk[lane] : 0.0f;
-            if (lane == kWave - 1) vec[192] = decay;
+            const double sum = wave_scan_f64(in ? scan_log(raw_g) * 1.4426950408889634 : 0.0);
+            lds.sum[wave][lane] = sum;
+            lds.beta[wave][lane] = in ? scan_beta(beta) : 0.0f;
+            if (hv + wave < a.group) {
+                if constexpr (GRAD) w.sums[(by_head + wave) * kChunk + lane] = sum;
+                const double last = __shfl(sum, kWave - 1);
+                const float decay = power(sum), rest = power(last - sum);
+                float* vec = w.vec + (by_head + wave) * 256;
+                vec[lane] = in ? decay * lds.rk[lane] : 0.0f;
+                vec[64 + lane] = in ? decay * lds.rq[lane] * a.scale : 0.0f;
+                vec[128 + lane] = in ? rest * lds.rk[lane] : 0.0f;
+                if (lane == kWave - 1) vec[192] = decay;
+            }
+            load_gates(hv + 4);
+            __syncthreads();
         }
-        __syncthreads();
+        const double* sums = lds.sum[hv % 4];
+        const float* betas = lds.beta[hv % 4];
+        float fade[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if (t > wave) continue;
@@ -269,49 +285,52 @@ __global__ __launch_bounds__(kThreads, 3) void scan_prepare(ScanArgs a, ScanChun
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * wave + 4 * g + r;
-                const float fade = power(lds.sum[i] - lds.sum[j]) * lds.rk[j];
-                lds.a[i * kPitch + j] = j < i ? fade * lds.rk[i] * lds.beta[j] * kk[t][r] : 0.0f;
-                lds.b[i * kPitch + j] = j <= i ? fade * lds.rq[i] * a.scale * qk[t][r] : 0.0f;
+                fade[t][r] = power(sums[i] - sums[j]) * lds.rk[j];
+                lds.a[i * kPitch + j] = j < i ? fade[t][r] * lds.rk[i] * betas[j] * kk[t][r] : 0.0f;
             }
         }
         __syncthreads();
         invert(lds, wave, lane);
+        // A fragment of the wave's rows (for the gradient: of its columns) is eight
+        // numbers of a lane.
         const int row = 16 * wave + n;
-        if constexpr (GRAD) {
+        auto eight = [&](const float* m, int ks, float (&x)[8], auto&& factor) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (2 * ks + 1 < wave) continue;
-                float x[8], y[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int i = 32 * ks + 16 * (j / 4) + 4 * g + j % 4;
-                    const bool in = 2 * ks + j / 4 >= wave;
-                    x[j] = in ? lds.beta[i] * lds.t[i * kPitch + row] : 0.0f;
-                    y[j] = in ? lds.b[i * kPitch + row] : 0.0f;
-                }
-                const int64_t block = by_head * kBlocks + upper_block(ks, wave);
-                store_parts<3>(w.t + block * 3 * kFragBytes + lane * 16, x);
-                store_parts<3>(w.p + block * 3 * kFragBytes + lane * 16, y);
+            for (int j = 0; j < 8; ++j) {
+                const int o = 32 * ks + 16 * (j / 4) + 4 * g + j % 4, block = 2 * ks + j / 4;
+                const bool in = GRAD ? block >= wave : block <= wave;
+                x[j] = in ? m[GRAD ? o * kPitch + row : row * kPitch + o] * factor(GRAD ? o : row) : 0.0f;
             }
-            continue;
-        }
-        const float b = lds.beta[row];
+        };
+        const int64_t blocks = by_head * kBlocks;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if (2 * ks > wave) continue;
-            float x[8], y[8];
-            const int at = row * kPitch + 32 * ks + 4 * g;
-            const bool half = 2 * ks + 1 <= wave;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j] = b * lds.t[at + j];
-                x[4 + j] = half ? b * lds.t[at + 16 + j] : 0.0f;
-                y[j] = lds.b[at + j];
-                y[4 + j] = half ? lds.b[at + 16 + j] : 0.0f;
-            }
-            const int64_t block = by_head * kBlocks + lower_block(ks, wave);
+            if (GRAD ? 2 * ks + 1 < wave : 2 * ks > wave) continue;
+            float x[8];
+            eight(lds.t, ks, x, [&](int i) { return betas[i]; });
+            const int64_t block = blocks + (GRAD ? upper_block(ks, wave) : lower_block(ks, wave));
             store_parts<3>(w.t + block * 3 * kFragBytes + lane * 16, x);
-            store_parts<2>(w.p + block * 2 * kFragBytes + lane * 16, y);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (t > wave) continue;
+            const int j = 16 * t + n;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * wave + 4 * g + r;
+                lds.a[i * kPitch + j] = j <= i ? fade[t][r] * lds.rq[i] * a.scale * qk[t][r] : 0.0f;
+            }
+        }
+        if constexpr (GRAD) __syncthreads();   // (else a wave reads its own rows)
+        else wave_sync();
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (GRAD ? 2 * ks + 1 < wave : 2 * ks > wave) continue;
+            constexpr int P = GRAD ? 3 : 2;
+            float x[8];
+            eight(lds.a, ks, x, [](int) { return 1.0f; });
+            const int64_t block = blocks + (GRAD ? upper_block(ks, wave) : lower_block(ks, wave));
+            store_parts<P>(w.p + block * P * kFragBytes + lane * 16, x);
         }
     }
 }
