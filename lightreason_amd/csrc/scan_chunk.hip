@@ -435,6 +435,7 @@ struct ScanLds {
     f32x4 vec[2][3][16];         // the factors, of two chunks
     float decay[2];
     uint32_t v[4][4][kWave];
+    int odd[4];                  // whether a wave has met a number that is not finite
 };
 
 template <int D, int NC, bool FP16, bool TAPE>
@@ -567,7 +568,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             load_blocks(t, w.t, after);
             __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads_or(0);
+        __syncthreads();
         return;
     }
     if (role >= 4) {
@@ -626,7 +627,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             for (int i = 0; i < 4; ++i)
                 if (r0 + i < left) store_cols<NC, FP16>(to + i * a.out_token, o, i);
         }
-        __syncthreads_or(0);
+        __syncthreads();
         return;
     }
     const int64_t size = static_cast<int64_t>(D) * a.value_dim;
@@ -648,6 +649,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
     float* tape_s = reinterpret_cast<float*>(a.tape);
     float* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
     __builtin_amdgcn_s_setprio(2);
+    if (lane == 0) lds.odd[wave] = 0;
     bool odd = false;   // a number that is not finite
     for (int ch = 0; ch < chunks; ++ch) {
 #pragma unroll
@@ -739,7 +741,9 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
     }
     // Where a value was not finite, a product's zero weights have let it through
     // to earlier tokens: the next launch goes through these columns again.
-    if (__syncthreads_or(odd)) {
+    if (__ballot(odd) != 0 && lane == 0) lds.odd[wave] = 1;
+    __syncthreads();
+    if ((lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]) != 0) {
         if (tid < NC) flag[tid] = 1;
         return;
     }

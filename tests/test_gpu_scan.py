@@ -23,7 +23,8 @@ def _compare(name, x, got, initial, **kw):
 
 
 @pytest.mark.parametrize("lengths", [[1], [2, 0, 1], [17], [63, 64, 65], [0, 130], [300, 5], [129, 0, 0, 256]])
-@pytest.mark.parametrize("layout", [(2, 4, 128, 128, BF), (3, 3, 64, 64, FP), (1, 3, 64, 96, BF), (2, 2, 128, 32, FP)])
+@pytest.mark.parametrize("layout", [(2, 4, 128, 128, BF), (3, 3, 64, 64, FP), (1, 3, 64, 96, BF), (2, 2, 128, 32, FP),
+                                    (1, 6, 64, 256, BF), (2, 10, 128, 32, FP)])
 def test_scan_of_packed_sequences(device, lengths, layout):
     K, H, D, E, dtype = layout
     print(f"[scan] {lengths} {layout}", flush=True)
@@ -252,3 +253,44 @@ def test_many_short_sequences(device):
         y = {k: v[starts[s]:starts[s + 1]] for k, v in x.items() if k != "starts"}
         y["starts"] = torch.tensor([0, lengths[s]], dtype=torch.int32, device=device)
         _compare(f"sequence {s}", y, (out[starts[s]:starts[s + 1]], pool[s:s + 1]), first[s:s + 1])
+
+
+def test_a_step_of_long_and_short_sequences(device):
+    """Prompts among single tokens: either form's sequences in one call, in place."""
+    lengths = [1, 1, 500, 1, 24, 25, 40, 41, 0, 1, 64, 3, 130]
+    x = R.inputs(lengths, 2, 8, 128, 128, BF, 80)
+    pool = R.states(len(lengths), 8, 128, 128, 9)
+    first = pool.clone()
+    out = delta_step(**x, states=pool)
+    _compare("mixed", x, (out, pool), first)
+
+
+def test_a_long_sequence_of_slow_decays(device):
+    """4000 tokens whose state hardly fades."""
+    x = R.inputs([4000], 1, 2, 64, 32, BF, 81, decay=(1e-6, 1e-4))
+    _compare("slow", x, delta_scan(**x), R.states(1, 2, 64, 32, 1) * 0)
+
+
+def test_growing_states(device):
+    """Positive log decays within fp32's range, token by token and in chunks."""
+    for n in (10, 80):
+        x = R.inputs([n], 1, 2, 64, 32, BF, 82)
+        x["g"].fill_(0.05)
+        initial = R.states(1, 2, 64, 32, 1)
+        out, final, size = R.rule(x, initial)
+        b_out, b_final = R.bounds(x, out, size)
+        # An error grows as the state does, e^(0.05 n) at most.
+        grow = 2.718281828 ** (0.05 * n)
+        got = delta_scan(**x, initial=initial)
+        R.check("growing out", got[0], out, b_out * grow)
+        R.check("growing final", got[1], final, b_final * grow)
+
+
+def test_heads_and_tokens_in_any_order_and_repeated_rows(device):
+    """Expanded rows (stride 0) and heads that are stored first."""
+    x = R.inputs([90], 2, 4, 64, 64, BF, 83)
+    y = dict(x)
+    y["query"] = x["query"][:1].expand(90, 2, 64)
+    y["value"] = x["value"].transpose(0, 1).contiguous().transpose(0, 1)
+    y["beta"] = x["beta"][:1].expand(90, 4)
+    _compare("expanded", y, delta_scan(**y), R.states(1, 4, 64, 64, 1) * 0)

@@ -65,7 +65,8 @@ def _check(x, initial, seed=0, normalize=False, scale=None):
 
 
 @pytest.mark.parametrize("lengths", [[1], [2, 0, 1], [17], [63, 64, 65], [0, 130], [200, 5]])
-@pytest.mark.parametrize("layout", [(2, 4, 128, 128, BF), (3, 3, 64, 64, FP), (1, 3, 64, 96, BF), (2, 2, 128, 32, FP)])
+@pytest.mark.parametrize("layout", [(2, 4, 128, 128, BF), (3, 3, 64, 64, FP), (1, 3, 64, 96, BF), (2, 2, 128, 32, FP),
+                                    (1, 6, 64, 256, BF), (2, 10, 128, 32, FP)])
 def test_gradients_of_packed_sequences(device, lengths, layout):
     K, H, D, E, dtype = layout
     print(f"[scan] {lengths} {layout}", flush=True)
