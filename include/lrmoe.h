@@ -687,8 +687,8 @@ int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t
  * v 16-byte and out 8-byte aligned; out shares no element with q, k and v
  * (refused) or anything else that is read.  dim 64 or 128, value_dim a multiple
  * of 32 up to 256, at most 2^20 tokens, 65536 sequences and tokens * heads of
- * 2^26.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes, 256-byte
- * aligned, not cleared, used by one stream at a time. */
+ * 2^26.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes (0: none),
+ * 256-byte aligned, not cleared, used by one stream at a time. */
 typedef struct lrmoe_delta_scan_args {
     int32_t seqs, tokens, max_new, heads, key_heads, dim, value_dim, fp16;
     int32_t normalize, beta_fp32, clear, pool;

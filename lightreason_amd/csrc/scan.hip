@@ -158,7 +158,7 @@ static int token_wise(const ScanArgs& a) {
 }
 
 size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
-    return max_new <= token_wise(a) ? 256 : scan_chunk_bytes(a, fp16);
+    return max_new <= token_wise(a) ? 0 : scan_chunk_bytes(a, fp16);
 }
 
 hipError_t launch_delta_scan(ScanArgs a, bool fp16, int max_new, void* workspace, hipStream_t stream) {

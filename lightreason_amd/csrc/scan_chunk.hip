@@ -370,9 +370,14 @@ __device__ __forceinline__ float col_value(uint32_t v, int c) {
     return elem16<FP16>(static_cast<uint16_t>(c ? v >> 16 : v));
 }
 template <int NC, bool FP16>
-__device__ __forceinline__ void store_cols(uint16_t* to, const f32x4 (&x)[NC], int i) {
-    if constexpr (NC == 1) *to = static_cast<uint16_t>(pack16_2<FP16>(x[0][i], 0.0f));
-    else *reinterpret_cast<uint32_t*>(to) = pack16_2<FP16>(x[0][i], x[1][i]);
+__device__ __forceinline__ uint32_t pack_cols(const f32x4 (&x)[NC], int i) {
+    if constexpr (NC == 1) return pack16_2<FP16>(x[0][i], 0.0f);
+    return pack16_2<FP16>(x[0][i], x[1][i]);
+}
+template <int NC>
+__device__ __forceinline__ void store_cols(uint16_t* to, uint32_t v) {
+    if constexpr (NC == 1) *to = static_cast<uint16_t>(v);
+    else *reinterpret_cast<uint32_t*>(to) = v;
 }
 
 // A workgroup's part of the work: a sequence, a value head and a block of
@@ -574,6 +579,14 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
     if (role >= 4) {
         __builtin_amdgcn_s_setprio(1);
         uint4 q[KS][PARTS], p[2][2];
+        uint32_t packed[4];   // the last chunk's outputs
+        auto store = [&](int ch) {
+            const int left = seq.n - ch * kChunk;
+            uint16_t* to = a.out + static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.out_token + h * a.out_head + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + i < left) store_cols<NC>(to + i * a.out_token, packed[i]);
+        };
         if (chunks > 0) {
             load_rows(q, a.q, a.q_token, a.q_head, w.qf, 0);
             __builtin_amdgcn_sched_barrier(0);
@@ -605,6 +618,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                 for (int c = 0; c < NC; ++c) o[c] *= fq;
             }
             __syncthreads();
+            if (ch > 0) store(ch - 1);   // (these waves have nothing else between here)
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -621,12 +635,10 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             __builtin_amdgcn_sched_barrier(0);
             load_blocks(p, w.p, next);
             __builtin_amdgcn_sched_barrier(0);
-            const int left = seq.n - ch * kChunk;
-            uint16_t* to = a.out + static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.out_token + h * a.out_head + col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r0 + i < left) store_cols<NC, FP16>(to + i * a.out_token, o, i);
+            for (int i = 0; i < 4; ++i) packed[i] = pack_cols<NC, FP16>(o, i);
         }
+        if (chunks > 0) store(chunks - 1);
         __syncthreads();
         return;
     }
@@ -1034,7 +1046,7 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
             uint16_t* to = d.dv + (static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.heads + h) * a.value_dim + col;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (r0 + i < left) store_cols<NC, FP16>(to + static_cast<int64_t>(i) * a.heads * a.value_dim, dr, i);
+                if (r0 + i < left) store_cols<NC>(to + static_cast<int64_t>(i) * a.heads * a.value_dim, pack_cols<NC, FP16>(dr, i));
         }
         __syncthreads();
 #pragma unroll

@@ -111,8 +111,8 @@ def _scratch(a) -> int:
 
 def _launch(a, dev, nbytes):
     with _on(dev):
-        ws = _native.workspace(dev, nbytes)
-        _native.call("lrmoe_delta_scan", C.addressof(a), ws.data_ptr(), ws.numel(), _stream(dev))
+        ws = _native.workspace(dev, nbytes) if nbytes else None
+        _native.call("lrmoe_delta_scan", C.addressof(a), _ptr(ws), nbytes, _stream(dev))
 
 
 # ---- whole sequences ------------------------------------------------------------

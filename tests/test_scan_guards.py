@@ -53,7 +53,7 @@ def test_scan_refuses_host_tensors_and_shapes():
 
 def test_c_entry_points_refuse_misuse():
     lib = _native.library()
-    good = dict(seqs=1, tokens=4, max_new=4, heads=4, key_heads=2, dim=64, value_dim=64, pool=1, scale=1.0,
+    good = dict(seqs=1, tokens=4, max_new=100, heads=4, key_heads=2, dim=64, value_dim=64, pool=1, scale=1.0,
                 q=256, k=256, v=1 << 20, g=256, beta=256, starts=256, initial=256, final=256, out=1 << 24,
                 q_token_stride=128, q_head_stride=64, k_token_stride=128, k_head_stride=64, v_token_stride=256,
                 v_head_stride=64, g_token_stride=4, beta_token_stride=4, out_token_stride=256, out_head_stride=64)
