@@ -6,7 +6,8 @@ layers of the 35B model, for any head layout of width 64, 128 or 256.
   the device: ``plan`` turns the rows' new position counts into block table
   entries, slots and offsets (``lrmoe_page_plan``), ``commit`` takes a plan
   into the pool (with the verified counts of a speculative step), ``release``
-  returns finished rows' pages.
+  returns finished rows' pages, ``fork`` copies rows' pages to other rows
+  (``lrmoe_page_fork``).
 * ``paged_append`` -- per-head q/k RMSNorm, rotary embedding and the append of
   keys and values into their slots (``lrmoe_paged_append``).
 * ``paged_attention`` -- the causal attention of the new positions over the
