@@ -190,6 +190,7 @@ class _DeltaScan(torch.autograd.Function):
     def forward(ctx, form, *tensors):
         out, final, tape = _scan(form, tensors, taped=True)
         ctx.form = form
+        ctx.strides = [t.stride() for t in tensors[:5]]
         ctx.first = tensors[6] is not None
         ctx.save_for_backward(*tensors[:6], *(() if tape is None else (tape,)))
         return out, final
@@ -205,6 +206,13 @@ class _DeltaScan(torch.autograd.Function):
             first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
             return None, *zeros, None, first
         a = _native.DeltaScanArgs.from_buffer_copy(template)
+        if any(t.stride() != s for t, s in zip((query, key, value, g, beta), ctx.strides)):
+            # Hooks on saved tensors (those that keep them on the host) have laid them out anew.
+            query, key, value, g, beta = (t.contiguous() for t in (query, key, value, g, beta))
+            a.q_token_stride, a.q_head_stride = _strides(query)
+            a.k_token_stride, a.k_head_stride = _strides(key)
+            a.v_token_stride, a.v_head_stride = _strides(value)
+            (a.g_token_stride,), (a.beta_token_stride,) = _strides(g), _strides(beta)
         _addresses(a, query, key, value, g, beta, starts)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value, g, beta)]
         first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None

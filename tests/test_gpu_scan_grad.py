@@ -181,6 +181,19 @@ def test_forward_with_and_without_a_tape_are_the_same(device):
     assert torch.equal(plain[0], taped[0]) and torch.equal(plain[1], taped[1])
 
 
+def test_saved_tensors_kept_on_the_host(device):
+    """Hooks that hand the inputs back in another layout."""
+    x = R.inputs([70, 20], 2, 4, 64, 64, BF, 16)
+    leaves = [x[n].detach().requires_grad_() for n in NAMES]
+    assert not leaves[0].is_contiguous()
+    d_out = torch.randn(x["value"].shape, generator=torch.Generator().manual_seed(3)).to(BF).to(device)
+    want = torch.autograd.grad(delta_scan(*leaves, x["starts"])[0], leaves, d_out)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().cpu(), lambda t: t.to(device)):
+        out, _ = delta_scan(*leaves, x["starts"])
+    for a, b in zip(torch.autograd.grad(out, leaves, d_out), want):
+        assert torch.equal(a, b)
+
+
 def test_a_training_step_in_a_graph(device):
     """Forward and backward captured, replayed on changing inputs between the
     program's own eager steps."""
