@@ -86,8 +86,9 @@ struct ScanChunks {
     float *ds, *dr;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
 };
 
-// A beta of 0 is taken as 2^-40: u = beta w then still tells w, which beta's
-// gradient is made of; no output changes by more than 2^-40 of its terms.
+// Where a gradient is wanted a beta of 0 is taken as 2^-40: u = beta w then still
+// tells w, which beta's gradient is made of; what that adds is 2^-40 of what a
+// beta of 1 would.
 __device__ __forceinline__ float scan_beta(float b) {
     return __builtin_fabsf(b) < 0x1p-40f ? __builtin_copysignf(0x1p-40f, b) : b;
 }

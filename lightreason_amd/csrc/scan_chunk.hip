@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
             const bool in = lane < count;   // (rows past the sequence repeat its last one)
             const double sum = wave_scan_f64(in ? scan_log(raw_g) * 1.4426950408889634 : 0.0);
             lds.sum[wave][lane] = sum;
-            lds.beta[wave][lane] = in ? scan_beta(beta) : 0.0f;
+            lds.beta[wave][lane] = !in ? 0.0f : GRAD || a.tape != nullptr ? scan_beta(beta) : beta;
             if (hv + wave < a.group) {
                 if constexpr (GRAD) w.sums[(by_head + wave) * kChunk + lane] = sum;
                 const double last = __shfl(sum, kWave - 1);

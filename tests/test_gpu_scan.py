@@ -109,6 +109,23 @@ def test_decays_of_zero_and_steps_without_weight(device):
         _compare("reads only", x, delta_scan(**x, initial=initial), initial)
 
 
+def test_a_step_without_weight_before_growth(device):
+    """What beta = 0 leaves out stays out, however much a state grows after it."""
+    for n in (9, 140):
+        x = R.inputs([n], 2, 2, 64, 64, BF, 14)
+        at = n // 2
+        x["beta"][:at + 1] = 0.0
+        x["beta"][-1] = 0.0
+        x["value"][at] = 100.0
+        x["g"][at + 1] = 30.0
+        out, final = delta_scan(**x)
+        # A state of zero, until the first step with a weight.
+        assert not out[:at + 1].any()
+        want = {k: v[at + 1:] for k, v in x.items() if k != "starts"}
+        want["starts"] = torch.tensor([0, n - at - 1], dtype=torch.int32, device=device)
+        _compare("after", want, (out[at + 1:], final), R.states(1, 2, 64, 64, 1) * 0)
+
+
 def test_repeated_keys(device):
     """The same key again and again: nothing cancels in the chunk's inverse."""
     x = R.inputs([200], 1, 2, 128, 64, BF, 13)
