@@ -678,16 +678,17 @@ int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t
  * (NULL: s).  initial may be final, and a sequence's slots the same; no two
  * sequences write one slot, and none writes a slot that another reads.  A
  * sequence without tokens passes its state on.  One whose slot lies outside the
- * pool is left out, its rows too; one whose starts are not in order within
- * [0, tokens] counts as empty.  Rows outside starts[0] .. starts[seqs] - 1 stay
+ * pool is left out, its rows too.  starts never decrease and lie within [0,
+ * tokens]: a sequence whose own do not counts as empty, and what a call with
+ * such starts gives for the others is not defined.  Rows outside starts[0] .. starts[seqs] - 1 stay
  * as they were, or are set to 0 with clear.  What is not finite reaches later
  * tokens of its sequence only.  max_new only chooses the kernel: at least every
  * sequence's count where they are short.  Strides in elements, those of q, k, v
  * and out multiples of 8 (4 for out) with the last dimension contiguous; q, k,
  * v 16-byte and out 8-byte aligned; out shares no element with q, k and v
  * (refused) or anything else that is read.  dim 64 or 128, value_dim a multiple
- * of 32 up to 256, at most 2^20 tokens, 65536 sequences and tokens * heads of
- * 2^26.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes (0: none),
+ * of 32 up to 256, at most 2^20 tokens, 65536 sequences, tokens * heads of 2^26
+ * and seqs * heads * value_dim of 2^27.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes (0: none),
  * 256-byte aligned, not cleared, used by one stream at a time. */
 typedef struct lrmoe_delta_scan_args {
     int32_t seqs, tokens, max_new, heads, key_heads, dim, value_dim, fp16;
@@ -742,7 +743,7 @@ int lrmoe_delta_scan_grad(const lrmoe_delta_scan_args *args, const lrmoe_delta_g
  * finite take no part; neither does a beam whose score is not finite; a beam
  * with finished (uint8, may be NULL) != 0 has one continuation, itself, with
  * token -1 and its score.  Of a group's continuations the `beams` best are kept
- * (ties: lowest beam, then lowest token).  A beam's best one that is kept takes
+ * (ties: lowest beam, in one its larger logit, then the lowest token).  A beam's best one that is kept takes
  * the beam's own row, the others in order of their scores the rows left over,
  * lowest first, so that rows whose parent is another are those that died: their
  * states and pages may be overwritten by the parents' (lrmoe_fork_rows,
@@ -760,7 +761,8 @@ int lrmoe_beam_select(int groups, int beams, int vocab, int type, const void *lo
  * parent stays; so does one whose parent lies outside [0, rows) or is not its
  * own parent (nothing that is read is written).  tensors (on the host, as its
  * numbers) holds a base address, the rows' stride and the bytes of a row, three
- * int64 per tensor; at most LRMOE_FORK_TENSORS of them. */
+ * int64 per tensor; at most LRMOE_FORK_TENSORS of them, and 2^24 pieces of
+ * 32 KB, rows' last ones included. */
 #define LRMOE_FORK_TENSORS 64
 int lrmoe_fork_rows(int rows, const int32_t *parents, int tensors, const int64_t *table, void *stream);
 

@@ -992,8 +992,12 @@ static bool bad_scan(const lrmoe_delta_scan_args* p) {
     return p->seqs < 0 || p->seqs > 65536 || p->tokens < 0 || p->tokens > (1 << 20) || p->max_new < 0 || p->heads < 1 ||
            p->heads > 1024 || p->key_heads < 1 || p->heads % p->key_heads != 0 || (p->dim != 64 && p->dim != 128) ||
            p->value_dim < 32 || p->value_dim > 256 || p->value_dim % 32 != 0 || p->pool < 0 ||
-           static_cast<int64_t>(p->tokens) * p->heads > (1 << 26);
+           static_cast<int64_t>(p->tokens) * p->heads > (1 << 26) ||
+           static_cast<int64_t>(p->seqs) * p->heads * p->value_dim > (1 << 27);   // (a launch's threads, 2^32)
 }
+
+// (A tape is written by the chunked form only.)
+static int scan_max_new(const lrmoe_delta_scan_args* p) { return p->tape ? p->tokens : p->max_new; }
 
 static lrmoe::ScanArgs scan_args(const lrmoe_delta_scan_args* p) {
     lrmoe::ScanArgs a{};
@@ -1037,7 +1041,7 @@ static lrmoe::ScanArgs scan_args(const lrmoe_delta_scan_args* p) {
 
 size_t lrmoe_delta_scan_workspace_bytes(const lrmoe_delta_scan_args* p) {
     if (!p || bad_scan(p)) return 0;
-    return lrmoe::delta_scan_workspace_bytes(scan_args(p), p->fp16 != 0, p->max_new);
+    return lrmoe::delta_scan_workspace_bytes(scan_args(p), p->fp16 != 0, scan_max_new(p));
 }
 
 // What forward and gradient ask of a call's inputs.
@@ -1087,7 +1091,8 @@ int lrmoe_delta_scan(const lrmoe_delta_scan_args* p, void* workspace, size_t wor
             return LRMOE_E_ARG;
     }
     if (int d = check_device()) return d;
-    return status_of(lrmoe::launch_delta_scan(scan_args(p), p->fp16 != 0, p->max_new, workspace, as_stream(stream)));
+    return status_of(
+        lrmoe::launch_delta_scan(scan_args(p), p->fp16 != 0, scan_max_new(p), workspace, as_stream(stream)));
 }
 
 size_t lrmoe_delta_scan_tape_bytes(const lrmoe_delta_scan_args* p) {
@@ -1170,12 +1175,13 @@ int lrmoe_fork_rows(int rows, const int32_t* parents, int tensors, const int64_t
     for (int i = 0; i < tensors; ++i) {
         const int64_t base = table[3 * i], stride = table[3 * i + 1], bytes = table[3 * i + 2];
         // Rows lie behind one another, and their pieces can be counted.
-        if ((base == 0 && bytes > 0) || bytes < 0 || bytes > (INT64_C(1) << 40) || (rows > 1 && stride < bytes)) return LRMOE_E_ARG;
+        if ((base == 0 && bytes > 0) || bytes < 0 || bytes > (INT64_C(1) << 40) || (rows > 1 && stride < bytes))
+            return LRMOE_E_ARG;
         a.t[i] = {reinterpret_cast<uint8_t*>(base), stride, bytes, 0, 0};
     }
     int64_t pieces = 0;
     for (int i = 0; i < tensors; ++i) pieces += ((a.t[i].bytes + 32767) / 32768) * rows;
-    if (pieces > 0x7fffffff) return LRMOE_E_ARG;
+    if (pieces >= (1 << 24)) return LRMOE_E_ARG;   // (a launch holds 2^32 threads)
     if (int d = check_device()) return d;
     return status_of(lrmoe::launch_fork_rows(a, as_stream(stream)));
 }

@@ -361,7 +361,6 @@ hipError_t launch_fork_rows(ForkRowsArgs a, hipStream_t stream) {
         blocks += (t.bytes + kForkBytes - 1) / kForkBytes * a.rows;
     }
     if (blocks == 0) return hipSuccess;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     fork_rows_kernel<<<static_cast<uint32_t>(blocks), kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }

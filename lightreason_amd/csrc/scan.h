@@ -1,5 +1,5 @@
 // Arguments and shared pieces of the gated delta rule over packed sequences
-// (scan.hip: forward; scan_grad.hip: gradient).
+// (scan.hip: token by token; scan_chunk.hip: in chunks, and the gradient).
 #pragma once
 
 #include "lrmoe_device.h"

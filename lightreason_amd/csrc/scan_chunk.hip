@@ -435,7 +435,7 @@ struct ScanLds {
     uint4 r[3][2][NC][kWave];
     uint4 u[2][2][NC][kWave];    // for the outputs
     uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
-    // What waves 4 to 7 have read for waves 0 to 3.
+    // What waves 8 to 11 have read for waves 0 to 3.
     uint4 k[4][D / 32 * PARTS][kWave], t[4][6][kWave], kt[4][D / 64 * 2 * PARTS][kWave];
     f32x4 vec[2][3][16];         // the factors, of two chunks
     float decay[2];
@@ -1610,8 +1610,8 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
     return w;
 }
 
-// A launch holds fewer than 2^31 workgroups: slots * key_heads stay below
-// (2^14 + 2^16) 2^10.
+// Launches hold fewer than 2^32 threads: tokens / 64 * heads are at most 2^20,
+// seqs * heads * value_dim / 32 at most 2^22.
 template <int D, bool FP16>
 void launch(const ScanArgs& a, const ScanChunks& w, hipStream_t stream) {
     scan_prepare<D, FP16, false><<<static_cast<uint32_t>(w.slots) * a.key_heads, kThreads, 0, stream>>>(a, w);

@@ -82,9 +82,9 @@ def _check(query, key, value, g, beta, starts, normalize, scale):
         raise ValueError("starts must be int32 [seqs + 1]")
     S = starts.shape[0] - 1
     _require(starts, "starts", (torch.int32,), (S + 1,), dev)
-    if S > 65536 or N > 1 << 20 or N * H > 1 << 26 or H > 1024:
-        raise ValueError(f"at most 65536 sequences, 2^20 tokens, 1024 heads and tokens * heads of 2^26, got {S}, {N}, "
-                         f"{H} and {N * H}")
+    if S > 65536 or N > 1 << 20 or N * H > 1 << 26 or H > 1024 or S * H * E > 1 << 27:
+        raise ValueError(f"at most 65536 sequences, 2^20 tokens, 1024 heads, tokens * heads of 2^26 and sequences * heads * "
+                         f"width of 2^27, got {S}, {N}, {H}, {N * H} and {S * H * E}")
     a = _native.DeltaScanArgs(seqs=S, tokens=N, max_new=N, heads=H, key_heads=K, dim=D, value_dim=E,
                               fp16=int(dtype == torch.float16), normalize=int(bool(normalize)),
                               beta_fp32=int(beta.dtype == torch.float32), scale=D ** -0.5 if scale is None else scale)
@@ -134,16 +134,20 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     ``normalize`` divides q and k by sqrt(sum x^2 + 1e-6) first; ``scale``
     defaults to dim ** -0.5.  Returns (out [tokens, heads, value_dim], the last
     states [seqs, heads, dim, value_dim] fp32).  A sequence without tokens
-    passes its state on; rows of no sequence are 0; starts that are not in
-    order within [0, tokens] make a sequence empty.  What is not finite reaches
-    only later tokens of its sequence.  Tensors may be strided views with a
-    contiguous last dimension and strides that are multiples of 8.
+    passes its state on; rows of no sequence are 0.  ``starts`` never decrease
+    and lie within [0, tokens] (a batch is padded with their last value): a
+    sequence whose own do not counts as empty, and what such a call gives for
+    the others is not defined.  What is not finite reaches only later tokens of
+    its sequence.  Tensors may be strided views with a contiguous last dimension
+    and strides that are multiples of 8.
 
     Gradients flow to query, key, value, g, beta and initial, once (no second
     derivatives); they take the same bits every time.  For them the call keeps
     the states before every 64 tokens and u, 4 (dim + 64) value_dim / 64 bytes a
     token and head.  The gradient of a sequence with values that are not finite
-    is not defined."""
+    is not defined.  A captured training step takes its gradients with
+    torch.autograd.grad, or from leaves of which no eager graph lives
+    (torch's rule for every captured backward pass)."""
     if scale is not None:
         scale = float(scale)
     tensors = (query, key, value, g, beta, starts, initial)
@@ -315,18 +319,20 @@ def fused_scan(model):
     included: what the layers hand to ``torch_chunk_gated_delta_rule`` of their
     Transformers module, any batch and any length.  (The function is the
     module's, so other models of the class run through it meanwhile.)  Tensors
-    on the CPU or of another type than bf16 and fp16, and calls with
-    ``cu_seqlens``, run as before."""
+    on the CPU, of another type than bf16 and fp16 or of several, and calls with
+    ``cu_seqlens``, run as before; a call holds up to 2^20 tokens."""
     name = "torch_chunk_gated_delta_rule"
     def native(original):
         def rule(query, key, value, g, beta, chunk_size=64, initial_state=None, output_final_state=False,
                  use_qk_l2norm_in_kernel=False, **kwargs):
-            if query.device.type != "cuda" or query.dtype not in _TYPES or kwargs.get("cu_seqlens") is not None:
+            if (query.device.type != "cuda" or query.dtype not in _TYPES or key.dtype != query.dtype
+                    or value.dtype != query.dtype or kwargs.get("cu_seqlens") is not None):
                 return original(query, key, value, g=g, beta=beta, chunk_size=chunk_size, initial_state=initial_state,
                                 output_final_state=output_final_state, use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel,
                                 **kwargs)
             batch, tokens = query.shape[:2]
             starts = torch.arange(batch + 1, dtype=torch.int32, device=query.device) * tokens
+            beta = beta if beta.dtype == query.dtype else beta.float()
             rows = [x.reshape(batch * tokens, *x.shape[2:]) for x in (query, key, value, g.float(), beta)]
             first = None if initial_state is None else initial_state.float().contiguous()
             out, final = delta_scan(*(x if x.stride(-1) == 1 else x.contiguous() for x in rows), starts, initial=first,

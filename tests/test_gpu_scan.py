@@ -45,6 +45,22 @@ def test_normalized_inputs_scale_and_fp32_beta(device, dtype, lengths):
     _compare("normalized", x, delta_scan(**x, initial=initial, **kw), initial, **kw)
 
 
+@pytest.mark.parametrize("n", [5, 70])
+def test_fp16_below_its_normal_range(device, n):
+    """Keys that are subnormal in fp16 against large queries and states."""
+    x = R.inputs([n], 2, 2, 64, 64, FP, 17)
+    x["key"].copy_((x["key"].double() * 2.0 ** -16).to(FP))
+    assert 0 < x["key"].abs().max() < torch.finfo(FP).tiny
+    initial = R.states(1, 2, 64, 64, 2)
+    kw = dict(normalize=False, scale=2.0 ** 12)
+    _compare("subnormal", x, delta_scan(**x, initial=initial, **kw), initial, **kw)
+    # From zero, the outputs are of the keys alone.
+    x["g"].zero_()
+    out, _ = delta_scan(**x, scale=2.0 ** 16)
+    want, _, _ = R.rule(x, torch.zeros_like(initial), scale=2.0 ** 16)
+    R.check("of keys", out, want, R.half(FP) * want.abs() + 2.0 ** -16 * want.abs().max())
+
+
 def test_rows_of_no_sequence_are_zero(device):
     x = R.inputs([5, 0, 70], 2, 2, 64, 64, BF, 8, lead=3, tail=40)
     out, final = delta_scan(**x)

@@ -69,10 +69,14 @@ def test_c_entry_points_refuse_misuse():
                dict(q=264), dict(out=(1 << 24) + 4), dict(q_token_stride=129), dict(v_head_stride=4),
                dict(k_token_stride=-8), dict(v_token_stride=1 << 23), dict(out_token_stride=2), dict(g=258),
                dict(beta=257), dict(final=264), dict(workspace=None), dict(workspace=C.c_void_p(128)),
-               dict(tokens=1 << 20, heads=128, key_heads=1)):
+               dict(tokens=1 << 20, heads=128, key_heads=1), dict(seqs=65536, heads=64, key_heads=2)):
         assert call(**kw) == _native.LRMOE_E_ARG, kw
     assert call(nbytes=0) == _native.LRMOE_E_WORKSPACE
     assert call(seqs=0) == 0
+    # max_new is a hint: a tape is the chunked form's, which has its workspace.
+    nbytes = lambda **kw: lib.lrmoe_delta_scan_workspace_bytes(C.byref(_native.DeltaScanArgs(**{**good, **kw})))
+    assert nbytes(max_new=1) == 0 and nbytes(max_new=1, tape=256) == nbytes(max_new=4, tape=256) > 0
+    assert call(max_new=1, tape=256, nbytes=0) == _native.LRMOE_E_WORKSPACE
     assert lib.lrmoe_delta_scan(None, ws, 1 << 40, None) == _native.LRMOE_E_ARG
     # out over what is read, and over itself
     assert call(out=1 << 20) == _native.LRMOE_E_ARG
@@ -113,6 +117,7 @@ def test_c_entry_points_refuse_misuse():
     assert lib.lrmoe_fork_rows(4, p, 1, (C.c_int64 * 3)(256, 63, 64), None) == _native.LRMOE_E_ARG
     assert lib.lrmoe_fork_rows(4, p, 1, (C.c_int64 * 3)(0, 64, 64), None) == _native.LRMOE_E_ARG
     assert lib.lrmoe_fork_rows(1 << 20, p, 1, (C.c_int64 * 3)(256, 1 << 30, 1 << 30), None) == _native.LRMOE_E_ARG
+    assert lib.lrmoe_fork_rows(1 << 24, p, 1, (C.c_int64 * 3)(256, 4, 4), None) == _native.LRMOE_E_ARG
     assert lib.lrmoe_fork_rows(0, None, 1, table, None) == 0
 
     row = (256, 2, 2, 128, 1 << 20, 1 << 12, 1 << 11, 128)
