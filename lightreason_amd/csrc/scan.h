@@ -78,7 +78,7 @@ struct ScanChunks {
     uint8_t *t, *p;        // [slots][heads]: 3 and 2 parts of 6 blocks
     float* vec;            // [slots][heads][256]: factors of K S, of Q S and of K^T U per token, then the chunk's decay
     uint8_t *kt, *qt;      // [slots][key_heads][dim / 16][2][parts]: K^T, and for the gradient Q^T
-    uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of fp16 inputs as bf16 parts
+    uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of K, and for the outputs of Q
     uint32_t* flags;       // [seqs][heads][value_dim / 16]
     // For the gradient: t and p hold the transposed matrices, 3 parts each, and
     double* sums;          // [slots][heads][64]: running sums of g
