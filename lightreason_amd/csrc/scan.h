@@ -84,6 +84,7 @@ struct ScanChunks {
     double* sums;          // [slots][heads][64]: running sums of g
     float* norms;          // [slots][key_heads][128]: factors of k and of q
     float *ds, *dr;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
+    f32x4* pairs;          // [slots][key_heads][4][512]: q . k and k . k, by threads
 };
 
 // Where a gradient is wanted a beta of 0 is taken as 2^-40: u = beta w then still
