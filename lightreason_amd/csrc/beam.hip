@@ -86,7 +86,9 @@ __device__ __forceinline__ uint64_t wave_best(int W, int lane, Each&& each) {
 // exponentials, and the W best. Those are no smaller than the W-th largest of the
 // lanes' maxima, so that only what reaches it is gathered and ranked, W numbers
 // and a few more; where equal values make them more than a list holds, the
-// registers are gone through W times instead.
+// registers are gone through W times instead.  Bound by the logits (256 rows of
+// 151936 fp32, a tenth of them finished: 20.9 us, 6.8 TB/s; with W passes for every
+// slice 55 us); 4 rows in bf16 5.7 us, launch and latency.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void beam_slices(BeamArgs a) {
     __shared__ uint64_t lists[kThreads / kWave][kGather], bests[kThreads / kWave][kBeamMax];
@@ -178,7 +180,8 @@ __global__ __launch_bounds__(kThreads) void beam_slices(BeamArgs a) {
 
 // One workgroup per group: each wave joins the slices of a row, then the W W
 // candidates are ranked by counting those ahead of each, in 64 bits (distinct
-// logits of a row stay distinct).
+// logits of a row stay distinct).  Bound by its chain of loads and W maxima over a
+// wave: 5.6 us for 1 x 4 beams, 9.9 for 32 x 8.
 __global__ __launch_bounds__(kJoinThreads) void beam_join(BeamArgs a) {
     __shared__ double score[kBeamMax * kBeamMax];
     __shared__ int token[kBeamMax * kBeamMax];
@@ -308,7 +311,8 @@ __device__ __forceinline__ void fork_copy(uint8_t* to, const uint8_t* from, int6
 
 // A workgroup copies a piece of a row.  Rows that are read keep their places
 // (a row whose parent moves itself is left alone), so nothing that is read is
-// written.  Bound by HBM: each byte that moves is read and written once.
+// written.  Bound by HBM: each byte that moves is read and written once (60 tensors
+// of states of 32 rows, two thirds of them moving: 5.3 to 6 TB/s).
 __global__ __launch_bounds__(kThreads) void fork_rows_kernel(ForkRowsArgs a) {
     int i = 0;
     while (i + 1 < a.tensors && static_cast<int>(blockIdx.x) >= a.t[i + 1].first) ++i;
