@@ -312,7 +312,7 @@ __device__ __forceinline__ void fork_copy(uint8_t* to, const uint8_t* from, int6
 // A workgroup copies a piece of a row.  Rows that are read keep their places
 // (a row whose parent moves itself is left alone), so nothing that is read is
 // written.  Bound by HBM: each byte that moves is read and written once (60 tensors
-// of states of 32 rows, two thirds of them moving: 5.3 to 6 TB/s).
+// of 32 rows' states: 5.3 to 6 TB/s of what moves).
 __global__ __launch_bounds__(kThreads) void fork_rows_kernel(ForkRowsArgs a) {
     int i = 0;
     while (i + 1 < a.tensors && static_cast<int>(blockIdx.x) >= a.t[i + 1].first) ++i;
