@@ -181,6 +181,43 @@ def test_forward_with_and_without_a_tape_are_the_same(device):
     assert torch.equal(plain[0], taped[0]) and torch.equal(plain[1], taped[1])
 
 
+def test_more_sequences_than_a_wave_has_lanes(device):
+    lengths = [(11 * i) % 71 for i in range(90)]
+    x = R.inputs(lengths, 1, 2, 64, 32, BF, 18)
+    _check(x, R.states(90, 2, 64, 32, 3))
+
+
+def test_offsets_past_32_bits(device):
+    """One sequence of more than 2^31 values against its halves one after the
+    other, which makes the same chunks: the same bits, gradients too."""
+    N, K, H, D, half = 2**19 + 100, 2, 32, 128, 2**18
+    gen = torch.Generator(device=device).manual_seed(19)
+    row = torch.empty(N, (2 * K + H) * D, dtype=BF, device=device).normal_(generator=gen)
+    q, k, v = row[:, :K * D].view(N, K, D), row[:, K * D:2 * K * D].view(N, K, D), row[:, 2 * K * D:].view(N, H, D)
+    assert v.numel() > 2**31
+    g = -torch.rand(N, H, generator=gen, device=device)
+    beta = torch.rand(N, H, generator=gen, device=device)
+    leaves = [t.requires_grad_() for t in (q.detach(), k.detach(), v.detach(), g, beta)]
+    d_out = torch.empty(N, H, D, dtype=BF, device=device).normal_(generator=gen)
+    starts = lambda n: torch.tensor([0, n], dtype=torch.int32, device=device)
+    out, final = delta_scan(*leaves, starts(N), normalize=True)
+    whole = torch.autograd.grad([out, final], leaves, [d_out, torch.ones_like(final)])
+    out, final = out.detach(), final.detach()
+    torch.cuda.empty_cache()
+    for i, t in enumerate(whole):
+        assert torch.isfinite(t).all(), NAMES[i]
+    first, last = [t[:half] for t in leaves], [t[half:] for t in leaves]
+    out1, middle = delta_scan(*first, starts(half), normalize=True)
+    out2, end = delta_scan(*last, starts(N - half), initial=middle, normalize=True)
+    assert torch.equal(out[:half], out1) and torch.equal(out[half:], out2) and torch.equal(final, end)
+    got = torch.autograd.grad([out1, out2, end], first + last, [d_out[:half], d_out[half:], torch.ones_like(end)])
+    for i, name in enumerate(NAMES):
+        print(f"[scan] d{name}", flush=True)
+        assert torch.equal(whole[i][:half], got[i]) and torch.equal(whole[i][half:], got[5 + i]), name
+    del out, out1, out2, whole, got
+    torch.cuda.empty_cache()
+
+
 def test_saved_tensors_kept_on_the_host(device):
     """Hooks that hand the inputs back in another layout."""
     x = R.inputs([70, 20], 2, 4, 64, 64, BF, 16)
