@@ -75,12 +75,12 @@ __host__ __device__ __forceinline__ constexpr int upper_block(int ks, int w) { r
 // key head), in this order in the workspace.
 struct ScanChunks {
     int slots, parts;      // parts: bf16 numbers that a q or k is (1, or 2 for fp16)
-    uint8_t *t, *p;        // [slots][heads]: 3 and 2 parts of 6 blocks
+    uint8_t *t, *p;        // [slots][heads]: 3 parts of 6 blocks
     float* vec;            // [slots][heads][256]: factors of K S, of Q S and of K^T U per token, then the chunk's decay
     uint8_t *kt, *qt;      // [slots][key_heads][dim / 16][2][parts]: K^T, and for the gradient Q^T
     uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of K, and for the outputs of Q
     uint32_t* flags;       // [seqs][heads][value_dim / 16]
-    // For the gradient: t and p hold the transposed matrices, 3 parts each, and
+    // For the gradient: t and p hold the transposed matrices, and
     double* sums;          // [slots][heads][64]: running sums of g
     float* norms;          // [slots][key_heads][128]: factors of k and of q
     float *ds, *dr;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
@@ -102,7 +102,7 @@ __host__ __device__ __forceinline__ int64_t tape_states(int64_t slots, int heads
 }
 
 // An fp32 number as the sum of bf16 ones, each the rest rounded to nearest: two
-// are within 2^-17 of it, three all of its 24 bits.
+// hold an fp16 number, three all of fp32's 24 bits.
 struct Split2 {
     uint32_t part[3];   // pairs
 };

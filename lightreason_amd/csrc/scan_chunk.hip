@@ -11,10 +11,11 @@
 //
 // Products are of bf16 matrix instructions with nothing rounded: q and k are
 // bf16 as they come (an fp16 number is two bf16 ones), and an fp32 factor is
-// split into three bf16 numbers whose sum it is (two for the products that only
-// reach the outputs, which are rounded to 16 bits themselves), so that states
-// are as good as sums in fp32.  The raw q and k enter the products; their
-// norms are factors of rows.
+// split into three bf16 numbers whose sum it is, so that states, outputs and
+// gradients are as good as sums in fp32.  (Two would leave 2^-18 of each factor
+// out: of outputs that are rounded to bf16 0.3 % then came out a step off, 0.02 %
+// of a recurrence in fp32, and what cancels is off without a bound.)  The raw q
+// and k enter the products; their norms are factors of rows.
 #include "scan.h"
 
 namespace lrmoe {
@@ -339,11 +340,10 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (GRAD ? 2 * ks + 1 < wave : 2 * ks > wave) continue;
-            constexpr int P = GRAD ? 3 : 2;
             float x[8];
             eight(lds.a, ks, x, [](int) { return 1.0f; });
             const int64_t block = blocks + (GRAD ? upper_block(ks, wave) : lower_block(ks, wave));
-            store_parts<P>(w.p + block * P * kFragBytes + lane * 16, x);
+            store_parts<3>(w.p + block * 3 * kFragBytes + lane * 16, x);
         }
     }
 }
@@ -449,7 +449,7 @@ template <int D, int NC, int PARTS>
 struct ScanLds {
     uint4 s[3][D / 32][NC][kWave];
     uint4 r[3][2][NC][kWave];
-    uint4 u[2][2][NC][kWave];    // for the outputs
+    uint4 u[3][2][NC][kWave];    // for the outputs
     uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
     // What waves 8 to 11 have read for waves 0 to 3.
     uint4 k[4][D / 32 * PARTS][kWave], t[4][6][kWave], kt[4][D / 64 * 2 * PARTS][kWave];
@@ -500,13 +500,12 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
 #pragma unroll
         for (int i = 0; i < KS * PARTS; ++i) to[i / PARTS][i % PARTS] = frag16(at + i * kFragBytes, frag);
     };
-    auto load_blocks = [&](auto& to, const uint8_t* blocks, int ch) {
-        constexpr int P = sizeof(to) / sizeof(uint4) / 2;
-        const uint8_t* at = blocks + ((slot0 + ch) * a.heads + h) * kBlocks * P * kFragBytes;
+    auto load_blocks = [&](uint4 (&to)[2][3], const uint8_t* blocks, int ch) {
+        const uint8_t* at = blocks + ((slot0 + ch) * a.heads + h) * kBlocks * 3 * kFragBytes;
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            to[0][p] = frag16(at + (lower_block(0, wave) * P + p) * kFragBytes, frag);
-            to[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * P + p) * kFragBytes, frag);
+        for (int p = 0; p < 3; ++p) {
+            to[0][p] = frag16(at + (lower_block(0, wave) * 3 + p) * kFragBytes, frag);
+            to[1][p] = frag16(at + (lower_block(1, max(wave, 2)) * 3 + p) * kFragBytes, frag);
         }
     };
     if (role >= 8) {
@@ -585,7 +584,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
     }
     if (role >= 4) {
         __builtin_amdgcn_s_setprio(1);
-        uint4 q[KS][PARTS], p[2][2];
+        uint4 q[KS][PARTS], p[2][3];
         uint32_t packed[4];   // the last chunk's outputs
         auto store = [&](int ch) {
             const int left = seq.n - ch * kChunk;
@@ -609,12 +608,12 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 3; ++b)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
                         const uint4 f = lds.s[b][i][c][lane];
 #pragma unroll
-                        for (int r = 0; r < PARTS && r + b < 2; ++r) o[c] = mfma16x16x32(q[i][r], f, o[c]);
+                        for (int r = 0; r < PARTS && r + b < 3; ++r) o[c] = mfma16x16x32(q[i][r], f, o[c]);
                     }
             __builtin_amdgcn_sched_barrier(0);
             load_rows(q, w.qf, next);
@@ -631,12 +630,12 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             for (int j = 0; j < 2; ++j) {
                 if (2 * j > wave) continue;
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 3; ++b)
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
                         const uint4 f = lds.u[b][j][c][lane];
 #pragma unroll
-                        for (int r = 0; r + b < 2; ++r) o[c] = mfma16x16x32(p[j][r], f, o[c]);
+                        for (int r = 0; r + b < 3; ++r) o[c] = mfma16x16x32(p[j][r], f, o[c]);
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -730,7 +729,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            put_parts<2>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
+            put_parts<3>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
             put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * fu);
 #pragma unroll
             for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[c][i]) & 0x7f800000u) == 0x7f800000u;
@@ -1096,9 +1095,7 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
 // dq and dk each. What is fp32 (S, dS, u, dR) is read once by the workgroup, 32
 // columns at a time, split into three bf16 numbers and shared through LDS, the
 // next 32 while the products of those before run (training step of 4000 tokens:
-// 300 -> 257 us): the decays' gradient is fp32 and as exact as that. The second
-// products, over tokens, only reach dq and dk, which are rounded to 16 bits: two
-// parts. Bound by its one workgroup per CU: 208 KB of S, dS, u and dR per chunk and
+// 300 -> 257 us): the decays' gradient is fp32 and as exact as that. Bound by its one workgroup per CU: 208 KB of S, dS, u and dR per chunk and
 // value head come at 1.3 TB/s.
 constexpr int kGradThreads = 512;
 template <int D>
@@ -1111,7 +1108,7 @@ struct ScanInputsLds {
         struct {
             float b1[kChunk * kPitch], b2[kChunk * kPitch];   // at first q . k and k . k, in the end dq and dk
             float sum[kChunk * kPitch];         // M
-            uint4 frag[4][kBlocks][2][kWave];   // B1 and B2 by rows (lower blocks), by columns (upper ones)
+            uint4 frag[4][kBlocks][3][kWave];   // B1 and B2 by rows (lower blocks), by columns (upper ones)
         } m;
     };
     double sum[kChunk];
@@ -1126,13 +1123,14 @@ __device__ __forceinline__ float sum_over_16(float v) {
     return butterfly_step8(v);
 }
 
-// Eight floats as a fragment of two parts.
-__device__ __forceinline__ void two_parts(uint4 (&to)[2], const float (&f)[8]) {
+// Eight floats as a fragment of so many parts.
+template <int PARTS>
+__device__ __forceinline__ void parts_of(uint4 (&to)[PARTS], const float (&f)[8]) {
     Split2 p[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = split2<2>(f[2 * j], f[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) p[j] = split2<PARTS>(f[2 * j], f[2 * j + 1]);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) to[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
+    for (int j = 0; j < PARTS; ++j) to[j] = make_uint4(p[0].part[j], p[1].part[j], p[2].part[j], p[3].part[j]);
 }
 
 template <int D, bool FP16>
@@ -1326,7 +1324,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
                 if constexpr (FP16) {
                     float f[8];
                     unpack16<true>(o[x][0], f);
-                    two_parts(reinterpret_cast<uint4 (&)[2]>(o[x]), f);
+                    parts_of(reinterpret_cast<uint4 (&)[2]>(o[x]), f);
                 }
             }
             uint4 u[2][3], r[2][3];
@@ -1422,14 +1420,14 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
             }
             by_row = butterfly_step32(butterfly_step16(by_row));
             if (g == 0) lds.row[half][own] = by_row;
-            uint4 parts[2];
+            uint4 parts[3];
             const int block = lower_block(half, tile);
-            two_parts(parts, x1);
-            lds.m.frag[0][block][0][lane] = parts[0];
-            lds.m.frag[0][block][1][lane] = parts[1];
-            two_parts(parts, x2);
-            lds.m.frag[1][block][0][lane] = parts[0];
-            lds.m.frag[1][block][1][lane] = parts[1];
+            parts_of(parts, x1);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) lds.m.frag[0][block][p][lane] = parts[p];
+            parts_of(parts, x2);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) lds.m.frag[1][block][p][lane] = parts[p];
         } else if (g == 0) {
             lds.row[half][own] = 0.0f;
         }
@@ -1449,14 +1447,14 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
             }
             by_col = butterfly_step32(butterfly_step16(by_col));
             if (g == 0) lds.col[half][own] = by_col;
-            uint4 parts[2];
+            uint4 parts[3];
             const int block = upper_block(half, tile);
-            two_parts(parts, x1);
-            lds.m.frag[2][block][0][lane] = parts[0];
-            lds.m.frag[2][block][1][lane] = parts[1];
-            two_parts(parts, x2);
-            lds.m.frag[3][block][0][lane] = parts[0];
-            lds.m.frag[3][block][1][lane] = parts[1];
+            parts_of(parts, x1);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) lds.m.frag[2][block][p][lane] = parts[p];
+            parts_of(parts, x2);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) lds.m.frag[3][block][p][lane] = parts[p];
         } else if (g == 0) {
             lds.col[half][own] = 0.0f;
         }
@@ -1502,20 +1500,19 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
                 for (int kind = 0; kind < 4; ++kind) {
                     if (kind < 2 ? 2 * ks > tile : 2 * ks + 1 < tile) continue;
                     const int block = kind < 2 ? lower_block(ks, tile) : upper_block(ks, tile);
-                    uint4 f[2];
-                    f[0] = lds.m.frag[kind][block][0][lane];
-                    f[1] = lds.m.frag[kind][block][1][lane];
 #pragma unroll
-                    for (int t = 0; t < TPQ; ++t)
+                    for (int y = 0; y < 3; ++y) {
+                        const uint4 f = lds.m.frag[kind][block][y][lane];
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
+                        for (int t = 0; t < TPQ; ++t)
 #pragma unroll
-                            for (int y = 0; y + p < 2; ++y) {
-                                if (kind == 0) so[x][t] = mfma16x16x32(f[y], kt[t][ks][p], so[x][t]);
-                                if (kind == 1) sr[x][t] = mfma16x16x32(f[y], kt[t][ks][p], sr[x][t]);
-                                if (kind == 2) su[x][t] = mfma16x16x32(f[y], qt[t][ks][p], su[x][t]);
-                                if (kind == 3) su[x][t] = mfma16x16x32(f[y], kt[t][ks][p], su[x][t]);
+                            for (int p = 0; p < PARTS && p + y < 3; ++p) {
+                                if (kind == 0) so[x][t] = mfma16x16x32(f, kt[t][ks][p], so[x][t]);
+                                if (kind == 1) sr[x][t] = mfma16x16x32(f, kt[t][ks][p], sr[x][t]);
+                                if (kind == 2) su[x][t] = mfma16x16x32(f, qt[t][ks][p], su[x][t]);
+                                if (kind == 3) su[x][t] = mfma16x16x32(f, kt[t][ks][p], su[x][t]);
                             }
+                    }
                 }
             }
 #pragma unroll
@@ -1621,7 +1618,7 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
     const size_t by_head = static_cast<size_t>(w.slots) * a.heads, by_key = static_cast<size_t>(w.slots) * a.key_heads;
     const size_t transposed = by_key * (a.dim / 16) * 2 * w.parts * kFragBytes;
     w.t = take(by_head * kBlocks * 3 * kFragBytes);
-    w.p = take(by_head * kBlocks * (grad ? 3 : 2) * kFragBytes);
+    w.p = take(by_head * kBlocks * 3 * kFragBytes);
     w.vec = reinterpret_cast<float*>(take(by_head * 256 * sizeof(float)));
     w.kt = take(transposed);
     w.kf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
