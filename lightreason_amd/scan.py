@@ -189,6 +189,12 @@ def _scan(form, tensors, taped=False):
     return out, final, tape
 
 
+def _aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
+    """t, or a contiguous copy where it begins off the kernels' alignment (one that
+    is contiguous by its strides stays where it is under ``contiguous``)."""
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % to else t
+
+
 class _DeltaScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, form, *tensors):
@@ -210,9 +216,10 @@ class _DeltaScan(torch.autograd.Function):
             first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
             return None, *zeros, None, first
         a = _native.DeltaScanArgs.from_buffer_copy(template)
-        if any(t.stride() != s for t, s in zip((query, key, value, g, beta), ctx.strides)):
+        if any(t.stride() != s or t.data_ptr() % 16 and t.dim() == 3
+               for t, s in zip((query, key, value, g, beta), ctx.strides)):
             # Hooks on saved tensors (those that keep them on the host) have laid them out anew.
-            query, key, value, g, beta = (t.contiguous() for t in (query, key, value, g, beta))
+            query, key, value, g, beta = (_aligned(t.contiguous()) for t in (query, key, value, g, beta))
             a.q_token_stride, a.q_head_stride = _strides(query)
             a.k_token_stride, a.k_head_stride = _strides(key)
             a.v_token_stride, a.v_head_stride = _strides(value)
@@ -220,12 +227,13 @@ class _DeltaScan(torch.autograd.Function):
         _addresses(a, query, key, value, g, beta, starts)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value, g, beta)]
         first = torch.empty(shape, dtype=torch.float32, device=dev) if ctx.first and need[7] else None
-        d = _native.DeltaGradArgs(tape=tape[0].data_ptr(), d_initial=_ptr(first))
-        # Of a gradient that torch hands in, expanded or transposed, a plain copy is taken.
-        bad = d_out.stride(-1) != 1 or d_out.data_ptr() % 16 or any(x % 8 or not 0 <= x < 1 << 23 for x in d_out.stride()[:-1])
-        d_out = d_out.contiguous() if bad else d_out
-        d_final = d_final.contiguous()
-        d_final = d_final.clone() if d_final.data_ptr() % 16 else d_final
+        tape = _aligned(tape[0], 256)
+        d = _native.DeltaGradArgs(tape=tape.data_ptr(), d_initial=_ptr(first))
+        # Of a gradient that torch hands in, expanded, transposed or cut from a longer
+        # one at any element, a plain copy is taken.
+        if d_out.stride(-1) != 1 or any(x % 8 or not 0 <= x < 1 << 23 for x in d_out.stride()[:-1]):
+            d_out = d_out.contiguous()
+        d_out, d_final = _aligned(d_out), _aligned(d_final.contiguous())
         d.d_out_token_stride, d.d_out_head_stride = _strides(d_out)
         d.d_final = d_final.data_ptr()
         if a.tokens:

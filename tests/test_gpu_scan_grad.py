@@ -259,3 +259,37 @@ def test_a_training_step_in_a_graph(device):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lead", [1, 3, 8])
+def test_gradients_that_begin_at_any_element(device, lead):
+    """Results that are joined to something else: their gradients are pieces of a
+    longer one, contiguous and off any alignment."""
+    x = R.inputs([70, 20], 2, 4, 64, 64, BF, 17)
+    leaves = [x[n].detach().requires_grad_() for n in NAMES]
+    gen = torch.Generator().manual_seed(4)
+    out, final = delta_scan(*leaves, x["starts"])
+    weight = torch.randn(lead + out.numel(), generator=gen).to(BF).to(device)
+    more = torch.randn(lead + final.numel(), generator=gen).to(device)
+    want = torch.autograd.grad([out, final], leaves, [weight[lead:].view_as(out).clone(),
+                                                      more[lead:].view_as(final).clone()], retain_graph=True)
+    joined = [torch.cat([w.new_zeros(lead), t.flatten()]) for w, t in ((weight, out), (more, final))]
+    for a, b in zip(torch.autograd.grad(joined, leaves, [weight, more]), want):
+        assert torch.equal(a, b)
+
+
+def test_saved_tensors_kept_in_pieces_of_a_longer_one(device):
+    """Hooks that hand everything back off its alignment, in its own layout or
+    another."""
+    x = R.inputs([70, 20], 2, 4, 64, 64, BF, 18)
+    d_out = torch.randn(x["value"].shape, generator=torch.Generator().manual_seed(3)).to(BF).to(device)
+    for leaves in ([x[n].detach().requires_grad_() for n in NAMES],
+                   [x[n].detach().clone(memory_format=torch.contiguous_format).requires_grad_() for n in NAMES]):
+        want = torch.autograd.grad(delta_scan(*leaves, x["starts"])[0], leaves, d_out)
+
+        def unpack(t):
+            return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            out, _ = delta_scan(*leaves, x["starts"])
+        for a, b in zip(torch.autograd.grad(out, leaves, d_out), want):
+            assert torch.equal(a, b)

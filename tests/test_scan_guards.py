@@ -153,3 +153,13 @@ def test_page_fork_refuses_host_tensors_and_shapes():
         pool.fork(torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="GPU|cpu"):
         pool.fork(torch.zeros(2, dtype=torch.int32))
+
+
+def test_gradients_off_the_alignment_are_copied():
+    whole = torch.arange(64, dtype=BF)
+    assert whole.data_ptr() % 16 == 0 and scan._aligned(whole) is whole
+    piece = whole[3:51].view(2, 3, 8)
+    assert piece.is_contiguous() and piece.contiguous().data_ptr() % 16
+    for t in (piece, piece.transpose(0, 1), piece[:1, :1].expand(4, 2, 8)):
+        copy = scan._aligned(t)
+        assert copy.data_ptr() % 16 == 0 and copy.is_contiguous() and torch.equal(copy, t)
