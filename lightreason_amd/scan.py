@@ -30,6 +30,7 @@ import sys
 from contextlib import contextmanager
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .paged import _TYPES, _int, _on, _ptr, _require, _stream, _strided, _strides
@@ -142,7 +143,7 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     and strides that are multiples of 8.
 
     Gradients flow to query, key, value, g, beta and initial, once (no second
-    derivatives); they take the same bits every time.  For them the call keeps
+    and no forward-mode derivatives: inputs with tangents are refused); they take the same bits every time.  For them the call keeps
     the states before every 64 tokens and u, 4 (dim + 64) value_dim / 64 bytes a
     token and head.  The gradient of a sequence with values that are not finite
     is not defined.  A captured training step takes its gradients with
@@ -161,9 +162,19 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
         a.out_token_stride, a.out_head_stride = a.heads * a.value_dim, a.value_dim
         form = a, dev, shape
         _native.remember(_SCANS, key_, form)
+    if _has_tangents(tensors):
+        raise NotImplementedError("delta_scan has no forward-mode derivatives")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return _DeltaScan.apply(form, *tensors)
     return _scan(form, tensors)[:2]
+
+
+def _has_tangents(tensors) -> bool:
+    """Whether any tensor is a dual one of torch.autograd.forward_ad, which does not
+    show in requires_grad.  (Outside its levels, with a torch that tells, 5 us
+    less a call.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _SCANS: dict = {}   # arguments of a form (types, shapes, strides) that was checked, without the addresses

@@ -293,3 +293,19 @@ def test_saved_tensors_kept_in_pieces_of_a_longer_one(device):
             out, _ = delta_scan(*leaves, x["starts"])
         for a, b in zip(torch.autograd.grad(out, leaves, d_out), want):
             assert torch.equal(a, b)
+
+
+def test_forward_mode_derivatives_are_refused(device):
+    """A result without a tangent would be a derivative of zero."""
+    x = R.inputs([70, 3], 2, 4, 64, 64, BF, 19)
+    want = delta_scan(**x)
+    initial = R.states(2, 4, 64, 64, 3)
+    for name in NAMES + ("initial",):
+        with torch.autograd.forward_ad.dual_level():
+            base = initial if name == "initial" else x[name]
+            dual = torch.autograd.forward_ad.make_dual(base, torch.ones_like(base))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    delta_scan(**{**x, name: dual})
+            got = delta_scan(**x)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -163,3 +163,13 @@ def test_gradients_off_the_alignment_are_copied():
     for t in (piece, piece.transpose(0, 1), piece[:1, :1].expand(4, 2, 8)):
         copy = scan._aligned(t)
         assert copy.data_ptr() % 16 == 0 and copy.is_contiguous() and torch.equal(copy, t)
+
+
+def test_dual_tensors_are_told_apart():
+    x = [torch.zeros(2, 3), None, torch.zeros(3, dtype=torch.int32)]
+    assert not scan._has_tangents(x)
+    with torch.autograd.forward_ad.dual_level():
+        assert not scan._has_tangents(x)
+        dual = torch.autograd.forward_ad.make_dual(x[0], torch.ones(2, 3))
+        assert scan._has_tangents([*x, dual]) and not dual.requires_grad
+    assert not scan._has_tangents([*x, dual])
