@@ -711,7 +711,7 @@ int lrmoe_delta_scan(const lrmoe_delta_scan_args *args, void *workspace, size_t 
 
 /* The gradient of lrmoe_delta_scan: args as in the forward call, which was given
  * a tape of lrmoe_delta_scan_tape_bytes(args) bytes (256-byte aligned; the
- * states before every 64 tokens and the rows u, in fp32) and
+ * states before every 64 tokens and the rows v - S^T k, in fp32) and
  * whose slots and pool are the sequences themselves (slots, into and fresh NULL,
  * pool = seqs); initial, final and out are not read.  From the gradients of out
  * and (d_final, may be NULL) of final it writes those of q, k, v, g, beta and

@@ -24,7 +24,7 @@ struct ScanArgs {
     float* final;
     uint16_t* out;
     int64_t out_token, out_head;
-    uint8_t* tape;   // what the gradient needs: the chunks' first states and u, or NULL
+    uint8_t* tape;   // what the gradient needs: the chunks' first states and w, or NULL
 };
 struct ScanGradArgs {
     const uint16_t* d_out;
@@ -71,32 +71,27 @@ constexpr int kFragBytes = 1024;
 __host__ __device__ __forceinline__ constexpr int lower_block(int ks, int w) { return ks == 0 ? w : 2 + w; }
 __host__ __device__ __forceinline__ constexpr int upper_block(int ks, int w) { return ks == 1 ? w : 4 + w; }
 
+constexpr int kVec = 4 * kChunk + 64;   // (whole cache lines)
+
 // What the first launch leaves the second, per chunk slot and value head (or
 // key head), in this order in the workspace.
 struct ScanChunks {
     int slots, parts;      // parts: bf16 numbers that a q or k is (1, or 2 for fp16)
     uint8_t *t, *p;        // [slots][heads]: 3 parts of 6 blocks
-    float* vec;            // [slots][heads][256]: factors of K S, of Q S and of K^T U per token, then the chunk's decay
+    float* vec;            // [slots][heads][kVec]: factors of K S, of Q S, of K^T U and beta per token, then the chunk's decay
     uint8_t *kt, *qt;      // [slots][key_heads][dim / 16][2][parts]: K^T, and for the gradient Q^T
     uint8_t *kf, *qf;      // [slots][key_heads][4][dim / 32][parts]: rows of K, and for the outputs of Q
     uint32_t* flags;       // [seqs][heads][value_dim / 16]
     // For the gradient: t and p hold the transposed matrices, and
     double* sums;          // [slots][heads][64]: running sums of g
     float* norms;          // [slots][key_heads][128]: factors of k and of q
-    float *ds, *dr;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
+    float *ds, *du;        // [slots][heads][dim][value_dim], [slots][heads][64][value_dim]
     f32x4* pairs;          // [slots][key_heads][4][512]: q . k and k . k, by threads
 };
 
-// Where a gradient is wanted a beta of 0 is taken as 2^-40: u = beta w then still
-// tells w, which beta's gradient is made of; what that adds is 2^-40 of what a
-// beta of 1 would.
-__device__ __forceinline__ float scan_beta(float b) {
-    return __builtin_fabsf(b) < 0x1p-40f ? __builtin_copysignf(0x1p-40f, b) : b;
-}
-
 __host__ __device__ __forceinline__ int scan_slots(int tokens, int seqs) { return tokens / kChunk + seqs; }
-// The tape, fp32: states [slots][heads][dim][value_dim], then u [slots][heads][64]
-// [value_dim].
+// The tape, fp32: states [slots][heads][dim][value_dim], then w [slots][heads][64]
+// [value_dim] (u = beta w).
 __host__ __device__ __forceinline__ int64_t tape_states(int64_t slots, int heads, int dim, int value_dim) {
     return slots * heads * dim * value_dim;
 }

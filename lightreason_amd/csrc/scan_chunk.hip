@@ -6,7 +6,7 @@
 //     out_i = scale e^(G_i) S^T q_i + sum_j P_ij u_j,
 //     S <- e^(G_63) S + sum_j e^(G_63 - G_j) k_j u_j^T.
 // Launch one computes what does not depend on the state for all chunks at once:
-// T = beta (I + L beta)^-1, P and the factors.  Launch two goes through a
+// T = (I + L beta)^-1, P and the factors.  Launch two goes through a
 // sequence's chunks one after another, per value head and block of columns.
 //
 // Products are of bf16 matrix instructions with nothing rounded: q and k are
@@ -275,16 +275,17 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
             const bool in = lane < count;   // (rows past the sequence repeat its last one)
             const double sum = wave_scan_f64(in ? scan_log(raw_g) * 1.4426950408889634 : 0.0);
             lds.sum[wave][lane] = sum;
-            lds.beta[wave][lane] = !in ? 0.0f : GRAD || a.tape != nullptr ? scan_beta(beta) : beta;
+            lds.beta[wave][lane] = in ? beta : 0.0f;
             if (hv + wave < a.group) {
                 if constexpr (GRAD) w.sums[(by_head + wave) * kChunk + lane] = sum;
                 const double last = __shfl(sum, kWave - 1);
                 const float decay = power(sum), rest = power(last - sum);
-                float* vec = w.vec + (by_head + wave) * 256;
+                float* vec = w.vec + (by_head + wave) * kVec;
                 vec[lane] = in ? decay * lds.rk[lane] : 0.0f;
                 vec[64 + lane] = in ? decay * lds.rq[lane] * a.scale : 0.0f;
                 vec[128 + lane] = in ? rest * lds.rk[lane] : 0.0f;
-                if (lane == kWave - 1) vec[192] = decay;
+                vec[192 + lane] = in ? beta : 0.0f;
+                if (lane == kWave - 1) vec[256] = decay;
             }
             load_gates(hv + 4);
             __syncthreads();
@@ -300,7 +301,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * wave + 4 * g + r;
                 fade[t][r] = power(sums[i] - sums[j]) * lds.rk[j];
-                lds.a[i * kPitch + j] = j < i ? fade[t][r] * lds.rk[i] * betas[j] * kk[t][r] : 0.0f;
+                // (The gradient's T is (I + beta L)^-1: T beta is the same.)
+                lds.a[i * kPitch + j] = j < i ? fade[t][r] * lds.rk[i] * betas[GRAD ? i : j] * kk[t][r] : 0.0f;
             }
         }
         __syncthreads();
@@ -308,12 +310,12 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
         // A fragment of the wave's rows (for the gradient: of its columns) is eight
         // numbers of a lane.
         const int row = 16 * wave + n;
-        auto eight = [&](const float* m, int ks, float (&x)[8], auto&& factor) {
+        auto eight = [&](const float* m, int ks, float (&x)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int o = 32 * ks + 16 * (j / 4) + 4 * g + j % 4, block = 2 * ks + j / 4;
                 const bool in = GRAD ? block >= wave : block <= wave;
-                x[j] = in ? m[GRAD ? o * kPitch + row : row * kPitch + o] * factor(GRAD ? o : row) : 0.0f;
+                x[j] = in ? m[GRAD ? o * kPitch + row : row * kPitch + o] : 0.0f;
             }
         };
         const int64_t blocks = by_head * kBlocks;
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
         for (int ks = 0; ks < 2; ++ks) {
             if (GRAD ? 2 * ks + 1 < wave : 2 * ks > wave) continue;
             float x[8];
-            eight(lds.t, ks, x, [&](int i) { return betas[i]; });
+            eight(lds.t, ks, x);
             const int64_t block = blocks + (GRAD ? upper_block(ks, wave) : lower_block(ks, wave));
             store_parts<3>(w.t + block * 3 * kFragBytes + lane * 16, x);
         }
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
         for (int ks = 0; ks < 2; ++ks) {
             if (GRAD ? 2 * ks + 1 < wave : 2 * ks > wave) continue;
             float x[8];
-            eight(lds.a, ks, x, [](int) { return 1.0f; });
+            eight(lds.a, ks, x);
             const int64_t block = blocks + (GRAD ? upper_block(ks, wave) : lower_block(ks, wave));
             store_parts<3>(w.p + block * 3 * kFragBytes + lane * 16, x);
         }
@@ -453,7 +455,7 @@ struct ScanLds {
     uint4 uk[3][2][NC][kWave];   // times the factors of K^T U
     // What waves 8 to 11 have read for waves 0 to 3.
     uint4 k[4][D / 32 * PARTS][kWave], t[4][6][kWave], kt[4][D / 64 * 2 * PARTS][kWave];
-    f32x4 vec[2][3][16];         // the factors, of two chunks
+    f32x4 vec[2][4][16];         // the factors, of two chunks
     float decay[2];
     uint32_t v[4][4][kWave];
     int odd[4];                  // whether a wave has met a number that is not finite
@@ -520,9 +522,9 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                 kt[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
         };
         auto load_values = [&](int ch) {
-            const float* from = w.vec + ((slot0 + ch) * a.heads + h) * 256;
-            vec = *reinterpret_cast<const f32x4*>(from + 64 * min(wave, 2) + 4 * n);
-            decay = from[192];
+            const float* from = w.vec + ((slot0 + ch) * a.heads + h) * kVec;
+            vec = *reinterpret_cast<const f32x4*>(from + 64 * wave + 4 * n);
+            decay = from[256];
             const uint8_t* at = reinterpret_cast<const uint8_t*>(a.v + static_cast<int64_t>(seq.a + ch * kChunk) * a.v_token +
                                                                  h * a.v_head + col0);
 #pragma unroll
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             for (int i = 0; i < KS * PARTS; ++i) lds.k[wave][i][lane] = k[i / PARTS][i % PARTS];
 #pragma unroll
             for (int i = 0; i < 4; ++i) lds.v[wave][i][lane] = v[i];
-            if (wave < 3 && g == 0) lds.vec[ch % 2][wave][n] = vec;
+            if (g == 0) lds.vec[ch % 2][wave][n] = vec;
             if (wave == 3) lds.decay[ch % 2] = decay;
         };
         auto put_t = [&] {
@@ -665,7 +667,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                                    : a.initial[(static_cast<int64_t>(from) * a.heads + h) * size +
                                                static_cast<int64_t>(row_of(x) + i) * a.value_dim + col + c];
     float* tape_s = reinterpret_cast<float*>(a.tape);
-    float* tape_u = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
+    float* tape_w = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
     __builtin_amdgcn_s_setprio(2);
     if (lane == 0) lds.odd[wave] = 0;
     bool odd = false;   // a number that is not finite
@@ -693,6 +695,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                     for (int x = 0; x < PARTS && x + p < 3; ++x) r[c] = mfma16x16x32(k[i * PARTS + x], b, r[c]);
                 }
         const f32x4 fk = lds.vec[ch % 2][0][4 * wave + g], fu = lds.vec[ch % 2][2][4 * wave + g];
+        const f32x4 beta = lds.vec[ch % 2][3][4 * wave + g];
         const float decay = lds.decay[ch % 2];
         uint32_t v[4];
 #pragma unroll
@@ -709,9 +712,9 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             for (int i = 0; i < TPW; ++i) put_rows<NC>(to + row_of(i) * a.value_dim, a.value_dim, S[i]);
         }
         __syncthreads();
-        f32x4 u[NC];
+        f32x4 bare[NC];   // w: u before its beta
 #pragma unroll
-        for (int c = 0; c < NC; ++c) u[c] = zero;
+        for (int c = 0; c < NC; ++c) bare[c] = zero;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (2 * i > wave) continue;
@@ -724,18 +727,19 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                 for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.r[p][i][c][lane];
 #pragma unroll
-                    for (int x = 0; x + p < 3; ++x) u[c] = mfma16x16x32(t[x], b, u[c]);
+                    for (int x = 0; x + p < 3; ++x) bare[c] = mfma16x16x32(t[x], b, bare[c]);
                 }
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            put_parts<3>(lds.u, wave / 2, wave % 2, c, lane, u[c]);
-            put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u[c] * fu);
+            const f32x4 u = bare[c] * beta;
+            put_parts<3>(lds.u, wave / 2, wave % 2, c, lane, u);
+            put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u * fu);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[c][i]) & 0x7f800000u) == 0x7f800000u;
+            for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[i]) & 0x7f800000u) == 0x7f800000u;
         }
         if constexpr (TAPE)
-            put_rows<NC>(tape_u + (((slot0 + ch) * a.heads + h) * kChunk + r0) * a.value_dim + col, a.value_dim, u);
+            put_rows<NC>(tape_w + (((slot0 + ch) * a.heads + h) * kChunk + r0) * a.value_dim + col, a.value_dim, bare);
         __syncthreads();
         uint4 kt[TPW * 2 * PARTS];
 #pragma unroll
@@ -776,7 +780,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
 // ---- the gradient: chunk after chunk, backwards -----------------------------------
 
 // With dS the gradient of the state after a chunk and do that of its outputs,
-//     X_j = sum_i P_ij do_i + e^(G_63 - G_j) dS^T k_j,     dR = (beta (I + L beta)^-1)^T X = dv,
+//     X_j = sum_i P_ij do_i + e^(G_63 - G_j) dS^T k_j,     du = ((I + beta L)^-1)^T X,     dR = beta du = dv,
 //     dS <- e^(G_63) dS + sum_i scale e^(G_i) q_i do_i^T - sum_i e^(G_i) k_i dR_i^T:
 // the forward launch with the matrices transposed, for the same columns. Waves 0
 // to 3 have the chain; waves 4 to 7 compute the two sums over do, which need no
@@ -847,7 +851,7 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
             to[i / (2 * PARTS)][i / PARTS % 2][i % PARTS] = frag16(at + i * kFragBytes, frag);
     };
     auto factors = [&](int ch, int kind) {
-        return *reinterpret_cast<const f32x4*>(w.vec + ((slot0 + ch) * a.heads + h) * 256 + 64 * kind + r0);
+        return *reinterpret_cast<const f32x4*>(w.vec + ((slot0 + ch) * a.heads + h) * kVec + 64 * kind + r0);
     };
     if (role >= 4) {
         if (chunks == 0) return;
@@ -958,7 +962,7 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
             for (int c = 0; c < NC; ++c)
                 S[x][c][i] = d.d_final != nullptr ? d.d_final[state_at(x) + i * a.value_dim + c] : 0.0f;
     uint4 k[KS][PARTS], tt[2][3], kt[TPW][2][PARTS];
-    f32x4 fk, fu;
+    f32x4 fk, fu, beta;
     float decay = 0.0f;
     auto load_k = [&](int ch) {
         fu = factors(ch, 2);
@@ -968,10 +972,11 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
     };
     auto load_t = [&](int ch) {
         fk = factors(ch, 0);
+        beta = factors(ch, 3);
         load_blocks(tt, w.t, ch);
     };
     auto load_rest = [&](int ch) {
-        decay = w.vec[((slot0 + ch) * a.heads + h) * 256 + 192];
+        decay = w.vec[((slot0 + ch) * a.heads + h) * kVec + 256];
         load_transposed(kt, w.kt, ch);
     };
     if (chunks > 0) {
@@ -1019,9 +1024,9 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
             for (int i = 0; i < TPW; ++i) put_rows<NC>(to + row_of(i) * a.value_dim, a.value_dim, S[i]);
         }
         __syncthreads();
-        f32x4 dr[NC];
+        f32x4 du[NC], dr[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dr[c] = zero;
+        for (int c = 0; c < NC; ++c) du[c] = zero;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (2 * i + 1 < wave) continue;
@@ -1031,15 +1036,18 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
                 for (int c = 0; c < NC; ++c) {
                     const uint4 b = lds.x[p][i][c][lane];
 #pragma unroll
-                    for (int r = 0; r + p < 3; ++r) dr[c] = mfma16x16x32(tt[i][r], b, dr[c]);
+                    for (int r = 0; r + p < 3; ++r) du[c] = mfma16x16x32(tt[i][r], b, du[c]);
                 }
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) put_parts<3>(lds.rk, wave / 2, wave % 2, c, lane, -(dr[c] * fk));
+        for (int c = 0; c < NC; ++c) {
+            dr[c] = du[c] * beta;
+            put_parts<3>(lds.rk, wave / 2, wave % 2, c, lane, -(dr[c] * fk));
+        }
         __builtin_amdgcn_sched_barrier(0);
         load_t(next);
         __builtin_amdgcn_sched_barrier(0);
-        put_rows<NC>(w.dr + (by_head * kChunk + r0) * a.value_dim + col, a.value_dim, dr);
+        put_rows<NC>(w.du + (by_head * kChunk + r0) * a.value_dim + col, a.value_dim, du);
         {
             const int left = seq.n - ch * kChunk;
             uint16_t* to = d.dv + (static_cast<int64_t>(seq.a + ch * kChunk + r0) * a.heads + h) * a.value_dim + col;
@@ -1082,7 +1090,8 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
 //     dq_i = scale (e^(G_i) S do_i + sum_j B1_ij k_j),
 //     dk_i = -(e^(G_i) S dR_i + sum_j B2_ij k_j) + e^(G_63 - G_i) dS u_i
 //            + sum_j (B1_ji scale q_j - B2_ji k_j).
-// dbeta_i = w_i . du_i = u_i . dR_i / beta_i^2.  A decay g_t acts on what passes
+// dbeta_i = w_i . du_i.  What is read are w and du, so that a beta of 0 has its
+// gradient too; u = beta w and dR = beta du are factors of rows.  A decay g_t acts on what passes
 // from before t to t or later: its gradient is, with M_ij = scale B1_ij q_i . k_j
 // - B2_ij k_i . k_j,
 //     sum_(i >= t) e^(G_i) (scale q_i . S do_i - k_i . S dR_i) + sum_(j < t) e^(G_63 - G_j) k_j . dS u_j
@@ -1092,10 +1101,10 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
 //
 // A workgroup has a chunk and a key head and goes through its value heads.  Its
 // eight waves have two row tiles (of 16 tokens) and a quarter of the columns of
-// dq and dk each. What is fp32 (S, dS, u, dR) is read once by the workgroup, 32
+// dq and dk each. What is fp32 (S, dS, w, du) is read once by the workgroup, 32
 // columns at a time, split into three bf16 numbers and shared through LDS, the
 // next 32 while the products of those before run (training step of 4000 tokens:
-// 300 -> 257 us): the decays' gradient is fp32 and as exact as that. Bound by its one workgroup per CU: 208 KB of S, dS, u and dR per chunk and
+// 300 -> 257 us): the decays' gradient is fp32 and as exact as that. Bound by its one workgroup per CU: 208 KB of S, dS, w and du per chunk and
 // value head come at 1.3 TB/s.
 constexpr int kGradThreads = 512;
 template <int D>
@@ -1235,15 +1244,15 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
         const int h = kh * a.group + hv;
         const int64_t by_head = static_cast<int64_t>(slot) * a.heads + h;
         const float* tape = reinterpret_cast<const float*>(d.tape);
-        // The wave's share of a step's staging: a tile of S and dS, one of u or dR.
+        // The wave's share of a step's staging: a tile of S and dS, one of w or du.
         const bool has_tile = wave < TILES;
         const uint32_t tile_at = 4 * (element_of(wave) * E + 8 * g), rows_at = 4 * ((16 * (wave % 4) + n) * E + 8 * g);
         const uint8_t* at_s = bytes(tape + by_head * size);
         const uint8_t* at_ds = bytes(w.ds + by_head * size);
-        const uint8_t* at_rows = bytes(wave < 4 ? tape + states + by_head * rows : w.dr + by_head * rows);
+        const uint8_t* at_rows = bytes(wave < 4 ? tape + states + by_head * rows : w.du + by_head * rows);
         const uint16_t* out = d.d_out + static_cast<int64_t>(t0) * d.d_out_token + h * d.d_out_head;
-        // S do, S dR and dS u of the wave's rows and columns; of do . u (the first
-        // two quarters) and dR . u the tiles of its rows and every other column.
+        // S do, S du and dS w of the wave's rows and columns; of do . w (the first
+        // two quarters) and du . w the tiles of its rows and every other column.
         f32x4 so[2][TPQ], sr[2][TPQ], su[2][TPQ], xu[2][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -1384,7 +1393,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
             lds.sum[tid] = sum;
             lds.decay[tid] = power(sum);
             lds.rest[tid] = power(last - sum);
-            lds.beta[tid] = scan_beta(a.beta_fp32 ? __uint_as_float(raw_beta) : elem16<FP16>(static_cast<uint16_t>(raw_beta)));
+            const float beta = a.beta_fp32 ? __uint_as_float(raw_beta) : elem16<FP16>(static_cast<uint16_t>(raw_beta));
+            lds.beta[tid] = tid < count ? beta : 0.0f;   // (rows past the sequence have a w)
         }
         __syncthreads();   // (the staging is done with)
         {
@@ -1403,13 +1413,15 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
         const float own_q = lds.rq[own] * a.scale, own_k = lds.rk[own];
         if (2 * half <= tile) {
             const double own_sum = lds.sum[own];
+            const float own_beta = lds.beta[own];
             float by_row = 0.0f, x1[8], x2[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int o = 32 * half + 16 * (j / 4) + 4 * g + j % 4, at = own * kPitch + o;
                 const float fade = power(own_sum - lds.sum[o]), rk = lds.rk[o], raw2 = lds.m.b2[at];
-                if (o == own) lds.dbeta[own] = raw2 / lds.beta[own] / lds.beta[own];
-                const float b1 = o <= own ? fade * lds.m.b1[at] : 0.0f, b2 = o < own ? fade * raw2 : 0.0f;
+                if (o == own) lds.dbeta[own] = raw2;
+                const float beta = fade * lds.beta[o];
+                const float b1 = o <= own ? beta * lds.m.b1[at] : 0.0f, b2 = o < own ? beta * own_beta * raw2 : 0.0f;
                 lds.m.b1[at] = b1;
                 lds.m.b2[at] = b2;
                 const float m = b1 * of_qk[j / 4][j % 4] * (own_q * rk) - b2 * of_kk[j / 4][j % 4] * (own_k * rk);
@@ -1477,8 +1489,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
 #pragma unroll
                 for (int t = 0; t < TPQ; ++t) {
                     so[x][t][i] *= lds.decay[row];
-                    sr[x][t][i] *= lds.decay[row];
-                    su[x][t][i] *= lds.rest[row];
+                    sr[x][t][i] *= lds.decay[row] * lds.beta[row];
+                    su[x][t][i] *= lds.rest[row] * lds.beta[row];
                     of_q = __builtin_fmaf(raw(q[x][t], i), so[x][t][i], of_q);
                     of_k = __builtin_fmaf(raw(k[x][t], i), sr[x][t][i], of_k);
                     of_u = __builtin_fmaf(raw(k[x][t], i), su[x][t][i], of_u);
@@ -1619,7 +1631,7 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
     const size_t transposed = by_key * (a.dim / 16) * 2 * w.parts * kFragBytes;
     w.t = take(by_head * kBlocks * 3 * kFragBytes);
     w.p = take(by_head * kBlocks * 3 * kFragBytes);
-    w.vec = reinterpret_cast<float*>(take(by_head * 256 * sizeof(float)));
+    w.vec = reinterpret_cast<float*>(take(by_head * kVec * sizeof(float)));
     w.kt = take(transposed);
     w.kf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);
     if (grad) {
@@ -1628,7 +1640,7 @@ ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t
         w.sums = reinterpret_cast<double*>(take(by_head * kChunk * sizeof(double)));
         w.norms = reinterpret_cast<float*>(take(by_key * 2 * kChunk * sizeof(float)));
         w.ds = reinterpret_cast<float*>(take(by_head * a.dim * columns));
-        w.dr = reinterpret_cast<float*>(take(by_head * kChunk * columns));
+        w.du = reinterpret_cast<float*>(take(by_head * kChunk * columns));
         w.pairs = reinterpret_cast<f32x4*>(take(by_key * 4 * kGradThreads * sizeof(f32x4)));
     } else {
         w.qf = take(by_key * 4 * (a.dim / 32) * w.parts * kFragBytes);

@@ -309,3 +309,32 @@ def test_forward_mode_derivatives_are_refused(device):
                     delta_scan(**{**x, name: dual})
             got = delta_scan(**x)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("n", [9, 140])
+def test_steps_without_weight_before_growth(device, n):
+    """A beta of 0 is exactly 0 with a tape too: what it leaves out stays out,
+    however much a state grows after it, and its value's gradient is 0; its own
+    gradient is that of w."""
+    x = R.inputs([n], 2, 2, 64, 64, BF, 14)
+    at = n // 2
+    x["beta"][:at + 1] = 0.0
+    x["beta"][-1] = 0.0
+    x["value"][at] = 100.0
+    x["g"][at + 1] = 30.0
+    initial = R.states(1, 2, 64, 64, 1) * 0
+    leaves = [x[k].detach().requires_grad_() for k in NAMES]
+    out, final = (t.detach() for t in delta_scan(*leaves, x["starts"]))
+    assert not out[:at + 1].any()
+    if n > 40:   # (shorter ones go token by token without a tape, which rounds elsewhere)
+        plain = delta_scan(**x)
+        assert torch.equal(out, plain[0]) and torch.equal(final, plain[1])
+    # A state of zero, until the first step with a weight.
+    after = {k: v[at + 1:] for k, v in x.items() if k != "starts"}
+    after["starts"] = torch.tensor([0, n - at - 1], dtype=torch.int32, device=device)
+    want, last, size = R.rule(after, initial)
+    b_out, b_final = R.bounds(after, want, size)
+    R.check("after out", out[at + 1:], want, b_out)
+    R.check("after final", final, last, b_final)
+    got = _check(x, initial)
+    assert not got[2][:at + 1].any() and not got[2][-1].any() and got[2][at + 1:-1].any()
