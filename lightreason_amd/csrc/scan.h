@@ -2,6 +2,8 @@
 // (scan.hip: token by token; scan_chunk.hip: in chunks, and the gradient).
 #pragma once
 
+#include <algorithm>
+
 #include "lrmoe_device.h"
 #include "lrmoe_internal.h"
 #include "paged.h"
@@ -37,7 +39,7 @@ struct ScanGradArgs {
     float* d_initial;
 };
 hipError_t launch_delta_scan(ScanArgs a, bool fp16, int max_new, void* workspace, hipStream_t stream);
-size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new);
+size_t delta_scan_workspace_bytes(ScanArgs a, bool fp16, int max_new);
 
 size_t delta_scan_tape_bytes(const ScanArgs& a);
 size_t delta_scan_grad_workspace_bytes(const ScanArgs& a, bool fp16);
@@ -52,12 +54,21 @@ hipError_t launch_scan_chunks(const ScanArgs& a, bool fp16, void* workspace, con
 // ---- chunks ------------------------------------------------------------------
 //
 // Sequences are cut into chunks of 64 tokens.  Sequence s has the chunk slots
-// from starts[s] / 64 + s on (rounded down): ceil(n / 64) of them never reach
-// the next sequence's, whatever the counts, and tokens / 64 + seqs hold all, so
-// that slots need no scan over the sequences.
+// from min(starts[s] / c, starts[s] / 64 + s) on (rounded down), with c the fewest
+// tokens of a sequence that goes in chunks, 32 at most: with n >= c tokens either
+// number grows by ceil(n / 64) or more up to the next sequence, so that slots
+// never meet, whatever the counts, and need no scan over the sequences.  Those of
+// the tokens' end are enough for all: empty sequences and those that go token by
+// token cost none where there are few tokens.
 constexpr int kChunk = 64;
 
-__device__ __forceinline__ int scan_first_chunk(const int32_t* starts, int s) { return (starts[s] >> 6) + s; }
+__host__ __device__ __forceinline__ int scan_slot_tokens(const ScanArgs& a) { return a.token_wise < 31 ? a.token_wise + 1 : 32; }
+__device__ __forceinline__ int scan_first_chunk(const ScanArgs& a, int s) {
+    return min(a.starts[s] / scan_slot_tokens(a), (a.starts[s] >> 6) + s);
+}
+__host__ __forceinline__ int scan_slots(const ScanArgs& a) {
+    return std::max(std::min(a.tokens / scan_slot_tokens(a), a.tokens / kChunk + a.seqs), 1);
+}
 
 // Fragments of 16 bytes per lane, as the matrix instructions' A operands.  The
 // tokens of a chunk, where they are summed over, come in this order: step ks
@@ -89,7 +100,6 @@ struct ScanChunks {
     f32x4* pairs;          // [slots][key_heads][4][512]: q . k and k . k, by threads
 };
 
-__host__ __device__ __forceinline__ int scan_slots(int tokens, int seqs) { return tokens / kChunk + seqs; }
 // The tape, fp32: states [slots][heads][dim][value_dim], then w [slots][heads][64]
 // [value_dim] (u = beta w).
 __host__ __device__ __forceinline__ int64_t tape_states(int64_t slots, int heads, int dim, int value_dim) {

@@ -159,8 +159,9 @@ static int token_wise(const ScanArgs& a) {
     return static_cast<int64_t>(a.seqs) * a.heads * (a.value_dim / 32) <= 1024 ? 24 : 40;
 }
 
-size_t delta_scan_workspace_bytes(const ScanArgs& a, bool fp16, int max_new) {
-    return max_new <= token_wise(a) ? 0 : scan_chunk_bytes(a, fp16);
+size_t delta_scan_workspace_bytes(ScanArgs a, bool fp16, int max_new) {
+    a.token_wise = token_wise(a);
+    return max_new <= a.token_wise ? 0 : scan_chunk_bytes(a, fp16);
 }
 
 hipError_t launch_delta_scan(ScanArgs a, bool fp16, int max_new, void* workspace, hipStream_t stream) {

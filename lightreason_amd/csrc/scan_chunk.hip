@@ -35,12 +35,12 @@ __device__ __forceinline__ f32x4 mfma_raw(uint4 a, uint4 b, f32x4 c) {
 
 // The sequence whose chunk slots hold slot c (the last one that begins at or
 // before it), a wave at a time: 64 of them are looked at in one step.
-__device__ __forceinline__ int find_sequence(const int32_t* starts, int seqs, int c) {
-    int lo = 0, hi = seqs;
+__device__ __forceinline__ int find_sequence(const ScanArgs& a, int c) {
+    int lo = 0, hi = a.seqs;
     while (hi - lo > 1) {
         const int step = (hi - lo + kWave - 1) / kWave;
         const int at = lo + (static_cast<int>(__lane_id()) + 1) * step;
-        const bool before = at < hi && scan_first_chunk(starts, at) <= c;
+        const bool before = at < hi && scan_first_chunk(a, at) <= c;
         const int n = __popcll(__ballot(before));
         lo += n * step;
         hi = min(lo + step, hi);
@@ -164,9 +164,9 @@ __global__ __launch_bounds__(kThreads, 4) void scan_prepare(ScanArgs a, ScanChun
     const int tid = threadIdx.x, lane = tid % kWave, n = lane % 16, g = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
-    const int s = find_sequence(a.starts, a.seqs, slot);
+    const int s = find_sequence(a, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
-    const int first = (slot - scan_first_chunk(a.starts, s)) * kChunk;
+    const int first = (slot - scan_first_chunk(a, s)) * kChunk;
     if (first < 0 || first >= seq.n || seq.n <= a.token_wise) return;
     const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
     // g and beta of the wave's head among four.
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
         return;
     }
     const int chunks = (seq.n + kChunk - 1) / kChunk;
-    const int64_t slot0 = scan_first_chunk(a.starts, s);
+    const int64_t slot0 = scan_first_chunk(a, s);
     // Addresses are a scalar base per chunk and offsets of 32 bits; rows past the
     // sequence repeat its last one (their factors are 0, and their u).
     const int r0 = 16 * wave + 4 * g;
@@ -832,7 +832,7 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
         if (s == a.seqs - 1) clear(tail, a.tokens);
     }
     const int chunks = (seq.n + kChunk - 1) / kChunk;
-    const int64_t slot0 = scan_first_chunk(a.starts, s);
+    const int64_t slot0 = scan_first_chunk(a, s);
     const int r0 = 16 * wave + 4 * g;
     const uint32_t frag = lane * 16;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1150,9 +1150,9 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
     int lane = tid % kWave, n = lane % 16, g = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), pair = wave % 2, quarter = wave / 2;
     const int slot = blockIdx.x / a.key_heads, kh = blockIdx.x % a.key_heads;
-    const int s = find_sequence(a.starts, a.seqs, slot);
+    const int s = find_sequence(a, slot);
     const ScanSeq seq = scan_seq(a.starts, s, a.tokens);
-    const int first = (slot - scan_first_chunk(a.starts, s)) * kChunk;
+    const int first = (slot - scan_first_chunk(a, s)) * kChunk;
     if (first < 0 || first >= seq.n) return;
     const int count = min(seq.n - first, kChunk), t0 = seq.a + first;
     const int64_t by_key = static_cast<int64_t>(slot) * a.key_heads + kh;
@@ -1619,7 +1619,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void scan_inputs_grad(ScanArgs a, 
 
 ScanChunks layout(const ScanArgs& a, bool fp16, bool grad, uint8_t* base, size_t* bytes) {
     ScanChunks w{};
-    w.slots = scan_slots(a.tokens, a.seqs);
+    w.slots = scan_slots(a);
     w.parts = fp16 ? 2 : 1;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -1694,7 +1694,7 @@ hipError_t launch_scan_chunks(const ScanArgs& a, bool fp16, void* workspace, con
 }
 
 size_t delta_scan_tape_bytes(const ScanArgs& a) {
-    return static_cast<size_t>(scan_slots(a.tokens, a.seqs)) * a.heads * (a.dim + kChunk) * a.value_dim * sizeof(float);
+    return static_cast<size_t>(scan_slots(a)) * a.heads * (a.dim + kChunk) * a.value_dim * sizeof(float);
 }
 
 size_t delta_scan_grad_workspace_bytes(const ScanArgs& a, bool fp16) {

@@ -143,12 +143,14 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     and strides that are multiples of 8.
 
     Gradients flow to query, key, value, g, beta and initial, once (no second
-    and no forward-mode derivatives: inputs with tangents are refused); they take the same bits every time.  For them the call keeps
-    the states before every 64 tokens and v - S^T k, 4 (dim + 64) value_dim / 64 bytes a
-    token and head.  The gradient of a sequence with values that are not finite
-    is not defined.  A captured training step takes its gradients with
-    torch.autograd.grad, or from leaves of which no eager graph lives
-    (torch's rule for every captured backward pass)."""
+    and no forward-mode derivatives: inputs with tangents are refused); they
+    take the same bits every time.  For them the call keeps the states before
+    every 64 tokens and v - S^T k: 4 (dim + 64) value_dim bytes a head for every
+    64 tokens, and once more for every sequence (in all no more than for every
+    token).  The gradient of a sequence with values that are not finite is not
+    defined.  A captured training step takes its gradients with
+    torch.autograd.grad, or from leaves of which no eager graph lives (torch's
+    rule for every captured backward pass)."""
     if scale is not None:
         scale = float(scale)
     tensors = (query, key, value, g, beta, starts, initial)

@@ -327,3 +327,21 @@ def test_heads_and_tokens_in_any_order_and_repeated_rows(device):
     y["value"] = x["value"].transpose(0, 1).contiguous().transpose(0, 1)
     y["beta"] = x["beta"][:1].expand(90, 4)
     _compare("expanded", y, delta_scan(**y), R.states(1, 4, 64, 64, 1) * 0)
+
+
+def test_counts_around_the_edges_of_chunks_and_forms(device):
+    """Slots of one sequence right behind another's, empty ones and short ones between,
+    in few heads (from 25 tokens on in chunks) and in many (from 41)."""
+    lengths = [25, 0, 65, 1, 26, 24, 64, 0, 0, 41, 40, 129, 42, 63, 3, 32, 33, 128]
+    for H in (2, 64):
+        x = R.inputs(lengths, 2, H, 64, 32, BF, 84, lead=5)
+        initial = R.states(len(lengths), H, 64, 32, 5)
+        _compare(f"{H} heads", x, delta_scan(**x, initial=initial), initial)
+
+
+def test_a_batch_padded_with_empty_sequences(device):
+    x = R.inputs([70, 30, 1] + [0] * 3000, 2, 2, 64, 64, BF, 85)
+    initial = R.states(3003, 2, 64, 64, 5)
+    got = delta_scan(**x, initial=initial)
+    _compare("padded", x, got, initial)
+    assert torch.equal(got[1][3:], initial[3:])

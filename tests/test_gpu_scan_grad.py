@@ -338,3 +338,11 @@ def test_steps_without_weight_before_growth(device, n):
     R.check("after final", final, last, b_final)
     got = _check(x, initial)
     assert not got[2][:at + 1].any() and not got[2][-1].any() and got[2][at + 1:-1].any()
+
+
+def test_gradients_of_a_padded_batch_and_of_single_tokens(device):
+    """Slots of sequences that are empty, or of one token each."""
+    for lengths in ([70, 30, 1] + [0] * 500, [1, 2, 1, 0, 1, 3, 1, 1, 65, 1, 64, 1]):
+        x = R.inputs(lengths, 2, 2, 64, 64, BF, 86)
+        got = _check(x, R.states(len(lengths), 2, 64, 64, 5))
+        assert got[5].shape[0] == len(lengths)

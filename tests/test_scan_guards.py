@@ -173,3 +173,44 @@ def test_dual_tensors_are_told_apart():
         dual = torch.autograd.forward_ad.make_dual(x[0], torch.ones(2, 3))
         assert scan._has_tangents([*x, dual]) and not dual.requires_grad
     assert not scan._has_tangents([*x, dual])
+
+
+def test_scratch_and_tape_hold_a_slot_per_chunk_or_token():
+    """A slot per 64 tokens and per sequence, but no more than there are tokens (of
+    sequences that go in chunks: 25 each)."""
+    lib = _native.library()
+
+    def sizes(tokens, seqs, **kw):
+        a = _native.DeltaScanArgs(**{**dict(seqs=seqs, tokens=tokens, max_new=tokens, heads=2, key_heads=1, dim=64,
+                                            value_dim=32, pool=seqs), **kw})
+        return [getattr(lib, f"lrmoe_delta_scan_{n}_bytes")(C.byref(a)) for n in ("tape", "grad_workspace", "workspace")]
+    tape, grad, _ = sizes(1, 1)
+    assert tape == 2 * (64 + 64) * 32 * 4
+    for tokens, seqs in ((6400, 3), (8, 1000), (64, 1), (63, 1), (1000, 1000), (0, 5)):
+        slots = max(1, min(tokens, tokens // 64 + seqs))
+        assert sizes(tokens, seqs)[0] == tape * slots
+        assert sizes(tokens, seqs)[1] <= grad * slots
+    # Without a tape: 256 single tokens have no chunk, padding takes none.
+    one = sizes(100, 1)[2]
+    assert sizes(256, 256)[2] < 8 * one and sizes(100, 60000)[2] < 4 * one + 4 * 60000 * 2 * 2 + 256
+
+
+def test_chunk_slots_never_meet():
+    """The kernels' rule for a sequence's first slot, over counts around its edges."""
+    import random
+    rng = random.Random(3)
+    first = lambda start, s, c: min(start // c, start // 64 + s)
+    for token_wise in (0, 24, 40):   # (sequences of up to so many tokens have none)
+        c = min(token_wise + 1, 32)
+        edges = [0, 0, 1, 2, token_wise, token_wise + 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 300]
+        for _ in range(2000):
+            counts = [rng.choice(edges) for _ in range(rng.choice([1, 3, 10, 80]))]
+            at, used = rng.choice([0, 1, 63, 64, 500]), 0
+            tokens = at + sum(counts) + rng.choice([0, 7])
+            for s, n in enumerate(counts):
+                if n > token_wise:
+                    assert first(at, s, c) >= used
+                    used = first(at, s, c) + (n + 63) // 64
+                    assert used <= first(at + n, s + 1, c)
+                at += n
+            assert used <= min(tokens // c, tokens // 64 + len(counts))
