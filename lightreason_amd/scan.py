@@ -110,10 +110,17 @@ def _scratch(a) -> int:
     return int(_native.library().lrmoe_delta_scan_workspace_bytes(C.addressof(a)))
 
 
-def _launch(a, dev, nbytes):
+def _launch(a, dev, nbytes, scratch=None):
+    """``scratch``: where the call's memory comes from, the thread's own by
+    default.  That stays; whole sequences and their gradient, of any length and the
+    latter on a thread of autograd's, take theirs from torch for the call."""
     with _on(dev):
-        ws = _native.workspace(dev, nbytes) if nbytes else None
+        ws = (scratch or _native.workspace)(dev, nbytes) if nbytes else None
         _native.call("lrmoe_delta_scan", C.addressof(a), _ptr(ws), nbytes, _stream(dev))
+
+
+def _for_the_call(dev, nbytes):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 # ---- whole sequences ------------------------------------------------------------
@@ -198,7 +205,7 @@ def _scan(form, tensors, taped=False):
         nbytes = int(_native.library().lrmoe_delta_scan_tape_bytes(C.addressof(a)))
         tape = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         a.tape = tape.data_ptr()
-    _launch(a, dev, _scratch(a))
+    _launch(a, dev, _scratch(a), _for_the_call)
     return out, final, tape
 
 
@@ -253,7 +260,7 @@ class _DeltaScan(torch.autograd.Function):
             d.d_out, d.dq, d.dk, d.dv, d.dg, d.dbeta = (t.data_ptr() for t in (d_out, *grads))
         with _on(dev):
             nbytes = int(_native.library().lrmoe_delta_scan_grad_workspace_bytes(C.addressof(a)))
-            ws = _native.workspace(dev, nbytes)
+            ws = _for_the_call(dev, nbytes)
             _native.call("lrmoe_delta_scan_grad", C.addressof(a), C.addressof(d), ws.data_ptr(), ws.numel(),
                          _stream(dev))
         return None, *(t if n else None for t, n in zip(grads, need[1:6])), None, first

@@ -346,3 +346,17 @@ def test_gradients_of_a_padded_batch_and_of_single_tokens(device):
         x = R.inputs(lengths, 2, 2, 64, 64, BF, 86)
         got = _check(x, R.states(len(lengths), 2, 64, 64, 5))
         assert got[5].shape[0] == len(lengths)
+
+
+def test_a_training_step_leaves_no_memory_behind(device):
+    """Scratch of whole sequences goes back to torch, the backward pass's on its own
+    thread too."""
+    x = R.inputs([3000], 2, 4, 128, 128, BF, 87)
+    leaves = [x[n].detach().requires_grad_() for n in NAMES]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(2):
+        out, final = delta_scan(*leaves, x["starts"])
+        grads = torch.autograd.grad([out, final], leaves, [torch.ones_like(out), torch.ones_like(final)])
+        del out, final, grads
+    assert torch.cuda.memory_allocated() - before < 1 << 20
