@@ -52,6 +52,22 @@ def _per_head(t, name, dtypes, shape, dev):
         raise ValueError(f"{name} needs a contiguous last dimension")
 
 
+def _beyond(N, S, K, H, D, E) -> str | None:
+    """What of these sizes the kernels cannot do, if anything."""
+    if D not in HEAD_DIMS:
+        return f"query must have a head width of 64 or 128, got {D}"
+    if K < 1:
+        return "query has no heads"
+    if H < 1 or H % K:
+        return f"value must have a multiple of the {K} key heads, got {H}"
+    if E % 32 or not 32 <= E <= 256:
+        return f"value must have a head width that is a multiple of 32 up to 256, got {E}"
+    if S > 65536 or N > 1 << 20 or N * H > 1 << 26 or H > 1024 or S * H * E > 1 << 27:
+        return (f"at most 65536 sequences, 2^20 tokens, 1024 heads, tokens * heads of 2^26 and sequences * heads * "
+                f"width of 2^27, got {S}, {N}, {H}, {N * H} and {S * H * E}")
+    return None
+
+
 def _check(query, key, value, g, beta, starts, normalize, scale):
     """Checks what every call has; returns the argument structure with sizes
     and strides, and the device."""
@@ -61,31 +77,26 @@ def _check(query, key, value, g, beta, starts, normalize, scale):
     dtype, dev = query.dtype, query.device
     if dtype not in _TYPES:
         raise ValueError(f"query must be bfloat16 or float16, got {dtype}")
-    if D not in HEAD_DIMS:
-        raise ValueError(f"query must have a head width of 64 or 128, got {D}")
+    if (text := _beyond(0, 0, K, K, D, 32)) is not None:
+        raise ValueError(text)
     if dev.type != "cuda":
         raise ValueError(f"query must be on a GPU, got {dev}")
-    if K < 1:
-        raise ValueError("query has no heads")
     _strided(query, "query", 8)
     _rows(key, "key", N, dtype, dev)
     if tuple(key.shape) != (N, K, D):
         raise ValueError(f"key must have shape {(N, K, D)}, got {tuple(key.shape)}")
     _rows(value, "value", N, dtype, dev)
     H, E = value.shape[1:]
-    if H < 1 or H % K:
-        raise ValueError(f"value must have a multiple of the {K} key heads, got {H}")
-    if E % 32 or not 32 <= E <= 256:
-        raise ValueError(f"value must have a head width that is a multiple of 32 up to 256, got {E}")
+    if (text := _beyond(0, 0, K, H, D, E)) is not None:
+        raise ValueError(text)
     _per_head(g, "g", (torch.float32,), (N, H), dev)
     _per_head(beta, "beta", (torch.float32, dtype), (N, H), dev)
     if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] < 1:
         raise ValueError("starts must be int32 [seqs + 1]")
     S = starts.shape[0] - 1
     _require(starts, "starts", (torch.int32,), (S + 1,), dev)
-    if S > 65536 or N > 1 << 20 or N * H > 1 << 26 or H > 1024 or S * H * E > 1 << 27:
-        raise ValueError(f"at most 65536 sequences, 2^20 tokens, 1024 heads, tokens * heads of 2^26 and sequences * heads * "
-                         f"width of 2^27, got {S}, {N}, {H}, {N * H} and {S * H * E}")
+    if (text := _beyond(N, S, K, H, D, E)) is not None:
+        raise ValueError(text)
     a = _native.DeltaScanArgs(seqs=S, tokens=N, max_new=N, heads=H, key_heads=K, dim=D, value_dim=E,
                               fp16=int(dtype == torch.float16), normalize=int(bool(normalize)),
                               beta_fp32=int(beta.dtype == torch.float32), scale=D ** -0.5 if scale is None else scale)
@@ -340,21 +351,47 @@ def _check_step(query, key, value, g, beta, starts, states, slots, into, fresh, 
 
 # ---- under a Transformers model -------------------------------------------------
 
+def _takes(query, key, value, g, beta, initial) -> bool:
+    """Whether ``delta_scan`` does a layer's call, of [batch, tokens, heads, width]."""
+    if query.device.type != "cuda" or query.dtype not in _TYPES or any(t.dim() != 4 for t in (query, key, value)):
+        return False
+    batch, tokens, K, D = query.shape
+    H, E = value.shape[2:]
+    return (key.dtype == value.dtype == query.dtype and key.shape == query.shape
+            and value.shape[:2] == query.shape[:2] and g.shape == beta.shape == value.shape[:3]
+            and all(t.device == query.device for t in (key, value, g, beta))
+            and (initial is None or initial.device == query.device and initial.shape == (batch, H, D, E))
+            and _beyond(batch * tokens, batch, K, H, D, E) is None
+            and not _has_tangents((query, key, value, g, beta, initial)))
+
+
+def _laid_out(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where the kernels cannot read its rows in place."""
+    if t.stride(-1) != 1:
+        return t.clone(memory_format=torch.contiguous_format)
+    if t.dim() == 2:
+        return t
+    if any(x % 8 or x >= 1 << 23 for x in _strides(t)):
+        return t.clone(memory_format=torch.contiguous_format)
+    return _aligned(t)
+
+
 @contextmanager
 def fused_scan(model):
     """Run the recurrence of every linear-attention layer's prompt and training
     forward as one ``delta_scan`` call for the duration of the block, gradients
     included: what the layers hand to ``torch_chunk_gated_delta_rule`` of their
     Transformers module, any batch and any length.  (The function is the
-    module's, so other models of the class run through it meanwhile.)  Tensors
-    on the CPU, of another type than bf16 and fp16 or of several, and calls with
-    ``cu_seqlens``, run as before; a call holds up to 2^20 tokens."""
+    module's, so other models of the class run through it meanwhile.)  What
+    ``delta_scan`` does not do runs as before: tensors on the CPU, of another type
+    than bf16 and fp16 or of several, widths and sizes beyond its own, calls with
+    ``cu_seqlens`` and forward-mode derivatives.  Rows that it could not read in
+    place are copied."""
     name = "torch_chunk_gated_delta_rule"
     def native(original):
         def rule(query, key, value, g, beta, chunk_size=64, initial_state=None, output_final_state=False,
                  use_qk_l2norm_in_kernel=False, **kwargs):
-            if (query.device.type != "cuda" or query.dtype not in _TYPES or key.dtype != query.dtype
-                    or value.dtype != query.dtype or kwargs.get("cu_seqlens") is not None):
+            if kwargs.get("cu_seqlens") is not None or not _takes(query, key, value, g, beta, initial_state):
                 return original(query, key, value, g=g, beta=beta, chunk_size=chunk_size, initial_state=initial_state,
                                 output_final_state=output_final_state, use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel,
                                 **kwargs)
@@ -362,9 +399,8 @@ def fused_scan(model):
             starts = torch.arange(batch + 1, dtype=torch.int32, device=query.device) * tokens
             beta = beta if beta.dtype == query.dtype else beta.float()
             rows = [x.reshape(batch * tokens, *x.shape[2:]) for x in (query, key, value, g.float(), beta)]
-            first = None if initial_state is None else initial_state.float().contiguous()
-            out, final = delta_scan(*(x if x.stride(-1) == 1 else x.contiguous() for x in rows), starts, initial=first,
-                                    normalize=use_qk_l2norm_in_kernel)
+            first = None if initial_state is None else _aligned(initial_state.float().contiguous())
+            out, final = delta_scan(*map(_laid_out, rows), starts, initial=first, normalize=use_qk_l2norm_in_kernel)
             return out.view(batch, tokens, *out.shape[1:]), final if output_final_state else None
 
         rule.lrmoe_native = True

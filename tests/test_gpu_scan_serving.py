@@ -265,3 +265,95 @@ def test_fused_scan_and_fused_delta_fill_one_cache(model, device):
     for a, b in zip(states, after):
         assert a.shape == (1, 32, 128, 128) and not torch.equal(a, b) and torch.isfinite(b).all()
     assert torch.isfinite(logits).all()
+
+
+def _layers_of(rule):
+    """A model of one linear-attention layer whose module's rule is ``rule``."""
+    import sys
+    import types
+
+    module = types.ModuleType("lrmoe_test_layers")
+    module.torch_chunk_gated_delta_rule = rule
+    Mixer = type("Mixer", (), {"__module__": module.__name__})
+    sys.modules[module.__name__] = module
+    layer = types.SimpleNamespace(linear_attn=Mixer())
+    return module, types.SimpleNamespace(model=types.SimpleNamespace(layers=[layer]))
+
+
+def _layer_call(D, E, device, dtype=BF, T=70):
+    x = R.inputs([2 * T], 3, 3, D, E, dtype, 92)
+    return {n: t.unflatten(0, (2, T)) for n, t in x.items() if n != "starts"}
+
+
+@pytest.mark.parametrize("case", ["width 96", "values of 48", "fp32", "several types", "cu_seqlens", "tangents"])
+def test_fused_scan_leaves_other_calls_to_the_stock_rule(device, case):
+    given = []
+
+    def stock(query, key, value, g, beta, chunk_size=64, initial_state=None, output_final_state=False,
+              use_qk_l2norm_in_kernel=False, **kwargs):
+        given.append((query, key, value, g, beta, initial_state, kwargs))
+        return "stock", None
+    module, model = _layers_of(stock)
+    x = _layer_call(96 if case == "width 96" else 64, 48 if case == "values of 48" else 64, device,
+                    torch.float32 if case == "fp32" else BF)
+    more = {}
+    if case == "several types":
+        x["value"] = x["value"].half()
+    if case == "cu_seqlens":
+        more["cu_seqlens"] = torch.tensor([0, 70], device=device)
+    with torch.autograd.forward_ad.dual_level(), fused_scan(model):
+        if case == "tangents":
+            x["value"] = torch.autograd.forward_ad.make_dual(x["value"], torch.ones_like(x["value"]))
+        assert module.torch_chunk_gated_delta_rule is not stock
+        assert module.torch_chunk_gated_delta_rule(**x, output_final_state=True, **more)[0] == "stock"
+    assert module.torch_chunk_gated_delta_rule is stock and len(given) == 1
+    assert all(a is b for a, b in zip(given[0], (x[n] for n in ("query", "key", "value", "g", "beta"))))
+    assert given[0][5] is None and given[0][6].keys() == more.keys()
+
+
+def test_fused_scan_copies_rows_that_cannot_be_read_in_place(device):
+    def stock(*args, **kw):
+        raise AssertionError("not native")
+    module, model = _layers_of(stock)
+    x = _layer_call(64, 64, device)
+    first = R.states(2, 3, 64, 64, 4)
+    with fused_scan(model):
+        want = module.torch_chunk_gated_delta_rule(**x, initial_state=first, output_final_state=True)
+        y = dict(x)
+        for n in ("query", "key", "value"):   # off any alignment; strides of 68; heads' elements apart
+            t = x[n]
+            y[n] = {"query": torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape),
+                    "key": torch.cat([t, t[..., :4]], -1)[..., :64],
+                    "value": t.transpose(2, 3).contiguous().transpose(2, 3)}[n]
+        y["g"], y["beta"] = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (x["g"], x["beta"]))
+        shifted = torch.cat([first.new_zeros(1), first.flatten()])[1:].view(first.shape)
+        got = module.torch_chunk_gated_delta_rule(**y, initial_state=shifted, output_final_state=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@torch.no_grad()
+def test_a_prompts_cached_states_are_the_scans(model, device, monkeypatch):
+    """What fused_scan leaves in the cache, bit for bit, and what it should be."""
+    from transformers.cache_utils import DynamicCache
+
+    import lightreason_amd.scan as scan
+    from lightreason_amd.delta import _live
+
+    cfg, m = model
+    calls = []
+
+    def spy(*args, **kw):
+        calls.append((args, kw, delta_scan(*args, **kw)))
+        return calls[-1][2]
+    monkeypatch.setattr(scan, "delta_scan", spy)
+    ids = torch.randint(0, 512, (1, 60), generator=torch.Generator().manual_seed(5)).to(device)
+    with fused_scan(m):
+        cache = DynamicCache(config=cfg)
+        m(ids, past_key_values=cache, use_cache=True)
+    states = [_live(layer.recurrent_states) for layer in cache.layers if hasattr(layer, "recurrent_states")]
+    assert len(states) == len(calls) == 3
+    for state, (args, kw, (out, final)) in zip(states, calls):
+        assert torch.equal(state, final)
+        x = dict(zip(("query", "key", "value", "g", "beta", "starts"), args))
+        want, last, size = R.rule(x, torch.zeros_like(final), normalize=kw["normalize"])
+        R.check("state", state, last, R.bounds(x, want, size, normalize=kw["normalize"])[1])

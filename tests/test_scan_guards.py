@@ -214,3 +214,39 @@ def test_chunk_slots_never_meet():
                     assert used <= first(at + n, s + 1, c)
                 at += n
             assert used <= min(tokens // c, tokens // 64 + len(counts))
+
+
+def test_fused_scan_tells_what_it_takes():
+    class Shape:   # what is looked at of a tensor
+        def __init__(self, *shape, dtype=BF, device="cuda"):
+            self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
+
+        def dim(self):
+            return len(self.shape)
+
+    def call(B=2, T=10, K=4, H=4, D=64, E=64, **kw):
+        q, k, v, g, beta = (Shape(B, T, K, D), Shape(B, T, K, D), Shape(B, T, H, E), Shape(B, T, H, dtype=torch.float32),
+                            Shape(B, T, H))
+        args = dict(query=q, key=k, value=v, g=g, beta=beta, initial=None)
+        return scan._takes(**{**args, **kw})
+    assert call() and call(E=256, H=8) and call(D=128, initial=Shape(2, 4, 128, 64, dtype=torch.float32))
+    for kw in (dict(D=96), dict(D=256), dict(E=48), dict(E=288), dict(K=3), dict(T=1 << 20), dict(K=1026, H=1026),
+               dict(B=65537, T=1), dict(query=Shape(2, 10, 4, 64, device="cpu")), dict(key=Shape(2, 10, 4, 64, dtype=torch.half)),
+               dict(value=Shape(2, 10, 4, 64, dtype=torch.float32)), dict(query=Shape(2, 10, 4, 64, dtype=torch.float32)),
+               dict(key=Shape(2, 9, 4, 64)), dict(g=Shape(2, 10, 4, dtype=torch.float32, device="cpu")),
+               dict(initial=Shape(2, 4, 64, 128, dtype=torch.float32)), dict(query=Shape(10, 4, 64))):
+        assert not call(**kw), kw
+
+
+def test_rows_that_cannot_be_read_in_place_are_copied():
+    whole = torch.randn(5 * 3 * 80 + 8).to(BF)
+    good = whole[8:8 + 5 * 3 * 80].view(5, 3, 80)[:, :, :64]
+    assert scan._laid_out(good) is good
+    off = whole[3:3 + 5 * 3 * 64].view(5, 3, 64)
+    narrow = whole[:5 * 3 * 68].view(5, 3, 68)[:, :, :64]
+    turned = whole[:5 * 3 * 64].view(5, 64, 3).transpose(1, 2)
+    for t in (off, narrow, turned):
+        copy = scan._laid_out(t)
+        assert copy is not t and copy.is_contiguous() and copy.data_ptr() % 16 == 0 and torch.equal(copy, t)
+    g = torch.randn(5, 9)[:, 1:4]
+    assert scan._laid_out(g) is g
