@@ -761,9 +761,11 @@ int lrmoe_beam_select(int groups, int beams, int vocab, int type, const void *lo
  * parent stays; so does one whose parent lies outside [0, rows) or is not its
  * own parent (nothing that is read is written).  tensors (on the host, as its
  * numbers) holds a base address, the rows' stride and the bytes of a row, three
- * int64 per tensor; at most LRMOE_FORK_TENSORS of them, and 2^24 pieces of
- * 32 KB, rows' last ones included. */
+ * int64 per tensor; at most LRMOE_FORK_TENSORS of them, and fewer than
+ * LRMOE_FORK_PIECES pieces of LRMOE_FORK_BYTES, rows' last ones included. */
 #define LRMOE_FORK_TENSORS 64
+#define LRMOE_FORK_BYTES 32768
+#define LRMOE_FORK_PIECES (1 << 24)
 int lrmoe_fork_rows(int rows, const int32_t *parents, int tensors, const int64_t *table, void *stream);
 
 /* Row r of a page pool takes over the cached positions of row parents[r] where

@@ -140,6 +140,8 @@ class DeltaGradArgs(C.Structure):
 
 BEAM_MAX = 32            # beams of a group
 FORK_TENSORS = 64        # tensors of one lrmoe_fork_rows call
+FORK_BYTES = 32768       # its pieces of a row, of which a call has fewer than
+FORK_PIECES = 1 << 24
 FORK_CACHES = 32         # caches of one lrmoe_page_fork call
 PAGE_MAX_ROWS = 4096     # rows (sequences) of a page pool
 PAGE_MAX_POSITIONS = 1 << 30  # max_pages * page at most

@@ -107,7 +107,8 @@ def fork_rows(parents: torch.Tensor, tensors) -> None:
     the list counts rows, the others are contiguous within a row (any type;
     states of several layers as one tensor per layer).  A row that is its own
     parent stays; so does one whose parent lies outside 0 .. rows - 1 or is not
-    its own parent.  Tensors must not overlap."""
+    its own parent.  Tensors must not overlap.  A call that is refused has moved
+    nothing."""
     if isinstance(tensors, torch.Tensor):
         tensors = (tensors,)
     tensors = tuple(tensors)
@@ -150,8 +151,24 @@ def _check_rows(parents, tensors):
         if stride < nbytes:
             raise ValueError(f"tensor {i} has rows that overlap")
         layout.append((stride, nbytes))
-    parts = []   # of up to FORK_TENSORS tensors: the first, and the call's table but for the addresses
-    for i in range(0, len(tensors), _native.FORK_TENSORS):
-        part = layout[i:i + _native.FORK_TENSORS]
-        parts.append((i, (C.c_int64 * (3 * len(part)))(*[x for row in part for x in (0, *row)])))
-    return rows, dev, parts
+    # The parts' first tensors, and the calls' tables but for the addresses.
+    return rows, dev, [(i, (C.c_int64 * (3 * len(part)))(*[x for row in part for x in (0, *row)]))
+                       for i, part in _fork_parts(rows, layout)]
+
+
+def _fork_parts(rows, layout):
+    """(first, layouts) of the tensors of each library call: up to FORK_TENSORS of
+    them, and pieces that a call can count.  Refused is what does not fit one,
+    before anything is copied."""
+    parts, room = [], 0
+    for i, (stride, nbytes) in enumerate(layout):
+        pieces = -(-nbytes // _native.FORK_BYTES) * rows
+        if pieces >= _native.FORK_PIECES:
+            raise ValueError(f"tensor {i} has {pieces} pieces of {_native.FORK_BYTES} bytes, at most "
+                             f"{_native.FORK_PIECES - 1} fit a call")
+        if not parts or len(parts[-1][1]) == _native.FORK_TENSORS or pieces >= room:
+            parts.append((i, []))
+            room = _native.FORK_PIECES
+        parts[-1][1].append((stride, nbytes))
+        room -= pieces
+    return parts

@@ -1180,8 +1180,8 @@ int lrmoe_fork_rows(int rows, const int32_t* parents, int tensors, const int64_t
         a.t[i] = {reinterpret_cast<uint8_t*>(base), stride, bytes, 0, 0};
     }
     int64_t pieces = 0;
-    for (int i = 0; i < tensors; ++i) pieces += ((a.t[i].bytes + 32767) / 32768) * rows;
-    if (pieces >= (1 << 24)) return LRMOE_E_ARG;   // (a launch holds 2^32 threads)
+    for (int i = 0; i < tensors; ++i) pieces += ((a.t[i].bytes + LRMOE_FORK_BYTES - 1) / LRMOE_FORK_BYTES) * rows;
+    if (pieces >= LRMOE_FORK_PIECES) return LRMOE_E_ARG;   // (a launch holds 2^32 threads)
     if (int d = check_device()) return d;
     return status_of(lrmoe::launch_fork_rows(a, as_stream(stream)));
 }

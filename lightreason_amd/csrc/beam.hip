@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join(BeamArgs a) {
 
 // ---- rows that follow their parents ------------------------------------------
 
-constexpr int kForkBytes = 32768;   // of a row per workgroup
+constexpr int kForkBytes = LRMOE_FORK_BYTES;   // of a row per workgroup
 
 template <typename T>
 __device__ __forceinline__ void fork_copy(uint8_t* to, const uint8_t* from, int64_t bytes) {

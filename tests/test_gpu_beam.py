@@ -313,3 +313,20 @@ def test_many_rows(device):
     for r, p in enumerate(parents):
         for a, b in zip(_content(pool, caches, r), before[p]):
             assert torch.equal(a, b), r
+
+
+def test_forks_of_more_rows_than_a_call_counts(device):
+    """Tensors that need several calls by their pieces, and one that fits none: it
+    is refused, and nothing has moved."""
+    rows = 1 << 22
+    parents = torch.arange(rows, dtype=torch.int32, device=device)
+    parents[1::2] -= 1
+    tensors = [torch.randint(0, 2**15, (rows,), device=device, dtype=torch.int16) for _ in range(5)]
+    before = [t.clone() for t in tensors]
+    fork_rows(parents, tensors)
+    for t, b in zip(tensors, before):
+        assert torch.equal(t, b[parents.long()])
+    more = torch.zeros(1 << 24, 1, dtype=torch.uint8, device=device)
+    parents = torch.arange(1 << 24, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError, match="tensor 0 has"):
+        fork_rows(parents, [more])

@@ -250,3 +250,26 @@ def test_rows_that_cannot_be_read_in_place_are_copied():
         assert copy is not t and copy.is_contiguous() and copy.data_ptr() % 16 == 0 and torch.equal(copy, t)
     g = torch.randn(5, 9)[:, 1:4]
     assert scan._laid_out(g) is g
+
+
+def test_forks_are_cut_to_what_a_call_holds():
+    text = (Path(__file__).resolve().parents[1] / "include" / "lrmoe.h").read_text()
+    assert f"#define LRMOE_FORK_BYTES {_native.FORK_BYTES}\n" in text and "#define LRMOE_FORK_PIECES (1 << 24)\n" in text
+    assert _native.FORK_PIECES == 1 << 24
+    counts = lambda rows, layout: [(i, len(part)) for i, part in beam._fork_parts(rows, layout)]
+    assert counts(4, []) == [] and counts(0, [(8, 8)] * 3) == [(0, 3)] and counts(4, [(0, 0)] * 65) == [(0, 64), (64, 1)]
+    assert counts(4, [(64, 64)] * 130) == [(0, 64), (64, 64), (128, 2)]
+    # 2^18 - 1 rows: 64 pieces of a row fit a call, 65 do not.
+    rows, small, two = (1 << 18) - 1, (4, 4), (40000, 40000)
+    assert counts(rows, [small] * 64 + [small] * 62 + [two] + [small]) == [(0, 64), (64, 63), (127, 1)]
+    for rows, layout in ((rows, [two] * 70), (1 << 22, [small] * 9), (1, [(1 << 38, 1 << 38)] * 3)):
+        parts = beam._fork_parts(rows, layout)
+        assert [x for _, part in parts for x in part] == layout
+        assert [i for i, _ in parts] == [sum(len(part) for _, part in parts[:n]) for n in range(len(parts))]
+        for _, part in parts:
+            assert sum(-(-b // 32768) * rows for _, b in part) < 1 << 24
+    # One that fits no call, behind others, is refused before any of them.
+    with pytest.raises(ValueError, match="tensor 70 has"):
+        beam._fork_parts(1 << 18, [small] * 70 + [(1 << 21, 1 << 21)])
+    with pytest.raises(ValueError, match="tensor 0 has"):
+        beam._fork_parts(1 << 24, [(4, 4)])
