@@ -14,6 +14,13 @@ constexpr int kSlice = 2048;          // logits that a wave takes
 constexpr int kPer = kSlice / kWave;  // and a lane
 constexpr int kThreads = 256;
 constexpr int kJoinThreads = 512;
+// Candidates of a row (its slices' W best) that a lane of the join keeps in
+// registers, so that each of the W passes over them reads none from memory: up to 10,
+// 640 in all.  The join takes, with room for 10, 20 and 40 and always from memory:
+// 4 beams of 151936 (300 candidates) 6.1, 7.0, 9.8, 7.6 us; 8 beams (600) 9.6, 11.4,
+// 16.8, 19.0; 9 beams (675) 34, 17, 26, 34; 16 beams (1200) 98, 33, 49, 98; 32 beams
+// (2400) 713, 709, 196, 713: room that is not used costs searches of few beams as
+// much, in proportion, as it would spare those of many.
 constexpr int kKeep = 10;
 
 // A finite value and its token as one key: the larger value first, then the

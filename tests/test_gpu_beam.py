@@ -330,3 +330,29 @@ def test_forks_of_more_rows_than_a_call_counts(device):
     parents = torch.arange(1 << 24, dtype=torch.int32, device=device)
     with pytest.raises(ValueError, match="tensor 0 has"):
         fork_rows(parents, [more])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups,beams,vocab", [(1, 16, 151936), (2, 32, 50001), (1, 32, 151936), (1, 9, 151936),
+                                               (1, 8, 163840), (1, 8, 163841), (1, 1, 1400000)])
+def test_more_candidates_than_a_wave_keeps_in_registers(device, dtype, groups, beams, vocab):
+    """Slices times beams around and above what the join holds."""
+    logits = _logits(groups * beams, vocab, dtype, vocab + beams, device)
+    scores = (-torch.rand(groups, beams, generator=torch.Generator().manual_seed(beams)) * 6).to(device)
+    _check(logits, scores)
+    scores[:, 1:] = -INF    # a first step
+    _check(logits, scores)
+
+
+def test_ties_over_many_slices(device):
+    """Equal values in every slice, and a few that are larger far apart."""
+    logits = torch.randint(-2, 2, (32, 50001), generator=torch.Generator().manual_seed(2)).float().to(device)
+    logits[:, 40000] = logits[:, 7] = 3.0
+    logits[5:9] = 0.0
+    logits[9, :] = -INF
+    logits[9, ::4000] = 1.0
+    for dtype in (torch.float32, torch.bfloat16):
+        _check(logits.to(dtype), torch.zeros(1, 32, device=device))
+        scores = torch.full((1, 32), -INF, device=device)
+        scores[0, 9] = 0.0   # 13 continuations for 32 beams
+        _check(logits.to(dtype), scores)
