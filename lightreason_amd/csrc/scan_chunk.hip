@@ -670,7 +670,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
     float* tape_w = tape_s + tape_states(w.slots, a.heads, D, a.value_dim);
     __builtin_amdgcn_s_setprio(2);
     if (lane == 0) lds.odd[wave] = 0;
-    bool odd = false;   // a number that is not finite
+    bool odd = false;   // a number that is not finite, or whose first bf16 part may not be (from 2^127 on)
     for (int ch = 0; ch < chunks; ++ch) {
 #pragma unroll
         for (int i = 0; i < TPW; ++i)
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
             put_parts<3>(lds.u, wave / 2, wave % 2, c, lane, u);
             put_parts<3>(lds.uk, wave / 2, wave % 2, c, lane, u * fu);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[i]) & 0x7f800000u) == 0x7f800000u;
+            for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(u[i]) & 0x7f800000u) >= 0x7f000000u;
         }
         if constexpr (TAPE)
             put_rows<NC>(tape_w + (((slot0 + ch) * a.heads + h) * kChunk + r0) * a.value_dim + col, a.value_dim, bare);
@@ -761,6 +761,13 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
                         for (int x = 0; x < PARTS && x + p < 3; ++x) S[i][c] = mfma16x16x32(kt[(2 * i + j) * PARTS + x], b, S[i][c]);
                 }
     }
+    // (What u times its factor, or the last update, may have come to.)
+#pragma unroll
+    for (int x = 0; x < TPW; ++x)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= (__float_as_uint(S[x][c][i]) & 0x7f800000u) == 0x7f800000u;
     // Where a value was not finite, a product's zero weights have let it through
     // to earlier tokens: the next launch goes through these columns again.
     if (__ballot(odd) != 0 && lane == 0) lds.odd[wave] = 1;

@@ -345,3 +345,33 @@ def test_a_batch_padded_with_empty_sequences(device):
     got = delta_scan(**x, initial=initial)
     _compare("padded", x, got, initial)
     assert torch.equal(got[1][3:], initial[3:])
+
+
+@pytest.mark.parametrize("n", [6, 70])
+def test_values_next_to_the_end_of_fp32(device, n):
+    """u above bf16's largest number, and u e^G above fp32's with a key that is
+    small: outputs and states are finite."""
+    x = R.inputs([n], 2, 2, 64, 32, BF, 88, beta_dtype=torch.float32)
+    for t in ("query", "key", "value", "g"):
+        x[t].zero_()
+    x["beta"].fill_(1.0)
+    x["key"][n - 3, :, 0], x["query"][n - 2:, :, 0] = 1.0, 1.0
+    x["value"][n - 3] = torch.finfo(BF).max
+    x["beta"][n - 3] = 1.0025
+    initial = R.states(1, 2, 64, 32, 1) * 0
+    u = torch.finfo(BF).max * float(x["beta"][n - 3, 0])
+    assert 3.3962e38 < u < torch.finfo(torch.float32).max
+    got = delta_scan(**x, initial=initial, scale=2.0 ** -20)
+    want, last, _ = R.rule(x, initial, scale=2.0 ** -20)
+    R.check("large u out", got[0], want, R.half(BF) * want.abs() + 4 * 2.0 ** -24 * want.abs())
+    R.check("large u state", got[1], last, 4 * 2.0 ** -24 * last.abs())
+    # A key of 2^-20, then growth by e^5.
+    x["key"].mul_(2.0 ** -20)
+    x["value"].mul_(2.0 ** -1)
+    x["g"][n - 1] = 5.0
+    assert u / 2 * 2.718 ** 5 > torch.finfo(torch.float32).max
+    got = delta_scan(**x, initial=initial)
+    want, last, _ = R.rule(x, initial)
+    # (The factor e^5: the exponential's own step and its argument's, 5 2^-24, as a factor.)
+    R.check("grown out", got[0], want, R.half(BF) * want.abs() + 16 * 2.0 ** -24 * want.abs())
+    R.check("grown state", got[1], last, 16 * 2.0 ** -24 * last.abs())
