@@ -748,7 +748,8 @@ int lrmoe_delta_scan_grad(const lrmoe_delta_scan_args *args, const lrmoe_delta_g
  * lowest first, so that rows whose parent is another are those that died: their
  * states and pages may be overwritten by the parents' (lrmoe_fork_rows,
  * lrmoe_page_fork).  Rows without a continuation have token -1, their own row
- * as parent and score -inf.  Sums are joined and scores compared in 64 bits.
+ * as parent and score -inf.  Exponentials and their sums over 2048 logits are in
+ * fp32 (2^-18 of the sum at most), sums are joined and scores compared in 64 bits.
  * scores_out may be scores; beams 1..32, groups * beams at most 65535.
  * Workspace of lrmoe_beam_workspace_bytes bytes, 16-byte aligned. */
 #define LRMOE_BEAM_MAX 32

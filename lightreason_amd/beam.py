@@ -37,9 +37,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, finished: torch.T
     have ended: such a beam competes as it is.
 
     Beam w's continuation by token t scores ``scores[w] + log_softmax(
-    logits[w])[t]``, in 64 bits; equal scores go to the lower beam, a beam's own
-    by its logits, then to the lower token.  Logits that are not finite take no
-    part.
+    logits[w])[t]``.  Exponentials and their sums over 2048 logits are in fp32, what
+    joins and compares them in 64 bits: a beam's continuations keep the order of
+    their logits, those of two beams closer than the sums' error (about 1e-7; 2^-18 at
+    most) may change places.  Equal scores go to the lower beam, a beam's own by its
+    logits, then to the lower token.  Logits that are not finite take no part.
 
     Returns (tokens [groups, beams] int64, parents [groups, beams] int32, scores
     [groups, beams] fp32).  Parents are rows 0 .. groups * beams - 1.  The best

@@ -77,8 +77,8 @@ __device__ __forceinline__ double wave_scan_f64(double v) {
 //
 // A workgroup has a chunk and a key head: its rows once, their products with one
 // another, then per value head the inverse and the fragments.  Bound by what it
-// writes, 30 KB per chunk and value head and 48 KB per chunk and key head of 128
-// bf16 (8192 tokens, 16 / 32 heads: 67-70 us, 4.5 TB/s read and written).  38 KB
+// writes, 37 KB per chunk and value head and 48 KB per chunk and key head of 128
+// bf16 (8192 tokens, 16 / 32 heads: 69-73 us, 4.5 TB/s read and written).  38 KB
 // of LDS, four workgroups per CU: one's stores hide the next one's substitution.
 
 struct PrepareLds {
@@ -444,8 +444,8 @@ ScanGrid scan_grid(const ScanArgs& a, int columns) {
 // the next ones, which the lanes write as they hold them. A step is a chain of
 // three products and hand-overs, and the instructions of one wave on each SIMD;
 // the other waves' fill the gaps.  That chain bounds a long sequence (8192 tokens,
-// 32 heads of 128: 128 steps of 1.9 us, 238-247 us; the chain by itself 145), and
-// with a tape HBM joins it (4000 tokens of five sequences: 126 us for 343 MB).
+// 32 heads of 128: 128 steps of 2.1 us, 262-271 us; the chain by itself 145), and
+// with a tape HBM joins it (4000 tokens of five sequences: 136 us for 350 MB).
 // Loads by the chain's own waves took 9 % longer.
 template <int D, int NC, int PARTS>
 struct ScanLds {
@@ -791,7 +791,7 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
 //     dS <- e^(G_63) dS + sum_i scale e^(G_i) q_i do_i^T - sum_i e^(G_i) k_i dR_i^T:
 // the forward launch with the matrices transposed, for the same columns. Waves 0
 // to 3 have the chain; waves 4 to 7 compute the two sums over do, which need no
-// dS, a chunk ahead.  Bound as the forward launch is (the same 4000 tokens: 154 us
+// dS, a chunk ahead.  Bound as the forward launch is (the same 4000 tokens: 159 us
 // for 345 MB).
 template <int D, int NC, int PARTS>
 struct ScanGradLds {
