@@ -672,24 +672,26 @@ int lrmoe_verify_drafts(int blocks, int rows, int vocab, int type, const int64_t
  * [value_dim] of its slot,
  *     S *= exp(g);  u = beta (v - S^T k);  S += k u^T;  out = scale S^T q,
  * q and k of key head h / (heads / key_heads), divided by sqrt(sum x^2 + 1e-6)
- * with normalize.  Nothing is rounded but out.  initial [pool][heads][dim]
- * [value_dim] fp32 is read at slot slots[s] (NULL: s), or is zero where it
- * is NULL or fresh[s] != 0; final, of the same shape, is written at into[s]
- * (NULL: s).  initial may be final, and a sequence's slots the same; no two
- * sequences write one slot, and none writes a slot that another reads.  A
- * sequence without tokens passes its state on.  One whose slot lies outside the
- * pool is left out, its rows too.  starts never decrease and lie within [0,
+ * with normalize.  Nothing is rounded below fp32 but out.  initial
+ * [pool][heads][dim][value_dim] fp32 is read at slot slots[s] (NULL: s), or is
+ * zero where it is NULL or fresh[s] != 0; final, of the same shape, is written
+ * at into[s] (NULL: s).  initial may be final, and a sequence's slots the same;
+ * no two sequences write one slot, and none writes a slot that another reads.
+ * A sequence without tokens passes its state on.  One whose slot lies outside
+ * the pool is left out, its rows too.  starts never decrease and lie within [0,
  * tokens]: a sequence whose own do not counts as empty, and what a call with
- * such starts gives for the others is not defined.  Rows outside starts[0] .. starts[seqs] - 1 stay
- * as they were, or are set to 0 with clear.  What is not finite reaches later
- * tokens of its sequence only.  max_new only chooses the kernel: at least every
- * sequence's count where they are short.  Strides in elements, those of q, k, v
- * and out multiples of 8 (4 for out) with the last dimension contiguous; q, k,
- * v 16-byte and out 8-byte aligned; out shares no element with q, k and v
+ * such starts gives for the others is not defined.  Rows outside starts[0] ..
+ * starts[seqs] - 1 stay as they were, or are set to 0 with clear.  What is not
+ * finite reaches later tokens of its sequence only.  max_new only chooses the
+ * kernel, whose sums in fp32 have another order: at least every sequence's
+ * count where they are short.  Strides in elements, those of q, k, v and out
+ * multiples of 8 (4 for out) with the last dimension contiguous; q, k, v
+ * 16-byte and out 8-byte aligned; out shares no element with q, k and v
  * (refused) or anything else that is read.  dim 64 or 128, value_dim a multiple
  * of 32 up to 256, at most 2^20 tokens, 65536 sequences, tokens * heads of 2^26
- * and seqs * heads * value_dim of 2^27.  Workspace of lrmoe_delta_scan_workspace_bytes(args) bytes (0: none),
- * 256-byte aligned, not cleared, used by one stream at a time. */
+ * and seqs * heads * value_dim of 2^27.  Workspace of
+ * lrmoe_delta_scan_workspace_bytes(args) bytes (0: none), 256-byte aligned, not
+ * cleared, used by one stream at a time. */
 typedef struct lrmoe_delta_scan_args {
     int32_t seqs, tokens, max_new, heads, key_heads, dim, value_dim, fp16;
     int32_t normalize, beta_fp32, clear, pool;

@@ -157,7 +157,12 @@ def delta_scan(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     and lie within [0, tokens] (a batch is padded with their last value): a
     sequence whose own do not counts as empty, and what such a call gives for
     the others is not defined.  What is not finite reaches only later tokens of
-    its sequence.  Tensors may be strided views with a contiguous last dimension
+    its sequence; the columns that meet it are done again token by token (one of
+    a prompt of 8192: 11 ms instead of 0.3).  Longer sequences go in chunks and
+    short ones token by token, by their own counts, the call's heads and
+    sequences and whether a gradient is wanted: both are fp32, with sums in
+    another order, so that a result may round the other way among other
+    neighbours.  Tensors may be strided views with a contiguous last dimension
     and strides that are multiples of 8.
 
     Gradients flow to query, key, value, g, beta and initial, once (no second
@@ -298,7 +303,8 @@ def delta_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, g: t
     memory held where it is not given).  No two sequences of a call write one
     slot, and none writes a slot that another reads.  ``max_new`` -- at least
     every sequence's count of tokens, default ``tokens`` -- only chooses the
-    kernel: give it where the counts are known to be small.  ``out`` shares no
+    kernel, whose sums may round the other way: give it where the counts are
+    known to be small.  ``out`` shares no
     element with query, key and value (refused).  No gradient is recorded."""
     if scale is not None:
         scale = float(scale)
