@@ -110,9 +110,10 @@ __device__ __forceinline__ uint64_t wave_best(int W, int lane, Each&& each) {
 // exponentials, and the W best. Those are no smaller than the W-th largest of the
 // lanes' maxima, so that only what reaches it is gathered and ranked, W numbers
 // and a few more; where equal values make them more than a list holds, the
-// registers are gone through W times instead.  Bound by the logits (256 rows of
-// 151936 fp32, a tenth of them finished: 20.9 us, 6.8 TB/s; with W passes for every
-// slice 55 us); 4 rows in bf16 5.7 us, launch and latency.
+// registers are gone through W times instead.  Bound by the logits where they are
+// fp32 (256 rows of 151936, a tenth of them finished: 20.4 us, 6.9 TB/s; with W
+// passes for every slice 55 us), by its instructions in 16 bits (256 rows in bf16
+// 25 us, 3.1 TB/s); 4 rows in bf16 5.4 us, launch and latency.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void beam_slices(BeamArgs a) {
     __shared__ uint64_t lists[kThreads / kWave][kGather], bests[kThreads / kWave][kBeamMax];

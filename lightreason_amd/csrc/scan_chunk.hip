@@ -445,7 +445,7 @@ ScanGrid scan_grid(const ScanArgs& a, int columns) {
 // three products and hand-overs, and the instructions of one wave on each SIMD;
 // the other waves' fill the gaps.  That chain bounds a long sequence (8192 tokens,
 // 32 heads of 128: 128 steps of 2.1 us, 262-271 us; the chain by itself 145), and
-// with a tape HBM joins it (4000 tokens of five sequences: 136 us for 350 MB).
+// with a tape HBM joins it (4378 tokens of five sequences: 136 us for 448 MB).
 // Loads by the chain's own waves took 9 % longer.
 template <int D, int NC, int PARTS>
 struct ScanLds {
@@ -791,8 +791,8 @@ __global__ __launch_bounds__(kChainThreads, 3) void scan_chunks(ScanArgs a, Scan
 //     dS <- e^(G_63) dS + sum_i scale e^(G_i) q_i do_i^T - sum_i e^(G_i) k_i dR_i^T:
 // the forward launch with the matrices transposed, for the same columns. Waves 0
 // to 3 have the chain; waves 4 to 7 compute the two sums over do, which need no
-// dS, a chunk ahead.  Bound as the forward launch is (the same 4000 tokens: 159 us
-// for 345 MB).
+// dS, a chunk ahead.  Bound as the forward launch is (the same 4378 tokens: 159 us
+// for 448 MB).
 template <int D, int NC, int PARTS>
 struct ScanGradLds {
     uint4 s[3][D / 32][NC][kWave];
@@ -1111,8 +1111,10 @@ __global__ __launch_bounds__(kChainGradThreads, 2) void scan_chunks_grad(ScanArg
 // dq and dk each. What is fp32 (S, dS, w, du) is read once by the workgroup, 32
 // columns at a time, split into three bf16 numbers and shared through LDS, the
 // next 32 while the products of those before run (training step of 4000 tokens:
-// 300 -> 257 us): the decays' gradient is fp32 and as exact as that. Bound by its one workgroup per CU: 208 KB of S, dS, w and du per chunk and
-// value head come at 1.3 TB/s.
+// 300 -> 257 us with two parts in the products over tokens, 274-289 with three):
+// the decays' gradient is fp32 and as exact as that. Bound by its one workgroup
+// per CU: 208 KB of S, dS, w and du per chunk and value head, and with the rest
+// 775 MB in all, come and go at 2.7 TB/s.
 constexpr int kGradThreads = 512;
 template <int D>
 struct ScanInputsLds {
